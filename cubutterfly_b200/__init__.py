@@ -263,6 +263,13 @@ B200PeerBufferDestroy      p
 B200FourStepScatterColumns p p i i z z z z i p
 B200FourStepScatterRows    p p i i z z z z i i p
 B200FourStepScatterTranspose p p i i z z z z i p
+B200BlockNormForward       p p
+B200BlockNormGetWorkspaceSize p Z
+B200BlockNormBackward      p p
+B200GatedScanForward       p p
+B200GatedScanGetWorkspaceSize p Z
+B200GatedScanBackward      p p
+B200GatedScanStep          p p
 """
 
 

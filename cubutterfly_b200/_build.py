@@ -25,6 +25,8 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 # (operator, storage) units of the FWHT / zeta tile kernels
 BW_UNITS = [(0, 0), (0, 1), (0, 2), (1, 3), (1, 4), (2, 3), (2, 4)]
+# (block type, backward) units of the block norm
+BN_UNITS = [(t, b) for t in range(5) for b in (0, 1)]
 
 
 def _json_include() -> str:
@@ -45,7 +47,8 @@ def _units():
     for name in ("c_api.cpp", "descriptor.cpp", "planner.cpp", "rns_api.cpp", "launch_bitwise_dispatch.cpp",
                  "launch_ntt_dispatch.cpp", "launch_fft.cu", "noalloc.cu", "fourstep.cu", "bitrev.cu", "fwht_tc.cu",
                  "real_adapter.cu", "real_fft.cu", "calibrate.cu", "fourstep_peer.cu", "unaligned.cu", "structured.cu", "fwht_native.cu", "fft64.cu", "fft_chain.cu",
-                 "heongpu_adapter.cpp", "bluestein.cu"):
+                 "heongpu_adapter.cpp", "bluestein.cu", "block_ops_api.cpp", "launch_block_norm_dispatch.cpp",
+                 "launch_gated_scan.cu"):
         src = CSRC / name
         obj = OBJ / (src.stem + ".o")
         units.append((common + ["-c", str(src), "-o", str(obj)], src, obj))
@@ -53,6 +56,11 @@ def _units():
         src = CSRC / "launch_ntt.cu"
         obj = OBJ / f"ntt_w{word}.o"
         units.append((common + [f"-DCUBF_NTT_WORD={word}", "-c", str(src), "-o", str(obj)], src, obj))
+    for ty, backward in BN_UNITS:
+        src = CSRC / "launch_block_norm.cu"
+        obj = OBJ / f"block_norm_{ty}_{backward}.o"
+        units.append((common + [f"-DCUBF_BN_TYPE={ty}", f"-DCUBF_BN_BACKWARD={backward}", "-c", str(src), "-o",
+                                str(obj)], src, obj))
     for op, ty in BW_UNITS:
         src = CSRC / "launch_bitwise.cu"
         obj = OBJ / f"bitwise_{op}_{ty}.o"

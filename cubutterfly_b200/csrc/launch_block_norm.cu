@@ -1,0 +1,164 @@
+// launch_block_norm.cu -- launches of the block norm; compiled once per
+// CUBF_BN_TYPE (0 fp16, 1 fp16 with an fp32 residual, 2 bf16, 3 bf16 with an
+// fp32 residual, 4 fp32) and CUBF_BN_BACKWARD.
+#include <algorithm>
+
+#include "block_norm.cuh"
+#include "launch_util.cuh"
+
+#ifndef CUBF_BN_TYPE
+#define CUBF_BN_TYPE 2
+#endif
+#ifndef CUBF_BN_BACKWARD
+#define CUBF_BN_BACKWARD 0
+#endif
+
+namespace cubf {
+
+template <int TYPE>
+cudaError_t launch_block_norm_unit(const BlockNormArgs& a, cudaStream_t stream);
+template <int TYPE>
+cudaError_t launch_block_norm_backward_unit(const BlockNormArgs& a, size_t groups, cudaStream_t stream);
+
+namespace {
+
+using namespace norm;
+
+constexpr int kType = CUBF_BN_TYPE;
+using T = std::conditional_t<kType <= 1, __half, std::conditional_t<kType <= 3, __nv_bfloat16, float>>;
+using R = std::conditional_t<kType == 1 || kType == 3 || kType == 4, float, T>;
+constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+
+// Whole 16-byte vectors everywhere: every pointer aligned, every row stride
+// and the row length a multiple of the vector.
+bool aligned(const BlockNormArgs& a) {
+    uintptr_t bits = 0;
+    for (const void* p : {a.x, a.y, a.gate, a.pre, a.post, a.scales, a.d_residual, a.d_normed,
+                          static_cast<const void*>(a.residual), static_cast<const void*>(a.normed),
+                          static_cast<const void*>(a.d_x), static_cast<const void*>(a.d_y),
+                          static_cast<const void*>(a.d_gate), static_cast<const void*>(a.partials)})
+        bits |= reinterpret_cast<uintptr_t>(p) & 15u;
+    for (size_t s : {a.x_row, a.y_row, a.gate_row, a.d_residual_row, a.d_normed_row, static_cast<size_t>(a.dim)})
+        bits |= s & (kVec - 1);
+    return bits == 0;
+}
+
+template <typename S, bool ROTATE, bool BACKWARD>
+constexpr int shared_bytes() {
+    const int row = ROTATE || (BACKWARD && S::kRows > 1) ? S::kRows * S::TPR * S::EPT : 0;
+    return 4 * (row + 4 * S::kWarps);
+}
+
+template <typename S, bool ROTATE>
+cudaError_t run(const BlockNormArgs& a, size_t groups, cudaStream_t stream) {
+    static KernelSetup setup;
+#if CUBF_BN_BACKWARD
+    auto kernel = &block_norm_backward_kernel<T, R, S, ROTATE>;
+#else
+    auto kernel = &block_norm_kernel<T, R, S, ROTATE>;
+#endif
+    constexpr int smem = shared_bytes<S, ROTATE, CUBF_BN_BACKWARD>();
+    int cap = 0;
+    cudaError_t e = setup_kernel(setup, kernel, S::kThreads, smem, &cap);
+    if (e != cudaSuccess) return e;
+#if CUBF_BN_BACKWARD
+    (void)cap;
+    const size_t grid = groups * a.parts_per_group;
+#else
+    (void)groups;
+    const size_t grid = std::min<size_t>((a.rows + S::kRows - 1) / S::kRows, static_cast<size_t>(cap));
+#endif
+    if (grid > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
+    return launch_dependent(kernel, static_cast<unsigned>(grid), static_cast<unsigned>(S::kThreads), smem, stream, a);
+}
+
+template <int TPR, int EPT, int VW, bool ROTATE>
+cudaError_t shape(const BlockNormArgs& a, size_t groups, cudaStream_t stream) {
+    return run<Shape<TPR, EPT, VW>, ROTATE>(a, groups, stream);
+}
+
+cudaError_t dispatch(const BlockNormArgs& a, size_t groups, cudaStream_t s) {
+    constexpr int V = kVec;
+    const bool vec = aligned(a);
+    const int d = a.dim;
+    if (a.rotate) {
+        if (vec && d >= 256) {
+#if CUBF_BN_BACKWARD
+            switch (d) {
+                case 256: return shape<32, 8, V, true>(a, groups, s);
+                case 512: return shape<32, 16, V, true>(a, groups, s);
+                case 1024: return shape<64, 16, V, true>(a, groups, s);
+                case 2048: return shape<128, 16, V, true>(a, groups, s);
+                case 4096: return shape<256, 16, V, true>(a, groups, s);
+                case 8192: return shape<512, 16, V, true>(a, groups, s);
+                case 16384: return shape<1024, 16, V, true>(a, groups, s);
+            }
+#else
+            switch (d) {
+                case 256: return shape<32, 8, V, true>(a, groups, s);
+                case 512: return shape<32, 16, V, true>(a, groups, s);
+                case 1024: return shape<32, 32, V, true>(a, groups, s);
+                case 2048: return shape<64, 32, V, true>(a, groups, s);
+                case 4096: return shape<64, 64, V, true>(a, groups, s);
+                case 8192: return shape<128, 64, V, true>(a, groups, s);
+                case 16384: return shape<256, 64, V, true>(a, groups, s);
+            }
+#endif
+        }
+        switch (d) {
+            case 64: return shape<32, 2, 1, true>(a, groups, s);
+            case 128: return shape<32, 4, 1, true>(a, groups, s);
+            case 256: return shape<32, 8, 1, true>(a, groups, s);
+            case 512: return shape<32, 16, 1, true>(a, groups, s);
+            case 1024: return shape<64, 16, 1, true>(a, groups, s);
+            case 2048: return shape<128, 16, 1, true>(a, groups, s);
+            case 4096: return shape<256, 16, 1, true>(a, groups, s);
+            case 8192: return shape<512, 16, 1, true>(a, groups, s);
+            case 16384: return shape<1024, 16, 1, true>(a, groups, s);
+        }
+        return cudaErrorInvalidValue;
+    }
+    if (vec) {
+        if (d <= 256) return shape<32, 8, V, false>(a, groups, s);
+        if (d <= 512) return shape<64, 8, V, false>(a, groups, s);
+        if (d <= 1024) return shape<128, 8, V, false>(a, groups, s);
+        if (d <= 2048) return shape<256, 8, V, false>(a, groups, s);
+        if (d <= 4096) return shape<512, 8, V, false>(a, groups, s);
+        if (d <= 8192) return shape<512, 16, V, false>(a, groups, s);
+        if (d <= kBlockNormMaxDim) return shape<1024, 16, V, false>(a, groups, s);
+    } else {
+        if (d <= 256) return shape<32, 8, 1, false>(a, groups, s);
+        if (d <= 1024) return shape<128, 8, 1, false>(a, groups, s);
+        if (d <= 4096) return shape<512, 8, 1, false>(a, groups, s);
+        if (d <= kBlockNormMaxDim) return shape<1024, 16, 1, false>(a, groups, s);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+#if CUBF_BN_BACKWARD
+template <>
+cudaError_t launch_block_norm_backward_unit<CUBF_BN_TYPE>(const BlockNormArgs& a, size_t groups, cudaStream_t stream) {
+    cudaError_t e = dispatch(a, groups, stream);
+    if (e != cudaSuccess || !(a.need_p || a.need_q || a.need_z)) return e;
+    const bool per_group = a.gate_mode == kGateChannel || a.gate_mode == kGateGroups;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>((a.dim + 31) / 32), 3u + (per_group ? static_cast<unsigned>(groups) : 0u));
+    cfg.blockDim = dim3(1024);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, &block_norm_sums_kernel<T>, a, static_cast<int>(groups * a.parts_per_group));
+}
+#else
+template <>
+cudaError_t launch_block_norm_unit<CUBF_BN_TYPE>(const BlockNormArgs& a, cudaStream_t stream) {
+    return dispatch(a, 1, stream);
+}
+#endif
+
+}  // namespace cubf

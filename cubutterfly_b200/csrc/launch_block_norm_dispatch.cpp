@@ -1,0 +1,62 @@
+// launch_block_norm_dispatch.cpp -- picks the block norm unit of a type pair.
+#include <algorithm>
+
+#include "block_ops.hpp"
+
+namespace cubf {
+
+template <int TYPE>
+cudaError_t launch_block_norm_unit(const BlockNormArgs& a, cudaStream_t stream);
+template <int TYPE>
+cudaError_t launch_block_norm_backward_unit(const BlockNormArgs& a, size_t groups, cudaStream_t stream);
+
+#define CUBF_BN_UNIT(TYPE)                                                                  \
+    template <>                                                                             \
+    cudaError_t launch_block_norm_unit<TYPE>(const BlockNormArgs&, cudaStream_t);           \
+    template <>                                                                             \
+    cudaError_t launch_block_norm_backward_unit<TYPE>(const BlockNormArgs&, size_t, cudaStream_t);
+CUBF_BN_UNIT(0)
+CUBF_BN_UNIT(1)
+CUBF_BN_UNIT(2)
+CUBF_BN_UNIT(3)
+CUBF_BN_UNIT(4)
+#undef CUBF_BN_UNIT
+
+namespace {
+int unit_of(BlockType type, bool residual32) {
+    if (type == BlockType::kF32) return 4;
+    return (type == BlockType::kBF16 ? 2 : 0) + (residual32 ? 1 : 0);
+}
+}  // namespace
+
+int block_norm_parts(size_t rows_per_gate, size_t groups, int dim) {
+    // rows side by side in a CTA of the narrow shapes; then at least four
+    // turns per CTA, and no more CTAs than two per SM
+    const size_t side = dim <= 256 ? 4 : 1;
+    const size_t most = std::max<size_t>(1, (rows_per_gate + 4 * side - 1) / (4 * side));
+    const size_t share = std::max<size_t>(1, 296 / std::max<size_t>(1, groups));
+    return static_cast<int>(std::min(most, share));
+}
+
+cudaError_t launch_block_norm(BlockType type, bool residual32, const BlockNormArgs& a, cudaStream_t stream) {
+    switch (unit_of(type, residual32)) {
+        case 0: return launch_block_norm_unit<0>(a, stream);
+        case 1: return launch_block_norm_unit<1>(a, stream);
+        case 2: return launch_block_norm_unit<2>(a, stream);
+        case 3: return launch_block_norm_unit<3>(a, stream);
+        default: return launch_block_norm_unit<4>(a, stream);
+    }
+}
+
+cudaError_t launch_block_norm_backward(BlockType type, bool residual32, const BlockNormArgs& a, size_t groups,
+                                       cudaStream_t stream) {
+    switch (unit_of(type, residual32)) {
+        case 0: return launch_block_norm_backward_unit<0>(a, groups, stream);
+        case 1: return launch_block_norm_backward_unit<1>(a, groups, stream);
+        case 2: return launch_block_norm_backward_unit<2>(a, groups, stream);
+        case 3: return launch_block_norm_backward_unit<3>(a, groups, stream);
+        default: return launch_block_norm_backward_unit<4>(a, groups, stream);
+    }
+}
+
+}  // namespace cubf

@@ -1,0 +1,141 @@
+// launch_gated_scan.cu -- launches of the gated linear recurrence.
+#include <algorithm>
+
+#include "gated_scan.cuh"
+#include "launch_util.cuh"
+
+namespace cubf {
+namespace {
+
+using namespace scan;
+
+int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+template <typename... Args>
+cudaError_t launch_clusters(void (*kernel)(Args...), unsigned grid, unsigned threads, int cluster, cudaStream_t stream,
+                            Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Pair accesses need every row of every tensor to start on a pair boundary.
+template <typename T>
+struct PairAligned {
+    uintptr_t bits = 0;
+    PairAligned& pointer(const void* p) {
+        bits |= reinterpret_cast<uintptr_t>(p) & (2 * sizeof(T) - 1);
+        return *this;
+    }
+    PairAligned& stride(size_t elements) {
+        bits |= elements & 1;
+        return *this;
+    }
+};
+
+template <typename T>
+bool pair_aligned(const GatedScanArgs& a, bool backward) {
+    PairAligned<T> v;
+    v.stride(static_cast<size_t>(a.dim)).pointer(a.x).pointer(a.r).pointer(a.i);
+    v.stride(a.x_batch).stride(a.r_batch).stride(a.i_batch).stride(a.x_token).stride(a.r_token).stride(a.i_token);
+    if (backward)
+        v.pointer(a.d_h).pointer(a.d_x).pointer(a.d_r).pointer(a.d_i).stride(a.dh_batch).stride(a.dh_token);
+    else
+        v.pointer(a.h);
+    return v.bits == 0;
+}
+
+template <typename T, bool PACKED, bool VEC>
+cudaError_t launch_shape(const GatedScanArgs& a, bool backward, cudaStream_t stream) {
+    const int tiles = ceil_div(a.dim, kChannels);
+    const int cluster = gated_scan_cluster(a.batch, a.length, a.dim, backward);
+    const size_t grid = static_cast<size_t>(tiles) * a.batch * cluster;
+    if (grid > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
+    return launch_clusters(backward ? &gated_scan_backward_kernel<T, PACKED, VEC> : &gated_scan_kernel<T, PACKED, VEC>,
+                           static_cast<unsigned>(grid), kWarps * 32u, cluster, stream, a, cluster, tiles);
+}
+
+template <typename T>
+cudaError_t launch_typed(const GatedScanArgs& a, bool backward, cudaStream_t stream) {
+    const bool vec = pair_aligned<T>(a, backward);
+    if (a.offsets) return vec ? launch_shape<T, true, true>(a, backward, stream) : launch_shape<T, true, false>(a, backward, stream);
+    return vec ? launch_shape<T, false, true>(a, backward, stream) : launch_shape<T, false, false>(a, backward, stream);
+}
+
+cudaError_t launch_any(BlockType type, const GatedScanArgs& a, bool backward, cudaStream_t stream) {
+    switch (type) {
+        case BlockType::kF16: return launch_typed<__half>(a, backward, stream);
+        case BlockType::kBF16: return launch_typed<__nv_bfloat16>(a, backward, stream);
+        case BlockType::kF32: return launch_typed<float>(a, backward, stream);
+    }
+    return cudaErrorInvalidValue;
+}
+
+template <typename T>
+cudaError_t launch_step_typed(const GatedStepArgs& a, cudaStream_t stream) {
+    PairAligned<T> v;
+    v.stride(static_cast<size_t>(a.dim)).pointer(a.x).pointer(a.r).pointer(a.i).pointer(a.h);
+    v.stride(a.x_row).stride(a.r_row).stride(a.i_row);
+    const int tiles = ceil_div(a.dim, kChannels);
+    // about 32 warps per SM before a warp takes a second request
+    const size_t groups = std::max<size_t>(1, static_cast<size_t>(148 * 32) / tiles);
+    const size_t rows = (a.batch + groups - 1) / groups;
+    const size_t tasks = (a.batch + rows - 1) / rows * tiles;
+    const size_t grid = (tasks + 3) / 4;
+    if (grid > 0x7fffffffULL || rows > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
+    return launch_dependent(v.bits == 0 ? &gated_scan_step_kernel<T, true> : &gated_scan_step_kernel<T, false>,
+                            static_cast<unsigned>(grid), 128u, 0, stream, a, tiles, static_cast<int>(rows));
+}
+
+}  // namespace
+
+int gated_scan_cluster(int batch, int length, int dim, bool backward) {
+    (void)backward;
+    const size_t columns = static_cast<size_t>(ceil_div(dim, kChannels)) * batch;
+    const int tiles = ceil_div(length, kTile);
+    int best = 1;
+    double least = 0;
+    for (int k = 1; k <= kGatedScanMaxCluster; k *= 2) {
+        const double waves = static_cast<double>((columns * k + 295) / 296);
+        const double cost = waves * ceil_div(tiles, k) * (k > 1 ? 1.15 : 1.0);
+        if (k == 1 || cost < least) {
+            best = k;
+            least = cost;
+        }
+    }
+    return best;
+}
+
+cudaError_t launch_gated_scan(BlockType type, const GatedScanArgs& a, cudaStream_t stream) {
+    return launch_any(type, a, false, stream);
+}
+
+cudaError_t launch_gated_scan_backward(BlockType type, const GatedScanArgs& a, cudaStream_t stream) {
+    cudaError_t e = launch_any(type, a, true, stream);
+    if (e != cudaSuccess) return e;
+    const int parts = a.batch * gated_scan_cluster(a.batch, a.length, a.dim, true);
+    return launch_dependent(&gated_scan_decay_kernel, static_cast<unsigned>(ceil_div(a.dim, 32)), 256u, 0, stream, a,
+                            parts);
+}
+
+cudaError_t launch_gated_scan_step(BlockType type, const GatedStepArgs& a, cudaStream_t stream) {
+    switch (type) {
+        case BlockType::kF16: return launch_step_typed<__half>(a, stream);
+        case BlockType::kBF16: return launch_step_typed<__nv_bfloat16>(a, stream);
+        case BlockType::kF32: return launch_step_typed<float>(a, stream);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace cubf

@@ -21,10 +21,19 @@ import threading
 import cubutterfly_b200 as cb
 
 __all__ = ["fwht", "hadamard_rotate", "fft", "zeta", "ntt", "plan_cache_size", "clear_plan_cache",
-           "InferenceGraph"]
+           "InferenceGraph", "block_norm", "gated_scan", "gated_scan_step"]
 
 _LOCK = threading.Lock()
 _PLANS: dict = {}
+
+
+def __getattr__(name):
+    # the block operators import torch at module level, so they are loaded at first use
+    if name in ("block_norm", "gated_scan", "gated_scan_step"):
+        from cubutterfly_b200 import block_ops
+
+        return getattr(block_ops, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 class _CachedPlan:

@@ -164,6 +164,136 @@ CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200HeongpuTransform(const uint64_
 CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200HeongpuControl(int freeze, int clear_cache, int reset_counters,
                                                                 size_t* calls, size_t* polynomials);
 
+/* ---- Block operators of recurrent language models (no counterpart in the
+ * reference ABI; torch_ops.block_norm, gated_scan and gated_scan_step) -------
+ *
+ * Every call only enqueues kernels on `stream`: no allocation, no copy, no
+ * synchronisation; buffers must outlive the work.  Strides count elements,
+ * the channel stride is one, outputs and gradients are contiguous.  A null
+ * optional pointer leaves its part out.  Types are CUBUTTERFLY_DATA_FP16,
+ * _BF16 or _FP32; arithmetic is fp32 with one rounding per output.
+ * struct_size must be sizeof the struct (CUBUTTERFLY_STATUS_INVALID_VALUE
+ * otherwise, and for null required pointers, sizes of zero where a row or
+ * channel is needed, strides below the row length or aliasing outputs);
+ * sizes and types outside the ranges below are
+ * CUBUTTERFLY_STATUS_NOT_SUPPORTED.  Zero rows or tokens are valid. */
+
+enum {
+    CUBUTTERFLY_B200_GATE_LINEAR = 0,  /* act(g) = g */
+    CUBUTTERFLY_B200_GATE_SIGMOID = 1,
+    CUBUTTERFLY_B200_GATE_SILU = 2     /* g sigmoid(g) */
+};
+enum {
+    CUBUTTERFLY_B200_POST_NORM = 1,    /* norm the block output y */
+    CUBUTTERFLY_B200_PRE_NORM = 2,     /* norm the sum for the next block */
+    CUBUTTERFLY_B200_ROTATE = 4        /* and rotate it: u H_dim / sqrt(dim) */
+};
+
+/* The boundary between two blocks, per row (RMS norms, r(v) = 1/sqrt(mean(v^2) + eps)):
+ *   n = y r(y) post_weight               (POST_NORM; else n = y)
+ *   residual = scale x + act(gate) n     (residual = scale x without y)
+ *   normed = residual r(residual) pre_weight, rotated with ROTATE   (PRE_NORM)
+ * The norm is taken of the sum before it is rounded to residual_type.
+ * dim in [1, 16384]; ROTATE needs a power of two in [64, 16384].
+ * data_type is y's, normed's and a per-row gate's; residual_type is data_type
+ * or FP32; each per-channel vector's type is data_type or FP32.
+ * gate_rows: 0 no gate, 1 a gate per channel, rows a gate per row, else a
+ * divisor of rows: a gate per group of rows / gate_rows consecutive rows (the
+ * per-channel and per-group gates have type gate_type, a per-row gate
+ * data_type).  residual may be x itself (x_row = dim).
+ * A call whose backward follows keeps r(y) and r(residual) of every row in
+ * post_rms and pre_rms (fp32, rows values each; both or neither null). */
+typedef struct cubutterflyB200BlockNorm_s {
+    size_t struct_size;
+    size_t rows, dim, gate_rows;
+    int data_type, residual_type;            /* cubutterflyDataType_t */
+    int pre_type, post_type, scale_type, gate_type;
+    int flags, activation;
+    double residual_scale, epsilon;
+    const void *x, *y, *gate;
+    const void *pre_weight, *post_weight, *scale;  /* scale: per channel, or null: residual_scale */
+    size_t x_row, y_row, gate_row;
+    void *residual, *normed;
+    float *post_rms, *pre_rms;
+    /* backward only */
+    const void *d_residual, *d_normed;       /* null: zero */
+    size_t d_residual_row, d_normed_row;
+    void *d_x, *d_y, *d_gate;                /* required with x, y, gate; d_gate (gate_rows, dim) */
+    void *d_pre_weight, *d_post_weight, *d_scale;  /* required with their vectors, in their types */
+    void* workspace;
+    size_t workspace_bytes;
+} cubutterflyB200BlockNorm_t;
+
+CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200BlockNormForward(const cubutterflyB200BlockNorm_t* args,
+                                                                  cudaStream_t stream);
+/* Reads rows, dim and gate_rows. */
+CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200BlockNormGetWorkspaceSize(const cubutterflyB200BlockNorm_t* args,
+                                                                           size_t* bytes);
+CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200BlockNormBackward(const cubutterflyB200BlockNorm_t* args,
+                                                                   cudaStream_t stream);
+
+/* The gated linear recurrence, per channel along `length` tokens:
+ *   la_t = -exponent softplus(decay) sigmoid(recurrence_gate_t),  a_t = exp(la_t)
+ *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(input_gate_t) x_t
+ * from initial_state (fp32, (states, dim); null: zero) to final_state (fp32,
+ * required).  Dense: `batch` sequences, states = batch, sequences = 0, offsets
+ * null.  Packed: batch = 1, offsets a device array of sequences + 1 ascending
+ * ints from 0 to length; sequence j is tokens [offsets[j], offsets[j + 1]),
+ * possibly none (its final state is its initial state); states = sequences.
+ * Values of one sequence, NaN and infinities included, do not reach another.
+ * dim >= 1, length <= 2^30; decay (dim) is fp32; exponent > 0.
+ * A call whose backward follows keeps the state before every 64th token in
+ * chunk_states (fp32, (batch, ceil(length / 64), dim)). */
+typedef struct cubutterflyB200GatedScan_s {
+    size_t struct_size;
+    size_t batch, length, dim, sequences;
+    int data_type, reserved;
+    double exponent;
+    const void *x, *recurrence_gate, *input_gate;
+    size_t x_batch, x_token, recurrence_batch, recurrence_token, input_batch, input_token;
+    const float *decay, *initial_state;
+    const int* offsets;
+    void* h;
+    float *final_state, *chunk_states;
+    /* backward only (chunk_states then an input) */
+    const void* d_h;                         /* required */
+    size_t dh_batch, dh_token;
+    const float* d_final_state;              /* null: zero */
+    void *d_x, *d_recurrence_gate, *d_input_gate;
+    float *d_decay, *d_initial_state;        /* d_initial_state: null: not computed */
+    void* workspace;
+    size_t workspace_bytes;
+} cubutterflyB200GatedScan_t;
+
+CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200GatedScanForward(const cubutterflyB200GatedScan_t* args,
+                                                                  cudaStream_t stream);
+/* Reads batch, length and dim. */
+CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200GatedScanGetWorkspaceSize(const cubutterflyB200GatedScan_t* args,
+                                                                           size_t* bytes);
+CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200GatedScanBackward(const cubutterflyB200GatedScan_t* args,
+                                                                   cudaStream_t stream);
+
+/* One token of the recurrence for `batch` requests: request b's state is row
+ * slots[b] (b where slots is null) of `state` ((pool, dim) fp32, contiguous);
+ * the new one goes to the same row of new_state (state itself: in place).  A
+ * slot outside [0, pool) marks padding: that request's h is zero and no state
+ * is read or written.  Distinct requests need distinct slots. */
+typedef struct cubutterflyB200GatedScanStep_s {
+    size_t struct_size;
+    size_t batch, dim, pool;
+    int data_type, reserved;
+    double exponent;
+    const void *x, *recurrence_gate, *input_gate;
+    size_t x_row, recurrence_row, input_row;
+    const float *decay, *state;
+    float* new_state;
+    const int* slots;
+    void* h;
+} cubutterflyB200GatedScanStep_t;
+
+CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200GatedScanStep(const cubutterflyB200GatedScanStep_t* args,
+                                                               cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
