@@ -6,59 +6,98 @@
 //   h_t = a_t h_{t-1} + u_t,   u_t = sqrt(1 - a_t^2) sigmoid(i_t) x_t.
 // A run of tokens is the affine map h -> A h + H (A the product of its a, H
 // its last h from h = 0), and runs join by (A1, H1) . (A2, H2) =
-// (A1 A2, A2 H1 + H2), so time is split three ways: a thread runs kSteps
+// (A1 A2, A2 H1 + H2), so time is split three ways: a thread runs STEPS
 // tokens of two channels in registers, the kWarps warps of a CTA join their
 // maps through shared memory, and the CTAs of a cluster, which hold
 // consecutive tiles of the same channels, join theirs through distributed
 // shared memory; the cluster then walks along the sequence.  Every input is
 // read once, every output written once, and no CTA waits on one outside its
 // cluster.
+//
+// What bounds it is issue slots before memory: at the rate of a device copy
+// (8 bytes a bf16 element forward) an element may take 45 of them, and the
+// gates alone take five special-function instructions.  So the two channels
+// of a lane are computed as packed fp32 pairs, and a is formed on the FMA pipe.
 #pragma once
 
 #include "block_ops.hpp"
 #include "common.cuh"
+#include "f32x2.cuh"
 
 namespace cubf::scan {
 
-constexpr int kSteps = 8;                  // tokens per thread and tile
-constexpr int kWarps = 8;                  // warps per CTA, consecutive in time
-constexpr int kTile = kSteps * kWarps;     // tokens per CTA tile
-constexpr int kChannels = 64;              // channels per CTA, two per lane
-static_assert(kTile == kGatedScanChunk, "the backward kernel restarts from the forward's chunk states");
+using f32x2::add2;
+using f32x2::fma2;
+using f32x2::mul2;
+using f32x2::sub2;
+using Pair = f32x2::P;
 
-// Two channels of one token as loaded: 16-bit pairs in a word, fp32 in two.
+constexpr int kWarps = 8;                  // warps per CTA, consecutive in time
+constexpr int kChannels = 64;              // channels per CTA, two per lane
+constexpr int kForwardSteps = 16;          // tokens per thread and tile
+constexpr int kBackwardSteps = 8;
+constexpr int kForwardTile = kForwardSteps * kWarps;    // tokens per CTA tile
+constexpr int kBackwardTile = kBackwardSteps * kWarps;
+static_assert(kBackwardTile == kGatedScanChunk, "the backward restarts from the states the forward kept");
+static_assert(kGatedScanChunk % kForwardSteps == 0, "chunks begin where a forward thread does");
+
+CUBF_DEV Pair both(float v) { return f32x2::pk(v, v); }
+CUBF_DEV Pair pair(float2 v) { return f32x2::pk(v.x, v.y); }
+CUBF_DEV float2 floats(Pair p) {
+    float2 f;
+    f32x2::up(p, f.x, f.y);
+    return f;
+}
+template <typename F>
+CUBF_DEV Pair each(Pair p, F f) {
+    const float2 v = floats(p);
+    return f32x2::pk(f(v.x), f(v.y));
+}
+
+// ---- access to two channels of a token --------------------------------------------------------
+// 16-bit pairs come in a word, fp32 pairs in two.
 template <typename T>
 struct Raw {
     using Word = uint32_t;
     static CUBF_DEV Word zero() { return 0u; }
+    static CUBF_DEV Word lowest() { return std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u; }  // -inf
     static CUBF_DEV Word vec(const T* p) { return __ldcs(reinterpret_cast<const unsigned int*>(p)); }
     static CUBF_DEV Word two(const T* p, bool ok0, bool ok1) {
         const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
         const uint32_t lo = ok0 ? __ldcs(q) : 0u, hi = ok1 ? __ldcs(q + 32) : 0u;
         return lo | (hi << 16);
     }
-    static CUBF_DEV float2 get(Word w) {
-        T v[2];
-        memcpy(v, &w, 4);
-        return make_float2(Convert<T, float>::load(v[0]), Convert<T, float>::load(v[1]));
+    static CUBF_DEV Pair get(Word w) {
+        if constexpr (std::is_same<T, __half>::value) {
+            __half2 h;
+            memcpy(&h, &w, 4);
+            return pair(__half22float2(h));
+        } else {
+            return f32x2::pk(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+        }
     }
-    static CUBF_DEV Word put(float2 f) {
-        const T v[2] = {Convert<T, float>::store(f.x), Convert<T, float>::store(f.y)};
-        Word w;
-        memcpy(&w, v, 4);
-        return w;
+    static CUBF_DEV void store_vec(T* p, float2 f) {
+        uint32_t w;
+        if constexpr (std::is_same<T, __half>::value) {
+            const __half2 h = __float22half2_rn(f);
+            memcpy(&w, &h, 4);
+        } else {
+            const __nv_bfloat162 h = __float22bfloat162_rn(f);
+            memcpy(&w, &h, 4);
+        }
+        __stcs(reinterpret_cast<unsigned int*>(p), w);
     }
-    static CUBF_DEV void store_vec(T* p, float2 f) { __stcs(reinterpret_cast<unsigned int*>(p), put(f)); }
 };
 template <>
 struct Raw<float> {
     using Word = float2;
     static CUBF_DEV Word zero() { return make_float2(0.f, 0.f); }
+    static CUBF_DEV Word lowest() { return make_float2(-INFINITY, -INFINITY); }
     static CUBF_DEV Word vec(const float* p) { return __ldcs(reinterpret_cast<const float2*>(p)); }
     static CUBF_DEV Word two(const float* p, bool ok0, bool ok1) {
         return make_float2(ok0 ? __ldcs(p) : 0.f, ok1 ? __ldcs(p + 32) : 0.f);
     }
-    static CUBF_DEV float2 get(Word w) { return w; }
+    static CUBF_DEV Pair get(Word w) { return pair(w); }
     static CUBF_DEV void store_vec(float* p, float2 f) { __stcs(reinterpret_cast<float2*>(p), f); }
 };
 
@@ -81,7 +120,8 @@ struct Lane {
             return Raw<T>::two(row + ch, ok0, ok1);
     }
     template <typename T>
-    CUBF_DEV void store(T* row, float2 f) const {
+    CUBF_DEV void store(T* row, Pair p) const {
+        const float2 f = floats(p);
         if constexpr (VEC) {
             if (ok0) Raw<T>::store_vec(row + ch, f);
         } else {
@@ -89,15 +129,26 @@ struct Lane {
             if (ok1) row[ch + 32] = Convert<T, float>::store(f.y);
         }
     }
-    CUBF_DEV float2 load32(const float* row) const {
-        return make_float2(ok0 ? row[ch] : 0.f, ok1 ? row[ch + (VEC ? 1 : 32)] : 0.f);
+    CUBF_DEV Pair load32(const float* row) const {
+        return f32x2::pk(ok0 ? row[ch] : 0.f, ok1 ? row[ch + (VEC ? 1 : 32)] : 0.f);
     }
-    CUBF_DEV void store32(float* row, float2 f) const {
+    CUBF_DEV void store32(float* row, Pair p) const {
+        const float2 f = floats(p);
         if (ok0) row[ch] = f.x;
         if (ok1) row[ch + (VEC ? 1 : 32)] = f.y;
     }
 };
 
+// Brings the rows [t, t + ROWS) of a CTA's channels towards L2: the loads of
+// the next turn then wait for L2 only, and hold no registers meanwhile.
+template <int ROWS, typename T>
+CUBF_DEV void prefetch_rows(const T* base, size_t stride, int c0, int t, int lane, int length, int dim) {
+    const int row = t + lane % ROWS, col = c0 + lane / ROWS * (kChannels * ROWS / 32);
+    if (row < length && col < dim)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(base + static_cast<size_t>(row) * stride + col));
+}
+
+// ---- the arithmetic of a token ----------------------------------------------------------------
 CUBF_DEV float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -113,61 +164,74 @@ CUBF_DEV float rsq(float x) {
     asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+CUBF_DEV float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 
-CUBF_DEV float sigmoid(float v) { return rcp(1.f + ex2(-kLog2e * v)); }
+CUBF_DEV Pair sigmoid(Pair v) {
+    const Pair e = each(mul2(v, both(-kLog2e)), [](float x) { return ex2(x); });
+    return each(add2(e, both(1.f)), [](float x) { return rcp(x); });
+}
 
 // c softplus(Lambda) log2(e): la in units of log2 is -rate sigmoid(r).
 CUBF_DEV float softplus(float v) { return v > 20.f ? v : log1pf(expf(v)); }
-CUBF_DEV float rate_of(float lambda, float exponent) { return exponent * softplus(lambda) * kLog2e; }
-
-// 1 - a^2 = 1 - 2^(2 w) for w = log2(a) <= 0.  Near a = 1 the difference
-// cancels, so for 2 la = 2 ln(2) w > -1/8 the series of -(e^z - 1) is used
-// (five terms; the next is z^5/720 < 5e-8 of the sum); beyond it 1 - a^2 is
-// at least 0.117, and a's rounding costs under 3e-6 of it.
-CUBF_DEV float one_minus_square(float w, float a) {
-    constexpr float z = 1.3862943611198906f;  // 2 ln 2
-    constexpr float c1 = z, c2 = z * z / 2, c3 = z * z * z / 6, c4 = z * z * z * z / 24, c5 = z * z * z * z * z / 120;
-    const float series = -w * (c1 + w * (c2 + w * (c3 + w * (c4 + w * c5))));
-    return w > -0.09f ? series : 1.f - a * a;
+CUBF_DEV Pair rates(Pair lambda, float exponent) {
+    return each(lambda, [&](float v) { return exponent * softplus(v) * kLog2e; });
 }
 
-// One token of one channel, from its gate inputs.
-struct Coefficients {
-    float sr, si;  // the gates
-    float w;       // log2(a)
-    float a;
-    float m;       // sqrt(1 - a^2)
-};
-constexpr float kSmallestNormal = 1.1754944e-38f;
-CUBF_DEV Coefficients coefficients(float rate, float r, float i) {
-    Coefficients c;
-    c.sr = sigmoid(r);
-    c.si = sigmoid(i);
-    c.w = -rate * c.sr;
-    c.a = ex2(c.w);
-    const float m2 = one_minus_square(c.w, c.a);
-    // a shut gate (a = 1) keeps h as it is; NaN passes
-    c.m = m2 >= kSmallestNormal ? m2 * rsq(m2) : m2;
-    return c;
+// a = 2^w and 1 - a^2 for w = log2(a) <= 0.  A recurrence forgets over
+// 1/(1 - a) tokens and multiplies by a every time, so a has to be rounded
+// without a bias and 1 - a must not cancel.  With w = n + f, n the nearest
+// integer and |f| <= 1/2, t = 2^f - 1 = f P(f) comes from a polynomial (the
+// Chebyshev-node least-squares fit of (2^f - 1)/f of degree five, weighted to
+// equal ripples: 1.1e-8 relative), s = 2^n is put together from n's bits, and
+//   a = s + s t,   1 - a = (1 - s) - s t,   1 - a^2 = (1 - a)(1 + a);
+// for n = 0 the second is -t itself.  w below -126 is taken as -126: 1e-38.
+CUBF_DEV void decay(Pair w, Pair& a, Pair& m2) {
+    const Pair magic = both(12582912.f + 127.f);  // 1.5 2^23: n + 127 lands in the low bits
+    w = each(w, [](float x) { return max_nan(x, -126.f); });
+    const Pair r = add2(w, magic);
+    const Pair f = sub2(w, sub2(r, magic));
+    Pair t = fma2(f, both(0.00015403512f), both(0.0013390735f));
+    t = fma2(f, t, both(0.0096182376f));
+    t = fma2(f, t, both(0.055503573f));
+    t = fma2(f, t, both(0.24022649f));
+    t = fma2(f, t, both(0.69314718f));
+    const Pair s = each(r, [](float x) { return __uint_as_float(__float_as_uint(x) << 23); });
+    const Pair st = mul2(s, mul2(f, t));
+    a = add2(s, st);
+    const Pair q = sub2(sub2(both(1.f), s), st);
+    m2 = fma2(q, a, q);
+}
+// 1/sqrt(1 - a^2); where a = 1 (a gate that is shut) finite, so that its
+// products with 1 - a^2 = 0 and log a = 0 vanish as their limits do.
+CUBF_DEV Pair inverse_root(Pair m2) {
+    return each(add2(m2, both(1e-37f)), [](float x) { return rsq(x); });
 }
 
+// ---- joining runs -----------------------------------------------------------------------------
 // In packed batches a run that holds a sequence's first token forgets what
 // came before it whatever that was (a product with zero would keep its NaN):
-// its A is the marker -0, which no product of decays (all >= +0) produces.
+// its A is the marker -0 in both channels, which no product of decays (all
+// >= +0) produces.
+constexpr Pair kMarker = 0x8000000080000000ULL;
+CUBF_DEV bool marked(Pair a) { return static_cast<uint32_t>(a) == 0x80000000u; }
+
 template <bool PACKED>
-CUBF_DEV float through(float a, float h, float carry) {
-    if (PACKED && __float_as_uint(a) == 0x80000000u) return h;
-    return fmaf(a, carry, h);
+CUBF_DEV Pair through(Pair a, Pair h, Pair carry) {
+    if (PACKED && marked(a)) return h;
+    return fma2(a, carry, h);
 }
 template <bool PACKED>
-CUBF_DEV float product(float first, float second) {
-    if (PACKED && __float_as_uint(second) == 0x80000000u) return second;
-    if (PACKED && __float_as_uint(first) == 0x80000000u) return first;
-    return first * second;
+CUBF_DEV Pair product(Pair first, Pair second) {
+    if (PACKED && (marked(first) || marked(second))) return kMarker;
+    return mul2(first, second);
 }
-CUBF_DEV float marker() { return __uint_as_float(0x80000000u); }
 
 // Walks the sequences of a packed batch along increasing tokens.
 struct Walker {
@@ -178,9 +242,12 @@ struct Walker {
     CUBF_DEV void init(const int* o, int sequences) {
         offsets = o;
         last = sequences - 1;
+        rewind();
+    }
+    CUBF_DEV void rewind() {
         at = 0;
-        start = o[0];
-        stop = o[1];
+        start = offsets[0];
+        stop = offsets[1];
     }
     // Moves to the last sequence that starts at or before token t (doubling
     // steps, then halving: the next sequence in one comparison, far ones in
@@ -199,11 +266,8 @@ struct Walker {
         start = offsets[lo];
         stop = offsets[lo + 1];
     }
-    CUBF_DEV void rewind() {
-        at = 0;
-        start = offsets[0];
-        stop = offsets[1];
-    }
+    // Tokens [t, t + n) lie inside one sequence, its first and last token not among them.
+    CUBF_DEV bool inside(int t, int n) const { return start < t && t + n < stop; }
 };
 
 CUBF_DEV uint32_t cluster_rank() {
@@ -214,166 +278,165 @@ CUBF_DEV uint32_t cluster_rank() {
 CUBF_DEV void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-CUBF_DEV void store_remote(const void* local, uint32_t rank, float4 v) {
+
+// An affine map of a lane's two channels.
+struct alignas(16) Map {
+    Pair a, h;
+};
+CUBF_DEV void store_remote(const Map* local, uint32_t rank, Map v) {
     const uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(local));
     uint32_t remote;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-    asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "f"(v.x), "f"(v.y), "f"(v.z),
-                 "f"(v.w)
-                 : "memory");
+    asm volatile("st.shared::cluster.v2.u64 [%0], {%1, %2};" ::"r"(remote), "l"(v.a), "l"(v.h) : "memory");
 }
 
-// {A, A, H, H} of the lane's two channels.
+// ---- forward ----------------------------------------------------------------------------------
 struct Maps {
-    float4 warp[2][kWarps][32];
-    float4 cta[2][kGatedScanMaxCluster][32];
+    Map warp[2][kWarps][32];
+    Map cta[2][kGatedScanMaxCluster][32];
 };
 
-// ---- forward -----------------------------------------------------------------------------------
 template <typename T, bool PACKED, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArgs p, int cluster, int tiles) {
+    constexpr int kSteps = kForwardSteps, kTile = kForwardTile;
     __shared__ Maps maps;
     pdl_begin();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rank = cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
     const unsigned column = blockIdx.x / cluster;
-    const Lane<VEC> ln(static_cast<int>(column % tiles) * kChannels, lane, p.dim);
+    const int c0 = static_cast<int>(column % tiles) * kChannels;
+    const Lane<VEC> ln(c0, lane, p.dim);
     const size_t b = column / tiles;
     const T* x = static_cast<const T*>(p.x) + b * p.x_batch;
     const T* r = static_cast<const T*>(p.r) + b * p.r_batch;
     const T* g = static_cast<const T*>(p.i) + b * p.i_batch;
     T* out = static_cast<T*>(p.h) + b * static_cast<size_t>(p.length) * p.dim;
-    const float2 lambda = ln.load32(p.decay);
-    const float2 rate = make_float2(rate_of(lambda.x, p.exponent), rate_of(lambda.y, p.exponent));
+    const Pair rate = mul2(rates(ln.load32(p.decay), p.exponent), both(-1.f));
     const int stride = cluster * kTile;
+    const size_t chunks = static_cast<size_t>((p.length + kGatedScanChunk - 1) / kGatedScanChunk);
     int t0 = rank * kTile + warp * kSteps;
 
-    typename Raw<T>::Word rx[kSteps], rr[kSteps], ri[kSteps];
-    auto load = [&](int t) {
-        const T *px = x + static_cast<size_t>(t) * p.x_token, *pr = r + static_cast<size_t>(t) * p.r_token,
-                *pi = g + static_cast<size_t>(t) * p.i_token;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const bool in = t + s < p.length;
-            rx[s] = in ? ln.load(px) : Raw<T>::zero();
-            rr[s] = in ? ln.load(pr) : Raw<T>::zero();
-            ri[s] = in ? ln.load(pi) : Raw<T>::zero();
-            px += p.x_token;
-            pr += p.r_token;
-            pi += p.i_token;
-        }
-    };
-    load(t0);
-
     Walker seq;
-    if constexpr (PACKED) seq.init(p.offsets, p.sequences);
-    if constexpr (PACKED) {  // sequences without tokens end where they began
-        if (rank == 0)
+    if constexpr (PACKED) {
+        seq.init(p.offsets, p.sequences);
+        if (rank == 0)  // sequences without tokens end where they began
             for (int j = warp; j < p.sequences; j += kWarps)
                 if (p.offsets[j] >= p.offsets[j + 1])
                     ln.store32(p.last + static_cast<size_t>(j) * p.dim,
-                               p.initial ? ln.load32(p.initial + static_cast<size_t>(j) * p.dim)
-                                         : make_float2(0.f, 0.f));
+                               p.initial ? ln.load32(p.initial + static_cast<size_t>(j) * p.dim) : both(0.f));
     }
-    float2 carry = make_float2(0.f, 0.f);  // h before the cluster's tiles
+    Pair carry = both(0.f);  // h before the cluster's tiles
     if (!PACKED && p.initial) carry = ln.load32(p.initial + b * p.dim);
 
     const int rounds = (p.length + stride - 1) / stride;
     for (int round = 0; round < rounds; ++round, t0 += stride) {
         const int buf = round & 1;
-        float2 a[kSteps], u[kSteps];
-        float2 A = make_float2(1.f, 1.f), H = make_float2(0.f, 0.f);
-        unsigned starts = 0;
-        if constexpr (PACKED) seq.seek(t0);
-        Walker from = seq;
+        // Tokens past the end are a shut gate (r = -inf: a = 1) over x = 0:
+        // the identity map.
+        Pair a[kSteps], u[kSteps];
+        {
+            typename Raw<T>::Word rx[kSteps], rr[kSteps], ri[kSteps];
+            const T *px = x + static_cast<size_t>(t0) * p.x_token, *pr = r + static_cast<size_t>(t0) * p.r_token,
+                    *pi = g + static_cast<size_t>(t0) * p.i_token;
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            if (t0 + s < p.length) {
-                const float2 fx = Raw<T>::get(rx[s]), fr = Raw<T>::get(rr[s]), fi = Raw<T>::get(ri[s]);
-                const Coefficients c0 = coefficients(rate.x, fr.x, fi.x), c1 = coefficients(rate.y, fr.y, fi.y);
-                a[s] = make_float2(c0.a, c1.a);
-                u[s] = make_float2(c0.m * c0.si * fx.x, c1.m * c1.si * fx.y);
-                bool first = false;
-                if constexpr (PACKED) {
-                    seq.seek(t0 + s);
-                    first = t0 + s == seq.start;
-                }
-                if (PACKED && first) {
+            for (int s = 0; s < kSteps; ++s) {
+                const bool in = t0 + s < p.length;
+                rx[s] = in ? ln.load(px) : Raw<T>::zero();
+                rr[s] = in ? ln.load(pr) : Raw<T>::lowest();
+                ri[s] = in ? ln.load(pi) : Raw<T>::zero();
+                px += p.x_token;
+                pr += p.r_token;
+                pi += p.i_token;
+            }
+            if (round + 1 < rounds) {
+                prefetch_rows<kSteps>(x, p.x_token, c0, t0 + stride, lane, p.length, p.dim);
+                prefetch_rows<kSteps>(r, p.r_token, c0, t0 + stride, lane, p.length, p.dim);
+                prefetch_rows<kSteps>(g, p.i_token, c0, t0 + stride, lane, p.length, p.dim);
+            }
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                Pair m2;
+                decay(mul2(rate, sigmoid(Raw<T>::get(rr[s]))), a[s], m2);
+                const Pair m = mul2(m2, inverse_root(m2));
+                u[s] = mul2(mul2(m, sigmoid(Raw<T>::get(ri[s]))), Raw<T>::get(rx[s]));
+            }
+        }
+        Pair A = both(1.f), H = both(0.f);
+        unsigned starts = 0;
+        Walker from;
+        bool plain = true;
+        if constexpr (PACKED) {
+            seq.seek(t0);
+            from = seq;
+            plain = seq.inside(t0, kSteps);
+        }
+        if (plain) {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                A = mul2(A, a[s]);
+                H = fma2(a[s], H, u[s]);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                if (t0 + s >= p.length) continue;
+                seq.seek(t0 + s);
+                if (t0 + s == seq.start) {
                     starts |= 1u << s;
-                    if (p.initial) {
-                        const float2 h0 = ln.load32(p.initial + static_cast<size_t>(seq.at) * p.dim);
-                        u[s].x = fmaf(a[s].x, h0.x, u[s].x);
-                        u[s].y = fmaf(a[s].y, h0.y, u[s].y);
-                    }
-                    A = make_float2(marker(), marker());
+                    if (p.initial)
+                        u[s] = fma2(a[s], ln.load32(p.initial + static_cast<size_t>(seq.at) * p.dim), u[s]);
+                    A = kMarker;
                     H = u[s];
                 } else {
-                    A.x = product<PACKED>(A.x, a[s].x);
-                    A.y = product<PACKED>(A.y, a[s].y);
-                    H.x = fmaf(a[s].x, H.x, u[s].x);
-                    H.y = fmaf(a[s].y, H.y, u[s].y);
+                    A = product<PACKED>(A, a[s]);
+                    H = fma2(a[s], H, u[s]);
                 }
-            } else {
-                a[s] = make_float2(1.f, 1.f);
-                u[s] = make_float2(0.f, 0.f);
             }
         }
-        if (round + 1 < rounds) load(t0 + stride);  // in flight while the maps are joined and h is written
-        maps.warp[buf][warp][lane] = make_float4(A.x, A.y, H.x, H.y);
+        maps.warp[buf][warp][lane] = Map{A, H};
         __syncthreads();
         // the CTA's map, and the map of the warps before this one
-        float2 preA = make_float2(1.f, 1.f), preH = make_float2(0.f, 0.f), totA = preA, totH = preH;
+        Map before{both(1.f), both(0.f)}, total = before;
 #pragma unroll
         for (int k = 0; k < kWarps; ++k) {
-            if (k == warp) {
-                preA = totA;
-                preH = totH;
-            }
-            const float4 m = maps.warp[buf][k][lane];
-            totH.x = through<PACKED>(m.x, m.z, totH.x);
-            totH.y = through<PACKED>(m.y, m.w, totH.y);
-            totA.x = product<PACKED>(totA.x, m.x);
-            totA.y = product<PACKED>(totA.y, m.y);
+            if (k == warp) before = total;
+            const Map m = maps.warp[buf][k][lane];
+            total.h = through<PACKED>(m.a, m.h, total.h);
+            total.a = product<PACKED>(total.a, m.a);
         }
-        float2 in = carry;  // h before this CTA's tile
+        Pair in = carry;  // h before this CTA's tile
         if (cluster == 1) {
-            carry.x = through<PACKED>(totA.x, totH.x, carry.x);
-            carry.y = through<PACKED>(totA.y, totH.y, carry.y);
+            carry = through<PACKED>(total.a, total.h, carry);
         } else {
-            for (int k = warp; k < cluster; k += kWarps)
-                store_remote(&maps.cta[buf][rank][lane], k, make_float4(totA.x, totA.y, totH.x, totH.y));
+            for (int k = warp; k < cluster; k += kWarps) store_remote(&maps.cta[buf][rank][lane], k, total);
             cluster_sync();
             for (int k = 0; k < cluster; ++k) {
                 if (k == rank) in = carry;
-                const float4 m = maps.cta[buf][k][lane];
-                carry.x = through<PACKED>(m.x, m.z, carry.x);
-                carry.y = through<PACKED>(m.y, m.w, carry.y);
+                const Map m = maps.cta[buf][k][lane];
+                carry = through<PACKED>(m.a, m.h, carry);
             }
         }
-        float2 h;
-        h.x = through<PACKED>(preA.x, preH.x, in.x);
-        h.y = through<PACKED>(preA.y, preH.y, in.y);
-        if (p.chunk_states && warp == 0 && t0 < p.length)
-            ln.store32(p.chunk_states +
-                           (b * ((p.length + kTile - 1) / kTile) + static_cast<size_t>(t0 / kTile)) * p.dim,
-                       h);
+        Pair h = through<PACKED>(before.a, before.h, in);
+        if (p.chunk_states && t0 % kGatedScanChunk == 0 && t0 < p.length)
+            ln.store32(p.chunk_states + (b * chunks + static_cast<size_t>(t0 / kGatedScanChunk)) * p.dim, h);
         T* po = out + static_cast<size_t>(t0) * p.dim;
+        if (plain) {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            if (t0 + s < p.length) {
-                if (PACKED && ((starts >> s) & 1u)) {
-                    h = u[s];
-                } else {
-                    h.x = fmaf(a[s].x, h.x, u[s].x);
-                    h.y = fmaf(a[s].y, h.y, u[s].y);
-                }
-                ln.store(po, h);
-                if constexpr (PACKED) {
-                    from.seek(t0 + s);
-                    if (t0 + s + 1 == from.stop) ln.store32(p.last + static_cast<size_t>(from.at) * p.dim, h);
-                }
+            for (int s = 0; s < kSteps; ++s) {
+                h = fma2(a[s], h, u[s]);
+                if (t0 + s < p.length) ln.store(po, h);
+                po += p.dim;
             }
-            po += p.dim;
+        } else {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                if (t0 + s >= p.length) continue;
+                h = (starts >> s) & 1u ? u[s] : fma2(a[s], h, u[s]);
+                ln.store(po, h);
+                from.seek(t0 + s);
+                if (t0 + s + 1 == from.stop) ln.store32(p.last + static_cast<size_t>(from.at) * p.dim, h);
+                po += p.dim;
+            }
         }
     }
     if (!PACKED && rank == 0 && warp == 0) ln.store32(p.last + b * p.dim, carry);
@@ -383,22 +446,31 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
 // ---- backward ----------------------------------------------------------------------------------
 // G_t = dh_t + P_{t+1}, P_t = a_t G_t runs from the end of time by the same
 // joins; h_{t-1} is run again from the chunk state the forward kept, in fp32,
-// instead of read back in the outputs' type.
+// instead of read back in the outputs' type.  With m = sqrt(1 - a^2),
+// v = m sigmoid(i) and e = dL/d(la) la (d m/d la = -a^2/m):
+//   dx = G v                  di = dx x (1 - sigmoid(i))
+//   e  = a G la (h_{t-1} - sigmoid(i) x a/m)
+//   dr = e (1 - sigmoid(r))   dLambda = sum e sigmoid(Lambda)/softplus(Lambda)
+// A thread keeps a, v, 1/m and sigmoid(r) of its tokens and gets sigmoid(i)
+// back as v/m, which leaves room for two CTAs per SM.
 struct BackMaps {
-    float4 warp[2][kWarps][32];  // {A, A, H, H}
-    float2 back[2][kWarps][32];  // P out of the warp's tokens from P = 0 after them
-    float4 cta[2][kGatedScanMaxCluster][32];
-    float2 sum[kWarps][32];
+    Map warp[2][kWarps][32];
+    Pair back[2][kWarps][32];  // P out of the warp's tokens from P = 0 after them
+    Map cta[2][kGatedScanMaxCluster][32];
+    Pair sum[kWarps][32];
 };
 
 template <typename T, bool PACKED, bool VEC>
-__global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(GatedScanArgs p, int cluster, int tiles) {
+__global__ void __launch_bounds__(kWarps * 32, 2)
+    gated_scan_backward_kernel(GatedScanArgs p, int cluster, int tiles) {
+    constexpr int kSteps = kBackwardSteps, kTile = kBackwardTile;
     __shared__ BackMaps maps;
     pdl_begin();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rank = cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
     const unsigned column = blockIdx.x / cluster;
-    const Lane<VEC> ln(static_cast<int>(column % tiles) * kChannels, lane, p.dim);
+    const int c0 = static_cast<int>(column % tiles) * kChannels;
+    const Lane<VEC> ln(c0, lane, p.dim);
     const size_t b = column / tiles;
     const T* x = static_cast<const T*>(p.x) + b * p.x_batch;
     const T* r = static_cast<const T*>(p.r) + b * p.r_batch;
@@ -408,31 +480,29 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(Gat
     T* dx = static_cast<T*>(p.d_x) + out;
     T* dr = static_cast<T*>(p.d_r) + out;
     T* di = static_cast<T*>(p.d_i) + out;
-    const float2 lambda = ln.load32(p.decay);
-    const float2 rate = make_float2(rate_of(lambda.x, p.exponent), rate_of(lambda.y, p.exponent));
+    const Pair rate = mul2(rates(ln.load32(p.decay), p.exponent), both(-1.f));
     const int stride = cluster * kTile;
     const int chunks = (p.length + kTile - 1) / kTile;
     const int rounds = (p.length + stride - 1) / stride;
 
-    if constexpr (PACKED) {  // sequences without tokens pass their gradient through
-        if (p.d_initial && rank == 0)
+    Walker seq;
+    if constexpr (PACKED) {
+        seq.init(p.offsets, p.sequences);
+        if (p.d_initial && rank == 0)  // sequences without tokens pass their gradient through
             for (int j = warp; j < p.sequences; j += kWarps)
                 if (p.offsets[j] >= p.offsets[j + 1])
                     ln.store32(p.d_initial + static_cast<size_t>(j) * p.dim,
-                               p.d_last ? ln.load32(p.d_last + static_cast<size_t>(j) * p.dim)
-                                        : make_float2(0.f, 0.f));
+                               p.d_last ? ln.load32(p.d_last + static_cast<size_t>(j) * p.dim) : both(0.f));
     }
-    Walker seq;
-    if constexpr (PACKED) seq.init(p.offsets, p.sequences);
-    float2 carry = make_float2(0.f, 0.f);  // P from the tokens after the cluster's tiles
+    Pair carry = both(0.f);  // P from the tokens after the cluster's tiles
     if (!PACKED && p.d_last) carry = ln.load32(p.d_last + b * p.dim);
-    float2 sum = make_float2(0.f, 0.f);    // of e, for the gradient of Lambda
+    Pair sum = both(0.f);    // of e
 
     for (int round = rounds - 1; round >= 0; --round) {
         const int buf = round & 1;
         const int t0 = round * stride + rank * kTile + warp * kSteps;
         typename Raw<T>::Word rx[kSteps], rd[kSteps];
-        float2 a[kSteps], m[kSteps], sr[kSteps], si[kSteps];
+        Pair a[kSteps], v[kSteps], im[kSteps], sr[kSteps];
         {
             typename Raw<T>::Word rr[kSteps], ri[kSteps];
             const T *px = x + static_cast<size_t>(t0) * p.x_token, *pr = r + static_cast<size_t>(t0) * p.r_token,
@@ -441,7 +511,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(Gat
             for (int s = 0; s < kSteps; ++s) {
                 const bool in = t0 + s < p.length;
                 rx[s] = in ? ln.load(px) : Raw<T>::zero();
-                rr[s] = in ? ln.load(pr) : Raw<T>::zero();
+                rr[s] = in ? ln.load(pr) : Raw<T>::lowest();
                 ri[s] = in ? ln.load(pi) : Raw<T>::zero();
                 rd[s] = in ? ln.load(pd) : Raw<T>::zero();
                 px += p.x_token;
@@ -449,176 +519,156 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(Gat
                 pi += p.i_token;
                 pd += p.dh_token;
             }
+            if (round > 0) {
+                prefetch_rows<kSteps>(x, p.x_token, c0, t0 - stride, lane, p.length, p.dim);
+                prefetch_rows<kSteps>(r, p.r_token, c0, t0 - stride, lane, p.length, p.dim);
+                prefetch_rows<kSteps>(g, p.i_token, c0, t0 - stride, lane, p.length, p.dim);
+                prefetch_rows<kSteps>(dh, p.dh_token, c0, t0 - stride, lane, p.length, p.dim);
+            }
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
-                const float2 fr = Raw<T>::get(rr[s]), fi = Raw<T>::get(ri[s]);
-                const Coefficients c0 = coefficients(rate.x, fr.x, fi.x), c1 = coefficients(rate.y, fr.y, fi.y);
-                a[s] = make_float2(c0.a, c1.a);
-                m[s] = make_float2(c0.m, c1.m);
-                sr[s] = make_float2(c0.sr, c1.sr);
-                si[s] = make_float2(c0.si, c1.si);
+                Pair m2;
+                sr[s] = sigmoid(Raw<T>::get(rr[s]));
+                decay(mul2(rate, sr[s]), a[s], m2);
+                im[s] = inverse_root(m2);
+                v[s] = mul2(mul2(m2, im[s]), sigmoid(Raw<T>::get(ri[s])));
             }
         }
-        float2 h = make_float2(0.f, 0.f);  // before the tile, from the forward
+        Pair h = both(0.f);  // before the tile, from the forward
         const int chunk = round * cluster + rank;
         if (chunk < chunks) h = ln.load32(p.chunk_states + (b * chunks + chunk) * static_cast<size_t>(p.dim));
 
-        // the maps of the warp's tokens
+        // the maps of the warp's tokens, forward and backward
         unsigned starts = 0, ends = 0;
-        float2 A = make_float2(1.f, 1.f), H = make_float2(0.f, 0.f);
+        Pair A = both(1.f), H = both(0.f), R = both(0.f);
         Walker from;
+        bool plain = true;
         if constexpr (PACKED) {
             seq.rewind();
             seq.seek(t0);
             from = seq;
-        }
-        // the token's u, with the sequence's initial state where it begins one
-        auto drive = [&](int s, const Walker& w, bool first) {
-            const float2 fx = Raw<T>::get(rx[s]);
-            float2 u = make_float2(m[s].x * si[s].x * fx.x, m[s].y * si[s].y * fx.y);
-            if (PACKED && first && p.initial) {
-                const float2 h0 = ln.load32(p.initial + static_cast<size_t>(w.at) * p.dim);
-                u.x = fmaf(a[s].x, h0.x, u.x);
-                u.y = fmaf(a[s].y, h0.y, u.y);
-            }
-            return u;
-        };
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            if (t0 + s >= p.length) continue;
-            bool first = false;
-            if constexpr (PACKED) {
-                seq.seek(t0 + s);
-                first = t0 + s == seq.start;
-                if (t0 + s + 1 == seq.stop) ends |= 1u << s;
-            }
-            const float2 u = drive(s, seq, first);
-            if (PACKED && first) {
-                starts |= 1u << s;
-                A = make_float2(marker(), marker());
-                H = u;
-            } else {
-                A.x = product<PACKED>(A.x, a[s].x);
-                A.y = product<PACKED>(A.y, a[s].y);
-                H.x = fmaf(a[s].x, H.x, u.x);
-                H.y = fmaf(a[s].y, H.y, u.y);
-            }
+            plain = seq.inside(t0, kSteps);
         }
         // dh with the final states' gradients where a sequence ends
         auto arriving = [&](int s, int at) {
-            float2 d = Raw<T>::get(rd[s]);
-            if (PACKED && ((ends >> s) & 1u) && p.d_last) {
-                const float2 l = ln.load32(p.d_last + static_cast<size_t>(at) * p.dim);
-                d.x += l.x;
-                d.y += l.y;
-            }
+            Pair d = Raw<T>::get(rd[s]);
+            if (PACKED && ((ends >> s) & 1u) && p.d_last)
+                d = add2(d, ln.load32(p.d_last + static_cast<size_t>(at) * p.dim));
             return d;
         };
-        float2 R = make_float2(0.f, 0.f);
-        int at = PACKED ? seq.at : 0;
+        // the sequence of the token before a sequence's first one
+        auto previous = [&](int at, int t) {
+            while (at > 0 && p.offsets[at] >= t) --at;
+            return at;
+        };
+        if (plain) {
 #pragma unroll
-        for (int s = kSteps - 1; s >= 0; --s) {
-            if (t0 + s >= p.length) continue;
-            const float2 d = arriving(s, at);
-            R.x = a[s].x * (d.x + R.x);
-            R.y = a[s].y * (d.y + R.y);
-            if (PACKED && ((starts >> s) & 1u)) {
-                R = make_float2(0.f, 0.f);
-                // the token before belongs to the last sequence with tokens before this one
-                while (at > 0 && p.offsets[at] > t0 + s - 1) --at;
+            for (int s = 0; s < kSteps; ++s) {
+                A = mul2(A, a[s]);
+                H = fma2(a[s], H, mul2(v[s], Raw<T>::get(rx[s])));
+            }
+#pragma unroll
+            for (int s = kSteps - 1; s >= 0; --s) R = mul2(a[s], add2(Raw<T>::get(rd[s]), R));
+        } else {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                if (t0 + s >= p.length) continue;
+                seq.seek(t0 + s);
+                Pair u = mul2(v[s], Raw<T>::get(rx[s]));
+                if (t0 + s + 1 == seq.stop) ends |= 1u << s;
+                if (t0 + s == seq.start) {
+                    starts |= 1u << s;
+                    if (p.initial) u = fma2(a[s], ln.load32(p.initial + static_cast<size_t>(seq.at) * p.dim), u);
+                    A = kMarker;
+                    H = u;
+                } else {
+                    A = product<PACKED>(A, a[s]);
+                    H = fma2(a[s], H, u);
+                }
+            }
+            int at = seq.at;
+#pragma unroll
+            for (int s = kSteps - 1; s >= 0; --s) {
+                if (t0 + s >= p.length) continue;
+                R = mul2(a[s], add2(arriving(s, at), R));
+                if ((starts >> s) & 1u) {
+                    R = both(0.f);
+                    at = previous(at, t0 + s);
+                }
             }
         }
-        maps.warp[buf][warp][lane] = make_float4(A.x, A.y, H.x, H.y);
+        maps.warp[buf][warp][lane] = Map{A, H};
         maps.back[buf][warp][lane] = R;
         __syncthreads();
-        float2 totA = make_float2(1.f, 1.f), totR = make_float2(0.f, 0.f), postA = totA, postR = totR;
+        Map after{both(1.f), both(0.f)}, total = after;  // of P, from the end of time
 #pragma unroll
         for (int k = 0; k < kWarps; ++k) {
             if (k >= warp) break;
-            const float4 q = maps.warp[buf][k][lane];
-            h.x = through<PACKED>(q.x, q.z, h.x);
-            h.y = through<PACKED>(q.y, q.w, h.y);
+            const Map q = maps.warp[buf][k][lane];
+            h = through<PACKED>(q.a, q.h, h);
         }
 #pragma unroll
         for (int k = kWarps - 1; k >= 0; --k) {
-            if (k == warp) {
-                postA = totA;
-                postR = totR;
-            }
-            const float4 q = maps.warp[buf][k][lane];
-            const float2 back = maps.back[buf][k][lane];
-            totR.x = through<PACKED>(q.x, back.x, totR.x);
-            totR.y = through<PACKED>(q.y, back.y, totR.y);
-            totA.x = product<PACKED>(totA.x, q.x);
-            totA.y = product<PACKED>(totA.y, q.y);
+            if (k == warp) after = total;
+            const Pair qa = maps.warp[buf][k][lane].a;
+            total.h = through<PACKED>(qa, maps.back[buf][k][lane], total.h);
+            total.a = product<PACKED>(total.a, qa);
         }
-        float2 in = carry;  // P from the tokens after this CTA's tile
+        Pair in = carry;  // P from the tokens after this CTA's tile
         if (cluster == 1) {
-            carry.x = through<PACKED>(totA.x, totR.x, carry.x);
-            carry.y = through<PACKED>(totA.y, totR.y, carry.y);
+            carry = through<PACKED>(total.a, total.h, carry);
         } else {
-            for (int k = warp; k < cluster; k += kWarps)
-                store_remote(&maps.cta[buf][rank][lane], k, make_float4(totA.x, totA.y, totR.x, totR.y));
+            for (int k = warp; k < cluster; k += kWarps) store_remote(&maps.cta[buf][rank][lane], k, total);
             cluster_sync();
             for (int k = cluster - 1; k >= 0; --k) {
                 if (k == rank) in = carry;
-                const float4 q = maps.cta[buf][k][lane];
-                carry.x = through<PACKED>(q.x, q.z, carry.x);
-                carry.y = through<PACKED>(q.y, q.w, carry.y);
+                const Map q = maps.cta[buf][k][lane];
+                carry = through<PACKED>(q.a, q.h, carry);
             }
         }
-        float2 P;
-        P.x = through<PACKED>(postA.x, postR.x, in.x);
-        P.y = through<PACKED>(postA.y, postR.y, in.y);
+        Pair P = through<PACKED>(after.a, after.h, in);
 
         // h before each token, then the gradients from the last token back
-        float2 before[kSteps];
+        Pair before[kSteps];
+        int at = 0;
+        if (plain) {
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            before[s] = h;
-            if (t0 + s >= p.length) continue;
-            const bool first = PACKED && ((starts >> s) & 1u);
-            if constexpr (PACKED) {
-                from.seek(t0 + s);
-                if (first)
-                    before[s] = p.initial ? ln.load32(p.initial + static_cast<size_t>(from.at) * p.dim)
-                                          : make_float2(0.f, 0.f);
+            for (int s = 0; s < kSteps; ++s) {
+                before[s] = h;
+                h = fma2(a[s], h, mul2(v[s], Raw<T>::get(rx[s])));
             }
-            const float2 fx = Raw<T>::get(rx[s]);
-            h.x = fmaf(a[s].x, before[s].x, m[s].x * si[s].x * fx.x);
-            h.y = fmaf(a[s].y, before[s].y, m[s].y * si[s].y * fx.y);
+        } else {
+            at = seq.at;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                before[s] = h;
+                if (t0 + s >= p.length) continue;
+                from.seek(t0 + s);
+                if ((starts >> s) & 1u)
+                    before[s] = p.initial ? ln.load32(p.initial + static_cast<size_t>(from.at) * p.dim) : both(0.f);
+                h = fma2(a[s], before[s], mul2(v[s], Raw<T>::get(rx[s])));
+            }
         }
-        at = PACKED ? seq.at : 0;
+        const size_t o = static_cast<size_t>(t0) * p.dim;
 #pragma unroll
         for (int s = kSteps - 1; s >= 0; --s) {
             if (t0 + s >= p.length) continue;
-            const float2 d = arriving(s, at);
-            const float2 G = make_float2(d.x + P.x, d.y + P.y);
-            const float2 fx = Raw<T>::get(rx[s]);
-            float2 ox, orr, oi;
-            auto channel = [&](float Gv, float av, float mv, float srv, float siv, float xv, float hv, float rt,
-                               float& gx, float& gr, float& gi, float& total) {
-                const float la = -0.6931471805599453f * rt * srv;
-                const float gm = Gv * mv, gs = siv * xv;
-                gx = gm * siv;
-                gi = gm * gs * (1.f - siv);
-                // d sqrt(1 - a^2)/d la = -a^2/m; times la it tends to 0 with la
-                const float ratio = mv > 1e-18f ? -la * rcp(mv) : la;
-                const float e = Gv * av * fmaf(hv, la, gs * av * ratio);
-                gr = e * (1.f - srv);
-                total += e;
-            };
-            channel(G.x, a[s].x, m[s].x, sr[s].x, si[s].x, fx.x, before[s].x, rate.x, ox.x, orr.x, oi.x, sum.x);
-            channel(G.y, a[s].y, m[s].y, sr[s].y, si[s].y, fx.y, before[s].y, rate.y, ox.y, orr.y, oi.y, sum.y);
-            const size_t o = static_cast<size_t>(t0 + s) * p.dim;
-            ln.store(dx + o, ox);
-            ln.store(dr + o, orr);
-            ln.store(di + o, oi);
-            P = make_float2(a[s].x * G.x, a[s].y * G.y);
-            if (PACKED && ((starts >> s) & 1u)) {
+            const Pair fx = Raw<T>::get(rx[s]);
+            const Pair G = add2(plain ? Raw<T>::get(rd[s]) : arriving(s, at), P);
+            const Pair gx = mul2(G, v[s]), si = mul2(v[s], im[s]);
+            const Pair gi = mul2(mul2(gx, fx), sub2(both(1.f), si));
+            P = mul2(a[s], G);
+            const Pair la = mul2(mul2(rate, both(kLn2)), sr[s]);
+            const Pair e = mul2(mul2(P, la), sub2(before[s], mul2(mul2(mul2(si, fx), a[s]), im[s])));
+            sum = add2(sum, e);
+            const size_t row = o + static_cast<size_t>(s) * p.dim;
+            ln.store(dx + row, gx);
+            ln.store(dr + row, mul2(e, sub2(both(1.f), sr[s])));
+            ln.store(di + row, gi);
+            if (!plain && ((starts >> s) & 1u)) {
                 if (p.d_initial) ln.store32(p.d_initial + static_cast<size_t>(at) * p.dim, P);
-                P = make_float2(0.f, 0.f);
-                while (at > 0 && p.offsets[at] > t0 + s - 1) --at;
+                P = both(0.f);
+                at = previous(at, t0 + s);
             }
         }
     }
@@ -626,10 +676,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(Gat
     maps.sum[warp][lane] = sum;
     __syncthreads();
     if (warp == 0) {
-        for (int k = 1; k < kWarps; ++k) {
-            sum.x += maps.sum[k][lane].x;
-            sum.y += maps.sum[k][lane].y;
-        }
+        for (int k = 1; k < kWarps; ++k) sum = add2(sum, maps.sum[k][lane]);
         ln.store32(p.partials + (b * cluster + rank) * static_cast<size_t>(p.dim), sum);
     }
     if (cluster > 1) cluster_sync();
@@ -668,23 +715,23 @@ __global__ void __launch_bounds__(128) gated_scan_step_kernel(GatedStepArgs p, i
     const size_t first = static_cast<size_t>(task / tiles) * rows;
     if (first >= p.batch) return;
     const size_t end = first + rows < p.batch ? first + rows : p.batch;
-    const float2 lambda = ln.load32(p.decay);
-    const float2 rate = make_float2(rate_of(lambda.x, p.exponent), rate_of(lambda.y, p.exponent));
+    const Pair rate = mul2(rates(ln.load32(p.decay), p.exponent), both(-1.f));
 #pragma unroll 4
     for (size_t b = first; b < end; ++b) {
         long long slot = static_cast<long long>(b);
         if (p.slots) slot = p.slots[b];
         T* h = static_cast<T*>(p.h) + b * p.dim;
         if (slot < 0 || slot >= static_cast<long long>(p.pool)) {
-            ln.store(h, make_float2(0.f, 0.f));
+            ln.store(h, both(0.f));
             continue;
         }
-        const float2 x = Raw<T>::get(ln.load(static_cast<const T*>(p.x) + b * p.x_row));
-        const float2 r = Raw<T>::get(ln.load(static_cast<const T*>(p.r) + b * p.r_row));
-        const float2 i = Raw<T>::get(ln.load(static_cast<const T*>(p.i) + b * p.i_row));
-        const float2 s = ln.load32(p.state + static_cast<size_t>(slot) * p.dim);
-        const Coefficients c0 = coefficients(rate.x, r.x, i.x), c1 = coefficients(rate.y, r.y, i.y);
-        const float2 n = make_float2(fmaf(c0.a, s.x, c0.m * c0.si * x.x), fmaf(c1.a, s.y, c1.m * c1.si * x.y));
+        const Pair x = Raw<T>::get(ln.load(static_cast<const T*>(p.x) + b * p.x_row));
+        const Pair r = Raw<T>::get(ln.load(static_cast<const T*>(p.r) + b * p.r_row));
+        const Pair i = Raw<T>::get(ln.load(static_cast<const T*>(p.i) + b * p.i_row));
+        const Pair s = ln.load32(p.state + static_cast<size_t>(slot) * p.dim);
+        Pair a, m2;
+        decay(mul2(rate, sigmoid(r)), a, m2);
+        const Pair n = fma2(a, s, mul2(mul2(mul2(m2, inverse_root(m2)), sigmoid(i)), x));
         ln.store(h, n);
         ln.store32(p.new_state + static_cast<size_t>(slot) * p.dim, n);
     }

@@ -101,9 +101,8 @@ cudaError_t launch_step_typed(const GatedStepArgs& a, cudaStream_t stream) {
 }  // namespace
 
 int gated_scan_cluster(int batch, int length, int dim, bool backward) {
-    (void)backward;
     const size_t columns = static_cast<size_t>(ceil_div(dim, kChannels)) * batch;
-    const int tiles = ceil_div(length, kTile);
+    const int tiles = ceil_div(length, backward ? kBackwardTile : kForwardTile);
     int best = 1;
     double least = 0;
     for (int k = 1; k <= kGatedScanMaxCluster; k *= 2) {
