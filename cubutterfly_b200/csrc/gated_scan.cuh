@@ -101,10 +101,16 @@ struct Raw<float> {
     static CUBF_DEV void store_vec(float* p, float2 f) { __stcs(reinterpret_cast<float2*>(p), f); }
 };
 
-// The lane's two channels: adjacent where every row is aligned for pair
-// accesses (VEC), else 32 apart, so that scalar accesses still coalesce.
-template <bool VEC>
+// How a kernel reaches its rows, by the alignment of every row of every
+// tensor: copied to shared memory in 16-byte pieces ahead of their use; pair
+// by pair; or value by value.
+enum Access : int { kScalar = 0, kPairs = 1, kAsync = 2 };
+
+// The lane's two channels: adjacent with pair accesses, else 32 apart, so
+// that scalar accesses still coalesce.
+template <Access ACCESS>
 struct Lane {
+    static constexpr bool VEC = ACCESS != kScalar;
     int ch;
     bool ok0, ok1;
     CUBF_DEV Lane(int c0, int lane, int dim) {
@@ -139,14 +145,68 @@ struct Lane {
     }
 };
 
-// Brings the rows [t, t + ROWS) of a CTA's channels towards L2: the loads of
-// the next turn then wait for L2 only, and hold no registers meanwhile.
-template <int ROWS, typename T>
-CUBF_DEV void prefetch_rows(const T* base, size_t stride, int c0, int t, int lane, int length, int dim) {
-    const int row = t + lane % ROWS, col = c0 + lane / ROWS * (kChannels * ROWS / 32);
-    if (row < length && col < dim)
-        asm volatile("prefetch.global.L2 [%0];" ::"l"(base + static_cast<size_t>(row) * stride + col));
-}
+// The rows of a warp's tokens, N tensors of STEPS tokens x 64 channels each.
+// With kAsync a warp copies its own rows into its own shared memory (no
+// barrier beyond the warp's), STAGES tiles deep: the copies of a later tile
+// are in flight while this one is worked on, and hold no registers.  Channels
+// past the end are zero; tokens past the end are what `tail` says.
+template <typename T, int N, int STEPS, int STAGES, Access ACCESS>
+struct Rows {
+    static constexpr int kBytes = ACCESS == kAsync ? N * STEPS * kChannels * static_cast<int>(sizeof(T)) : 0;
+    static constexpr int kCopies = STEPS * kChannels * static_cast<int>(sizeof(T)) / 16 / 32;  // per lane and tensor
+    static constexpr int kPerRow = kChannels * static_cast<int>(sizeof(T)) / 16;               // 16-byte pieces of a row
+    const T* base[N];
+    size_t stride[N];
+    unsigned char* mine;  // this warp's stages
+    int lane, c0, length, dim;
+
+    CUBF_DEV const T* word(int stage, int n, int s) const {
+        return reinterpret_cast<const T*>(mine + stage * kBytes) + (n * STEPS + s) * kChannels;
+    }
+    // starts the copies of tokens [t, t + STEPS) and closes their group
+    CUBF_DEV void fetch(int stage, int t) const {
+        if constexpr (ACCESS == kAsync) {
+            const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(mine + stage * kBytes)) + lane * 16;
+            const int row = t + lane / kPerRow, col = c0 + lane % kPerRow * (16 / static_cast<int>(sizeof(T)));
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const T* src = base[n] + static_cast<size_t>(row) * stride[n] + col;
+#pragma unroll
+                for (int k = 0; k < kCopies; ++k) {
+                    const int bytes = row + k * (32 / kPerRow) < length && row >= 0 && col < dim ? 16 : 0;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (n * kCopies + k) * 512),
+                                 "l"(bytes ? src : base[n]), "r"(bytes)
+                                 : "memory");
+                    src += (32 / kPerRow) * stride[n];
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+    }
+    // waits for the oldest of STAGES groups
+    CUBF_DEV void arrive() const {
+        if constexpr (ACCESS == kAsync) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+            __syncwarp();
+        }
+    }
+    CUBF_DEV typename Raw<T>::Word get(const Lane<ACCESS>& ln, int stage, int n, int t, int s,
+                                       typename Raw<T>::Word tail) const {
+        if constexpr (ACCESS == kAsync)
+            return *reinterpret_cast<const typename Raw<T>::Word*>(word(stage, n, s) + 2 * lane);
+        else
+            return t + s < length ? ln.load(base[n] + static_cast<size_t>(t + s) * stride[n]) : tail;
+    }
+    // gives tokens past the end the value `tail` (async copies leave zeros there)
+    CUBF_DEV void close(int stage, int n, int t, typename Raw<T>::Word tail) const {
+        if constexpr (ACCESS == kAsync) {
+            if (t + STEPS <= length) return;
+            for (int s = 0; s < STEPS; ++s)
+                if (t + s >= length)
+                    *reinterpret_cast<typename Raw<T>::Word*>(const_cast<T*>(word(stage, n, s)) + 2 * lane) = tail;
+        }
+    }
+};
 
 // ---- the arithmetic of a token ----------------------------------------------------------------
 CUBF_DEV float ex2(float x) {
@@ -296,20 +356,28 @@ struct Maps {
     Map cta[2][kGatedScanMaxCluster][32];
 };
 
-template <typename T, bool PACKED, bool VEC>
+template <typename T, Access ACCESS>
+using ForwardRows = Rows<T, 3, kForwardSteps, sizeof(T) == 2 ? 2 : 1, ACCESS>;
+
+template <typename T, bool PACKED, Access ACCESS>
 __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArgs p, int cluster, int tiles) {
     constexpr int kSteps = kForwardSteps, kTile = kForwardTile;
+    constexpr int kStages = sizeof(T) == 2 ? 2 : 1;
+    using Word = typename Raw<T>::Word;
+    extern __shared__ __align__(16) unsigned char staged[];
     __shared__ Maps maps;
     pdl_begin();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rank = cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
     const unsigned column = blockIdx.x / cluster;
     const int c0 = static_cast<int>(column % tiles) * kChannels;
-    const Lane<VEC> ln(c0, lane, p.dim);
+    const Lane<ACCESS> ln(c0, lane, p.dim);
     const size_t b = column / tiles;
-    const T* x = static_cast<const T*>(p.x) + b * p.x_batch;
-    const T* r = static_cast<const T*>(p.r) + b * p.r_batch;
-    const T* g = static_cast<const T*>(p.i) + b * p.i_batch;
+    ForwardRows<T, ACCESS> rows{{static_cast<const T*>(p.x) + b * p.x_batch, static_cast<const T*>(p.r) + b * p.r_batch,
+                                 static_cast<const T*>(p.i) + b * p.i_batch},
+                                {p.x_token, p.r_token, p.i_token},
+                                staged + warp * kStages * ForwardRows<T, ACCESS>::kBytes,
+                                lane, c0, p.length, p.dim};
     T* out = static_cast<T*>(p.h) + b * static_cast<size_t>(p.length) * p.dim;
     const Pair rate = mul2(rates(ln.load32(p.decay), p.exponent), both(-1.f));
     const int stride = cluster * kTile;
@@ -329,38 +397,27 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
     if (!PACKED && p.initial) carry = ln.load32(p.initial + b * p.dim);
 
     const int rounds = (p.length + stride - 1) / stride;
+#pragma unroll
+    for (int k = 0; k < kStages; ++k) rows.fetch(k, t0 + k * stride);
     for (int round = 0; round < rounds; ++round, t0 += stride) {
-        const int buf = round & 1;
+        const int buf = round & 1, stage = kStages == 2 ? buf : 0;
         // Tokens past the end are a shut gate (r = -inf: a = 1) over x = 0:
         // the identity map.
         Pair a[kSteps], u[kSteps];
-        {
-            typename Raw<T>::Word rx[kSteps], rr[kSteps], ri[kSteps];
-            const T *px = x + static_cast<size_t>(t0) * p.x_token, *pr = r + static_cast<size_t>(t0) * p.r_token,
-                    *pi = g + static_cast<size_t>(t0) * p.i_token;
+        rows.arrive();
+        rows.close(stage, 1, t0, Raw<T>::lowest());
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                const bool in = t0 + s < p.length;
-                rx[s] = in ? ln.load(px) : Raw<T>::zero();
-                rr[s] = in ? ln.load(pr) : Raw<T>::lowest();
-                ri[s] = in ? ln.load(pi) : Raw<T>::zero();
-                px += p.x_token;
-                pr += p.r_token;
-                pi += p.i_token;
-            }
-            if (round + 1 < rounds) {
-                prefetch_rows<kSteps>(x, p.x_token, c0, t0 + stride, lane, p.length, p.dim);
-                prefetch_rows<kSteps>(r, p.r_token, c0, t0 + stride, lane, p.length, p.dim);
-                prefetch_rows<kSteps>(g, p.i_token, c0, t0 + stride, lane, p.length, p.dim);
-            }
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                Pair m2;
-                decay(mul2(rate, sigmoid(Raw<T>::get(rr[s]))), a[s], m2);
-                const Pair m = mul2(m2, inverse_root(m2));
-                u[s] = mul2(mul2(m, sigmoid(Raw<T>::get(ri[s]))), Raw<T>::get(rx[s]));
-            }
+        for (int s = 0; s < kSteps; ++s) {
+            const Word rx = rows.get(ln, stage, 0, t0, s, Raw<T>::zero());
+            const Word rr = rows.get(ln, stage, 1, t0, s, Raw<T>::lowest());
+            const Word ri = rows.get(ln, stage, 2, t0, s, Raw<T>::zero());
+            Pair m2;
+            decay(mul2(rate, sigmoid(Raw<T>::get(rr))), a[s], m2);
+            const Pair m = mul2(m2, inverse_root(m2));
+            u[s] = mul2(mul2(m, sigmoid(Raw<T>::get(ri))), Raw<T>::get(rx));
         }
+        __syncwarp();  // the warp has read the tile
+        rows.fetch(stage, t0 + kStages * stride);
         Pair A = both(1.f), H = both(0.f);
         unsigned starts = 0;
         Walker from;
@@ -420,11 +477,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
         if (p.chunk_states && t0 % kGatedScanChunk == 0 && t0 < p.length)
             ln.store32(p.chunk_states + (b * chunks + static_cast<size_t>(t0 / kGatedScanChunk)) * p.dim, h);
         T* po = out + static_cast<size_t>(t0) * p.dim;
-        if (plain) {
+        if (plain && t0 + kSteps <= p.length) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 h = fma2(a[s], h, u[s]);
-                if (t0 + s < p.length) ln.store(po, h);
+                ln.store(po, h);
                 po += p.dim;
             }
         } else {
@@ -433,8 +490,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
                 if (t0 + s >= p.length) continue;
                 h = (starts >> s) & 1u ? u[s] : fma2(a[s], h, u[s]);
                 ln.store(po, h);
-                from.seek(t0 + s);
-                if (t0 + s + 1 == from.stop) ln.store32(p.last + static_cast<size_t>(from.at) * p.dim, h);
+                if constexpr (PACKED) {
+                    from.seek(t0 + s);
+                    if (t0 + s + 1 == from.stop) ln.store32(p.last + static_cast<size_t>(from.at) * p.dim, h);
+                }
                 po += p.dim;
             }
         }
@@ -460,22 +519,30 @@ struct BackMaps {
     Pair sum[kWarps][32];
 };
 
-template <typename T, bool PACKED, bool VEC>
+template <typename T, Access ACCESS>
+using BackwardRows = Rows<T, 4, kBackwardSteps, sizeof(T) == 2 ? 2 : 1, ACCESS>;
+
+template <typename T, bool PACKED, Access ACCESS>
 __global__ void __launch_bounds__(kWarps * 32, 2)
     gated_scan_backward_kernel(GatedScanArgs p, int cluster, int tiles) {
     constexpr int kSteps = kBackwardSteps, kTile = kBackwardTile;
+    constexpr int kStages = sizeof(T) == 2 ? 2 : 1;
+    using Word = typename Raw<T>::Word;
+    extern __shared__ __align__(16) unsigned char staged[];
     __shared__ BackMaps maps;
     pdl_begin();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int rank = cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
     const unsigned column = blockIdx.x / cluster;
     const int c0 = static_cast<int>(column % tiles) * kChannels;
-    const Lane<VEC> ln(c0, lane, p.dim);
+    const Lane<ACCESS> ln(c0, lane, p.dim);
     const size_t b = column / tiles;
-    const T* x = static_cast<const T*>(p.x) + b * p.x_batch;
-    const T* r = static_cast<const T*>(p.r) + b * p.r_batch;
-    const T* g = static_cast<const T*>(p.i) + b * p.i_batch;
-    const T* dh = static_cast<const T*>(p.d_h) + b * p.dh_batch;
+    BackwardRows<T, ACCESS> rows{{static_cast<const T*>(p.x) + b * p.x_batch, static_cast<const T*>(p.r) + b * p.r_batch,
+                                  static_cast<const T*>(p.i) + b * p.i_batch,
+                                  static_cast<const T*>(p.d_h) + b * p.dh_batch},
+                                 {p.x_token, p.r_token, p.i_token, p.dh_token},
+                                 staged + warp * kStages * BackwardRows<T, ACCESS>::kBytes,
+                                 lane, c0, p.length, p.dim};
     const size_t out = b * static_cast<size_t>(p.length) * p.dim;
     T* dx = static_cast<T*>(p.d_x) + out;
     T* dr = static_cast<T*>(p.d_r) + out;
@@ -498,42 +565,43 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     if (!PACKED && p.d_last) carry = ln.load32(p.d_last + b * p.dim);
     Pair sum = both(0.f);    // of e
 
+#pragma unroll
+    for (int k = 0; k < kStages; ++k) rows.fetch((rounds - 1 - k) & (kStages - 1), (rounds - 1 - k) * stride + rank * kTile + warp * kSteps);
     for (int round = rounds - 1; round >= 0; --round) {
-        const int buf = round & 1;
+        const int buf = round & 1, stage = kStages == 2 ? buf : 0;
         const int t0 = round * stride + rank * kTile + warp * kSteps;
-        typename Raw<T>::Word rx[kSteps], rd[kSteps];
+        // x and dh are read where they are used, from shared memory; other
+        // accesses keep them
+        Word kx[ACCESS == kAsync ? 1 : kSteps], kd[ACCESS == kAsync ? 1 : kSteps];
         Pair a[kSteps], v[kSteps], im[kSteps], sr[kSteps];
-        {
-            typename Raw<T>::Word rr[kSteps], ri[kSteps];
-            const T *px = x + static_cast<size_t>(t0) * p.x_token, *pr = r + static_cast<size_t>(t0) * p.r_token,
-                    *pi = g + static_cast<size_t>(t0) * p.i_token, *pd = dh + static_cast<size_t>(t0) * p.dh_token;
+        rows.arrive();
+        rows.close(stage, 1, t0, Raw<T>::lowest());
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                const bool in = t0 + s < p.length;
-                rx[s] = in ? ln.load(px) : Raw<T>::zero();
-                rr[s] = in ? ln.load(pr) : Raw<T>::lowest();
-                ri[s] = in ? ln.load(pi) : Raw<T>::zero();
-                rd[s] = in ? ln.load(pd) : Raw<T>::zero();
-                px += p.x_token;
-                pr += p.r_token;
-                pi += p.i_token;
-                pd += p.dh_token;
+        for (int s = 0; s < kSteps; ++s) {
+            if constexpr (ACCESS != kAsync) {
+                kx[s] = rows.get(ln, stage, 0, t0, s, Raw<T>::zero());
+                kd[s] = rows.get(ln, stage, 3, t0, s, Raw<T>::zero());
             }
-            if (round > 0) {
-                prefetch_rows<kSteps>(x, p.x_token, c0, t0 - stride, lane, p.length, p.dim);
-                prefetch_rows<kSteps>(r, p.r_token, c0, t0 - stride, lane, p.length, p.dim);
-                prefetch_rows<kSteps>(g, p.i_token, c0, t0 - stride, lane, p.length, p.dim);
-                prefetch_rows<kSteps>(dh, p.dh_token, c0, t0 - stride, lane, p.length, p.dim);
-            }
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                Pair m2;
-                sr[s] = sigmoid(Raw<T>::get(rr[s]));
-                decay(mul2(rate, sr[s]), a[s], m2);
-                im[s] = inverse_root(m2);
-                v[s] = mul2(mul2(m2, im[s]), sigmoid(Raw<T>::get(ri[s])));
-            }
+            const Word rr = rows.get(ln, stage, 1, t0, s, Raw<T>::lowest());
+            const Word ri = rows.get(ln, stage, 2, t0, s, Raw<T>::zero());
+            Pair m2;
+            sr[s] = sigmoid(Raw<T>::get(rr));
+            decay(mul2(rate, sr[s]), a[s], m2);
+            im[s] = inverse_root(m2);
+            v[s] = mul2(mul2(m2, im[s]), sigmoid(Raw<T>::get(ri)));
         }
+        auto x_of = [&](int s) {
+            if constexpr (ACCESS == kAsync)
+                return Raw<T>::get(rows.get(ln, stage, 0, t0, s, Raw<T>::zero()));
+            else
+                return Raw<T>::get(kx[s]);
+        };
+        auto dh_of = [&](int s) {
+            if constexpr (ACCESS == kAsync)
+                return Raw<T>::get(rows.get(ln, stage, 3, t0, s, Raw<T>::zero()));
+            else
+                return Raw<T>::get(kd[s]);
+        };
         Pair h = both(0.f);  // before the tile, from the forward
         const int chunk = round * cluster + rank;
         if (chunk < chunks) h = ln.load32(p.chunk_states + (b * chunks + chunk) * static_cast<size_t>(p.dim));
@@ -551,7 +619,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         }
         // dh with the final states' gradients where a sequence ends
         auto arriving = [&](int s, int at) {
-            Pair d = Raw<T>::get(rd[s]);
+            Pair d = dh_of(s);
             if (PACKED && ((ends >> s) & 1u) && p.d_last)
                 d = add2(d, ln.load32(p.d_last + static_cast<size_t>(at) * p.dim));
             return d;
@@ -565,16 +633,16 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 A = mul2(A, a[s]);
-                H = fma2(a[s], H, mul2(v[s], Raw<T>::get(rx[s])));
+                H = fma2(a[s], H, mul2(v[s], x_of(s)));
             }
 #pragma unroll
-            for (int s = kSteps - 1; s >= 0; --s) R = mul2(a[s], add2(Raw<T>::get(rd[s]), R));
+            for (int s = kSteps - 1; s >= 0; --s) R = mul2(a[s], add2(dh_of(s), R));
         } else {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 if (t0 + s >= p.length) continue;
                 seq.seek(t0 + s);
-                Pair u = mul2(v[s], Raw<T>::get(rx[s]));
+                Pair u = mul2(v[s], x_of(s));
                 if (t0 + s + 1 == seq.stop) ends |= 1u << s;
                 if (t0 + s == seq.start) {
                     starts |= 1u << s;
@@ -635,7 +703,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 before[s] = h;
-                h = fma2(a[s], h, mul2(v[s], Raw<T>::get(rx[s])));
+                h = fma2(a[s], h, mul2(v[s], x_of(s)));
             }
         } else {
             at = seq.at;
@@ -646,15 +714,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
                 from.seek(t0 + s);
                 if ((starts >> s) & 1u)
                     before[s] = p.initial ? ln.load32(p.initial + static_cast<size_t>(from.at) * p.dim) : both(0.f);
-                h = fma2(a[s], before[s], mul2(v[s], Raw<T>::get(rx[s])));
+                h = fma2(a[s], before[s], mul2(v[s], x_of(s)));
             }
         }
         const size_t o = static_cast<size_t>(t0) * p.dim;
 #pragma unroll
         for (int s = kSteps - 1; s >= 0; --s) {
             if (t0 + s >= p.length) continue;
-            const Pair fx = Raw<T>::get(rx[s]);
-            const Pair G = add2(plain ? Raw<T>::get(rd[s]) : arriving(s, at), P);
+            const Pair fx = x_of(s);
+            const Pair G = add2(plain ? dh_of(s) : arriving(s, at), P);
             const Pair gx = mul2(G, v[s]), si = mul2(v[s], im[s]);
             const Pair gi = mul2(mul2(gx, fx), sub2(both(1.f), si));
             P = mul2(a[s], G);
@@ -671,6 +739,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
                 at = previous(at, t0 + s);
             }
         }
+        __syncwarp();  // the warp has read the tile
+        rows.fetch(stage, t0 - kStages * stride);
     }
     if (!PACKED && p.d_initial && rank == 0 && warp == 0) ln.store32(p.d_initial + b * p.dim, carry);
     maps.sum[warp][lane] = sum;
@@ -706,12 +776,12 @@ __global__ void __launch_bounds__(256) gated_scan_decay_kernel(GatedScanArgs p, 
 // A warp takes 64 channels of `rows` consecutive requests; a request whose
 // slot lies outside the pool is padding: its output is zero and no state is
 // touched.
-template <typename T, bool VEC>
+template <typename T, Access ACCESS>
 __global__ void __launch_bounds__(128) gated_scan_step_kernel(GatedStepArgs p, int tiles, int rows) {
     pdl_begin();
     const int lane = threadIdx.x & 31;
     const unsigned task = blockIdx.x * 4 + (threadIdx.x >> 5);
-    const Lane<VEC> ln(static_cast<int>(task % tiles) * kChannels, lane, p.dim);
+    const Lane<ACCESS> ln(static_cast<int>(task % tiles) * kChannels, lane, p.dim);
     const size_t first = static_cast<size_t>(task / tiles) * rows;
     if (first >= p.batch) return;
     const size_t end = first + rows < p.batch ? first + rows : p.batch;

@@ -12,9 +12,10 @@ using namespace scan;
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 template <typename... Args>
-cudaError_t launch_clusters(void (*kernel)(Args...), unsigned grid, unsigned threads, int cluster, cudaStream_t stream,
-                            Args... args) {
+cudaError_t launch_clusters(void (*kernel)(Args...), unsigned grid, unsigned threads, int smem, int cluster,
+                            cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg{};
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(threads);
     cfg.stream = stream;
@@ -30,47 +31,71 @@ cudaError_t launch_clusters(void (*kernel)(Args...), unsigned grid, unsigned thr
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-// Pair accesses need every row of every tensor to start on a pair boundary.
+// The widest access every row of every tensor is aligned for.
 template <typename T>
-struct PairAligned {
-    uintptr_t bits = 0;
-    PairAligned& pointer(const void* p) {
-        bits |= reinterpret_cast<uintptr_t>(p) & (2 * sizeof(T) - 1);
+struct Alignment {
+    uintptr_t bits = 0;  // of addresses and strides in bytes
+    Alignment& pointer(const void* p) {
+        bits |= reinterpret_cast<uintptr_t>(p);
         return *this;
     }
-    PairAligned& stride(size_t elements) {
-        bits |= elements & 1;
+    Alignment& stride(size_t elements) {
+        bits |= elements * sizeof(T);
         return *this;
+    }
+    Access access() const {
+        if ((bits & 15) == 0) return kAsync;
+        return (bits & (2 * sizeof(T) - 1)) == 0 ? kPairs : kScalar;
     }
 };
 
 template <typename T>
-bool pair_aligned(const GatedScanArgs& a, bool backward) {
-    PairAligned<T> v;
+Access access_of(const GatedScanArgs& a, bool backward) {
+    Alignment<T> v;
     v.stride(static_cast<size_t>(a.dim)).pointer(a.x).pointer(a.r).pointer(a.i);
     v.stride(a.x_batch).stride(a.r_batch).stride(a.i_batch).stride(a.x_token).stride(a.r_token).stride(a.i_token);
     if (backward)
         v.pointer(a.d_h).pointer(a.d_x).pointer(a.d_r).pointer(a.d_i).stride(a.dh_batch).stride(a.dh_token);
     else
         v.pointer(a.h);
-    return v.bits == 0;
+    return v.access();
 }
 
-template <typename T, bool PACKED, bool VEC>
-cudaError_t launch_shape(const GatedScanArgs& a, bool backward, cudaStream_t stream) {
+template <typename T, bool PACKED, Access ACCESS, bool BACKWARD>
+cudaError_t launch_kernel(const GatedScanArgs& a, cudaStream_t stream) {
+    static KernelSetup setup;
+    const auto kernel = [] {
+        if constexpr (BACKWARD)
+            return &gated_scan_backward_kernel<T, PACKED, ACCESS>;
+        else
+            return &gated_scan_kernel<T, PACKED, ACCESS>;
+    }();
+    constexpr int kStages = sizeof(T) == 2 ? 2 : 1;
+    constexpr int smem = kWarps * kStages * (BACKWARD ? BackwardRows<T, ACCESS>::kBytes : ForwardRows<T, ACCESS>::kBytes);
+    int cap = 0;
+    // two CTAs per SM fit only in the largest carveout
+    cudaError_t e = setup_kernel(setup, kernel, kWarps * 32, smem, &cap, ACCESS == kAsync);
+    if (e != cudaSuccess) return e;
     const int tiles = ceil_div(a.dim, kChannels);
-    const int cluster = gated_scan_cluster(a.batch, a.length, a.dim, backward);
+    const int cluster = gated_scan_cluster(a.batch, a.length, a.dim, BACKWARD);
     const size_t grid = static_cast<size_t>(tiles) * a.batch * cluster;
     if (grid > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
-    return launch_clusters(backward ? &gated_scan_backward_kernel<T, PACKED, VEC> : &gated_scan_kernel<T, PACKED, VEC>,
-                           static_cast<unsigned>(grid), kWarps * 32u, cluster, stream, a, cluster, tiles);
+    return launch_clusters(kernel, static_cast<unsigned>(grid), kWarps * 32u, smem, cluster, stream, a, cluster, tiles);
+}
+
+template <typename T, bool PACKED, bool BACKWARD>
+cudaError_t launch_access(const GatedScanArgs& a, cudaStream_t stream) {
+    switch (access_of<T>(a, BACKWARD)) {
+        case kAsync: return launch_kernel<T, PACKED, kAsync, BACKWARD>(a, stream);
+        case kPairs: return launch_kernel<T, PACKED, kPairs, BACKWARD>(a, stream);
+        default: return launch_kernel<T, PACKED, kScalar, BACKWARD>(a, stream);
+    }
 }
 
 template <typename T>
 cudaError_t launch_typed(const GatedScanArgs& a, bool backward, cudaStream_t stream) {
-    const bool vec = pair_aligned<T>(a, backward);
-    if (a.offsets) return vec ? launch_shape<T, true, true>(a, backward, stream) : launch_shape<T, true, false>(a, backward, stream);
-    return vec ? launch_shape<T, false, true>(a, backward, stream) : launch_shape<T, false, false>(a, backward, stream);
+    if (a.offsets) return backward ? launch_access<T, true, true>(a, stream) : launch_access<T, true, false>(a, stream);
+    return backward ? launch_access<T, false, true>(a, stream) : launch_access<T, false, false>(a, stream);
 }
 
 cudaError_t launch_any(BlockType type, const GatedScanArgs& a, bool backward, cudaStream_t stream) {
@@ -84,7 +109,7 @@ cudaError_t launch_any(BlockType type, const GatedScanArgs& a, bool backward, cu
 
 template <typename T>
 cudaError_t launch_step_typed(const GatedStepArgs& a, cudaStream_t stream) {
-    PairAligned<T> v;
+    Alignment<T> v;
     v.stride(static_cast<size_t>(a.dim)).pointer(a.x).pointer(a.r).pointer(a.i).pointer(a.h);
     v.stride(a.x_row).stride(a.r_row).stride(a.i_row);
     const int tiles = ceil_div(a.dim, kChannels);
@@ -94,7 +119,7 @@ cudaError_t launch_step_typed(const GatedStepArgs& a, cudaStream_t stream) {
     const size_t tasks = (a.batch + rows - 1) / rows * tiles;
     const size_t grid = (tasks + 3) / 4;
     if (grid > 0x7fffffffULL || rows > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
-    return launch_dependent(v.bits == 0 ? &gated_scan_step_kernel<T, true> : &gated_scan_step_kernel<T, false>,
+    return launch_dependent(v.access() == kScalar ? &gated_scan_step_kernel<T, kScalar> : &gated_scan_step_kernel<T, kPairs>,
                             static_cast<unsigned>(grid), 128u, 0, stream, a, tiles, static_cast<int>(rows));
 }
 
