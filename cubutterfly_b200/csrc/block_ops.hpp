@@ -57,8 +57,9 @@ struct GatedStepArgs {
     float exponent;
 };
 
-// CTAs per cluster along time for a batch of this shape (1, 2, 4 or 8).
-int gated_scan_cluster(int batch, int length, int dim, bool backward);
+// CTAs per cluster along time for a batch of this shape (1, 2, 4 or 8), each
+// with `tile` tokens at a time; the backward's tile is kGatedScanChunk.
+int gated_scan_cluster(int batch, int length, int dim, int tile);
 cudaError_t launch_gated_scan(BlockType type, const GatedScanArgs& args, cudaStream_t stream);
 cudaError_t launch_gated_scan_backward(BlockType type, const GatedScanArgs& args, cudaStream_t stream);
 cudaError_t launch_gated_scan_step(BlockType type, const GatedStepArgs& args, cudaStream_t stream);

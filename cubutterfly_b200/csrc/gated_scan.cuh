@@ -34,12 +34,14 @@ using Pair = f32x2::P;
 
 constexpr int kWarps = 8;                  // warps per CTA, consecutive in time
 constexpr int kChannels = 64;              // channels per CTA, two per lane
-constexpr int kForwardSteps = 16;          // tokens per thread and tile
+static_assert(kGatedScanMaxCluster <= kWarps, "a warp reads the map of each CTA of the cluster");
+// Tokens per thread and tile: as many as two CTAs' registers and shared
+// memory allow.
+template <typename T>
+constexpr int kForwardSteps = sizeof(T) == 2 ? 16 : 8;
 constexpr int kBackwardSteps = 8;
-constexpr int kForwardTile = kForwardSteps * kWarps;    // tokens per CTA tile
-constexpr int kBackwardTile = kBackwardSteps * kWarps;
-static_assert(kBackwardTile == kGatedScanChunk, "the backward restarts from the states the forward kept");
-static_assert(kGatedScanChunk % kForwardSteps == 0, "chunks begin where a forward thread does");
+static_assert(kBackwardSteps * kWarps == kGatedScanChunk, "the backward restarts from the states the forward kept");
+static_assert(kGatedScanChunk % kForwardSteps<__half> == 0, "chunks begin where a forward thread does");
 
 CUBF_DEV Pair both(float v) { return f32x2::pk(v, v); }
 CUBF_DEV Pair pair(float2 v) { return f32x2::pk(v.x, v.y); }
@@ -76,7 +78,7 @@ struct Raw {
             return f32x2::pk(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
         }
     }
-    static CUBF_DEV void store_vec(T* p, float2 f) {
+    static CUBF_DEV Word word_of(float2 f) {
         uint32_t w;
         if constexpr (std::is_same<T, __half>::value) {
             const __half2 h = __float22half2_rn(f);
@@ -85,8 +87,9 @@ struct Raw {
             const __nv_bfloat162 h = __float22bfloat162_rn(f);
             memcpy(&w, &h, 4);
         }
-        __stcs(reinterpret_cast<unsigned int*>(p), w);
+        return w;
     }
+    static CUBF_DEV void store_vec(T* p, float2 f) { __stcs(reinterpret_cast<unsigned int*>(p), word_of(f)); }
 };
 template <>
 struct Raw<float> {
@@ -98,6 +101,7 @@ struct Raw<float> {
         return make_float2(ok0 ? __ldcs(p) : 0.f, ok1 ? __ldcs(p + 32) : 0.f);
     }
     static CUBF_DEV Pair get(Word w) { return pair(w); }
+    static CUBF_DEV Word word_of(float2 f) { return f; }
     static CUBF_DEV void store_vec(float* p, float2 f) { __stcs(reinterpret_cast<float2*>(p), f); }
 };
 
@@ -148,39 +152,80 @@ struct Lane {
 // The rows of a warp's tokens, N tensors of STEPS tokens x 64 channels each.
 // With kAsync a warp copies its own rows into its own shared memory (no
 // barrier beyond the warp's), STAGES tiles deep: the copies of a later tile
-// are in flight while this one is worked on, and hold no registers.  Channels
-// past the end are zero; tokens past the end are what `tail` says.
-template <typename T, int N, int STEPS, int STAGES, Access ACCESS>
+// are in flight while this one is worked on, and hold no registers.  Results
+// take the place of words that have been read and leave in 16-byte pieces:
+// stored from registers, each pair would cost as many instructions in
+// addresses as its arithmetic.  Channels past the end are zero; tokens past
+// the end are what `tail` says.
+template <typename T, int N, int STEPS_, int STAGES_, Access ACCESS>
 struct Rows {
+    static constexpr int STEPS = STEPS_, STAGES = STAGES_;
     static constexpr int kBytes = ACCESS == kAsync ? N * STEPS * kChannels * static_cast<int>(sizeof(T)) : 0;
-    static constexpr int kCopies = STEPS * kChannels * static_cast<int>(sizeof(T)) / 16 / 32;  // per lane and tensor
-    static constexpr int kPerRow = kChannels * static_cast<int>(sizeof(T)) / 16;               // 16-byte pieces of a row
+    static constexpr int kPerRow = kChannels * static_cast<int>(sizeof(T)) / 16;  // 16-byte pieces of a row
+    static constexpr int kRowsPer = 32 / kPerRow;                                 // rows a warp copies at a time
+    static constexpr int kCopies = STEPS / kRowsPer;                              // per lane and tensor
+    using Word = typename Raw<T>::Word;
     const T* base[N];
     size_t stride[N];
+    const T* next[N];     // this lane's first piece of the tile fetched next
     unsigned char* mine;  // this warp's stages
     int lane, c0, length, dim;
 
-    CUBF_DEV const T* word(int stage, int n, int s) const {
-        return reinterpret_cast<const T*>(mine + stage * kBytes) + (n * STEPS + s) * kChannels;
+    CUBF_DEV int piece() const { return lane % kPerRow * (16 / static_cast<int>(sizeof(T))); }
+
+    CUBF_DEV void init(unsigned char* shared, int lane_, int c0_, int length_, int dim_, int first) {
+        mine = shared;
+        lane = lane_;
+        c0 = c0_;
+        length = length_;
+        dim = dim_;
+        if constexpr (ACCESS == kAsync) {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                next[n] = base[n] + static_cast<ptrdiff_t>(first + lane / kPerRow) * static_cast<ptrdiff_t>(stride[n]) +
+                          c0 + piece();
+        }
     }
-    // starts the copies of tokens [t, t + STEPS) and closes their group
-    CUBF_DEV void fetch(int stage, int t) const {
+    CUBF_DEV Word* word(int stage, int n, int s) const {
+        return reinterpret_cast<Word*>(reinterpret_cast<T*>(mine + stage * kBytes) + (n * STEPS + s) * kChannels +
+                                       2 * lane);
+    }
+    // starts the copies of tokens [t, t + STEPS), closes their group, and
+    // moves on by `advance` tokens
+    CUBF_DEV void fetch(int stage, int t, int advance) {
         if constexpr (ACCESS == kAsync) {
             const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(mine + stage * kBytes)) + lane * 16;
-            const int row = t + lane / kPerRow, col = c0 + lane % kPerRow * (16 / static_cast<int>(sizeof(T)));
+            if (t >= 0 && t + STEPS <= length && c0 + kChannels <= dim) {
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const T* src = base[n] + static_cast<size_t>(row) * stride[n] + col;
+                for (int n = 0; n < N; ++n) {
+                    const T* src = next[n];
 #pragma unroll
-                for (int k = 0; k < kCopies; ++k) {
-                    const int bytes = row + k * (32 / kPerRow) < length && row >= 0 && col < dim ? 16 : 0;
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (n * kCopies + k) * 512),
-                                 "l"(bytes ? src : base[n]), "r"(bytes)
-                                 : "memory");
-                    src += (32 / kPerRow) * stride[n];
+                    for (int k = 0; k < kCopies; ++k) {
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + (n * kCopies + k) * 512),
+                                     "l"(src)
+                                     : "memory");
+                        src += kRowsPer * stride[n];
+                    }
                 }
+            } else if (t < length && t + STEPS > 0) {
+                for (int n = 0; n < N; ++n)
+                    for (int k = 0; k < kCopies; ++k) {
+                        const int at = t + lane / kPerRow + k * kRowsPer, col = c0 + piece();
+                        const bool in = at >= 0 && at < length && col < dim;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                         dst + (n * kCopies + k) * 512),
+                                     "l"(in ? base[n] + static_cast<size_t>(at) * stride[n] + col : base[n]),
+                                     "r"(in ? 16 : 0)
+                                     : "memory");
+                    }
+            } else {
+                // nothing of the sequence: zeros, so that no stale word is computed with
+                for (int k = 0; k < N * kCopies; ++k)
+                    *reinterpret_cast<uint4*>(mine + stage * kBytes + lane * 16 + k * 512) = make_uint4(0, 0, 0, 0);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll
+            for (int n = 0; n < N; ++n) next[n] += static_cast<ptrdiff_t>(advance) * static_cast<ptrdiff_t>(stride[n]);
         }
     }
     // waits for the oldest of STAGES groups
@@ -190,20 +235,48 @@ struct Rows {
             __syncwarp();
         }
     }
-    CUBF_DEV typename Raw<T>::Word get(const Lane<ACCESS>& ln, int stage, int n, int t, int s,
-                                       typename Raw<T>::Word tail) const {
+    CUBF_DEV Word get(const Lane<ACCESS>& ln, int stage, int n, int t, int s, Word tail) const {
         if constexpr (ACCESS == kAsync)
-            return *reinterpret_cast<const typename Raw<T>::Word*>(word(stage, n, s) + 2 * lane);
+            return *word(stage, n, s);
         else
             return t + s < length ? ln.load(base[n] + static_cast<size_t>(t + s) * stride[n]) : tail;
     }
     // gives tokens past the end the value `tail` (async copies leave zeros there)
-    CUBF_DEV void close(int stage, int n, int t, typename Raw<T>::Word tail) const {
+    CUBF_DEV void close(int stage, int n, int t, Word tail) const {
         if constexpr (ACCESS == kAsync) {
             if (t + STEPS <= length) return;
             for (int s = 0; s < STEPS; ++s)
-                if (t + s >= length)
-                    *reinterpret_cast<typename Raw<T>::Word*>(const_cast<T*>(word(stage, n, s)) + 2 * lane) = tail;
+                if (t + s >= length) *word(stage, n, s) = tail;
+        }
+    }
+    // Token t + s of an output (rows of `dim` channels from `out`): into the
+    // place of tensor n's word, or straight to memory.  The caller has checked
+    // that the token exists unless ACCESS is kAsync.
+    CUBF_DEV void put(const Lane<ACCESS>& ln, int stage, int n, T* out, int t, int s, Pair v) const {
+        if constexpr (ACCESS == kAsync)
+            *word(stage, n, s) = Raw<T>::word_of(floats(v));
+        else
+            ln.store(out + static_cast<size_t>(t + s) * dim, v);
+    }
+    // writes the tile put in tensor n's place out
+    CUBF_DEV void flush(int stage, int n, T* out, int t) const {
+        if constexpr (ACCESS == kAsync) {
+            const unsigned char* src = mine + stage * kBytes + n * kCopies * 512 + lane * 16;
+            const int row = t + lane / kPerRow, col = c0 + piece();
+            T* dst = out + static_cast<size_t>(row) * dim + col;
+            if (t + STEPS <= length && c0 + kChannels <= dim) {
+#pragma unroll
+                for (int k = 0; k < kCopies; ++k) {
+                    __stcs(reinterpret_cast<uint4*>(dst), *reinterpret_cast<const uint4*>(src + k * 512));
+                    dst += static_cast<size_t>(kRowsPer) * dim;
+                }
+            } else {
+                for (int k = 0; k < kCopies; ++k) {
+                    if (row + k * kRowsPer < length && col < dim)
+                        __stcs(reinterpret_cast<uint4*>(dst), *reinterpret_cast<const uint4*>(src + k * 512));
+                    dst += static_cast<size_t>(kRowsPer) * dim;
+                }
+            }
         }
     }
 };
@@ -357,32 +430,36 @@ struct Maps {
 };
 
 template <typename T, Access ACCESS>
-using ForwardRows = Rows<T, 3, kForwardSteps, sizeof(T) == 2 ? 2 : 1, ACCESS>;
+using ForwardRows = Rows<T, 3, kForwardSteps<T>, 2, ACCESS>;
 
 template <typename T, bool PACKED, Access ACCESS>
 __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArgs p, int cluster, int tiles) {
-    constexpr int kSteps = kForwardSteps, kTile = kForwardTile;
-    constexpr int kStages = sizeof(T) == 2 ? 2 : 1;
+    using Tile = ForwardRows<T, ACCESS>;
+    constexpr int kSteps = Tile::STEPS, kTile = kSteps * kWarps;
     using Word = typename Raw<T>::Word;
     extern __shared__ __align__(16) unsigned char staged[];
     __shared__ Maps maps;
     pdl_begin();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int rank = cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
     const unsigned column = blockIdx.x / cluster;
     const int c0 = static_cast<int>(column % tiles) * kChannels;
     const Lane<ACCESS> ln(c0, lane, p.dim);
     const size_t b = column / tiles;
-    ForwardRows<T, ACCESS> rows{{static_cast<const T*>(p.x) + b * p.x_batch, static_cast<const T*>(p.r) + b * p.r_batch,
-                                 static_cast<const T*>(p.i) + b * p.i_batch},
-                                {p.x_token, p.r_token, p.i_token},
-                                staged + warp * kStages * ForwardRows<T, ACCESS>::kBytes,
-                                lane, c0, p.length, p.dim};
+    const int stride = cluster * kTile;
+    int t0 = rank * kTile + warp * kSteps;
+    Tile rows{{static_cast<const T*>(p.x) + b * p.x_batch, static_cast<const T*>(p.r) + b * p.r_batch,
+               static_cast<const T*>(p.i) + b * p.i_batch},
+              {p.x_token, p.r_token, p.i_token}};
+    rows.init(staged + warp * Tile::STAGES * Tile::kBytes, lane, c0, p.length, p.dim, t0);
+#pragma unroll
+    for (int k = 0; k < Tile::STAGES; ++k) rows.fetch(k, t0 + k * stride, stride);
     T* out = static_cast<T*>(p.h) + b * static_cast<size_t>(p.length) * p.dim;
     const Pair rate = mul2(rates(ln.load32(p.decay), p.exponent), both(-1.f));
-    const int stride = cluster * kTile;
-    const size_t chunks = static_cast<size_t>((p.length + kGatedScanChunk - 1) / kGatedScanChunk);
-    int t0 = rank * kTile + warp * kSteps;
+    float* chunk_states = nullptr;
+    if (p.chunk_states)
+        chunk_states = p.chunk_states +
+                       b * static_cast<size_t>((p.length + kGatedScanChunk - 1) / kGatedScanChunk) * p.dim;
 
     Walker seq;
     if constexpr (PACKED) {
@@ -397,37 +474,33 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
     if (!PACKED && p.initial) carry = ln.load32(p.initial + b * p.dim);
 
     const int rounds = (p.length + stride - 1) / stride;
-#pragma unroll
-    for (int k = 0; k < kStages; ++k) rows.fetch(k, t0 + k * stride);
     for (int round = 0; round < rounds; ++round, t0 += stride) {
-        const int buf = round & 1, stage = kStages == 2 ? buf : 0;
+        const int buf = round & 1;
         // Tokens past the end are a shut gate (r = -inf: a = 1) over x = 0:
         // the identity map.
         Pair a[kSteps], u[kSteps];
         rows.arrive();
-        rows.close(stage, 1, t0, Raw<T>::lowest());
+        rows.close(buf, 1, t0, Raw<T>::lowest());
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            const Word rx = rows.get(ln, stage, 0, t0, s, Raw<T>::zero());
-            const Word rr = rows.get(ln, stage, 1, t0, s, Raw<T>::lowest());
-            const Word ri = rows.get(ln, stage, 2, t0, s, Raw<T>::zero());
+            const Word rx = rows.get(ln, buf, 0, t0, s, Raw<T>::zero());
+            const Word rr = rows.get(ln, buf, 1, t0, s, Raw<T>::lowest());
+            const Word ri = rows.get(ln, buf, 2, t0, s, Raw<T>::zero());
             Pair m2;
             decay(mul2(rate, sigmoid(Raw<T>::get(rr))), a[s], m2);
             const Pair m = mul2(m2, inverse_root(m2));
             u[s] = mul2(mul2(m, sigmoid(Raw<T>::get(ri))), Raw<T>::get(rx));
         }
-        __syncwarp();  // the warp has read the tile
-        rows.fetch(stage, t0 + kStages * stride);
         Pair A = both(1.f), H = both(0.f);
         unsigned starts = 0;
         Walker from;
-        bool plain = true;
+        bool plain = t0 + kSteps <= p.length;  // every token exists, and none is a sequence's first or last
         if constexpr (PACKED) {
             seq.seek(t0);
             from = seq;
-            plain = seq.inside(t0, kSteps);
+            plain = plain && seq.inside(t0, kSteps);
         }
-        if (plain) {
+        if (!PACKED || plain) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 A = mul2(A, a[s]);
@@ -452,51 +525,58 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
         }
         maps.warp[buf][warp][lane] = Map{A, H};
         __syncthreads();
-        // the CTA's map, and the map of the warps before this one
-        Map before{both(1.f), both(0.f)}, total = before;
-#pragma unroll
-        for (int k = 0; k < kWarps; ++k) {
-            if (k == warp) before = total;
-            const Map m = maps.warp[buf][k][lane];
-            total.h = through<PACKED>(m.a, m.h, total.h);
-            total.a = product<PACKED>(total.a, m.a);
-        }
-        Pair in = carry;  // h before this CTA's tile
+        Pair h;  // before this warp's tokens
         if (cluster == 1) {
-            carry = through<PACKED>(total.a, total.h, carry);
+            h = carry;
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) {
+                const Map m = maps.warp[buf][k][lane];
+                carry = through<PACKED>(m.a, m.h, carry);
+                if (k + 1 == warp) h = carry;
+            }
         } else {
-            for (int k = warp; k < cluster; k += kWarps) store_remote(&maps.cta[buf][rank][lane], k, total);
+            Map before{both(1.f), both(0.f)}, total = before;
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) {
+                const Map m = maps.warp[buf][k][lane];
+                total.h = through<PACKED>(m.a, m.h, total.h);
+                total.a = product<PACKED>(total.a, m.a);
+                if (k + 1 == warp) before = total;
+            }
+            if (warp < cluster) store_remote(&maps.cta[buf][rank][lane], warp, total);
             cluster_sync();
+            h = carry;  // then before this CTA's tile
             for (int k = 0; k < cluster; ++k) {
-                if (k == rank) in = carry;
                 const Map m = maps.cta[buf][k][lane];
                 carry = through<PACKED>(m.a, m.h, carry);
+                if (k + 1 == rank) h = carry;
             }
+            if (warp > 0) h = through<PACKED>(before.a, before.h, h);
         }
-        Pair h = through<PACKED>(before.a, before.h, in);
-        if (p.chunk_states && t0 % kGatedScanChunk == 0 && t0 < p.length)
-            ln.store32(p.chunk_states + (b * chunks + static_cast<size_t>(t0 / kGatedScanChunk)) * p.dim, h);
-        T* po = out + static_cast<size_t>(t0) * p.dim;
-        if (plain && t0 + kSteps <= p.length) {
+        if (chunk_states && t0 % kGatedScanChunk == 0 && t0 < p.length)
+            ln.store32(chunk_states + static_cast<size_t>(t0 / kGatedScanChunk) * p.dim, h);
+        if (plain) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 h = fma2(a[s], h, u[s]);
-                ln.store(po, h);
-                po += p.dim;
+                rows.put(ln, buf, 0, out, t0, s, h);
             }
         } else {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 if (t0 + s >= p.length) continue;
                 h = (starts >> s) & 1u ? u[s] : fma2(a[s], h, u[s]);
-                ln.store(po, h);
+                rows.put(ln, buf, 0, out, t0, s, h);
                 if constexpr (PACKED) {
                     from.seek(t0 + s);
                     if (t0 + s + 1 == from.stop) ln.store32(p.last + static_cast<size_t>(from.at) * p.dim, h);
                 }
-                po += p.dim;
             }
         }
+        __syncwarp();
+        rows.flush(buf, 0, out, t0);
+        __syncwarp();  // the tile has been read
+        rows.fetch(buf, t0 + Tile::STAGES * stride, stride);
     }
     if (!PACKED && rank == 0 && warp == 0) ln.store32(p.last + b * p.dim, carry);
     if (cluster > 1) cluster_sync();  // no CTA leaves while another may still store into it
@@ -525,32 +605,34 @@ using BackwardRows = Rows<T, 4, kBackwardSteps, sizeof(T) == 2 ? 2 : 1, ACCESS>;
 template <typename T, bool PACKED, Access ACCESS>
 __global__ void __launch_bounds__(kWarps * 32, 2)
     gated_scan_backward_kernel(GatedScanArgs p, int cluster, int tiles) {
-    constexpr int kSteps = kBackwardSteps, kTile = kBackwardTile;
-    constexpr int kStages = sizeof(T) == 2 ? 2 : 1;
+    using Tile = BackwardRows<T, ACCESS>;
+    constexpr int kSteps = Tile::STEPS, kTile = kSteps * kWarps;
     using Word = typename Raw<T>::Word;
     extern __shared__ __align__(16) unsigned char staged[];
     __shared__ BackMaps maps;
     pdl_begin();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int rank = cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
     const unsigned column = blockIdx.x / cluster;
     const int c0 = static_cast<int>(column % tiles) * kChannels;
     const Lane<ACCESS> ln(c0, lane, p.dim);
     const size_t b = column / tiles;
-    BackwardRows<T, ACCESS> rows{{static_cast<const T*>(p.x) + b * p.x_batch, static_cast<const T*>(p.r) + b * p.r_batch,
-                                  static_cast<const T*>(p.i) + b * p.i_batch,
-                                  static_cast<const T*>(p.d_h) + b * p.dh_batch},
-                                 {p.x_token, p.r_token, p.i_token, p.dh_token},
-                                 staged + warp * kStages * BackwardRows<T, ACCESS>::kBytes,
-                                 lane, c0, p.length, p.dim};
+    const int stride = cluster * kTile;
+    const int rounds = (p.length + stride - 1) / stride;
+    int t0 = (rounds - 1) * stride + rank * kTile + warp * kSteps;
+    Tile rows{{static_cast<const T*>(p.x) + b * p.x_batch, static_cast<const T*>(p.r) + b * p.r_batch,
+               static_cast<const T*>(p.i) + b * p.i_batch, static_cast<const T*>(p.d_h) + b * p.dh_batch},
+              {p.x_token, p.r_token, p.i_token, p.dh_token}};
+    rows.init(staged + warp * Tile::STAGES * Tile::kBytes, lane, c0, p.length, p.dim, t0);
+#pragma unroll
+    for (int k = 0; k < Tile::STAGES; ++k) rows.fetch(k, t0 - k * stride, -stride);
     const size_t out = b * static_cast<size_t>(p.length) * p.dim;
     T* dx = static_cast<T*>(p.d_x) + out;
     T* dr = static_cast<T*>(p.d_r) + out;
     T* di = static_cast<T*>(p.d_i) + out;
     const Pair rate = mul2(rates(ln.load32(p.decay), p.exponent), both(-1.f));
-    const int stride = cluster * kTile;
-    const int chunks = (p.length + kTile - 1) / kTile;
-    const int rounds = (p.length + stride - 1) / stride;
+    const Pair rate_e = mul2(rate, both(kLn2));  // of la itself
+    const float* chunk_states = p.chunk_states + b * static_cast<size_t>((p.length + kTile - 1) / kTile) * p.dim;
 
     Walker seq;
     if constexpr (PACKED) {
@@ -565,11 +647,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     if (!PACKED && p.d_last) carry = ln.load32(p.d_last + b * p.dim);
     Pair sum = both(0.f);    // of e
 
-#pragma unroll
-    for (int k = 0; k < kStages; ++k) rows.fetch((rounds - 1 - k) & (kStages - 1), (rounds - 1 - k) * stride + rank * kTile + warp * kSteps);
-    for (int round = rounds - 1; round >= 0; --round) {
-        const int buf = round & 1, stage = kStages == 2 ? buf : 0;
-        const int t0 = round * stride + rank * kTile + warp * kSteps;
+    for (int round = 0; round < rounds; ++round, t0 -= stride) {  // from the end of time
+        const int buf = round & 1, stage = Tile::STAGES == 2 ? buf : 0;
+        const int tile = t0 - warp * kSteps;
+        Pair h = both(0.f);  // before the tile, from the forward
+        if (tile < p.length) h = ln.load32(chunk_states + static_cast<size_t>(tile / kTile) * p.dim);
         // x and dh are read where they are used, from shared memory; other
         // accesses keep them
         Word kx[ACCESS == kAsync ? 1 : kSteps], kd[ACCESS == kAsync ? 1 : kSteps];
@@ -602,20 +684,17 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
             else
                 return Raw<T>::get(kd[s]);
         };
-        Pair h = both(0.f);  // before the tile, from the forward
-        const int chunk = round * cluster + rank;
-        if (chunk < chunks) h = ln.load32(p.chunk_states + (b * chunks + chunk) * static_cast<size_t>(p.dim));
 
         // the maps of the warp's tokens, forward and backward
         unsigned starts = 0, ends = 0;
         Pair A = both(1.f), H = both(0.f), R = both(0.f);
         Walker from;
-        bool plain = true;
+        bool plain = t0 + kSteps <= p.length;  // every token exists, and none is a sequence's first or last
         if constexpr (PACKED) {
             seq.rewind();
             seq.seek(t0);
             from = seq;
-            plain = seq.inside(t0, kSteps);
+            plain = plain && seq.inside(t0, kSteps);
         }
         // dh with the final states' gradients where a sequence ends
         auto arriving = [&](int s, int at) {
@@ -629,7 +708,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
             while (at > 0 && p.offsets[at] >= t) --at;
             return at;
         };
-        if (plain) {
+        if (!PACKED || plain) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 A = mul2(A, a[s]);
@@ -668,79 +747,90 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         maps.warp[buf][warp][lane] = Map{A, H};
         maps.back[buf][warp][lane] = R;
         __syncthreads();
-        Map after{both(1.f), both(0.f)}, total = after;  // of P, from the end of time
+        Pair P;  // from the tokens after this warp's
+        if (cluster == 1) {
+            P = carry;
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) {
-            if (k >= warp) break;
+            for (int k = kWarps - 1; k >= 0; --k) {
+                carry = through<PACKED>(maps.warp[buf][k][lane].a, maps.back[buf][k][lane], carry);
+                if (k == warp + 1) P = carry;
+            }
+        } else {
+            Map after{both(1.f), both(0.f)}, total = after;
+#pragma unroll
+            for (int k = kWarps - 1; k >= 0; --k) {
+                const Pair qa = maps.warp[buf][k][lane].a;
+                total.h = through<PACKED>(qa, maps.back[buf][k][lane], total.h);
+                total.a = product<PACKED>(total.a, qa);
+                if (k == warp + 1) after = total;
+            }
+            if (warp < cluster) store_remote(&maps.cta[buf][rank][lane], warp, total);
+            cluster_sync();
+            P = carry;  // then from the tokens after this CTA's tile
+            for (int k = cluster - 1; k >= 0; --k) {
+                const Map q = maps.cta[buf][k][lane];
+                carry = through<PACKED>(q.a, q.h, carry);
+                if (k == rank + 1) P = carry;
+            }
+            if (warp + 1 < kWarps) P = through<PACKED>(after.a, after.h, P);
+        }
+        for (int k = 0; k < warp; ++k) {
             const Map q = maps.warp[buf][k][lane];
             h = through<PACKED>(q.a, q.h, h);
         }
-#pragma unroll
-        for (int k = kWarps - 1; k >= 0; --k) {
-            if (k == warp) after = total;
-            const Pair qa = maps.warp[buf][k][lane].a;
-            total.h = through<PACKED>(qa, maps.back[buf][k][lane], total.h);
-            total.a = product<PACKED>(total.a, qa);
-        }
-        Pair in = carry;  // P from the tokens after this CTA's tile
-        if (cluster == 1) {
-            carry = through<PACKED>(total.a, total.h, carry);
-        } else {
-            for (int k = warp; k < cluster; k += kWarps) store_remote(&maps.cta[buf][rank][lane], k, total);
-            cluster_sync();
-            for (int k = cluster - 1; k >= 0; --k) {
-                if (k == rank) in = carry;
-                const Map q = maps.cta[buf][k][lane];
-                carry = through<PACKED>(q.a, q.h, carry);
-            }
-        }
-        Pair P = through<PACKED>(after.a, after.h, in);
 
         // h before each token, then the gradients from the last token back
         Pair before[kSteps];
-        int at = 0;
+        auto gradients = [&](int s, Pair d) {
+            const Pair fx = x_of(s);
+            const Pair G = add2(d, P);
+            const Pair gx = mul2(G, v[s]), si = mul2(v[s], im[s]);
+            const Pair gi = mul2(mul2(gx, fx), sub2(both(1.f), si));
+            P = mul2(a[s], G);
+            const Pair e = mul2(mul2(P, mul2(rate_e, sr[s])), sub2(before[s], mul2(mul2(mul2(si, fx), a[s]), im[s])));
+            sum = add2(sum, e);
+            rows.put(ln, stage, 0, dx, t0, s, gx);
+            rows.put(ln, stage, 1, dr, t0, s, mul2(e, sub2(both(1.f), sr[s])));
+            rows.put(ln, stage, 2, di, t0, s, gi);
+        };
         if (plain) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 before[s] = h;
                 h = fma2(a[s], h, mul2(v[s], x_of(s)));
             }
+#pragma unroll
+            for (int s = kSteps - 1; s >= 0; --s) gradients(s, dh_of(s));
         } else {
-            at = seq.at;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 before[s] = h;
                 if (t0 + s >= p.length) continue;
-                from.seek(t0 + s);
-                if ((starts >> s) & 1u)
-                    before[s] = p.initial ? ln.load32(p.initial + static_cast<size_t>(from.at) * p.dim) : both(0.f);
+                if constexpr (PACKED) {
+                    from.seek(t0 + s);
+                    if ((starts >> s) & 1u)
+                        before[s] = p.initial ? ln.load32(p.initial + static_cast<size_t>(from.at) * p.dim) : both(0.f);
+                }
                 h = fma2(a[s], before[s], mul2(v[s], x_of(s)));
             }
-        }
-        const size_t o = static_cast<size_t>(t0) * p.dim;
+            int at = PACKED ? seq.at : 0;
 #pragma unroll
-        for (int s = kSteps - 1; s >= 0; --s) {
-            if (t0 + s >= p.length) continue;
-            const Pair fx = x_of(s);
-            const Pair G = add2(plain ? dh_of(s) : arriving(s, at), P);
-            const Pair gx = mul2(G, v[s]), si = mul2(v[s], im[s]);
-            const Pair gi = mul2(mul2(gx, fx), sub2(both(1.f), si));
-            P = mul2(a[s], G);
-            const Pair la = mul2(mul2(rate, both(kLn2)), sr[s]);
-            const Pair e = mul2(mul2(P, la), sub2(before[s], mul2(mul2(mul2(si, fx), a[s]), im[s])));
-            sum = add2(sum, e);
-            const size_t row = o + static_cast<size_t>(s) * p.dim;
-            ln.store(dx + row, gx);
-            ln.store(dr + row, mul2(e, sub2(both(1.f), sr[s])));
-            ln.store(di + row, gi);
-            if (!plain && ((starts >> s) & 1u)) {
-                if (p.d_initial) ln.store32(p.d_initial + static_cast<size_t>(at) * p.dim, P);
-                P = both(0.f);
-                at = previous(at, t0 + s);
+            for (int s = kSteps - 1; s >= 0; --s) {
+                if (t0 + s >= p.length) continue;
+                gradients(s, arriving(s, at));
+                if (PACKED && ((starts >> s) & 1u)) {
+                    if (p.d_initial) ln.store32(p.d_initial + static_cast<size_t>(at) * p.dim, P);
+                    P = both(0.f);
+                    at = previous(at, t0 + s);
+                }
             }
         }
-        __syncwarp();  // the warp has read the tile
-        rows.fetch(stage, t0 - kStages * stride);
+        __syncwarp();
+        rows.flush(stage, 0, dx, t0);
+        rows.flush(stage, 1, dr, t0);
+        rows.flush(stage, 2, di, t0);
+        __syncwarp();  // the tile has been read
+        rows.fetch(stage, t0 - Tile::STAGES * stride, -stride);
     }
     if (!PACKED && p.d_initial && rank == 0 && warp == 0) ln.store32(p.d_initial + b * p.dim, carry);
     maps.sum[warp][lane] = sum;

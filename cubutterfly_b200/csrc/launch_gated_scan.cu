@@ -70,14 +70,14 @@ cudaError_t launch_kernel(const GatedScanArgs& a, cudaStream_t stream) {
         else
             return &gated_scan_kernel<T, PACKED, ACCESS>;
     }();
-    constexpr int kStages = sizeof(T) == 2 ? 2 : 1;
-    constexpr int smem = kWarps * kStages * (BACKWARD ? BackwardRows<T, ACCESS>::kBytes : ForwardRows<T, ACCESS>::kBytes);
+    using Tile = std::conditional_t<BACKWARD, BackwardRows<T, ACCESS>, ForwardRows<T, ACCESS>>;
+    constexpr int smem = kWarps * Tile::STAGES * Tile::kBytes;
     int cap = 0;
     // two CTAs per SM fit only in the largest carveout
     cudaError_t e = setup_kernel(setup, kernel, kWarps * 32, smem, &cap, ACCESS == kAsync);
     if (e != cudaSuccess) return e;
     const int tiles = ceil_div(a.dim, kChannels);
-    const int cluster = gated_scan_cluster(a.batch, a.length, a.dim, BACKWARD);
+    const int cluster = gated_scan_cluster(a.batch, a.length, a.dim, Tile::STEPS * kWarps);
     const size_t grid = static_cast<size_t>(tiles) * a.batch * cluster;
     if (grid > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
     return launch_clusters(kernel, static_cast<unsigned>(grid), kWarps * 32u, smem, cluster, stream, a, cluster, tiles);
@@ -125,9 +125,9 @@ cudaError_t launch_step_typed(const GatedStepArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-int gated_scan_cluster(int batch, int length, int dim, bool backward) {
+int gated_scan_cluster(int batch, int length, int dim, int tile) {
     const size_t columns = static_cast<size_t>(ceil_div(dim, kChannels)) * batch;
-    const int tiles = ceil_div(length, backward ? kBackwardTile : kForwardTile);
+    const int tiles = ceil_div(length, tile);
     int best = 1;
     double least = 0;
     for (int k = 1; k <= kGatedScanMaxCluster; k *= 2) {
@@ -148,7 +148,7 @@ cudaError_t launch_gated_scan(BlockType type, const GatedScanArgs& a, cudaStream
 cudaError_t launch_gated_scan_backward(BlockType type, const GatedScanArgs& a, cudaStream_t stream) {
     cudaError_t e = launch_any(type, a, true, stream);
     if (e != cudaSuccess) return e;
-    const int parts = a.batch * gated_scan_cluster(a.batch, a.length, a.dim, true);
+    const int parts = a.batch * gated_scan_cluster(a.batch, a.length, a.dim, kGatedScanChunk);
     return launch_dependent(&gated_scan_decay_kernel, static_cast<unsigned>(ceil_div(a.dim, 32)), 256u, 0, stream, a,
                             parts);
 }
