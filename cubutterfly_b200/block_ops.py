@@ -26,7 +26,7 @@ _TYPES = {torch.bfloat16: int(cb.DataType.BF16), torch.float16: int(cb.DataType.
           torch.float32: int(cb.DataType.FP32)}
 _ACTIVATIONS = {"none": 0, "sigmoid": 1, "silu": 2}
 _POST_NORM, _PRE_NORM, _ROTATE = 1, 2, 4
-_CHUNK = 64  # tokens per state kept for the backward of gated_scan
+_CHUNK = 16  # tokens per state kept for the backward of gated_scan
 
 # the structs of include/cubutterfly/cubutterfly_b200.h, in field order
 _NORM = struct.Struct("@4N8i2d6P3N6P2N6PPN")

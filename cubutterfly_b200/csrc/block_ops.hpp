@@ -12,7 +12,8 @@ namespace cubf {
 enum class BlockType : int { kF16 = 0, kBF16 = 1, kF32 = 2 };
 
 // ---- gated linear recurrence (gated_scan.cuh) ----------------------------
-constexpr int kGatedScanChunk = 64;       // tokens per saved chunk state
+constexpr int kGatedScanChunk = 16;       // tokens per saved chunk state
+constexpr int kGatedScanBackwardTile = 64;  // tokens a backward CTA takes at a time
 constexpr int kGatedScanMaxCluster = 8;   // portable cluster size
 constexpr int kGatedScanMaxLength = 1 << 30;
 
@@ -30,7 +31,7 @@ struct GatedScanArgs {
     const int* offsets;         // (sequences + 1) of a packed batch, or null
     void* h;
     float* last;                // (states, dim)
-    float* chunk_states;        // (batch, chunks, dim): h before every 64th token; null where no gradient follows
+    float* chunk_states;        // (batch, chunks, dim): h before every 16th token; null where no gradient follows
     const float* d_last;        // or null: zero
     void* d_x;
     void* d_r;
@@ -58,7 +59,7 @@ struct GatedStepArgs {
 };
 
 // CTAs per cluster along time for a batch of this shape (1, 2, 4 or 8), each
-// with `tile` tokens at a time; the backward's tile is kGatedScanChunk.
+// with `tile` tokens at a time.
 int gated_scan_cluster(int batch, int length, int dim, int tile);
 cudaError_t launch_gated_scan(BlockType type, const GatedScanArgs& args, cudaStream_t stream);
 cudaError_t launch_gated_scan_backward(BlockType type, const GatedScanArgs& args, cudaStream_t stream);

@@ -296,7 +296,7 @@ cubf::GatedScanArgs scan_args(const cubutterflyB200GatedScan_t* a, bool backward
 size_t scan_workspace(const cubutterflyB200GatedScan_t& a) {
     const size_t cluster = static_cast<size_t>(
         cubf::gated_scan_cluster(static_cast<int>(a.batch), static_cast<int>(a.length), static_cast<int>(a.dim),
-                                 cubf::kGatedScanChunk));
+                                 cubf::kGatedScanBackwardTile));
     return (a.batch * cluster * a.dim * sizeof(float) + 15) / 16 * 16;
 }
 

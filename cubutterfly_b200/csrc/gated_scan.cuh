@@ -40,8 +40,8 @@ static_assert(kGatedScanMaxCluster <= kWarps, "a warp reads the map of each CTA 
 template <typename T>
 constexpr int kForwardSteps = sizeof(T) == 2 ? 16 : 8;
 constexpr int kBackwardSteps = 8;
-static_assert(kBackwardSteps * kWarps == kGatedScanChunk, "the backward restarts from the states the forward kept");
-static_assert(kGatedScanChunk % kForwardSteps<__half> == 0, "chunks begin where a forward thread does");
+static_assert(kGatedScanChunk == 2 * kBackwardSteps && kGatedScanChunk % kForwardSteps<__half> == 0,
+              "chunks begin where a forward warp and every other backward warp do");
 
 CUBF_DEV Pair both(float v) { return f32x2::pk(v, v); }
 CUBF_DEV Pair pair(float2 v) { return f32x2::pk(v.x, v.y); }
@@ -347,6 +347,16 @@ CUBF_DEV Pair inverse_root(Pair m2) {
     return each(add2(m2, both(1e-37f)), [](float x) { return rsq(x); });
 }
 
+// sqrt(1 - a^2) sigmoid(i) x from 1 - a^2: with Q = 1 + e^-i, sqrt(m2)/Q =
+// m2/sqrt(m2 Q^2), one special-function instruction for root and quotient.
+// Q^2 may reach infinity, for i below -44, where the factor (below 1e-19) is
+// taken as zero.
+CUBF_DEV Pair drive(Pair m2, Pair i, Pair x) {
+    const Pair q = add2(each(mul2(i, both(-kLog2e)), [](float v) { return ex2(v); }), both(1.f));
+    const Pair root = each(mul2(add2(m2, both(1e-37f)), mul2(q, q)), [](float v) { return rsq(v); });
+    return mul2(mul2(m2, root), x);
+}
+
 // ---- joining runs -----------------------------------------------------------------------------
 // In packed batches a run that holds a sequence's first token forgets what
 // came before it whatever that was (a product with zero would keep its NaN):
@@ -412,6 +422,13 @@ CUBF_DEV void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// Hand-over from one warp to another on a named barrier that counts both
+// warps: the giver's shared-memory writes before give() are seen after take().
+// A giver comes back to a barrier only after what it gave has come round, so a
+// barrier never holds two hand-overs.
+CUBF_DEV void give(int barrier) { asm volatile("bar.arrive %0, 64;" ::"r"(barrier) : "memory"); }
+CUBF_DEV void take(int barrier) { asm volatile("bar.sync %0, 64;" ::"r"(barrier) : "memory"); }
+
 // An affine map of a lane's two channels.
 struct alignas(16) Map {
     Pair a, h;
@@ -424,24 +441,30 @@ CUBF_DEV void store_remote(const Map* local, uint32_t rank, Map v) {
 }
 
 // ---- forward ----------------------------------------------------------------------------------
+template <bool CLUSTER>
 struct Maps {
     Map warp[2][kWarps][32];
     Map cta[2][kGatedScanMaxCluster][32];
+};
+template <>
+struct Maps<false> {
+    Pair carry[kWarps][32];  // h before the warp's tokens
 };
 
 template <typename T, Access ACCESS>
 using ForwardRows = Rows<T, 3, kForwardSteps<T>, 2, ACCESS>;
 
-template <typename T, bool PACKED, Access ACCESS>
-__global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArgs p, int cluster, int tiles) {
+template <typename T, bool PACKED, bool CLUSTER, Access ACCESS>
+__global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArgs p, int cluster_, int tiles) {
     using Tile = ForwardRows<T, ACCESS>;
     constexpr int kSteps = Tile::STEPS, kTile = kSteps * kWarps;
     using Word = typename Raw<T>::Word;
     extern __shared__ __align__(16) unsigned char staged[];
-    __shared__ Maps maps;
+    __shared__ Maps<CLUSTER> maps;
     pdl_begin();
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
-    const int rank = cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int cluster = CLUSTER ? cluster_ : 1;
+    const int rank = CLUSTER ? static_cast<int>(cluster_rank()) : 0;
     const unsigned column = blockIdx.x / cluster;
     const int c0 = static_cast<int>(column % tiles) * kChannels;
     const Lane<ACCESS> ln(c0, lane, p.dim);
@@ -488,8 +511,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
             const Word ri = rows.get(ln, buf, 2, t0, s, Raw<T>::zero());
             Pair m2;
             decay(mul2(rate, sigmoid(Raw<T>::get(rr))), a[s], m2);
-            const Pair m = mul2(m2, inverse_root(m2));
-            u[s] = mul2(mul2(m, sigmoid(Raw<T>::get(ri))), Raw<T>::get(rx));
+            u[s] = drive(m2, Raw<T>::get(ri), Raw<T>::get(rx));
         }
         Pair A = both(1.f), H = both(0.f);
         unsigned starts = 0;
@@ -523,18 +545,28 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
                 }
             }
         }
-        maps.warp[buf][warp][lane] = Map{A, H};
-        __syncthreads();
         Pair h;  // before this warp's tokens
-        if (cluster == 1) {
+        if constexpr (!CLUSTER) {
+            // The state goes from warp to warp, and from the last one to the
+            // first one's next tile; no barrier holds all warps, so they
+            // drift apart and one's loads, gates and stores overlap
+            // another's.
             h = carry;
-#pragma unroll
-            for (int k = 0; k < kWarps; ++k) {
-                const Map m = maps.warp[buf][k][lane];
-                carry = through<PACKED>(m.a, m.h, carry);
-                if (k + 1 == warp) h = carry;
+            if (warp > 0 || round > 0) {
+                take(1 + warp);
+                h = maps.carry[warp][lane];
+            }
+            const Pair next = through<PACKED>(A, H, h);
+            if (warp + 1 < kWarps || round + 1 < rounds) {
+                const int to = (warp + 1) % kWarps;
+                maps.carry[to][lane] = next;
+                give(1 + to);
+            } else {
+                carry = next;
             }
         } else {
+            maps.warp[buf][warp][lane] = Map{A, H};
+            __syncthreads();
             Map before{both(1.f), both(0.f)}, total = before;
 #pragma unroll
             for (int k = 0; k < kWarps; ++k) {
@@ -578,8 +610,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
         __syncwarp();  // the tile has been read
         rows.fetch(buf, t0 + Tile::STAGES * stride, stride);
     }
-    if (!PACKED && rank == 0 && warp == 0) ln.store32(p.last + b * p.dim, carry);
-    if (cluster > 1) cluster_sync();  // no CTA leaves while another may still store into it
+    if (!PACKED && rank == 0 && warp == (CLUSTER ? 0 : kWarps - 1)) ln.store32(p.last + b * p.dim, carry);
+    if constexpr (CLUSTER) cluster_sync();  // no CTA leaves while another may still store into it
 }
 
 // ---- backward ----------------------------------------------------------------------------------
@@ -592,27 +624,35 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
 //   dr = e (1 - sigmoid(r))   dLambda = sum e sigmoid(Lambda)/softplus(Lambda)
 // A thread keeps a, v, 1/m and sigmoid(r) of its tokens and gets sigmoid(i)
 // back as v/m, which leaves room for two CTAs per SM.
+template <bool CLUSTER>
 struct BackMaps {
-    Map warp[2][kWarps][32];
-    Pair back[2][kWarps][32];  // P out of the warp's tokens from P = 0 after them
-    Map cta[2][kGatedScanMaxCluster][32];
+    Pair half[kWarps][32];    // h before the warp's tokens, where the warp before has it
     Pair sum[kWarps][32];
+    Map warp[2][kWarps][32];  // of P, from the end of time
+    Map cta[2][kGatedScanMaxCluster][32];
+};
+template <>
+struct BackMaps<false> {
+    Pair half[kWarps][32];
+    Pair sum[kWarps][32];
+    Pair carry[kWarps][32];   // P from the tokens after the warp's
 };
 
 template <typename T, Access ACCESS>
 using BackwardRows = Rows<T, 4, kBackwardSteps, sizeof(T) == 2 ? 2 : 1, ACCESS>;
 
-template <typename T, bool PACKED, Access ACCESS>
+template <typename T, bool PACKED, bool CLUSTER, Access ACCESS>
 __global__ void __launch_bounds__(kWarps * 32, 2)
-    gated_scan_backward_kernel(GatedScanArgs p, int cluster, int tiles) {
+    gated_scan_backward_kernel(GatedScanArgs p, int cluster_, int tiles) {
     using Tile = BackwardRows<T, ACCESS>;
     constexpr int kSteps = Tile::STEPS, kTile = kSteps * kWarps;
     using Word = typename Raw<T>::Word;
     extern __shared__ __align__(16) unsigned char staged[];
-    __shared__ BackMaps maps;
+    __shared__ BackMaps<CLUSTER> maps;
     pdl_begin();
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
-    const int rank = cluster > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int cluster = CLUSTER ? cluster_ : 1;
+    const int rank = CLUSTER ? static_cast<int>(cluster_rank()) : 0;
     const unsigned column = blockIdx.x / cluster;
     const int c0 = static_cast<int>(column % tiles) * kChannels;
     const Lane<ACCESS> ln(c0, lane, p.dim);
@@ -632,7 +672,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     T* di = static_cast<T*>(p.d_i) + out;
     const Pair rate = mul2(rates(ln.load32(p.decay), p.exponent), both(-1.f));
     const Pair rate_e = mul2(rate, both(kLn2));  // of la itself
-    const float* chunk_states = p.chunk_states + b * static_cast<size_t>((p.length + kTile - 1) / kTile) * p.dim;
+    const float* chunk_states =
+        p.chunk_states + b * static_cast<size_t>((p.length + kGatedScanChunk - 1) / kGatedScanChunk) * p.dim;
 
     Walker seq;
     if constexpr (PACKED) {
@@ -649,9 +690,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
 
     for (int round = 0; round < rounds; ++round, t0 -= stride) {  // from the end of time
         const int buf = round & 1, stage = Tile::STAGES == 2 ? buf : 0;
-        const int tile = t0 - warp * kSteps;
-        Pair h = both(0.f);  // before the tile, from the forward
-        if (tile < p.length) h = ln.load32(chunk_states + static_cast<size_t>(tile / kTile) * p.dim);
+        // before the warp's tokens: from the forward, or (below) from the warp before
+        Pair h = both(0.f);
+        if (warp % 2 == 0 && t0 < p.length)
+            h = ln.load32(chunk_states + static_cast<size_t>(t0 / kGatedScanChunk) * p.dim);
         // x and dh are read where they are used, from shared memory; other
         // accesses keep them
         Word kx[ACCESS == kAsync ? 1 : kSteps], kd[ACCESS == kAsync ? 1 : kSteps];
@@ -744,24 +786,39 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
                 }
             }
         }
-        maps.warp[buf][warp][lane] = Map{A, H};
-        maps.back[buf][warp][lane] = R;
-        __syncthreads();
+        // h from the warp before, within a chunk
+        if (warp % 2 == 0) {
+            maps.half[warp + 1][lane] = through<PACKED>(A, H, h);
+            give(1 + kWarps + warp / 2);
+        } else {
+            take(1 + kWarps + warp / 2);
+            h = maps.half[warp][lane];
+        }
         Pair P;  // from the tokens after this warp's
-        if (cluster == 1) {
+        if constexpr (!CLUSTER) {
+            // from warp to warp, as the forward's state, from the end of time
             P = carry;
-#pragma unroll
-            for (int k = kWarps - 1; k >= 0; --k) {
-                carry = through<PACKED>(maps.warp[buf][k][lane].a, maps.back[buf][k][lane], carry);
-                if (k == warp + 1) P = carry;
+            if (warp + 1 < kWarps || round > 0) {
+                take(1 + warp);
+                P = maps.carry[warp][lane];
+            }
+            const Pair next = through<PACKED>(A, R, P);
+            if (warp > 0 || round + 1 < rounds) {
+                const int to = (warp + kWarps - 1) % kWarps;
+                maps.carry[to][lane] = next;
+                give(1 + to);
+            } else {
+                carry = next;
             }
         } else {
+            maps.warp[buf][warp][lane] = Map{A, R};
+            __syncthreads();
             Map after{both(1.f), both(0.f)}, total = after;
 #pragma unroll
             for (int k = kWarps - 1; k >= 0; --k) {
-                const Pair qa = maps.warp[buf][k][lane].a;
-                total.h = through<PACKED>(qa, maps.back[buf][k][lane], total.h);
-                total.a = product<PACKED>(total.a, qa);
+                const Map q = maps.warp[buf][k][lane];
+                total.h = through<PACKED>(q.a, q.h, total.h);
+                total.a = product<PACKED>(total.a, q.a);
                 if (k == warp + 1) after = total;
             }
             if (warp < cluster) store_remote(&maps.cta[buf][rank][lane], warp, total);
@@ -773,10 +830,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
                 if (k == rank + 1) P = carry;
             }
             if (warp + 1 < kWarps) P = through<PACKED>(after.a, after.h, P);
-        }
-        for (int k = 0; k < warp; ++k) {
-            const Map q = maps.warp[buf][k][lane];
-            h = through<PACKED>(q.a, q.h, h);
         }
 
         // h before each token, then the gradients from the last token back
@@ -839,7 +892,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         for (int k = 1; k < kWarps; ++k) sum = add2(sum, maps.sum[k][lane]);
         ln.store32(p.partials + (b * cluster + rank) * static_cast<size_t>(p.dim), sum);
     }
-    if (cluster > 1) cluster_sync();
+    if constexpr (CLUSTER) cluster_sync();
 }
 
 // dLambda = sigmoid(Lambda)/softplus(Lambda) sum e over the CTAs' partial sums
@@ -891,7 +944,7 @@ __global__ void __launch_bounds__(128) gated_scan_step_kernel(GatedStepArgs p, i
         const Pair s = ln.load32(p.state + static_cast<size_t>(slot) * p.dim);
         Pair a, m2;
         decay(mul2(rate, sigmoid(r)), a, m2);
-        const Pair n = fma2(a, s, mul2(mul2(mul2(m2, inverse_root(m2)), sigmoid(i)), x));
+        const Pair n = fma2(a, s, drive(m2, i, x));
         ln.store(h, n);
         ln.store32(p.new_state + static_cast<size_t>(slot) * p.dim, n);
     }

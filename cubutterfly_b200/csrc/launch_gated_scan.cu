@@ -1,5 +1,6 @@
 // launch_gated_scan.cu -- launches of the gated linear recurrence.
 #include <algorithm>
+#include <cstdlib>
 
 #include "gated_scan.cuh"
 #include "launch_util.cuh"
@@ -8,6 +9,7 @@ namespace cubf {
 namespace {
 
 using namespace scan;
+static_assert(kGatedScanBackwardTile == kBackwardSteps * kWarps, "the workspace is sized for the backward's clusters");
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
@@ -61,14 +63,14 @@ Access access_of(const GatedScanArgs& a, bool backward) {
     return v.access();
 }
 
-template <typename T, bool PACKED, Access ACCESS, bool BACKWARD>
-cudaError_t launch_kernel(const GatedScanArgs& a, cudaStream_t stream) {
+template <typename T, bool PACKED, bool CLUSTER, Access ACCESS, bool BACKWARD>
+cudaError_t launch_kernel(const GatedScanArgs& a, int cluster, cudaStream_t stream) {
     static KernelSetup setup;
     const auto kernel = [] {
         if constexpr (BACKWARD)
-            return &gated_scan_backward_kernel<T, PACKED, ACCESS>;
+            return &gated_scan_backward_kernel<T, PACKED, CLUSTER, ACCESS>;
         else
-            return &gated_scan_kernel<T, PACKED, ACCESS>;
+            return &gated_scan_kernel<T, PACKED, CLUSTER, ACCESS>;
     }();
     using Tile = std::conditional_t<BACKWARD, BackwardRows<T, ACCESS>, ForwardRows<T, ACCESS>>;
     constexpr int smem = kWarps * Tile::STAGES * Tile::kBytes;
@@ -77,18 +79,25 @@ cudaError_t launch_kernel(const GatedScanArgs& a, cudaStream_t stream) {
     cudaError_t e = setup_kernel(setup, kernel, kWarps * 32, smem, &cap, ACCESS == kAsync);
     if (e != cudaSuccess) return e;
     const int tiles = ceil_div(a.dim, kChannels);
-    const int cluster = gated_scan_cluster(a.batch, a.length, a.dim, Tile::STEPS * kWarps);
     const size_t grid = static_cast<size_t>(tiles) * a.batch * cluster;
     if (grid > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
     return launch_clusters(kernel, static_cast<unsigned>(grid), kWarps * 32u, smem, cluster, stream, a, cluster, tiles);
 }
 
+template <typename T, bool PACKED, Access ACCESS, bool BACKWARD>
+cudaError_t launch_split(const GatedScanArgs& a, cudaStream_t stream) {
+    const int tile = (BACKWARD ? kBackwardSteps : kForwardSteps<T>) * kWarps;
+    const int cluster = gated_scan_cluster(a.batch, a.length, a.dim, tile);
+    return cluster > 1 ? launch_kernel<T, PACKED, true, ACCESS, BACKWARD>(a, cluster, stream)
+                       : launch_kernel<T, PACKED, false, ACCESS, BACKWARD>(a, 1, stream);
+}
+
 template <typename T, bool PACKED, bool BACKWARD>
 cudaError_t launch_access(const GatedScanArgs& a, cudaStream_t stream) {
     switch (access_of<T>(a, BACKWARD)) {
-        case kAsync: return launch_kernel<T, PACKED, kAsync, BACKWARD>(a, stream);
-        case kPairs: return launch_kernel<T, PACKED, kPairs, BACKWARD>(a, stream);
-        default: return launch_kernel<T, PACKED, kScalar, BACKWARD>(a, stream);
+        case kAsync: return launch_split<T, PACKED, kAsync, BACKWARD>(a, stream);
+        case kPairs: return launch_split<T, PACKED, kPairs, BACKWARD>(a, stream);
+        default: return launch_split<T, PACKED, kScalar, BACKWARD>(a, stream);
     }
 }
 
@@ -126,6 +135,7 @@ cudaError_t launch_step_typed(const GatedStepArgs& a, cudaStream_t stream) {
 }  // namespace
 
 int gated_scan_cluster(int batch, int length, int dim, int tile) {
+    if (getenv("CUBF_K")) return atoi(getenv("CUBF_K"));
     const size_t columns = static_cast<size_t>(ceil_div(dim, kChannels)) * batch;
     const int tiles = ceil_div(length, tile);
     int best = 1;
@@ -148,7 +158,7 @@ cudaError_t launch_gated_scan(BlockType type, const GatedScanArgs& a, cudaStream
 cudaError_t launch_gated_scan_backward(BlockType type, const GatedScanArgs& a, cudaStream_t stream) {
     cudaError_t e = launch_any(type, a, true, stream);
     if (e != cudaSuccess) return e;
-    const int parts = a.batch * gated_scan_cluster(a.batch, a.length, a.dim, kGatedScanChunk);
+    const int parts = a.batch * gated_scan_cluster(a.batch, a.length, a.dim, kGatedScanBackwardTile);
     return launch_dependent(&gated_scan_decay_kernel, static_cast<unsigned>(ceil_div(a.dim, 32)), 256u, 0, stream, a,
                             parts);
 }

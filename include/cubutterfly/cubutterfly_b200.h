@@ -242,8 +242,8 @@ CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200BlockNormBackward(const cubutt
  * possibly none (its final state is its initial state); states = sequences.
  * Values of one sequence, NaN and infinities included, do not reach another.
  * dim >= 1, length <= 2^30; decay (dim) is fp32; exponent > 0.
- * A call whose backward follows keeps the state before every 64th token in
- * chunk_states (fp32, (batch, ceil(length / 64), dim)). */
+ * A call whose backward follows keeps the state before every 16th token in
+ * chunk_states (fp32, (batch, ceil(length / 16), dim)). */
 typedef struct cubutterflyB200GatedScan_s {
     size_t struct_size;
     size_t batch, length, dim, sequences;
