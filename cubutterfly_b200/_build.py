@@ -47,8 +47,7 @@ def _units():
     for name in ("c_api.cpp", "descriptor.cpp", "planner.cpp", "rns_api.cpp", "launch_bitwise_dispatch.cpp",
                  "launch_ntt_dispatch.cpp", "launch_fft.cu", "noalloc.cu", "fourstep.cu", "bitrev.cu", "fwht_tc.cu",
                  "real_adapter.cu", "real_fft.cu", "calibrate.cu", "fourstep_peer.cu", "unaligned.cu", "structured.cu", "fwht_native.cu", "fft64.cu", "fft_chain.cu",
-                 "heongpu_adapter.cpp", "bluestein.cu", "block_ops_api.cpp", "launch_block_norm_dispatch.cpp",
-                 "launch_gated_scan.cu"):
+                 "heongpu_adapter.cpp", "bluestein.cu", "block_ops_api.cpp", "launch_block_dispatch.cpp"):
         src = CSRC / name
         obj = OBJ / (src.stem + ".o")
         units.append((common + ["-c", str(src), "-o", str(obj)], src, obj))
@@ -61,6 +60,10 @@ def _units():
         obj = OBJ / f"block_norm_{ty}_{backward}.o"
         units.append((common + [f"-DCUBF_BN_TYPE={ty}", f"-DCUBF_BN_BACKWARD={backward}", "-c", str(src), "-o",
                                 str(obj)], src, obj))
+    for ty in range(3):  # gated scan block types
+        src = CSRC / "launch_gated_scan.cu"
+        obj = OBJ / f"gated_scan_{ty}.o"
+        units.append((common + [f"-DCUBF_GS_TYPE={ty}", "-c", str(src), "-o", str(obj)], src, obj))
     for op, ty in BW_UNITS:
         src = CSRC / "launch_bitwise.cu"
         obj = OBJ / f"bitwise_{op}_{ty}.o"

@@ -13,8 +13,6 @@ enum class BlockType : int { kF16 = 0, kBF16 = 1, kF32 = 2 };
 
 // ---- gated linear recurrence (gated_scan.cuh) ----------------------------
 constexpr int kGatedScanChunk = 16;       // tokens per saved chunk state
-constexpr int kGatedScanBackwardTile = 64;  // tokens a backward CTA takes at a time
-constexpr int kGatedScanMaxCluster = 8;   // portable cluster size
 constexpr int kGatedScanMaxLength = 1 << 30;
 
 // Strides in elements; the channel stride of every tensor is one.  Outputs
@@ -38,7 +36,7 @@ struct GatedScanArgs {
     void* d_i;
     float* d_initial;           // or null
     float* d_decay;
-    float* partials;            // (batch * cluster, dim)
+    float* partials;            // (batch, dim)
     int batch, length, dim, sequences;
     float exponent;
 };
@@ -58,11 +56,7 @@ struct GatedStepArgs {
     float exponent;
 };
 
-// CTAs per cluster along time for a batch of this shape (1, 2, 4 or 8), each
-// with `tile` tokens at a time.
-int gated_scan_cluster(int batch, int length, int dim, int tile);
-cudaError_t launch_gated_scan(BlockType type, const GatedScanArgs& args, cudaStream_t stream);
-cudaError_t launch_gated_scan_backward(BlockType type, const GatedScanArgs& args, cudaStream_t stream);
+cudaError_t launch_gated_scan(BlockType type, const GatedScanArgs& args, bool backward, cudaStream_t stream);
 cudaError_t launch_gated_scan_step(BlockType type, const GatedStepArgs& args, cudaStream_t stream);
 
 // ---- block norm (block_norm.cuh) ------------------------------------------

@@ -294,10 +294,7 @@ cubf::GatedScanArgs scan_args(const cubutterflyB200GatedScan_t* a, bool backward
 }
 
 size_t scan_workspace(const cubutterflyB200GatedScan_t& a) {
-    const size_t cluster = static_cast<size_t>(
-        cubf::gated_scan_cluster(static_cast<int>(a.batch), static_cast<int>(a.length), static_cast<int>(a.dim),
-                                 cubf::kGatedScanBackwardTile));
-    return (a.batch * cluster * a.dim * sizeof(float) + 15) / 16 * 16;
+    return (a.batch * a.dim * sizeof(float) + 15) / 16 * 16;
 }
 
 }  // namespace
@@ -344,7 +341,7 @@ extern "C" cubutterflyStatus_t cubutterflyB200GatedScanForward(const cubutterfly
         const cubf::GatedScanArgs a = scan_args(args, false, &block);
         supported(a.length > 0 || a.batch == 0, "gated scan: of zero tokens the final states are the initial ones");
         if (a.batch == 0) return;
-        check(cubf::launch_gated_scan(block, a, stream), "gated scan launch");
+        check(cubf::launch_gated_scan(block, a, false, stream), "gated scan launch");
     });
 }
 
@@ -366,7 +363,7 @@ extern "C" cubutterflyStatus_t cubutterflyB200GatedScanBackward(const cubutterfl
         require(args->workspace && args->workspace_bytes >= scan_workspace(*args) && element_aligned(args->workspace, 16),
                 "gated scan: the backward needs a 16-byte aligned workspace of the queried size");
         a.partials = static_cast<float*>(args->workspace);
-        check(cubf::launch_gated_scan_backward(block, a, stream), "gated scan backward launch");
+        check(cubf::launch_gated_scan(block, a, true, stream), "gated scan backward launch");
     });
 }
 

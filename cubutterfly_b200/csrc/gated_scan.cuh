@@ -6,13 +6,12 @@
 //   h_t = a_t h_{t-1} + u_t,   u_t = sqrt(1 - a_t^2) sigmoid(i_t) x_t.
 // A run of tokens is the affine map h -> A h + H (A the product of its a, H
 // its last h from h = 0), and runs join by (A1, H1) . (A2, H2) =
-// (A1 A2, A2 H1 + H2), so time is split three ways: a thread runs STEPS
-// tokens of two channels in registers, the kWarps warps of a CTA join their
-// maps through shared memory, and the CTAs of a cluster, which hold
-// consecutive tiles of the same channels, join theirs through distributed
-// shared memory; the cluster then walks along the sequence.  Every input is
-// read once, every output written once, and no CTA waits on one outside its
-// cluster.
+// (A1 A2, A2 H1 + H2).  A thread runs STEPS tokens of two channels in
+// registers; GROUPS groups of lanes hold consecutive runs of the same
+// channels and join them by shuffles; the state then goes from warp to warp
+// of a CTA, and from its last warp to the first one's next tile, one fused
+// multiply-add a warp.  Every input is read once, every output written once,
+// and no CTA waits on another.
 //
 // What bounds it is issue slots before memory: at the rate of a device copy
 // (8 bytes a bf16 element forward) an element may take 45 of them, and the
@@ -33,8 +32,7 @@ using f32x2::sub2;
 using Pair = f32x2::P;
 
 constexpr int kWarps = 8;                  // warps per CTA, consecutive in time
-constexpr int kChannels = 64;              // channels per CTA, two per lane
-static_assert(kGatedScanMaxCluster <= kWarps, "a warp reads the map of each CTA of the cluster");
+constexpr int kWarpChannels = 64;          // channels times lane groups of a warp: two channels per lane
 // Tokens per thread and tile: as many as two CTAs' registers and shared
 // memory allow.
 template <typename T>
@@ -64,9 +62,9 @@ struct Raw {
     static CUBF_DEV Word zero() { return 0u; }
     static CUBF_DEV Word lowest() { return std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u; }  // -inf
     static CUBF_DEV Word vec(const T* p) { return __ldcs(reinterpret_cast<const unsigned int*>(p)); }
-    static CUBF_DEV Word two(const T* p, bool ok0, bool ok1) {
+    static CUBF_DEV Word two(const T* p, int apart, bool ok0, bool ok1) {
         const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
-        const uint32_t lo = ok0 ? __ldcs(q) : 0u, hi = ok1 ? __ldcs(q + 32) : 0u;
+        const uint32_t lo = ok0 ? __ldcs(q) : 0u, hi = ok1 ? __ldcs(q + apart) : 0u;
         return lo | (hi << 16);
     }
     static CUBF_DEV Pair get(Word w) {
@@ -97,8 +95,8 @@ struct Raw<float> {
     static CUBF_DEV Word zero() { return make_float2(0.f, 0.f); }
     static CUBF_DEV Word lowest() { return make_float2(-INFINITY, -INFINITY); }
     static CUBF_DEV Word vec(const float* p) { return __ldcs(reinterpret_cast<const float2*>(p)); }
-    static CUBF_DEV Word two(const float* p, bool ok0, bool ok1) {
-        return make_float2(ok0 ? __ldcs(p) : 0.f, ok1 ? __ldcs(p + 32) : 0.f);
+    static CUBF_DEV Word two(const float* p, int apart, bool ok0, bool ok1) {
+        return make_float2(ok0 ? __ldcs(p) : 0.f, ok1 ? __ldcs(p + apart) : 0.f);
     }
     static CUBF_DEV Pair get(Word w) { return pair(w); }
     static CUBF_DEV Word word_of(float2 f) { return f; }
@@ -110,24 +108,26 @@ struct Raw<float> {
 // by pair; or value by value.
 enum Access : int { kScalar = 0, kPairs = 1, kAsync = 2 };
 
-// The lane's two channels: adjacent with pair accesses, else 32 apart, so
-// that scalar accesses still coalesce.
-template <Access ACCESS>
+// The lane's two channels: adjacent with pair accesses, else as far apart as
+// its group has lanes, so that scalar accesses still coalesce.
+// Lanes of a group are adjacent; groups hold consecutive runs of tokens.
+template <Access ACCESS, int GROUPS>
 struct Lane {
     static constexpr bool VEC = ACCESS != kScalar;
+    static constexpr int kLanes = 32 / GROUPS;
     int ch;
     bool ok0, ok1;
     CUBF_DEV Lane(int c0, int lane, int dim) {
-        ch = c0 + (VEC ? 2 * lane : lane);
+        ch = c0 + (VEC ? 2 : 1) * (lane % kLanes);
         ok0 = ch < dim;
-        ok1 = VEC ? ok0 : ch + 32 < dim;
+        ok1 = VEC ? ok0 : ch + kLanes < dim;
     }
     template <typename T>
     CUBF_DEV typename Raw<T>::Word load(const T* row) const {
         if constexpr (VEC)
             return ok0 ? Raw<T>::vec(row + ch) : Raw<T>::zero();
         else
-            return Raw<T>::two(row + ch, ok0, ok1);
+            return Raw<T>::two(row + ch, kLanes, ok0, ok1);
     }
     template <typename T>
     CUBF_DEV void store(T* row, Pair p) const {
@@ -136,34 +136,38 @@ struct Lane {
             if (ok0) Raw<T>::store_vec(row + ch, f);
         } else {
             if (ok0) row[ch] = Convert<T, float>::store(f.x);
-            if (ok1) row[ch + 32] = Convert<T, float>::store(f.y);
+            if (ok1) row[ch + kLanes] = Convert<T, float>::store(f.y);
         }
     }
     CUBF_DEV Pair load32(const float* row) const {
-        return f32x2::pk(ok0 ? row[ch] : 0.f, ok1 ? row[ch + (VEC ? 1 : 32)] : 0.f);
+        return f32x2::pk(ok0 ? row[ch] : 0.f, ok1 ? row[ch + (VEC ? 1 : kLanes)] : 0.f);
     }
     CUBF_DEV void store32(float* row, Pair p) const {
         const float2 f = floats(p);
         if (ok0) row[ch] = f.x;
-        if (ok1) row[ch + (VEC ? 1 : 32)] = f.y;
+        if (ok1) row[ch + (VEC ? 1 : kLanes)] = f.y;
     }
 };
 
-// The rows of a warp's tokens, N tensors of STEPS tokens x 64 channels each.
-// With kAsync a warp copies its own rows into its own shared memory (no
-// barrier beyond the warp's), STAGES tiles deep: the copies of a later tile
-// are in flight while this one is worked on, and hold no registers.  Results
-// take the place of words that have been read and leave in 16-byte pieces:
-// stored from registers, each pair would cost as many instructions in
-// addresses as its arithmetic.  Channels past the end are zero; tokens past
-// the end are what `tail` says.
-template <typename T, int N, int STEPS_, int STAGES_, Access ACCESS>
+// The rows of a warp's tokens: N tensors of GROUPS x STEPS tokens x CHANNELS
+// channels.  With kAsync a warp copies its own rows into its own shared
+// memory (no barrier beyond the warp's), STAGES tiles deep: the copies of a
+// later tile are in flight while this one is worked on, and hold no registers.
+// Token g STEPS + s lies at row s GROUPS + g, so that the lanes of all groups
+// read adjacent words.  Results take the place of words that have been read
+// and leave in 16-byte pieces: stored from registers, each pair would cost as
+// many instructions in addresses as its arithmetic.  Channels past the end are
+// zero; tokens past the end are what `tail` says.
+template <typename T, int N, int STEPS_, int STAGES_, int GROUPS, Access ACCESS>
 struct Rows {
-    static constexpr int STEPS = STEPS_, STAGES = STAGES_;
-    static constexpr int kBytes = ACCESS == kAsync ? N * STEPS * kChannels * static_cast<int>(sizeof(T)) : 0;
-    static constexpr int kPerRow = kChannels * static_cast<int>(sizeof(T)) / 16;  // 16-byte pieces of a row
-    static constexpr int kRowsPer = 32 / kPerRow;                                 // rows a warp copies at a time
-    static constexpr int kCopies = STEPS / kRowsPer;                              // per lane and tensor
+    static constexpr int STEPS = STEPS_, STAGES = STAGES_, TOKENS = STEPS * GROUPS;
+    static constexpr int kChannels = kWarpChannels / GROUPS;
+    static constexpr int kRowBytes = kChannels * static_cast<int>(sizeof(T));
+    static constexpr int kTensorBytes = TOKENS * kRowBytes;
+    static constexpr int kBytes = ACCESS == kAsync ? N * kTensorBytes : 0;
+    static constexpr int kPerRow = kRowBytes / 16;        // 16-byte pieces of a row
+    static constexpr int kRowsPer = 32 / kPerRow;         // rows a warp copies at a time
+    static constexpr int kCopies = TOKENS / kRowsPer;     // per lane and tensor
     using Word = typename Raw<T>::Word;
     const T* base[N];
     size_t stride[N];
@@ -172,6 +176,14 @@ struct Rows {
     int lane, c0, length, dim;
 
     CUBF_DEV int piece() const { return lane % kPerRow * (16 / static_cast<int>(sizeof(T))); }
+    // where this lane's piece of the k-th rows lies: what follows from the lane, and from k
+    CUBF_DEV int piece_place() const {
+        const int r = lane / kPerRow;
+        return (r % STEPS * GROUPS + r / STEPS) * kRowBytes + lane % kPerRow * 16;
+    }
+    static constexpr int row_place(int k) {
+        return (k * kRowsPer % STEPS * GROUPS + k * kRowsPer / STEPS) * kRowBytes;
+    }
 
     CUBF_DEV void init(unsigned char* shared, int lane_, int c0_, int length_, int dim_, int first) {
         mine = shared;
@@ -186,34 +198,37 @@ struct Rows {
                           c0 + piece();
         }
     }
-    CUBF_DEV Word* word(int stage, int n, int s) const {
-        return reinterpret_cast<Word*>(reinterpret_cast<T*>(mine + stage * kBytes) + (n * STEPS + s) * kChannels +
-                                       2 * lane);
+    CUBF_DEV Word* word(int stage, int n, int s) const {  // of the lane's own token s
+        return reinterpret_cast<Word*>(mine + stage * kBytes + n * kTensorBytes + s * GROUPS * kRowBytes) + lane;
     }
-    // starts the copies of tokens [t, t + STEPS), closes their group, and
+    // starts the copies of tokens [t, t + TOKENS), closes their group, and
     // moves on by `advance` tokens
     CUBF_DEV void fetch(int stage, int t, int advance) {
         if constexpr (ACCESS == kAsync) {
-            const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(mine + stage * kBytes)) + lane * 16;
-            if (t >= 0 && t + STEPS <= length && c0 + kChannels <= dim) {
+            const uint32_t dst =
+                static_cast<uint32_t>(__cvta_generic_to_shared(mine + stage * kBytes)) + piece_place();
+            if (t >= 0 && t + TOKENS <= length && c0 + kChannels <= dim) {
 #pragma unroll
                 for (int n = 0; n < N; ++n) {
                     const T* src = next[n];
 #pragma unroll
                     for (int k = 0; k < kCopies; ++k) {
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + (n * kCopies + k) * 512),
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + n * kTensorBytes +
+                                                                                      row_place(k)),
                                      "l"(src)
                                      : "memory");
                         src += kRowsPer * stride[n];
                     }
                 }
-            } else if (t < length && t + STEPS > 0) {
+            } else if (t < length && t + TOKENS > 0) {
+#pragma unroll
                 for (int n = 0; n < N; ++n)
+#pragma unroll
                     for (int k = 0; k < kCopies; ++k) {
                         const int at = t + lane / kPerRow + k * kRowsPer, col = c0 + piece();
                         const bool in = at >= 0 && at < length && col < dim;
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                                         dst + (n * kCopies + k) * 512),
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + n * kTensorBytes +
+                                                                                          row_place(k)),
                                      "l"(in ? base[n] + static_cast<size_t>(at) * stride[n] + col : base[n]),
                                      "r"(in ? 16 : 0)
                                      : "memory");
@@ -235,7 +250,8 @@ struct Rows {
             __syncwarp();
         }
     }
-    CUBF_DEV Word get(const Lane<ACCESS>& ln, int stage, int n, int t, int s, Word tail) const {
+    // The lane's token t + s (t the first of its run).
+    CUBF_DEV Word get(const Lane<ACCESS, GROUPS>& ln, int stage, int n, int t, int s, Word tail) const {
         if constexpr (ACCESS == kAsync)
             return *word(stage, n, s);
         else
@@ -252,28 +268,29 @@ struct Rows {
     // Token t + s of an output (rows of `dim` channels from `out`): into the
     // place of tensor n's word, or straight to memory.  The caller has checked
     // that the token exists unless ACCESS is kAsync.
-    CUBF_DEV void put(const Lane<ACCESS>& ln, int stage, int n, T* out, int t, int s, Pair v) const {
+    CUBF_DEV void put(const Lane<ACCESS, GROUPS>& ln, int stage, int n, T* out, int t, int s, Pair v) const {
         if constexpr (ACCESS == kAsync)
             *word(stage, n, s) = Raw<T>::word_of(floats(v));
         else
             ln.store(out + static_cast<size_t>(t + s) * dim, v);
     }
-    // writes the tile put in tensor n's place out
+    // writes the tile put in tensor n's place, the warp's tokens from t, out
     CUBF_DEV void flush(int stage, int n, T* out, int t) const {
         if constexpr (ACCESS == kAsync) {
-            const unsigned char* src = mine + stage * kBytes + n * kCopies * 512 + lane * 16;
+            const unsigned char* src = mine + stage * kBytes + n * kTensorBytes + piece_place();
             const int row = t + lane / kPerRow, col = c0 + piece();
             T* dst = out + static_cast<size_t>(row) * dim + col;
-            if (t + STEPS <= length && c0 + kChannels <= dim) {
+            if (t + TOKENS <= length && c0 + kChannels <= dim) {
 #pragma unroll
                 for (int k = 0; k < kCopies; ++k) {
-                    __stcs(reinterpret_cast<uint4*>(dst), *reinterpret_cast<const uint4*>(src + k * 512));
+                    __stcs(reinterpret_cast<uint4*>(dst), *reinterpret_cast<const uint4*>(src + row_place(k)));
                     dst += static_cast<size_t>(kRowsPer) * dim;
                 }
             } else {
+#pragma unroll
                 for (int k = 0; k < kCopies; ++k) {
                     if (row + k * kRowsPer < length && col < dim)
-                        __stcs(reinterpret_cast<uint4*>(dst), *reinterpret_cast<const uint4*>(src + k * 512));
+                        __stcs(reinterpret_cast<uint4*>(dst), *reinterpret_cast<const uint4*>(src + row_place(k)));
                     dst += static_cast<size_t>(kRowsPer) * dim;
                 }
             }
@@ -413,15 +430,6 @@ struct Walker {
     CUBF_DEV bool inside(int t, int n) const { return start < t && t + n < stop; }
 };
 
-CUBF_DEV uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-CUBF_DEV void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 // Hand-over from one warp to another on a named barrier that counts both
 // warps: the giver's shared-memory writes before give() are seen after take().
 // A giver comes back to a barrier only after what it gave has come round, so a
@@ -429,54 +437,69 @@ CUBF_DEV void cluster_sync() {
 CUBF_DEV void give(int barrier) { asm volatile("bar.arrive %0, 64;" ::"r"(barrier) : "memory"); }
 CUBF_DEV void take(int barrier) { asm volatile("bar.sync %0, 64;" ::"r"(barrier) : "memory"); }
 
-// An affine map of a lane's two channels.
-struct alignas(16) Map {
-    Pair a, h;
+// The affine map of a run, and of the runs of the lane groups before (or with
+// REVERSE after) this lane's own, and of all of them.
+template <int GROUPS, bool PACKED, bool REVERSE>
+struct Joined {
+    Pair before_a, before_h, a, h;
+
+    static CUBF_DEV Pair from(Pair v, int lane) {
+        return __shfl_sync(0xffffffffu, v, lane);
+    }
+    CUBF_DEV void join(Pair run_a, Pair run_h, int lane) {
+        a = run_a;
+        h = run_h;
+        before_a = both(1.f);
+        before_h = both(0.f);
+        if constexpr (GROUPS > 1) {
+            constexpr int kLanes = 32 / GROUPS;
+            const int group = REVERSE ? GROUPS - 1 - lane / kLanes : lane / kLanes;
+#pragma unroll
+            for (int d = 1; d < GROUPS; d *= 2) {  // inclusive over the groups
+                const int src = (lane + (REVERSE ? d : -d) * kLanes) & 31;
+                const Pair pa = from(a, src), ph = from(h, src);
+                if (group >= d) {
+                    h = through<PACKED>(a, h, ph);
+                    a = product<PACKED>(pa, a);
+                }
+            }
+            const int src = (lane + (REVERSE ? 1 : -1) * kLanes) & 31;
+            const Pair pa = from(a, src), ph = from(h, src);
+            if (group > 0) {
+                before_a = pa;
+                before_h = ph;
+            }
+            const int last = lane % kLanes + (REVERSE ? 0 : (GROUPS - 1) * kLanes);
+            a = from(a, last);
+            h = from(h, last);
+        }
+    }
 };
-CUBF_DEV void store_remote(const Map* local, uint32_t rank, Map v) {
-    const uint32_t addr = static_cast<uint32_t>(__cvta_generic_to_shared(local));
-    uint32_t remote;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-    asm volatile("st.shared::cluster.v2.u64 [%0], {%1, %2};" ::"r"(remote), "l"(v.a), "l"(v.h) : "memory");
-}
 
 // ---- forward ----------------------------------------------------------------------------------
-template <bool CLUSTER>
-struct Maps {
-    Map warp[2][kWarps][32];
-    Map cta[2][kGatedScanMaxCluster][32];
-};
-template <>
-struct Maps<false> {
-    Pair carry[kWarps][32];  // h before the warp's tokens
-};
+template <typename T, int GROUPS, Access ACCESS>
+using ForwardRows = Rows<T, 3, kForwardSteps<T>, 2, GROUPS, ACCESS>;
 
-template <typename T, Access ACCESS>
-using ForwardRows = Rows<T, 3, kForwardSteps<T>, 2, ACCESS>;
-
-template <typename T, bool PACKED, bool CLUSTER, Access ACCESS>
-__global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArgs p, int cluster_, int tiles) {
-    using Tile = ForwardRows<T, ACCESS>;
-    constexpr int kSteps = Tile::STEPS, kTile = kSteps * kWarps;
+template <typename T, bool PACKED, int GROUPS, Access ACCESS>
+__global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArgs p, int tiles) {
+    using Tile = ForwardRows<T, GROUPS, ACCESS>;
+    constexpr int kSteps = Tile::STEPS, stride = Tile::TOKENS * kWarps;  // tokens a CTA takes a round
     using Word = typename Raw<T>::Word;
     extern __shared__ __align__(16) unsigned char staged[];
-    __shared__ Maps<CLUSTER> maps;
+    __shared__ Pair handed[kWarps][32];  // h before the warp's tokens
     pdl_begin();
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
-    const int cluster = CLUSTER ? cluster_ : 1;
-    const int rank = CLUSTER ? static_cast<int>(cluster_rank()) : 0;
-    const unsigned column = blockIdx.x / cluster;
-    const int c0 = static_cast<int>(column % tiles) * kChannels;
-    const Lane<ACCESS> ln(c0, lane, p.dim);
-    const size_t b = column / tiles;
-    const int stride = cluster * kTile;
-    int t0 = rank * kTile + warp * kSteps;
+    const int group = lane / (32 / GROUPS);
+    const int c0 = static_cast<int>(blockIdx.x % tiles) * Tile::kChannels;
+    const Lane<ACCESS, GROUPS> ln(c0, lane, p.dim);
+    const size_t b = blockIdx.x / tiles;
+    int w0 = warp * Tile::TOKENS;  // the warp's first token; the lane's run begins at t0
     Tile rows{{static_cast<const T*>(p.x) + b * p.x_batch, static_cast<const T*>(p.r) + b * p.r_batch,
                static_cast<const T*>(p.i) + b * p.i_batch},
               {p.x_token, p.r_token, p.i_token}};
-    rows.init(staged + warp * Tile::STAGES * Tile::kBytes, lane, c0, p.length, p.dim, t0);
+    rows.init(staged + warp * Tile::STAGES * Tile::kBytes, lane, c0, p.length, p.dim, w0);
 #pragma unroll
-    for (int k = 0; k < Tile::STAGES; ++k) rows.fetch(k, t0 + k * stride, stride);
+    for (int k = 0; k < Tile::STAGES; ++k) rows.fetch(k, w0 + k * stride, stride);
     T* out = static_cast<T*>(p.h) + b * static_cast<size_t>(p.length) * p.dim;
     const Pair rate = mul2(rates(ln.load32(p.decay), p.exponent), both(-1.f));
     float* chunk_states = nullptr;
@@ -487,18 +510,18 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
     Walker seq;
     if constexpr (PACKED) {
         seq.init(p.offsets, p.sequences);
-        if (rank == 0)  // sequences without tokens end where they began
+        if (group == 0)  // sequences without tokens end where they began
             for (int j = warp; j < p.sequences; j += kWarps)
                 if (p.offsets[j] >= p.offsets[j + 1])
                     ln.store32(p.last + static_cast<size_t>(j) * p.dim,
                                p.initial ? ln.load32(p.initial + static_cast<size_t>(j) * p.dim) : both(0.f));
     }
-    Pair carry = both(0.f);  // h before the cluster's tiles
+    Pair carry = both(0.f);  // h before the sequence, in the end after it
     if (!PACKED && p.initial) carry = ln.load32(p.initial + b * p.dim);
 
     const int rounds = (p.length + stride - 1) / stride;
-    for (int round = 0; round < rounds; ++round, t0 += stride) {
-        const int buf = round & 1;
+    for (int round = 0; round < rounds; ++round, w0 += stride) {
+        const int buf = round & 1, t0 = w0 + group * kSteps;
         // Tokens past the end are a shut gate (r = -inf: a = 1) over x = 0:
         // the identity map.
         Pair a[kSteps], u[kSteps];
@@ -545,46 +568,25 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
                 }
             }
         }
-        Pair h;  // before this warp's tokens
-        if constexpr (!CLUSTER) {
-            // The state goes from warp to warp, and from the last one to the
-            // first one's next tile; no barrier holds all warps, so they
-            // drift apart and one's loads, gates and stores overlap
-            // another's.
-            h = carry;
-            if (warp > 0 || round > 0) {
-                take(1 + warp);
-                h = maps.carry[warp][lane];
-            }
-            const Pair next = through<PACKED>(A, H, h);
-            if (warp + 1 < kWarps || round + 1 < rounds) {
-                const int to = (warp + 1) % kWarps;
-                maps.carry[to][lane] = next;
-                give(1 + to);
-            } else {
-                carry = next;
-            }
-        } else {
-            maps.warp[buf][warp][lane] = Map{A, H};
-            __syncthreads();
-            Map before{both(1.f), both(0.f)}, total = before;
-#pragma unroll
-            for (int k = 0; k < kWarps; ++k) {
-                const Map m = maps.warp[buf][k][lane];
-                total.h = through<PACKED>(m.a, m.h, total.h);
-                total.a = product<PACKED>(total.a, m.a);
-                if (k + 1 == warp) before = total;
-            }
-            if (warp < cluster) store_remote(&maps.cta[buf][rank][lane], warp, total);
-            cluster_sync();
-            h = carry;  // then before this CTA's tile
-            for (int k = 0; k < cluster; ++k) {
-                const Map m = maps.cta[buf][k][lane];
-                carry = through<PACKED>(m.a, m.h, carry);
-                if (k + 1 == rank) h = carry;
-            }
-            if (warp > 0) h = through<PACKED>(before.a, before.h, h);
+        // The state goes from warp to warp, and from the last one to the first
+        // one's next tile; no barrier holds all warps, so they drift apart and
+        // one's loads, gates and stores overlap another's.
+        Joined<GROUPS, PACKED, false> runs;
+        runs.join(A, H, lane);
+        Pair h = carry;
+        if (warp > 0 || round > 0) {
+            take(1 + warp);
+            h = handed[warp][lane];
         }
+        const Pair next = through<PACKED>(runs.a, runs.h, h);
+        if (warp + 1 < kWarps || round + 1 < rounds) {
+            const int to = (warp + 1) % kWarps;
+            handed[to][lane] = next;
+            give(1 + to);
+        } else {
+            carry = next;
+        }
+        if (GROUPS > 1 && group > 0) h = through<PACKED>(runs.before_a, runs.before_h, h);  // before the lane's run
         if (chunk_states && t0 % kGatedScanChunk == 0 && t0 < p.length)
             ln.store32(chunk_states + static_cast<size_t>(t0 / kGatedScanChunk) * p.dim, h);
         if (plain) {
@@ -606,12 +608,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
             }
         }
         __syncwarp();
-        rows.flush(buf, 0, out, t0);
+        rows.flush(buf, 0, out, w0);
         __syncwarp();  // the tile has been read
-        rows.fetch(buf, t0 + Tile::STAGES * stride, stride);
+        rows.fetch(buf, w0 + Tile::STAGES * stride, stride);
     }
-    if (!PACKED && rank == 0 && warp == (CLUSTER ? 0 : kWarps - 1)) ln.store32(p.last + b * p.dim, carry);
-    if constexpr (CLUSTER) cluster_sync();  // no CTA leaves while another may still store into it
+    if (!PACKED && warp == kWarps - 1 && group == 0) ln.store32(p.last + b * p.dim, carry);
 }
 
 // ---- backward ----------------------------------------------------------------------------------
@@ -624,48 +625,32 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
 //   dr = e (1 - sigmoid(r))   dLambda = sum e sigmoid(Lambda)/softplus(Lambda)
 // A thread keeps a, v, 1/m and sigmoid(r) of its tokens and gets sigmoid(i)
 // back as v/m, which leaves room for two CTAs per SM.
-template <bool CLUSTER>
-struct BackMaps {
-    Pair half[kWarps][32];    // h before the warp's tokens, where the warp before has it
-    Pair sum[kWarps][32];
-    Map warp[2][kWarps][32];  // of P, from the end of time
-    Map cta[2][kGatedScanMaxCluster][32];
-};
-template <>
-struct BackMaps<false> {
-    Pair half[kWarps][32];
-    Pair sum[kWarps][32];
-    Pair carry[kWarps][32];   // P from the tokens after the warp's
-};
+template <typename T, int GROUPS, Access ACCESS>
+using BackwardRows = Rows<T, 4, kBackwardSteps, sizeof(T) == 2 ? 2 : 1, GROUPS, ACCESS>;
 
-template <typename T, Access ACCESS>
-using BackwardRows = Rows<T, 4, kBackwardSteps, sizeof(T) == 2 ? 2 : 1, ACCESS>;
-
-template <typename T, bool PACKED, bool CLUSTER, Access ACCESS>
-__global__ void __launch_bounds__(kWarps * 32, 2)
-    gated_scan_backward_kernel(GatedScanArgs p, int cluster_, int tiles) {
-    using Tile = BackwardRows<T, ACCESS>;
-    constexpr int kSteps = Tile::STEPS, kTile = kSteps * kWarps;
+template <typename T, bool PACKED, int GROUPS, Access ACCESS>
+__global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(GatedScanArgs p, int tiles) {
+    using Tile = BackwardRows<T, GROUPS, ACCESS>;
+    constexpr int kSteps = Tile::STEPS, stride = Tile::TOKENS * kWarps;  // tokens a CTA takes a round
     using Word = typename Raw<T>::Word;
     extern __shared__ __align__(16) unsigned char staged[];
-    __shared__ BackMaps<CLUSTER> maps;
+    __shared__ Pair handed[kWarps][32];  // P from the tokens after the warp's
+    __shared__ Pair middle[kWarps][32];  // h before the warp's tokens, where the warp before has it
+    __shared__ Pair sums[kWarps][32];
     pdl_begin();
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
-    const int cluster = CLUSTER ? cluster_ : 1;
-    const int rank = CLUSTER ? static_cast<int>(cluster_rank()) : 0;
-    const unsigned column = blockIdx.x / cluster;
-    const int c0 = static_cast<int>(column % tiles) * kChannels;
-    const Lane<ACCESS> ln(c0, lane, p.dim);
-    const size_t b = column / tiles;
-    const int stride = cluster * kTile;
+    const int group = lane / (32 / GROUPS);
+    const int c0 = static_cast<int>(blockIdx.x % tiles) * Tile::kChannels;
+    const Lane<ACCESS, GROUPS> ln(c0, lane, p.dim);
+    const size_t b = blockIdx.x / tiles;
     const int rounds = (p.length + stride - 1) / stride;
-    int t0 = (rounds - 1) * stride + rank * kTile + warp * kSteps;
+    int w0 = (rounds - 1) * stride + warp * Tile::TOKENS;  // the warp's first token; the lane's run begins at t0
     Tile rows{{static_cast<const T*>(p.x) + b * p.x_batch, static_cast<const T*>(p.r) + b * p.r_batch,
                static_cast<const T*>(p.i) + b * p.i_batch, static_cast<const T*>(p.d_h) + b * p.dh_batch},
               {p.x_token, p.r_token, p.i_token, p.dh_token}};
-    rows.init(staged + warp * Tile::STAGES * Tile::kBytes, lane, c0, p.length, p.dim, t0);
+    rows.init(staged + warp * Tile::STAGES * Tile::kBytes, lane, c0, p.length, p.dim, w0);
 #pragma unroll
-    for (int k = 0; k < Tile::STAGES; ++k) rows.fetch(k, t0 - k * stride, -stride);
+    for (int k = 0; k < Tile::STAGES; ++k) rows.fetch(k, w0 - k * stride, -stride);
     const size_t out = b * static_cast<size_t>(p.length) * p.dim;
     T* dx = static_cast<T*>(p.d_x) + out;
     T* dr = static_cast<T*>(p.d_r) + out;
@@ -678,21 +663,22 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     Walker seq;
     if constexpr (PACKED) {
         seq.init(p.offsets, p.sequences);
-        if (p.d_initial && rank == 0)  // sequences without tokens pass their gradient through
+        if (p.d_initial && group == 0)  // sequences without tokens pass their gradient through
             for (int j = warp; j < p.sequences; j += kWarps)
                 if (p.offsets[j] >= p.offsets[j + 1])
                     ln.store32(p.d_initial + static_cast<size_t>(j) * p.dim,
                                p.d_last ? ln.load32(p.d_last + static_cast<size_t>(j) * p.dim) : both(0.f));
     }
-    Pair carry = both(0.f);  // P from the tokens after the cluster's tiles
+    Pair carry = both(0.f);  // P from after the sequence, in the end from all of it
     if (!PACKED && p.d_last) carry = ln.load32(p.d_last + b * p.dim);
     Pair sum = both(0.f);    // of e
 
-    for (int round = 0; round < rounds; ++round, t0 -= stride) {  // from the end of time
-        const int buf = round & 1, stage = Tile::STAGES == 2 ? buf : 0;
-        // before the warp's tokens: from the forward, or (below) from the warp before
+    for (int round = 0; round < rounds; ++round, w0 -= stride) {  // from the end of time
+        const int stage = Tile::STAGES == 2 ? round & 1 : 0, t0 = w0 + group * kSteps;
+        // before the run: from the forward, or (below) from the run before in its chunk
         Pair h = both(0.f);
-        if (warp % 2 == 0 && t0 < p.length)
+        const bool second = (GROUPS > 1 ? group : warp) % 2;
+        if (!second && t0 < p.length)
             h = ln.load32(chunk_states + static_cast<size_t>(t0 / kGatedScanChunk) * p.dim);
         // x and dh are read where they are used, from shared memory; other
         // accesses keep them
@@ -786,51 +772,35 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
                 }
             }
         }
-        // h from the warp before, within a chunk
-        if (warp % 2 == 0) {
-            maps.half[warp + 1][lane] = through<PACKED>(A, H, h);
+        // h from the run before, within a chunk
+        const Pair middle_h = through<PACKED>(A, H, h);
+        if constexpr (GROUPS > 1) {
+            const Pair before = __shfl_sync(0xffffffffu, middle_h, (lane - 32 / GROUPS) & 31);
+            if (second) h = before;
+        } else if (!second) {
+            middle[warp + 1][lane] = middle_h;
             give(1 + kWarps + warp / 2);
         } else {
             take(1 + kWarps + warp / 2);
-            h = maps.half[warp][lane];
+            h = middle[warp][lane];
         }
-        Pair P;  // from the tokens after this warp's
-        if constexpr (!CLUSTER) {
-            // from warp to warp, as the forward's state, from the end of time
-            P = carry;
-            if (warp + 1 < kWarps || round > 0) {
-                take(1 + warp);
-                P = maps.carry[warp][lane];
-            }
-            const Pair next = through<PACKED>(A, R, P);
-            if (warp > 0 || round + 1 < rounds) {
-                const int to = (warp + kWarps - 1) % kWarps;
-                maps.carry[to][lane] = next;
-                give(1 + to);
-            } else {
-                carry = next;
-            }
+        // P from warp to warp, as the forward's state, from the end of time
+        Joined<GROUPS, PACKED, true> runs;
+        runs.join(A, R, lane);
+        Pair P = carry;
+        if (warp + 1 < kWarps || round > 0) {
+            take(1 + warp);
+            P = handed[warp][lane];
+        }
+        const Pair next = through<PACKED>(runs.a, runs.h, P);
+        if (warp > 0 || round + 1 < rounds) {
+            const int to = (warp + kWarps - 1) % kWarps;
+            handed[to][lane] = next;
+            give(1 + to);
         } else {
-            maps.warp[buf][warp][lane] = Map{A, R};
-            __syncthreads();
-            Map after{both(1.f), both(0.f)}, total = after;
-#pragma unroll
-            for (int k = kWarps - 1; k >= 0; --k) {
-                const Map q = maps.warp[buf][k][lane];
-                total.h = through<PACKED>(q.a, q.h, total.h);
-                total.a = product<PACKED>(total.a, q.a);
-                if (k == warp + 1) after = total;
-            }
-            if (warp < cluster) store_remote(&maps.cta[buf][rank][lane], warp, total);
-            cluster_sync();
-            P = carry;  // then from the tokens after this CTA's tile
-            for (int k = cluster - 1; k >= 0; --k) {
-                const Map q = maps.cta[buf][k][lane];
-                carry = through<PACKED>(q.a, q.h, carry);
-                if (k == rank + 1) P = carry;
-            }
-            if (warp + 1 < kWarps) P = through<PACKED>(after.a, after.h, P);
+            carry = next;
         }
+        if (GROUPS > 1 && group + 1 < GROUPS) P = through<PACKED>(runs.before_a, runs.before_h, P);
 
         // h before each token, then the gradients from the last token back
         Pair before[kSteps];
@@ -879,24 +849,26 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
             }
         }
         __syncwarp();
-        rows.flush(stage, 0, dx, t0);
-        rows.flush(stage, 1, dr, t0);
-        rows.flush(stage, 2, di, t0);
+        rows.flush(stage, 0, dx, w0);
+        rows.flush(stage, 1, dr, w0);
+        rows.flush(stage, 2, di, w0);
         __syncwarp();  // the tile has been read
-        rows.fetch(stage, t0 - Tile::STAGES * stride, -stride);
+        rows.fetch(stage, w0 - Tile::STAGES * stride, -stride);
     }
-    if (!PACKED && p.d_initial && rank == 0 && warp == 0) ln.store32(p.d_initial + b * p.dim, carry);
-    maps.sum[warp][lane] = sum;
+    if (!PACKED && p.d_initial && warp == 0 && group == 0) ln.store32(p.d_initial + b * p.dim, carry);
+    sums[warp][lane] = sum;
     __syncthreads();
-    if (warp == 0) {
-        for (int k = 1; k < kWarps; ++k) sum = add2(sum, maps.sum[k][lane]);
-        ln.store32(p.partials + (b * cluster + rank) * static_cast<size_t>(p.dim), sum);
+    if (warp == 0 && group == 0) {
+        sum = both(0.f);
+        for (int k = 0; k < kWarps; ++k)
+            for (int q = 0; q < GROUPS; ++q) sum = add2(sum, sums[k][lane + q * (32 / GROUPS)]);
+        ln.store32(p.partials + b * static_cast<size_t>(p.dim), sum);
     }
-    if constexpr (CLUSTER) cluster_sync();
 }
 
 // dLambda = sigmoid(Lambda)/softplus(Lambda) sum e over the CTAs' partial sums
 // (the ratio tends to 1 as both vanish).
+template <typename T>
 __global__ void __launch_bounds__(256) gated_scan_decay_kernel(GatedScanArgs p, int parts) {
     __shared__ float slice[8][32];
     pdl_begin();
@@ -924,7 +896,7 @@ __global__ void __launch_bounds__(128) gated_scan_step_kernel(GatedStepArgs p, i
     pdl_begin();
     const int lane = threadIdx.x & 31;
     const unsigned task = blockIdx.x * 4 + (threadIdx.x >> 5);
-    const Lane<ACCESS> ln(static_cast<int>(task % tiles) * kChannels, lane, p.dim);
+    const Lane<ACCESS, 1> ln(static_cast<int>(task % tiles) * kWarpChannels, lane, p.dim);
     const size_t first = static_cast<size_t>(task / tiles) * rows;
     if (first >= p.batch) return;
     const size_t end = first + rows < p.batch ? first + rows : p.batch;

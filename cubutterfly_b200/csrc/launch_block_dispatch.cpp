@@ -1,4 +1,5 @@
-// launch_block_norm_dispatch.cpp -- picks the block norm unit of a type pair.
+// launch_block_dispatch.cpp -- picks the unit of a type for the block norm and
+// the gated linear recurrence.
 #include <algorithm>
 
 #include "block_ops.hpp"
@@ -56,6 +57,37 @@ cudaError_t launch_block_norm_backward(BlockType type, bool residual32, const Bl
         case 2: return launch_block_norm_backward_unit<2>(a, groups, stream);
         case 3: return launch_block_norm_backward_unit<3>(a, groups, stream);
         default: return launch_block_norm_backward_unit<4>(a, groups, stream);
+    }
+}
+
+template <int TYPE>
+cudaError_t launch_gated_scan_unit(const GatedScanArgs& a, bool backward, cudaStream_t stream);
+template <int TYPE>
+cudaError_t launch_gated_scan_step_unit(const GatedStepArgs& a, cudaStream_t stream);
+
+#define CUBF_GS_UNIT(TYPE)                                                                  \
+    template <>                                                                             \
+    cudaError_t launch_gated_scan_unit<TYPE>(const GatedScanArgs&, bool, cudaStream_t);     \
+    template <>                                                                             \
+    cudaError_t launch_gated_scan_step_unit<TYPE>(const GatedStepArgs&, cudaStream_t);
+CUBF_GS_UNIT(0)
+CUBF_GS_UNIT(1)
+CUBF_GS_UNIT(2)
+#undef CUBF_GS_UNIT
+
+cudaError_t launch_gated_scan(BlockType type, const GatedScanArgs& a, bool backward, cudaStream_t stream) {
+    switch (type) {
+        case BlockType::kF16: return launch_gated_scan_unit<0>(a, backward, stream);
+        case BlockType::kBF16: return launch_gated_scan_unit<1>(a, backward, stream);
+        default: return launch_gated_scan_unit<2>(a, backward, stream);
+    }
+}
+
+cudaError_t launch_gated_scan_step(BlockType type, const GatedStepArgs& a, cudaStream_t stream) {
+    switch (type) {
+        case BlockType::kF16: return launch_gated_scan_step_unit<0>(a, stream);
+        case BlockType::kBF16: return launch_gated_scan_step_unit<1>(a, stream);
+        default: return launch_gated_scan_step_unit<2>(a, stream);
     }
 }
 
