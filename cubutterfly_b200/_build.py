@@ -2,7 +2,8 @@
 
 Run ``python -m cubutterfly_b200._build`` (or ``__graft_entry__.build()``).
 Objects go to ``cubutterfly_b200/_build/``, the library to
-``cubutterfly_b200/lib/libcubutterfly_b200.so``.  Compilation units are built
+``cubutterfly_b200/lib/libcubutterfly_b200.so``, the torch extension of the
+block operators to ``cubutterfly_b200/_block_ops.so``.  Compilation units are built
 in parallel and only when their sources changed.
 """
 from __future__ import annotations
@@ -20,6 +21,7 @@ CSRC = PKG / "csrc"
 OBJ = PKG / "_build"
 LIB_DIR = PKG / "lib"
 LIB = LIB_DIR / "libcubutterfly_b200.so"
+TORCH_EXT = PKG / "_block_ops.so"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -80,6 +82,28 @@ def _stale(obj: Path) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def _build_torch_extension() -> None:
+    """The block operators' torch extension (host code only; it links against torch, not against the library)."""
+    src = CSRC / "block_ops_torch.cpp"
+    deps = [src, ROOT / "include" / "cubutterfly" / "cubutterfly_b200.h", Path(__file__)]
+    if TORCH_EXT.exists() and all(d.stat().st_mtime <= TORCH_EXT.stat().st_mtime for d in deps):
+        return
+    import sysconfig
+
+    import torch
+
+    torch_dir = Path(torch.__file__).parent
+    includes = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include",
+                Path(NVCC).parents[1] / "include", sysconfig.get_paths()["include"], ROOT / "include"]
+    cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{i}" for i in includes], str(src),
+           "-o", str(TORCH_EXT), f"-L{torch_dir / 'lib'}", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10",
+           "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+
+
 def build(verbose: bool = False, jobs: int | None = None) -> Path:
     OBJ.mkdir(exist_ok=True)
     LIB_DIR.mkdir(exist_ok=True)
@@ -95,9 +119,10 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
             print("built", obj.name, flush=True)
         return obj
 
-    if todo:
-        with ThreadPoolExecutor(max_workers=jobs or max(2, os.cpu_count() or 2)) as ex:
-            list(ex.map(run, todo))
+    with ThreadPoolExecutor(max_workers=jobs or max(2, os.cpu_count() or 2)) as ex:
+        extension = ex.submit(_build_torch_extension)
+        list(ex.map(run, todo))
+        extension.result()
     if todo or not LIB.exists():
         cmd = [NVCC, *ARCH, "-shared", "-o", str(LIB), *[str(u[2]) for u in units], "-cudart", "static",
                "-Xlinker", "--no-undefined", "-lpthread", "-ldl", "-lrt"]

@@ -2,6 +2,7 @@
 before anything is launched)."""
 import ctypes as ct
 import math
+import struct
 
 import pytest
 import torch
@@ -10,6 +11,11 @@ import cubutterfly_b200 as cb
 from cubutterfly_b200 import block_ops, torch_ops
 
 STATUS = cb.Status
+
+# the structs of include/cubutterfly/cubutterfly_b200.h, in field order
+NORM = struct.Struct("@4N8i2d6P3N6P2N6PPN")
+SCAN = struct.Struct("@5N2id3P6N7P2N6PPN")
+STEP = struct.Struct("@4N2id3P3N5P")
 
 
 def test_cpu_tensors_are_rejected():
@@ -32,7 +38,7 @@ def test_torch_ops_exports_the_block_operators():
 def test_gate_shapes():
     """A gate is one row per channel vector, leading index or row; what does not broadcast so is refused."""
     x = torch.empty(6, 5, 8)
-    rows = lambda *shape: block_ops._gate_rows(torch.empty(*shape), x, 30)
+    rows = lambda *shape: block_ops._block_ops.gate_rows(torch.empty(*shape), x, 30)
     assert rows(8) == rows(1, 8) == rows(1, 1, 8) == 1
     assert rows(6, 1, 8) == 6 and rows(6, 5, 8) == 30
     for shape in ((6, 5, 1), (5, 8), (1, 5, 8), (2, 1, 8), (6, 8), (1, 6, 5, 8), (4,)):
@@ -42,14 +48,14 @@ def test_gate_shapes():
 
 def test_row_strides():
     t = torch.empty(4, 6, 16)
-    assert block_ops._rows(t, 16)[1] == 16
-    assert block_ops._rows(t[..., :8], 8)[1] == 16            # collapses to rows 16 apart
-    assert block_ops._rows(t[:, :3, :8], 8)[0].is_contiguous()  # two strides: copied
-    assert block_ops._rows(t.transpose(0, 2), 4)[1] == 4
-    assert block_ops._rows(torch.empty(1, 16).expand(5, 16), 16)[1] == 16
-    assert block_ops._tokens(t[..., :8], 8)[1:] == (96, 16)
-    assert block_ops._tokens(t[:1, :, :8], 8)[1:] == (0, 16)
-    assert block_ops._tokens(torch.empty(4, 1, 16).expand(4, 6, 16), 16)[1:] == (96, 16)
+    assert block_ops._block_ops.rows(t, 16)[1] == 16
+    assert block_ops._block_ops.rows(t[..., :8], 8)[1] == 16            # collapses to rows 16 apart
+    assert block_ops._block_ops.rows(t[:, :3, :8], 8)[0].is_contiguous()  # two strides: copied
+    assert block_ops._block_ops.rows(t.transpose(0, 2), 4)[1] == 4
+    assert block_ops._block_ops.rows(torch.empty(1, 16).expand(5, 16), 16)[1] == 16
+    assert block_ops._block_ops.tokens(t[..., :8], 8)[1:] == (96, 16)
+    assert block_ops._block_ops.tokens(t[:1, :, :8], 8)[1:] == (0, 16)
+    assert block_ops._block_ops.tokens(torch.empty(4, 1, 16).expand(4, 6, 16), 16)[1:] == (96, 16)
 
 
 # Fields of a valid call; device pointers are never dereferenced by the checks.
@@ -57,29 +63,29 @@ P = 4096
 
 
 def norm_fields(**change):
-    f = dict(size=block_ops._NORM.size, rows=4, dim=64, gate_rows=0, data=1, residual_type=1, pre_type=2, post_type=2,
+    f = dict(size=NORM.size, rows=4, dim=64, gate_rows=0, data=1, residual_type=1, pre_type=2, post_type=2,
              scale_type=2, gate_type=2, flags=3, activation=0, scale=1.0, eps=1e-6, x=P, y=P * 2, gate=0, pre=0, post=0,
              scales=0, x_row=64, y_row=64, gate_row=0, residual=P * 3, normed=P * 4, post_rms=0, pre_rms=0, d_res=0,
              d_normed=0, dr_row=0, dn_row=0, d_x=0, d_y=0, d_gate=0, d_pre=0, d_post=0, d_scale=0, workspace=0, bytes=0)
     unknown = set(change) - set(f)
     assert not unknown
-    return block_ops._NORM.pack(*{**f, **change}.values())
+    return NORM.pack(*{**f, **change}.values())
 
 
 def scan_fields(**change):
-    f = dict(size=block_ops._SCAN.size, batch=2, length=10, dim=64, sequences=0, data=1, reserved=0, exponent=8.0, x=P,
+    f = dict(size=SCAN.size, batch=2, length=10, dim=64, sequences=0, data=1, reserved=0, exponent=8.0, x=P,
              r=P, i=P, xb=640, xt=64, rb=640, rt=64, ib=640, it=64, decay=P, initial=0, offsets=0, h=2 * P,
              final=3 * P, chunks=0, d_h=0, db=0, dt=0, d_final=0, d_x=0, d_r=0, d_i=0, d_decay=0, d_initial=0,
              workspace=0, bytes=0)
     assert not set(change) - set(f)
-    return block_ops._SCAN.pack(*{**f, **change}.values())
+    return SCAN.pack(*{**f, **change}.values())
 
 
 def step_fields(**change):
-    f = dict(size=block_ops._STEP.size, batch=2, dim=64, pool=2, data=1, reserved=0, exponent=8.0, x=P, r=P, i=P,
+    f = dict(size=STEP.size, batch=2, dim=64, pool=2, data=1, reserved=0, exponent=8.0, x=P, r=P, i=P,
              x_row=64, r_row=64, i_row=64, decay=P, state=P, new_state=P, slots=0, h=P)
     assert not set(change) - set(f)
-    return block_ops._STEP.pack(*{**f, **change}.values())
+    return STEP.pack(*{**f, **change}.values())
 
 
 def refused(lib, name, packed, status, text):
