@@ -7,108 +7,184 @@
 //   u = s r(s) w_pre,   u <- u H_D / sqrt(D) where the next block is rotated
 //
 // Rows are independent.  TPR threads hold a row in registers (EPT values
-// each), so x and y are read once and s and u written once; the two row sums
-// go through warp shuffles and, in rows of several warps, shared memory.  A
-// CTA walks over rows and loads the next one while it works on this one.
+// each, as packed fp32 pairs), so x and y are read once and s and u written
+// once; the two row sums go through warp shuffles and, in rows of several
+// warps, shared memory.  A CTA walks over rows and loads the next one while it
+// works on this one; what depends on the channel alone is formed once.
 #pragma once
 
 #include "block_ops.hpp"
 #include "common.cuh"
+#include "f32x2.cuh"
 
 namespace cubf::norm {
 
-// ---- memory access: VW consecutive values -----------------------------------------------------
-// Values of a row as loaded, kept packed until they are used.
-template <typename T, int VW>
-struct Piece {
-    static constexpr int kWords = VW * static_cast<int>(sizeof(T)) / 4 > 0 ? VW * static_cast<int>(sizeof(T)) / 4 : 1;
+using f32x2::add2;
+using f32x2::fma2;
+using f32x2::mul2;
+using f32x2::sub2;
+using Pair = f32x2::P;
+
+CUBF_DEV Pair both(float v) { return f32x2::pk(v, v); }
+CUBF_DEV float2 floats(Pair p) {
+    float2 f;
+    f32x2::up(p, f.x, f.y);
+    return f;
+}
+CUBF_DEV float sum_of(Pair p) {
+    const float2 f = floats(p);
+    return f.x + f.y;
+}
+
+// ---- memory access ----------------------------------------------------------------------------
+// Thread j of a row holds chunks c = 0 .. C - 1 of VW consecutive values:
+// value (c, e) is element (c TPR + j) VW + e of the row, and register c VW + e.
+template <int TPR_, int EPT_, int VW_, int THREADS_ = 0>
+struct Shape {
+    static constexpr int TPR = TPR_, EPT = EPT_, VW = VW_, C = EPT / VW, HALF = EPT / 2;
+    static constexpr int kThreads = THREADS_ > 0 ? THREADS_ : TPR == 32 ? 128 : TPR;
+    static constexpr int kRows = kThreads / TPR;    // rows a CTA works on at a time
+    static constexpr int kWarps = TPR / 32;
+    static_assert(C * VW == EPT && TPR >= 32 && EPT >= 2 && kRows <= 15, "whole chunks over whole warps");
+    static CUBF_DEV int at(int c, int j) { return (c * TPR + j) * VW; }
+};
+
+// A row as loaded: EPT values, packed.  Values past the end of the row are zero.
+template <typename T, typename S>
+struct Values {
+    static constexpr int kWords = S::EPT * static_cast<int>(sizeof(T)) / 4;
+    static constexpr int kPer = S::VW * static_cast<int>(sizeof(T)) / 4;  // words of a chunk (VW > 1)
     uint32_t w[kWords];
 
     CUBF_DEV void clear() {
 #pragma unroll
         for (int k = 0; k < kWords; ++k) w[k] = 0;
     }
-    CUBF_DEV void load(const T* p) {
-        if constexpr (VW == 1 && sizeof(T) == 2) {
-            w[0] = __ldcs(reinterpret_cast<const unsigned short*>(p));
-        } else if constexpr (VW == 1) {
-            w[0] = __ldcs(reinterpret_cast<const unsigned int*>(p));
+    template <bool STREAM = true>
+    CUBF_DEV void load(const T* row, int j, int dim) {
+        if constexpr (S::VW == 1) {
+            clear();
+#pragma unroll
+            for (int c = 0; c < S::EPT; ++c)
+                if (S::at(c, j) < dim) {
+                    if constexpr (sizeof(T) == 2) {
+                        const uint32_t h = __ldcs(reinterpret_cast<const unsigned short*>(row + S::at(c, j)));
+                        w[c / 2] |= h << (16 * (c & 1));
+                    } else {
+                        w[c] = __ldcs(reinterpret_cast<const unsigned int*>(row + S::at(c, j)));
+                    }
+                }
         } else {
 #pragma unroll
-            for (int k = 0; k < kWords / 4; ++k) {
-                const uint4 q = __ldcs(reinterpret_cast<const uint4*>(p) + k);
-                w[4 * k] = q.x;
-                w[4 * k + 1] = q.y;
-                w[4 * k + 2] = q.z;
-                w[4 * k + 3] = q.w;
+            for (int c = 0; c < S::C; ++c) {
+                const bool in = S::at(c, j) < dim;
+                const uint4* p = reinterpret_cast<const uint4*>(row + S::at(c, j));
+#pragma unroll
+                for (int k = 0; k < kPer / 4; ++k) {
+                    uint4 q = make_uint4(0, 0, 0, 0);
+                    if (in) q = STREAM ? __ldcs(p + k) : __ldg(p + k);
+                    w[c * kPer + 4 * k] = q.x;
+                    w[c * kPer + 4 * k + 1] = q.y;
+                    w[c * kPer + 4 * k + 2] = q.z;
+                    w[c * kPer + 4 * k + 3] = q.w;
+                }
             }
         }
     }
-    CUBF_DEV float get(int i) const {
+    // registers 2 k and 2 k + 1
+    CUBF_DEV Pair pair(int k) const {
         if constexpr (sizeof(T) == 4) {
-            return __uint_as_float(w[i]);
+            return f32x2::pk(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
+        } else if constexpr (std::is_same<T, __half>::value) {
+            __half2 h;
+            memcpy(&h, &w[k], 4);
+            const float2 f = __half22float2(h);
+            return f32x2::pk(f.x, f.y);
         } else {
-            const unsigned short h = static_cast<unsigned short>(w[i / 2] >> (16 * (i & 1)));
-            T v;
-            memcpy(&v, &h, 2);
-            return Convert<T, float>::load(v);
+            return f32x2::pk(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
         }
     }
 };
 
-template <typename T, int VW>
-CUBF_DEV void store_values(T* p, const float (&v)[VW]) {
-    if constexpr (VW == 1) {
-        p[0] = Convert<T, float>::store(v[0]);
+template <typename T>
+CUBF_DEV uint32_t packed(float lo, float hi) {
+    uint32_t w;
+    if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        memcpy(&w, &h, 4);
     } else {
-        constexpr int kVec = 16 / sizeof(T);
-        static_assert(VW % kVec == 0, "whole 16-byte vectors");
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        memcpy(&w, &h, 4);
+    }
+    return w;
+}
+
+// writes the row held as pairs, each rounded once
+template <typename S, typename T, typename Get>
+CUBF_DEV void store_row(T* row, int j, int dim, Get&& pair) {
 #pragma unroll
-        for (int k = 0; k < VW / kVec; ++k) {
-            Vec16<T> q;
+    for (int c = 0; c < S::C; ++c) {
+        if constexpr (S::VW == 1) {
+            const float2 f = floats(pair(c / 2));
+            if (S::at(c, j) < dim) row[S::at(c, j)] = Convert<T, float>::store(c & 1 ? f.y : f.x);
+        } else {
+            uint32_t w[S::VW * static_cast<int>(sizeof(T)) / 4];
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) q.v[e] = Convert<T, float>::store(v[k * kVec + e]);
-            stg_stream(reinterpret_cast<Vec16<T>*>(p) + k, q);
+            for (int k = 0; k < S::VW / 2; ++k) {
+                const float2 f = floats(pair(c * (S::VW / 2) + k));
+                if constexpr (sizeof(T) == 4) {
+                    w[2 * k] = __float_as_uint(f.x);
+                    w[2 * k + 1] = __float_as_uint(f.y);
+                } else {
+                    w[k] = packed<T>(f.x, f.y);
+                }
+            }
+            if (S::at(c, j) < dim) {
+                uint4* p = reinterpret_cast<uint4*>(row + S::at(c, j));
+#pragma unroll
+                for (int k = 0; k < S::VW * static_cast<int>(sizeof(T)) / 16; ++k)
+                    __stcs(p + k, make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]));
+            }
         }
     }
 }
 
-// VW consecutive values of a per-channel vector (in T, or in fp32), through L1.
-template <typename T, int VW>
-CUBF_DEV void load_vector(const void* base, bool is32, size_t idx, float (&v)[VW]) {
-    if (is32) {
-        const float* p = static_cast<const float*>(base) + idx;
-        if constexpr (VW == 1) {
-            v[0] = __ldg(p);
-        } else {
+// A per-channel vector, in T or in fp32, through L1; `fill` where it is null
+// and past the end of the row.
+template <typename T, typename S>
+CUBF_DEV void load_vector(const void* base, bool is32, int j, int dim, float fill, Pair (&v)[S::HALF]) {
 #pragma unroll
-            for (int k = 0; k < VW / 4; ++k) {
-                const float4 q = __ldg(reinterpret_cast<const float4*>(p) + k);
-                v[4 * k] = q.x;
-                v[4 * k + 1] = q.y;
-                v[4 * k + 2] = q.z;
-                v[4 * k + 3] = q.w;
-            }
+    for (int k = 0; k < S::HALF; ++k) v[k] = both(fill);
+    if (!base) return;
+    if constexpr (S::VW == 1) {
+        float f[S::EPT];
+#pragma unroll
+        for (int c = 0; c < S::EPT; ++c) {
+            f[c] = fill;
+            if (S::at(c, j) < dim)
+                f[c] = is32 || sizeof(T) == 4 ? __ldg(static_cast<const float*>(base) + S::at(c, j))
+                                              : Convert<T, float>::load(static_cast<const T*>(base)[S::at(c, j)]);
         }
-    } else if constexpr (sizeof(T) == 2) {
-        const T* p = static_cast<const T*>(base) + idx;
-        if constexpr (VW == 1) {
-            v[0] = Convert<T, float>::load(p[0]);
-        } else {
 #pragma unroll
-            for (int k = 0; k < VW / 8; ++k) {
-                Vec16<T> q;
-                *reinterpret_cast<uint4*>(&q) = __ldg(reinterpret_cast<const uint4*>(p) + k);
+        for (int k = 0; k < S::HALF; ++k) v[k] = f32x2::pk(f[2 * k], f[2 * k + 1]);
+    } else if (is32 || sizeof(T) == 4) {
+        Values<float, S> q;
+        q.template load<false>(static_cast<const float*>(base), j, dim);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[8 * k + e] = Convert<T, float>::load(q.v[e]);
-            }
-        }
+        for (int k = 0; k < S::HALF; ++k)
+            if (S::at(2 * k / S::VW, j) < dim) v[k] = q.pair(k);
+    } else {
+        Values<T, S> q;
+        q.template load<false>(static_cast<const T*>(base), j, dim);
+#pragma unroll
+        for (int k = 0; k < S::HALF; ++k)
+            if (S::at(2 * k / S::VW, j) < dim) v[k] = q.pair(k);
     }
 }
 
 CUBF_DEV float sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
 
-// act(g), and its slope where SLOPE
+// act(g), or its slope where SLOPE
 template <bool SLOPE>
 CUBF_DEV float activation(int act, float g) {
     if (act == 0) return SLOPE ? 1.f : g;
@@ -116,33 +192,40 @@ CUBF_DEV float activation(int act, float g) {
     if (act == 1) return SLOPE ? s * (1.f - s) : s;
     return SLOPE ? s * (1.f + g * (1.f - s)) : g * s;
 }
+template <bool SLOPE>
+CUBF_DEV Pair activation(int act, Pair g) {
+    const float2 f = floats(g);
+    return f32x2::pk(activation<SLOPE>(act, f.x), activation<SLOPE>(act, f.y));
+}
 
-// ---- a row over TPR threads -------------------------------------------------------------------
-// Thread j holds chunks c = 0 .. C - 1 of VW consecutive values: value (c, e)
-// is element (c TPR + j) VW + e of the row.
-template <int TPR_, int EPT_, int VW_>
-struct Shape {
-    static constexpr int TPR = TPR_, EPT = EPT_, VW = VW_, C = EPT / VW;
-    static constexpr int kThreads = TPR == 32 ? 128 : TPR;
-    static constexpr int kRows = kThreads / TPR;    // rows a CTA works on at a time
-    static constexpr int kWarps = TPR / 32 > 0 ? TPR / 32 : 1;
-    static_assert(C * VW == EPT && TPR >= 32, "whole chunks over whole warps");
-};
-
-// Sum over the row's threads, the same in each.  Rows of several warps are
-// alone in their CTA; `slot` (0, 1, ...) names the shared words used, so that
-// sums in turn need one barrier each.
+// ---- a row over its threads -------------------------------------------------------------------
+// Rows of several warps that share a CTA with others meet on a barrier of
+// their own.
 template <typename S>
-CUBF_DEV float row_sum(float v, float* shared, int slot) {
+CUBF_DEV void row_barrier() {
+    if constexpr (S::TPR == 32) {
+        __syncwarp();
+    } else if constexpr (S::kRows == 1) {
+        __syncthreads();
+    } else {
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + static_cast<int>(threadIdx.x) / S::TPR), "n"(S::TPR) : "memory");
+    }
+}
+
+// Sum over the row's threads, the same in each.  `words` is the row's own
+// shared memory; `slot` (0, 1, ...) picks the words used, so that sums in turn
+// need one barrier each.
+template <typename S>
+CUBF_DEV float row_sum(float v, float* words, int slot) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     if constexpr (S::kWarps > 1) {
-        float* words = shared + slot * S::kWarps;
-        if ((threadIdx.x & 31) == 0) words[threadIdx.x >> 5] = v;
-        __syncthreads();
+        float* w = words + slot * S::kWarps;
+        if ((threadIdx.x & 31) == 0) w[threadIdx.x % S::TPR / 32] = v;
+        row_barrier<S>();
         v = 0.f;
 #pragma unroll
-        for (int k = 0; k < S::kWarps; ++k) v += words[k];
+        for (int k = 0; k < S::kWarps; ++k) v += w[k];
     }
     return v;
 }
@@ -154,9 +237,14 @@ constexpr int log2_of(int n) { return n <= 1 ? 0 : 1 + log2_of(n / 2); }
 // thread number.  Butterflies run over the register bits; then the row is
 // written to shared memory and read back with other bits in registers, until
 // every bit has had its turn, and at the end back in the layout of the loads.
-// Words are swizzled (the 16-byte group index is XORed with the index bits
-// above it), and the thread bits are ordered so that the 32 lanes fall into
-// different banks.
+// Four words of padding after every 2^5, 2^8 and 2^11 keep 16-byte accesses
+// aligned and, with the thread bits ordered so that the 32 lanes fall into
+// different banks, every access without conflicts; being linear in disjoint
+// index bits, the padded address is a sum of what the thread and what the
+// register contributes, so registers differ by immediate offsets.
+CUBF_DEV constexpr uint32_t padded(uint32_t w) { return w + ((w >> 5) << 2) + ((w >> 8) << 2) + ((w >> 11) << 2); }
+constexpr int padded_row(int dim) { return static_cast<int>(padded(static_cast<uint32_t>(dim))); }
+
 struct Layout {
     uint32_t regs;      // index bits held in registers, ascending
     int order[16];      // index bit of each thread bit
@@ -206,29 +294,38 @@ constexpr uint32_t pass_work(int k) {
     for (int i = 0; i < k; ++i) done |= pass_bits<LOGD, LOGE, VB>(i);
     return pass_bits<LOGD, LOGE, VB>(k) & ~done;
 }
-CUBF_DEV uint32_t swizzle(uint32_t w) { return w ^ ((((w >> 5) ^ (w >> 8) ^ (w >> 11)) & 7u) << 2); }
 
+// E registers as E / 2 pairs; register bit 0 lies inside a pair.
 template <int E, uint32_t REGS, uint32_t WORK>
-CUBF_DEV void butterflies(float (&v)[E]) {
+CUBF_DEV void butterflies(Pair (&v)[E / 2]) {
     int bit = 0;
 #pragma unroll
     for (int p = 0; p < 16; ++p) {
         if (!((REGS >> p) & 1u)) continue;
         if ((WORK >> p) & 1u) {
+            if (bit == 0) {
 #pragma unroll
-            for (int r = 0; r < E; ++r)
-                if (!(r & (1 << bit))) {
-                    const float a = v[r], b = v[r | (1 << bit)];
-                    v[r] = a + b;
-                    v[r | (1 << bit)] = a - b;
+                for (int k = 0; k < E / 2; ++k) {
+                    const float2 f = floats(v[k]);
+                    v[k] = f32x2::pk(f.x + f.y, f.x - f.y);
                 }
+            } else {
+                const int step = 1 << (bit - 1);
+#pragma unroll
+                for (int k = 0; k < E / 2; ++k)
+                    if (!(k & step)) {
+                        const Pair a = v[k], b = v[k | step];
+                        v[k] = add2(a, b);
+                        v[k | step] = sub2(a, b);
+                    }
+            }
         }
         ++bit;
     }
 }
 
 template <int LOGD, int LOGE, int VB, int K, bool WRITE>
-CUBF_DEV void move_row(float (&v)[1 << LOGE], float* row, int j) {
+CUBF_DEV void move_row(Pair (&v)[1 << LOGE >> 1], float* row, int j) {
     constexpr int E = 1 << LOGE;
     constexpr uint32_t regs = pass_bits<LOGD, LOGE, VB>(K);
     constexpr Layout l = make_layout<LOGD, LOGE>(regs, K == 0);
@@ -236,190 +333,185 @@ CUBF_DEV void move_row(float (&v)[1 << LOGE], float* row, int j) {
     uint32_t base = 0;
 #pragma unroll
     for (int k = 0; k < LOGD - LOGE; ++k) base |= ((static_cast<uint32_t>(j) >> k) & 1u) << l.order[k];
-    // the swizzle is linear over XOR, and base and at[] share no bits
-    const uint32_t sb = swizzle(base);
+    float* const mine = row + padded(base);
     if constexpr (K == 0 && VB >= 2) {
 #pragma unroll
         for (int r = 0; r < E; r += 4) {
-            float4* q = reinterpret_cast<float4*>(row + (sb ^ swizzle(at.v[r])));
+            float4* q = reinterpret_cast<float4*>(mine + padded(at.v[r]));
             if (WRITE) {
-                *q = make_float4(v[r], v[r + 1], v[r + 2], v[r + 3]);
+                const float2 a = floats(v[r / 2]), b = floats(v[r / 2 + 1]);
+                *q = make_float4(a.x, a.y, b.x, b.y);
             } else {
                 const float4 f = *q;
-                v[r] = f.x;
-                v[r + 1] = f.y;
-                v[r + 2] = f.z;
-                v[r + 3] = f.w;
+                v[r / 2] = f32x2::pk(f.x, f.y);
+                v[r / 2 + 1] = f32x2::pk(f.z, f.w);
             }
         }
     } else {
 #pragma unroll
-        for (int r = 0; r < E; ++r) {
-            float* q = row + (sb ^ swizzle(at.v[r]));
-            if (WRITE)
-                *q = v[r];
-            else
-                v[r] = *q;
+        for (int r = 0; r < E; r += 2) {
+            float* const a = mine + padded(at.v[r]);
+            float* const b = mine + padded(at.v[r + 1]);
+            if (WRITE) {
+                const float2 f = floats(v[r / 2]);
+                *a = f.x;
+                *b = f.y;
+            } else {
+                v[r / 2] = f32x2::pk(*a, *b);
+            }
         }
     }
 }
 
-template <int TPR>
-CUBF_DEV void row_barrier() {
-    if constexpr (TPR > 32)
-        __syncthreads();
-    else
-        __syncwarp();
-}
-
-template <int LOGD, int LOGE, int VB, int TPR, int K>
-CUBF_DEV void rotate_passes(float (&v)[1 << LOGE], float* row, int j) {
+template <typename S, int K>
+CUBF_DEV void rotate_passes(Pair (&v)[S::HALF], float* row, int j) {
+    constexpr int LOGE = log2_of(S::EPT), LOGD = log2_of(S::TPR * S::EPT), VB = log2_of(S::VW);
     constexpr int kPasses = 1 + (LOGD - LOGE + LOGE - 1) / LOGE;
-    butterflies<(1 << LOGE), pass_bits<LOGD, LOGE, VB>(K), pass_work<LOGD, LOGE, VB>(K)>(v);
+    butterflies<S::EPT, pass_bits<LOGD, LOGE, VB>(K), pass_work<LOGD, LOGE, VB>(K)>(v);
     if constexpr (kPasses > 1) {
         constexpr int next = K + 1 < kPasses ? K + 1 : 0;
-        if constexpr (K > 0) row_barrier<TPR>();  // everyone has read the pass before
+        if constexpr (K > 0) row_barrier<S>();  // everyone has read the pass before
         move_row<LOGD, LOGE, VB, K, true>(v, row, j);
-        row_barrier<TPR>();
+        row_barrier<S>();
         move_row<LOGD, LOGE, VB, next, false>(v, row, j);
-        if constexpr (next > 0) rotate_passes<LOGD, LOGE, VB, TPR, next>(v, row, j);
+        if constexpr (next > 0) rotate_passes<S, next>(v, row, j);
     }
 }
 
-// v <- v H_D (unscaled); D = TPR EPT.  `row` holds D floats.
+// v <- v H_D (unscaled); D = TPR EPT.  `row` holds padded_row(D) floats.  The
+// caller passes a row barrier (a row sum's, say) before the next rotation.
 template <typename S>
-CUBF_DEV void rotate_row(float (&v)[S::EPT], float* row, int j) {
-    constexpr int loge = log2_of(S::EPT), logd = log2_of(S::TPR * S::EPT);
-    rotate_passes<logd, loge, log2_of(S::VW), S::TPR, 0>(v, row, j);
-    row_barrier<S::TPR>();  // the next row may write
+CUBF_DEV void rotate_row(Pair (&v)[S::HALF], float* row, int j) {
+    rotate_passes<S, 0>(v, row, j);
 }
 
 // ---- forward ----------------------------------------------------------------------------------
-template <typename T, typename R, typename S, bool ROTATE>
-struct Forward {
-    static constexpr int C = S::C, VW = S::VW;
-
-    struct Row {
-        Piece<R, VW> x[C];
-        Piece<T, VW> y[C], g[C];
-    };
-
-    static CUBF_DEV void load(const BlockNormArgs& p, size_t row, int j, Row& in) {
-        const R* x = static_cast<const R*>(p.x) + row * p.x_row;
-        const T* y = static_cast<const T*>(p.y) + row * p.y_row;
-        const T* g = static_cast<const T*>(p.gate) + row * p.gate_row;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int at = (c * S::TPR + j) * VW;
-            in.x[c].clear();
-            in.y[c].clear();
-            in.g[c].clear();
-            if (at < p.dim) {
-                in.x[c].load(x + at);
-                if (p.y) in.y[c].load(y + at);
-                if (p.gate_mode == kGateFull) in.g[c].load(g + at);
-            }
-        }
-    }
-
-    static CUBF_DEV void run(const BlockNormArgs& p, float* shared) {
-        const int j = threadIdx.x % S::TPR, sub = threadIdx.x / S::TPR;
-        float* words = shared + (ROTATE ? S::kRows * S::TPR * S::EPT : 0);
-        float* row_words = shared + sub * S::TPR * S::EPT;
-        const size_t stride = static_cast<size_t>(gridDim.x) * S::kRows;
-        size_t row = static_cast<size_t>(blockIdx.x) * S::kRows + sub;
-        const float inv_dim = 1.f / static_cast<float>(p.dim);
-        Row in;
-        if (row < p.rows) load(p, row, j, in);
-        int slot = 0;
-        for (; row < p.rows; row += stride) {
-            float s[S::EPT];
-            float sum = 0.f;
-#pragma unroll
-            for (int c = 0; c < C; ++c)
-#pragma unroll
-                for (int e = 0; e < VW; ++e) {
-                    const float y = in.y[c].get(e);
-                    s[c * VW + e] = y;
-                    sum = fmaf(y, y, sum);
-                }
-            const Row now = in;
-            if (row + stride < p.rows) load(p, row + stride, j, in);
-            float ry = 1.f;
-            if (p.post_norm) {
-                ry = rsqrtf(row_sum<S>(sum, words, slot) * inv_dim + p.eps);
-                if (p.r_post && j == 0) p.r_post[row] = ry;
-            }
-            slot ^= 1;
-            sum = 0.f;
-            const size_t gate_row = p.gate_mode == kGateGroups ? row / p.rows_per_gate * p.gate_row : 0;
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const int at = (c * S::TPR + j) * VW;
-                const bool in_row = at < p.dim;
-                float w[VW], a[VW];
-#pragma unroll
-                for (int e = 0; e < VW; ++e) w[e] = ry;
-                if (p.post && in_row) {
-                    load_vector<T, VW>(p.post, p.post32, at, w);
-#pragma unroll
-                    for (int e = 0; e < VW; ++e) w[e] *= ry;
-                }
-                if (p.gate_mode == kGateFull) {
-#pragma unroll
-                    for (int e = 0; e < VW; ++e) w[e] *= activation<false>(p.act, now.g[c].get(e));
-                } else if (p.gate_mode != kGateNone && in_row) {
-                    load_vector<T, VW>(p.gate, p.gate32, gate_row + at, a);
-#pragma unroll
-                    for (int e = 0; e < VW; ++e) w[e] *= activation<false>(p.act, a[e]);
-                }
-#pragma unroll
-                for (int e = 0; e < VW; ++e) a[e] = p.scale;
-                if (p.scales && in_row) load_vector<T, VW>(p.scales, p.scales32, at, a);
-                float out[VW];
-#pragma unroll
-                for (int e = 0; e < VW; ++e) {
-                    const float x = a[e] * now.x[c].get(e);
-                    const float v = p.y ? fmaf(w[e], s[c * VW + e], x) : x;
-                    out[e] = v;
-                    s[c * VW + e] = v;
-                    sum = fmaf(v, v, sum);
-                }
-                if (p.residual && in_row) store_values<R, VW>(static_cast<R*>(p.residual) + row * p.dim + at, out);
-            }
-            if (p.normed) {
-                const float rs = rsqrtf(row_sum<S>(sum, words, 2 + slot) * inv_dim + p.eps);
-                if (p.r_pre && j == 0) p.r_pre[row] = rs;
-                const float scale = ROTATE ? rs * p.rotate_scale : rs;
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const int at = (c * S::TPR + j) * VW;
-                    float w[VW];
-#pragma unroll
-                    for (int e = 0; e < VW; ++e) w[e] = 1.f;
-                    if (p.pre && at < p.dim) load_vector<T, VW>(p.pre, p.pre32, at, w);
-#pragma unroll
-                    for (int e = 0; e < VW; ++e) s[c * VW + e] *= scale * w[e];
-                }
-                if constexpr (ROTATE) rotate_row<S>(s, row_words, j);
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const int at = (c * S::TPR + j) * VW;
-                    float out[VW];
-#pragma unroll
-                    for (int e = 0; e < VW; ++e) out[e] = s[c * VW + e];
-                    if (at < p.dim) store_values<T, VW>(static_cast<T*>(p.normed) + row * p.dim + at, out);
-                }
-            }
-        }
-    }
+// Shared memory, in floats: the rotated rows, then the words of the row sums,
+// then (shapes of many values a thread) the channel factors of s and u.
+template <typename S, bool ROTATE>
+struct ForwardPlan {
+    static constexpr int kDim = S::TPR * S::EPT;
+    static constexpr bool kShared = S::EPT > 16;  // factors in shared memory instead of registers
+    // Rows of many values a thread are not loaded ahead: their registers go to
+    // more rows at a time, whose loads overlap each other's work.
+    static constexpr bool kAhead = S::EPT <= 16;
+    static constexpr int kRow = ROTATE ? padded_row(kDim) : 0;
+    static constexpr int kWordsAt = S::kRows * kRow;
+    static constexpr int kFactorsAt = kWordsAt + S::kRows * 4 * S::kWarps;
+    static constexpr int kFloats = kFactorsAt + (kShared ? 2 * kDim : 0);
 };
 
 template <typename T, typename R, typename S, bool ROTATE>
 __global__ void __launch_bounds__(S::kThreads, 1) block_norm_kernel(BlockNormArgs p) {
+    using Plan = ForwardPlan<S, ROTATE>;
     extern __shared__ __align__(16) float shared[];
     pdl_begin();
-    Forward<T, R, S, ROTATE>::run(p, shared);
+    const int j = threadIdx.x % S::TPR, sub = threadIdx.x / S::TPR, dim = p.dim;
+    float* const exchange = shared + sub * Plan::kRow;
+    float* const words = shared + Plan::kWordsAt + sub * 4 * S::kWarps;
+    float2* const factors = reinterpret_cast<float2*>(shared + Plan::kFactorsAt);
+    const size_t stride = static_cast<size_t>(gridDim.x) * S::kRows;
+    size_t row = static_cast<size_t>(blockIdx.x) * S::kRows + sub;
+    const float inv_dim = 1.f / static_cast<float>(dim);
+
+    Values<R, S> x;
+    Values<T, S> y, g;
+    auto load = [&](size_t at) {
+        x.load(static_cast<const R*>(p.x) + at * p.x_row, j, dim);
+        if (p.y) y.load(static_cast<const T*>(p.y) + at * p.y_row, j, dim);
+        if (p.gate_mode == kGateFull) g.load(static_cast<const T*>(p.gate) + at * p.gate_row, j, dim);
+    };
+    y.clear();
+    if (Plan::kAhead && row < p.rows) load(row);
+
+    // What multiplies y r(y) in s (post_weight, and the gate where it is one
+    // per channel) and s r(s) in u.
+    Pair fy[Plan::kShared ? 1 : S::HALF], fu[Plan::kShared ? 1 : S::HALF];
+    {
+        Pair a[S::HALF], b[S::HALF];
+        load_vector<T, S>(p.post, p.post32, j, dim, 1.f, a);
+        if (p.gate_mode == kGateChannel) {
+            load_vector<T, S>(p.gate, p.gate32, j, dim, 0.f, b);
+#pragma unroll
+            for (int k = 0; k < S::HALF; ++k) a[k] = mul2(a[k], activation<false>(p.act, b[k]));
+        }
+        load_vector<T, S>(p.pre, p.pre32, j, dim, 1.f, b);
+#pragma unroll
+        for (int k = 0; k < S::HALF; ++k) {
+            const Pair u = ROTATE ? mul2(b[k], both(p.rotate_scale)) : b[k];
+            if constexpr (Plan::kShared) {
+                if (sub == 0) {
+                    factors[k * S::TPR + j] = floats(a[k]);
+                    factors[(S::HALF + k) * S::TPR + j] = floats(u);
+                }
+            } else {
+                fy[k] = a[k];
+                fu[k] = u;
+            }
+        }
+        if constexpr (Plan::kShared) __syncthreads();
+    }
+    auto factor = [&](int which, int k) {
+        if constexpr (Plan::kShared) {
+            const float2 f = factors[(which * S::HALF + k) * S::TPR + j];
+            return f32x2::pk(f.x, f.y);
+        } else {
+            return which ? fu[k] : fy[k];
+        }
+    };
+
+    for (int slot = 0; row < p.rows; row += stride, slot ^= 1) {
+        if (!Plan::kAhead) load(row);
+        Pair s[S::HALF];
+        Pair sum = both(0.f);
+        float ry = 1.f;
+        if (p.post_norm) {
+#pragma unroll
+            for (int k = 0; k < S::HALF; ++k) sum = fma2(y.pair(k), y.pair(k), sum);
+            ry = rsqrtf(row_sum<S>(sum_of(sum), words, slot) * inv_dim + p.eps);
+            if (p.r_post && j == 0) p.r_post[row] = ry;
+        }
+        if (p.scales) {
+            load_vector<T, S>(p.scales, p.scales32, j, dim, 0.f, s);
+#pragma unroll
+            for (int k = 0; k < S::HALF; ++k) s[k] = mul2(s[k], x.pair(k));
+        } else {
+#pragma unroll
+            for (int k = 0; k < S::HALF; ++k) s[k] = mul2(both(p.scale), x.pair(k));
+        }
+        if (p.y) {
+            if (p.gate_mode == kGateFull) {
+#pragma unroll
+                for (int k = 0; k < S::HALF; ++k)
+                    s[k] = fma2(mul2(mul2(factor(0, k), both(ry)), activation<false>(p.act, g.pair(k))), y.pair(k), s[k]);
+            } else if (p.gate_mode == kGateGroups) {
+                Pair a[S::HALF];
+                const size_t at = row / p.rows_per_gate * p.gate_row;
+                load_vector<T, S>(p.gate32 ? static_cast<const void*>(static_cast<const float*>(p.gate) + at)
+                                           : static_cast<const void*>(static_cast<const T*>(p.gate) + at),
+                                  p.gate32, j, dim, 0.f, a);
+#pragma unroll
+                for (int k = 0; k < S::HALF; ++k)
+                    s[k] = fma2(mul2(mul2(factor(0, k), both(ry)), activation<false>(p.act, a[k])), y.pair(k), s[k]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < S::HALF; ++k) s[k] = fma2(mul2(factor(0, k), both(ry)), y.pair(k), s[k]);
+            }
+        }
+        if (Plan::kAhead && row + stride < p.rows) load(row + stride);
+        if (p.residual)
+            store_row<S>(static_cast<R*>(p.residual) + row * dim, j, dim, [&](int k) { return s[k]; });
+        if (!p.normed) continue;
+        sum = both(0.f);
+#pragma unroll
+        for (int k = 0; k < S::HALF; ++k) sum = fma2(s[k], s[k], sum);
+        const float rs = rsqrtf(row_sum<S>(sum_of(sum), words, 2 + slot) * inv_dim + p.eps);
+        if (p.r_pre && j == 0) p.r_pre[row] = rs;
+#pragma unroll
+        for (int k = 0; k < S::HALF; ++k) s[k] = mul2(s[k], mul2(factor(1, k), both(rs)));
+        if constexpr (ROTATE) rotate_row<S>(s, exchange, j);
+        store_row<S>(static_cast<T*>(p.normed) + row * dim, j, dim, [&](int k) { return s[k]; });
+    }
 }
 
 // ---- backward ---------------------------------------------------------------------------------
@@ -429,219 +521,252 @@ __global__ void __launch_bounds__(S::kThreads, 1) block_norm_kernel(BlockNormArg
 //   dn = act(gate) dS            dalpha   = sum dS x         (Z)
 //   t' = dn w_post               dy = r(y) (t' - yn mean(t' yn))
 //   dgate = act'(gate) dS n      dw_post  = sum dn yn
-// The sums over rows stay in registers: a thread owns its columns for every
-// row of its CTA, whose rows share one gate row, so that for a gate per
-// channel or per group dw_post and dgate both follow from P = sum dS yn; with
-// a gate per row P = sum dn yn.  Each CTA writes its sums once and a second
-// kernel adds them in a fixed order.
-template <typename T, typename R, typename S, bool ROTATE>
-struct Backward {
-    static constexpr int C = S::C, VW = S::VW;
+// A thread owns its columns for every row of its CTA, so the sums over rows
+// stay in registers (in shared memory, by the same thread, for shapes of many
+// values a thread; Z, which few calls need, always).  A CTA's rows share one
+// gate row, so that for a gate per channel or per group dw_post and dgate both
+// follow from P = sum dS yn; with a gate per row P = sum dn yn.  Each CTA
+// writes its sums once and a second kernel adds them in a fixed order.
+template <typename S, bool ROTATE>
+struct BackwardPlan {
+    static constexpr int kDim = S::TPR * S::EPT;
+    static constexpr bool kLean = S::EPT * S::kThreads > 4096 || ROTATE;  // no room for the next row in registers
+    static constexpr bool kSharedSums = S::EPT > 8 && !(ROTATE && S::kThreads <= 256);
+    static constexpr int kRow = ROTATE ? padded_row(kDim) : 0;
+    static constexpr int kWordsAt = S::kRows * kRow;
+    static constexpr int kSumsAt = kWordsAt + S::kRows * 4 * S::kWarps;   // Z, then P and Q if shared
+    static constexpr int kFloats = kSumsAt + S::kRows * kDim * (kSharedSums ? 3 : 1);
+};
 
-    // t - vn mean(t vn), the part of t that a norm lets through.  In a row of
-    // one value vn^2 = 1 - eps r^2, and the difference would cancel.
-    static CUBF_DEV float through_norm(const BlockNormArgs& p, float t, float vn, float mean, float r) {
-        return p.dim == 1 ? t * p.eps * r * r : t - vn * mean;
-    }
+// t - vn mean(t vn), the part of t that a norm lets through.  In a row of one
+// value vn^2 = 1 - eps r^2, and the difference would cancel.
+CUBF_DEV Pair through_norm(const BlockNormArgs& p, Pair t, Pair vn, float mean, float r) {
+    return p.dim == 1 ? mul2(t, both(p.eps * r * r)) : fma2(vn, both(-mean), t);
+}
+
+template <typename T, typename R, typename S, bool ROTATE>
+__global__ void __launch_bounds__(S::kThreads, S::kThreads <= 256 && ROTATE ? 2 : 1)
+    block_norm_backward_kernel(BlockNormArgs p) {
+    using Plan = BackwardPlan<S, ROTATE>;
+    extern __shared__ __align__(16) float shared[];
+    pdl_begin();
+    const int j = threadIdx.x % S::TPR, sub = threadIdx.x / S::TPR, dim = p.dim;
+    float* const exchange = shared + sub * Plan::kRow;
+    float* const words = shared + Plan::kWordsAt + sub * 4 * S::kWarps;
+    // the thread's own sums: pair k at [k][thread]
+    float2* const mine = reinterpret_cast<float2*>(shared + Plan::kSumsAt) + threadIdx.x;
+    constexpr int kSumStride = S::HALF * S::kThreads;
+    const float inv_dim = 1.f / static_cast<float>(dim);
+    // this CTA's rows: a share of one gate group's
+    const size_t group = blockIdx.x / p.parts_per_group;
+    const size_t share = (p.rows_per_gate + p.parts_per_group - 1) / p.parts_per_group;
+    const size_t from = (blockIdx.x % p.parts_per_group) * share;
+    const size_t to = from + share < p.rows_per_gate ? from + share : p.rows_per_gate;
+    const size_t end = group * p.rows_per_gate + to;
+    size_t row = group * p.rows_per_gate + from + sub;
 
     struct Row {
-        Piece<R, VW> x[C], ds[C];
-        Piece<T, VW> y[C], g[C], du[C];
+        Values<R, S> x, ds;
+        Values<T, S> y, g, du;
         float ry, rs;
     };
+    auto load = [&](size_t at, Row& in) {
+        in.x.load(static_cast<const R*>(p.x) + at * p.x_row, j, dim);
+        if (p.y) in.y.load(static_cast<const T*>(p.y) + at * p.y_row, j, dim);
+        if (p.d_residual) in.ds.load(static_cast<const R*>(p.d_residual) + at * p.d_residual_row, j, dim);
+        if (p.d_normed) in.du.load(static_cast<const T*>(p.d_normed) + at * p.d_normed_row, j, dim);
+        if (p.gate_mode == kGateFull) in.g.load(static_cast<const T*>(p.gate) + at * p.gate_row, j, dim);
+        in.ry = p.post_norm ? p.r_post[at] : 1.f;
+        in.rs = p.d_normed ? p.r_pre[at] : 0.f;
+    };
+    Row in;
+    in.y.clear();
+    in.ds.clear();
+    in.du.clear();
+    in.g.clear();
+    if (row < end) load(row, in);
 
-    static CUBF_DEV void load(const BlockNormArgs& p, size_t row, int j, Row& in) {
-        const R* x = static_cast<const R*>(p.x) + row * p.x_row;
-        const R* ds = static_cast<const R*>(p.d_residual) + row * p.d_residual_row;
-        const T* y = static_cast<const T*>(p.y) + row * p.y_row;
-        const T* du = static_cast<const T*>(p.d_normed) + row * p.d_normed_row;
-        const T* g = static_cast<const T*>(p.gate) + row * p.gate_row;
+    // channel factors: w_post, act(gate) where the CTA's rows share it, and w_pre
+    constexpr bool kKeep = !Plan::kLean;
+    Pair kw[kKeep ? S::HALF : 1], ka[kKeep ? S::HALF : 1], kp[kKeep ? S::HALF : 1];
+    const bool row_gate = p.gate_mode == kGateFull, shared_gate = p.gate_mode == kGateChannel || p.gate_mode == kGateGroups;
+    auto gate_factor = [&](Pair(&a)[S::HALF]) {
+        const size_t at = p.gate_mode == kGateGroups ? group * p.gate_row : 0;
+        load_vector<T, S>(!shared_gate ? nullptr
+                          : p.gate32   ? static_cast<const void*>(static_cast<const float*>(p.gate) + at)
+                                       : static_cast<const void*>(static_cast<const T*>(p.gate) + at),
+                          p.gate32, j, dim, 1.f, a);
+        if (shared_gate) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int at = (c * S::TPR + j) * VW;
-            in.x[c].clear();
-            in.y[c].clear();
-            in.ds[c].clear();
-            in.du[c].clear();
-            in.g[c].clear();
-            if (at < p.dim) {
-                in.x[c].load(x + at);
-                if (p.y) in.y[c].load(y + at);
-                if (p.d_residual) in.ds[c].load(ds + at);
-                if (p.d_normed) in.du[c].load(du + at);
-                if (p.gate_mode == kGateFull) in.g[c].load(g + at);
-            }
+            for (int k = 0; k < S::HALF; ++k) a[k] = activation<false>(p.act, a[k]);
         }
-        in.ry = p.post_norm ? p.r_post[row] : 1.f;
-        in.rs = p.d_normed ? p.r_pre[row] : 0.f;
+    };
+    if constexpr (kKeep) {
+        load_vector<T, S>(p.post, p.post32, j, dim, 1.f, kw);
+        gate_factor(ka);
+        load_vector<T, S>(p.pre, p.pre32, j, dim, 1.f, kp);
     }
+    Pair P[Plan::kSharedSums ? 1 : S::HALF], Q[Plan::kSharedSums ? 1 : S::HALF];
+#pragma unroll
+    for (int k = 0; k < (Plan::kSharedSums ? 1 : S::HALF); ++k) P[k] = Q[k] = both(0.f);
+#pragma unroll
+    for (int k = 0; k < S::HALF * (Plan::kSharedSums ? 3 : 1); ++k) mine[k * S::kThreads] = make_float2(0.f, 0.f);
+    auto add_sum = [&](Pair* regs, int which, int k, Pair a, Pair b) {  // += a b
+        if (!Plan::kSharedSums && which > 0) {
+            regs[k] = fma2(a, b, regs[k]);
+        } else {
+            float2* at = mine + which * kSumStride + k * S::kThreads;
+            const float2 f = *at;
+            *at = floats(fma2(a, b, f32x2::pk(f.x, f.y)));
+        }
+    };
 
-    static CUBF_DEV void run(const BlockNormArgs& p, float* shared) {
-        const int j = threadIdx.x % S::TPR, sub = threadIdx.x / S::TPR;
-        float* words = shared + (ROTATE ? S::kRows * S::TPR * S::EPT : 0);
-        float* row_words = shared + sub * S::TPR * S::EPT;
-        const float inv_dim = 1.f / static_cast<float>(p.dim);
-        // this CTA's rows: a share of one gate group's
-        const size_t group = blockIdx.x / p.parts_per_group;
-        const size_t share = (p.rows_per_gate + p.parts_per_group - 1) / p.parts_per_group;
-        const size_t from = (blockIdx.x % p.parts_per_group) * share;
-        const size_t to = from + share < p.rows_per_gate ? from + share : p.rows_per_gate;
-        const size_t end = group * p.rows_per_gate + to;
-        size_t row = group * p.rows_per_gate + from + sub;
-        const size_t gate_row = p.gate_mode == kGateGroups ? group * p.gate_row : 0;
-        float P[S::EPT], Q[S::EPT], Z[S::EPT];
+    for (int slot = 0; row < end; row += S::kRows, slot ^= 1) {
+        Row ahead;
+        if constexpr (!Plan::kLean) {
+            ahead = in;
+            if (row + S::kRows < end) load(row + S::kRows, ahead);
+        }
+        Pair d[S::HALF];   // du, t, then t'
+        Pair sn[S::HALF];  // s r(s)
+        float dot = 0.f;
+        if (p.d_normed) {
 #pragma unroll
-        for (int k = 0; k < S::EPT; ++k) P[k] = Q[k] = Z[k] = 0.f;
-        Row in;
-        if (row < end) load(p, row, j, in);
-        int slot = 0;
-        for (; row < end; row += S::kRows) {
-            const Row now = in;
-            if (row + S::kRows < end) load(p, row + S::kRows, j, in);
-            float d[S::EPT];   // du, then dS
-            float n[S::EPT];   // act(gate) w_post, the factor of yn in s
-            if (p.d_normed) {
+            for (int k = 0; k < S::HALF; ++k) d[k] = in.du.pair(k);
+            if constexpr (ROTATE) {
+                rotate_row<S>(d, exchange, j);
 #pragma unroll
-                for (int c = 0; c < C; ++c)
+                for (int k = 0; k < S::HALF; ++k) d[k] = mul2(d[k], both(p.rotate_scale));
+            }
+            if (p.scales) {
+                load_vector<T, S>(p.scales, p.scales32, j, dim, 0.f, sn);
 #pragma unroll
-                    for (int e = 0; e < VW; ++e) d[c * VW + e] = now.du[c].get(e);
-                if constexpr (ROTATE) {
-                    rotate_row<S>(d, row_words, j);
+                for (int k = 0; k < S::HALF; ++k) sn[k] = mul2(sn[k], in.x.pair(k));
+            } else {
 #pragma unroll
-                    for (int k = 0; k < S::EPT; ++k) d[k] *= p.rotate_scale;
+                for (int k = 0; k < S::HALF; ++k) sn[k] = mul2(both(p.scale), in.x.pair(k));
+            }
+            if (p.y) {
+                Pair lw[kKeep ? 1 : S::HALF], la[kKeep ? 1 : S::HALF];
+                if constexpr (!kKeep) {
+                    load_vector<T, S>(p.post, p.post32, j, dim, 1.f, lw);
+                    gate_factor(la);
+                }
+#pragma unroll
+                for (int k = 0; k < S::HALF; ++k) {
+                    Pair f = kKeep ? kw[k] : lw[k];
+                    f = mul2(f, row_gate ? activation<false>(p.act, in.g.pair(k)) : kKeep ? ka[k] : la[k]);
+                    sn[k] = fma2(mul2(f, both(in.ry)), in.y.pair(k), sn[k]);
+                }
+            }
+            {
+                Pair lp[kKeep ? 1 : S::HALF];
+                if constexpr (!kKeep) load_vector<T, S>(p.pre, p.pre32, j, dim, 1.f, lp);
+                Pair sum = both(0.f);
+#pragma unroll
+                for (int k = 0; k < S::HALF; ++k) {
+                    sn[k] = mul2(sn[k], both(in.rs));
+                    if (p.need_q) add_sum(Q, 2, k, d[k], sn[k]);
+                    d[k] = mul2(d[k], kKeep ? kp[k] : lp[k]);
+                    sum = fma2(d[k], sn[k], sum);
+                }
+                dot = row_sum<S>(sum_of(sum), words, slot) * inv_dim;
+            }
+            // dS
+#pragma unroll
+            for (int k = 0; k < S::HALF; ++k)
+                d[k] = fma2(through_norm(p, d[k], sn[k], dot, in.rs), both(in.rs), in.ds.pair(k));
+        } else {
+#pragma unroll
+            for (int k = 0; k < S::HALF; ++k) d[k] = in.ds.pair(k);
+        }
+        {
+            if (p.scales) {
+                load_vector<T, S>(p.scales, p.scales32, j, dim, 0.f, sn);
+#pragma unroll
+                for (int k = 0; k < S::HALF; ++k) {
+                    add_sum(nullptr, 0, k, d[k], in.x.pair(k));
+                    sn[k] = mul2(sn[k], d[k]);
                 }
             } else {
 #pragma unroll
-                for (int k = 0; k < S::EPT; ++k) d[k] = 0.f;
+                for (int k = 0; k < S::HALF; ++k) sn[k] = mul2(both(p.scale), d[k]);
             }
-            float dot = 0.f;
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const int at = (c * S::TPR + j) * VW;
-                const bool in_row = at < p.dim;
-                float w[VW], a[VW], al[VW];
-#pragma unroll
-                for (int e = 0; e < VW; ++e) {
-                    w[e] = a[e] = 1.f;
-                    al[e] = p.scale;
-                }
-                if (p.post && in_row) load_vector<T, VW>(p.post, p.post32, at, w);
-                if (p.gate_mode == kGateFull) {
-#pragma unroll
-                    for (int e = 0; e < VW; ++e) a[e] = activation<false>(p.act, now.g[c].get(e));
-                } else if (p.gate_mode != kGateNone && in_row) {
-                    load_vector<T, VW>(p.gate, p.gate32, gate_row + at, a);
-#pragma unroll
-                    for (int e = 0; e < VW; ++e) a[e] = activation<false>(p.act, a[e]);
-                }
-                if (p.scales && in_row) load_vector<T, VW>(p.scales, p.scales32, at, al);
-#pragma unroll
-                for (int e = 0; e < VW; ++e) n[c * VW + e] = a[e];
-                if (p.d_normed) {
-                    float wp[VW];
-#pragma unroll
-                    for (int e = 0; e < VW; ++e) wp[e] = 1.f;
-                    if (p.pre && in_row) load_vector<T, VW>(p.pre, p.pre32, at, wp);
-#pragma unroll
-                    for (int e = 0; e < VW; ++e) {
-                        const int k = c * VW + e;
-                        float s = al[e] * now.x[c].get(e);
-                        if (p.y) s = fmaf(a[e] * w[e], now.y[c].get(e) * now.ry, s);
-                        const float sn = s * now.rs;
-                        Q[k] = fmaf(d[k], sn, Q[k]);
-                        d[k] *= wp[e];
-                        dot = fmaf(d[k], sn, dot);
-                    }
-                }
-            }
-            if (p.d_normed) dot = row_sum<S>(dot, words, slot) * inv_dim;
-            float dot2 = 0.f;
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const int at = (c * S::TPR + j) * VW;
-                const bool in_row = at < p.dim;
-                float w[VW], al[VW], out[VW], dg[VW];
-#pragma unroll
-                for (int e = 0; e < VW; ++e) {
-                    w[e] = 1.f;
-                    al[e] = p.scale;
-                }
-                if (p.post && in_row) load_vector<T, VW>(p.post, p.post32, at, w);
-                if (p.scales && in_row) load_vector<T, VW>(p.scales, p.scales32, at, al);
-#pragma unroll
-                for (int e = 0; e < VW; ++e) {
-                    const int k = c * VW + e;
-                    const float x = now.x[c].get(e), yn = now.y[c].get(e) * now.ry;
-                    float dS = now.ds[c].get(e);
-                    if (p.d_normed) {
-                        float s = al[e] * x;
-                        if (p.y) s = fmaf(n[k] * w[e], yn, s);
-                        dS = fmaf(now.rs, through_norm(p, d[k], s * now.rs, dot, now.rs), dS);
-                    }
-                    out[e] = al[e] * dS;
-                    if (p.scales) Z[k] = fmaf(dS, x, Z[k]);
-                    const float dn = n[k] * dS;
-                    P[k] = fmaf(p.gate_mode == kGateFull ? dn : dS, yn, P[k]);
-                    if (p.gate_mode == kGateFull)
-                        dg[e] = dS * yn * w[e] * activation<true>(p.act, now.g[c].get(e));
-                    d[k] = dn * w[e];
-                    dot2 = fmaf(d[k], yn, dot2);
-                }
-                if (in_row) {
-                    store_values<R, VW>(static_cast<R*>(p.d_x) + row * p.dim + at, out);
-                    if (p.gate_mode == kGateFull)
-                        store_values<T, VW>(static_cast<T*>(p.d_gate) + row * p.dim + at, dg);
-                }
-            }
-            if (p.y) {
-                if (p.post_norm) dot2 = row_sum<S>(dot2, words, 2 + slot) * inv_dim;
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    const int at = (c * S::TPR + j) * VW;
-                    float out[VW];
-#pragma unroll
-                    for (int e = 0; e < VW; ++e) {
-                        const float yn = now.y[c].get(e) * now.ry;
-                        out[e] = p.post_norm ? now.ry * through_norm(p, d[c * VW + e], yn, dot2, now.ry) : d[c * VW + e];
-                    }
-                    if (at < p.dim) store_values<T, VW>(static_cast<T*>(p.d_y) + row * p.dim + at, out);
-                }
-            }
-            slot ^= 1;
+            store_row<S>(static_cast<R*>(p.d_x) + row * dim, j, dim, [&](int k) { return sn[k]; });
         }
-        // the CTA's sums; rows side by side in a CTA are added first
-        float* part = p.partials + static_cast<size_t>(blockIdx.x) * 3 * p.dim;
-        auto write = [&](float (&v)[S::EPT], float* dst) {
-            if constexpr (S::kRows > 1) {
-                __syncthreads();
-#pragma unroll
-                for (int k = 0; k < S::EPT; ++k) shared[(sub * S::EPT + k) * S::TPR + j] = v[k];
-                __syncthreads();
-                if (sub > 0) return;
-#pragma unroll
-                for (int k = 0; k < S::EPT; ++k)
-                    for (int o = 1; o < S::kRows; ++o) v[k] += shared[(o * S::EPT + k) * S::TPR + j];
+        if (p.y) {
+            Pair lw[kKeep ? 1 : S::HALF], la[kKeep ? 1 : S::HALF];
+            if constexpr (!kKeep) {
+                load_vector<T, S>(p.post, p.post32, j, dim, 1.f, lw);
+                gate_factor(la);
             }
+            Pair sum = both(0.f);
+            if (row_gate) {
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const int at = (c * S::TPR + j) * VW;
-                float out[VW];
+                for (int k = 0; k < S::HALF; ++k) {
+                    const Pair w = kKeep ? kw[k] : lw[k], g = in.g.pair(k);
+                    const Pair yn = mul2(in.y.pair(k), both(in.ry));
+                    sn[k] = mul2(mul2(mul2(d[k], yn), w), activation<true>(p.act, g));  // dgate
+                    d[k] = mul2(d[k], activation<false>(p.act, g));                       // dn
+                    if (p.need_p) add_sum(P, 1, k, d[k], yn);
+                    d[k] = mul2(d[k], w);
+                    sum = fma2(d[k], yn, sum);
+                }
+                store_row<S>(static_cast<T*>(p.d_gate) + row * dim, j, dim, [&](int k) { return sn[k]; });
+            } else {
 #pragma unroll
-                for (int e = 0; e < VW; ++e) out[e] = v[c * VW + e];
-                if (at < p.dim) store_values<float, VW>(dst + at, out);
+                for (int k = 0; k < S::HALF; ++k) {
+                    const Pair yn = mul2(in.y.pair(k), both(in.ry));
+                    if (p.need_p) add_sum(P, 1, k, d[k], yn);
+                    d[k] = mul2(d[k], mul2(kKeep ? kw[k] : lw[k], kKeep ? ka[k] : la[k]));
+                    sum = fma2(d[k], yn, sum);
+                }
             }
-        };
-        if (p.need_p) write(P, part);
-        if (p.need_q) write(Q, part + p.dim);
-        if (p.need_z) write(Z, part + 2 * static_cast<size_t>(p.dim));
+            if (p.post_norm) {
+                const float mean = row_sum<S>(sum_of(sum), words, 2 + slot) * inv_dim;
+#pragma unroll
+                for (int k = 0; k < S::HALF; ++k)
+                    d[k] = mul2(through_norm(p, d[k], mul2(in.y.pair(k), both(in.ry)), mean, in.ry), both(in.ry));
+            }
+            store_row<S>(static_cast<T*>(p.d_y) + row * dim, j, dim, [&](int k) { return d[k]; });
+        }
+        if constexpr (Plan::kLean) {
+            if (row + S::kRows < end) load(row + S::kRows, in);
+        } else {
+            in = ahead;
+        }
     }
-};
-
-template <typename T, typename R, typename S, bool ROTATE>
-__global__ void __launch_bounds__(S::kThreads, 1) block_norm_backward_kernel(BlockNormArgs p) {
-    extern __shared__ __align__(16) float shared[];
-    pdl_begin();
-    Backward<T, R, S, ROTATE>::run(p, shared);
+    // The CTA's sums; rows side by side in a CTA are added first, in shared memory.
+    float* const part = p.partials + static_cast<size_t>(blockIdx.x) * 3 * dim;
+    auto write = [&](Pair* regs, int which, float* dst) {
+        float2* const at = mine + (Plan::kSharedSums ? which : 0) * kSumStride;
+        if (!Plan::kSharedSums && which > 0 && S::kRows > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < S::HALF; ++k) at[k * S::kThreads] = floats(regs[k]);
+        }
+        if constexpr (S::kRows > 1) {
+            __syncthreads();
+            if (sub > 0) return;
+        }
+        Pair v[S::HALF];
+#pragma unroll
+        for (int k = 0; k < S::HALF; ++k) {
+            if (!Plan::kSharedSums && which > 0 && S::kRows == 1) {
+                v[k] = regs[k];
+            } else {
+                v[k] = both(0.f);
+                for (int o = 0; o < S::kRows; ++o) {
+                    const float2 f = at[k * S::kThreads + o * S::TPR];
+                    v[k] = add2(v[k], f32x2::pk(f.x, f.y));
+                }
+            }
+        }
+        store_row<S>(dst, j, dim, [&](int k) { return v[k]; });
+    };
+    if (p.need_z) write(nullptr, 0, part + 2 * static_cast<size_t>(dim));
+    if (p.need_p) write(P, 1, part);
+    if (p.need_q) write(Q, 2, part + dim);
 }
 
 // The gradients of the per-channel vectors from the CTAs' sums: 32 columns
@@ -660,9 +785,8 @@ __global__ void __launch_bounds__(1024) block_norm_sums_kernel(BlockNormArgs p, 
     const int first = what > 2 ? static_cast<int>(what - 3) * p.parts_per_group : 0;
     const int last = what > 2 ? first + p.parts_per_group : parts;
     auto vector_at = [&](const void* v, bool is32, size_t at) {
-        float f[1];
-        load_vector<T, 1>(v, is32 || sizeof(T) == 4, at, f);
-        return f[0];
+        return is32 || sizeof(T) == 4 ? static_cast<const float*>(v)[at]
+                                      : Convert<T, float>::load(static_cast<const T*>(v)[at]);
     };
     float sum = 0.f;
     if (col < p.dim)

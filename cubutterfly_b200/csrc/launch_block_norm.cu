@@ -43,12 +43,6 @@ bool aligned(const BlockNormArgs& a) {
     return bits == 0;
 }
 
-template <typename S, bool ROTATE, bool BACKWARD>
-constexpr int shared_bytes() {
-    const int row = ROTATE || (BACKWARD && S::kRows > 1) ? S::kRows * S::TPR * S::EPT : 0;
-    return 4 * (row + 4 * S::kWarps);
-}
-
 template <typename S, bool ROTATE>
 cudaError_t run(const BlockNormArgs& a, size_t groups, cudaStream_t stream) {
     static KernelSetup setup;
@@ -57,7 +51,8 @@ cudaError_t run(const BlockNormArgs& a, size_t groups, cudaStream_t stream) {
 #else
     auto kernel = &block_norm_kernel<T, R, S, ROTATE>;
 #endif
-    constexpr int smem = shared_bytes<S, ROTATE, CUBF_BN_BACKWARD>();
+    using Plan = std::conditional_t<CUBF_BN_BACKWARD, BackwardPlan<S, ROTATE>, ForwardPlan<S, ROTATE>>;
+    constexpr int smem = 4 * Plan::kFloats;
     int cap = 0;
     cudaError_t e = setup_kernel(setup, kernel, S::kThreads, smem, &cap);
     if (e != cudaSuccess) return e;
@@ -72,9 +67,9 @@ cudaError_t run(const BlockNormArgs& a, size_t groups, cudaStream_t stream) {
     return launch_dependent(kernel, static_cast<unsigned>(grid), static_cast<unsigned>(S::kThreads), smem, stream, a);
 }
 
-template <int TPR, int EPT, int VW, bool ROTATE>
+template <int TPR, int EPT, int VW, bool ROTATE, int THREADS = 0>
 cudaError_t shape(const BlockNormArgs& a, size_t groups, cudaStream_t stream) {
-    return run<Shape<TPR, EPT, VW>, ROTATE>(a, groups, stream);
+    return run<Shape<TPR, EPT, VW, THREADS>, ROTATE>(a, groups, stream);
 }
 
 cudaError_t dispatch(const BlockNormArgs& a, size_t groups, cudaStream_t s) {
@@ -94,14 +89,23 @@ cudaError_t dispatch(const BlockNormArgs& a, size_t groups, cudaStream_t s) {
                 case 16384: return shape<1024, 16, V, true>(a, groups, s);
             }
 #else
+            if (a.rows > 296 || d < 2048) {
+                switch (d) {
+                    case 256: return shape<32, 8, V, true>(a, groups, s);
+                    case 512: return shape<32, 16, V, true>(a, groups, s);
+                    case 1024: return shape<32, 32, V, true, 256>(a, groups, s);
+                    case 2048: return shape<64, 32, V, true, 512>(a, groups, s);
+                    case 4096: return shape<64, 64, V, true, 512>(a, groups, s);
+                    case 8192: return shape<128, 64, V, true, 512>(a, groups, s);
+                    case 16384: return shape<512, 32, V, true>(a, groups, s);
+                }
+            }
+            // few rows: more threads a row
             switch (d) {
-                case 256: return shape<32, 8, V, true>(a, groups, s);
-                case 512: return shape<32, 16, V, true>(a, groups, s);
-                case 1024: return shape<32, 32, V, true>(a, groups, s);
-                case 2048: return shape<64, 32, V, true>(a, groups, s);
-                case 4096: return shape<64, 64, V, true>(a, groups, s);
-                case 8192: return shape<128, 64, V, true>(a, groups, s);
-                case 16384: return shape<256, 64, V, true>(a, groups, s);
+                case 2048: return shape<256, 8, V, true>(a, groups, s);
+                case 4096: return shape<512, 8, V, true>(a, groups, s);
+                case 8192: return shape<1024, 8, V, true>(a, groups, s);
+                case 16384: return shape<1024, 16, V, true>(a, groups, s);
             }
 #endif
         }
@@ -124,7 +128,7 @@ cudaError_t dispatch(const BlockNormArgs& a, size_t groups, cudaStream_t s) {
         if (d <= 1024) return shape<128, 8, V, false>(a, groups, s);
         if (d <= 2048) return shape<256, 8, V, false>(a, groups, s);
         if (d <= 4096) return shape<512, 8, V, false>(a, groups, s);
-        if (d <= 8192) return shape<512, 16, V, false>(a, groups, s);
+        if (d <= 8192) return shape<1024, 8, V, false>(a, groups, s);
         if (d <= kBlockNormMaxDim) return shape<1024, 16, V, false>(a, groups, s);
     } else {
         if (d <= 256) return shape<32, 8, 1, false>(a, groups, s);
