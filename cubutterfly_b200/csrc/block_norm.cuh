@@ -45,7 +45,8 @@ struct Shape {
     static constexpr int kThreads = THREADS_ > 0 ? THREADS_ : TPR == 32 ? 128 : TPR;
     static constexpr int kRows = kThreads / TPR;    // rows a CTA works on at a time
     static constexpr int kWarps = TPR / 32;
-    static_assert(C * VW == EPT && TPR >= 32 && EPT >= 2 && kRows <= 15, "whole chunks over whole warps");
+    static_assert(C * VW == EPT && TPR >= 32 && EPT >= 2, "whole chunks over whole warps");
+    static_assert(TPR == 32 || kRows <= 15, "a barrier for each row of several warps");
     static CUBF_DEV int at(int c, int j) { return (c * TPR + j) * VW; }
 };
 
@@ -399,10 +400,16 @@ struct ForwardPlan {
     static constexpr int kWordsAt = S::kRows * kRow;
     static constexpr int kFactorsAt = kWordsAt + S::kRows * 4 * S::kWarps;
     static constexpr int kFloats = kFactorsAt + (kShared ? 2 * kDim : 0);
+    // 16-bit rows of eight values a thread fit 1024 threads an SM
+    template <typename T, typename R>
+    static constexpr int ctas() {
+        return S::EPT == 8 && S::VW == 8 && sizeof(R) == 2 && !ROTATE && S::kThreads < 1024 ? 1024 / S::kThreads : 1;
+    }
 };
 
 template <typename T, typename R, typename S, bool ROTATE>
-__global__ void __launch_bounds__(S::kThreads, 1) block_norm_kernel(BlockNormArgs p) {
+__global__ void __launch_bounds__(S::kThreads, ForwardPlan<S, ROTATE>::template ctas<T, R>())
+    block_norm_kernel(BlockNormArgs p) {
     using Plan = ForwardPlan<S, ROTATE>;
     extern __shared__ __align__(16) float shared[];
     pdl_begin();
@@ -530,12 +537,13 @@ __global__ void __launch_bounds__(S::kThreads, 1) block_norm_kernel(BlockNormArg
 template <typename S, bool ROTATE>
 struct BackwardPlan {
     static constexpr int kDim = S::TPR * S::EPT;
-    static constexpr bool kLean = S::EPT * S::kThreads > 4096 || ROTATE;  // no room for the next row in registers
+    static constexpr bool kLean = S::EPT * S::kThreads > 4096 || S::EPT > 8;  // no room for the next row in registers
     static constexpr bool kSharedSums = S::EPT > 8 && !(ROTATE && S::kThreads <= 256);
+    static constexpr bool kSharedZ = !(ROTATE && kDim > 8192);  // else Z is summed in the CTA's part of the workspace
     static constexpr int kRow = ROTATE ? padded_row(kDim) : 0;
     static constexpr int kWordsAt = S::kRows * kRow;
-    static constexpr int kSumsAt = kWordsAt + S::kRows * 4 * S::kWarps;   // Z, then P and Q if shared
-    static constexpr int kFloats = kSumsAt + S::kRows * kDim * (kSharedSums ? 3 : 1);
+    static constexpr int kSumsAt = kWordsAt + S::kRows * 4 * S::kWarps;   // P and Q if shared, then Z
+    static constexpr int kFloats = kSumsAt + S::kRows * kDim * ((kSharedSums ? 2 : 0) + (kSharedZ ? 1 : 0));
 };
 
 // t - vn mean(t vn), the part of t that a norm lets through.  In a row of one
@@ -545,8 +553,7 @@ CUBF_DEV Pair through_norm(const BlockNormArgs& p, Pair t, Pair vn, float mean, 
 }
 
 template <typename T, typename R, typename S, bool ROTATE>
-__global__ void __launch_bounds__(S::kThreads, S::kThreads <= 256 && ROTATE ? 2 : 1)
-    block_norm_backward_kernel(BlockNormArgs p) {
+__global__ void __launch_bounds__(S::kThreads, 1) block_norm_backward_kernel(BlockNormArgs p) {
     using Plan = BackwardPlan<S, ROTATE>;
     extern __shared__ __align__(16) float shared[];
     pdl_begin();
@@ -610,12 +617,18 @@ __global__ void __launch_bounds__(S::kThreads, S::kThreads <= 256 && ROTATE ? 2 
 #pragma unroll
     for (int k = 0; k < (Plan::kSharedSums ? 1 : S::HALF); ++k) P[k] = Q[k] = both(0.f);
 #pragma unroll
-    for (int k = 0; k < S::HALF * (Plan::kSharedSums ? 3 : 1); ++k) mine[k * S::kThreads] = make_float2(0.f, 0.f);
+    for (int k = 0; k < S::HALF * ((Plan::kSharedSums ? 2 : 0) + (Plan::kSharedZ ? 1 : 0)); ++k)
+        mine[k * S::kThreads] = make_float2(0.f, 0.f);
+    float* const part = p.partials + static_cast<size_t>(blockIdx.x) * 3 * dim;
+    if (!Plan::kSharedZ && p.need_z)
+        store_row<S>(part + 2 * static_cast<size_t>(dim), j, dim, [&](int) { return both(0.f); });
+    constexpr int kP = 0, kQ = 1, kZ = 2;
+    constexpr int kPlaceZ = Plan::kSharedSums ? 2 : 0;
     auto add_sum = [&](Pair* regs, int which, int k, Pair a, Pair b) {  // += a b
-        if (!Plan::kSharedSums && which > 0) {
+        if (!Plan::kSharedSums && which != kZ) {
             regs[k] = fma2(a, b, regs[k]);
         } else {
-            float2* at = mine + which * kSumStride + k * S::kThreads;
+            float2* at = mine + (which == kZ ? kPlaceZ : which) * kSumStride + k * S::kThreads;
             const float2 f = *at;
             *at = floats(fma2(a, b, f32x2::pk(f.x, f.y)));
         }
@@ -666,7 +679,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kThreads <= 256 && ROTATE ? 2 
 #pragma unroll
                 for (int k = 0; k < S::HALF; ++k) {
                     sn[k] = mul2(sn[k], both(in.rs));
-                    if (p.need_q) add_sum(Q, 2, k, d[k], sn[k]);
+                    if (p.need_q) add_sum(Q, kQ, k, d[k], sn[k]);
                     d[k] = mul2(d[k], kKeep ? kp[k] : lp[k]);
                     sum = fma2(d[k], sn[k], sum);
                 }
@@ -683,11 +696,17 @@ __global__ void __launch_bounds__(S::kThreads, S::kThreads <= 256 && ROTATE ? 2 
         {
             if (p.scales) {
                 load_vector<T, S>(p.scales, p.scales32, j, dim, 0.f, sn);
+                if constexpr (Plan::kSharedZ) {
 #pragma unroll
-                for (int k = 0; k < S::HALF; ++k) {
-                    add_sum(nullptr, 0, k, d[k], in.x.pair(k));
-                    sn[k] = mul2(sn[k], d[k]);
+                    for (int k = 0; k < S::HALF; ++k) add_sum(nullptr, kZ, k, d[k], in.x.pair(k));
+                } else {
+                    float* const z = part + 2 * static_cast<size_t>(dim);
+                    Values<float, S> old;
+                    old.load(z, j, dim);
+                    store_row<S>(z, j, dim, [&](int k) { return fma2(d[k], in.x.pair(k), old.pair(k)); });
                 }
+#pragma unroll
+                for (int k = 0; k < S::HALF; ++k) sn[k] = mul2(sn[k], d[k]);
             } else {
 #pragma unroll
                 for (int k = 0; k < S::HALF; ++k) sn[k] = mul2(both(p.scale), d[k]);
@@ -708,7 +727,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kThreads <= 256 && ROTATE ? 2 
                     const Pair yn = mul2(in.y.pair(k), both(in.ry));
                     sn[k] = mul2(mul2(mul2(d[k], yn), w), activation<true>(p.act, g));  // dgate
                     d[k] = mul2(d[k], activation<false>(p.act, g));                       // dn
-                    if (p.need_p) add_sum(P, 1, k, d[k], yn);
+                    if (p.need_p) add_sum(P, kP, k, d[k], yn);
                     d[k] = mul2(d[k], w);
                     sum = fma2(d[k], yn, sum);
                 }
@@ -717,7 +736,7 @@ __global__ void __launch_bounds__(S::kThreads, S::kThreads <= 256 && ROTATE ? 2 
 #pragma unroll
                 for (int k = 0; k < S::HALF; ++k) {
                     const Pair yn = mul2(in.y.pair(k), both(in.ry));
-                    if (p.need_p) add_sum(P, 1, k, d[k], yn);
+                    if (p.need_p) add_sum(P, kP, k, d[k], yn);
                     d[k] = mul2(d[k], mul2(kKeep ? kw[k] : lw[k], kKeep ? ka[k] : la[k]));
                     sum = fma2(d[k], yn, sum);
                 }
@@ -737,10 +756,11 @@ __global__ void __launch_bounds__(S::kThreads, S::kThreads <= 256 && ROTATE ? 2 
         }
     }
     // The CTA's sums; rows side by side in a CTA are added first, in shared memory.
-    float* const part = p.partials + static_cast<size_t>(blockIdx.x) * 3 * dim;
     auto write = [&](Pair* regs, int which, float* dst) {
-        float2* const at = mine + (Plan::kSharedSums ? which : 0) * kSumStride;
-        if (!Plan::kSharedSums && which > 0 && S::kRows > 1) {
+        const bool held = !Plan::kSharedSums && which != kZ;  // in registers
+        float2* const at = mine + (which == kZ ? kPlaceZ : Plan::kSharedSums ? which : 0) * kSumStride;
+        Pair v[S::HALF];
+        if (held && S::kRows > 1) {
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < S::HALF; ++k) at[k * S::kThreads] = floats(regs[k]);
@@ -749,10 +769,9 @@ __global__ void __launch_bounds__(S::kThreads, S::kThreads <= 256 && ROTATE ? 2 
             __syncthreads();
             if (sub > 0) return;
         }
-        Pair v[S::HALF];
 #pragma unroll
         for (int k = 0; k < S::HALF; ++k) {
-            if (!Plan::kSharedSums && which > 0 && S::kRows == 1) {
+            if (held && S::kRows == 1) {
                 v[k] = regs[k];
             } else {
                 v[k] = both(0.f);
@@ -764,9 +783,9 @@ __global__ void __launch_bounds__(S::kThreads, S::kThreads <= 256 && ROTATE ? 2 
         }
         store_row<S>(dst, j, dim, [&](int k) { return v[k]; });
     };
-    if (p.need_z) write(nullptr, 0, part + 2 * static_cast<size_t>(dim));
-    if (p.need_p) write(P, 1, part);
-    if (p.need_q) write(Q, 2, part + dim);
+    if (Plan::kSharedZ && p.need_z) write(nullptr, kZ, part + 2 * static_cast<size_t>(dim));
+    if (p.need_p) write(P, kP, part);
+    if (p.need_q) write(Q, kQ, part + dim);
 }
 
 // The gradients of the per-channel vectors from the CTAs' sums: 32 columns

@@ -31,11 +31,11 @@ int unit_of(BlockType type, bool residual32) {
 }  // namespace
 
 int block_norm_parts(size_t rows_per_gate, size_t groups, int dim) {
-    // rows side by side in a CTA of the narrow shapes; then at least four
-    // turns per CTA, and no more CTAs than two per SM
-    const size_t side = dim <= 256 ? 4 : 1;
-    const size_t most = std::max<size_t>(1, (rows_per_gate + 4 * side - 1) / (4 * side));
-    const size_t share = std::max<size_t>(1, 296 / std::max<size_t>(1, groups));
+    // A CTA of 512 threads takes 512 x 8 values of rows side by side; at least
+    // two turns of it, and no more CTAs than SMs.
+    const size_t side = std::max<size_t>(1, 4096 / static_cast<size_t>(dim));
+    const size_t most = std::max<size_t>(1, (rows_per_gate + 2 * side - 1) / (2 * side));
+    const size_t share = std::max<size_t>(1, (148 + groups - 1) / std::max<size_t>(1, groups));
     return static_cast<int>(std::min(most, share));
 }
 

@@ -80,11 +80,11 @@ cudaError_t dispatch(const BlockNormArgs& a, size_t groups, cudaStream_t s) {
         if (vec && d >= 256) {
 #if CUBF_BN_BACKWARD
             switch (d) {
-                case 256: return shape<32, 8, V, true>(a, groups, s);
-                case 512: return shape<32, 16, V, true>(a, groups, s);
-                case 1024: return shape<64, 16, V, true>(a, groups, s);
-                case 2048: return shape<128, 16, V, true>(a, groups, s);
-                case 4096: return shape<256, 16, V, true>(a, groups, s);
+                case 256: return shape<32, 8, V, true, 512>(a, groups, s);
+                case 512: return shape<64, 8, V, true, 512>(a, groups, s);
+                case 1024: return shape<128, 8, V, true, 512>(a, groups, s);
+                case 2048: return shape<256, 8, V, true, 512>(a, groups, s);
+                case 4096: return shape<512, 8, V, true>(a, groups, s);
                 case 8192: return shape<512, 16, V, true>(a, groups, s);
                 case 16384: return shape<1024, 16, V, true>(a, groups, s);
             }
@@ -95,8 +95,8 @@ cudaError_t dispatch(const BlockNormArgs& a, size_t groups, cudaStream_t s) {
                     case 512: return shape<32, 16, V, true>(a, groups, s);
                     case 1024: return shape<32, 32, V, true, 256>(a, groups, s);
                     case 2048: return shape<64, 32, V, true, 512>(a, groups, s);
-                    case 4096: return shape<64, 64, V, true, 512>(a, groups, s);
-                    case 8192: return shape<128, 64, V, true, 512>(a, groups, s);
+                    case 4096: return shape<64, 64, V, true, 384>(a, groups, s);
+                    case 8192: return shape<128, 64, V, true, 384>(a, groups, s);
                     case 16384: return shape<512, 32, V, true>(a, groups, s);
                 }
             }
@@ -122,17 +122,22 @@ cudaError_t dispatch(const BlockNormArgs& a, size_t groups, cudaStream_t s) {
         }
         return cudaErrorInvalidValue;
     }
+#if CUBF_BN_BACKWARD
+    constexpr int kThreads = 512;  // rows side by side, so that there is one part of the sums per SM
+#else
+    constexpr int kThreads = 0;
+#endif
     if (vec) {
-        if (d <= 256) return shape<32, 8, V, false>(a, groups, s);
-        if (d <= 512) return shape<64, 8, V, false>(a, groups, s);
-        if (d <= 1024) return shape<128, 8, V, false>(a, groups, s);
-        if (d <= 2048) return shape<256, 8, V, false>(a, groups, s);
+        if (d <= 256) return shape<32, 8, V, false, kThreads>(a, groups, s);
+        if (d <= 512) return shape<64, 8, V, false, kThreads>(a, groups, s);
+        if (d <= 1024) return shape<128, 8, V, false, kThreads>(a, groups, s);
+        if (d <= 2048) return shape<256, 8, V, false, kThreads>(a, groups, s);
         if (d <= 4096) return shape<512, 8, V, false>(a, groups, s);
         if (d <= 8192) return shape<1024, 8, V, false>(a, groups, s);
         if (d <= kBlockNormMaxDim) return shape<1024, 16, V, false>(a, groups, s);
     } else {
-        if (d <= 256) return shape<32, 8, 1, false>(a, groups, s);
-        if (d <= 1024) return shape<128, 8, 1, false>(a, groups, s);
+        if (d <= 256) return shape<32, 8, 1, false, kThreads>(a, groups, s);
+        if (d <= 1024) return shape<128, 8, 1, false, kThreads>(a, groups, s);
         if (d <= 4096) return shape<512, 8, 1, false>(a, groups, s);
         if (d <= kBlockNormMaxDim) return shape<1024, 16, 1, false>(a, groups, s);
     }
