@@ -198,6 +198,16 @@ CUBF_DEV Pair activation(int act, Pair g) {
     const float2 f = floats(g);
     return f32x2::pk(activation<SLOPE>(act, f.x), activation<SLOPE>(act, f.y));
 }
+// body(act) with the activation a constant in it
+template <typename Body>
+CUBF_DEV void with_activation(int act, Body&& body) {
+    if (act == 0)
+        body(std::integral_constant<int, 0>());
+    else if (act == 1)
+        body(std::integral_constant<int, 1>());
+    else
+        body(std::integral_constant<int, 2>());
+}
 
 // ---- a row over its threads -------------------------------------------------------------------
 // Rows of several warps that share a CTA with others meet on a barrier of
@@ -224,9 +234,17 @@ CUBF_DEV float row_sum(float v, float* words, int slot) {
         float* w = words + slot * S::kWarps;
         if ((threadIdx.x & 31) == 0) w[threadIdx.x % S::TPR / 32] = v;
         row_barrier<S>();
-        v = 0.f;
+        if constexpr (S::kWarps >= 4) {
+            Pair t = both(0.f);
 #pragma unroll
-        for (int k = 0; k < S::kWarps; ++k) v += w[k];
+            for (int k = 0; k < S::kWarps; k += 4) {
+                const float4 q = *reinterpret_cast<const float4*>(w + k);
+                t = add2(t, add2(f32x2::pk(q.x, q.y), f32x2::pk(q.z, q.w)));
+            }
+            v = sum_of(t);
+        } else {
+            v = w[0] + w[1];
+        }
     }
     return v;
 }
@@ -386,6 +404,11 @@ CUBF_DEV void rotate_row(Pair (&v)[S::HALF], float* row, int j) {
     rotate_passes<S, 0>(v, row, j);
 }
 
+template <typename T>
+CUBF_DEV uint32_t dim_bytes(int dim) {
+    return static_cast<uint32_t>(dim) * static_cast<uint32_t>(sizeof(T));
+}
+
 // ---- forward ----------------------------------------------------------------------------------
 // Shared memory, in floats: the rotated rows, then the words of the row sums,
 // then (shapes of many values a thread) the channel factors of s and u.
@@ -417,19 +440,25 @@ __global__ void __launch_bounds__(S::kThreads, ForwardPlan<S, ROTATE>::template 
     float* const exchange = shared + sub * Plan::kRow;
     float* const words = shared + Plan::kWordsAt + sub * 4 * S::kWarps;
     float2* const factors = reinterpret_cast<float2*>(shared + Plan::kFactorsAt);
-    const size_t stride = static_cast<size_t>(gridDim.x) * S::kRows;
-    size_t row = static_cast<size_t>(blockIdx.x) * S::kRows + sub;
+    const uint32_t stride = gridDim.x * S::kRows, rows = static_cast<uint32_t>(p.rows);
+    uint32_t row = blockIdx.x * S::kRows + sub;
     const float inv_dim = 1.f / static_cast<float>(dim);
 
     Values<R, S> x;
     Values<T, S> y, g;
-    auto load = [&](size_t at) {
-        x.load(static_cast<const R*>(p.x) + at * p.x_row, j, dim);
-        if (p.y) y.load(static_cast<const T*>(p.y) + at * p.y_row, j, dim);
-        if (p.gate_mode == kGateFull) g.load(static_cast<const T*>(p.gate) + at * p.gate_row, j, dim);
+    // row `n` of a tensor: one multiply-add, its operands in constant memory
+    auto at = [&](auto* base, uint32_t bytes, uint32_t n) {
+        using E = std::remove_pointer_t<decltype(base)>;
+        using Byte = std::conditional_t<std::is_const<E>::value, const char, char>;
+        return reinterpret_cast<E*>(reinterpret_cast<Byte*>(base) + static_cast<unsigned long long>(n) * bytes);
+    };
+    auto load = [&](uint32_t n) {
+        x.load(at(static_cast<const R*>(p.x), p.x_bytes, n), j, dim);
+        if (p.y) y.load(at(static_cast<const T*>(p.y), p.y_bytes, n), j, dim);
+        if (p.gate_mode == kGateFull) g.load(at(static_cast<const T*>(p.gate), p.gate_bytes, n), j, dim);
     };
     y.clear();
-    if (Plan::kAhead && row < p.rows) load(row);
+    if (Plan::kAhead && row < rows) load(row);
 
     // What multiplies y r(y) in s (post_weight, and the gate where it is one
     // per channel) and s r(s) in u.
@@ -467,7 +496,7 @@ __global__ void __launch_bounds__(S::kThreads, ForwardPlan<S, ROTATE>::template 
         }
     };
 
-    for (int slot = 0; row < p.rows; row += stride, slot ^= 1) {
+    for (int slot = 0; row < rows; row += stride, slot ^= 1) {
         if (!Plan::kAhead) load(row);
         Pair s[S::HALF];
         Pair sum = both(0.f);
@@ -488,14 +517,16 @@ __global__ void __launch_bounds__(S::kThreads, ForwardPlan<S, ROTATE>::template 
         }
         if (p.y) {
             if (p.gate_mode == kGateFull) {
+                with_activation(p.act, [&](auto act) {
 #pragma unroll
-                for (int k = 0; k < S::HALF; ++k)
-                    s[k] = fma2(mul2(mul2(factor(0, k), both(ry)), activation<false>(p.act, g.pair(k))), y.pair(k), s[k]);
+                    for (int k = 0; k < S::HALF; ++k)
+                        s[k] = fma2(mul2(mul2(factor(0, k), both(ry)), activation<false>(act, g.pair(k))), y.pair(k), s[k]);
+                });
             } else if (p.gate_mode == kGateGroups) {
                 Pair a[S::HALF];
-                const size_t at = row / p.rows_per_gate * p.gate_row;
-                load_vector<T, S>(p.gate32 ? static_cast<const void*>(static_cast<const float*>(p.gate) + at)
-                                           : static_cast<const void*>(static_cast<const T*>(p.gate) + at),
+                const size_t from = row / static_cast<uint32_t>(p.rows_per_gate) * p.gate_row;
+                load_vector<T, S>(p.gate32 ? static_cast<const void*>(static_cast<const float*>(p.gate) + from)
+                                           : static_cast<const void*>(static_cast<const T*>(p.gate) + from),
                                   p.gate32, j, dim, 0.f, a);
 #pragma unroll
                 for (int k = 0; k < S::HALF; ++k)
@@ -505,9 +536,9 @@ __global__ void __launch_bounds__(S::kThreads, ForwardPlan<S, ROTATE>::template 
                 for (int k = 0; k < S::HALF; ++k) s[k] = fma2(mul2(factor(0, k), both(ry)), y.pair(k), s[k]);
             }
         }
-        if (Plan::kAhead && row + stride < p.rows) load(row + stride);
+        if (Plan::kAhead && row + stride < rows) load(row + stride);
         if (p.residual)
-            store_row<S>(static_cast<R*>(p.residual) + row * dim, j, dim, [&](int k) { return s[k]; });
+            store_row<S>(at(static_cast<R*>(p.residual), dim_bytes<R>(dim), row), j, dim, [&](int k) { return s[k]; });
         if (!p.normed) continue;
         sum = both(0.f);
 #pragma unroll
@@ -517,7 +548,7 @@ __global__ void __launch_bounds__(S::kThreads, ForwardPlan<S, ROTATE>::template 
 #pragma unroll
         for (int k = 0; k < S::HALF; ++k) s[k] = mul2(s[k], mul2(factor(1, k), both(rs)));
         if constexpr (ROTATE) rotate_row<S>(s, exchange, j);
-        store_row<S>(static_cast<T*>(p.normed) + row * dim, j, dim, [&](int k) { return s[k]; });
+        store_row<S>(at(static_cast<T*>(p.normed), dim_bytes<T>(dim), row), j, dim, [&](int k) { return s[k]; });
     }
 }
 
@@ -534,23 +565,39 @@ __global__ void __launch_bounds__(S::kThreads, ForwardPlan<S, ROTATE>::template 
 // gate row, so that for a gate per channel or per group dw_post and dgate both
 // follow from P = sum dS yn; with a gate per row P = sum dn yn.  Each CTA
 // writes its sums once and a second kernel adds them in a fixed order.
+// Up to 512 threads a CTA have registers for the sums P and Q, and with eight
+// values a thread for the channel factors of y r(y) and s r(s) too; else those
+// lie in shared memory, or are loaded through L1 where a row does not leave
+// room.  Shared memory, in floats: the rotated rows, the words of the row
+// sums, the factors, the sums (with P and Q or without), and Z where needed.
 template <typename S, bool ROTATE>
 struct BackwardPlan {
     static constexpr int kDim = S::TPR * S::EPT;
-    static constexpr bool kLean = S::EPT * S::kThreads > 4096 || S::EPT > 8;  // no room for the next row in registers
-    static constexpr bool kSharedSums = S::EPT > 8 && !(ROTATE && S::kThreads <= 256);
+    static constexpr bool kHeldSums = S::kThreads <= 512 && S::EPT <= 8;
+    static constexpr bool kHeldFactors = kHeldSums;
+    static constexpr bool kSharedFactors = !kHeldFactors && kDim <= 8192;
     static constexpr bool kSharedZ = !(ROTATE && kDim > 8192);  // else Z is summed in the CTA's part of the workspace
     static constexpr int kRow = ROTATE ? padded_row(kDim) : 0;
     static constexpr int kWordsAt = S::kRows * kRow;
-    static constexpr int kSumsAt = kWordsAt + S::kRows * 4 * S::kWarps;   // P and Q if shared, then Z
-    static constexpr int kFloats = kSumsAt + S::kRows * kDim * ((kSharedSums ? 2 : 0) + (kSharedZ ? 1 : 0));
+    static constexpr int kFactorsAt = kWordsAt + S::kRows * 4 * S::kWarps;
+    static constexpr int kSumsAt = kFactorsAt + (kSharedFactors ? 2 * kDim : 0);
+    static constexpr int kSum = S::kThreads * S::EPT;
+    static constexpr int kPlaces = kHeldSums ? (S::kRows > 1 ? 1 : 0) : 2;  // rows side by side add their sums there
+    static constexpr int kPlaceZ = kHeldSums ? 0 : 2;
+    static constexpr int floats_needed(bool z) {
+        const int places = z && kSharedZ ? kPlaceZ + 1 : 0;
+        return kSumsAt + kSum * (places > kPlaces ? places : kPlaces);
+    }
 };
 
-// t - vn mean(t vn), the part of t that a norm lets through.  In a row of one
-// value vn^2 = 1 - eps r^2, and the difference would cancel.
-CUBF_DEV Pair through_norm(const BlockNormArgs& p, Pair t, Pair vn, float mean, float r) {
-    return p.dim == 1 ? mul2(t, both(p.eps * r * r)) : fma2(vn, both(-mean), t);
-}
+// r (t - vn mean(t vn)), the part of t that a norm lets through, is taken as
+// r' (t - vn m).  In a row of one value vn^2 = 1 - eps r^2, and the difference
+// would cancel: there m = 0 and r' = eps r^3.
+struct Through {
+    float m, r;
+    CUBF_DEV Through(const BlockNormArgs& p, float mean, float factor)
+        : m(p.dim == 1 ? 0.f : -mean), r(p.dim == 1 ? p.eps * factor * factor * factor : factor) {}
+};
 
 template <typename T, typename R, typename S, bool ROTATE>
 __global__ void __launch_bounds__(S::kThreads, 1) block_norm_backward_kernel(BlockNormArgs p) {
@@ -560,9 +607,9 @@ __global__ void __launch_bounds__(S::kThreads, 1) block_norm_backward_kernel(Blo
     const int j = threadIdx.x % S::TPR, sub = threadIdx.x / S::TPR, dim = p.dim;
     float* const exchange = shared + sub * Plan::kRow;
     float* const words = shared + Plan::kWordsAt + sub * 4 * S::kWarps;
-    // the thread's own sums: pair k at [k][thread]
+    float2* const factors = reinterpret_cast<float2*>(shared + Plan::kFactorsAt);
+    // the thread's own sums: pair k of sum n at [n][k][thread]
     float2* const mine = reinterpret_cast<float2*>(shared + Plan::kSumsAt) + threadIdx.x;
-    constexpr int kSumStride = S::HALF * S::kThreads;
     const float inv_dim = 1.f / static_cast<float>(dim);
     // this CTA's rows: a share of one gate group's
     const size_t group = blockIdx.x / p.parts_per_group;
@@ -572,80 +619,128 @@ __global__ void __launch_bounds__(S::kThreads, 1) block_norm_backward_kernel(Blo
     const size_t end = group * p.rows_per_gate + to;
     size_t row = group * p.rows_per_gate + from + sub;
 
-    struct Row {
-        Values<R, S> x, ds;
-        Values<T, S> y, g, du;
-        float ry, rs;
+    // The row in work, and of the next one what has been loaded already: each
+    // tensor's registers are loaded again as soon as they have been used.
+    Values<R, S> x, ds;
+    Values<T, S> y, g, du;
+    float ry = 1.f, rs = 0.f, next_ry = 1.f, next_rs = 0.f;
+    const bool row_gate = p.gate_mode == kGateFull;
+    // row `n` of a tensor: one multiply-add, its operands in constant memory
+    uint32_t n = static_cast<uint32_t>(row);
+    const uint32_t last = static_cast<uint32_t>(end);
+    auto at = [&](auto* base, uint32_t bytes, uint32_t ahead) {
+        using E = std::remove_pointer_t<decltype(base)>;
+        using Byte = std::conditional_t<std::is_const<E>::value, const char, char>;
+        return reinterpret_cast<E*>(reinterpret_cast<Byte*>(base) + static_cast<unsigned long long>(n + ahead) * bytes);
     };
-    auto load = [&](size_t at, Row& in) {
-        in.x.load(static_cast<const R*>(p.x) + at * p.x_row, j, dim);
-        if (p.y) in.y.load(static_cast<const T*>(p.y) + at * p.y_row, j, dim);
-        if (p.d_residual) in.ds.load(static_cast<const R*>(p.d_residual) + at * p.d_residual_row, j, dim);
-        if (p.d_normed) in.du.load(static_cast<const T*>(p.d_normed) + at * p.d_normed_row, j, dim);
-        if (p.gate_mode == kGateFull) in.g.load(static_cast<const T*>(p.gate) + at * p.gate_row, j, dim);
-        in.ry = p.post_norm ? p.r_post[at] : 1.f;
-        in.rs = p.d_normed ? p.r_pre[at] : 0.f;
+    auto load_du = [&](uint32_t ahead) {
+        if (p.d_normed) du.load(at(static_cast<const T*>(p.d_normed), p.d_normed_bytes, ahead), j, dim);
     };
-    Row in;
-    in.y.clear();
-    in.ds.clear();
-    in.du.clear();
-    in.g.clear();
-    if (row < end) load(row, in);
+    auto load_ds = [&](uint32_t ahead) {
+        if (p.d_residual) ds.load(at(static_cast<const R*>(p.d_residual), p.d_residual_bytes, ahead), j, dim);
+    };
+    auto load_x = [&](uint32_t ahead) { x.load(at(static_cast<const R*>(p.x), p.x_bytes, ahead), j, dim); };
+    auto load_y = [&](Values<T, S>& y, Values<T, S>& g, uint32_t ahead) {
+        if (p.y) y.load(at(static_cast<const T*>(p.y), p.y_bytes, ahead), j, dim);
+        if (row_gate) g.load(at(static_cast<const T*>(p.gate), p.gate_bytes, ahead), j, dim);
+    };
+    y.clear();
+    ds.clear();
+    du.clear();
+    if (n < last) {
+        load_du(0);
+        load_x(0);
+        load_y(y, g, 0);
+        load_ds(0);
+        if (p.post_norm) ry = p.r_post[n];
+        if (p.d_normed) rs = p.r_pre[n];
+    }
 
-    // channel factors: w_post, act(gate) where the CTA's rows share it, and w_pre
-    constexpr bool kKeep = !Plan::kLean;
-    Pair kw[kKeep ? S::HALF : 1], ka[kKeep ? S::HALF : 1], kp[kKeep ? S::HALF : 1];
-    const bool row_gate = p.gate_mode == kGateFull, shared_gate = p.gate_mode == kGateChannel || p.gate_mode == kGateGroups;
-    auto gate_factor = [&](Pair(&a)[S::HALF]) {
-        const size_t at = p.gate_mode == kGateGroups ? group * p.gate_row : 0;
-        load_vector<T, S>(!shared_gate ? nullptr
-                          : p.gate32   ? static_cast<const void*>(static_cast<const float*>(p.gate) + at)
+    // channel factors: w_post times act(gate) where the CTA's rows share it, and w_pre
+    auto factor_y = [&](Pair(&a)[S::HALF]) {
+        load_vector<T, S>(p.post, p.post32, j, dim, 1.f, a);
+        if (p.gate_mode == kGateChannel || p.gate_mode == kGateGroups) {
+            const size_t at = p.gate_mode == kGateGroups ? group * p.gate_row : 0;
+            Pair b[S::HALF];
+            load_vector<T, S>(p.gate32 ? static_cast<const void*>(static_cast<const float*>(p.gate) + at)
                                        : static_cast<const void*>(static_cast<const T*>(p.gate) + at),
-                          p.gate32, j, dim, 1.f, a);
-        if (shared_gate) {
+                              p.gate32, j, dim, 1.f, b);
 #pragma unroll
-            for (int k = 0; k < S::HALF; ++k) a[k] = activation<false>(p.act, a[k]);
+            for (int k = 0; k < S::HALF; ++k) a[k] = mul2(a[k], activation<false>(p.act, b[k]));
         }
     };
-    if constexpr (kKeep) {
-        load_vector<T, S>(p.post, p.post32, j, dim, 1.f, kw);
-        gate_factor(ka);
-        load_vector<T, S>(p.pre, p.pre32, j, dim, 1.f, kp);
+    Pair held[Plan::kHeldFactors ? 2 : 1][Plan::kHeldFactors || !Plan::kSharedFactors ? S::HALF : 1];
+    if constexpr (Plan::kHeldFactors) {
+        factor_y(held[0]);
+        load_vector<T, S>(p.pre, p.pre32, j, dim, 1.f, held[1]);
+    } else if constexpr (Plan::kSharedFactors) {
+        Pair a[S::HALF];
+        if (sub == 0) {
+            factor_y(a);
+#pragma unroll
+            for (int k = 0; k < S::HALF; ++k) factors[k * S::TPR + j] = floats(a[k]);
+            load_vector<T, S>(p.pre, p.pre32, j, dim, 1.f, a);
+#pragma unroll
+            for (int k = 0; k < S::HALF; ++k) factors[(S::HALF + k) * S::TPR + j] = floats(a[k]);
+        }
+        __syncthreads();
     }
-    Pair P[Plan::kSharedSums ? 1 : S::HALF], Q[Plan::kSharedSums ? 1 : S::HALF];
+    auto bring = [&](int which) {  // factors that have no place are loaded each time
+        if constexpr (!Plan::kHeldFactors && !Plan::kSharedFactors) {
+            if (which == 0)
+                factor_y(held[0]);
+            else
+                load_vector<T, S>(p.pre, p.pre32, j, dim, 1.f, held[0]);
+        }
+    };
+    auto factor = [&](int which, int k) {
+        if constexpr (Plan::kSharedFactors) {
+            const float2 f = factors[(which * S::HALF + k) * S::TPR + j];
+            return f32x2::pk(f.x, f.y);
+        } else {
+            return held[Plan::kHeldFactors ? which : 0][k];
+        }
+    };
+    constexpr int kP = 0, kQ = 1, kZ = 2;
+    Pair sums[Plan::kHeldSums ? 2 : 1][Plan::kHeldSums ? S::HALF : 1];
 #pragma unroll
-    for (int k = 0; k < (Plan::kSharedSums ? 1 : S::HALF); ++k) P[k] = Q[k] = both(0.f);
-#pragma unroll
-    for (int k = 0; k < S::HALF * ((Plan::kSharedSums ? 2 : 0) + (Plan::kSharedZ ? 1 : 0)); ++k)
-        mine[k * S::kThreads] = make_float2(0.f, 0.f);
+    for (int k = 0; k < S::HALF; ++k) {
+        if constexpr (Plan::kHeldSums)
+            sums[kP][k] = sums[kQ][k] = both(0.f);
+        else
+            mine[k * S::kThreads] = mine[(S::HALF + k) * S::kThreads] = make_float2(0.f, 0.f);
+        if (Plan::kSharedZ && p.need_z) mine[(Plan::kPlaceZ * S::HALF + k) * S::kThreads] = make_float2(0.f, 0.f);
+    }
     float* const part = p.partials + static_cast<size_t>(blockIdx.x) * 3 * dim;
     if (!Plan::kSharedZ && p.need_z)
         store_row<S>(part + 2 * static_cast<size_t>(dim), j, dim, [&](int) { return both(0.f); });
-    constexpr int kP = 0, kQ = 1, kZ = 2;
-    constexpr int kPlaceZ = Plan::kSharedSums ? 2 : 0;
-    auto add_sum = [&](Pair* regs, int which, int k, Pair a, Pair b) {  // += a b
-        if (!Plan::kSharedSums && which != kZ) {
-            regs[k] = fma2(a, b, regs[k]);
-        } else {
-            float2* at = mine + (which == kZ ? kPlaceZ : which) * kSumStride + k * S::kThreads;
-            const float2 f = *at;
-            *at = floats(fma2(a, b, f32x2::pk(f.x, f.y)));
+    auto add_sum = [&](int which, int k, Pair a, Pair b) {  // += a b
+        if constexpr (Plan::kHeldSums) {
+            if (which != kZ) {
+                sums[which][k] = fma2(a, b, sums[which][k]);
+                return;
+            }
         }
+        float2* const at = mine + ((which == kZ ? Plan::kPlaceZ : which) * S::HALF + k) * S::kThreads;
+        const float2 f = *at;
+        *at = floats(fma2(a, b, f32x2::pk(f.x, f.y)));
     };
 
-    for (int slot = 0; row < end; row += S::kRows, slot ^= 1) {
-        Row ahead;
-        if constexpr (!Plan::kLean) {
-            ahead = in;
-            if (row + S::kRows < end) load(row + S::kRows, ahead);
+    for (int slot = 0; n < last; n += S::kRows, slot ^= 1) {
+        const bool more = n + S::kRows < last;
+        Values<T, S> y_next, g_next;  // used first in the next row, and last in this one
+        y_next.clear();
+        if (more) {
+            load_y(y_next, g_next, S::kRows);
+            if (p.post_norm) next_ry = p.r_post[n + S::kRows];
+            if (p.d_normed) next_rs = p.r_pre[n + S::kRows];
         }
         Pair d[S::HALF];   // du, t, then t'
-        Pair sn[S::HALF];  // s r(s)
-        float dot = 0.f;
+        Pair sn[S::HALF];  // s r(s), then dx, dgate and y r(y)
         if (p.d_normed) {
 #pragma unroll
-            for (int k = 0; k < S::HALF; ++k) d[k] = in.du.pair(k);
+            for (int k = 0; k < S::HALF; ++k) d[k] = du.pair(k);
+            if (more) load_du(S::kRows);
             if constexpr (ROTATE) {
                 rotate_row<S>(d, exchange, j);
 #pragma unroll
@@ -654,186 +749,221 @@ __global__ void __launch_bounds__(S::kThreads, 1) block_norm_backward_kernel(Blo
             if (p.scales) {
                 load_vector<T, S>(p.scales, p.scales32, j, dim, 0.f, sn);
 #pragma unroll
-                for (int k = 0; k < S::HALF; ++k) sn[k] = mul2(sn[k], in.x.pair(k));
+                for (int k = 0; k < S::HALF; ++k) sn[k] = mul2(sn[k], x.pair(k));
             } else {
 #pragma unroll
-                for (int k = 0; k < S::HALF; ++k) sn[k] = mul2(both(p.scale), in.x.pair(k));
+                for (int k = 0; k < S::HALF; ++k) sn[k] = mul2(both(p.scale), x.pair(k));
             }
             if (p.y) {
-                Pair lw[kKeep ? 1 : S::HALF], la[kKeep ? 1 : S::HALF];
-                if constexpr (!kKeep) {
-                    load_vector<T, S>(p.post, p.post32, j, dim, 1.f, lw);
-                    gate_factor(la);
-                }
+                bring(0);
+                if (row_gate) {
+                    with_activation(p.act, [&](auto act) {
 #pragma unroll
-                for (int k = 0; k < S::HALF; ++k) {
-                    Pair f = kKeep ? kw[k] : lw[k];
-                    f = mul2(f, row_gate ? activation<false>(p.act, in.g.pair(k)) : kKeep ? ka[k] : la[k]);
-                    sn[k] = fma2(mul2(f, both(in.ry)), in.y.pair(k), sn[k]);
+                        for (int k = 0; k < S::HALF; ++k)
+                            sn[k] = fma2(mul2(mul2(factor(0, k), both(ry)), activation<false>(act, g.pair(k))),
+                                         y.pair(k), sn[k]);
+                    });
+                } else {
+#pragma unroll
+                    for (int k = 0; k < S::HALF; ++k)
+                        sn[k] = fma2(mul2(factor(0, k), both(ry)), y.pair(k), sn[k]);
                 }
             }
-            {
-                Pair lp[kKeep ? 1 : S::HALF];
-                if constexpr (!kKeep) load_vector<T, S>(p.pre, p.pre32, j, dim, 1.f, lp);
-                Pair sum = both(0.f);
+            bring(1);
+            Pair sum = both(0.f);
 #pragma unroll
-                for (int k = 0; k < S::HALF; ++k) {
-                    sn[k] = mul2(sn[k], both(in.rs));
-                    if (p.need_q) add_sum(Q, kQ, k, d[k], sn[k]);
-                    d[k] = mul2(d[k], kKeep ? kp[k] : lp[k]);
-                    sum = fma2(d[k], sn[k], sum);
-                }
-                dot = row_sum<S>(sum_of(sum), words, slot) * inv_dim;
+            for (int k = 0; k < S::HALF; ++k) {
+                sn[k] = mul2(sn[k], both(rs));
+                add_sum(kQ, k, d[k], sn[k]);
+                d[k] = mul2(d[k], factor(1, k));
+                sum = fma2(d[k], sn[k], sum);
             }
+            const Through through(p, row_sum<S>(sum_of(sum), words, slot) * inv_dim, rs);
             // dS
 #pragma unroll
             for (int k = 0; k < S::HALF; ++k)
-                d[k] = fma2(through_norm(p, d[k], sn[k], dot, in.rs), both(in.rs), in.ds.pair(k));
+                d[k] = fma2(fma2(sn[k], both(through.m), d[k]), both(through.r), ds.pair(k));
         } else {
 #pragma unroll
-            for (int k = 0; k < S::HALF; ++k) d[k] = in.ds.pair(k);
+            for (int k = 0; k < S::HALF; ++k) d[k] = ds.pair(k);
         }
-        {
-            if (p.scales) {
-                load_vector<T, S>(p.scales, p.scales32, j, dim, 0.f, sn);
-                if constexpr (Plan::kSharedZ) {
+        if (more) load_ds(S::kRows);
+        if (p.scales) {
+            load_vector<T, S>(p.scales, p.scales32, j, dim, 0.f, sn);
+            if constexpr (Plan::kSharedZ) {
 #pragma unroll
-                    for (int k = 0; k < S::HALF; ++k) add_sum(nullptr, kZ, k, d[k], in.x.pair(k));
-                } else {
-                    float* const z = part + 2 * static_cast<size_t>(dim);
-                    Values<float, S> old;
-                    old.load(z, j, dim);
-                    store_row<S>(z, j, dim, [&](int k) { return fma2(d[k], in.x.pair(k), old.pair(k)); });
-                }
-#pragma unroll
-                for (int k = 0; k < S::HALF; ++k) sn[k] = mul2(sn[k], d[k]);
+                for (int k = 0; k < S::HALF; ++k) add_sum(kZ, k, d[k], x.pair(k));
             } else {
+                float* const z = part + 2 * static_cast<size_t>(dim);
+                Values<float, S> old;
+                old.load(z, j, dim);
+                store_row<S>(z, j, dim, [&](int k) { return fma2(d[k], x.pair(k), old.pair(k)); });
+            }
 #pragma unroll
-                for (int k = 0; k < S::HALF; ++k) sn[k] = mul2(both(p.scale), d[k]);
-            }
-            store_row<S>(static_cast<R*>(p.d_x) + row * dim, j, dim, [&](int k) { return sn[k]; });
+            for (int k = 0; k < S::HALF; ++k) sn[k] = mul2(sn[k], d[k]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < S::HALF; ++k) sn[k] = mul2(both(p.scale), d[k]);
         }
+        if (more) load_x(S::kRows);
+        store_row<S>(at(static_cast<R*>(p.d_x), dim_bytes<R>(dim), 0), j, dim, [&](int k) { return sn[k]; });
         if (p.y) {
-            Pair lw[kKeep ? 1 : S::HALF], la[kKeep ? 1 : S::HALF];
-            if constexpr (!kKeep) {
-                load_vector<T, S>(p.post, p.post32, j, dim, 1.f, lw);
-                gate_factor(la);
-            }
+            bring(0);
             Pair sum = both(0.f);
             if (row_gate) {
+                with_activation(p.act, [&](auto act) {
 #pragma unroll
-                for (int k = 0; k < S::HALF; ++k) {
-                    const Pair w = kKeep ? kw[k] : lw[k], g = in.g.pair(k);
-                    const Pair yn = mul2(in.y.pair(k), both(in.ry));
-                    sn[k] = mul2(mul2(mul2(d[k], yn), w), activation<true>(p.act, g));  // dgate
-                    d[k] = mul2(d[k], activation<false>(p.act, g));                       // dn
-                    if (p.need_p) add_sum(P, kP, k, d[k], yn);
-                    d[k] = mul2(d[k], w);
-                    sum = fma2(d[k], yn, sum);
-                }
-                store_row<S>(static_cast<T*>(p.d_gate) + row * dim, j, dim, [&](int k) { return sn[k]; });
+                    for (int k = 0; k < S::HALF; ++k)  // dgate
+                        sn[k] = mul2(mul2(mul2(mul2(d[k], y.pair(k)), both(ry)), factor(0, k)),
+                                     activation<true>(act, g.pair(k)));
+                });
+                store_row<S>(at(static_cast<T*>(p.d_gate), dim_bytes<T>(dim), 0), j, dim, [&](int k) { return sn[k]; });
+                with_activation(p.act, [&](auto act) {
+#pragma unroll
+                    for (int k = 0; k < S::HALF; ++k) {
+                        sn[k] = mul2(y.pair(k), both(ry));
+                        d[k] = mul2(d[k], activation<false>(act, g.pair(k)));  // dn
+                        add_sum(kP, k, d[k], sn[k]);
+                        d[k] = mul2(d[k], factor(0, k));
+                        sum = fma2(d[k], sn[k], sum);
+                    }
+                });
             } else {
 #pragma unroll
                 for (int k = 0; k < S::HALF; ++k) {
-                    const Pair yn = mul2(in.y.pair(k), both(in.ry));
-                    if (p.need_p) add_sum(P, kP, k, d[k], yn);
-                    d[k] = mul2(d[k], mul2(kKeep ? kw[k] : lw[k], kKeep ? ka[k] : la[k]));
-                    sum = fma2(d[k], yn, sum);
+                    sn[k] = mul2(y.pair(k), both(ry));
+                    add_sum(kP, k, d[k], sn[k]);
+                    d[k] = mul2(d[k], factor(0, k));
+                    sum = fma2(d[k], sn[k], sum);
                 }
             }
             if (p.post_norm) {
-                const float mean = row_sum<S>(sum_of(sum), words, 2 + slot) * inv_dim;
+                const Through through(p, row_sum<S>(sum_of(sum), words, 2 + slot) * inv_dim, ry);
 #pragma unroll
                 for (int k = 0; k < S::HALF; ++k)
-                    d[k] = mul2(through_norm(p, d[k], mul2(in.y.pair(k), both(in.ry)), mean, in.ry), both(in.ry));
+                    d[k] = mul2(fma2(sn[k], both(through.m), d[k]), both(through.r));
             }
-            store_row<S>(static_cast<T*>(p.d_y) + row * dim, j, dim, [&](int k) { return d[k]; });
+            store_row<S>(at(static_cast<T*>(p.d_y), dim_bytes<T>(dim), 0), j, dim, [&](int k) { return d[k]; });
         }
-        if constexpr (Plan::kLean) {
-            if (row + S::kRows < end) load(row + S::kRows, in);
-        } else {
-            in = ahead;
-        }
+        y = y_next;
+        g = g_next;
+        ry = next_ry;
+        rs = next_rs;
     }
     // The CTA's sums; rows side by side in a CTA are added first, in shared memory.
-    auto write = [&](Pair* regs, int which, float* dst) {
-        const bool held = !Plan::kSharedSums && which != kZ;  // in registers
-        float2* const at = mine + (which == kZ ? kPlaceZ : Plan::kSharedSums ? which : 0) * kSumStride;
+    auto write = [&](int which, float* dst) {
+        const bool in_registers = Plan::kHeldSums && which != kZ;
+        float2* const place = mine + (which == kZ ? Plan::kPlaceZ : in_registers ? 0 : which) * S::HALF * S::kThreads;
         Pair v[S::HALF];
-        if (held && S::kRows > 1) {
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < S::HALF; ++k) at[k * S::kThreads] = floats(regs[k]);
-        }
         if constexpr (S::kRows > 1) {
             __syncthreads();
+            if (in_registers) {
+#pragma unroll
+                for (int k = 0; k < S::HALF; ++k)
+                    place[k * S::kThreads] = floats(sums[Plan::kHeldSums ? which & 1 : 0][Plan::kHeldSums ? k : 0]);
+                __syncthreads();
+            }
             if (sub > 0) return;
         }
 #pragma unroll
         for (int k = 0; k < S::HALF; ++k) {
-            if (held && S::kRows == 1) {
-                v[k] = regs[k];
+            if (in_registers && S::kRows == 1) {
+                v[k] = sums[Plan::kHeldSums ? which & 1 : 0][Plan::kHeldSums ? k : 0];
             } else {
                 v[k] = both(0.f);
                 for (int o = 0; o < S::kRows; ++o) {
-                    const float2 f = at[k * S::kThreads + o * S::TPR];
+                    const float2 f = place[k * S::kThreads + o * S::TPR];
                     v[k] = add2(v[k], f32x2::pk(f.x, f.y));
                 }
             }
         }
         store_row<S>(dst, j, dim, [&](int k) { return v[k]; });
     };
-    if (Plan::kSharedZ && p.need_z) write(nullptr, kZ, part + 2 * static_cast<size_t>(dim));
-    if (p.need_p) write(P, kP, part);
-    if (p.need_q) write(Q, kQ, part + dim);
+    if (Plan::kSharedZ && p.need_z) write(kZ, part + 2 * static_cast<size_t>(dim));
+    if (p.need_p) write(kP, part);
+    if (p.need_q) write(kQ, part + dim);
 }
 
-// The gradients of the per-channel vectors from the CTAs' sums: 32 columns
-// per CTA, 32 slices of the parts, added in a fixed order.  blockIdx.y: 0
-// d_pre, 1 d_post, 2 d_scale, 3 + g the gate row of group g.
+// The gradients of the per-channel vectors from the CTAs' sums, added in a
+// fixed order: 32 columns per CTA, four a thread, in 32 slices of the parts.
+// blockIdx.y: 0 Q -> d_pre, 1 Z -> d_scale, 2 P -> d_post, and the gate's
+// gradient where one gate row serves all; 3 + g that of group g.
 template <typename T>
-__global__ void __launch_bounds__(1024) block_norm_sums_kernel(BlockNormArgs p, int parts) {
-    __shared__ float slice[32][33];
+__global__ void __launch_bounds__(256) block_norm_sums_kernel(BlockNormArgs p, int parts) {
+    __shared__ float slice[32][36];
     pdl_begin();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int col = blockIdx.x * 32 + lane;
     const unsigned what = blockIdx.y;
-    void* out = what == 0 ? p.d_pre : what == 1 ? p.d_post : what == 2 ? p.d_scale : p.d_gate;
-    if (!out || (what > 2 && (p.gate_mode == kGateFull || p.gate_mode == kGateNone))) return;
-    const float* src = p.partials + (what == 0 ? 1 : what == 2 ? 2 : 0) * static_cast<size_t>(p.dim) + col;
-    const int first = what > 2 ? static_cast<int>(what - 3) * p.parts_per_group : 0;
-    const int last = what > 2 ? first + p.parts_per_group : parts;
+    if ((what == 0 && !p.need_q) || (what == 1 && !p.need_z) || (what >= 2 && !p.need_p)) return;
+    const int quad = threadIdx.x & 7, part = threadIdx.x >> 3;
+    const int col = blockIdx.x * 32 + 4 * quad;
+    const bool grouped = p.gate_mode == kGateGroups;
     auto vector_at = [&](const void* v, bool is32, size_t at) {
         return is32 || sizeof(T) == 4 ? static_cast<const float*>(v)[at]
                                       : Convert<T, float>::load(static_cast<const T*>(v)[at]);
     };
-    float sum = 0.f;
-    if (col < p.dim)
-        for (int k = first + warp; k < last; k += 32) {
-            float v = src[static_cast<size_t>(k) * 3 * p.dim];
-            if (what == 1 && (p.gate_mode == kGateChannel || p.gate_mode == kGateGroups)) {
-                const size_t g = p.gate_mode == kGateGroups ? static_cast<size_t>(k / p.parts_per_group) * p.gate_row : 0;
-                v *= activation<false>(p.act, vector_at(p.gate, p.gate32, g + col));
-            }
-            sum += v;
+    const float* src = p.partials + (what == 0 ? 1 : what == 1 ? 2 : 0) * static_cast<size_t>(p.dim) + col;
+    const int first = what > 2 ? static_cast<int>(what - 3) * p.parts_per_group : 0;
+    const int last = what > 2 ? first + p.parts_per_group : parts;
+    const size_t step = 3 * static_cast<size_t>(p.dim);
+    const bool vec = p.dim % 4 == 0;  // the workspace is 16-byte aligned
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](int k, float4& to) {
+        const float* q = src + k * step;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (vec) {
+            if (col < p.dim) v = __ldcg(reinterpret_cast<const float4*>(q));
+        } else {
+            if (col < p.dim) v.x = q[0];
+            if (col + 1 < p.dim) v.y = q[1];
+            if (col + 2 < p.dim) v.z = q[2];
+            if (col + 3 < p.dim) v.w = q[3];
         }
-    slice[warp][lane] = sum;
-    __syncthreads();
-    if (warp > 0 || col >= p.dim) return;
-    sum = 0.f;
-    for (int k = 0; k < 32; ++k) sum += slice[k][lane];
-    size_t at = col;
-    bool is32 = what == 0 ? p.pre32 : what == 1 ? p.post32 : what == 2 ? p.scales32 : p.gate32;
-    if (what > 2) {
-        const size_t g = p.gate_mode == kGateGroups ? static_cast<size_t>(what - 3) * p.gate_row : 0;
-        if (p.post) sum *= vector_at(p.post, p.post32, col);
-        sum *= activation<true>(p.act, vector_at(p.gate, p.gate32, g + col));
-        at += static_cast<size_t>(what - 3) * p.dim;
+        if (what == 2 && grouped) {  // d_post: each group's own gate
+            const size_t g = static_cast<size_t>(k / p.parts_per_group) * p.gate_row;
+            if (col < p.dim) v.x *= activation<false>(p.act, vector_at(p.gate, p.gate32, g + col));
+            if (col + 1 < p.dim) v.y *= activation<false>(p.act, vector_at(p.gate, p.gate32, g + col + 1));
+            if (col + 2 < p.dim) v.z *= activation<false>(p.act, vector_at(p.gate, p.gate32, g + col + 2));
+            if (col + 3 < p.dim) v.w *= activation<false>(p.act, vector_at(p.gate, p.gate32, g + col + 3));
+        }
+        to.x += v.x;
+        to.y += v.y;
+        to.z += v.z;
+        to.w += v.w;
+    };
+    float4 other = sum;
+    int k = first + part;
+#pragma unroll 2
+    for (; k + 32 < last; k += 64) {
+        add(k, sum);
+        add(k + 32, other);
     }
-    if (is32 || sizeof(T) == 4)
-        static_cast<float*>(out)[at] = sum;
-    else
-        static_cast<T*>(out)[at] = Convert<T, float>::store(sum);
+    if (k < last) add(k, sum);
+    *reinterpret_cast<float4*>(&slice[part][4 * quad]) =
+        make_float4(sum.x + other.x, sum.y + other.y, sum.z + other.z, sum.w + other.w);
+    __syncthreads();
+    const int lane = threadIdx.x, c = blockIdx.x * 32 + lane;
+    if (lane >= 32 || c >= p.dim) return;
+    float total = 0.f;
+#pragma unroll
+    for (int q = 0; q < 32; ++q) total += slice[q][lane];
+    auto write = [&](void* out, bool is32, size_t at, float v) {
+        if (!out) return;
+        if (is32 || sizeof(T) == 4)
+            static_cast<float*>(out)[at] = v;
+        else
+            static_cast<T*>(out)[at] = Convert<T, float>::store(v);
+    };
+    if (what == 0) return write(p.d_pre, p.pre32, c, total);
+    if (what == 1) return write(p.d_scale, p.scales32, c, total);
+    const bool channel = p.gate_mode == kGateChannel;
+    if (channel || what > 2) {
+        const size_t row = what > 2 ? what - 3 : 0;
+        const float g = vector_at(p.gate, p.gate32, row * p.gate_row + c);
+        const float w = p.post ? vector_at(p.post, p.post32, c) : 1.f;
+        write(p.d_gate, p.gate32, row * p.dim + c, total * w * activation<true>(p.act, g));
+        if (channel) total *= activation<false>(p.act, g);
+    }
+    if (what == 2) write(p.d_post, p.post32, c, total);
 }
 
 }  // namespace cubf::norm

@@ -64,7 +64,7 @@ enum GateMode : int { kGateNone = 0, kGateChannel = 1, kGateGroups = 2, kGateFul
 constexpr int kBlockNormMaxDim = 16384;
 constexpr int kBlockNormMinRotate = 64;   // rotated rows: powers of two from here
 
-// Row strides in elements; outputs and gradients are contiguous.  The
+// Outputs and gradients are contiguous.  The
 // per-channel vectors are in the block's type or, flagged, in fp32.
 struct BlockNormArgs {
     const void* x;              // residual type
@@ -75,7 +75,9 @@ struct BlockNormArgs {
     const void* scales;         // residual scale per channel, or null: `scale`
     const void* d_residual;     // or null: zero
     const void* d_normed;       // or null: zero
-    size_t x_row, y_row, gate_row, d_residual_row, d_normed_row;
+    size_t gate_row;            // elements, of a gate per group
+    // from a row to the next, in bytes
+    uint32_t x_bytes, y_bytes, gate_bytes, d_residual_bytes, d_normed_bytes;
     void* residual;             // or null: not written
     void* normed;               // or null: no norm of the sum
     float* r_post;              // r(y) and r(s) of every row, kept for the backward; or null

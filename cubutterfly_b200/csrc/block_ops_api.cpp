@@ -129,9 +129,15 @@ cubf::BlockNormArgs norm_args(const cubutterflyB200BlockNorm_t* a, bool backward
     n.pre = a->pre_weight;
     n.post = a->post_weight;
     n.scales = a->scale;
-    n.x_row = a->x_row;
-    n.y_row = a->y ? a->y_row : 0;
+    // a row's place is one 32 x 32 bit product
+    auto bytes = [](size_t elements, size_t size) {
+        supported(elements <= 0xffffffffULL / size, "block norm: a row stride is limited to 4 GiB");
+        return static_cast<uint32_t>(elements * size);
+    };
+    n.x_bytes = bytes(a->x_row, er);
+    n.y_bytes = a->y ? bytes(a->y_row, es) : 0;
     n.gate_row = a->gate_rows > 1 ? a->gate_row : 0;
+    n.gate_bytes = bytes(n.gate_row, es);
     n.rows = a->rows;
     n.dim = static_cast<int>(a->dim);
     n.act = a->activation;
@@ -186,8 +192,8 @@ cubf::BlockNormArgs norm_args(const cubutterflyB200BlockNorm_t* a, bool backward
             "block norm: misaligned gradient");
     n.d_residual = a->d_residual;
     n.d_normed = a->d_normed;
-    n.d_residual_row = a->d_residual ? a->d_residual_row : 0;
-    n.d_normed_row = a->d_normed ? a->d_normed_row : 0;
+    n.d_residual_bytes = a->d_residual ? bytes(a->d_residual_row, er) : 0;
+    n.d_normed_bytes = a->d_normed ? bytes(a->d_normed_row, es) : 0;
     n.r_post = a->post_rms;
     n.r_pre = a->pre_rms;
     n.d_x = a->d_x;

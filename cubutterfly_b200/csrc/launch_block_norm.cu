@@ -28,6 +28,11 @@ constexpr int kType = CUBF_BN_TYPE;
 using T = std::conditional_t<kType <= 1, __half, std::conditional_t<kType <= 3, __nv_bfloat16, float>>;
 using R = std::conditional_t<kType == 1 || kType == 3 || kType == 4, float, T>;
 constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+// values a thread of the backward: 16 fit the registers where every tensor is 16-bit
+#ifndef WIDE
+#define WIDE 16
+#endif
+constexpr int kWide = sizeof(R) == 2 ? WIDE : 8;
 
 // Whole 16-byte vectors everywhere: every pointer aligned, every row stride
 // and the row length a multiple of the vector.
@@ -38,8 +43,8 @@ bool aligned(const BlockNormArgs& a) {
                           static_cast<const void*>(a.d_x), static_cast<const void*>(a.d_y),
                           static_cast<const void*>(a.d_gate), static_cast<const void*>(a.partials)})
         bits |= reinterpret_cast<uintptr_t>(p) & 15u;
-    for (size_t s : {a.x_row, a.y_row, a.gate_row, a.d_residual_row, a.d_normed_row, static_cast<size_t>(a.dim)})
-        bits |= s & (kVec - 1);
+    for (uint32_t s : {a.x_bytes, a.y_bytes, a.gate_bytes, a.d_residual_bytes, a.d_normed_bytes}) bits |= s & 15u;
+    bits |= (a.gate_row | static_cast<size_t>(a.dim)) & (kVec - 1);
     return bits == 0;
 }
 
@@ -51,10 +56,15 @@ cudaError_t run(const BlockNormArgs& a, size_t groups, cudaStream_t stream) {
 #else
     auto kernel = &block_norm_kernel<T, R, S, ROTATE>;
 #endif
-    using Plan = std::conditional_t<CUBF_BN_BACKWARD, BackwardPlan<S, ROTATE>, ForwardPlan<S, ROTATE>>;
-    constexpr int smem = 4 * Plan::kFloats;
+#if CUBF_BN_BACKWARD
+    using Plan = BackwardPlan<S, ROTATE>;
+    const int smem = 4 * Plan::floats_needed(a.need_z);
+    constexpr int most = 4 * Plan::floats_needed(true);
+#else
+    constexpr int smem = 4 * ForwardPlan<S, ROTATE>::kFloats, most = smem;
+#endif
     int cap = 0;
-    cudaError_t e = setup_kernel(setup, kernel, S::kThreads, smem, &cap);
+    cudaError_t e = setup_kernel(setup, kernel, S::kThreads, most, &cap, CUBF_BN_BACKWARD);
     if (e != cudaSuccess) return e;
 #if CUBF_BN_BACKWARD
     (void)cap;
@@ -81,10 +91,10 @@ cudaError_t dispatch(const BlockNormArgs& a, size_t groups, cudaStream_t s) {
 #if CUBF_BN_BACKWARD
             switch (d) {
                 case 256: return shape<32, 8, V, true, 512>(a, groups, s);
-                case 512: return shape<64, 8, V, true, 512>(a, groups, s);
-                case 1024: return shape<128, 8, V, true, 512>(a, groups, s);
-                case 2048: return shape<256, 8, V, true, 512>(a, groups, s);
-                case 4096: return shape<512, 8, V, true>(a, groups, s);
+                case 512: return shape<512 / kWide, kWide, V, true, 512>(a, groups, s);
+                case 1024: return shape<1024 / kWide, kWide, V, true, 512>(a, groups, s);
+                case 2048: return shape<2048 / kWide, kWide, V, true, 512>(a, groups, s);
+                case 4096: return shape<4096 / kWide, kWide, V, true, 512>(a, groups, s);
                 case 8192: return shape<512, 16, V, true>(a, groups, s);
                 case 16384: return shape<1024, 16, V, true>(a, groups, s);
             }
@@ -124,16 +134,23 @@ cudaError_t dispatch(const BlockNormArgs& a, size_t groups, cudaStream_t s) {
     }
 #if CUBF_BN_BACKWARD
     constexpr int kThreads = 512;  // rows side by side, so that there is one part of the sums per SM
+    if (vec) {
+        if (d <= 256) return shape<32, 8, V, false, 512>(a, groups, s);
+        if (d <= 512) return shape<512 / kWide, kWide, V, false, 512>(a, groups, s);
+        if (d <= 1024) return shape<1024 / kWide, kWide, V, false, 512>(a, groups, s);
+        if (d <= 2048) return shape<2048 / kWide, kWide, V, false, 512>(a, groups, s);
+        if (d <= 4096) return shape<4096 / kWide, kWide, V, false, 512>(a, groups, s);
+        if (d <= 8192) return shape<8192 / kWide, kWide, V, false>(a, groups, s);
 #else
     constexpr int kThreads = 0;
-#endif
     if (vec) {
-        if (d <= 256) return shape<32, 8, V, false, kThreads>(a, groups, s);
-        if (d <= 512) return shape<64, 8, V, false, kThreads>(a, groups, s);
-        if (d <= 1024) return shape<128, 8, V, false, kThreads>(a, groups, s);
-        if (d <= 2048) return shape<256, 8, V, false, kThreads>(a, groups, s);
+        if (d <= 256) return shape<32, 8, V, false>(a, groups, s);
+        if (d <= 512) return shape<64, 8, V, false>(a, groups, s);
+        if (d <= 1024) return shape<128, 8, V, false>(a, groups, s);
+        if (d <= 2048) return shape<256, 8, V, false>(a, groups, s);
         if (d <= 4096) return shape<512, 8, V, false>(a, groups, s);
         if (d <= 8192) return shape<1024, 8, V, false>(a, groups, s);
+#endif
         if (d <= kBlockNormMaxDim) return shape<1024, 16, V, false>(a, groups, s);
     } else {
         if (d <= 256) return shape<32, 8, 1, false, kThreads>(a, groups, s);
@@ -151,10 +168,9 @@ template <>
 cudaError_t launch_block_norm_backward_unit<CUBF_BN_TYPE>(const BlockNormArgs& a, size_t groups, cudaStream_t stream) {
     cudaError_t e = dispatch(a, groups, stream);
     if (e != cudaSuccess || !(a.need_p || a.need_q || a.need_z)) return e;
-    const bool per_group = a.gate_mode == kGateChannel || a.gate_mode == kGateGroups;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>((a.dim + 31) / 32), 3u + (per_group ? static_cast<unsigned>(groups) : 0u));
-    cfg.blockDim = dim3(1024);
+    cfg.gridDim = dim3(static_cast<unsigned>((a.dim + 31) / 32), 3u + (a.gate_mode == kGateGroups ? static_cast<unsigned>(groups) : 0u));
+    cfg.blockDim = dim3(256);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
