@@ -426,7 +426,7 @@ struct ForwardPlan {
     // 16-bit rows of eight values a thread fit 1024 threads an SM
     template <typename T, typename R>
     static constexpr int ctas() {
-        return S::EPT == 8 && S::VW == 8 && sizeof(R) == 2 && !ROTATE && S::kThreads < 1024 ? 1024 / S::kThreads : 1;
+        return S::EPT == 8 && S::VW == 8 && !ROTATE && S::kThreads < 1024 ? 1024 / S::kThreads : 1;
     }
 };
 

@@ -105,8 +105,8 @@ cudaError_t dispatch(const BlockNormArgs& a, size_t groups, cudaStream_t s) {
                     case 512: return shape<32, 16, V, true>(a, groups, s);
                     case 1024: return shape<32, 32, V, true, 256>(a, groups, s);
                     case 2048: return shape<64, 32, V, true, 512>(a, groups, s);
-                    case 4096: return shape<64, 64, V, true, 384>(a, groups, s);
-                    case 8192: return shape<128, 64, V, true, 384>(a, groups, s);
+                    case 4096: return shape<128, 32, V, true, 512>(a, groups, s);
+                    case 8192: return shape<256, 32, V, true, 512>(a, groups, s);
                     case 16384: return shape<512, 32, V, true>(a, groups, s);
                 }
             }
