@@ -62,11 +62,6 @@ struct Raw {
     static CUBF_DEV Word zero() { return 0u; }
     static CUBF_DEV Word lowest() { return std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u; }  // -inf
     static CUBF_DEV Word vec(const T* p) { return __ldcs(reinterpret_cast<const unsigned int*>(p)); }
-    static CUBF_DEV Word two(const T* p, int apart, bool ok0, bool ok1) {
-        const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
-        const uint32_t lo = ok0 ? __ldcs(q) : 0u, hi = ok1 ? __ldcs(q + apart) : 0u;
-        return lo | (hi << 16);
-    }
     static CUBF_DEV Pair get(Word w) {
         if constexpr (std::is_same<T, __half>::value) {
             __half2 h;
@@ -95,79 +90,75 @@ struct Raw<float> {
     static CUBF_DEV Word zero() { return make_float2(0.f, 0.f); }
     static CUBF_DEV Word lowest() { return make_float2(-INFINITY, -INFINITY); }
     static CUBF_DEV Word vec(const float* p) { return __ldcs(reinterpret_cast<const float2*>(p)); }
-    static CUBF_DEV Word two(const float* p, int apart, bool ok0, bool ok1) {
-        return make_float2(ok0 ? __ldcs(p) : 0.f, ok1 ? __ldcs(p + apart) : 0.f);
-    }
     static CUBF_DEV Pair get(Word w) { return pair(w); }
     static CUBF_DEV Word word_of(float2 f) { return f; }
     static CUBF_DEV void store_vec(float* p, float2 f) { __stcs(reinterpret_cast<float2*>(p), f); }
 };
 
-// How a kernel reaches its rows, by the alignment of every row of every
-// tensor: copied to shared memory in 16-byte pieces ahead of their use; pair
-// by pair; or value by value.
-enum Access : int { kScalar = 0, kPairs = 1, kAsync = 2 };
-
-// The lane's two channels: adjacent with pair accesses, else as far apart as
-// its group has lanes, so that scalar accesses still coalesce.
-// Lanes of a group are adjacent; groups hold consecutive runs of tokens.
-template <Access ACCESS, int GROUPS>
+// The lane's two channels of a row, which are adjacent.  Lanes of a group are
+// adjacent; groups hold consecutive runs of tokens.
+template <int GROUPS>
 struct Lane {
-    static constexpr bool VEC = ACCESS != kScalar;
     static constexpr int kLanes = 32 / GROUPS;
     int ch;
     bool ok0, ok1;
     CUBF_DEV Lane(int c0, int lane, int dim) {
-        ch = c0 + (VEC ? 2 : 1) * (lane % kLanes);
+        ch = c0 + 2 * (lane % kLanes);
         ok0 = ch < dim;
-        ok1 = VEC ? ok0 : ch + kLanes < dim;
-    }
-    template <typename T>
-    CUBF_DEV typename Raw<T>::Word load(const T* row) const {
-        if constexpr (VEC)
-            return ok0 ? Raw<T>::vec(row + ch) : Raw<T>::zero();
-        else
-            return Raw<T>::two(row + ch, kLanes, ok0, ok1);
-    }
-    template <typename T>
-    CUBF_DEV void store(T* row, Pair p) const {
-        const float2 f = floats(p);
-        if constexpr (VEC) {
-            if (ok0) Raw<T>::store_vec(row + ch, f);
-        } else {
-            if (ok0) row[ch] = Convert<T, float>::store(f.x);
-            if (ok1) row[ch + kLanes] = Convert<T, float>::store(f.y);
-        }
+        ok1 = ch + 1 < dim;
     }
     CUBF_DEV Pair load32(const float* row) const {
-        return f32x2::pk(ok0 ? row[ch] : 0.f, ok1 ? row[ch + (VEC ? 1 : kLanes)] : 0.f);
+        return f32x2::pk(ok0 ? row[ch] : 0.f, ok1 ? row[ch + 1] : 0.f);
     }
     CUBF_DEV void store32(float* row, Pair p) const {
         const float2 f = floats(p);
         if (ok0) row[ch] = f.x;
-        if (ok1) row[ch + (VEC ? 1 : kLanes)] = f.y;
+        if (ok1) row[ch + 1] = f.y;
+    }
+    // rows of T, pair by pair where they are aligned for it
+    template <bool PAIRS, typename T>
+    CUBF_DEV Pair load(const T* row) const {
+        if constexpr (PAIRS)
+            return Raw<T>::get(ok0 ? Raw<T>::vec(row + ch) : Raw<T>::zero());
+        else
+            return f32x2::pk(ok0 ? Convert<T, float>::load(row[ch]) : 0.f, ok1 ? Convert<T, float>::load(row[ch + 1]) : 0.f);
+    }
+    template <bool PAIRS, typename T>
+    CUBF_DEV void store(T* row, Pair p) const {
+        const float2 f = floats(p);
+        if constexpr (PAIRS) {
+            if (ok0) Raw<T>::store_vec(row + ch, f);
+        } else {
+            if (ok0) row[ch] = Convert<T, float>::store(f.x);
+            if (ok1) row[ch + 1] = Convert<T, float>::store(f.y);
+        }
     }
 };
 
 // The rows of a warp's tokens: N tensors of GROUPS x STEPS tokens x CHANNELS
-// channels.  With kAsync a warp copies its own rows into its own shared
-// memory (no barrier beyond the warp's), STAGES tiles deep: the copies of a
-// later tile are in flight while this one is worked on, and hold no registers.
-// Token g STEPS + s lies at row s GROUPS + g, so that the lanes of all groups
-// read adjacent words.  Results take the place of words that have been read
-// and leave in 16-byte pieces: stored from registers, each pair would cost as
-// many instructions in addresses as its arithmetic.  Channels past the end are
-// zero; tokens past the end are what `tail` says.
-template <typename T, int N, int STEPS_, int STAGES_, int GROUPS, Access ACCESS>
+// channels.  A warp copies its own rows into its own shared memory (no barrier
+// beyond the warp's), STAGES tiles deep: the copies of a later tile are in
+// flight while this one is worked on, and hold no registers.  Token g STEPS + s
+// lies at row s GROUPS + g, so that the lanes of all groups read adjacent
+// words.  Results take the place of words that have been read and leave the
+// same way: stored from registers, each pair would cost as many instructions in
+// addresses as its arithmetic.  Rows are copied in pieces of PIECE bytes, what
+// every row of every tensor is aligned for: 16 and 4 asynchronously, 2 (rows of
+// an odd number of 16-bit values) through registers.  Channels past the end are
+// zero; tokens past the end are what `close` says.
+template <typename T, int N, int STEPS_, int STAGES_, int GROUPS, int PIECE>
 struct Rows {
     static constexpr int STEPS = STEPS_, STAGES = STAGES_, TOKENS = STEPS * GROUPS;
     static constexpr int kChannels = kWarpChannels / GROUPS;
     static constexpr int kRowBytes = kChannels * static_cast<int>(sizeof(T));
     static constexpr int kTensorBytes = TOKENS * kRowBytes;
-    static constexpr int kBytes = ACCESS == kAsync ? N * kTensorBytes : 0;
-    static constexpr int kPerRow = kRowBytes / 16;        // 16-byte pieces of a row
-    static constexpr int kRowsPer = 32 / kPerRow;         // rows a warp copies at a time
-    static constexpr int kCopies = TOKENS / kRowsPer;     // per lane and tensor
+    static constexpr int kBytes = N * kTensorBytes;
+    static constexpr int kPerRow = kRowBytes / PIECE;                     // pieces of a row
+    static constexpr int kAcross = kPerRow < 32 ? kPerRow : 32;           // lanes along a row
+    static constexpr int kRowsPer = 32 / kAcross;                         // rows a warp copies at a time
+    static constexpr int kTimes = kPerRow / kAcross;                      // pieces a lane copies of a row
+    static constexpr int kCopies = TOKENS / kRowsPer;                     // rows a lane copies of a tensor
+    static constexpr int kElements = PIECE / static_cast<int>(sizeof(T));
     using Word = typename Raw<T>::Word;
     const T* base[N];
     size_t stride[N];
@@ -175,11 +166,11 @@ struct Rows {
     unsigned char* mine;  // this warp's stages
     int lane, c0, length, dim;
 
-    CUBF_DEV int piece() const { return lane % kPerRow * (16 / static_cast<int>(sizeof(T))); }
+    CUBF_DEV int column() const { return c0 + lane % kAcross * kElements; }
     // where this lane's piece of the k-th rows lies: what follows from the lane, and from k
     CUBF_DEV int piece_place() const {
-        const int r = lane / kPerRow;
-        return (r % STEPS * GROUPS + r / STEPS) * kRowBytes + lane % kPerRow * 16;
+        const int r = lane / kAcross;
+        return (r % STEPS * GROUPS + r / STEPS) * kRowBytes + lane % kAcross * PIECE;
     }
     static constexpr int row_place(int k) {
         return (k * kRowsPer % STEPS * GROUPS + k * kRowsPer / STEPS) * kRowBytes;
@@ -191,12 +182,10 @@ struct Rows {
         c0 = c0_;
         length = length_;
         dim = dim_;
-        if constexpr (ACCESS == kAsync) {
 #pragma unroll
-            for (int n = 0; n < N; ++n)
-                next[n] = base[n] + static_cast<ptrdiff_t>(first + lane / kPerRow) * static_cast<ptrdiff_t>(stride[n]) +
-                          c0 + piece();
-        }
+        for (int n = 0; n < N; ++n)
+            next[n] = base[n] + static_cast<ptrdiff_t>(first + lane / kAcross) * static_cast<ptrdiff_t>(stride[n]) +
+                      column();
     }
     CUBF_DEV Word* word(int stage, int n, int s) const {  // of the lane's own token s
         return reinterpret_cast<Word*>(mine + stage * kBytes + n * kTensorBytes + s * GROUPS * kRowBytes) + lane;
@@ -204,96 +193,99 @@ struct Rows {
     // starts the copies of tokens [t, t + TOKENS), closes their group, and
     // moves on by `advance` tokens
     CUBF_DEV void fetch(int stage, int t, int advance) {
-        if constexpr (ACCESS == kAsync) {
-            const uint32_t dst =
-                static_cast<uint32_t>(__cvta_generic_to_shared(mine + stage * kBytes)) + piece_place();
-            if (t >= 0 && t + TOKENS <= length && c0 + kChannels <= dim) {
+        unsigned char* const to = mine + stage * kBytes + piece_place();
+        const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+        if (t >= 0 && t + TOKENS <= length && c0 + kChannels <= dim) {
 #pragma unroll
-                for (int n = 0; n < N; ++n) {
-                    const T* src = next[n];
+            for (int n = 0; n < N; ++n) {
+                const T* src = next[n];
 #pragma unroll
-                    for (int k = 0; k < kCopies; ++k) {
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + n * kTensorBytes +
-                                                                                      row_place(k)),
-                                     "l"(src)
-                                     : "memory");
-                        src += kRowsPer * stride[n];
+                for (int k = 0; k < kCopies; ++k) {
+#pragma unroll
+                    for (int m = 0; m < kTimes; ++m) {
+                        const int place = n * kTensorBytes + row_place(k) + m * 32 * PIECE;
+                        if constexpr (PIECE == 16)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + place), "l"(src)
+                                         : "memory");
+                        else if constexpr (PIECE == 4)
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + place),
+                                         "l"(src + m * 32 * kElements)
+                                         : "memory");
+                        else
+                            *reinterpret_cast<unsigned short*>(to + place) =
+                                __ldcs(reinterpret_cast<const unsigned short*>(src + m * 32 * kElements));
                     }
+                    src += kRowsPer * stride[n];
                 }
-            } else if (t < length && t + TOKENS > 0) {
-#pragma unroll
-                for (int n = 0; n < N; ++n)
-#pragma unroll
-                    for (int k = 0; k < kCopies; ++k) {
-                        const int at = t + lane / kPerRow + k * kRowsPer, col = c0 + piece();
-                        const bool in = at >= 0 && at < length && col < dim;
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + n * kTensorBytes +
-                                                                                          row_place(k)),
-                                     "l"(in ? base[n] + static_cast<size_t>(at) * stride[n] + col : base[n]),
-                                     "r"(in ? 16 : 0)
-                                     : "memory");
-                    }
-            } else {
-                // nothing of the sequence: zeros, so that no stale word is computed with
-                for (int k = 0; k < N * kCopies; ++k)
-                    *reinterpret_cast<uint4*>(mine + stage * kBytes + lane * 16 + k * 512) = make_uint4(0, 0, 0, 0);
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
+        } else if (t < length && t + TOKENS > 0) {
+            for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int n = 0; n < N; ++n) next[n] += static_cast<ptrdiff_t>(advance) * static_cast<ptrdiff_t>(stride[n]);
+                for (int k = 0; k < kCopies; ++k)
+#pragma unroll
+                    for (int m = 0; m < kTimes; ++m) {
+                        const int at = t + lane / kAcross + k * kRowsPer, col = column() + m * 32 * kElements;
+                        const bool in = at >= 0 && at < length && col < dim;
+                        const T* src = in ? base[n] + static_cast<size_t>(at) * stride[n] + col : base[n];
+                        const int place = n * kTensorBytes + row_place(k) + m * 32 * PIECE;
+                        if constexpr (PIECE == 16)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + place), "l"(src),
+                                         "r"(in ? 16 : 0)
+                                         : "memory");
+                        else if constexpr (PIECE == 4)
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + place), "l"(src),
+                                         "r"(in ? 4 : 0)
+                                         : "memory");
+                        else
+                            *reinterpret_cast<unsigned short*>(to + place) =
+                                in ? __ldcs(reinterpret_cast<const unsigned short*>(src)) : static_cast<unsigned short>(0);
+                    }
+        } else {
+            // nothing of the sequence: zeros, so that no stale word is computed with
+            for (int k = 0; k < kBytes / 512; ++k)
+                *reinterpret_cast<uint4*>(mine + stage * kBytes + lane * 16 + k * 512) = make_uint4(0, 0, 0, 0);
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll
+        for (int n = 0; n < N; ++n) next[n] += static_cast<ptrdiff_t>(advance) * static_cast<ptrdiff_t>(stride[n]);
     }
     // waits for the oldest of STAGES groups
     CUBF_DEV void arrive() const {
-        if constexpr (ACCESS == kAsync) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-            __syncwarp();
-        }
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        __syncwarp();
     }
-    // The lane's token t + s (t the first of its run).
-    CUBF_DEV Word get(const Lane<ACCESS, GROUPS>& ln, int stage, int n, int t, int s, Word tail) const {
-        if constexpr (ACCESS == kAsync)
-            return *word(stage, n, s);
-        else
-            return t + s < length ? ln.load(base[n] + static_cast<size_t>(t + s) * stride[n]) : tail;
-    }
-    // gives tokens past the end the value `tail` (async copies leave zeros there)
+    // The lane's token s.
+    CUBF_DEV Pair get(int stage, int n, int s) const { return Raw<T>::get(*word(stage, n, s)); }
+    // gives the lane's tokens past the end, its run beginning at t, the value
+    // `tail` (the copies leave zeros there)
     CUBF_DEV void close(int stage, int n, int t, Word tail) const {
-        if constexpr (ACCESS == kAsync) {
-            if (t + STEPS <= length) return;
-            for (int s = 0; s < STEPS; ++s)
-                if (t + s >= length) *word(stage, n, s) = tail;
-        }
+        if (t + STEPS <= length) return;
+        for (int s = 0; s < STEPS; ++s)
+            if (t + s >= length) *word(stage, n, s) = tail;
     }
-    // Token t + s of an output (rows of `dim` channels from `out`): into the
-    // place of tensor n's word, or straight to memory.  The caller has checked
-    // that the token exists unless ACCESS is kAsync.
-    CUBF_DEV void put(const Lane<ACCESS, GROUPS>& ln, int stage, int n, T* out, int t, int s, Pair v) const {
-        if constexpr (ACCESS == kAsync)
-            *word(stage, n, s) = Raw<T>::word_of(floats(v));
-        else
-            ln.store(out + static_cast<size_t>(t + s) * dim, v);
-    }
-    // writes the tile put in tensor n's place, the warp's tokens from t, out
+    // A result of the lane's token s, into the place of tensor n's word.
+    CUBF_DEV void put(int stage, int n, int s, Pair v) const { *word(stage, n, s) = Raw<T>::word_of(floats(v)); }
+    // writes the tile put in tensor n's place, the warp's tokens from t, out to rows of `dim` channels
     CUBF_DEV void flush(int stage, int n, T* out, int t) const {
-        if constexpr (ACCESS == kAsync) {
-            const unsigned char* src = mine + stage * kBytes + n * kTensorBytes + piece_place();
-            const int row = t + lane / kPerRow, col = c0 + piece();
-            T* dst = out + static_cast<size_t>(row) * dim + col;
-            if (t + TOKENS <= length && c0 + kChannels <= dim) {
+        const unsigned char* src = mine + stage * kBytes + n * kTensorBytes + piece_place();
+        const int row = t + lane / kAcross, col = column();
+        T* dst = out + static_cast<size_t>(row) * dim + col;
+        const bool whole = t + TOKENS <= length && c0 + kChannels <= dim;
 #pragma unroll
-                for (int k = 0; k < kCopies; ++k) {
-                    __stcs(reinterpret_cast<uint4*>(dst), *reinterpret_cast<const uint4*>(src + row_place(k)));
-                    dst += static_cast<size_t>(kRowsPer) * dim;
-                }
-            } else {
+        for (int k = 0; k < kCopies; ++k) {
 #pragma unroll
-                for (int k = 0; k < kCopies; ++k) {
-                    if (row + k * kRowsPer < length && col < dim)
-                        __stcs(reinterpret_cast<uint4*>(dst), *reinterpret_cast<const uint4*>(src + row_place(k)));
-                    dst += static_cast<size_t>(kRowsPer) * dim;
+            for (int m = 0; m < kTimes; ++m)
+                if (whole || (row + k * kRowsPer < length && col + m * 32 * kElements < dim)) {
+                    const unsigned char* from = src + row_place(k) + m * 32 * PIECE;
+                    T* to = dst + m * 32 * kElements;
+                    if constexpr (PIECE == 16)
+                        __stcs(reinterpret_cast<uint4*>(to), *reinterpret_cast<const uint4*>(from));
+                    else if constexpr (PIECE == 4)
+                        __stcs(reinterpret_cast<unsigned int*>(to), *reinterpret_cast<const unsigned int*>(from));
+                    else
+                        __stcs(reinterpret_cast<unsigned short*>(to), *reinterpret_cast<const unsigned short*>(from));
                 }
-            }
+            dst += static_cast<size_t>(kRowsPer) * dim;
         }
     }
 };
@@ -426,9 +418,41 @@ struct Walker {
         start = offsets[lo];
         stop = offsets[lo + 1];
     }
-    // Tokens [t, t + n) lie inside one sequence, its first and last token not among them.
-    CUBF_DEV bool inside(int t, int n) const { return start < t && t + n < stop; }
 };
+
+// Which tokens of a run [t, t + n) are their sequence's first and last (bit s:
+// token t + s), and the sequences of its first and last token.
+struct Marks {
+    unsigned starts = 0, ends = 0;
+    int first = 0, last = 0;
+
+    CUBF_DEV bool none() const { return (starts | ends) == 0; }
+    // `seq` moves to the run's last token
+    CUBF_DEV void find(Walker& seq, int t, int n, int length) {
+        seq.seek(t);
+        first = last = seq.at;
+        n = n < length - t ? n : length - t;
+        if (n <= 0) return;
+        if (seq.start >= t && seq.start < t + n) starts = 1u << (seq.start - t);
+        while (seq.stop <= t + n) {
+            if (seq.stop > t) ends |= 1u << (seq.stop - 1 - t);
+            if (seq.stop == t + n || seq.at >= seq.last) break;
+            seq.seek(seq.stop);
+            if (seq.start < t || seq.start >= t + n) break;  // offsets that do not ascend
+            starts |= 1u << (seq.start - t);
+            last = seq.at;
+        }
+    }
+};
+// The next sequence after `at` that has tokens, and the one before.
+CUBF_DEV int following(const int* offsets, int sequences, int at) {
+    for (++at; at + 1 < sequences && offsets[at + 1] <= offsets[at];) ++at;
+    return at < sequences ? at : sequences - 1;
+}
+CUBF_DEV int preceding(const int* offsets, int at) {
+    for (--at; at > 0 && offsets[at + 1] <= offsets[at];) --at;
+    return at > 0 ? at : 0;
+}
 
 // Hand-over from one warp to another on a named barrier that counts both
 // warps: the giver's shared-memory writes before give() are seen after take().
@@ -477,12 +501,12 @@ struct Joined {
 };
 
 // ---- forward ----------------------------------------------------------------------------------
-template <typename T, int GROUPS, Access ACCESS>
-using ForwardRows = Rows<T, 3, kForwardSteps<T>, 2, GROUPS, ACCESS>;
+template <typename T, int GROUPS, int PIECE>
+using ForwardRows = Rows<T, 3, kForwardSteps<T>, 2, GROUPS, PIECE>;
 
-template <typename T, bool PACKED, int GROUPS, Access ACCESS>
+template <typename T, bool PACKED, int GROUPS, int PIECE>
 __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArgs p, int tiles) {
-    using Tile = ForwardRows<T, GROUPS, ACCESS>;
+    using Tile = ForwardRows<T, GROUPS, PIECE>;
     constexpr int kSteps = Tile::STEPS, stride = Tile::TOKENS * kWarps;  // tokens a CTA takes a round
     using Word = typename Raw<T>::Word;
     extern __shared__ __align__(16) unsigned char staged[];
@@ -491,7 +515,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int group = lane / (32 / GROUPS);
     const int c0 = static_cast<int>(blockIdx.x % tiles) * Tile::kChannels;
-    const Lane<ACCESS, GROUPS> ln(c0, lane, p.dim);
+    const Lane<GROUPS> ln(c0, lane, p.dim);
     const size_t b = blockIdx.x / tiles;
     int w0 = warp * Tile::TOKENS;  // the warp's first token; the lane's run begins at t0
     Tile rows{{static_cast<const T*>(p.x) + b * p.x_batch, static_cast<const T*>(p.r) + b * p.r_batch,
@@ -529,23 +553,27 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
         rows.close(buf, 1, t0, Raw<T>::lowest());
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            const Word rx = rows.get(ln, buf, 0, t0, s, Raw<T>::zero());
-            const Word rr = rows.get(ln, buf, 1, t0, s, Raw<T>::lowest());
-            const Word ri = rows.get(ln, buf, 2, t0, s, Raw<T>::zero());
             Pair m2;
-            decay(mul2(rate, sigmoid(Raw<T>::get(rr))), a[s], m2);
-            u[s] = drive(m2, Raw<T>::get(ri), Raw<T>::get(rx));
+            decay(mul2(rate, sigmoid(rows.get(buf, 1, s))), a[s], m2);
+            u[s] = drive(m2, rows.get(buf, 2, s), rows.get(buf, 0, s));
+        }
+        Marks marks;
+        if constexpr (PACKED) {
+            marks.find(seq, t0, kSteps, p.length);
+            if (marks.starts && p.initial) {  // the initial states enter with the first tokens
+                int at = marks.starts & 1u ? marks.first : following(p.offsets, p.sequences, marks.first);
+                for (unsigned left = marks.starts; left; left &= left - 1) {
+                    const Pair h0 = ln.load32(p.initial + static_cast<size_t>(at) * p.dim);
+                    const int token = __ffs(left) - 1;
+#pragma unroll
+                    for (int s = 0; s < kSteps; ++s)
+                        if (s == token) u[s] = fma2(a[s], h0, u[s]);
+                    at = following(p.offsets, p.sequences, at);
+                }
+            }
         }
         Pair A = both(1.f), H = both(0.f);
-        unsigned starts = 0;
-        Walker from;
-        bool plain = t0 + kSteps <= p.length;  // every token exists, and none is a sequence's first or last
-        if constexpr (PACKED) {
-            seq.seek(t0);
-            from = seq;
-            plain = plain && seq.inside(t0, kSteps);
-        }
-        if (!PACKED || plain) {
+        if (!PACKED || marks.starts == 0) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 A = mul2(A, a[s]);
@@ -553,20 +581,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
             }
         } else {
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                if (t0 + s >= p.length) continue;
-                seq.seek(t0 + s);
-                if (t0 + s == seq.start) {
-                    starts |= 1u << s;
-                    if (p.initial)
-                        u[s] = fma2(a[s], ln.load32(p.initial + static_cast<size_t>(seq.at) * p.dim), u[s]);
-                    A = kMarker;
-                    H = u[s];
-                } else {
-                    A = product<PACKED>(A, a[s]);
-                    H = fma2(a[s], H, u[s]);
-                }
-            }
+            for (int s = 0; s < kSteps; ++s) H = (marks.starts >> s) & 1u ? u[s] : fma2(a[s], H, u[s]);
+            A = kMarker;
         }
         // The state goes from warp to warp, and from the last one to the first
         // one's next tile; no barrier holds all warps, so they drift apart and
@@ -589,21 +605,21 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
         if (GROUPS > 1 && group > 0) h = through<PACKED>(runs.before_a, runs.before_h, h);  // before the lane's run
         if (chunk_states && t0 % kGatedScanChunk == 0 && t0 < p.length)
             ln.store32(chunk_states + static_cast<size_t>(t0 / kGatedScanChunk) * p.dim, h);
-        if (plain) {
+        if (!PACKED || marks.none()) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 h = fma2(a[s], h, u[s]);
-                rows.put(ln, buf, 0, out, t0, s, h);
+                rows.put(buf, 0, s, h);
             }
         } else {
+            int at = marks.first;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
-                if (t0 + s >= p.length) continue;
-                h = (starts >> s) & 1u ? u[s] : fma2(a[s], h, u[s]);
-                rows.put(ln, buf, 0, out, t0, s, h);
-                if constexpr (PACKED) {
-                    from.seek(t0 + s);
-                    if (t0 + s + 1 == from.stop) ln.store32(p.last + static_cast<size_t>(from.at) * p.dim, h);
+                h = (marks.starts >> s) & 1u ? u[s] : fma2(a[s], h, u[s]);
+                rows.put(buf, 0, s, h);
+                if ((marks.ends >> s) & 1u) {
+                    ln.store32(p.last + static_cast<size_t>(at) * p.dim, h);
+                    at = following(p.offsets, p.sequences, at);
                 }
             }
         }
@@ -625,12 +641,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
 //   dr = e (1 - sigmoid(r))   dLambda = sum e sigmoid(Lambda)/softplus(Lambda)
 // A thread keeps a, v, 1/m and sigmoid(r) of its tokens and gets sigmoid(i)
 // back as v/m, which leaves room for two CTAs per SM.
-template <typename T, int GROUPS, Access ACCESS>
-using BackwardRows = Rows<T, 4, kBackwardSteps, sizeof(T) == 2 ? 2 : 1, GROUPS, ACCESS>;
+template <typename T, int GROUPS, int PIECE>
+using BackwardRows = Rows<T, 4, kBackwardSteps, sizeof(T) == 2 ? 2 : 1, GROUPS, PIECE>;
 
-template <typename T, bool PACKED, int GROUPS, Access ACCESS>
+template <typename T, bool PACKED, int GROUPS, int PIECE>
 __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(GatedScanArgs p, int tiles) {
-    using Tile = BackwardRows<T, GROUPS, ACCESS>;
+    using Tile = BackwardRows<T, GROUPS, PIECE>;
     constexpr int kSteps = Tile::STEPS, stride = Tile::TOKENS * kWarps;  // tokens a CTA takes a round
     using Word = typename Raw<T>::Word;
     extern __shared__ __align__(16) unsigned char staged[];
@@ -641,7 +657,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(Gat
     const int lane = threadIdx.x & 31, warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const int group = lane / (32 / GROUPS);
     const int c0 = static_cast<int>(blockIdx.x % tiles) * Tile::kChannels;
-    const Lane<ACCESS, GROUPS> ln(c0, lane, p.dim);
+    const Lane<GROUPS> ln(c0, lane, p.dim);
     const size_t b = blockIdx.x / tiles;
     const int rounds = (p.length + stride - 1) / stride;
     int w0 = (rounds - 1) * stride + warp * Tile::TOKENS;  // the warp's first token; the lane's run begins at t0
@@ -680,63 +696,36 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(Gat
         const bool second = (GROUPS > 1 ? group : warp) % 2;
         if (!second && t0 < p.length)
             h = ln.load32(chunk_states + static_cast<size_t>(t0 / kGatedScanChunk) * p.dim);
-        // x and dh are read where they are used, from shared memory; other
-        // accesses keep them
-        Word kx[ACCESS == kAsync ? 1 : kSteps], kd[ACCESS == kAsync ? 1 : kSteps];
+        // x and dh are read where they are used, from shared memory
         Pair a[kSteps], v[kSteps], im[kSteps], sr[kSteps];
         rows.arrive();
         rows.close(stage, 1, t0, Raw<T>::lowest());
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            if constexpr (ACCESS != kAsync) {
-                kx[s] = rows.get(ln, stage, 0, t0, s, Raw<T>::zero());
-                kd[s] = rows.get(ln, stage, 3, t0, s, Raw<T>::zero());
-            }
-            const Word rr = rows.get(ln, stage, 1, t0, s, Raw<T>::lowest());
-            const Word ri = rows.get(ln, stage, 2, t0, s, Raw<T>::zero());
             Pair m2;
-            sr[s] = sigmoid(Raw<T>::get(rr));
+            sr[s] = sigmoid(rows.get(stage, 1, s));
             decay(mul2(rate, sr[s]), a[s], m2);
             im[s] = inverse_root(m2);
-            v[s] = mul2(mul2(m2, im[s]), sigmoid(Raw<T>::get(ri)));
+            v[s] = mul2(mul2(m2, im[s]), sigmoid(rows.get(stage, 2, s)));
         }
-        auto x_of = [&](int s) {
-            if constexpr (ACCESS == kAsync)
-                return Raw<T>::get(rows.get(ln, stage, 0, t0, s, Raw<T>::zero()));
-            else
-                return Raw<T>::get(kx[s]);
-        };
-        auto dh_of = [&](int s) {
-            if constexpr (ACCESS == kAsync)
-                return Raw<T>::get(rows.get(ln, stage, 3, t0, s, Raw<T>::zero()));
-            else
-                return Raw<T>::get(kd[s]);
-        };
+        auto x_of = [&](int s) { return rows.get(stage, 0, s); };
+        auto dh_of = [&](int s) { return rows.get(stage, 3, s); };
 
-        // the maps of the warp's tokens, forward and backward
-        unsigned starts = 0, ends = 0;
+        // the maps of the run, forward and backward
         Pair A = both(1.f), H = both(0.f), R = both(0.f);
-        Walker from;
-        bool plain = t0 + kSteps <= p.length;  // every token exists, and none is a sequence's first or last
+        Marks marks;
         if constexpr (PACKED) {
             seq.rewind();
-            seq.seek(t0);
-            from = seq;
-            plain = plain && seq.inside(t0, kSteps);
+            marks.find(seq, t0, kSteps, p.length);
         }
-        // dh with the final states' gradients where a sequence ends
-        auto arriving = [&](int s, int at) {
-            Pair d = dh_of(s);
-            if (PACKED && ((ends >> s) & 1u) && p.d_last)
-                d = add2(d, ln.load32(p.d_last + static_cast<size_t>(at) * p.dim));
-            return d;
+        // h before a sequence's first token, and the final state's gradient at its last
+        auto initial_of = [&](int at) {
+            return p.initial ? ln.load32(p.initial + static_cast<size_t>(at) * p.dim) : both(0.f);
         };
-        // the sequence of the token before a sequence's first one
-        auto previous = [&](int at, int t) {
-            while (at > 0 && p.offsets[at] >= t) --at;
-            return at;
+        auto last_of = [&](int at) {
+            return p.d_last ? ln.load32(p.d_last + static_cast<size_t>(at) * p.dim) : both(0.f);
         };
-        if (!PACKED || plain) {
+        if (!PACKED || marks.none()) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 A = mul2(A, a[s]);
@@ -745,30 +734,26 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(Gat
 #pragma unroll
             for (int s = kSteps - 1; s >= 0; --s) R = mul2(a[s], add2(dh_of(s), R));
         } else {
+            int at = marks.first;
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
-                if (t0 + s >= p.length) continue;
-                seq.seek(t0 + s);
-                Pair u = mul2(v[s], x_of(s));
-                if (t0 + s + 1 == seq.stop) ends |= 1u << s;
-                if (t0 + s == seq.start) {
-                    starts |= 1u << s;
-                    if (p.initial) u = fma2(a[s], ln.load32(p.initial + static_cast<size_t>(seq.at) * p.dim), u);
-                    A = kMarker;
-                    H = u;
-                } else {
-                    A = product<PACKED>(A, a[s]);
-                    H = fma2(a[s], H, u);
+                if ((marks.starts >> s) & 1u) {
+                    if (s > 0) at = following(p.offsets, p.sequences, at);
+                    H = initial_of(at);
                 }
+                A = mul2(A, a[s]);
+                H = fma2(a[s], H, mul2(v[s], x_of(s)));
             }
-            int at = seq.at;
+            if (marks.starts) A = kMarker;
+            at = marks.last;
 #pragma unroll
             for (int s = kSteps - 1; s >= 0; --s) {
-                if (t0 + s >= p.length) continue;
-                R = mul2(a[s], add2(arriving(s, at), R));
-                if ((starts >> s) & 1u) {
+                Pair d = dh_of(s);
+                if ((marks.ends >> s) & 1u) d = add2(d, last_of(at));
+                R = mul2(a[s], add2(d, R));
+                if ((marks.starts >> s) & 1u) {
                     R = both(0.f);
-                    at = previous(at, t0 + s);
+                    at = preceding(p.offsets, at);
                 }
             }
         }
@@ -811,40 +796,45 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(Gat
             const Pair gi = mul2(mul2(gx, fx), sub2(both(1.f), si));
             P = mul2(a[s], G);
             const Pair e = mul2(mul2(P, mul2(rate_e, sr[s])), sub2(before[s], mul2(mul2(mul2(si, fx), a[s]), im[s])));
-            sum = add2(sum, e);
-            rows.put(ln, stage, 0, dx, t0, s, gx);
-            rows.put(ln, stage, 1, dr, t0, s, mul2(e, sub2(both(1.f), sr[s])));
-            rows.put(ln, stage, 2, di, t0, s, gi);
+            rows.put(stage, 0, s, gx);
+            rows.put(stage, 1, s, mul2(e, sub2(both(1.f), sr[s])));
+            rows.put(stage, 2, s, gi);
+            return e;
         };
-        if (plain) {
+        if (!PACKED || marks.none()) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 before[s] = h;
                 h = fma2(a[s], h, mul2(v[s], x_of(s)));
             }
-#pragma unroll
-            for (int s = kSteps - 1; s >= 0; --s) gradients(s, dh_of(s));
-        } else {
-#pragma unroll
-            for (int s = 0; s < kSteps; ++s) {
-                before[s] = h;
-                if (t0 + s >= p.length) continue;
-                if constexpr (PACKED) {
-                    from.seek(t0 + s);
-                    if ((starts >> s) & 1u)
-                        before[s] = p.initial ? ln.load32(p.initial + static_cast<size_t>(from.at) * p.dim) : both(0.f);
-                }
-                h = fma2(a[s], before[s], mul2(v[s], x_of(s)));
-            }
-            int at = PACKED ? seq.at : 0;
+            const bool whole = t0 + kSteps <= p.length;
 #pragma unroll
             for (int s = kSteps - 1; s >= 0; --s) {
-                if (t0 + s >= p.length) continue;
-                gradients(s, arriving(s, at));
-                if (PACKED && ((starts >> s) & 1u)) {
+                const Pair e = gradients(s, dh_of(s));
+                if (whole || t0 + s < p.length) sum = add2(sum, e);
+            }
+        } else {
+            int at = marks.first;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                if ((marks.starts >> s) & 1u) {
+                    if (s > 0) at = following(p.offsets, p.sequences, at);
+                    h = initial_of(at);
+                }
+                before[s] = h;
+                h = fma2(a[s], h, mul2(v[s], x_of(s)));
+            }
+            at = marks.last;
+#pragma unroll
+            for (int s = kSteps - 1; s >= 0; --s) {
+                Pair d = dh_of(s);
+                if ((marks.ends >> s) & 1u) d = add2(d, last_of(at));
+                const Pair e = gradients(s, d);
+                if (t0 + s < p.length) sum = add2(sum, e);
+                if ((marks.starts >> s) & 1u) {
                     if (p.d_initial) ln.store32(p.d_initial + static_cast<size_t>(at) * p.dim, P);
                     P = both(0.f);
-                    at = previous(at, t0 + s);
+                    at = preceding(p.offsets, at);
                 }
             }
         }
@@ -891,12 +881,12 @@ __global__ void __launch_bounds__(256) gated_scan_decay_kernel(GatedScanArgs p, 
 // A warp takes 64 channels of `rows` consecutive requests; a request whose
 // slot lies outside the pool is padding: its output is zero and no state is
 // touched.
-template <typename T, Access ACCESS>
+template <typename T, bool PAIRS>
 __global__ void __launch_bounds__(128) gated_scan_step_kernel(GatedStepArgs p, int tiles, int rows) {
     pdl_begin();
     const int lane = threadIdx.x & 31;
     const unsigned task = blockIdx.x * 4 + (threadIdx.x >> 5);
-    const Lane<ACCESS, 1> ln(static_cast<int>(task % tiles) * kWarpChannels, lane, p.dim);
+    const Lane<1> ln(static_cast<int>(task % tiles) * kWarpChannels, lane, p.dim);
     const size_t first = static_cast<size_t>(task / tiles) * rows;
     if (first >= p.batch) return;
     const size_t end = first + rows < p.batch ? first + rows : p.batch;
@@ -907,17 +897,17 @@ __global__ void __launch_bounds__(128) gated_scan_step_kernel(GatedStepArgs p, i
         if (p.slots) slot = p.slots[b];
         T* h = static_cast<T*>(p.h) + b * p.dim;
         if (slot < 0 || slot >= static_cast<long long>(p.pool)) {
-            ln.store(h, both(0.f));
+            ln.template store<PAIRS>(h, both(0.f));
             continue;
         }
-        const Pair x = Raw<T>::get(ln.load(static_cast<const T*>(p.x) + b * p.x_row));
-        const Pair r = Raw<T>::get(ln.load(static_cast<const T*>(p.r) + b * p.r_row));
-        const Pair i = Raw<T>::get(ln.load(static_cast<const T*>(p.i) + b * p.i_row));
+        const Pair x = ln.template load<PAIRS>(static_cast<const T*>(p.x) + b * p.x_row);
+        const Pair r = ln.template load<PAIRS>(static_cast<const T*>(p.r) + b * p.r_row);
+        const Pair i = ln.template load<PAIRS>(static_cast<const T*>(p.i) + b * p.i_row);
         const Pair s = ln.load32(p.state + static_cast<size_t>(slot) * p.dim);
         Pair a, m2;
         decay(mul2(rate, sigmoid(r)), a, m2);
         const Pair n = fma2(a, s, drive(m2, i, x));
-        ln.store(h, n);
+        ln.template store<PAIRS>(h, n);
         ln.store32(p.new_state + static_cast<size_t>(slot) * p.dim, n);
     }
 }

@@ -23,7 +23,7 @@ using T = std::conditional_t<CUBF_GS_TYPE == 0, __half, std::conditional_t<CUBF_
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// The widest access every row of every tensor is aligned for.
+// The widest access, in bytes, that every row of every tensor is aligned for.
 struct Alignment {
     uintptr_t bits = 0;  // of addresses and strides in bytes
     Alignment& pointer(const void* p) {
@@ -34,13 +34,10 @@ struct Alignment {
         bits |= elements * sizeof(T);
         return *this;
     }
-    Access access() const {
-        if ((bits & 15) == 0) return kAsync;
-        return (bits & (2 * sizeof(T) - 1)) == 0 ? kPairs : kScalar;
-    }
+    int bytes() const { return static_cast<int>(16 | bits) & -static_cast<int>(16 | bits); }
 };
 
-Access access_of(const GatedScanArgs& a, bool backward) {
+int piece_of(const GatedScanArgs& a, bool backward) {
     Alignment v;
     v.stride(static_cast<size_t>(a.dim)).pointer(a.x).pointer(a.r).pointer(a.i);
     v.stride(a.x_batch).stride(a.r_batch).stride(a.i_batch).stride(a.x_token).stride(a.r_token).stride(a.i_token);
@@ -48,7 +45,7 @@ Access access_of(const GatedScanArgs& a, bool backward) {
         v.pointer(a.d_h).pointer(a.d_x).pointer(a.d_r).pointer(a.d_i).stride(a.dh_batch).stride(a.dh_token);
     else
         v.pointer(a.h);
-    return v.access();
+    return v.bytes();
 }
 
 // Lane groups along time: each doubling makes twice as many CTAs, of half the
@@ -66,20 +63,20 @@ int lane_groups(const GatedScanArgs& a, bool backward) {
     return g;
 }
 
-template <bool PACKED, int GROUPS, Access ACCESS, bool BACKWARD>
+template <bool PACKED, int GROUPS, int PIECE, bool BACKWARD>
 cudaError_t launch_kernel(const GatedScanArgs& a, cudaStream_t stream) {
     static KernelSetup setup;
     const auto kernel = [] {
         if constexpr (BACKWARD)
-            return &gated_scan_backward_kernel<T, PACKED, GROUPS, ACCESS>;
+            return &gated_scan_backward_kernel<T, PACKED, GROUPS, PIECE>;
         else
-            return &gated_scan_kernel<T, PACKED, GROUPS, ACCESS>;
+            return &gated_scan_kernel<T, PACKED, GROUPS, PIECE>;
     }();
-    using Tile = std::conditional_t<BACKWARD, BackwardRows<T, GROUPS, ACCESS>, ForwardRows<T, GROUPS, ACCESS>>;
+    using Tile = std::conditional_t<BACKWARD, BackwardRows<T, GROUPS, PIECE>, ForwardRows<T, GROUPS, PIECE>>;
     constexpr int smem = kWarps * Tile::STAGES * Tile::kBytes;
     int cap = 0;
     // two CTAs per SM fit only in the largest carveout
-    cudaError_t e = setup_kernel(setup, kernel, kWarps * 32, smem, &cap, ACCESS == kAsync);
+    cudaError_t e = setup_kernel(setup, kernel, kWarps * 32, smem, &cap, true);
     if (e != cudaSuccess) return e;
     const int tiles = ceil_div(a.dim, Tile::kChannels);
     const size_t grid = static_cast<size_t>(tiles) * a.batch;
@@ -89,17 +86,23 @@ cudaError_t launch_kernel(const GatedScanArgs& a, cudaStream_t stream) {
 
 template <bool PACKED, bool BACKWARD>
 cudaError_t launch_access(const GatedScanArgs& a, cudaStream_t stream) {
-    switch (access_of(a, BACKWARD)) {
-        case kAsync:
-            switch (lane_groups(a, BACKWARD)) {
-                case 1: return launch_kernel<PACKED, 1, kAsync, BACKWARD>(a, stream);
-                case 2: return launch_kernel<PACKED, 2, kAsync, BACKWARD>(a, stream);
-                case 4: return launch_kernel<PACKED, 4, kAsync, BACKWARD>(a, stream);
-                default: return launch_kernel<PACKED, 8, kAsync, BACKWARD>(a, stream);
-            }
-        case kPairs: return launch_kernel<PACKED, 2, kPairs, BACKWARD>(a, stream);
-        default: return launch_kernel<PACKED, 2, kScalar, BACKWARD>(a, stream);
+    const int piece = piece_of(a, BACKWARD);
+    const int groups = lane_groups(a, BACKWARD);
+    if (piece >= 16) {
+        switch (groups) {
+            case 1: return launch_kernel<PACKED, 1, 16, BACKWARD>(a, stream);
+            case 2: return launch_kernel<PACKED, 2, 16, BACKWARD>(a, stream);
+            case 4: return launch_kernel<PACKED, 4, 16, BACKWARD>(a, stream);
+            default: return launch_kernel<PACKED, 8, 16, BACKWARD>(a, stream);
+        }
     }
+    if (piece >= 4)
+        return groups <= 2 ? launch_kernel<PACKED, 2, 4, BACKWARD>(a, stream)
+                           : launch_kernel<PACKED, 8, 4, BACKWARD>(a, stream);
+    if constexpr (sizeof(T) == 2)
+        return groups <= 2 ? launch_kernel<PACKED, 2, 2, BACKWARD>(a, stream)
+                           : launch_kernel<PACKED, 8, 2, BACKWARD>(a, stream);
+    return cudaErrorMisalignedAddress;
 }
 
 }  // namespace
@@ -126,7 +129,7 @@ cudaError_t launch_gated_scan_step_unit<CUBF_GS_TYPE>(const GatedStepArgs& a, cu
     const size_t grid = (tasks + 3) / 4;
     if (grid > 0x7fffffffULL || rows > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
     return launch_dependent(
-        v.access() == kScalar ? &gated_scan_step_kernel<T, kScalar> : &gated_scan_step_kernel<T, kPairs>,
+        v.bytes() >= 2 * static_cast<int>(sizeof(T)) ? &gated_scan_step_kernel<T, true> : &gated_scan_step_kernel<T, false>,
         static_cast<unsigned>(grid), 128u, 0, stream, a, tiles, static_cast<int>(rows));
 }
 
