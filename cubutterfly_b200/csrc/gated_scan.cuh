@@ -881,7 +881,9 @@ __global__ void __launch_bounds__(256) gated_scan_decay_kernel(GatedScanArgs p, 
 // A warp takes 64 channels of `rows` consecutive requests; a request whose
 // slot lies outside the pool is padding: its output is zero and no state is
 // touched.
-template <typename T, bool PAIRS>
+constexpr int kStepRows = 4;
+// PAIRS, WIDE: pairs of channels of the rows, of the fp32 states are aligned.
+template <typename T, bool PAIRS, bool WIDE>
 __global__ void __launch_bounds__(128) gated_scan_step_kernel(GatedStepArgs p, int tiles, int rows) {
     pdl_begin();
     const int lane = threadIdx.x & 31;
@@ -891,24 +893,33 @@ __global__ void __launch_bounds__(128) gated_scan_step_kernel(GatedStepArgs p, i
     if (first >= p.batch) return;
     const size_t end = first + rows < p.batch ? first + rows : p.batch;
     const Pair rate = mul2(rates(ln.load32(p.decay), p.exponent), both(-1.f));
-#pragma unroll 4
-    for (size_t b = first; b < end; ++b) {
-        long long slot = static_cast<long long>(b);
-        if (p.slots) slot = p.slots[b];
-        T* h = static_cast<T*>(p.h) + b * p.dim;
-        if (slot < 0 || slot >= static_cast<long long>(p.pool)) {
-            ln.template store<PAIRS>(h, both(0.f));
-            continue;
+    // kStepRows requests at a time, all their loads before the arithmetic of the first
+    for (size_t b0 = first; b0 < end; b0 += kStepRows) {
+        long long slot[kStepRows];
+        Pair x[kStepRows], r[kStepRows], i[kStepRows], state[kStepRows];
+#pragma unroll
+        for (int k = 0; k < kStepRows; ++k) {
+            const size_t b = b0 + k < end ? b0 + k : end - 1;
+            slot[k] = p.slots ? p.slots[b] : static_cast<long long>(b);
+            x[k] = ln.template load<PAIRS>(static_cast<const T*>(p.x) + b * p.x_row);
+            r[k] = ln.template load<PAIRS>(static_cast<const T*>(p.r) + b * p.r_row);
+            i[k] = ln.template load<PAIRS>(static_cast<const T*>(p.i) + b * p.i_row);
         }
-        const Pair x = ln.template load<PAIRS>(static_cast<const T*>(p.x) + b * p.x_row);
-        const Pair r = ln.template load<PAIRS>(static_cast<const T*>(p.r) + b * p.r_row);
-        const Pair i = ln.template load<PAIRS>(static_cast<const T*>(p.i) + b * p.i_row);
-        const Pair s = ln.load32(p.state + static_cast<size_t>(slot) * p.dim);
-        Pair a, m2;
-        decay(mul2(rate, sigmoid(r)), a, m2);
-        const Pair n = fma2(a, s, drive(m2, i, x));
-        ln.template store<PAIRS>(h, n);
-        ln.store32(p.new_state + static_cast<size_t>(slot) * p.dim, n);
+#pragma unroll
+        for (int k = 0; k < kStepRows; ++k) {
+            const bool in = slot[k] >= 0 && slot[k] < static_cast<long long>(p.pool);
+            if (!in) slot[k] = -1;
+            state[k] = in ? ln.template load<WIDE>(p.state + static_cast<size_t>(slot[k]) * p.dim) : both(0.f);
+        }
+#pragma unroll
+        for (int k = 0; k < kStepRows; ++k) {
+            if (b0 + k >= end) break;
+            Pair a, m2;
+            decay(mul2(rate, sigmoid(r[k])), a, m2);
+            const Pair n = fma2(a, state[k], drive(m2, i[k], x[k]));
+            ln.template store<PAIRS>(static_cast<T*>(p.h) + (b0 + k) * p.dim, slot[k] < 0 ? both(0.f) : n);
+            if (slot[k] >= 0) ln.template store<WIDE>(p.new_state + static_cast<size_t>(slot[k]) * p.dim, n);
+        }
     }
 }
 

@@ -122,15 +122,18 @@ cudaError_t launch_gated_scan_step_unit<CUBF_GS_TYPE>(const GatedStepArgs& a, cu
     v.stride(static_cast<size_t>(a.dim)).pointer(a.x).pointer(a.r).pointer(a.i).pointer(a.h);
     v.stride(a.x_row).stride(a.r_row).stride(a.i_row);
     const int tiles = ceil_div(a.dim, kWarpChannels);
-    // about 32 warps per SM before a warp takes a second request
+    // one request a warp while that is no more than 32 warps per SM
     const size_t groups = std::max<size_t>(1, static_cast<size_t>(148 * 32) / tiles);
     const size_t rows = (a.batch + groups - 1) / groups;
     const size_t tasks = (a.batch + rows - 1) / rows * tiles;
     const size_t grid = (tasks + 3) / 4;
     if (grid > 0x7fffffffULL || rows > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
-    return launch_dependent(
-        v.bytes() >= 2 * static_cast<int>(sizeof(T)) ? &gated_scan_step_kernel<T, true> : &gated_scan_step_kernel<T, false>,
-        static_cast<unsigned>(grid), 128u, 0, stream, a, tiles, static_cast<int>(rows));
+    const bool pairs = v.bytes() >= 2 * static_cast<int>(sizeof(T));
+    const bool wide = a.dim % 2 == 0 &&
+                      ((reinterpret_cast<uintptr_t>(a.state) | reinterpret_cast<uintptr_t>(a.new_state)) & 7u) == 0;
+    const auto kernel = pairs ? (wide ? &gated_scan_step_kernel<T, true, true> : &gated_scan_step_kernel<T, true, false>)
+                              : (wide ? &gated_scan_step_kernel<T, false, true> : &gated_scan_step_kernel<T, false, false>);
+    return launch_dependent(kernel, static_cast<unsigned>(grid), 128u, 0, stream, a, tiles, static_cast<int>(rows));
 }
 
 }  // namespace cubf
