@@ -68,6 +68,9 @@ void check(cubutterflyStatus_t status) {
 }
 
 // ---- checks -------------------------------------------------------------------------------------
+// Messages are put together from text alone: numbers go through
+// std::to_string, since inserting one into the stream behind these macros
+// crashed here.
 #define REQUIRE(cond, ...) TORCH_CHECK_VALUE(cond, __VA_ARGS__)
 
 std::string text(at::IntArrayRef shape) {
@@ -606,7 +609,7 @@ Tensor gated_scan_step(py::handle hstate, py::handle hx, py::handle hr, py::hand
         REQUIRE(t->device() == x.device(), "gated_scan_step: a state pool is on ", t->device().str(), ", not on ",
                 x.device().str());
         REQUIRE(t->dim() == 2 && t->size(1) == dim && t->is_contiguous(),
-                "gated_scan_step: a state pool must be contiguous and (slots, ", dim, ")");
+                "gated_scan_step: a state pool must be contiguous and (slots, ", std::to_string(dim), ")");
     }
     REQUIRE(next.sizes() == state.sizes(), "gated_scan_step: new_state must have the shape of state");
     Tensor slots = tensor_of(hslots, "gated_scan_step: slots", true);
@@ -616,7 +619,8 @@ Tensor gated_scan_step(py::handle hstate, py::handle hx, py::handle hr, py::hand
         check_like(slots, "gated_scan_step: slots", x, {batch});
         slots = slots.contiguous();
     } else {
-        REQUIRE(state.size(0) >= batch, "gated_scan_step: ", batch, " requests without slots need a pool of as many rows");
+        REQUIRE(state.size(0) >= batch, "gated_scan_step: ", std::to_string(batch),
+                " requests without slots need a pool of as many rows");
     }
     REQUIRE(!any_requires_grad({&state, &x, &r, &i}), "gated_scan_step is inference only: an input requires grad");
     check_exponent(exponent, "gated_scan_step");

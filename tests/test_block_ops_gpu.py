@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import block_reference as ref
+import cubutterfly_b200 as cb
 from cubutterfly_b200 import torch_ops
 
 pytestmark = pytest.mark.gpu
@@ -97,6 +98,24 @@ def test_block_norm_gates(cuda, act, gate, scale, dtype, weights):
 @pytest.mark.parametrize("dim", [64, 128, 256, 512, 1024, 2048, 4096, 8192, 16384])
 def test_block_norm_rotation(cuda, dim, dtype, stream):
     check_norm(norm_case((7, dim), dtype, stream, gate="channel", seed=dim), cuda, rotate=True, act="sigmoid")
+
+
+@pytest.mark.parametrize("dtype,stream", [(BF16, None), (FP16, FP32), (FP32, None)])
+@pytest.mark.parametrize("dim", [256, 1024, 2048, 4096, 8192, 16384])
+def test_block_norm_rotation_of_many_rows(cuda, dim, dtype, stream):
+    """Beyond two rows per SM the rotated rows take another shape."""
+    check_norm(norm_case((301, dim), dtype, stream, gate="channel", scale="vector", seed=dim), cuda, rotate=True)
+
+
+@pytest.mark.parametrize("dtype,stream", [(BF16, None), (FP16, FP32)])
+@pytest.mark.parametrize("dim", [250, 264, 2048])
+def test_block_norm_groups_of_many_rows(cuda, dim, dtype, stream):
+    """Several CTAs sum each gate group's parameter gradients."""
+    check_norm(norm_case((3, 400, dim), dtype, stream, gate="group", scale="vector", seed=dim), cuda, act="sigmoid")
+
+
+def test_block_norm_many_groups(cuda):
+    check_norm(norm_case((300, 2, 40), FP32, gate="group", seed=2), cuda, act="silu")
 
 
 @pytest.mark.parametrize("rotate", [False, True])
@@ -297,6 +316,26 @@ def test_gated_scan_channels(cuda, dim, dtype):
 def test_gated_scan_splits_of_time(cuda, batch, length, dim):
     """Shapes whose time axis is split over clusters of different sizes."""
     check_scan(scan_case(batch, length, dim, BF16, states=batch), cuda)
+
+
+# (batch, length, dim) whose CTAs take 64, 32, 16 and 8 channels forward, and others backward
+SPLITS = [(120, 140, 128), (32, 700, 128), (16, 1100, 128), (3, 1100, 128)]
+
+
+@pytest.mark.parametrize("dtype", [FP16, FP32])
+@pytest.mark.parametrize("extra", [0, 2, 1])
+@pytest.mark.parametrize("batch,length,dim", SPLITS)
+def test_gated_scan_lane_groups(cuda, batch, length, dim, extra, dtype):
+    """Every number of lane groups along time, with rows aligned to 16 and 4 bytes and to single values."""
+    check_scan(scan_case(batch, length, dim + extra, dtype, states=batch, seed=extra), cuda)
+
+
+@pytest.mark.parametrize("dim", [8192, 4096, 2048, 1024, 4098, 4097, 1023])
+def test_gated_scan_packed_lane_groups(cuda, dim):
+    g = torch.Generator().manual_seed(dim)
+    cuts = sorted(torch.randint(0, 701, (25,), generator=g).tolist())
+    offsets = [0, 0, 1, 17, 17, *[c for c in cuts if c > 17], 700, 700]
+    check_scan(scan_case(1, 700, dim, BF16, states=len(offsets) - 1), cuda, offsets=offsets)
 
 
 @pytest.mark.parametrize("d_h,d_final", [(True, False), (False, True)])
@@ -590,3 +629,88 @@ def test_decode_in_an_inference_graph(cuda):
         want = [token(x * k) for k in range(1, 4)]
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(first, want))
+
+
+# ---- refusals and the frontend's errors --------------------------------------------------------
+def test_refusals_on_the_device(cuda):
+    x, y = torch.randn(2, 3, 64, device=cuda), torch.randn(2, 3, 64, device=cuda)
+    w, state = torch.ones(64, device=cuda), torch.zeros(3, 64, device=cuda)
+    i32 = dict(dtype=torch.int32, device=cuda)
+    bad = [
+        (lambda: torch_ops.block_norm(x, y[:1]), "shape"),
+        (lambda: torch_ops.block_norm(x, y.double()), "dtype"),
+        (lambda: torch_ops.block_norm(x.half(), y.bfloat16()), "residual stream"),
+        (lambda: torch_ops.block_norm(x, y, pre_weight=w[:32]), "shape"),
+        (lambda: torch_ops.block_norm(x, y, pre_weight=w, pre_norm=False), "turned off"),
+        (lambda: torch_ops.block_norm(x, y, rotate=True, pre_norm=False), "rotate"),
+        (lambda: torch_ops.block_norm(x, y, gate=w[:3]), "gate"),
+        (lambda: torch_ops.block_norm(x, y, gate=w, gate_activation="tanh"), "gate_activation"),
+        (lambda: torch_ops.block_norm(x, y, residual_scale=math.inf), "residual_scale"),
+        (lambda: torch_ops.block_norm(x, y, eps=-1.0), "eps"),
+        (lambda: torch_ops.block_norm(x, gate=w), "block output"),
+        (lambda: torch_ops.block_norm(x, residual_scale=0.5), "block output"),
+        (lambda: torch_ops.block_norm(x, pre_norm=False), "nothing to compute"),
+        (lambda: torch_ops.block_norm(x, y, dtype=BF16), "dtype"),
+        (lambda: torch_ops.block_norm(x.half(), y.half(), gate=y), "gate per row"),
+        (lambda: torch_ops.gated_scan(x[0], x[0], x[0], w), "must be"),
+        (lambda: torch_ops.gated_scan(x, x[:, :2], x, w), "shape"),
+        (lambda: torch_ops.gated_scan(x, x.half(), x, w), "dtype"),
+        (lambda: torch_ops.gated_scan(x, x, x, w[:8]), "shape"),
+        (lambda: torch_ops.gated_scan(x, x, x, w, exponent=0.0), "exponent"),
+        (lambda: torch_ops.gated_scan(x, x, x, w, initial_state=state), "shape"),
+        (lambda: torch_ops.gated_scan(x, x, x, w, initial_state=state[:2].half()), "dtype"),
+        (lambda: torch_ops.gated_scan(x, x, x, w, offsets=torch.zeros(3, **i32)), "packed"),
+        (lambda: torch_ops.gated_scan(x[0], x[0], x[0], w, offsets=torch.zeros(1, **i32)), "offsets"),
+        (lambda: torch_ops.gated_scan(x[0], x[0], x[0], w, offsets=torch.zeros(3, device=cuda).long()), "dtype"),
+        (lambda: torch_ops.gated_scan_step(state, x, x, x, w), "must be"),
+        (lambda: torch_ops.gated_scan_step(state[:2], x[0], x[0], x[0], w), "pool"),
+        (lambda: torch_ops.gated_scan_step(state.half(), x[0], x[0], x[0], w), "dtype"),
+        (lambda: torch_ops.gated_scan_step(state.t(), x[0], x[0], x[0], w), "pool"),
+        (lambda: torch_ops.gated_scan_step(state, x[0], x[0], x[0], w, slots=torch.zeros(2, **i32)), "shape"),
+        (lambda: torch_ops.gated_scan_step(state, x[0], x[0], x[0], w, new_state=state[:2]), "shape"),
+        (lambda: torch_ops.gated_scan_step(state, x[0].clone().requires_grad_(), x[0], x[0], w), "inference only"),
+        (lambda: torch_ops.block_norm([1.0]), "CUDA"),
+    ]
+    for call, text in bad:
+        with pytest.raises(ValueError, match=text):
+            call()
+
+
+def test_library_refusals_name_their_status(cuda):
+    x = torch.randn(2, 96, device=cuda)
+    with pytest.raises(cb.Error, match="power-of-two") as e:
+        torch_ops.block_norm(x, x, rotate=True)
+    assert e.value.status == cb.Status.NOT_SUPPORTED
+    wide = torch.randn(1, 16385, device=cuda)
+    with pytest.raises(cb.Error, match="16384"):
+        torch_ops.block_norm(wide, wide)
+
+
+def test_differentiable_once(cuda):
+    x = torch.randn(2, 8, 32, device=cuda, requires_grad=True)
+    w = torch.ones(32, device=cuda)
+    for out in (torch_ops.block_norm(x, x * 2)[1], torch_ops.gated_scan(x, x, x, w)[0]):
+        (g,) = torch.autograd.grad(out.sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            g.sum().backward()
+
+
+def test_only_asked_gradients_are_returned(cuda):
+    x, y = torch.randn(4, 64, device=cuda), torch.randn(4, 64, device=cuda, requires_grad=True)
+    w = torch.ones(64, device=cuda)
+    res, u = torch_ops.block_norm(x, y, pre_weight=w)
+    (res.sum() + u.sum()).backward()
+    assert y.grad is not None and x.grad is None and w.grad is None
+    with torch.no_grad():
+        assert not torch_ops.block_norm(x, y)[1].requires_grad
+
+
+def test_low_precision_decay(cuda):
+    """A decay in the block's type is widened, and its gradient comes back in that type."""
+    x = normal(1, 2, 20, 64, dtype=BF16).to(cuda)
+    decay = decay_of(64).to(BF16).to(cuda).requires_grad_()
+    h, _ = torch_ops.gated_scan(x, x, x, decay)
+    want, _ = torch_ops.gated_scan(x, x, x, decay.detach().float())
+    assert torch.equal(h, want)
+    h.float().sum().backward()
+    assert decay.grad.dtype == BF16 and torch.isfinite(decay.grad).all()
