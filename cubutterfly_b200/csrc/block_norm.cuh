@@ -198,6 +198,24 @@ CUBF_DEV Pair activation(int act, Pair g) {
     const float2 f = floats(g);
     return f32x2::pk(activation<SLOPE>(act, f.x), activation<SLOPE>(act, f.y));
 }
+// act(g) and its slope from one sigmoid
+template <typename Act>
+CUBF_DEV void activation_with_slope(Act act, Pair g, Pair& value, Pair& slope) {
+    if (act == 0) {
+        value = g;
+        slope = both(1.f);
+        return;
+    }
+    const float2 f = floats(g);
+    const Pair s = f32x2::pk(sigmoid(f.x), sigmoid(f.y)), rest = sub2(both(1.f), s);
+    if (act == 1) {
+        value = s;
+        slope = mul2(s, rest);
+    } else {
+        value = mul2(g, s);
+        slope = fma2(value, rest, s);  // s + g s (1 - s)
+    }
+}
 // body(act) with the activation a constant in it
 template <typename Body>
 CUBF_DEV void with_activation(int act, Body&& body) {
@@ -419,6 +437,7 @@ struct ForwardPlan {
     // Rows of many values a thread are not loaded ahead: their registers go to
     // more rows at a time, whose loads overlap each other's work.
     static constexpr bool kAhead = S::EPT <= 16;
+    static constexpr uint32_t kPrefetch = kAhead ? 2 : 1;  // turns ahead that a row is brought to L2
     static constexpr int kRow = ROTATE ? padded_row(kDim) : 0;
     static constexpr int kWordsAt = S::kRows * kRow;
     static constexpr int kFactorsAt = kWordsAt + S::kRows * 4 * S::kWarps;
@@ -498,6 +517,12 @@ __global__ void __launch_bounds__(S::kThreads, ForwardPlan<S, ROTATE>::template 
 
     for (int slot = 0; row < rows; row += stride, slot ^= 1) {
         if (!Plan::kAhead) load(row);
+        if (S::VW > 1 && j == 0 && row + Plan::kPrefetch * stride < rows) {  // towards L2, before it is loaded
+            const uint32_t n = row + Plan::kPrefetch * stride;
+            prefetch_l2(at(static_cast<const R*>(p.x), p.x_bytes, n), dim_bytes<R>(dim));
+            if (p.y) prefetch_l2(at(static_cast<const T*>(p.y), p.y_bytes, n), dim_bytes<T>(dim));
+            if (p.gate_mode == kGateFull) prefetch_l2(at(static_cast<const T*>(p.gate), p.gate_bytes, n), dim_bytes<T>(dim));
+        }
         Pair s[S::HALF];
         Pair sum = both(0.f);
         float ry = 1.f;
@@ -728,6 +753,14 @@ __global__ void __launch_bounds__(S::kThreads, 1) block_norm_backward_kernel(Blo
 
     for (int slot = 0; n < last; n += S::kRows, slot ^= 1) {
         const bool more = n + S::kRows < last;
+        if (S::VW > 1 && j == 0 && n + 2 * S::kRows < last) {  // towards L2, a row before it is loaded
+            constexpr uint32_t kTwo = 2 * S::kRows;
+            prefetch_l2(at(static_cast<const R*>(p.x), p.x_bytes, kTwo), dim_bytes<R>(dim));
+            if (p.d_residual) prefetch_l2(at(static_cast<const R*>(p.d_residual), p.d_residual_bytes, kTwo), dim_bytes<R>(dim));
+            if (p.y) prefetch_l2(at(static_cast<const T*>(p.y), p.y_bytes, kTwo), dim_bytes<T>(dim));
+            if (p.d_normed) prefetch_l2(at(static_cast<const T*>(p.d_normed), p.d_normed_bytes, kTwo), dim_bytes<T>(dim));
+            if (row_gate) prefetch_l2(at(static_cast<const T*>(p.gate), p.gate_bytes, kTwo), dim_bytes<T>(dim));
+        }
         Values<T, S> y_next, g_next;  // used first in the next row, and last in this one
         y_next.clear();
         if (more) {
@@ -813,21 +846,20 @@ __global__ void __launch_bounds__(S::kThreads, 1) block_norm_backward_kernel(Blo
             if (row_gate) {
                 with_activation(p.act, [&](auto act) {
 #pragma unroll
-                    for (int k = 0; k < S::HALF; ++k)  // dgate
-                        sn[k] = mul2(mul2(mul2(mul2(d[k], y.pair(k)), both(ry)), factor(0, k)),
-                                     activation<true>(act, g.pair(k)));
-                });
-                store_row<S>(at(static_cast<T*>(p.d_gate), dim_bytes<T>(dim), 0), j, dim, [&](int k) { return sn[k]; });
-                with_activation(p.act, [&](auto act) {
-#pragma unroll
                     for (int k = 0; k < S::HALF; ++k) {
-                        sn[k] = mul2(y.pair(k), both(ry));
-                        d[k] = mul2(d[k], activation<false>(act, g.pair(k)));  // dn
-                        add_sum(kP, k, d[k], sn[k]);
-                        d[k] = mul2(d[k], factor(0, k));
-                        sum = fma2(d[k], sn[k], sum);
+                        Pair value, slope;
+                        activation_with_slope(act, g.pair(k), value, slope);
+                        const Pair yn = mul2(y.pair(k), both(ry)), w = factor(0, k);
+                        sn[k] = mul2(mul2(mul2(d[k], yn), w), slope);  // dgate
+                        d[k] = mul2(d[k], value);                      // dn
+                        add_sum(kP, k, d[k], yn);
+                        d[k] = mul2(d[k], w);
+                        sum = fma2(d[k], yn, sum);
                     }
                 });
+                store_row<S>(at(static_cast<T*>(p.d_gate), dim_bytes<T>(dim), 0), j, dim, [&](int k) { return sn[k]; });
+#pragma unroll
+                for (int k = 0; k < S::HALF; ++k) sn[k] = mul2(y.pair(k), both(ry));
             } else {
 #pragma unroll
                 for (int k = 0; k < S::HALF; ++k) {

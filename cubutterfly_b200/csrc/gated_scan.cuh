@@ -715,7 +715,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(Gat
         Pair A = both(1.f), H = both(0.f), R = both(0.f);
         Marks marks;
         if constexpr (PACKED) {
-            seq.rewind();
+            if (t0 < seq.start) seq.rewind();
             marks.find(seq, t0, kSteps, p.length);
         }
         // h before a sequence's first token, and the final state's gradient at its last
