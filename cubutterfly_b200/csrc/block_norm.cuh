@@ -45,6 +45,7 @@ struct Shape {
     static constexpr int kThreads = THREADS_ > 0 ? THREADS_ : TPR == 32 ? 128 : TPR;
     static constexpr int kRows = kThreads / TPR;    // rows a CTA works on at a time
     static constexpr int kWarps = TPR / 32;
+    static constexpr bool kBulk = VW >= 4;          // rows are whole 16-byte vectors (see the launches)
     static_assert(C * VW == EPT && TPR >= 32 && EPT >= 2, "whole chunks over whole warps");
     static_assert(TPR == 32 || kRows <= 15, "a barrier for each row of several warps");
     static CUBF_DEV int at(int c, int j) { return (c * TPR + j) * VW; }
@@ -79,15 +80,29 @@ struct Values {
 #pragma unroll
             for (int c = 0; c < S::C; ++c) {
                 const bool in = S::at(c, j) < dim;
-                const uint4* p = reinterpret_cast<const uint4*>(row + S::at(c, j));
+                const T* from = row + S::at(c, j);
+                uint32_t* to = w + c * kPer;
+                if constexpr (kPer >= 4) {
 #pragma unroll
-                for (int k = 0; k < kPer / 4; ++k) {
-                    uint4 q = make_uint4(0, 0, 0, 0);
-                    if (in) q = STREAM ? __ldcs(p + k) : __ldg(p + k);
-                    w[c * kPer + 4 * k] = q.x;
-                    w[c * kPer + 4 * k + 1] = q.y;
-                    w[c * kPer + 4 * k + 2] = q.z;
-                    w[c * kPer + 4 * k + 3] = q.w;
+                    for (int k = 0; k < kPer; k += 4) {
+                        const uint4* p = reinterpret_cast<const uint4*>(from) + k / 4;
+                        uint4 q = make_uint4(0, 0, 0, 0);
+                        if (in) q = STREAM ? __ldcs(p) : __ldg(p);
+                        to[k] = q.x;
+                        to[k + 1] = q.y;
+                        to[k + 2] = q.z;
+                        to[k + 3] = q.w;
+                    }
+                } else if constexpr (kPer == 2) {
+                    const uint2* p = reinterpret_cast<const uint2*>(from);
+                    uint2 q = make_uint2(0, 0);
+                    if (in) q = STREAM ? __ldcs(p) : __ldg(p);
+                    to[0] = q.x;
+                    to[1] = q.y;
+                } else {
+                    const unsigned int* p = reinterpret_cast<const unsigned int*>(from);
+                    to[0] = 0;
+                    if (in) to[0] = STREAM ? __ldcs(p) : __ldg(p);
                 }
             }
         }
@@ -129,7 +144,8 @@ CUBF_DEV void store_row(T* row, int j, int dim, Get&& pair) {
             const float2 f = floats(pair(c / 2));
             if (S::at(c, j) < dim) row[S::at(c, j)] = Convert<T, float>::store(c & 1 ? f.y : f.x);
         } else {
-            uint32_t w[S::VW * static_cast<int>(sizeof(T)) / 4];
+            constexpr int kPer = S::VW * static_cast<int>(sizeof(T)) / 4;
+            uint32_t w[kPer];
 #pragma unroll
             for (int k = 0; k < S::VW / 2; ++k) {
                 const float2 f = floats(pair(c * (S::VW / 2) + k));
@@ -141,10 +157,16 @@ CUBF_DEV void store_row(T* row, int j, int dim, Get&& pair) {
                 }
             }
             if (S::at(c, j) < dim) {
-                uint4* p = reinterpret_cast<uint4*>(row + S::at(c, j));
+                T* to = row + S::at(c, j);
+                if constexpr (kPer >= 4) {
 #pragma unroll
-                for (int k = 0; k < S::VW * static_cast<int>(sizeof(T)) / 16; ++k)
-                    __stcs(p + k, make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]));
+                    for (int k = 0; k < kPer; k += 4)
+                        __stcs(reinterpret_cast<uint4*>(to) + k / 4, make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]));
+                } else if constexpr (kPer == 2) {
+                    __stcs(reinterpret_cast<uint2*>(to), make_uint2(w[0], w[1]));
+                } else {
+                    __stcs(reinterpret_cast<unsigned int*>(to), w[0]);
+                }
             }
         }
     }
@@ -517,7 +539,7 @@ __global__ void __launch_bounds__(S::kThreads, ForwardPlan<S, ROTATE>::template 
 
     for (int slot = 0; row < rows; row += stride, slot ^= 1) {
         if (!Plan::kAhead) load(row);
-        if (S::VW > 1 && j == 0 && row + Plan::kPrefetch * stride < rows) {  // towards L2, before it is loaded
+        if (S::kBulk && j == 0 && row + Plan::kPrefetch * stride < rows) {  // towards L2, before it is loaded
             const uint32_t n = row + Plan::kPrefetch * stride;
             prefetch_l2(at(static_cast<const R*>(p.x), p.x_bytes, n), dim_bytes<R>(dim));
             if (p.y) prefetch_l2(at(static_cast<const T*>(p.y), p.y_bytes, n), dim_bytes<T>(dim));
@@ -753,7 +775,7 @@ __global__ void __launch_bounds__(S::kThreads, 1) block_norm_backward_kernel(Blo
 
     for (int slot = 0; n < last; n += S::kRows, slot ^= 1) {
         const bool more = n + S::kRows < last;
-        if (S::VW > 1 && j == 0 && n + 2 * S::kRows < last) {  // towards L2, a row before it is loaded
+        if (S::kBulk && j == 0 && n + 2 * S::kRows < last) {  // towards L2, a row before it is loaded
             constexpr uint32_t kTwo = 2 * S::kRows;
             prefetch_l2(at(static_cast<const R*>(p.x), p.x_bytes, kTwo), dim_bytes<R>(dim));
             if (p.d_residual) prefetch_l2(at(static_cast<const R*>(p.d_residual), p.d_residual_bytes, kTwo), dim_bytes<R>(dim));

@@ -34,18 +34,31 @@ constexpr int kVec = 16 / static_cast<int>(sizeof(T));
 #endif
 constexpr int kWide = sizeof(R) == 2 ? WIDE : 8;
 
-// Whole 16-byte vectors everywhere: every pointer aligned, every row stride
-// and the row length a multiple of the vector.
-bool aligned(const BlockNormArgs& a) {
-    uintptr_t bits = 0;
-    for (const void* p : {a.x, a.y, a.gate, a.pre, a.post, a.scales, a.d_residual, a.d_normed,
-                          static_cast<const void*>(a.residual), static_cast<const void*>(a.normed),
-                          static_cast<const void*>(a.d_x), static_cast<const void*>(a.d_y),
-                          static_cast<const void*>(a.d_gate), static_cast<const void*>(a.partials)})
-        bits |= reinterpret_cast<uintptr_t>(p) & 15u;
-    for (uint32_t s : {a.x_bytes, a.y_bytes, a.gate_bytes, a.d_residual_bytes, a.d_normed_bytes}) bits |= s & 15u;
-    bits |= (a.gate_row | static_cast<size_t>(a.dim)) & (kVec - 1);
-    return bits == 0;
+// Consecutive values that every row of every tensor is aligned for: whole
+// 16-byte vectors (kVec), pairs, or one.
+int alignment(const BlockNormArgs& a) {
+    uintptr_t block = static_cast<uintptr_t>(a.dim) * sizeof(T);  // of 16-byte vectors of the block's type
+    uintptr_t wide = static_cast<uintptr_t>(a.dim) * 4;           // of fp32 tensors beside 16-bit ones
+    auto add = [](uintptr_t& bits, const void* p) { bits |= reinterpret_cast<uintptr_t>(p); };
+    for (const void* p : {a.y, a.d_normed, static_cast<const void*>(a.normed), static_cast<const void*>(a.d_y)})
+        add(block, p);
+    block |= a.y_bytes | a.d_normed_bytes;
+    uintptr_t& stream = sizeof(R) == 4 ? wide : block;
+    for (const void* p : {a.x, a.d_residual, static_cast<const void*>(a.residual), static_cast<const void*>(a.d_x)})
+        add(stream, p);
+    stream |= a.x_bytes | a.d_residual_bytes;
+    uintptr_t& gate = a.gate32 ? wide : block;
+    add(gate, a.gate);
+    add(gate, a.gate_mode == kGateFull ? a.d_gate : nullptr);
+    gate |= a.gate_mode == kGateFull ? a.gate_bytes : a.gate_row * (a.gate32 ? 4 : sizeof(T));
+    add(a.pre32 ? wide : block, a.pre);
+    add(a.post32 ? wide : block, a.post);
+    add(a.scales32 ? wide : block, a.scales);
+    add(wide, a.partials);
+    if (sizeof(T) == 4) block |= wide;
+    if (((block | wide) & 15) == 0 && a.dim % kVec == 0) return kVec;
+    // pairs: 2 values of the block's type, 8 bytes of fp32
+    return (block & (2 * sizeof(T) - 1)) == 0 && (wide & 7) == 0 ? 2 : 1;
 }
 
 template <typename S, bool ROTATE>
@@ -84,7 +97,8 @@ cudaError_t shape(const BlockNormArgs& a, size_t groups, cudaStream_t stream) {
 
 cudaError_t dispatch(const BlockNormArgs& a, size_t groups, cudaStream_t s) {
     constexpr int V = kVec;
-    const bool vec = aligned(a);
+    const int width = alignment(a);
+    const bool vec = width == V;
     const int d = a.dim;
     if (a.rotate) {
         if (vec && d >= 256) {
@@ -152,10 +166,19 @@ cudaError_t dispatch(const BlockNormArgs& a, size_t groups, cudaStream_t s) {
         if (d <= 8192) return shape<1024, 8, V, false>(a, groups, s);
 #endif
         if (d <= kBlockNormMaxDim) return shape<1024, 16, V, false>(a, groups, s);
+    } else if (width == 2) {
+        if (d <= 256) return shape<32, 8, 2, false, kThreads>(a, groups, s);
+        if (d <= 1024) return shape<128, 8, 2, false, kThreads>(a, groups, s);
+        if (d <= 2048) return shape<256, 8, 2, false, kThreads>(a, groups, s);
+        if (d <= 4096) return shape<512, 8, 2, false>(a, groups, s);
+        if (d <= 8192) return shape<1024, 8, 2, false>(a, groups, s);
+        if (d <= kBlockNormMaxDim) return shape<1024, 16, 2, false>(a, groups, s);
     } else {
         if (d <= 256) return shape<32, 8, 1, false, kThreads>(a, groups, s);
         if (d <= 1024) return shape<128, 8, 1, false, kThreads>(a, groups, s);
+        if (d <= 2048) return shape<256, 8, 1, false, kThreads>(a, groups, s);
         if (d <= 4096) return shape<512, 8, 1, false>(a, groups, s);
+        if (d <= 8192) return shape<1024, 8, 1, false>(a, groups, s);
         if (d <= kBlockNormMaxDim) return shape<1024, 16, 1, false>(a, groups, s);
     }
     return cudaErrorInvalidValue;
