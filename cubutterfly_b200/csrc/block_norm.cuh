@@ -205,6 +205,18 @@ CUBF_DEV void load_vector(const void* base, bool is32, int j, int dim, float fil
     }
 }
 
+// Brings a row of `bytes` bytes towards L2: as one bulk prefetch by the row's
+// first thread, which alone calls it, where rows are whole 16-byte vectors; else
+// a line a thread.
+template <typename S>
+CUBF_DEV void prefetch_row(const void* row, uint32_t bytes, int j) {
+    if constexpr (S::kBulk) {
+        prefetch_l2(row, bytes);
+    } else if (static_cast<uint32_t>(j) * 128 < bytes) {
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const char*>(row) + j * 128));
+    }
+}
+
 CUBF_DEV float sigmoid(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
 
 // act(g), or its slope where SLOPE
@@ -539,11 +551,11 @@ __global__ void __launch_bounds__(S::kThreads, ForwardPlan<S, ROTATE>::template 
 
     for (int slot = 0; row < rows; row += stride, slot ^= 1) {
         if (!Plan::kAhead) load(row);
-        if (S::kBulk && j == 0 && row + Plan::kPrefetch * stride < rows) {  // towards L2, before it is loaded
+        if ((!S::kBulk || j == 0) && row + Plan::kPrefetch * stride < rows) {  // towards L2, before it is loaded
             const uint32_t n = row + Plan::kPrefetch * stride;
-            prefetch_l2(at(static_cast<const R*>(p.x), p.x_bytes, n), dim_bytes<R>(dim));
-            if (p.y) prefetch_l2(at(static_cast<const T*>(p.y), p.y_bytes, n), dim_bytes<T>(dim));
-            if (p.gate_mode == kGateFull) prefetch_l2(at(static_cast<const T*>(p.gate), p.gate_bytes, n), dim_bytes<T>(dim));
+            prefetch_row<S>(at(static_cast<const R*>(p.x), p.x_bytes, n), dim_bytes<R>(dim), j);
+            if (p.y) prefetch_row<S>(at(static_cast<const T*>(p.y), p.y_bytes, n), dim_bytes<T>(dim), j);
+            if (p.gate_mode == kGateFull) prefetch_row<S>(at(static_cast<const T*>(p.gate), p.gate_bytes, n), dim_bytes<T>(dim), j);
         }
         Pair s[S::HALF];
         Pair sum = both(0.f);
@@ -775,13 +787,13 @@ __global__ void __launch_bounds__(S::kThreads, 1) block_norm_backward_kernel(Blo
 
     for (int slot = 0; n < last; n += S::kRows, slot ^= 1) {
         const bool more = n + S::kRows < last;
-        if (S::kBulk && j == 0 && n + 2 * S::kRows < last) {  // towards L2, a row before it is loaded
+        if ((!S::kBulk || j == 0) && n + 2 * S::kRows < last) {  // towards L2, a row before it is loaded
             constexpr uint32_t kTwo = 2 * S::kRows;
-            prefetch_l2(at(static_cast<const R*>(p.x), p.x_bytes, kTwo), dim_bytes<R>(dim));
-            if (p.d_residual) prefetch_l2(at(static_cast<const R*>(p.d_residual), p.d_residual_bytes, kTwo), dim_bytes<R>(dim));
-            if (p.y) prefetch_l2(at(static_cast<const T*>(p.y), p.y_bytes, kTwo), dim_bytes<T>(dim));
-            if (p.d_normed) prefetch_l2(at(static_cast<const T*>(p.d_normed), p.d_normed_bytes, kTwo), dim_bytes<T>(dim));
-            if (row_gate) prefetch_l2(at(static_cast<const T*>(p.gate), p.gate_bytes, kTwo), dim_bytes<T>(dim));
+            prefetch_row<S>(at(static_cast<const R*>(p.x), p.x_bytes, kTwo), dim_bytes<R>(dim), j);
+            if (p.d_residual) prefetch_row<S>(at(static_cast<const R*>(p.d_residual), p.d_residual_bytes, kTwo), dim_bytes<R>(dim), j);
+            if (p.y) prefetch_row<S>(at(static_cast<const T*>(p.y), p.y_bytes, kTwo), dim_bytes<T>(dim), j);
+            if (p.d_normed) prefetch_row<S>(at(static_cast<const T*>(p.d_normed), p.d_normed_bytes, kTwo), dim_bytes<T>(dim), j);
+            if (row_gate) prefetch_row<S>(at(static_cast<const T*>(p.gate), p.gate_bytes, kTwo), dim_bytes<T>(dim), j);
         }
         Values<T, S> y_next, g_next;  // used first in the next row, and last in this one
         y_next.clear();
