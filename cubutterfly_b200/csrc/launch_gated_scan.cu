@@ -50,10 +50,10 @@ int piece_of(const GatedScanArgs& a, bool backward) {
 
 // Lane groups along time: each doubling makes twice as many CTAs, of half the
 // channels and twice the tokens a round.  Whole rows of 64 channels run
-// fastest once the CTAs fill the GPU (8 x 2048 x 2048 bf16, 256 CTAs: 58 us
-// forward; 65 and 72 us as 512 and 1024); below that more CTAs win (16384 x
-// 4096: 64, 128, 256 CTAs: 215, 126, 128 us forward and 415, 305, 236 us
-// backward, whose longer turns want two CTAs per SM).
+// fastest once the CTAs fill the GPU (8 x 2048 x 2048 bf16, 256, 512, 1024 and
+// 2048 CTAs: 60, 62, 69, 105 us forward, 101, 119, 122, 208 backward); below
+// that more CTAs win (16384 x 4096, 64 to 512 CTAs: 230, 115, 119, 196 us
+// forward and 402, 290, 246, 442 backward, whose turns want two CTAs per SM).
 int lane_groups(const GatedScanArgs& a, bool backward) {
     const int tile = (backward ? kBackwardSteps : kForwardSteps<T>) * kWarps;
     const int enough = backward ? 240 : 120;

@@ -314,7 +314,7 @@ def test_gated_scan_channels(cuda, dim, dtype):
 
 @pytest.mark.parametrize("batch,length,dim", [(1, 4099, 64), (1, 2000, 640), (5, 700, 128), (40, 129, 256)])
 def test_gated_scan_splits_of_time(cuda, batch, length, dim):
-    """Shapes whose time axis is split over clusters of different sizes."""
+    """Long sequences of few channels, and short ones of many."""
     check_scan(scan_case(batch, length, dim, BF16, states=batch), cuda)
 
 
@@ -362,7 +362,7 @@ def test_gated_scan_packed(cuda, packing, dtype, state):
         check_scan(scan_case(1, 150, dim, dtype, states=len(offsets) - 1 if state else None), cuda, offsets=offsets)
 
 
-def test_gated_scan_packed_over_clusters(cuda):
+def test_gated_scan_packed_over_many_rounds(cuda):
     g = torch.Generator().manual_seed(1)
     cuts = sorted(torch.randint(0, 3001, (60,), generator=g).tolist())
     offsets = [0, 0, *cuts, 3000, 3000]
