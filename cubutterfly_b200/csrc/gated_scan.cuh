@@ -147,9 +147,9 @@ struct Lane {
 // words.  Results take the place of words that have been read and leave the
 // same way: stored from registers, each pair would cost as many instructions in
 // addresses as its arithmetic.  Rows are copied in pieces of PIECE bytes, what
-// every row of every tensor is aligned for: 16 and 4 asynchronously, 2 (rows of
-// an odd number of 16-bit values) through registers.  Channels past the end are
-// zero; tokens past the end are what `close` says.
+// every row of every tensor is aligned for, 16 or 4 (ShiftedRows: 16-bit values
+// whose rows start at odd ones).  Channels past the end are zero; tokens past the
+// end are what `close` says.
 template <typename T, int N, int STEPS_, int STAGES_, int GROUPS, int PIECE>
 struct Rows {
     static constexpr int STEPS = STEPS_, STAGES = STAGES_, TOKENS = STEPS * GROUPS;
@@ -197,8 +197,7 @@ struct Rows {
     // starts the copies of tokens [t, t + TOKENS), closes their group, and
     // moves on by `advance` tokens
     CUBF_DEV void fetch(int stage, int t, int advance) {
-        unsigned char* const to = mine + stage * kBytes + piece_place();
-        const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+        const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(mine + stage * kBytes)) + piece_place();
         if (t >= 0 && t + TOKENS <= length && c0 + kChannels <= dim) {
 #pragma unroll
             for (int n = 0; n < N; ++n) {
@@ -211,13 +210,10 @@ struct Rows {
                         if constexpr (PIECE == 16)
                             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + place), "l"(src)
                                          : "memory");
-                        else if constexpr (PIECE == 4)
+                        else
                             asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + place),
                                          "l"(src + m * 32 * kElements)
                                          : "memory");
-                        else
-                            *reinterpret_cast<unsigned short*>(to + place) =
-                                __ldcs(reinterpret_cast<const unsigned short*>(src + m * 32 * kElements));
                     }
                     src += kRowsPer * stride[n];
                 }
@@ -236,13 +232,10 @@ struct Rows {
                             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + place), "l"(src),
                                          "r"(in ? 16 : 0)
                                          : "memory");
-                        else if constexpr (PIECE == 4)
+                        else
                             asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + place), "l"(src),
                                          "r"(in ? 4 : 0)
                                          : "memory");
-                        else
-                            *reinterpret_cast<unsigned short*>(to + place) =
-                                in ? __ldcs(reinterpret_cast<const unsigned short*>(src)) : static_cast<unsigned short>(0);
                     }
         } else {
             // nothing of the sequence: zeros, so that no stale word is computed with
@@ -258,6 +251,7 @@ struct Rows {
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
         __syncwarp();
     }
+    CUBF_DEV void begin(int) const {}  // the lane's run
     // The lane's token s.
     CUBF_DEV Pair get(int stage, int n, int s) const { return Raw<T>::get(*word(stage, n, s)); }
     // gives the lane's tokens past the end, its run beginning at t, the value
@@ -284,14 +278,194 @@ struct Rows {
                     T* to = dst + m * 32 * kElements;
                     if constexpr (PIECE == 16)
                         __stcs(reinterpret_cast<uint4*>(to), *reinterpret_cast<const uint4*>(from));
-                    else if constexpr (PIECE == 4)
-                        __stcs(reinterpret_cast<unsigned int*>(to), *reinterpret_cast<const unsigned int*>(from));
                     else
-                        __stcs(reinterpret_cast<unsigned short*>(to), *reinterpret_cast<const unsigned short*>(from));
+                        __stcs(reinterpret_cast<unsigned int*>(to), *reinterpret_cast<const unsigned int*>(from));
                 }
             dst += static_cast<size_t>(kRowsPer) * dim;
         }
     }
+};
+
+// The same for 16-bit values whose rows start at odd ones: the aligned 16-byte
+// pieces over a row's channels are copied, one more than the row has, and lie in
+// shared memory as they do in memory; the row's address modulo 16, its shift,
+// says where in them its values are.  Results go to the bytes that the lane's own
+// values came from.  Whole pieces of them leave as such, the first and last,
+// which the row shares with its neighbours, value by value.  Channels past the
+// end hold what lies there; no result of theirs is kept.
+// 2 x 8501 x 3947 fp16: 312 us forward, 640 backward; loaded value by value into
+// registers 635 and 1921.
+template <typename T, int N, int STEPS_, int STAGES_, int GROUPS>
+struct ShiftedRows {
+    static_assert(sizeof(T) == 2, "wider values are 4-byte aligned");
+    static constexpr int STEPS = STEPS_, STAGES = STAGES_, TOKENS = STEPS * GROUPS;
+    static constexpr int kChannels = kWarpChannels / GROUPS;
+    static constexpr int kLanes = 32 / GROUPS;
+    static constexpr int kSpan = 2 * kChannels;  // bytes of a row's channels
+    static constexpr int kRowBytes = kSpan + 16;
+    static constexpr int kTensorBytes = TOKENS * kRowBytes;
+    static constexpr int kBytes = N * kTensorBytes;
+    static constexpr int kPieces = kSpan / 16;
+    static constexpr int kRowsPer = 32 / kPieces;  // rows a warp copies at a time
+    static constexpr int kCopies = TOKENS / kRowsPer;
+    using Word = typename Raw<T>::Word;
+    using Half = unsigned short;
+    const T* base[N];
+    size_t stride[N];
+    unsigned char* mine;  // this warp's stages
+    int lane, c0, length, dim;
+    int token;  // where the lane's run begins
+
+    CUBF_DEV void init(unsigned char* shared, int lane_, int c0_, int length_, int dim_, int) {
+        mine = shared;
+        lane = lane_;
+        c0 = c0_;
+        length = length_;
+        dim = dim_;
+    }
+    CUBF_DEV void begin(int t0) { token = t0; }
+    static CUBF_DEV int place_of(int row) { return (row % STEPS * GROUPS + row / STEPS) * kRowBytes; }
+    CUBF_DEV unsigned char* tensor(int stage, int n) const { return mine + stage * kBytes + n * kTensorBytes; }
+    CUBF_DEV uintptr_t row_address(int n, int t) const {
+        return reinterpret_cast<uintptr_t>(base[n] + static_cast<size_t>(t) * stride[n] + c0);
+    }
+    CUBF_DEV uint32_t shift_of(int n, int t) const {
+        return (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base[n])) +
+                2u * (static_cast<uint32_t>(t) * static_cast<uint32_t>(stride[n]) + static_cast<uint32_t>(c0))) &
+               15u;
+    }
+    // the lane's pair of its token s
+    CUBF_DEV unsigned char* own(int stage, int n, int s) const {
+        return tensor(stage, n) + (s * GROUPS + lane / kLanes) * kRowBytes + 4 * (lane % kLanes) + shift_of(n, token + s);
+    }
+    static CUBF_DEV void copy(uint32_t to, uintptr_t from) {
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    }
+    CUBF_DEV void fetch(int stage, int t, int) {
+        const int bytes = 2 * (dim - c0 < kChannels ? dim - c0 : kChannels);
+        // Pieces reach over the row's ends: not in the first and last rows, where
+        // that may be outside the tensor (rows below 16 bytes: the first and last 16).
+        const int apart = dim >= 8 ? 1 : 16;
+        if (t >= apart && t + TOKENS + apart <= length) {
+            const int piece = lane % kPieces * 16;
+            const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(tensor(stage, 0)));
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                uintptr_t src = row_address(n, t + lane / kPieces);
+#pragma unroll
+                for (int k = 0; k < kCopies; ++k) {
+                    if (piece < static_cast<int>(src & 15) + bytes)
+                        copy(dst + n * kTensorBytes + place_of(k * kRowsPer + lane / kPieces) + piece,
+                             (src & ~static_cast<uintptr_t>(15)) + piece);
+                    src += 2 * kRowsPer * stride[n];
+                }
+#pragma unroll
+                for (int row = lane; row < TOKENS; row += 32) {
+                    const uintptr_t last = row_address(n, t + row);
+                    if (kSpan < static_cast<int>(last & 15) + bytes)
+                        copy(dst + n * kTensorBytes + place_of(row) + kSpan,
+                             (last & ~static_cast<uintptr_t>(15)) + kSpan);
+                }
+            }
+        } else {
+#pragma unroll 1
+            for (int e = lane; e < N * TOKENS * (kPieces + 1); e += 32) {
+                const int piece = e % (kPieces + 1) * 16, row = e / (kPieces + 1) % TOKENS;
+                const int n = e / (kPieces + 1) / TOKENS, at = t + row;
+                const T* origin = base[0];
+                size_t apart_by = stride[0];
+#pragma unroll
+                for (int m = 1; m < N; ++m)
+                    if (n == m) {
+                        origin = base[m];
+                        apart_by = stride[m];
+                    }
+                unsigned char* to = tensor(stage, 0) + n * kTensorBytes + place_of(row) + piece;
+                const bool in = at >= 0 && at < length;
+                const uintptr_t src = reinterpret_cast<uintptr_t>(origin + (in ? at * apart_by : 0) + c0);
+                const uintptr_t from = (src & ~static_cast<uintptr_t>(15)) + piece;
+                const uintptr_t lo = reinterpret_cast<uintptr_t>(origin);
+                const uintptr_t hi = reinterpret_cast<uintptr_t>(origin + static_cast<size_t>(length - 1) * apart_by + dim);
+                if (in && from >= lo && from + 16 <= hi) {
+                    copy(static_cast<uint32_t>(__cvta_generic_to_shared(to)), from);
+                } else {
+                    for (int j = 0; j < 16; j += 2) {
+                        const uintptr_t value = from + j;
+                        *reinterpret_cast<Half*>(to + j) =
+                            in && value >= lo && value < hi ? *reinterpret_cast<const Half*>(value) : static_cast<Half>(0);
+                    }
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    CUBF_DEV void arrive() const {
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        __syncwarp();
+    }
+    CUBF_DEV Pair get(int stage, int n, int s) const {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(own(stage, n, s));
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(at & ~static_cast<uintptr_t>(3));
+        return Raw<T>::get(__funnelshift_r(w[0], w[1], static_cast<uint32_t>(at & 2) * 8));
+    }
+    CUBF_DEV void write(int stage, int n, int s, Word w) const {
+        Half* to = reinterpret_cast<Half*>(own(stage, n, s));
+        to[0] = static_cast<Half>(w);
+        to[1] = static_cast<Half>(w >> 16);
+    }
+    CUBF_DEV void close(int stage, int n, int t, Word tail) const {
+        if (t + STEPS <= length) return;
+        for (int s = 0; s < STEPS; ++s)
+            if (t + s >= length) write(stage, n, s, tail);
+    }
+    CUBF_DEV void put(int stage, int n, int s, Pair v) const { write(stage, n, s, Raw<T>::word_of(floats(v))); }
+    CUBF_DEV void flush(int stage, int n, T* out, int t) const {
+        const uint32_t differ = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(out)) -
+                                static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base[n]));
+        const bool same = ((differ | 2u * (static_cast<uint32_t>(dim) - static_cast<uint32_t>(stride[n]))) & 15u) == 0;
+        if (same && c0 + kChannels <= dim) {  // out's rows have the shifts that its values lie at
+            const int piece = lane % kPieces * 16;
+            const unsigned char* from = tensor(stage, n);
+            uintptr_t to = reinterpret_cast<uintptr_t>(out + static_cast<size_t>(t + lane / kPieces) * dim + c0);
+#pragma unroll
+            for (int k = 0; k < kCopies; ++k) {
+                const int row = k * kRowsPer + lane / kPieces;
+                if ((piece > 0 || (to & 15) == 0) && t + row < length)
+                    __stcs(reinterpret_cast<uint4*>((to & ~static_cast<uintptr_t>(15)) + piece),
+                           *reinterpret_cast<const uint4*>(from + place_of(row) + piece));
+                to += 2 * static_cast<size_t>(kRowsPer) * dim;
+            }
+            // the 8 values of a row that are not in its whole pieces
+#pragma unroll 4
+            for (int e = lane; e < TOKENS * 8; e += 32) {
+                const int row = e / 8;
+                const uintptr_t first = reinterpret_cast<uintptr_t>(out + static_cast<size_t>(t + row) * dim + c0);
+                const int shift = static_cast<int>(first & 15);
+                int at = shift + e % 8 * 2;
+                if (at >= 16) at += kSpan - 16;
+                if (shift && t + row < length)
+                    *reinterpret_cast<Half*>(first - shift + at) = *reinterpret_cast<const Half*>(from + place_of(row) + at);
+            }
+        } else {
+            const int ch = c0 + 2 * (lane % kLanes);
+#pragma unroll 1
+            for (int s = 0; s < STEPS; ++s)
+                if (token + s < length) {
+                    const T* from = reinterpret_cast<const T*>(own(stage, n, s));
+                    T* to = out + static_cast<size_t>(token + s) * dim + ch;
+                    if (ch < dim) to[0] = from[0];
+                    if (ch + 1 < dim) to[1] = from[1];
+                }
+        }
+    }
+};
+template <typename T, int N, int STEPS, int STAGES, int GROUPS, int PIECE>
+struct RowsOf {
+    using type = Rows<T, N, STEPS, STAGES, GROUPS, PIECE>;
+};
+template <typename T, int N, int STEPS, int STAGES, int GROUPS>
+struct RowsOf<T, N, STEPS, STAGES, GROUPS, 2> {
+    using type = ShiftedRows<T, N, STEPS, STAGES, GROUPS>;
 };
 
 // ---- the arithmetic of a token ----------------------------------------------------------------
@@ -506,7 +680,7 @@ struct Joined {
 
 // ---- forward ----------------------------------------------------------------------------------
 template <typename T, int GROUPS, int PIECE>
-using ForwardRows = Rows<T, 3, kForwardSteps<T>, 2, GROUPS, PIECE>;
+using ForwardRows = typename RowsOf<T, 3, kForwardSteps<T>, 2, GROUPS, PIECE>::type;
 
 template <typename T, bool PACKED, int GROUPS, int PIECE>
 __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArgs p, int tiles) {
@@ -554,6 +728,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
         // the identity map.
         Pair a[kSteps], u[kSteps];
         rows.arrive();
+        rows.begin(t0);
         rows.close(buf, 1, t0, Raw<T>::lowest());
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
@@ -646,7 +821,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
 // A thread keeps a, v, 1/m and sigmoid(r) of its tokens and gets sigmoid(i)
 // back as v/m, which leaves room for two CTAs per SM.
 template <typename T, int GROUPS, int PIECE>
-using BackwardRows = Rows<T, 4, kBackwardSteps, sizeof(T) == 2 ? 2 : 1, GROUPS, PIECE>;
+using BackwardRows = typename RowsOf<T, 4, kBackwardSteps, sizeof(T) == 2 ? 2 : 1, GROUPS, PIECE>::type;
 
 template <typename T, bool PACKED, int GROUPS, int PIECE>
 __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(GatedScanArgs p, int tiles) {
@@ -703,6 +878,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(Gat
         // x and dh are read where they are used, from shared memory
         Pair a[kSteps], v[kSteps], im[kSteps], sr[kSteps];
         rows.arrive();
+        rows.begin(t0);
         rows.close(stage, 1, t0, Raw<T>::lowest());
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {

@@ -54,12 +54,18 @@ int piece_of(const GatedScanArgs& a, bool backward) {
 // 2048 CTAs: 60, 62, 69, 105 us forward, 101, 119, 122, 208 backward); below
 // that more CTAs win (16384 x 4096, 64 to 512 CTAs: 230, 115, 119, 196 us
 // forward and 402, 290, 246, 442 backward, whose turns want two CTAs per SM).
-int lane_groups(const GatedScanArgs& a, bool backward) {
+// Shifted rows take more shared memory: but for a backward CTA of up to 4 groups,
+// one CTA fits on an SM, and more CTAs win while that makes no second wave
+// (13 x 8000 x 143 bf16, 117 and 234 CTAs: 105, 181 us forward, 259, 317
+// backward; 32730 x 425, 27 and 54: 976, 588 us backward).
+int lane_groups(const GatedScanArgs& a, bool backward, int piece) {
     const int tile = (backward ? kBackwardSteps : kForwardSteps<T>) * kWarps;
-    const int enough = backward ? 240 : 120;
     int g = 1;
-    while (g < 8 && ceil_div(a.dim, kWarpChannels / g) * static_cast<long long>(a.batch) < enough && a.length > g * tile)
+    while (g < 8 && a.length > g * tile) {
+        const int enough = piece == 2 && (!backward || g == 4) ? 74 : backward ? 240 : 120;
+        if (ceil_div(a.dim, kWarpChannels / g) * static_cast<long long>(a.batch) >= enough) break;
         g *= 2;
+    }
     return g;
 }
 
@@ -87,7 +93,7 @@ cudaError_t launch_kernel(const GatedScanArgs& a, cudaStream_t stream) {
 template <bool PACKED, bool BACKWARD>
 cudaError_t launch_access(const GatedScanArgs& a, cudaStream_t stream) {
     const int piece = piece_of(a, BACKWARD);
-    const int groups = lane_groups(a, BACKWARD);
+    const int groups = lane_groups(a, BACKWARD, piece);
     if (piece >= 16) {
         switch (groups) {
             case 1: return launch_kernel<PACKED, 1, 16, BACKWARD>(a, stream);
@@ -99,9 +105,14 @@ cudaError_t launch_access(const GatedScanArgs& a, cudaStream_t stream) {
     if (piece >= 4)
         return groups <= 2 ? launch_kernel<PACKED, 2, 4, BACKWARD>(a, stream)
                            : launch_kernel<PACKED, 8, 4, BACKWARD>(a, stream);
-    if constexpr (sizeof(T) == 2)
-        return groups <= 2 ? launch_kernel<PACKED, 2, 2, BACKWARD>(a, stream)
-                           : launch_kernel<PACKED, 8, 2, BACKWARD>(a, stream);
+    if constexpr (sizeof(T) == 2) {
+        switch (groups) {
+            case 1: return launch_kernel<PACKED, 1, 2, BACKWARD>(a, stream);
+            case 2: return launch_kernel<PACKED, 2, 2, BACKWARD>(a, stream);
+            case 4: return launch_kernel<PACKED, 4, 2, BACKWARD>(a, stream);
+            default: return launch_kernel<PACKED, 8, 2, BACKWARD>(a, stream);
+        }
+    }
     return cudaErrorMisalignedAddress;
 }
 

@@ -449,6 +449,22 @@ def test_gated_scan_strided_inputs(cuda, dim, dtype):
         check_scan(t, cuda, view=view)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("batch,length,dim", [*((b, s, d + 1) for b, s, d in SPLITS),
+                                              *((3, 700, d) for d in (1, 3, 5, 7, 9))])
+def test_gated_scan_odd_rows_in_wider_ones(cuda, batch, length, dim, dtype):
+    """Rows of an odd length whose neighbours in memory, read with them, are NaN; tensors of different shifts."""
+    t = scan_case(batch, length, dim, dtype, states=batch, seed=dim)
+    for left, right in ((0, 0), (1, 0), (5, 2), (0, 1)):
+
+        def view(v):
+            wide = torch.full((*v.shape[:2], left + dim + right), float("nan"), dtype=v.dtype, device=v.device)
+            wide[..., left:left + dim] = v
+            return wide[..., left:left + dim]
+
+        check_scan(t, cuda, view=view)
+
+
 def test_gated_scan_no_tokens(cuda):
     decay = decay_of(16).to(cuda).requires_grad_()
     x = torch.empty(2, 0, 16, device=cuda, requires_grad=True)
