@@ -146,23 +146,19 @@ struct Lane {
 // lies at row s GROUPS + g, so that the lanes of all groups read adjacent
 // words.  Results take the place of words that have been read and leave the
 // same way: stored from registers, each pair would cost as many instructions in
-// addresses as its arithmetic.  Rows are copied in pieces of PIECE bytes, what
-// every row of every tensor is aligned for, 16 or 4 (ShiftedRows: 16-bit values
-// whose rows start at odd ones).  Channels past the end are zero; tokens past the
-// end are what `close` says.
-template <typename T, int N, int STEPS_, int STAGES_, int GROUPS, int PIECE>
+// addresses as its arithmetic.  Rows are copied in 16-byte pieces (ShiftedRows:
+// where they are not aligned for that).  Channels past the end are zero; tokens
+// past the end are what `close` says.
+template <typename T, int N, int STEPS_, int STAGES_, int GROUPS>
 struct Rows {
     static constexpr int STEPS = STEPS_, STAGES = STAGES_, TOKENS = STEPS * GROUPS;
     static constexpr int kChannels = kWarpChannels / GROUPS;
     static constexpr int kRowBytes = kChannels * static_cast<int>(sizeof(T));
     static constexpr int kTensorBytes = TOKENS * kRowBytes;
     static constexpr int kBytes = N * kTensorBytes;
-    static constexpr int kPerRow = kRowBytes / PIECE;                     // pieces of a row
-    static constexpr int kAcross = kPerRow < 32 ? kPerRow : 32;           // lanes along a row
-    static constexpr int kRowsPer = 32 / kAcross;                         // rows a warp copies at a time
-    static constexpr int kTimes = kPerRow / kAcross;                      // pieces a lane copies of a row
-    static constexpr int kCopies = TOKENS / kRowsPer;                     // rows a lane copies of a tensor
-    static constexpr int kElements = PIECE / static_cast<int>(sizeof(T));
+    static constexpr int kPerRow = kRowBytes / 16;     // pieces of a row
+    static constexpr int kRowsPer = 32 / kPerRow;      // rows a warp copies at a time
+    static constexpr int kCopies = TOKENS / kRowsPer;  // rows a lane copies of a tensor
     using Word = typename Raw<T>::Word;
     const T* base[N];
     size_t stride[N];
@@ -170,11 +166,11 @@ struct Rows {
     unsigned char* mine;  // this warp's stages
     int lane, c0, length, dim;
 
-    CUBF_DEV int column() const { return c0 + lane % kAcross * kElements; }
+    CUBF_DEV int column() const { return c0 + lane % kPerRow * (16 / static_cast<int>(sizeof(T))); }
     // where this lane's piece of the k-th rows lies: what follows from the lane, and from k
     CUBF_DEV int piece_place() const {
-        const int r = lane / kAcross;
-        return (r % STEPS * GROUPS + r / STEPS) * kRowBytes + lane % kAcross * PIECE;
+        const int r = lane / kPerRow;
+        return (r % STEPS * GROUPS + r / STEPS) * kRowBytes + lane % kPerRow * 16;
     }
     static constexpr int row_place(int k) {
         return (k * kRowsPer % STEPS * GROUPS + k * kRowsPer / STEPS) * kRowBytes;
@@ -188,7 +184,7 @@ struct Rows {
         dim = dim_;
 #pragma unroll
         for (int n = 0; n < N; ++n)
-            next[n] = base[n] + static_cast<ptrdiff_t>(first + lane / kAcross) * static_cast<ptrdiff_t>(stride[n]) +
+            next[n] = base[n] + static_cast<ptrdiff_t>(first + lane / kPerRow) * static_cast<ptrdiff_t>(stride[n]) +
                       column();
     }
     CUBF_DEV Word* word(int stage, int n, int s) const {  // of the lane's own token s
@@ -204,39 +200,24 @@ struct Rows {
                 const T* src = next[n];
 #pragma unroll
                 for (int k = 0; k < kCopies; ++k) {
-#pragma unroll
-                    for (int m = 0; m < kTimes; ++m) {
-                        const int place = n * kTensorBytes + row_place(k) + m * 32 * PIECE;
-                        if constexpr (PIECE == 16)
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + place), "l"(src)
-                                         : "memory");
-                        else
-                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + place),
-                                         "l"(src + m * 32 * kElements)
-                                         : "memory");
-                    }
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + n * kTensorBytes + row_place(k)),
+                                 "l"(src)
+                                 : "memory");
                     src += kRowsPer * stride[n];
                 }
             }
         } else if (t < length && t + TOKENS > 0) {
             for (int n = 0; n < N; ++n)
 #pragma unroll
-                for (int k = 0; k < kCopies; ++k)
-#pragma unroll
-                    for (int m = 0; m < kTimes; ++m) {
-                        const int at = t + lane / kAcross + k * kRowsPer, col = column() + m * 32 * kElements;
-                        const bool in = at >= 0 && at < length && col < dim;
-                        const T* src = in ? base[n] + static_cast<size_t>(at) * stride[n] + col : base[n];
-                        const int place = n * kTensorBytes + row_place(k) + m * 32 * PIECE;
-                        if constexpr (PIECE == 16)
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + place), "l"(src),
-                                         "r"(in ? 16 : 0)
-                                         : "memory");
-                        else
-                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + place), "l"(src),
-                                         "r"(in ? 4 : 0)
-                                         : "memory");
-                    }
+                for (int k = 0; k < kCopies; ++k) {
+                    const int at = t + lane / kPerRow + k * kRowsPer;
+                    const bool in = at >= 0 && at < length && column() < dim;
+                    const T* src = in ? base[n] + static_cast<size_t>(at) * stride[n] + column() : base[n];
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + n * kTensorBytes +
+                                                                                      row_place(k)),
+                                 "l"(src), "r"(in ? 16 : 0)
+                                 : "memory");
+                }
         } else {
             // nothing of the sequence: zeros, so that no stale word is computed with
             for (int k = 0; k < kBytes / 512; ++k)
@@ -266,50 +247,47 @@ struct Rows {
     // writes the tile put in tensor n's place, the warp's tokens from t, out to rows of `dim` channels
     CUBF_DEV void flush(int stage, int n, T* out, int t) const {
         const unsigned char* src = mine + stage * kBytes + n * kTensorBytes + piece_place();
-        const int row = t + lane / kAcross, col = column();
+        const int row = t + lane / kPerRow, col = column();
         T* dst = out + static_cast<size_t>(row) * dim + col;
         const bool whole = t + TOKENS <= length && c0 + kChannels <= dim;
 #pragma unroll
         for (int k = 0; k < kCopies; ++k) {
-#pragma unroll
-            for (int m = 0; m < kTimes; ++m)
-                if (whole || (row + k * kRowsPer < length && col + m * 32 * kElements < dim)) {
-                    const unsigned char* from = src + row_place(k) + m * 32 * PIECE;
-                    T* to = dst + m * 32 * kElements;
-                    if constexpr (PIECE == 16)
-                        __stcs(reinterpret_cast<uint4*>(to), *reinterpret_cast<const uint4*>(from));
-                    else
-                        __stcs(reinterpret_cast<unsigned int*>(to), *reinterpret_cast<const unsigned int*>(from));
-                }
+            if (whole || (row + k * kRowsPer < length && col < dim))
+                __stcs(reinterpret_cast<uint4*>(dst), *reinterpret_cast<const uint4*>(src + row_place(k)));
             dst += static_cast<size_t>(kRowsPer) * dim;
         }
     }
 };
 
-// The same for 16-bit values whose rows start at odd ones: the aligned 16-byte
-// pieces over a row's channels are copied, one more than the row has, and lie in
+// The same for rows that are not 16-byte aligned: the aligned 16-byte pieces
+// over a row's channels are copied, one more than the row has, and lie in
 // shared memory as they do in memory; the row's address modulo 16, its shift,
 // says where in them its values are.  Results go to the bytes that the lane's own
 // values came from.  Whole pieces of them leave as such, the first and last,
-// which the row shares with its neighbours, value by value.  Channels past the
+// which the row shares with its neighbours, unit by unit.  Channels past the
 // end hold what lies there; no result of theirs is kept.
-// 2 x 8501 x 3947 fp16: 312 us forward, 640 backward; loaded value by value into
-// registers 635 and 1921.
-template <typename T, int N, int STEPS_, int STAGES_, int GROUPS>
+// 2 x 8501 x 3947 fp16: 313 us forward, 633 backward; loaded value by value into
+// registers 635 and 1921.  2 x 8500 x 3946: 233 and 416; copied in 4-byte pieces
+// 356 and 477.
+// PIECE is what shifts are multiples of: 4, or 2 where a pair of 16-bit values
+// may straddle two words.
+template <typename T, int N, int STEPS_, int STAGES_, int GROUPS, int PIECE>
 struct ShiftedRows {
-    static_assert(sizeof(T) == 2, "wider values are 4-byte aligned");
+    static_assert(PIECE == 4 || (PIECE == 2 && sizeof(T) == 2), "rows are aligned for their values");
     static constexpr int STEPS = STEPS_, STAGES = STAGES_, TOKENS = STEPS * GROUPS;
     static constexpr int kChannels = kWarpChannels / GROUPS;
     static constexpr int kLanes = 32 / GROUPS;
-    static constexpr int kSpan = 2 * kChannels;  // bytes of a row's channels
+    static constexpr int kSize = static_cast<int>(sizeof(T));
+    static constexpr int kSpan = kSize * kChannels;  // bytes of a row's channels
     static constexpr int kRowBytes = kSpan + 16;
     static constexpr int kTensorBytes = TOKENS * kRowBytes;
     static constexpr int kBytes = N * kTensorBytes;
     static constexpr int kPieces = kSpan / 16;
     static constexpr int kRowsPer = 32 / kPieces;  // rows a warp copies at a time
     static constexpr int kCopies = TOKENS / kRowsPer;
+    static constexpr int kEdge = 16 / PIECE;  // units of a shifted row outside its whole pieces
     using Word = typename Raw<T>::Word;
-    using Half = unsigned short;
+    using Unit = std::conditional_t<PIECE == 2, unsigned short, unsigned int>;
     const T* base[N];
     size_t stride[N];
     unsigned char* mine;  // this warp's stages
@@ -331,21 +309,22 @@ struct ShiftedRows {
     }
     CUBF_DEV uint32_t shift_of(int n, int t) const {
         return (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base[n])) +
-                2u * (static_cast<uint32_t>(t) * static_cast<uint32_t>(stride[n]) + static_cast<uint32_t>(c0))) &
+                kSize * (static_cast<uint32_t>(t) * static_cast<uint32_t>(stride[n]) + static_cast<uint32_t>(c0))) &
                15u;
     }
     // the lane's pair of its token s
     CUBF_DEV unsigned char* own(int stage, int n, int s) const {
-        return tensor(stage, n) + (s * GROUPS + lane / kLanes) * kRowBytes + 4 * (lane % kLanes) + shift_of(n, token + s);
+        return tensor(stage, n) + (s * GROUPS + lane / kLanes) * kRowBytes + 2 * kSize * (lane % kLanes) +
+               shift_of(n, token + s);
     }
     static CUBF_DEV void copy(uint32_t to, uintptr_t from) {
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
     }
     CUBF_DEV void fetch(int stage, int t, int) {
-        const int bytes = 2 * (dim - c0 < kChannels ? dim - c0 : kChannels);
+        const int bytes = kSize * (dim - c0 < kChannels ? dim - c0 : kChannels);
         // Pieces reach over the row's ends: not in the first and last rows, where
         // that may be outside the tensor (rows below 16 bytes: the first and last 16).
-        const int apart = dim >= 8 ? 1 : 16;
+        const int apart = dim * kSize >= 16 ? 1 : 16;
         if (t >= apart && t + TOKENS + apart <= length) {
             const int piece = lane % kPieces * 16;
             const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(tensor(stage, 0)));
@@ -357,7 +336,7 @@ struct ShiftedRows {
                     if (piece < static_cast<int>(src & 15) + bytes)
                         copy(dst + n * kTensorBytes + place_of(k * kRowsPer + lane / kPieces) + piece,
                              (src & ~static_cast<uintptr_t>(15)) + piece);
-                    src += 2 * kRowsPer * stride[n];
+                    src += kSize * kRowsPer * stride[n];
                 }
 #pragma unroll
                 for (int row = lane; row < TOKENS; row += 32) {
@@ -389,10 +368,10 @@ struct ShiftedRows {
                 if (in && from >= lo && from + 16 <= hi) {
                     copy(static_cast<uint32_t>(__cvta_generic_to_shared(to)), from);
                 } else {
-                    for (int j = 0; j < 16; j += 2) {
-                        const uintptr_t value = from + j;
-                        *reinterpret_cast<Half*>(to + j) =
-                            in && value >= lo && value < hi ? *reinterpret_cast<const Half*>(value) : static_cast<Half>(0);
+                    for (int j = 0; j < 16; j += PIECE) {
+                        const uintptr_t unit = from + j;
+                        *reinterpret_cast<Unit*>(to + j) =
+                            in && unit >= lo && unit < hi ? *reinterpret_cast<const Unit*>(unit) : static_cast<Unit>(0);
                     }
                 }
             }
@@ -404,14 +383,28 @@ struct ShiftedRows {
         __syncwarp();
     }
     CUBF_DEV Pair get(int stage, int n, int s) const {
-        const uintptr_t at = reinterpret_cast<uintptr_t>(own(stage, n, s));
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(at & ~static_cast<uintptr_t>(3));
-        return Raw<T>::get(__funnelshift_r(w[0], w[1], static_cast<uint32_t>(at & 2) * 8));
+        if constexpr (kSize == 4) {
+            const float* f = reinterpret_cast<const float*>(own(stage, n, s));
+            return f32x2::pk(f[0], f[1]);
+        } else if constexpr (PIECE == 2) {
+            const uintptr_t at = reinterpret_cast<uintptr_t>(own(stage, n, s));
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(at & ~static_cast<uintptr_t>(3));
+            return Raw<T>::get(__funnelshift_r(w[0], w[1], static_cast<uint32_t>(at & 2) * 8));
+        } else {
+            return Raw<T>::get(*reinterpret_cast<const Word*>(own(stage, n, s)));
+        }
     }
     CUBF_DEV void write(int stage, int n, int s, Word w) const {
-        Half* to = reinterpret_cast<Half*>(own(stage, n, s));
-        to[0] = static_cast<Half>(w);
-        to[1] = static_cast<Half>(w >> 16);
+        unsigned char* to = own(stage, n, s);
+        if constexpr (kSize == 4) {
+            reinterpret_cast<float*>(to)[0] = w.x;
+            reinterpret_cast<float*>(to)[1] = w.y;
+        } else if constexpr (PIECE == 2) {
+            reinterpret_cast<Unit*>(to)[0] = static_cast<Unit>(w);
+            reinterpret_cast<Unit*>(to)[1] = static_cast<Unit>(w >> 16);
+        } else {
+            *reinterpret_cast<Word*>(to) = w;
+        }
     }
     CUBF_DEV void close(int stage, int n, int t, Word tail) const {
         if (t + STEPS <= length) return;
@@ -422,7 +415,7 @@ struct ShiftedRows {
     CUBF_DEV void flush(int stage, int n, T* out, int t) const {
         const uint32_t differ = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(out)) -
                                 static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base[n]));
-        const bool same = ((differ | 2u * (static_cast<uint32_t>(dim) - static_cast<uint32_t>(stride[n]))) & 15u) == 0;
+        const bool same = ((differ | kSize * (static_cast<uint32_t>(dim) - static_cast<uint32_t>(stride[n]))) & 15u) == 0;
         if (same && c0 + kChannels <= dim) {  // out's rows have the shifts that its values lie at
             const int piece = lane % kPieces * 16;
             const unsigned char* from = tensor(stage, n);
@@ -433,18 +426,18 @@ struct ShiftedRows {
                 if ((piece > 0 || (to & 15) == 0) && t + row < length)
                     __stcs(reinterpret_cast<uint4*>((to & ~static_cast<uintptr_t>(15)) + piece),
                            *reinterpret_cast<const uint4*>(from + place_of(row) + piece));
-                to += 2 * static_cast<size_t>(kRowsPer) * dim;
+                to += kSize * static_cast<size_t>(kRowsPer) * dim;
             }
-            // the 8 values of a row that are not in its whole pieces
 #pragma unroll 4
-            for (int e = lane; e < TOKENS * 8; e += 32) {
-                const int row = e / 8;
+            for (int e = lane; e < TOKENS * kEdge; e += 32) {
+                const int row = e / kEdge;
                 const uintptr_t first = reinterpret_cast<uintptr_t>(out + static_cast<size_t>(t + row) * dim + c0);
                 const int shift = static_cast<int>(first & 15);
-                int at = shift + e % 8 * 2;
+                int at = shift + e % kEdge * PIECE;
                 if (at >= 16) at += kSpan - 16;
                 if (shift && t + row < length)
-                    *reinterpret_cast<Half*>(first - shift + at) = *reinterpret_cast<const Half*>(from + place_of(row) + at);
+                    *reinterpret_cast<Unit*>(first - shift + at) =
+                        *reinterpret_cast<const Unit*>(from + place_of(row) + at);
             }
         } else {
             const int ch = c0 + 2 * (lane % kLanes);
@@ -460,13 +453,8 @@ struct ShiftedRows {
     }
 };
 template <typename T, int N, int STEPS, int STAGES, int GROUPS, int PIECE>
-struct RowsOf {
-    using type = Rows<T, N, STEPS, STAGES, GROUPS, PIECE>;
-};
-template <typename T, int N, int STEPS, int STAGES, int GROUPS>
-struct RowsOf<T, N, STEPS, STAGES, GROUPS, 2> {
-    using type = ShiftedRows<T, N, STEPS, STAGES, GROUPS>;
-};
+using RowsOf = std::conditional_t<PIECE == 16, Rows<T, N, STEPS, STAGES, GROUPS>,
+                                  ShiftedRows<T, N, STEPS, STAGES, GROUPS, PIECE == 16 ? 4 : PIECE>>;
 
 // ---- the arithmetic of a token ----------------------------------------------------------------
 CUBF_DEV float ex2(float x) {
@@ -680,7 +668,7 @@ struct Joined {
 
 // ---- forward ----------------------------------------------------------------------------------
 template <typename T, int GROUPS, int PIECE>
-using ForwardRows = typename RowsOf<T, 3, kForwardSteps<T>, 2, GROUPS, PIECE>::type;
+using ForwardRows = RowsOf<T, 3, kForwardSteps<T>, 2, GROUPS, PIECE>;
 
 template <typename T, bool PACKED, int GROUPS, int PIECE>
 __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArgs p, int tiles) {
@@ -821,7 +809,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
 // A thread keeps a, v, 1/m and sigmoid(r) of its tokens and gets sigmoid(i)
 // back as v/m, which leaves room for two CTAs per SM.
 template <typename T, int GROUPS, int PIECE>
-using BackwardRows = typename RowsOf<T, 4, kBackwardSteps, sizeof(T) == 2 ? 2 : 1, GROUPS, PIECE>::type;
+using BackwardRows = RowsOf<T, 4, kBackwardSteps, sizeof(T) == 2 ? 2 : 1, GROUPS, PIECE>;
 
 template <typename T, bool PACKED, int GROUPS, int PIECE>
 __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(GatedScanArgs p, int tiles) {

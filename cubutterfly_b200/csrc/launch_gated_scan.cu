@@ -21,6 +21,8 @@ namespace {
 using namespace scan;
 using T = std::conditional_t<CUBF_GS_TYPE == 0, __half, std::conditional_t<CUBF_GS_TYPE == 1, __nv_bfloat16, float>>;
 
+constexpr int kTwoPerSM = 110 * 1024;  // dynamic shared memory of a CTA that fits twice beside the static 2 to 6 KB
+
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 // The widest access, in bytes, that every row of every tensor is aligned for.
@@ -54,15 +56,17 @@ int piece_of(const GatedScanArgs& a, bool backward) {
 // 2048 CTAs: 60, 62, 69, 105 us forward, 101, 119, 122, 208 backward); below
 // that more CTAs win (16384 x 4096, 64 to 512 CTAs: 230, 115, 119, 196 us
 // forward and 402, 290, 246, 442 backward, whose turns want two CTAs per SM).
-// Shifted rows take more shared memory: but for a backward CTA of up to 4 groups,
-// one CTA fits on an SM, and more CTAs win while that makes no second wave
-// (13 x 8000 x 143 bf16, 117 and 234 CTAs: 105, 181 us forward, 259, 317
-// backward; 32730 x 425, 27 and 54: 976, 588 us backward).
+// Shifted rows take more shared memory: where only one CTA of twice the groups
+// fits on an SM, those are taken while they make no second wave (13 x 8000 x 143
+// bf16, 117 and 234 CTAs: 105, 181 us forward, 259, 317 backward; 32730 x 425, 27
+// and 54: 976, 588 us backward).
 int lane_groups(const GatedScanArgs& a, bool backward, int piece) {
     const int tile = (backward ? kBackwardSteps : kForwardSteps<T>) * kWarps;
+    const int stage = (backward ? 4 * BackwardRows<T, 1, 16>::STAGES : 3 * ForwardRows<T, 1, 16>::STAGES) * tile;
     int g = 1;
     while (g < 8 && a.length > g * tile) {
-        const int enough = piece == 2 && (!backward || g == 4) ? 74 : backward ? 240 : 120;
+        const int shared = stage * (kWarpChannels * static_cast<int>(sizeof(T)) + (piece < 16 ? 2 * g * 16 : 0));
+        const int enough = shared > kTwoPerSM ? 74 : backward ? 240 : 120;
         if (ceil_div(a.dim, kWarpChannels / g) * static_cast<long long>(a.batch) >= enough) break;
         g *= 2;
     }
@@ -102,9 +106,14 @@ cudaError_t launch_access(const GatedScanArgs& a, cudaStream_t stream) {
             default: return launch_kernel<PACKED, 8, 16, BACKWARD>(a, stream);
         }
     }
-    if (piece >= 4)
-        return groups <= 2 ? launch_kernel<PACKED, 2, 4, BACKWARD>(a, stream)
-                           : launch_kernel<PACKED, 8, 4, BACKWARD>(a, stream);
+    if (piece >= 4) {
+        switch (groups) {
+            case 1: return launch_kernel<PACKED, 1, 4, BACKWARD>(a, stream);
+            case 2: return launch_kernel<PACKED, 2, 4, BACKWARD>(a, stream);
+            case 4: return launch_kernel<PACKED, 4, 4, BACKWARD>(a, stream);
+            default: return launch_kernel<PACKED, 8, 4, BACKWARD>(a, stream);
+        }
+    }
     if constexpr (sizeof(T) == 2) {
         switch (groups) {
             case 1: return launch_kernel<PACKED, 1, 2, BACKWARD>(a, stream);
