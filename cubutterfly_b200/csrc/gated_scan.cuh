@@ -739,8 +739,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
                 }
             }
         }
+        // One way for the whole warp: two in turn would take as long as both.
+        const bool plain = !PACKED || __all_sync(0xffffffffu, marks.none());
         Pair A = both(1.f), H = both(0.f);
-        if (!PACKED || marks.starts == 0) {
+        if (plain) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 A = mul2(A, a[s]);
@@ -748,8 +750,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
             }
         } else {
 #pragma unroll
-            for (int s = 0; s < kSteps; ++s) H = (marks.starts >> s) & 1u ? u[s] : fma2(a[s], H, u[s]);
-            A = kMarker;
+            for (int s = 0; s < kSteps; ++s) {
+                A = mul2(A, a[s]);
+                H = (marks.starts >> s) & 1u ? u[s] : fma2(a[s], H, u[s]);
+            }
+            if (marks.starts) A = kMarker;
         }
         // The state goes from warp to warp, and from the last one to the first
         // one's next tile; no barrier holds all warps, so they drift apart and
@@ -772,7 +777,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
         if (GROUPS > 1 && group > 0) h = through<PACKED>(runs.before_a, runs.before_h, h);  // before the lane's run
         if (chunk_states && t0 % kGatedScanChunk == 0 && t0 < p.length)
             ln.store32(chunk_states + static_cast<size_t>(t0 / kGatedScanChunk) * p.dim, h);
-        if (!PACKED || marks.none()) {
+        if (plain) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 h = fma2(a[s], h, u[s]);
@@ -886,6 +891,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(Gat
             if (t0 < seq.start) seq.rewind();
             marks.find(seq, t0, kSteps, p.length);
         }
+        const bool plain = !PACKED || __all_sync(0xffffffffu, marks.none());  // one way for the whole warp
         // h before a sequence's first token, and the final state's gradient at its last
         auto initial_of = [&](int at) {
             return p.initial ? ln.load32(p.initial + static_cast<size_t>(at) * p.dim) : both(0.f);
@@ -893,7 +899,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(Gat
         auto last_of = [&](int at) {
             return p.d_last ? ln.load32(p.d_last + static_cast<size_t>(at) * p.dim) : both(0.f);
         };
-        if (!PACKED || marks.none()) {
+        if (plain) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 A = mul2(A, a[s]);
@@ -969,7 +975,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(Gat
             rows.put(stage, 2, s, gi);
             return e;
         };
-        if (!PACKED || marks.none()) {
+        if (plain) {
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
                 before[s] = h;
