@@ -38,11 +38,13 @@ using Pair = f32x2::P;
 constexpr int kWarps = 8;                  // warps per CTA, consecutive in time
 constexpr int kWarpChannels = 64;          // channels times lane groups of a warp: two channels per lane
 // Tokens per thread and tile: as many as two CTAs' registers and shared
-// memory allow.
-template <typename T>
-constexpr int kForwardSteps = sizeof(T) == 2 ? 16 : 8;
+// memory allow.  Forward rows that are not 16-byte aligned take more of the
+// latter (6 x 3602 x 974 bf16 with 8 and 16 tokens: 91, 107 us; 16384 x 4098, of
+// one CTA per SM either way: 233, 217).
+template <typename T, int PIECE>
+constexpr int kForwardSteps = sizeof(T) == 2 && PIECE == 16 ? 16 : 8;
 constexpr int kBackwardSteps = 8;
-static_assert(kGatedScanChunk == 2 * kBackwardSteps && kGatedScanChunk % kForwardSteps<__half> == 0,
+static_assert(kGatedScanChunk == 2 * kBackwardSteps && kGatedScanChunk % kForwardSteps<__half, 16> == 0,
               "chunks begin where a forward warp and every other backward warp do");
 
 CUBF_DEV Pair both(float v) { return f32x2::pk(v, v); }
@@ -266,8 +268,8 @@ struct Rows {
 // values came from.  Whole pieces of them leave as such, the first and last,
 // which the row shares with its neighbours, unit by unit.  Channels past the
 // end hold what lies there; no result of theirs is kept.
-// 2 x 8501 x 3947 fp16: 313 us forward, 633 backward; loaded value by value into
-// registers 635 and 1921.  2 x 8500 x 3946: 233 and 416; copied in 4-byte pieces
+// 2 x 8501 x 3947 fp16: 304 us forward, 633 backward; loaded value by value into
+// registers 635 and 1921.  2 x 8500 x 3946: 239 and 416; copied in 4-byte pieces
 // 356 and 477.
 // PIECE is what shifts are multiples of: 4, or 2 where a pair of 16-bit values
 // may straddle two words.
@@ -668,7 +670,7 @@ struct Joined {
 
 // ---- forward ----------------------------------------------------------------------------------
 template <typename T, int GROUPS, int PIECE>
-using ForwardRows = RowsOf<T, 3, kForwardSteps<T>, 2, GROUPS, PIECE>;
+using ForwardRows = RowsOf<T, 3, kForwardSteps<T, PIECE>, 2, GROUPS, PIECE>;
 
 template <typename T, bool PACKED, int GROUPS, int PIECE>
 __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArgs p, int tiles) {

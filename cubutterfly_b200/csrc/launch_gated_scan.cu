@@ -58,10 +58,10 @@ int piece_of(const GatedScanArgs& a, bool backward) {
 // forward and 402, 290, 246, 442 backward, whose turns want two CTAs per SM).
 // Shifted rows take more shared memory: where only one CTA of twice the groups
 // fits on an SM, those are taken while they make no second wave (13 x 8000 x 143
-// bf16, 117 and 234 CTAs: 105, 181 us forward, 259, 317 backward; 32730 x 425, 27
-// and 54: 976, 588 us backward).
+// bf16 backward, 117 and 234 CTAs: 259, 317 us; 32730 x 425, 27 and 54: 976, 588).
 int lane_groups(const GatedScanArgs& a, bool backward, int piece) {
-    const int tile = (backward ? kBackwardSteps : kForwardSteps<T>) * kWarps;
+    const int steps = backward ? kBackwardSteps : piece < 16 ? kForwardSteps<T, 4> : kForwardSteps<T, 16>;
+    const int tile = steps * kWarps;
     const int stage = (backward ? 4 * BackwardRows<T, 1, 16>::STAGES : 3 * ForwardRows<T, 1, 16>::STAGES) * tile;
     int g = 1;
     while (g < 8 && a.length > g * tile) {
