@@ -111,19 +111,24 @@ struct Rows {
     Tensor t;  // as given, or a contiguous copy
     int64_t stride = 0;
 };
-// `t` as rows of `dim` consecutive values one stride apart.
+// `t` as rows of `dim` consecutive values one stride apart: as it is, where its
+// leading dimensions merge into one of separate rows, else copied.  Rows that
+// coincide or overlap (a broadcast dimension has stride zero, as the gradient of
+// a sum over it has) are copied.
 Rows rows_of(const Tensor& t, int64_t dim) {
     if (t.is_contiguous()) return {t, dim};
-    const int64_t n = t.dim();
-    bool fits = t.size(-1) == 1 || t.stride(-1) == 1;
-    int64_t stride = 0, expected = 0;  // of the dimensions before the last, merged from the inner one
-    for (int64_t d = n - 2; d >= 0 && fits; --d) {
+    bool fits = t.size(-1) == 1 || t.stride(-1) == 1, seen = false;
+    int64_t stride = dim, expected = 0;  // of the dimensions before the last, merged from the inner one
+    for (int64_t d = t.dim() - 2; d >= 0 && fits; --d) {
         if (t.size(d) == 1) continue;
-        if (stride == 0) stride = t.stride(d);
-        fits = expected == 0 || t.stride(d) == expected;
+        if (seen)
+            fits = t.stride(d) == expected;
+        else
+            stride = t.stride(d);
+        seen = true;
         expected = t.stride(d) * t.size(d);
     }
-    if (fits && (stride >= dim || (stride == 0 && expected == 0))) return {t, stride ? stride : dim};
+    if (fits && stride >= dim) return {t, stride};
     return {t.contiguous(), dim};
 }
 

@@ -58,6 +58,41 @@ def test_row_strides():
     assert block_ops._block_ops.tokens(torch.empty(4, 1, 16).expand(4, 6, 16), 16)[1:] == (96, 16)
 
 
+# (shape of the values, shape they are broadcast to)
+BROADCASTS = [((1, 16), (5, 16)), ((3, 1, 16), (3, 5, 16)), ((16,), (3, 5, 16)), ((1, 5, 16), (3, 5, 16)),
+              ((1, 1, 16), (3, 1, 16)), ((2, 1, 3, 16), (2, 4, 3, 16)), ((2, 3, 1, 16), (2, 3, 4, 16)), ((1, 1), (5, 1))]
+
+
+@pytest.mark.parametrize("small,wide", BROADCASTS)
+def test_broadcast_rows_are_copied(small, wide):
+    """Rows that share memory have no stride of their own; so has the gradient of a sum over rows."""
+    dim = wide[-1]
+    base = torch.randn(*small)
+    for t in (base.expand(*wide), base.expand(*wide).unsqueeze(0)):
+        rows, stride = block_ops._block_ops.rows(t, dim)
+        assert stride == dim and rows.is_contiguous() and torch.equal(rows, t)
+        assert rows.untyped_storage().nbytes() >= 4 * t.numel()
+    seen = []
+    v = torch.zeros(*wide, requires_grad=True)
+    w = v * 1
+    w.register_hook(seen.append)
+    (w.sum_to_size(*small) * base).sum().backward()
+    rows, stride = block_ops._block_ops.rows(seen[0], dim)
+    assert stride == dim and rows.is_contiguous() and torch.equal(rows, seen[0])
+    assert rows.untyped_storage().nbytes() >= 4 * v.numel()
+
+
+def test_overlapping_rows_are_copied():
+    base = torch.randn(200)
+    for size, strides in (((5, 16), (4, 1)), ((4, 1, 16), (7, 3, 1)), ((2, 5, 16), (75, 15, 1))):
+        t = base.as_strided(size, strides)
+        rows, stride = block_ops._block_ops.rows(t, 16)
+        assert stride == 16 and rows.is_contiguous() and torch.equal(rows, t)
+    one = base.as_strided((1, 3, 16), (0, 20, 1))   # a stride of a single index means nothing
+    rows, stride = block_ops._block_ops.rows(one, 16)
+    assert stride == 20 and rows.data_ptr() == base.data_ptr()
+
+
 # Fields of a valid call; device pointers are never dereferenced by the checks.
 P = 4096
 

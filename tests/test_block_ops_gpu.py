@@ -585,6 +585,74 @@ def test_steps_follow_the_scan(cuda):
     ref.assert_close(state, final, ref.SCAN_LOSS)
 
 
+# (which leading axes of (3, 5, D) are broadcast)
+@pytest.mark.parametrize("axes", [(0,), (1,), (0, 1)])
+@pytest.mark.parametrize("dtype,dim,rotate", [(BF16, 64, True), (FP16, 33, False), (FP32, 258, False)])
+def test_block_norm_broadcast_inputs(cuda, axes, dtype, dim, rotate):
+    """x, y and the gate as views whose rows share memory (strides of zero) are their values written out."""
+    t = norm_case((3, 5, dim), dtype, gate="full", seed=dim)
+
+    def first(v):
+        for a in axes:
+            v = v.narrow(a, 0, 1)
+        return v
+
+    for k in ("x", "y", "gate"):
+        t[k] = first(t[k]).expand(3, 5, dim).contiguous()
+    views = []
+
+    def view(v):
+        views.append(first(v).clone().expand(3, 5, dim))
+        return views[-1]
+
+    check_norm(t, cuda, act="silu", rotate=rotate, view=view)
+    assert len(views) == 3 and not any(v.is_contiguous() for v in views)
+
+
+def test_block_norm_broadcast_gate_per_group(cuda):
+    t = norm_case((4, 6, 72), BF16, gate="group")
+    t["gate"] = t["gate"][:1].expand(4, 1, 72).contiguous()
+    check_norm(t, cuda, act="sigmoid",
+               view=lambda v: v[:1].clone().expand(4, 1, 72) if v.shape[1] == 1 else v)
+
+
+@pytest.mark.parametrize("of", ["residual", "normed"])
+@pytest.mark.parametrize("axes", [(0,), (1,), (0, 1)])
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (FP32, 33)])
+def test_block_norm_gradient_of_sums_over_rows(cuda, of, axes, dtype, dim):
+    """The gradient of a sum over leading axes arrives with strides of zero there and one along the channels."""
+    t = norm_case((3, 5, dim), dtype, gate="channel", seed=dim + 1)
+    w = normal(77, dim, dtype=dtype)
+    dev = {k: v.to(cuda).requires_grad_() for k, v in t.items() if torch.is_tensor(v)}
+    exact = {k: v.double().requires_grad_() for k, v in t.items() if torch.is_tensor(v)}
+    call = lambda f, p: f(p["x"], p["y"], pre_weight=p["pre"], post_weight=p["post"], gate=p["gate"])
+    pick = 0 if of == "residual" else 1
+    seen = []
+    out = call(torch_ops.block_norm, dev)[pick]
+    out.register_hook(seen.append)
+    (out.sum(axes) * w.to(cuda)).sum().backward()
+    (call(ref.block_norm, exact)[pick].sum(axes) * w.double()).sum().backward()
+    assert seen[0].stride(-1) == 1 and any(seen[0].stride(a) == 0 for a in axes)
+    for k in dev:
+        if exact[k].grad is not None:
+            summed = k in ("pre", "post", "gate")
+            ref.assert_close(dev[k].grad, exact[k].grad, ref.NORM_LOSS * (math.sqrt(15) if summed else 2), "d_" + k)
+
+
+def test_gated_scan_step_broadcast_inputs(cuda):
+    """One token's x and gates shared by all requests of the batch."""
+    batch, dim = 5, 72
+    t = scan_case(1, 1, dim, BF16)
+    x, r, i = (t[k][0].to(cuda).expand(batch, dim) for k in "xri")
+    before = normal(9, batch, dim)
+    state = before.to(cuda)
+    h = torch_ops.gated_scan_step(state, x, r, i, t["decay"].to(cuda))
+    wide = doubles(*(t[k].expand(batch, 1, dim) for k in "xri"), t["decay"], before)
+    eh, ef = ref.gated_scan(*wide[:4], initial=wide[4])
+    ref.assert_close(h, eh[:, 0], ref.SCAN_LOSS)
+    ref.assert_close(state, ef, ref.SCAN_LOSS)
+
+
 # ---- streams, graphs, repeatability ------------------------------------------------------------
 def all_operators(cuda, seed=0):
     n = norm_case((40, 512), BF16, FP32, gate="channel", scale="vector", seed=seed)
