@@ -88,11 +88,19 @@ int data_type(at::ScalarType t) {
     }
 }
 
+// Refuses what these calls, which stand outside torch's dispatcher, would drop
+// without a word: a tangent.
+void check_plain(const Tensor& t, const char* what) {
+    REQUIRE(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), what,
+            " carries a forward-mode tangent: the block operators have reverse-mode gradients only");
+}
+
 // A CUDA tensor out of an argument; None where `optional`.
 Tensor tensor_of(py::handle h, const char* what, bool optional = false) {
     if (optional && h.is_none()) return {};
     REQUIRE(THPVariable_Check(h.ptr()), what, " must be a CUDA tensor");
     const Tensor& t = THPVariable_Unpack(h.ptr());
+    check_plain(t, what);
     REQUIRE(t.is_cuda(), what, " must be a CUDA tensor");
     return t;
 }

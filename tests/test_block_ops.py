@@ -28,6 +28,23 @@ def test_cpu_tensors_are_rejected():
         torch_ops.gated_scan_step(x, x, x, x, x[0])
 
 
+def test_forward_mode_tangents_are_refused():
+    """A tangent would be dropped, which reads as a derivative of zero."""
+    import torch.autograd.forward_ad as fwd
+
+    zeros = torch.zeros(4, 64, device="meta")  # no CUDA tensor either: the tangent is looked at first
+    with fwd.dual_level():
+        dual = fwd.make_dual(torch.zeros(4, 64), torch.ones(4, 64))
+        with pytest.raises(ValueError, match="x carries a forward-mode tangent"):
+            torch_ops.block_norm(dual)
+        with pytest.raises(ValueError, match="x carries a forward-mode tangent"):
+            torch_ops.gated_scan(dual[None], zeros, zeros, zeros)
+        with pytest.raises(ValueError, match="x carries a forward-mode tangent"):
+            torch_ops.gated_scan_step(zeros, dual, zeros, zeros, zeros)
+        with fwd._set_fwd_grad_enabled(False), pytest.raises(ValueError, match="CUDA"):
+            torch_ops.block_norm(dual)
+
+
 def test_torch_ops_exports_the_block_operators():
     for name in ("block_norm", "gated_scan", "gated_scan_step"):
         assert name in torch_ops.__all__ and getattr(torch_ops, name) is getattr(block_ops, name)

@@ -760,6 +760,28 @@ def test_refusals_on_the_device(cuda):
             call()
 
 
+def test_forward_mode_tangents_are_refused(cuda):
+    import torch.autograd.forward_ad as fwd
+
+    x = torch.randn(3, 64, device=cuda)
+    w, state = torch.ones(64, device=cuda), torch.zeros(3, 64, device=cuda)
+    with fwd.dual_level():
+        dual, dw = fwd.make_dual(x, torch.ones_like(x)), fwd.make_dual(w, torch.ones_like(w))
+        ds = fwd.make_dual(state, torch.ones_like(state))
+        for call in (lambda: torch_ops.block_norm(dual), lambda: torch_ops.block_norm(x, dual),
+                     lambda: torch_ops.block_norm(x, x, gate=dual), lambda: torch_ops.block_norm(x, x, pre_weight=dw),
+                     lambda: torch_ops.block_norm(x, x, post_weight=dw),
+                     lambda: torch_ops.block_norm(x, x, residual_scale=dw),
+                     lambda: torch_ops.gated_scan(x[None], dual[None], x[None], w),
+                     lambda: torch_ops.gated_scan(x[None], x[None], dual[None], w),
+                     lambda: torch_ops.gated_scan(x[None], x[None], x[None], dw),
+                     lambda: torch_ops.gated_scan(x[None], x[None], x[None], w, initial_state=ds[:1]),
+                     lambda: torch_ops.gated_scan_step(ds, x, x, x, w), lambda: torch_ops.gated_scan_step(state, x, x, x, dw)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+        torch_ops.block_norm(x, x, pre_weight=w)  # a level without a tangent among the arguments
+
+
 def test_library_refusals_name_their_status(cuda):
     x = torch.randn(2, 96, device=cuda)
     with pytest.raises(cb.Error, match="power-of-two") as e:
