@@ -11,6 +11,7 @@
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -89,8 +90,11 @@ int data_type(at::ScalarType t) {
 }
 
 // Refuses what these calls, which stand outside torch's dispatcher, would drop
-// without a word: a tangent.
+// without a word: a tangent, and what a subclass or a transform keeps elsewhere than in storage of the tensor's own (its data pointer
+// may be null, which here means an argument left out).
 void check_plain(const Tensor& t, const char* what) {
+    REQUIRE(t.has_storage() && !t.unsafeGetTensorImpl()->is_python_dispatch(), what,
+            " must be a CUDA tensor with storage of its own, not a wrapper of others");
     REQUIRE(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), what,
             " carries a forward-mode tangent: the block operators have reverse-mode gradients only");
 }

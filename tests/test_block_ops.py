@@ -45,6 +45,37 @@ def test_forward_mode_tangents_are_refused():
             torch_ops.block_norm(dual)
 
 
+class Wrapper(torch.Tensor):
+    """A tensor whose values are somewhere else: the data pointer is null."""
+    @staticmethod
+    def __new__(cls, *shape):
+        return torch.Tensor._make_wrapper_subclass(cls, shape, device="cuda", dtype=torch.float32)
+
+    def __init__(self, *shape):
+        pass
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError(func)
+
+
+def test_wrapper_tensors_are_refused():
+    """A wrapped weight's data pointer is null, as that of a weight left out."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    x = torch.zeros(4, 64)
+    with FakeTensorMode():
+        fake = torch.empty(4, 64, device="cuda")
+    for v in (Wrapper(4, 64), fake):
+        for call in (lambda: torch_ops.block_norm(v), lambda: torch_ops.gated_scan(v, x, x, x),
+                     lambda: torch_ops.gated_scan_step(x, v, x, x, x)):
+            with pytest.raises(ValueError, match="x must be a CUDA tensor with storage of its own"):
+                call()
+    for transform in (torch.func.vmap, torch.func.grad):
+        with pytest.raises(ValueError, match="storage of its own"):
+            transform(lambda v: torch_ops.block_norm(v)[1])(x)
+
+
 def test_torch_ops_exports_the_block_operators():
     for name in ("block_norm", "gated_scan", "gated_scan_step"):
         assert name in torch_ops.__all__ and getattr(torch_ops, name) is getattr(block_ops, name)

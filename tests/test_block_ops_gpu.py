@@ -782,6 +782,30 @@ def test_forward_mode_tangents_are_refused(cuda):
         torch_ops.block_norm(x, x, pre_weight=w)  # a level without a tangent among the arguments
 
 
+def test_wrapped_weights_are_refused(cuda):
+    """A weight without storage of its own is refused wherever it stands, not left out."""
+    from test_block_ops import Wrapper
+
+    x = torch.randn(3, 64, device=cuda)
+    w = Wrapper(64)
+    for call in (lambda: torch_ops.block_norm(x, x, pre_weight=w), lambda: torch_ops.block_norm(x, x, post_weight=w),
+                 lambda: torch_ops.block_norm(x, x, gate=w), lambda: torch_ops.block_norm(x, x, residual_scale=w),
+                 lambda: torch_ops.gated_scan(x[None], x[None], x[None], x[0], initial_state=Wrapper(1, 64)),
+                 lambda: torch_ops.gated_scan_step(x, x, x, x, x[0], slots=Wrapper(3))):
+        with pytest.raises(ValueError, match="storage of its own"):
+            call()
+
+
+def test_counting_modes_pass(cuda):
+    """Modes that only watch the dispatcher do not stand in the way."""
+    from torch.utils.flop_counter import FlopCounterMode
+
+    x = torch.randn(3, 64, device=cuda)
+    want = torch_ops.block_norm(x)[1]
+    with FlopCounterMode(display=False):
+        assert torch.equal(torch_ops.block_norm(x)[1], want)
+
+
 def test_library_refusals_name_their_status(cuda):
     x = torch.randn(2, 96, device=cuda)
     with pytest.raises(cb.Error, match="power-of-two") as e:
