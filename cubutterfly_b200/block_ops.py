@@ -8,7 +8,8 @@
 The calls run on the caller's current CUDA stream, allocate only through torch, never synchronise and can be captured
 in CUDA graphs.  ``block_norm`` and ``gated_scan`` are differentiable (once); arithmetic is fp32 whatever the tensors'
 type, with one rounding per output.  They take plain tensors: one with a forward-mode tangent, without storage of its
-own (DTensor, FakeTensor, under ``torch.func`` transforms) is refused.  ``cubutterfly_b200.torch_ops`` exports the operators beside the transforms.
+own (DTensor, FakeTensor, under ``torch.func`` transforms) or under a trace (``torch.jit.trace``, ``make_fx``) is
+refused.  ``cubutterfly_b200.torch_ops`` exports the operators beside the transforms.
 
 Arguments are checked, outputs allocated and gradients recorded by the extension ``_block_ops``
 (csrc/block_ops_torch.cpp), which calls the C entry points of the loaded library.

@@ -12,11 +12,13 @@
 
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/core/AutogradState.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
 #include <string>
@@ -90,9 +92,14 @@ int data_type(at::ScalarType t) {
 }
 
 // Refuses what these calls, which stand outside torch's dispatcher, would drop
-// without a word: a tangent, and what a subclass or a transform keeps elsewhere than in storage of the tensor's own (its data pointer
+// without a word: a tangent, the record of a trace, and what a subclass or a
+// transform keeps elsewhere than in storage of the tensor's own (its data pointer
 // may be null, which here means an argument left out).
 void check_plain(const Tensor& t, const char* what) {
+    const bool proxies = c10::impl::TorchDispatchModeTLS::any_modes_set() &&
+                         c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value();
+    REQUIRE(!proxies && !torch::jit::tracer::isTracing(), what,
+            " is being traced: the block operators cannot be recorded, only run or captured in a CUDA graph");
     REQUIRE(t.has_storage() && !t.unsafeGetTensorImpl()->is_python_dispatch(), what,
             " must be a CUDA tensor with storage of its own, not a wrapper of others");
     REQUIRE(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), what,

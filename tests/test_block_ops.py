@@ -76,6 +76,19 @@ def test_wrapper_tensors_are_refused():
             transform(lambda v: torch_ops.block_norm(v)[1])(x)
 
 
+def test_traces_are_refused():
+    """A trace would record the outputs as constants, or as the empty tensors they begin as."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = torch.zeros(4, 64)
+    for call in (lambda v: torch_ops.block_norm(v)[1], lambda v: torch_ops.gated_scan(v, v, v, v)[0],
+                 lambda v: torch_ops.gated_scan_step(v, v, v, v, v)):
+        with pytest.raises(ValueError, match="x is being traced"):
+            torch.jit.trace(call, (x,))
+        with pytest.raises(ValueError, match="x is being traced"):
+            make_fx(call)(x)
+
+
 def test_torch_ops_exports_the_block_operators():
     for name in ("block_norm", "gated_scan", "gated_scan_step"):
         assert name in torch_ops.__all__ and getattr(torch_ops, name) is getattr(block_ops, name)
