@@ -673,6 +673,8 @@ Tensor gated_scan_step(py::handle hstate, py::handle hx, py::handle hr, py::hand
     a.h = h.data_ptr();
     const c10::cuda::CUDAGuard guard(x.device());
     check(abi.scan_step(&a, c10::cuda::getCurrentCUDAStream()));
+    // a backward that kept this pool has to see that it changed
+    if (!next.is_inference()) next.unsafeGetTensorImpl()->bump_version();
     return h;
 }
 

@@ -653,6 +653,24 @@ def test_gated_scan_step_broadcast_inputs(cuda):
     ref.assert_close(state, ef, ref.SCAN_LOSS)
 
 
+def test_gated_scan_step_marks_its_writes(cuda):
+    """A pool that a backward still needs may not change unnoticed under it."""
+    x = normal(1, 2, 5, 64).to(cuda).requires_grad_()
+    decay = decay_of(64).to(cuda)
+    pool, other = normal(2, 2, 64).to(cuda), torch.zeros(2, 64, device=cuda)
+    token = normal(3, 2, 64).to(cuda)
+    h, _ = torch_ops.gated_scan(x, x, x, decay, initial_state=pool)
+    torch_ops.gated_scan_step(pool, token, token, token, decay, new_state=other)   # the pool stays
+    h.sum().backward()
+    h, _ = torch_ops.gated_scan(x, x, x, decay, initial_state=pool)
+    torch_ops.gated_scan_step(pool, token, token, token, decay)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        h.sum().backward()
+    with torch.inference_mode():   # tensors without a version
+        pool = torch.zeros(2, 64, device=cuda)
+        torch_ops.gated_scan_step(pool, token, token, token, decay)
+
+
 # ---- streams, graphs, repeatability ------------------------------------------------------------
 def all_operators(cuda, seed=0):
     n = norm_case((40, 512), BF16, FP32, gate="channel", scale="vector", seed=seed)
