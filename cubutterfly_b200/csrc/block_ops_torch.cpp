@@ -646,7 +646,7 @@ Tensor gated_scan_step(py::handle hstate, py::handle hx, py::handle hr, py::hand
         REQUIRE(state.size(0) >= batch, "gated_scan_step: ", std::to_string(batch),
                 " requests without slots need a pool of as many rows");
     }
-    REQUIRE(!any_requires_grad({&state, &x, &r, &i}), "gated_scan_step is inference only: an input requires grad");
+    REQUIRE(!any_requires_grad({&state, &next, &x, &r, &i, &decay}), "gated_scan_step is inference only: an input requires grad");
     check_exponent(exponent, "gated_scan_step");
     at::NoGradGuard no_grad;
     decay = decay.to(at::kFloat).contiguous();

@@ -824,6 +824,18 @@ def test_counting_modes_pass(cuda):
         assert torch.equal(torch_ops.block_norm(x)[1], want)
 
 
+def test_gated_scan_step_refuses_a_decay_that_requires_grad(cuda):
+    state, x = torch.zeros(3, 64, device=cuda), torch.randn(3, 64, device=cuda)
+    decay = decay_of(64).to(cuda).requires_grad_()
+    leaf = torch.zeros(3, 64, device=cuda, requires_grad=True)
+    with pytest.raises(ValueError, match="inference only"):
+        torch_ops.gated_scan_step(state, x, x, x, decay)
+    with pytest.raises(ValueError, match="inference only"):
+        torch_ops.gated_scan_step(state, x, x, x, decay.detach(), new_state=leaf)
+    with torch.no_grad():
+        torch_ops.gated_scan_step(state, x, x, x, decay)
+
+
 def test_library_refusals_name_their_status(cuda):
     x = torch.randn(2, 96, device=cuda)
     with pytest.raises(cb.Error, match="power-of-two") as e:
