@@ -3,8 +3,9 @@
 Run ``python -m cubutterfly_b200._build`` (or ``__graft_entry__.build()``).
 Objects go to ``cubutterfly_b200/_build/``, the library to
 ``cubutterfly_b200/lib/libcubutterfly_b200.so``, the torch extension of the
-block operators to ``cubutterfly_b200/_block_ops.so``.  Compilation units are built
-in parallel and only when their sources changed.
+block operators to ``cubutterfly_b200/_block_ops.so`` (where torch is
+installed).  Compilation units are built in parallel and only when their
+sources changed.
 """
 from __future__ import annotations
 
@@ -83,15 +84,18 @@ def _stale(obj: Path) -> bool:
 
 
 def _build_torch_extension() -> None:
-    """The block operators' torch extension (host code only; it links against torch, not against the library)."""
-    src = CSRC / "block_ops_torch.cpp"
-    deps = [src, ROOT / "include" / "cubutterfly" / "cubutterfly_b200.h", Path(__file__)]
-    if TORCH_EXT.exists() and all(d.stat().st_mtime <= TORCH_EXT.stat().st_mtime for d in deps):
+    """The block operators' torch extension (host code only; it links against torch, not against the library).
+
+    Nothing is built where torch is absent: the library and its other frontends do without it.
+    """
+    try:
+        import torch
+    except ImportError:
         return
     import sysconfig
 
-    import torch
-
+    src = CSRC / "block_ops_torch.cpp"
+    deps = [src, ROOT / "include" / "cubutterfly" / "cubutterfly_b200.h", Path(__file__)]
     torch_dir = Path(torch.__file__).parent
     includes = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include",
                 Path(NVCC).parents[1] / "include", sysconfig.get_paths()["include"], ROOT / "include"]
@@ -99,6 +103,8 @@ def _build_torch_extension() -> None:
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{i}" for i in includes], str(src),
            "-o", str(TORCH_EXT), f"-L{torch_dir / 'lib'}", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10",
            "-lc10_cuda"]
+    if TORCH_EXT.exists() and all(d.stat().st_mtime <= TORCH_EXT.stat().st_mtime for d in deps):
+        return
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")

@@ -1,0 +1,51 @@
+"""The build without a compiler: what is compiled, linked and rebuilt, and what a failure leaves behind."""
+import os
+import subprocess
+import sys
+from types import SimpleNamespace
+
+import pytest
+
+from cubutterfly_b200 import _build
+
+
+@pytest.fixture
+def build(tmp_path, monkeypatch):
+    """build() over one unit in a folder of its own; `ran` lists what was made, `failing` holds what fails."""
+    obj = tmp_path / "obj" / "unit.o"
+    paths = dict(OBJ=obj.parent, LIB_DIR=tmp_path / "lib", LIB=tmp_path / "lib" / "lib.so",
+                 TORCH_EXT=tmp_path / "ext.so")
+    for name, path in paths.items():
+        monkeypatch.setattr(_build, name, path)
+    monkeypatch.setattr(_build, "_units", lambda: [(["cc", "-o", str(obj)], _build.CSRC / "unit.cu", obj)])
+    ran, failing = [], set()
+
+    def run(cmd, **kwargs):
+        target = cmd[cmd.index("-o") + 1]
+        ran.append(os.path.basename(target))
+        if ran[-1] in failing:
+            return subprocess.CompletedProcess(cmd, 1, "", "it failed")
+        open(target, "w").close()
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    monkeypatch.setattr(_build.subprocess, "run", run)
+
+    def call():
+        ran.clear()
+        return _build.build()
+
+    return SimpleNamespace(call=call, ran=ran, failing=failing, obj=obj, **paths)
+
+
+def test_builds_once(build):
+    assert build.call() == build.LIB
+    assert sorted(build.ran) == ["ext.so", "lib.so", "unit.o"]
+    build.call()
+    assert build.ran == []
+
+
+def test_library_without_torch(build, monkeypatch):
+    """The C ABI needs no torch: a host without it gets the library."""
+    monkeypatch.setitem(sys.modules, "torch", None)
+    assert build.call() == build.LIB and build.LIB.exists()
+    assert "ext.so" not in build.ran
