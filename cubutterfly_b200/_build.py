@@ -128,13 +128,14 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
     with ThreadPoolExecutor(max_workers=jobs or max(2, os.cpu_count() or 2)) as ex:
         extension = ex.submit(_build_torch_extension)
         list(ex.map(run, todo))
-        extension.result()
-    if todo or not LIB.exists():
+    # linked whatever became of the extension, and whenever an object is newer (a build before may have stopped there)
+    if not LIB.exists() or any(u[2].stat().st_mtime > LIB.stat().st_mtime for u in units):
         cmd = [NVCC, *ARCH, "-shared", "-o", str(LIB), *[str(u[2]) for u in units], "-cudart", "static",
                "-Xlinker", "--no-undefined", "-lpthread", "-ldl", "-lrt"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    extension.result()
     return LIB
 
 

@@ -49,3 +49,22 @@ def test_library_without_torch(build, monkeypatch):
     monkeypatch.setitem(sys.modules, "torch", None)
     assert build.call() == build.LIB and build.LIB.exists()
     assert "ext.so" not in build.ran
+
+
+def test_library_is_linked_when_the_extension_fails(build):
+    build.failing.add("ext.so")
+    with pytest.raises(RuntimeError, match="it failed"):
+        build.call()
+    assert build.LIB.exists()
+    build.failing.clear()
+    build.call()
+    assert build.ran == ["ext.so"]
+
+
+def test_library_is_linked_from_newer_objects(build):
+    """Objects that a build compiled without linking them are linked by the next one."""
+    build.call()
+    later = build.LIB.stat().st_mtime + 10
+    os.utime(build.obj, (later, later))
+    build.call()
+    assert build.ran == ["lib.so"]
