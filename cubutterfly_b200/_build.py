@@ -5,7 +5,7 @@ Objects go to ``cubutterfly_b200/_build/``, the library to
 ``cubutterfly_b200/lib/libcubutterfly_b200.so``, the torch extension of the
 block operators to ``cubutterfly_b200/_block_ops.so`` (where torch is
 installed).  Compilation units are built in parallel and only when their
-sources changed.
+sources changed, the extension also when torch or Python did.
 """
 from __future__ import annotations
 
@@ -103,11 +103,14 @@ def _build_torch_extension() -> None:
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *[f"-I{i}" for i in includes], str(src),
            "-o", str(TORCH_EXT), f"-L{torch_dir / 'lib'}", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10",
            "-lc10_cuda"]
-    if TORCH_EXT.exists() and all(d.stat().st_mtime <= TORCH_EXT.stat().st_mtime for d in deps):
+    stamp, built_for = OBJ / "block_ops_torch.txt", f"python {sys.version}, torch {torch.__version__}"
+    if (TORCH_EXT.exists() and stamp.exists() and stamp.read_text() == built_for
+            and all(d.stat().st_mtime <= TORCH_EXT.stat().st_mtime for d in deps)):
         return
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    stamp.write_text(built_for)
 
 
 def build(verbose: bool = False, jobs: int | None = None) -> Path:

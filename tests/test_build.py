@@ -68,3 +68,14 @@ def test_library_is_linked_from_newer_objects(build):
     os.utime(build.obj, (later, later))
     build.call()
     assert build.ran == ["lib.so"]
+
+
+def test_extension_follows_torch(build, monkeypatch):
+    import torch
+
+    build.call()
+    monkeypatch.setattr(torch, "__version__", torch.__version__ + ".other")
+    build.call()
+    assert build.ran == ["ext.so"]
+    build.call()
+    assert build.ran == []
