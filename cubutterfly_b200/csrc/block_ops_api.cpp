@@ -146,6 +146,7 @@ cubf::BlockNormArgs norm_args(const cubutterflyB200BlockNorm_t* a, bool backward
     n.rotate_scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(a->dim)));
     n.post_norm = post;
     n.rotate = rotate;
+    require(element_aligned(a->post_rms, 4) && element_aligned(a->pre_rms, 4), "block norm: misaligned post_rms or pre_rms");
     n.pre32 = vector_is_32(a->pre_weight, a->pre_type, *block, "block norm pre_type");
     n.post32 = vector_is_32(a->post_weight, a->post_type, *block, "block norm post_type");
     n.scales32 = vector_is_32(a->scale, a->scale_type, *block, "block norm scale_type");
@@ -190,6 +191,10 @@ cubf::BlockNormArgs norm_args(const cubutterflyB200BlockNorm_t* a, bool backward
     require(element_aligned(a->d_residual, er) && element_aligned(a->d_normed, es) && element_aligned(a->d_x, er) &&
                 element_aligned(a->d_y, es),
             "block norm: misaligned gradient");
+    auto vector_aligned = [&](const void* p, bool is32) { return element_aligned(p, is32 ? 4 : es); };
+    require(vector_aligned(a->d_gate, n.gate32) && vector_aligned(a->d_pre_weight, n.pre32) &&
+                vector_aligned(a->d_post_weight, n.post32) && vector_aligned(a->d_scale, n.scales32),
+            "block norm: misaligned gradient of a gate, weight or scale");
     n.d_residual = a->d_residual;
     n.d_normed = a->d_normed;
     n.d_residual_bytes = a->d_residual ? bytes(a->d_residual_row, er) : 0;
@@ -246,7 +251,7 @@ cubf::GatedScanArgs scan_args(const cubutterflyB200GatedScan_t* a, bool backward
     for (const void* p : {static_cast<const void*>(a->decay), static_cast<const void*>(a->initial_state),
                           static_cast<const void*>(a->offsets), static_cast<const void*>(a->chunk_states),
                           static_cast<const void*>(a->final_state), static_cast<const void*>(a->d_final_state),
-                          static_cast<const void*>(a->d_initial_state)})
+                          static_cast<const void*>(a->d_initial_state), static_cast<const void*>(a->d_decay)})
         require(element_aligned(p, 4), "gated scan: misaligned vector or state");
     cubf::GatedScanArgs s{};
     s.x = a->x;

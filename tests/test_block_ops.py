@@ -296,6 +296,27 @@ def test_gated_scan_step_refusals(lib, change, status, text):
     refused(lib, "B200GatedScanStep", step_fields(**change), status, text)
 
 
+@pytest.mark.parametrize("change,text", [
+    (dict(post_rms=P + 2), "misaligned post_rms"),
+    (dict(pre_rms=P + 1), "misaligned post_rms"),
+    (dict(gate=P, gate_rows=1, d_gate=P + 2), "misaligned gradient of a gate"),
+    (dict(gate=P, gate_rows=4, gate_row=64, d_gate=P + 1), "misaligned gradient of a gate"),
+    (dict(pre=P, d_pre=P + 2), "misaligned gradient of a gate"),
+    (dict(post=P, post_type=1, d_post=P + 1), "misaligned gradient of a gate"),
+    (dict(scales=P, d_scale=P + 3), "misaligned gradient of a gate"),
+])
+def test_block_norm_backward_refuses_misaligned_vectors(lib, change, text):
+    valid = dict(post_rms=P, pre_rms=P, d_res=P, dr_row=64, d_x=P, d_y=P, workspace=P, bytes=1 << 20)
+    refused(lib, "B200BlockNormBackward", norm_fields(**{**valid, **change}), STATUS.INVALID_VALUE, text)
+
+
+def test_forward_and_scan_refuse_misaligned_vectors(lib):
+    refused(lib, "B200BlockNormForward", norm_fields(post_rms=P + 2, pre_rms=P), STATUS.INVALID_VALUE,
+            "misaligned post_rms")
+    valid = dict(chunks=P, d_h=P, db=640, dt=64, d_x=P, d_r=P, d_i=P, workspace=P, bytes=1 << 20)
+    refused(lib, "B200GatedScanBackward", scan_fields(**valid, d_decay=P + 2), STATUS.INVALID_VALUE, "misaligned")
+
+
 def test_null_arguments(lib):
     for name in ("BlockNormForward", "BlockNormBackward", "GatedScanForward", "GatedScanBackward", "GatedScanStep"):
         refused(lib, "B200" + name, None, STATUS.INVALID_VALUE, "null arguments")
