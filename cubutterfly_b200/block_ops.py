@@ -90,8 +90,9 @@ def gated_scan_step(state, x, recurrence_gate, input_gate, decay, *, exponent=8.
     """One token of ``gated_scan`` for a batch of requests: returns h (B, D) and updates the states.
 
     ``x`` and the gates are (B, D); ``state`` is a pool of fp32 states (P, D), contiguous, updated in place unless
-    ``new_state`` (another such pool) takes the new rows.  Request b's state is row ``slots[b]`` (int32, on the device;
-    row b without ``slots``).  A slot outside the pool, such as -1, marks padding: that request's h is zero and no
-    state changes.  Distinct requests need distinct slots.  Inference only: under grad mode no argument may require grad.
+    ``new_state`` (another such pool, apart from it) takes the new rows.  Request b's state is row ``slots[b]`` (int32,
+    on the device; row b without ``slots``).  A slot outside the pool, such as -1, marks padding: that request's h is
+    zero and no state changes.  Distinct requests need distinct slots.  Inference only: under grad mode no argument may
+    require grad.
     """
     return _block_ops.gated_scan_step(state, x, recurrence_gate, input_gate, decay, exponent, slots, new_state)

@@ -399,6 +399,11 @@ extern "C" cubutterflyStatus_t cubutterflyB200GatedScanStep(const cubutterflyB20
         for (const void* p : {static_cast<const void*>(a->decay), static_cast<const void*>(a->state),
                               static_cast<const void*>(a->new_state), static_cast<const void*>(a->slots)})
             require(element_aligned(p, 4), "gated scan step: misaligned vector or state");
+        // in place, or apart: between, a request would read a row that another one's step writes
+        const uintptr_t from = reinterpret_cast<uintptr_t>(a->state), to = reinterpret_cast<uintptr_t>(a->new_state);
+        const size_t bytes = a->pool * a->dim * sizeof(float);
+        require(from == to || from + bytes <= to || to + bytes <= from,
+                "gated scan step: new_state must be state or not overlap it");
         cubf::GatedStepArgs s{};
         s.x = a->x;
         s.r = a->recurrence_gate;

@@ -275,9 +275,10 @@ CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200GatedScanBackward(const cubutt
 
 /* One token of the recurrence for `batch` requests: request b's state is row
  * slots[b] (b where slots is null) of `state` ((pool, dim) fp32, contiguous);
- * the new one goes to the same row of new_state (state itself: in place).  A
- * slot outside [0, pool) marks padding: that request's h is zero and no state
- * is read or written.  Distinct requests need distinct slots. */
+ * the new one goes to the same row of new_state (state itself: in place; else
+ * a pool that does not overlap it).  A slot outside [0, pool) marks padding:
+ * that request's h is zero and no state is read or written.  Distinct requests
+ * need distinct slots. */
 typedef struct cubutterflyB200GatedScanStep_s {
     size_t struct_size;
     size_t batch, dim, pool;

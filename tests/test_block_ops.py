@@ -317,6 +317,12 @@ def test_forward_and_scan_refuse_misaligned_vectors(lib):
     refused(lib, "B200GatedScanBackward", scan_fields(**valid, d_decay=P + 2), STATUS.INVALID_VALUE, "misaligned")
 
 
+@pytest.mark.parametrize("rows", [-1, 1])
+def test_gated_scan_step_refuses_overlapping_pools(lib, rows):
+    """A new pool some rows beside the old one: a request's state could be overwritten before it is read."""
+    refused(lib, "B200GatedScanStep", step_fields(state=P, new_state=P + rows * 64 * 4), STATUS.INVALID_VALUE, "overlap")
+
+
 def test_null_arguments(lib):
     for name in ("BlockNormForward", "BlockNormBackward", "GatedScanForward", "GatedScanBackward", "GatedScanStep"):
         refused(lib, "B200" + name, None, STATUS.INVALID_VALUE, "null arguments")
