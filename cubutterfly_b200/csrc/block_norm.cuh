@@ -959,16 +959,17 @@ __global__ void __launch_bounds__(S::kThreads, 1) block_norm_backward_kernel(Blo
 
 // The gradients of the per-channel vectors from the CTAs' sums, added in a
 // fixed order: 32 columns per CTA, four a thread, in 32 slices of the parts.
-// blockIdx.y: 0 Q -> d_pre, 1 Z -> d_scale, 2 P -> d_post, and the gate's
+// CTAs of `what`: 0 Q -> d_pre, 1 Z -> d_scale, 2 P -> d_post, and the gate's
 // gradient where one gate row serves all; 3 + g that of group g.
 template <typename T>
 __global__ void __launch_bounds__(256) block_norm_sums_kernel(BlockNormArgs p, int parts) {
     __shared__ float slice[32][36];
     pdl_begin();
-    const unsigned what = blockIdx.y;
+    const unsigned blocks = static_cast<unsigned>(p.dim + 31) / 32, what = blockIdx.x / blocks;
+    const int c0 = static_cast<int>(blockIdx.x % blocks) * 32;
     if ((what == 0 && !p.need_q) || (what == 1 && !p.need_z) || (what >= 2 && !p.need_p)) return;
     const int quad = threadIdx.x & 7, part = threadIdx.x >> 3;
-    const int col = blockIdx.x * 32 + 4 * quad;
+    const int col = c0 + 4 * quad;
     const bool grouped = p.gate_mode == kGateGroups;
     auto vector_at = [&](const void* v, bool is32, size_t at) {
         return is32 || sizeof(T) == 4 ? static_cast<const float*>(v)[at]
@@ -1014,7 +1015,7 @@ __global__ void __launch_bounds__(256) block_norm_sums_kernel(BlockNormArgs p, i
     *reinterpret_cast<float4*>(&slice[part][4 * quad]) =
         make_float4(sum.x + other.x, sum.y + other.y, sum.z + other.z, sum.w + other.w);
     __syncthreads();
-    const int lane = threadIdx.x, c = blockIdx.x * 32 + lane;
+    const int lane = threadIdx.x, c = c0 + lane;
     if (lane >= 32 || c >= p.dim) return;
     float total = 0.f;
 #pragma unroll

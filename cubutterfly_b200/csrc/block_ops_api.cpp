@@ -92,8 +92,6 @@ void check_norm_sizes(const cubutterflyB200BlockNorm_t* a) {
     supported(a->rows <= 0x7fffffffULL, "block norm: rows are limited to 2^31 - 1");
     require(a->gate_rows <= 1 || a->rows == 0 || (a->gate_rows <= a->rows && a->rows % a->gate_rows == 0),
             "block norm: gate_rows must be 0, 1 or a divisor of rows");
-    // a grid row of the kernel that adds the parameter gradients belongs to each group
-    supported(gate_groups(*a) <= 65532, "block norm: at most 65532 gate groups (give one gate per row instead)");
 }
 
 cubf::BlockNormArgs norm_args(const cubutterflyB200BlockNorm_t* a, bool backward, BlockType* block, bool* residual32) {
@@ -178,6 +176,8 @@ cubf::BlockNormArgs norm_args(const cubutterflyB200BlockNorm_t* a, bool backward
         n.r_pre = a->pre_rms;
         return n;
     }
+    // the kernel that adds the parameter gradients has a CTA for 32 channels of each group
+    supported((groups + 3) * ((a->dim + 31) / 32) <= 0x7fffffffULL, "block norm: too many gate groups");
     require(!a->d_normed || pre, "block norm: d_normed without PRE_NORM");
     require(a->d_x != nullptr && (a->d_y != nullptr) == (a->y != nullptr), "block norm: d_x and, with y, d_y are needed");
     require((a->d_gate != nullptr) == (a->gate != nullptr) &&

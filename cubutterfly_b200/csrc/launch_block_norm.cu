@@ -192,7 +192,8 @@ cudaError_t launch_block_norm_backward_unit<CUBF_BN_TYPE>(const BlockNormArgs& a
     cudaError_t e = dispatch(a, groups, stream);
     if (e != cudaSuccess || !(a.need_p || a.need_q || a.need_z)) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>((a.dim + 31) / 32), 3u + (a.gate_mode == kGateGroups ? static_cast<unsigned>(groups) : 0u));
+    cfg.gridDim = dim3(static_cast<unsigned>((a.dim + 31) / 32) *
+                       (3u + (a.gate_mode == kGateGroups ? static_cast<unsigned>(groups) : 0u)));
     cfg.blockDim = dim3(256);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];

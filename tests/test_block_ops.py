@@ -236,6 +236,8 @@ def test_block_norm_refusals(lib, change, status, text):
     (dict(workspace=0), STATUS.INVALID_VALUE, "workspace"),
     (dict(bytes=16), STATUS.INVALID_VALUE, "workspace"),
     (dict(rows=0), STATUS.NOT_SUPPORTED, "zero rows"),
+    (dict(dim=16384, x_row=16384, y_row=16384, dr_row=16384, rows=1 << 23, gate=P, d_gate=P, gate_rows=1 << 22,
+          gate_row=16384), STATUS.NOT_SUPPORTED, "gate groups"),
 ])
 def test_block_norm_backward_refusals(lib, change, status, text):
     valid = dict(post_rms=P, pre_rms=P, d_res=P, dr_row=64, d_x=P, d_y=P, workspace=P, bytes=1 << 20)

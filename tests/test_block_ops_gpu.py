@@ -585,6 +585,11 @@ def test_steps_follow_the_scan(cuda):
     ref.assert_close(state, final, ref.SCAN_LOSS)
 
 
+def test_block_norm_many_gate_groups(cuda):
+    """More gate groups than a grid has rows."""
+    check_norm(norm_case((66000, 2, 32), BF16, gate="group", seed=3), cuda, act="sigmoid")
+
+
 # (which leading axes of (3, 5, D) are broadcast)
 @pytest.mark.parametrize("axes", [(0,), (1,), (0, 1)])
 @pytest.mark.parametrize("dtype,dim,rotate", [(BF16, 64, True), (FP16, 33, False), (FP32, 258, False)])
