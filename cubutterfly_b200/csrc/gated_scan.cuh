@@ -488,10 +488,15 @@ CUBF_DEV Pair sigmoid(Pair v) {
     return each(add2(e, both(1.f)), [](float x) { return rcp(x); });
 }
 
-// c softplus(Lambda) log2(e): la in units of log2 is -rate sigmoid(r).
+// c softplus(Lambda) log2(e): la in units of log2 is -rate sigmoid(r).  Kept
+// finite, so that a shut gate, such as the tokens past the end, makes a = 1 for
+// an infinite rate too.
 CUBF_DEV float softplus(float v) { return v > 20.f ? v : log1pf(expf(v)); }
 CUBF_DEV Pair rates(Pair lambda, float exponent) {
-    return each(lambda, [&](float v) { return exponent * softplus(v) * kLog2e; });
+    return each(lambda, [&](float v) {
+        const float rate = exponent * softplus(v) * kLog2e;
+        return rate > 1e30f ? 1e30f : rate;  // not fminf: NaN stays
+    });
 }
 
 // a = 2^w and 1 - a^2 for w = log2(a) <= 0.  A recurrence forgets over
@@ -501,10 +506,11 @@ CUBF_DEV Pair rates(Pair lambda, float exponent) {
 // Chebyshev-node least-squares fit of (2^f - 1)/f of degree five, weighted to
 // equal ripples: 1.1e-8 relative), s = 2^n is put together from n's bits, and
 //   a = s + s t,   1 - a = (1 - s) - s t,   1 - a^2 = (1 - a)(1 + a);
-// for n = 0 the second is -t itself.  w below -126 is taken as -126: 1e-38.
+// for n = 0 the second is -t itself.  For w below -126.5 n's bits are those of
+// zero, and a is zero: what is forgotten leaves no gradient either, whatever la.
 CUBF_DEV void decay(Pair w, Pair& a, Pair& m2) {
     const Pair magic = both(12582912.f + 127.f);  // 1.5 2^23: n + 127 lands in the low bits
-    w = each(w, [](float x) { return max_nan(x, -126.f); });
+    w = each(w, [](float x) { return max_nan(x, -127.f); });
     const Pair r = add2(w, magic);
     const Pair f = sub2(w, sub2(r, magic));
     Pair t = fma2(f, both(0.00015403512f), both(0.0013390735f));

@@ -429,6 +429,29 @@ def test_gated_scan_slow_decay(cuda):
     check_scan(t, cuda)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_gated_scan_infinite_decay(cuda, dtype):
+    """A channel that forgets everything: h is sigmoid(i) x, and so is the final state, whatever the length."""
+    for length in (1, 5, 200):
+        t = scan_case(2, length, 40, dtype, states=2)
+        t["decay"][::2] = math.inf
+        x, r, i = (t[k].double() for k in "xri")
+        dev = [t[k].to(cuda).requires_grad_() for k in ("x", "r", "i", "decay", "initial")]
+        h, final = torch_ops.gated_scan(*dev[:4], initial_state=dev[4])
+        want = (torch.sigmoid(i) * x)[..., ::2]
+        ref.assert_close(h[..., ::2], want, ref.SCAN_LOSS)
+        ref.assert_close(final[:, ::2], want[:, -1], ref.SCAN_LOSS)
+        d = normal(6, *h.shape, dtype=dtype)
+        grads = torch.autograd.grad((h, final), dev, (d.to(cuda), torch.ones_like(final)))
+        g = d.double()
+        g[:, -1] += 1
+        s = torch.sigmoid(i)
+        ref.assert_close(grads[0][..., ::2], (g * s)[..., ::2], ref.SCAN_LOSS)
+        ref.assert_close(grads[2][..., ::2], (g * x * s * (1 - s))[..., ::2], ref.SCAN_LOSS)
+        for k in (1, 3, 4):
+            assert torch.isfinite(grads[k]).all() and not grads[k][..., ::2].any()
+
+
 @pytest.mark.parametrize("dim", [64, 62, 33])
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_gated_scan_strided_inputs(cuda, dim, dtype):
