@@ -699,6 +699,31 @@ def test_gated_scan_step_marks_its_writes(cuda):
         torch_ops.gated_scan_step(pool, token, token, token, decay)
 
 
+# ---- the gates' accuracy -------------------------------------------------------------------------
+def relative(got, want):
+    want = want.double().cpu()
+    return float(((got.detach().double().cpu() - want) / want).abs().max())
+
+
+@pytest.mark.parametrize("dtype,stream,gate", [(FP32, None, "full"), (FP32, None, "channel"), (BF16, FP32, "full"),
+                                               (BF16, FP32, "channel"), (FP16, FP32, "group")])
+@pytest.mark.parametrize("act", ["sigmoid", "silu"])
+def test_block_norm_gates_to_the_last_bits(cuda, dtype, stream, gate, act):
+    """Where the residual is fp32 so are the gate's bits.  exp: one unit of 2^-23; 1 + exp, the quotient and silu's
+    product: half a one each."""
+    dim, rows = 1024, 4
+    wide = dtype if gate == "full" else FP32
+    g = torch.linspace(-30, 30, rows * dim).reshape(rows, dim)
+    g = {"full": g, "channel": g[1], "group": g[:, None]}[gate].to(wide)
+    shape = (rows, 2, dim) if gate == "group" else (rows, dim)
+    x, y = torch.zeros(shape, dtype=stream or dtype), torch.ones(shape, dtype=dtype)
+    res, _ = torch_ops.block_norm(x.to(cuda), y.to(cuda), gate=g.to(cuda), gate_activation=act, post_norm=False,
+                                  pre_norm=False)
+    s = torch.sigmoid(g.double())
+    want = (s if act == "sigmoid" else g.double() * s).expand(shape)
+    assert relative(res, want) <= 3e-7 + (2.0 ** -24 if act == "silu" else 0)
+
+
 # ---- streams, graphs, repeatability ------------------------------------------------------------
 def all_operators(cuda, seed=0):
     n = norm_case((40, 512), BF16, FP32, gate="channel", scale="vector", seed=seed)
