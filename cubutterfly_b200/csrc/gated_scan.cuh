@@ -26,6 +26,7 @@
 #include "block_ops.hpp"
 #include "common.cuh"
 #include "f32x2.cuh"
+#include "gate.cuh"
 
 namespace cubf::scan {
 
@@ -33,6 +34,13 @@ using f32x2::add2;
 using f32x2::fma2;
 using f32x2::mul2;
 using f32x2::sub2;
+using gate::both;
+using gate::each;
+using gate::ex2;
+using gate::kLn2;
+using gate::kLog2e;
+using gate::max_nan;
+using gate::rcp;
 using Pair = f32x2::P;
 
 constexpr int kWarps = 8;                  // warps per CTA, consecutive in time
@@ -47,17 +55,11 @@ constexpr int kBackwardSteps = 8;
 static_assert(kGatedScanChunk == 2 * kBackwardSteps && kGatedScanChunk % kForwardSteps<__half, 16> == 0,
               "chunks begin where a forward warp and every other backward warp do");
 
-CUBF_DEV Pair both(float v) { return f32x2::pk(v, v); }
 CUBF_DEV Pair pair(float2 v) { return f32x2::pk(v.x, v.y); }
 CUBF_DEV float2 floats(Pair p) {
     float2 f;
     f32x2::up(p, f.x, f.y);
     return f;
-}
-template <typename F>
-CUBF_DEV Pair each(Pair p, F f) {
-    const float2 v = floats(p);
-    return f32x2::pk(f(v.x), f(v.y));
 }
 
 // ---- access to two channels of a token --------------------------------------------------------
@@ -459,33 +461,25 @@ using RowsOf = std::conditional_t<PIECE == 16, Rows<T, N, STEPS, STAGES, GROUPS>
                                   ShiftedRows<T, N, STEPS, STAGES, GROUPS, PIECE == 16 ? 4 : PIECE>>;
 
 // ---- the arithmetic of a token ----------------------------------------------------------------
-CUBF_DEV float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-CUBF_DEV float rcp(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 CUBF_DEV float rsq(float x) {
     float y;
     asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-CUBF_DEV float max_nan(float a, float b) {
-    float y;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-    return y;
+
+// Gates of 16 bits, rounded by 2^-9 or 2^-12 of themselves, take the sigmoid by
+// 2^(-v log2 e) with the product as rounded, off by |v| 2^-24; fp32 calls, which
+// are bound by memory, the exact one (4 x 4096 x 1024: 47.0 us forward and 88
+// backward for 45.6 and 87; 10007 x 1000 packed: 55 and 128 for 52 and 127).
+template <typename T>
+constexpr bool kExactGates = sizeof(T) == 4;
+CUBF_DEV Pair exp_minus(Pair v) {
+    return each(mul2(v, both(-kLog2e)), [](float x) { return ex2(x); });
 }
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-
+template <typename T>
 CUBF_DEV Pair sigmoid(Pair v) {
-    const Pair e = each(mul2(v, both(-kLog2e)), [](float x) { return ex2(x); });
-    return each(add2(e, both(1.f)), [](float x) { return rcp(x); });
+    if constexpr (kExactGates<T>) return gate::sigmoid(v);
+    return each(add2(exp_minus(v), both(1.f)), [](float x) { return rcp(x); });
 }
 
 // c softplus(Lambda) log2(e): la in units of log2 is -rate sigmoid(r).  Kept
@@ -530,14 +524,19 @@ CUBF_DEV Pair inverse_root(Pair m2) {
     return each(add2(m2, both(1e-37f)), [](float x) { return rsq(x); });
 }
 
-// sqrt(1 - a^2) sigmoid(i) x from 1 - a^2: with Q = 1 + e^-i, sqrt(m2)/Q =
-// m2/sqrt(m2 Q^2), one special-function instruction for root and quotient.
-// Q^2 may reach infinity, for i below -44, where the factor (below 1e-19) is
-// taken as zero.
+// sqrt(1 - a^2) sigmoid(i) x from 1 - a^2.  In 16-bit calls with Q = 1 + e^-i,
+// sqrt(m2)/Q = m2/sqrt(m2 Q^2), one special-function instruction for root and
+// quotient.  Q^2 may reach infinity there, for i below -44, where the factor
+// (below 1e-19) is taken as zero.
+template <typename T>
 CUBF_DEV Pair drive(Pair m2, Pair i, Pair x) {
-    const Pair q = add2(each(mul2(i, both(-kLog2e)), [](float v) { return ex2(v); }), both(1.f));
-    const Pair root = each(mul2(add2(m2, both(1e-37f)), mul2(q, q)), [](float v) { return rsq(v); });
-    return mul2(mul2(m2, root), x);
+    if constexpr (kExactGates<T>) {
+        return mul2(mul2(mul2(m2, inverse_root(m2)), sigmoid<T>(i)), x);
+    } else {
+        const Pair q = add2(exp_minus(i), both(1.f));
+        const Pair root = each(mul2(add2(m2, both(1e-37f)), mul2(q, q)), [](float v) { return rsq(v); });
+        return mul2(mul2(m2, root), x);
+    }
 }
 
 // ---- joining runs -----------------------------------------------------------------------------
@@ -729,8 +728,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArg
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             Pair m2;
-            decay(mul2(rate, sigmoid(rows.get(buf, 1, s))), a[s], m2);
-            u[s] = drive(m2, rows.get(buf, 2, s), rows.get(buf, 0, s));
+            decay(mul2(rate, sigmoid<T>(rows.get(buf, 1, s))), a[s], m2);
+            u[s] = drive<T>(m2, rows.get(buf, 2, s), rows.get(buf, 0, s));
         }
         Marks marks;
         if constexpr (PACKED) {
@@ -884,10 +883,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(Gat
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             Pair m2;
-            sr[s] = sigmoid(rows.get(stage, 1, s));
+            sr[s] = sigmoid<T>(rows.get(stage, 1, s));
             decay(mul2(rate, sr[s]), a[s], m2);
             im[s] = inverse_root(m2);
-            v[s] = mul2(mul2(m2, im[s]), sigmoid(rows.get(stage, 2, s)));
+            v[s] = mul2(mul2(m2, im[s]), sigmoid<T>(rows.get(stage, 2, s)));
         }
         auto x_of = [&](int s) { return rows.get(stage, 0, s); };
         auto dh_of = [&](int s) { return rows.get(stage, 3, s); };
@@ -1097,8 +1096,8 @@ __global__ void __launch_bounds__(128) gated_scan_step_kernel(GatedStepArgs p, i
         for (int k = 0; k < kStepRows; ++k) {
             if (b0 + k >= end) break;
             Pair a, m2;
-            decay(mul2(rate, sigmoid(r[k])), a, m2);
-            const Pair n = fma2(a, state[k], drive(m2, i[k], x[k]));
+            decay(mul2(rate, sigmoid<T>(r[k])), a, m2);
+            const Pair n = fma2(a, state[k], drive<T>(m2, i[k], x[k]));
             ln.template store<PAIRS>(static_cast<T*>(p.h) + (b0 + k) * p.dim, slot[k] < 0 ? both(0.f) : n);
             if (slot[k] >= 0) ln.template store<WIDE>(p.new_state + static_cast<size_t>(slot[k]) * p.dim, n);
         }

@@ -724,6 +724,44 @@ def test_block_norm_gates_to_the_last_bits(cuda, dtype, stream, gate, act):
     assert relative(res, want) <= 3e-7 + (2.0 ** -24 if act == "silu" else 0)
 
 
+@pytest.mark.parametrize("what", ["step", "scan"])
+def test_scan_gates_to_the_last_bits(cuda, what):
+    """fp32 gates.  exp and the reciprocal: a unit of 2^-23 each, the reciprocal root two thirds of one, 1 + exp and
+    the products half a one each."""
+    dim = 4096
+    gate = torch.linspace(-30, 30, dim)
+    open_, one = torch.full((dim,), math.inf), torch.ones(dim)
+    decay = torch.full((dim,), 3.0)
+
+    def run(x, r, i, lam):
+        args = [v.to(cuda)[None] for v in (x, r, i)]
+        if what == "step":
+            return torch_ops.gated_scan_step(torch.zeros(1, dim, device=cuda), *args, lam.to(cuda))[0]
+        return torch_ops.gated_scan(*(v[None] for v in args), lam.to(cuda))[0][0, 0]
+
+    # the input gate: a recurrence gate that forgets everything leaves x sigmoid(i)
+    s = torch.sigmoid(gate.double())
+    assert relative(run(one, open_, gate, torch.full((dim,), 60.0)), s) <= 6e-7
+    # the recurrence gate: an open input gate leaves sqrt(1 - a^2)
+    la = -8 * torch.nn.functional.softplus(decay.double()) * s
+    assert relative(run(one, gate, open_, decay), torch.sqrt(-torch.expm1(2 * la))) <= 6.5e-7
+    # far out, with an x to match
+    far = torch.linspace(-80, -45, dim)
+    x = torch.exp(-far)
+    want = x.double() * torch.sigmoid(far.double())
+    assert relative(run(x, open_, far, torch.full((dim,), 60.0)), want) <= 6e-7
+
+
+def test_gated_scan_gradient_gates_to_the_last_bits(cuda):
+    dim = 4096
+    gate = torch.linspace(-30, 30, dim)
+    x = torch.ones(1, 1, dim, device=cuda, requires_grad=True)
+    r = torch.full((1, 1, dim), math.inf, device=cuda)
+    h, _ = torch_ops.gated_scan(x, r, gate[None, None].to(cuda), torch.full((dim,), 60.0, device=cuda))
+    h.backward(torch.ones_like(h))
+    assert relative(x.grad[0, 0], torch.sigmoid(gate.double())) <= 6e-7
+
+
 # ---- streams, graphs, repeatability ------------------------------------------------------------
 def all_operators(cuda, seed=0):
     n = norm_case((40, 512), BF16, FP32, gate="channel", scale="vector", seed=seed)
