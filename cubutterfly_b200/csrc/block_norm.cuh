@@ -510,14 +510,11 @@ struct ForwardPlan {
     static constexpr int kFactorsAt = kWordsAt + S::kRows * 4 * S::kWarps;
     static constexpr int kFloats = kFactorsAt + (kShared ? 2 * kDim : 0);
     // 16-bit rows of eight values a thread fit 1024 threads an SM
-    template <typename T, typename R>
-    static constexpr int ctas() {
-        return S::EPT == 8 && S::VW == 8 && !ROTATE && S::kThreads < 1024 ? 1024 / S::kThreads : 1;
-    }
+    static constexpr int kCtas = S::EPT == 8 && S::VW == 8 && !ROTATE && S::kThreads < 1024 ? 1024 / S::kThreads : 1;
 };
 
 template <typename T, typename R, typename S, bool ROTATE>
-__global__ void __launch_bounds__(S::kThreads, ForwardPlan<S, ROTATE>::template ctas<T, R>())
+__global__ void __launch_bounds__(S::kThreads, ForwardPlan<S, ROTATE>::kCtas)
     block_norm_kernel(BlockNormArgs p) {
     using Plan = ForwardPlan<S, ROTATE>;
     extern __shared__ __align__(16) float shared[];

@@ -681,7 +681,6 @@ template <typename T, bool PACKED, int GROUPS, int PIECE>
 __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_kernel(GatedScanArgs p, int tiles) {
     using Tile = ForwardRows<T, GROUPS, PIECE>;
     constexpr int kSteps = Tile::STEPS, stride = Tile::TOKENS * kWarps;  // tokens a CTA takes a round
-    using Word = typename Raw<T>::Word;
     extern __shared__ __align__(16) unsigned char staged[];
     __shared__ Pair handed[kWarps][32];  // h before the warp's tokens
     pdl_begin();
@@ -827,7 +826,6 @@ template <typename T, bool PACKED, int GROUPS, int PIECE>
 __global__ void __launch_bounds__(kWarps * 32, 2) gated_scan_backward_kernel(GatedScanArgs p, int tiles) {
     using Tile = BackwardRows<T, GROUPS, PIECE>;
     constexpr int kSteps = Tile::STEPS, stride = Tile::TOKENS * kWarps;  // tokens a CTA takes a round
-    using Word = typename Raw<T>::Word;
     extern __shared__ __align__(16) unsigned char staged[];
     __shared__ Pair handed[kWarps][32];  // P from the tokens after the warp's
     __shared__ Pair middle[kWarps][32];  // h before the warp's tokens, where the warp before has it

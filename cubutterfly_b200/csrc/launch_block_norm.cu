@@ -29,10 +29,7 @@ using T = std::conditional_t<kType <= 1, __half, std::conditional_t<kType <= 3, 
 using R = std::conditional_t<kType == 1 || kType == 3 || kType == 4, float, T>;
 constexpr int kVec = 16 / static_cast<int>(sizeof(T));
 // values a thread of the backward: 16 fit the registers where every tensor is 16-bit
-#ifndef WIDE
-#define WIDE 16
-#endif
-constexpr int kWide = sizeof(R) == 2 ? WIDE : 8;
+constexpr int kWide = sizeof(R) == 2 ? 16 : 8;
 
 // Consecutive values that every row of every tensor is aligned for: whole
 // 16-byte vectors (kVec), pairs, or one.
