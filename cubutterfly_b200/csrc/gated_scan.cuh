@@ -498,7 +498,8 @@ CUBF_DEV Pair rates(Pair lambda, float exponent) {
 // without a bias and 1 - a must not cancel.  With w = n + f, n the nearest
 // integer and |f| <= 1/2, t = 2^f - 1 = f P(f) comes from a polynomial (the
 // Chebyshev-node least-squares fit of (2^f - 1)/f of degree five, weighted to
-// equal ripples: 1.1e-8 relative), s = 2^n is put together from n's bits, and
+// equal ripples: 2.1e-8 relative with its coefficients in fp32, 6.5e-9 of 2^f),
+// s = 2^n is put together from n's bits, and
 //   a = s + s t,   1 - a = (1 - s) - s t,   1 - a^2 = (1 - a)(1 + a);
 // for n = 0 the second is -t itself.  For w below -126.5 n's bits are those of
 // zero, and a is zero: what is forgotten leaves no gradient either, whatever la.

@@ -3,6 +3,7 @@ before anything is launched)."""
 import ctypes as ct
 import math
 import struct
+from pathlib import Path
 
 import pytest
 import torch
@@ -152,6 +153,23 @@ def test_overlapping_rows_are_copied():
     one = base.as_strided((1, 3, 16), (0, 20, 1))   # a stride of a single index means nothing
     rows, stride = block_ops._block_ops.rows(one, 16)
     assert stride == 20 and rows.data_ptr() == base.data_ptr()
+
+
+def test_polynomial_of_the_decay():
+    """(2^f - 1)/f over [-1/2, 1/2] with the coefficients that the kernels hold: the bound stated beside them."""
+    import re
+    import numpy as np
+
+    source = (Path(cb.__file__).parent / "csrc" / "gated_scan.cuh").read_text()
+    body = source[source.index("CUBF_DEV void decay("):]
+    body = body[:body.index("\n}\n")]
+    coefficients = [float(np.float32(c)) for c in re.findall(r"both\((0\.\d+)f\)", body)]
+    assert len(coefficients) == 6
+    f = np.linspace(-0.5, 0.5, 200001)
+    f = f[f != 0]
+    p = np.polyval(coefficients, f)
+    assert np.abs(p * f / np.expm1(f * math.log(2)) - 1).max() <= 2.15e-8
+    assert np.abs((1 + f * p) / 2 ** f - 1).max() <= 6.6e-9
 
 
 # Fields of a valid call; device pointers are never dereferenced by the checks.
