@@ -14,10 +14,12 @@
 // channel alone is formed once.
 //
 // Bound by memory: 16384 x 4096 bf16 in 88 us (6.1 TB/s of the device copy's
-// 6.5), with an fp32 residual and a gate per row 8192 x 4096 in 79 us (6.0).
-// Rotated rows move through shared memory six times, which takes 66 % of its
-// bandwidth beside 4.7 TB/s: 114 us.  Backward, where two row sums depend on
-// each other: 167 us (4.8 TB/s), rotated 209, with the gate 147 (5.0).
+// 6.5), with an fp32 residual and a gate per row 8192 x 4096 in 78 us (6.0).
+// Rotated rows move through shared memory six times, beside 4.7 TB/s: 114 us, its
+// wavefronts at 67 % and the SM's one CTA waiting on exchanges and loads in turn.
+// Backward, where two row sums depend on each other: 168 us (4.8 TB/s), rotated
+// 209, with the gate 148 (5.0).  Rows that are not whole vectors wait for their
+// loads, one value or pair each: 16000 x 1001 in 43 and 104 us, 1002 in 26 and 49.
 #pragma once
 
 #include "block_ops.hpp"

@@ -13,14 +13,16 @@
 // multiply-add a warp.  Every input is read once, every output written once,
 // and no CTA waits on another.
 //
-// What bounds it is issue slots before memory: at the rate of a device copy
-// (8 bytes a bf16 element forward) an element may take 45 of them, and the
-// gates take special functions, of which there are 16 a cycle and SM.  So the
-// two channels of a lane are computed as packed fp32 pairs, and a is formed on
-// the FMA pipe.  That makes 31 instructions and four special functions an
-// element forward, 58 and five backward: 16384 x 4096 bf16 in 114 us (4.7 TB/s),
-// 8 x 2048 x 2048 in 61 us and 101 us backward (4.4 and 4.7 TB/s); fp32, with
-// half the elements a byte, 4 x 4096 x 1024 in 47 and 87 us (5.7 and 5.4 TB/s).
+// What bounds it is latency: 8 to 16 warps fit an SM beside their registers and
+// the rows copied ahead, and none of its units is near its limit (8 x 1024 x 2048
+// bf16: 53 % of the issue slots, 49 % of the FMA pipe and 55 % of the special
+// functions forward, 61, 49 and 42 % backward).  A warp's chain is as long as its
+// instructions are many, so the two channels of a lane are computed as packed
+// fp32 pairs, and a is formed on the FMA pipe.  That makes 31 instructions and
+// four special functions an element forward, 58 and five backward: 16384 x 4096
+// bf16 in 114 us (4.7 TB/s) and 246 us backward, 8 x 2048 x 2048 in 60 and 102 us
+// (4.5 and 4.6 TB/s); fp32, with half the elements a byte, 4 x 4096 x 1024 in 47
+// and 88 us (5.7 and 5.3 TB/s).
 #pragma once
 
 #include "block_ops.hpp"
@@ -47,8 +49,10 @@ constexpr int kWarps = 8;                  // warps per CTA, consecutive in time
 constexpr int kWarpChannels = 64;          // channels times lane groups of a warp: two channels per lane
 // Tokens per thread and tile: as many as two CTAs' registers and shared
 // memory allow.  Forward rows that are not 16-byte aligned take more of the
-// latter (6 x 3602 x 974 bf16 with 8 and 16 tokens: 91, 107 us; 16384 x 4098, of
-// one CTA per SM either way: 233, 217).
+// latter.  With 8 and 16 tokens, bf16: 6 x 3602 x 974 92, 107 us; 16384 x 2050 120,
+// 150; 32730 x 425 223, 257; 8 x 2048 x 2050 96, 97.  Only long even rows on fewer
+// CTAs than SMs, of one or two lane groups, gain: 16384 x 4098 233, 217 and 4 x
+// 4096 x 2050 120, 117 (but 2048 x 4098 36, 37, and four groups, as 16384 x 2050).
 template <typename T, int PIECE>
 constexpr int kForwardSteps = sizeof(T) == 2 && PIECE == 16 ? 16 : 8;
 constexpr int kBackwardSteps = 8;
