@@ -21,6 +21,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
+#include <mutex>
 #include <string>
 #include <vector>
 
@@ -288,8 +289,13 @@ struct BlockNormBackward : Node {
 
     variable_list apply(variable_list&& grads) override {
         variable_list in;
-        for (const auto& v : inputs) in.push_back(v.unpack());
-        const Tensor r = rms.unpack();
+        Tensor r;
+        {
+            // another thread's backward over the same graph may release them meanwhile
+            const std::lock_guard<std::mutex> lock(mutex_);
+            for (const auto& v : inputs) in.push_back(v.unpack());
+            r = rms.unpack();
+        }
         // the outputs that exist, in order: the residual (with y), the normed rows
         const bool has_residual = in[1].defined();
         const Tensor d_residual = has_residual ? grads[0] : Tensor();
@@ -304,6 +310,7 @@ struct BlockNormBackward : Node {
         return once(std::move(out), "block_norm");
     }
     void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
         for (auto& v : inputs) v.reset_data();
         rms.reset_data();
     }
@@ -526,8 +533,13 @@ struct GatedScanBackward : Node {
         variable_list out(5);
         if (grads[0].defined() || grads[1].defined()) {
             variable_list in;
-            for (const auto& v : inputs) in.push_back(v.unpack());
-            const Tensor o = offsets.unpack(), states = chunk_states.unpack();
+            Tensor o, states;
+            {
+                const std::lock_guard<std::mutex> lock(mutex_);
+                for (const auto& v : inputs) in.push_back(v.unpack());
+                o = offsets.unpack();
+                states = chunk_states.unpack();
+            }
             at::NoGradGuard no_grad;
             out = call.backward(in, o, states, grads[0], grads[1]);
             for (size_t i = 0; i < out.size(); ++i)
@@ -536,6 +548,7 @@ struct GatedScanBackward : Node {
         return once(std::move(out), "gated_scan");
     }
     void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
         for (auto& v : inputs) v.reset_data();
         offsets.reset_data();
         chunk_states.reset_data();

@@ -786,6 +786,36 @@ def test_results_repeat_bit_for_bit(cuda):
         assert all(torch.equal(a, b) for a, b in zip(first, run()))
 
 
+def test_backward_from_several_threads(cuda):
+    """Threads that run one graph's backward: each gets the gradients, or, once one has freed the graph, an error."""
+    import threading
+
+    x = normal(1, 3, 50, 64).to(cuda).requires_grad_()
+    w, decay = torch.ones(64, device=cuda), decay_of(64).to(cuda)
+
+    def graph():
+        u = torch_ops.block_norm(x, x * 2, pre_weight=w)[1]
+        return torch_ops.gated_scan(u, u, u, decay)[0].sum()
+
+    want = torch.autograd.grad(graph(), x)[0]
+    for _ in range(5):
+        loss, got, errors = graph(), [], []
+
+        def run(keep):
+            try:
+                got.append(torch.autograd.grad(loss, x, retain_graph=keep)[0])
+            except RuntimeError as e:
+                errors.append(str(e))
+
+        threads = [threading.Thread(target=run, args=(k != 5,)) for k in range(8)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert len(got) + len(errors) == 8 and got and all(torch.equal(g, want) for g in got)
+        assert all("second time" in e for e in errors), errors
+
+
 def test_side_streams(cuda):
     run = all_operators(cuda, 3)
     want = run()
