@@ -270,6 +270,10 @@ B200GatedScanForward       p p
 B200GatedScanGetWorkspaceSize p Z
 B200GatedScanBackward      p p
 B200GatedScanStep          p p
+B200GatedDeltaForward      p p
+B200GatedDeltaGetWorkspaceSize p i Z
+B200GatedDeltaBackward     p p
+B200GatedDeltaStep         p p
 """
 
 

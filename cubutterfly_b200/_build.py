@@ -30,6 +30,8 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 BW_UNITS = [(0, 0), (0, 1), (0, 2), (1, 3), (1, 4), (2, 3), (2, 4)]
 # (block type, backward) units of the block norm
 BN_UNITS = [(t, b) for t in range(5) for b in (0, 1)]
+# (block type, padded key size) units of the gated delta rule
+GD_UNITS = [(t, k) for t in range(3) for k in (64, 128)]
 
 
 def _json_include() -> str:
@@ -67,6 +69,10 @@ def _units():
         src = CSRC / "launch_gated_scan.cu"
         obj = OBJ / f"gated_scan_{ty}.o"
         units.append((common + [f"-DCUBF_GS_TYPE={ty}", "-c", str(src), "-o", str(obj)], src, obj))
+    for ty, k in GD_UNITS:
+        src = CSRC / "launch_gated_delta.cu"
+        obj = OBJ / f"gated_delta_{ty}_{k}.o"
+        units.append((common + [f"-DCUBF_GD_TYPE={ty}", f"-DCUBF_GD_K={k}", "-c", str(src), "-o", str(obj)], src, obj))
     for op, ty in BW_UNITS:
         src = CSRC / "launch_bitwise.cu"
         obj = OBJ / f"bitwise_{op}_{ty}.o"

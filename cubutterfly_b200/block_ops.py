@@ -3,10 +3,13 @@
 ``block_norm``       the boundary between two blocks: norm, gate and residual add of a block's output, and the norm
                      (and Hadamard rotation) that makes the next block's input, in one pass over the rows;
 ``gated_scan``       the gated linear recurrence along sequences, dense or packed;
-``gated_scan_step``  one token of it for a batch of requests with states in a pool.
+``gated_scan_step``  one token of it for a batch of requests with states in a pool;
+``gated_delta``      the gated delta rule, a recurrence of matrix states, along sequences;
+``gated_delta_step`` one token of it.
 
 The calls run on the caller's current CUDA stream, allocate only through torch, never synchronise and can be captured
-in CUDA graphs.  ``block_norm`` and ``gated_scan`` are differentiable (once); arithmetic is fp32 whatever the tensors'
+in CUDA graphs.  ``block_norm``, ``gated_scan`` and ``gated_delta`` are
+differentiable (once); arithmetic is fp32 whatever the tensors'
 type, with one rounding per output.  They take plain tensors: one with a forward-mode tangent, without storage of its
 own (DTensor, FakeTensor, under ``torch.func`` transforms) or under a trace (``torch.jit.trace``, ``make_fx``) is
 refused.  ``cubutterfly_b200.torch_ops`` exports the operators beside the transforms.
@@ -28,10 +31,11 @@ except ImportError as e:
     raise ImportError(f"the torch extension of the block operators is not built or does not load ({e}); build it with "
                       "`python -m cubutterfly_b200._build`") from e
 
-__all__ = ["block_norm", "gated_scan", "gated_scan_step"]
+__all__ = ["block_norm", "gated_scan", "gated_scan_step", "gated_delta", "gated_delta_step"]
 
 _ENTRIES = ("BlockNormForward", "BlockNormBackward", "BlockNormGetWorkspaceSize", "GatedScanForward",
-            "GatedScanBackward", "GatedScanGetWorkspaceSize", "GatedScanStep")
+            "GatedScanBackward", "GatedScanGetWorkspaceSize", "GatedScanStep", "GatedDeltaForward", "GatedDeltaBackward",
+            "GatedDeltaGetWorkspaceSize", "GatedDeltaStep")
 
 
 def _bind():
@@ -40,7 +44,7 @@ def _bind():
     def fail(status):
         raise cb.Error(lib.describe(status), status)
 
-    _block_ops.bind(*(ct.cast(lib.fn["B200" + name], ct.c_void_p).value for name in _ENTRIES), fail)
+    _block_ops.bind([ct.cast(lib.fn["B200" + name], ct.c_void_p).value for name in _ENTRIES], fail)
 
 
 _bind()
@@ -96,3 +100,36 @@ def gated_scan_step(state, x, recurrence_gate, input_gate, decay, *, exponent=8.
     require grad.
     """
     return _block_ops.gated_scan_step(state, x, recurrence_gate, input_gate, decay, exponent, slots, new_state)
+
+
+def gated_delta(q, k, v, log_decay, beta, *, scale=None, initial_state=None, offsets=None):
+    """The gated delta rule along sequences: returns (o, final_state).
+
+    Per head, with a state S of (K, V) values::
+
+        u_t = beta_t (v_t - exp(log_decay_t) S_{t-1}^T k_t)
+        S_t = exp(log_decay_t) S_{t-1} + k_t u_t^T
+        o_t = scale S_t^T q_t
+
+    ``q`` and ``k`` are (B, S, Hk, K), ``v`` and ``o`` (B, S, H, V) of one type (bf16, fp16 or fp32), ``log_decay`` (at
+    most 0; -inf drops the state) and ``beta`` (B, S, H) of that type or fp32.  H is a multiple of Hk: head h reads the
+    keys and queries of head h // (H // Hk).  K and V are at most 128; ``scale`` is K ** -0.5 unless given.  Tensors may
+    be strided (slices of one projection).  The states are fp32 (B, H, K, V), ``initial_state`` zero unless given.  With
+    ``offsets`` (int32 on the device, n + 1 ascending values from 0 to T) the batch is packed: q is (T, Hk, K) or
+    (1, T, Hk, K) and so on, sequence j the tokens offsets[j] .. offsets[j + 1] - 1 (there may be none: its final state
+    is its initial one), the states are (n, H, K, V), and nothing of one sequence, NaN included, reaches another.  In
+    its own sequence a value that is not finite reaches later tokens and up to 63 before it.  Keys are meant to be of
+    length about one (``qk_norm``): with beta (k . k) above 2 the rule itself diverges.  Differentiable in q, k, v, both
+    gates and initial_state; the backward computes the states again, so that nothing but the inputs is kept.
+    """
+    return _block_ops.gated_delta(q, k, v, log_decay, beta, scale, initial_state, offsets)
+
+
+def gated_delta_step(state, q, k, v, log_decay, beta, *, scale=None, slots=None, new_state=None):
+    """One token of ``gated_delta`` for a batch of requests: returns o (B, H, V) and updates the states.
+
+    ``q`` and ``k`` are (B, Hk, K), ``v`` (B, H, V), the gates (B, H); ``state`` is a pool of fp32 states (P, H, K, V),
+    contiguous, updated in place unless ``new_state`` (another such pool, apart from it) takes the new ones.  ``slots``
+    and padding are as in ``gated_scan_step``.  Inference only: under grad mode no argument may require grad.
+    """
+    return _block_ops.gated_delta_step(state, q, k, v, log_decay, beta, scale, slots, new_state)

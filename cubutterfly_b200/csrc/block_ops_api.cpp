@@ -1,5 +1,5 @@
-// block_ops_api.cpp -- C entry points of the block norm and the gated linear
-// recurrence: argument checks, then launches.  Nothing here allocates device
+// block_ops_api.cpp -- C entry points of the block norm, the gated linear
+// recurrence and the gated delta rule: argument checks, then launches.  Nothing here allocates device
 // memory, copies or synchronises.
 #include <cmath>
 #include <stdexcept>
@@ -8,6 +8,7 @@
 #include <cubutterfly/cubutterfly_b200.h>
 
 #include "block_ops.hpp"
+#include "gated_delta.hpp"
 
 namespace cubf {
 void set_last_error(const std::string& message);
@@ -308,6 +309,78 @@ size_t scan_workspace(const cubutterflyB200GatedScan_t& a) {
     return (a.batch * a.dim * sizeof(float) + 15) / 16 * 16;
 }
 
+// ---- gated delta rule ---------------------------------------------------------------------------
+template <typename Args>
+void check_delta_heads(const Args* a) {
+    require(a->k_heads >= 1 && a->heads >= 1 && a->k_dim >= 1 && a->v_dim >= 1,
+            "gated delta: heads and their sizes must be at least 1");
+    supported(a->heads <= 65536 && a->k_heads <= a->heads, "gated delta: at most 65536 heads, no more key heads than heads");
+    require(a->heads % a->k_heads == 0, "gated delta: heads must be a multiple of k_heads");
+    supported(a->k_dim <= cubf::kDeltaMaxDim && a->v_dim <= cubf::kDeltaMaxDim,
+              "gated delta: k_dim and v_dim are limited to 128");
+    require(std::isfinite(a->scale), "gated delta: scale must be finite");
+}
+
+cubf::HeadTensor head_tensor(const cubutterflyB200HeadTensor_t& t, size_t size, const char* what) {
+    require(t.data != nullptr, what);
+    require(element_aligned(t.data, size), what);
+    return {t.data, t.batch, t.token, t.head};
+}
+
+template <typename Args, typename Call>
+void delta_gates(const Args* a, BlockType block, Call& s) {
+    s.log_decay32 = vector_is_32(a->log_decay.data, a->log_decay_type, block, "gated delta log_decay_type");
+    s.beta32 = vector_is_32(a->beta.data, a->beta_type, block, "gated delta beta_type");
+    const size_t es = element(block);
+    s.q = head_tensor(a->q, es, "gated delta: null or misaligned q");
+    s.k = head_tensor(a->k, es, "gated delta: null or misaligned k");
+    s.v = head_tensor(a->v, es, "gated delta: null or misaligned v");
+    s.log_decay = head_tensor(a->log_decay, 2, "gated delta: null or misaligned log_decay");
+    s.beta = head_tensor(a->beta, 2, "gated delta: null or misaligned beta");
+    s.k_heads = static_cast<int>(a->k_heads);
+    s.heads = static_cast<int>(a->heads);
+    s.k_dim = static_cast<int>(a->k_dim);
+    s.v_dim = static_cast<int>(a->v_dim);
+    s.scale = static_cast<float>(a->scale);
+}
+
+cubf::GatedDeltaArgs delta_args(const cubutterflyB200GatedDelta_t* a, BlockType* block) {
+    require(a != nullptr, "gated delta: null arguments");
+    require(a->struct_size == sizeof(*a), "gated delta: struct_size does not match this library's");
+    check_delta_heads(a);
+    supported(a->length <= cubf::kDeltaMaxLength, "gated delta: length is limited to 2^30 tokens");
+    supported(a->batch <= (1u << 24) && a->sequences <= (1u << 30), "gated delta: too many sequences");
+    require(!a->offsets || (a->batch == 1 && a->sequences >= 1),
+            "gated delta: a packed batch has batch = 1 and at least one sequence");
+    require(a->offsets || a->sequences == 0, "gated delta: sequences without offsets");
+    *block = type_of(a->data_type, "gated delta data_type");
+    cubf::GatedDeltaArgs s{};
+    s.batch = static_cast<int>(a->batch);
+    s.length = static_cast<int>(a->length);
+    s.sequences = static_cast<int>(a->sequences);
+    s.initial = a->initial_state;
+    s.offsets = a->offsets;
+    if (a->batch > 0 && a->length > 0) delta_gates(a, *block, s);
+    // a CTA for each chunk of 64 tokens of each head
+    const size_t chunks = a->offsets ? a->length / cubf::kDeltaChunk + a->sequences
+                                     : a->batch * ((a->length + cubf::kDeltaChunk - 1) / cubf::kDeltaChunk);
+    supported(chunks <= 0x7fffffffULL / a->heads, "gated delta: too many chunks and heads");
+    const size_t states = a->offsets ? a->sequences : a->batch;
+    supported(states <= 0x7fffffffULL / 16 / a->heads, "gated delta: too many sequences and heads");
+    for (const void* p : {static_cast<const void*>(a->initial_state), static_cast<const void*>(a->offsets),
+                          static_cast<const void*>(a->final_state), static_cast<const void*>(a->d_final_state),
+                          static_cast<const void*>(a->d_initial_state)})
+        require(element_aligned(p, 4), "gated delta: misaligned state or offsets");
+    return s;
+}
+
+void delta_workspace(const cubutterflyB200GatedDelta_t* a, BlockType block, bool backward, cubf::GatedDeltaArgs& s) {
+    require(a->workspace && a->workspace_bytes >= cubf::gated_delta_workspace(block, s, backward) &&
+                element_aligned(a->workspace, 256),
+            "gated delta: a 256-byte aligned workspace of the queried size is needed");
+    s.workspace = a->workspace;
+}
+
 }  // namespace
 
 extern "C" cubutterflyStatus_t cubutterflyB200BlockNormForward(const cubutterflyB200BlockNorm_t* args,
@@ -421,5 +494,92 @@ extern "C" cubutterflyStatus_t cubutterflyB200GatedScanStep(const cubutterflyB20
         s.dim = static_cast<int>(a->dim);
         s.exponent = static_cast<float>(a->exponent);
         check(cubf::launch_gated_scan_step(block, s, stream), "gated scan step launch");
+    });
+}
+
+extern "C" cubutterflyStatus_t cubutterflyB200GatedDeltaGetWorkspaceSize(const cubutterflyB200GatedDelta_t* args,
+                                                                        int backward, size_t* bytes) {
+    return guarded([&] {
+        BlockType block;
+        const cubf::GatedDeltaArgs a = delta_args(args, &block);
+        require(bytes != nullptr, "gated delta: null size");
+        *bytes = a.batch == 0 || a.length == 0 ? 0 : cubf::gated_delta_workspace(block, a, backward != 0);
+    });
+}
+
+extern "C" cubutterflyStatus_t cubutterflyB200GatedDeltaForward(const cubutterflyB200GatedDelta_t* args,
+                                                               cudaStream_t stream) {
+    return guarded([&] {
+        BlockType block;
+        cubf::GatedDeltaArgs a = delta_args(args, &block);
+        supported(a.length > 0 || a.batch == 0, "gated delta: of zero tokens the final states are the initial ones");
+        if (a.batch == 0) return;
+        require(args->o && element_aligned(args->o, element(block)), "gated delta: null or misaligned o");
+        require(args->final_state != nullptr, "gated delta: null final_state");
+        require(args->o != args->q.data && args->o != args->k.data && args->o != args->v.data,
+                "gated delta: o must not alias an input");
+        require(args->final_state != args->initial_state, "gated delta: final_state must not alias initial_state");
+        a.o = args->o;
+        a.last = args->final_state;
+        delta_workspace(args, block, false, a);
+        check(cubf::launch_gated_delta(block, a, false, stream), "gated delta launch");
+    });
+}
+
+extern "C" cubutterflyStatus_t cubutterflyB200GatedDeltaBackward(const cubutterflyB200GatedDelta_t* args,
+                                                                cudaStream_t stream) {
+    return guarded([&] {
+        BlockType block;
+        cubf::GatedDeltaArgs a = delta_args(args, &block);
+        supported(a.length > 0 && a.batch > 0, "gated delta: the backward of zero tokens is the caller's zeros");
+        const size_t es = element(block);
+        a.d_o = head_tensor(args->d_o, es, "gated delta: null or misaligned d_o");
+        require(args->d_q && args->d_k && args->d_v && args->d_log_decay && args->d_beta, "gated delta: null gradient");
+        for (const void* p : {static_cast<const void*>(args->d_q), static_cast<const void*>(args->d_k),
+                              static_cast<const void*>(args->d_v)})
+            require(element_aligned(p, es), "gated delta: misaligned gradient");
+        require(element_aligned(args->d_log_decay, a.log_decay32 ? 4 : es) && element_aligned(args->d_beta, a.beta32 ? 4 : es),
+                "gated delta: misaligned gradient of a gate");
+        a.d_last = args->d_final_state;
+        a.d_q = args->d_q;
+        a.d_k = args->d_k;
+        a.d_v = args->d_v;
+        a.d_log_decay = args->d_log_decay;
+        a.d_beta = args->d_beta;
+        a.d_initial = args->d_initial_state;
+        delta_workspace(args, block, true, a);
+        check(cubf::launch_gated_delta(block, a, true, stream), "gated delta backward launch");
+    });
+}
+
+extern "C" cubutterflyStatus_t cubutterflyB200GatedDeltaStep(const cubutterflyB200GatedDeltaStep_t* a,
+                                                            cudaStream_t stream) {
+    return guarded([&] {
+        require(a != nullptr, "gated delta step: null arguments");
+        require(a->struct_size == sizeof(*a), "gated delta step: struct_size does not match this library's");
+        check_delta_heads(a);
+        supported(a->batch <= 0x7fffffffULL && a->pool <= 0x7fffffffULL, "gated delta step: too many requests or slots");
+        const BlockType block = type_of(a->data_type, "gated delta step data_type");
+        if (a->batch == 0) return;
+        cubf::GatedDeltaStepArgs s{};
+        delta_gates(a, block, s);
+        require(a->o && element_aligned(a->o, element(block)), "gated delta step: null or misaligned o");
+        require((a->state && a->new_state) || a->pool == 0, "gated delta step: null state");
+        require(a->slots || a->pool >= a->batch, "gated delta step: without slots the pool needs a state per request");
+        for (const void* p : {static_cast<const void*>(a->state), static_cast<const void*>(a->new_state),
+                              static_cast<const void*>(a->slots)})
+            require(element_aligned(p, 4), "gated delta step: misaligned state or slots");
+        // in place, or apart, as in the gated scan's step
+        const uintptr_t from = reinterpret_cast<uintptr_t>(a->state), to = reinterpret_cast<uintptr_t>(a->new_state);
+        const size_t bytes = a->pool * a->heads * a->k_dim * a->v_dim * sizeof(float);
+        require(from == to || from + bytes <= to || to + bytes <= from,
+                "gated delta step: new_state must be state or not overlap it");
+        s.state = a->state;
+        s.new_state = a->new_state;
+        s.slots = a->slots;
+        s.o = a->o;
+        s.batch = a->batch;
+        s.pool = a->pool;
+        check(cubf::launch_gated_delta_step(block, s, stream), "gated delta step launch");
     });
 }

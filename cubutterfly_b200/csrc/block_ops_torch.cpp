@@ -46,18 +46,27 @@ struct Abi {
     decltype(&cubutterflyB200GatedScanBackward) scan_backward = nullptr;
     decltype(&cubutterflyB200GatedScanGetWorkspaceSize) scan_workspace = nullptr;
     decltype(&cubutterflyB200GatedScanStep) scan_step = nullptr;
+    decltype(&cubutterflyB200GatedDeltaForward) delta_forward = nullptr;
+    decltype(&cubutterflyB200GatedDeltaBackward) delta_backward = nullptr;
+    decltype(&cubutterflyB200GatedDeltaGetWorkspaceSize) delta_workspace = nullptr;
+    decltype(&cubutterflyB200GatedDeltaStep) delta_step = nullptr;
     PyObject* fail = nullptr;  // called with a status: raises the frontend's error
 } abi;
 
-void bind(uintptr_t norm_forward, uintptr_t norm_backward, uintptr_t norm_workspace, uintptr_t scan_forward,
-          uintptr_t scan_backward, uintptr_t scan_workspace, uintptr_t scan_step, py::object fail) {
-    abi.norm_forward = reinterpret_cast<decltype(abi.norm_forward)>(norm_forward);
-    abi.norm_backward = reinterpret_cast<decltype(abi.norm_backward)>(norm_backward);
-    abi.norm_workspace = reinterpret_cast<decltype(abi.norm_workspace)>(norm_workspace);
-    abi.scan_forward = reinterpret_cast<decltype(abi.scan_forward)>(scan_forward);
-    abi.scan_backward = reinterpret_cast<decltype(abi.scan_backward)>(scan_backward);
-    abi.scan_workspace = reinterpret_cast<decltype(abi.scan_workspace)>(scan_workspace);
-    abi.scan_step = reinterpret_cast<decltype(abi.scan_step)>(scan_step);
+void bind(const std::vector<uintptr_t>& entries, py::object fail) {
+    size_t at = 0;
+    auto take = [&](auto& entry) { entry = reinterpret_cast<std::decay_t<decltype(entry)>>(entries.at(at++)); };
+    take(abi.norm_forward);
+    take(abi.norm_backward);
+    take(abi.norm_workspace);
+    take(abi.scan_forward);
+    take(abi.scan_backward);
+    take(abi.scan_workspace);
+    take(abi.scan_step);
+    take(abi.delta_forward);
+    take(abi.delta_backward);
+    take(abi.delta_workspace);
+    take(abi.delta_step);
     Py_XDECREF(abi.fail);
     abi.fail = fail.release().ptr();
 }
@@ -691,6 +700,309 @@ Tensor gated_scan_step(py::handle hstate, py::handle hx, py::handle hr, py::hand
     return h;
 }
 
+// ---- gated delta rule ---------------------------------------------------------------------------
+// A (batch, tokens, heads, channels) tensor with adjacent channels, or a copy that has them; packed ones have one
+// batch row, tensors of gates no channels, and tensors of a step no tokens.
+struct Heads {
+    Tensor t;
+    cubutterflyB200HeadTensor_t h{};
+};
+Heads heads_of(const Tensor& t, bool batched, bool tokens, bool channels) {
+    Heads r{t, {}};
+    if (channels && t.size(-1) > 1 && t.stride(-1) != 1) r.t = t.contiguous();
+    int64_t d = 0;
+    r.h.batch = batched ? r.t.stride(d++) : 0;
+    r.h.token = tokens ? r.t.stride(d++) : 0;
+    r.h.head = r.t.stride(d);
+    r.h.data = r.t.data_ptr();
+    return r;
+}
+
+struct DeltaSizes {
+    int64_t k_heads = 0, heads = 0, k_dim = 0, v_dim = 0;
+};
+// Shapes, types and devices of q, k, v and the gates, whose leading dimensions are `lead`.
+DeltaSizes check_delta(const std::string& name, const Tensor& q, const Tensor& k, const Tensor& v,
+                       const Tensor& log_decay, const Tensor& beta) {
+    const size_t n = q.dim();
+    DeltaSizes s{q.size(-2), v.size(-2), q.size(-1), v.size(-1)};
+    REQUIRE(s.k_heads >= 1 && s.heads >= 1 && s.k_dim >= 1 && s.v_dim >= 1, name, " requires non-empty heads");
+    REQUIRE(s.k_dim <= 128 && s.v_dim <= 128, name, ": heads of keys and of values are limited to 128 channels, got ",
+            std::to_string(s.k_dim), " and ", std::to_string(s.v_dim));
+    REQUIRE(s.heads % s.k_heads == 0, name, ": the ", std::to_string(s.heads), " heads of v must be a multiple of the ",
+            std::to_string(s.k_heads), " of k");
+    std::vector<int64_t> shape(q.sizes().begin(), q.sizes().end());
+    check_like(k, (name + ": k").c_str(), q, shape);
+    shape[n - 2] = s.heads;
+    shape[n - 1] = s.v_dim;
+    check_like(v, (name + ": v").c_str(), q, shape);
+    shape.pop_back();
+    check_like(log_decay, (name + ": log_decay").c_str(), q, shape);
+    check_like(beta, (name + ": beta").c_str(), q, shape);
+    REQUIRE(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), name,
+            ": k and v must have q's dtype ", c10::toString(q.scalar_type()));
+    for (const Tensor* t : {&log_decay, &beta})
+        REQUIRE(t->scalar_type() == q.scalar_type() || t->scalar_type() == at::kFloat, name,
+                ": a gate must have q's dtype ", c10::toString(q.scalar_type()), " or float32, got ",
+                c10::toString(t->scalar_type()));
+    return s;
+}
+double scale_of(py::handle h, int64_t k_dim, const char* what) {
+    const double scale = h.is_none() ? 1.0 / std::sqrt(static_cast<double>(k_dim)) : h.cast<double>();
+    REQUIRE(std::isfinite(scale), what, ": scale must be finite");
+    return scale;
+}
+
+struct DeltaCall {
+    DeltaSizes sizes;
+    int64_t batch = 0, length = 0, sequences = 0;
+    bool batched = false;        // the tensors have a batch dimension
+    at::ScalarType type = at::kFloat;
+    double scale = 1.0;
+
+    bool empty() const { return batch == 0 || length == 0; }
+    Tensor workspace(const cubutterflyB200GatedDelta_t& a, bool backward, const Tensor& like) const {
+        size_t bytes = 0;
+        check(abi.delta_workspace(&a, backward, &bytes));
+        return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte).requires_grad(false));
+    }
+    // The inputs q, k, v, log_decay, beta, initial state; copies are kept in `alive`.
+    cubutterflyB200GatedDelta_t pack(const variable_list& in, const Tensor& offsets, std::vector<Tensor>& alive) const {
+        cubutterflyB200GatedDelta_t a{};
+        a.struct_size = sizeof(a);
+        a.batch = batch;
+        a.length = length;
+        a.k_heads = sizes.k_heads;
+        a.heads = sizes.heads;
+        a.k_dim = sizes.k_dim;
+        a.v_dim = sizes.v_dim;
+        a.sequences = sequences;
+        a.data_type = data_type(type);
+        a.log_decay_type = data_type(in[3].scalar_type());
+        a.beta_type = data_type(in[4].scalar_type());
+        a.scale = scale;
+        cubutterflyB200HeadTensor_t* const places[] = {&a.q, &a.k, &a.v, &a.log_decay, &a.beta};
+        for (int i = 0; i < 5; ++i) {
+            Heads h = heads_of(in[i], batched, true, i < 3);
+            *places[i] = h.h;
+            alive.push_back(std::move(h.t));
+        }
+        a.initial_state = floats(in[5]);
+        a.offsets = offsets.defined() ? offsets.data_ptr<int>() : nullptr;
+        return a;
+    }
+    void forward(const variable_list& in, const Tensor& offsets, Tensor* o, Tensor* final) const {
+        const auto options = in[2].options().requires_grad(false);
+        const auto wide = options.dtype(at::kFloat);
+        const int64_t states = offsets.defined() ? sequences : batch;
+        const std::vector<int64_t> shape{states, sizes.heads, sizes.k_dim, sizes.v_dim};
+        *o = at::empty(in[2].sizes(), options);
+        if (empty()) {  // no tokens: the states stay as they are
+            *final = at::zeros(shape, wide);
+            if (in[5].defined()) final->copy_(in[5]);
+            return;
+        }
+        const c10::cuda::CUDAGuard guard(in[0].device());
+        *final = at::empty(shape, wide);
+        std::vector<Tensor> alive;
+        cubutterflyB200GatedDelta_t a = pack(in, offsets, alive);
+        a.o = o->data_ptr();
+        a.final_state = floats(*final);
+        const Tensor space = workspace(a, false, in[0]);
+        a.workspace = space.data_ptr();
+        a.workspace_bytes = space.numel();
+        check(abi.delta_forward(&a, c10::cuda::getCurrentCUDAStream()));
+    }
+    variable_list backward(const variable_list& in, const Tensor& offsets, Tensor d_o, Tensor d_final) const {
+        variable_list grads(6);
+        for (int i = 0; i < 6; ++i)
+            if (in[i].defined()) grads[i] = at::empty(in[i].sizes(), in[i].options().requires_grad(false));
+        if (empty()) {
+            if (in[5].defined()) {
+                if (d_final.defined())
+                    grads[5].copy_(d_final);
+                else
+                    grads[5].zero_();
+            }
+            return grads;
+        }
+        const c10::cuda::CUDAGuard guard(in[0].device());
+        if (!d_o.defined()) d_o = at::zeros(in[2].sizes(), in[2].options().requires_grad(false));
+        if (d_final.defined()) d_final = d_final.contiguous();
+        std::vector<Tensor> alive;
+        cubutterflyB200GatedDelta_t a = pack(in, offsets, alive);
+        const Heads h = heads_of(d_o, batched, true, true);
+        a.d_o = h.h;
+        a.d_final_state = floats(d_final);
+        a.d_q = pointer(grads[0]);
+        a.d_k = pointer(grads[1]);
+        a.d_v = pointer(grads[2]);
+        a.d_log_decay = pointer(grads[3]);
+        a.d_beta = pointer(grads[4]);
+        a.d_initial_state = floats(grads[5]);
+        const Tensor space = workspace(a, true, in[0]);
+        a.workspace = space.data_ptr();
+        a.workspace_bytes = space.numel();
+        check(abi.delta_backward(&a, c10::cuda::getCurrentCUDAStream()));
+        return grads;
+    }
+};
+
+struct GatedDeltaBackward : Node {
+    DeltaCall call;
+    std::vector<SavedVariable> inputs;
+    SavedVariable offsets;
+
+    variable_list apply(variable_list&& grads) override {
+        variable_list out(6);
+        if (grads[0].defined() || grads[1].defined()) {
+            variable_list in;
+            Tensor o;
+            {
+                const std::lock_guard<std::mutex> lock(mutex_);
+                for (const auto& v : inputs) in.push_back(v.unpack());
+                o = offsets.unpack();
+            }
+            at::NoGradGuard no_grad;
+            out = call.backward(in, o, grads[0], grads[1]);
+            for (size_t i = 0; i < out.size(); ++i)
+                if (!task_should_compute_output(i)) out[i] = Tensor();
+        }
+        return once(std::move(out), "gated_delta");
+    }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        for (auto& v : inputs) v.reset_data();
+        offsets.reset_data();
+    }
+    std::string name() const override { return "GatedDeltaBackward"; }
+};
+
+py::object gated_delta(py::handle hq, py::handle hk, py::handle hv, py::handle hdecay, py::handle hbeta,
+                       py::handle hscale, py::handle hinitial, py::handle hoffsets) {
+    const Tensor q = tensor_of(hq, "gated_delta: q");
+    check_type(q, "gated_delta: q");
+    const Tensor k = tensor_of(hk, "gated_delta: k"), v = tensor_of(hv, "gated_delta: v");
+    const Tensor decay = tensor_of(hdecay, "gated_delta: log_decay"), beta = tensor_of(hbeta, "gated_delta: beta");
+    Tensor offsets = tensor_of(hoffsets, "gated_delta: offsets", true);
+    DeltaCall call;
+    if (offsets.defined()) {
+        REQUIRE(offsets.scalar_type() == at::kInt, "gated_delta: offsets does not support dtype ",
+                c10::toString(offsets.scalar_type()));
+        REQUIRE(offsets.device() == q.device(), "gated_delta: offsets is on ", offsets.device().str(), ", not on ",
+                q.device().str());
+        REQUIRE(offsets.dim() == 1 && offsets.numel() >= 2, "gated_delta: offsets must hold n + 1 values, n at least 1");
+        REQUIRE(q.dim() == 3 || (q.dim() == 4 && q.size(0) == 1),
+                "gated_delta: a packed batch is (T, heads, K) or (1, T, heads, K)");
+        offsets = offsets.contiguous();
+        call.sequences = offsets.numel() - 1;
+    } else {
+        REQUIRE(q.dim() == 4, "gated_delta: q must be (B, S, heads, K), or packed with offsets");
+    }
+    REQUIRE(v.dim() == q.dim(), "gated_delta: v must have as many dimensions as q");
+    call.sizes = check_delta("gated_delta", q, k, v, decay, beta);
+    call.batched = q.dim() == 4;
+    call.batch = call.batched ? q.size(0) : 1;
+    call.length = q.size(-3);
+    call.type = q.scalar_type();
+    call.scale = scale_of(hscale, call.sizes.k_dim, "gated_delta");
+    Tensor initial = tensor_of(hinitial, "gated_delta: initial_state", true);
+    if (initial.defined()) {
+        REQUIRE(initial.scalar_type() == at::kFloat, "gated_delta: initial_state does not support dtype ",
+                c10::toString(initial.scalar_type()));
+        check_like(initial, "gated_delta: initial_state", q,
+                   {offsets.defined() ? call.sequences : call.batch, call.sizes.heads, call.sizes.k_dim, call.sizes.v_dim});
+        initial = initial.contiguous();
+    }
+    const bool differentiable = any_requires_grad({&q, &k, &v, &decay, &beta, &initial});
+    variable_list in{q, k, v, decay, beta, initial};
+    std::shared_ptr<GatedDeltaBackward> node;
+    if (differentiable) {
+        node = std::shared_ptr<GatedDeltaBackward>(new GatedDeltaBackward(), torch::autograd::deleteNode);
+        node->call = call;
+        node->set_next_edges(torch::autograd::collect_next_edges(q, k, v, decay, beta, initial));
+        for (const auto& t : in) node->inputs.push_back(saved(t));
+        node->offsets = saved(offsets);
+    }
+    Tensor o, final;
+    {
+        at::NoGradGuard no_grad;
+        call.forward(in, offsets, &o, &final);
+    }
+    if (differentiable) {
+        torch::autograd::set_history(o, node);
+        torch::autograd::set_history(final, node);
+    }
+    return py::make_tuple(o, final);
+}
+
+Tensor gated_delta_step(py::handle hstate, py::handle hq, py::handle hk, py::handle hv, py::handle hdecay,
+                        py::handle hbeta, py::handle hscale, py::handle hslots, py::handle hnew) {
+    const Tensor q = tensor_of(hq, "gated_delta_step: q");
+    check_type(q, "gated_delta_step: q");
+    const Tensor k = tensor_of(hk, "gated_delta_step: k"), v = tensor_of(hv, "gated_delta_step: v");
+    const Tensor decay = tensor_of(hdecay, "gated_delta_step: log_decay"), beta = tensor_of(hbeta, "gated_delta_step: beta");
+    REQUIRE(q.dim() == 3 && v.dim() == 3, "gated_delta_step: q must be (B, heads, K) and v (B, heads, V)");
+    const DeltaSizes sizes = check_delta("gated_delta_step", q, k, v, decay, beta);
+    const int64_t batch = q.size(0);
+    const Tensor state = tensor_of(hstate, "gated_delta_step: state");
+    const Tensor next = hnew.is_none() ? state : tensor_of(hnew, "gated_delta_step: new_state");
+    for (const Tensor* t : {&state, &next}) {
+        REQUIRE(t->scalar_type() == at::kFloat, "gated_delta_step: a state pool does not support dtype ",
+                c10::toString(t->scalar_type()));
+        REQUIRE(t->device() == q.device(), "gated_delta_step: a state pool is on ", t->device().str(), ", not on ",
+                q.device().str());
+        REQUIRE(t->dim() == 4 && t->size(1) == sizes.heads && t->size(2) == sizes.k_dim && t->size(3) == sizes.v_dim &&
+                    t->is_contiguous(),
+                "gated_delta_step: a state pool must be contiguous and (slots, ", std::to_string(sizes.heads), ", ",
+                std::to_string(sizes.k_dim), ", ", std::to_string(sizes.v_dim), ")");
+    }
+    REQUIRE(next.sizes() == state.sizes(), "gated_delta_step: new_state must have the shape of state");
+    Tensor slots = tensor_of(hslots, "gated_delta_step: slots", true);
+    if (slots.defined()) {
+        REQUIRE(slots.scalar_type() == at::kInt, "gated_delta_step: slots does not support dtype ",
+                c10::toString(slots.scalar_type()));
+        check_like(slots, "gated_delta_step: slots", q, {batch});
+        slots = slots.contiguous();
+    } else {
+        REQUIRE(state.size(0) >= batch, "gated_delta_step: ", std::to_string(batch),
+                " requests without slots need a pool of as many states");
+    }
+    REQUIRE(!any_requires_grad({&state, &next, &q, &k, &v, &decay, &beta}),
+            "gated_delta_step is inference only: an input requires grad");
+    const double scale = scale_of(hscale, sizes.k_dim, "gated_delta_step");
+    at::NoGradGuard no_grad;
+    Tensor o = at::empty({batch, sizes.heads, sizes.v_dim}, v.options().requires_grad(false));
+    if (batch == 0) return o;
+    const c10::cuda::CUDAGuard guard(q.device());
+    const Heads places[] = {heads_of(q, true, false, true), heads_of(k, true, false, true), heads_of(v, true, false, true),
+                            heads_of(decay, true, false, false), heads_of(beta, true, false, false)};
+    cubutterflyB200GatedDeltaStep_t a{};
+    a.struct_size = sizeof(a);
+    a.batch = batch;
+    a.k_heads = sizes.k_heads;
+    a.heads = sizes.heads;
+    a.k_dim = sizes.k_dim;
+    a.v_dim = sizes.v_dim;
+    a.pool = state.size(0);
+    a.data_type = data_type(q.scalar_type());
+    a.log_decay_type = data_type(decay.scalar_type());
+    a.beta_type = data_type(beta.scalar_type());
+    a.scale = scale;
+    a.q = places[0].h;
+    a.k = places[1].h;
+    a.v = places[2].h;
+    a.log_decay = places[3].h;
+    a.beta = places[4].h;
+    a.state = floats(state);
+    a.new_state = floats(next);
+    a.slots = slots.defined() ? slots.data_ptr<int>() : nullptr;
+    a.o = o.data_ptr();
+    check(abi.delta_step(&a, c10::cuda::getCurrentCUDAStream()));
+    if (!next.is_inference()) next.unsafeGetTensorImpl()->bump_version();
+    return o;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_block_ops, m) {
@@ -698,6 +1010,8 @@ PYBIND11_MODULE(_block_ops, m) {
     m.def("block_norm", &block_norm);
     m.def("gated_scan", &gated_scan);
     m.def("gated_scan_step", &gated_scan_step);
+    m.def("gated_delta", &gated_delta);
+    m.def("gated_delta_step", &gated_delta_step);
     // parts of the checks, for tests without a GPU
     m.def("gate_rows", &gate_rows_of);
     m.def("rows", [](const Tensor& t, int64_t dim) {

@@ -1,8 +1,9 @@
-// launch_block_dispatch.cpp -- picks the unit of a type for the block norm and
-// the gated linear recurrence.
+// launch_block_dispatch.cpp -- picks the unit of a type for the block norm, the
+// gated linear recurrence and the gated delta rule.
 #include <algorithm>
 
 #include "block_ops.hpp"
+#include "gated_delta.hpp"
 
 namespace cubf {
 
@@ -88,6 +89,64 @@ cudaError_t launch_gated_scan_step(BlockType type, const GatedStepArgs& a, cudaS
         case BlockType::kF16: return launch_gated_scan_step_unit<0>(a, stream);
         case BlockType::kBF16: return launch_gated_scan_step_unit<1>(a, stream);
         default: return launch_gated_scan_step_unit<2>(a, stream);
+    }
+}
+
+template <int TYPE, int KP>
+cudaError_t launch_gated_delta_unit(const GatedDeltaArgs& a, bool backward, cudaStream_t stream);
+template <int TYPE, int KP>
+size_t gated_delta_workspace_unit(const GatedDeltaArgs& a, bool backward);
+template <int TYPE>
+cudaError_t launch_gated_delta_step_unit(const GatedDeltaStepArgs& a, cudaStream_t stream);
+
+#define CUBF_GD_UNIT(TYPE, KP)                                                               \
+    template <>                                                                              \
+    cudaError_t launch_gated_delta_unit<TYPE, KP>(const GatedDeltaArgs&, bool, cudaStream_t); \
+    template <>                                                                              \
+    size_t gated_delta_workspace_unit<TYPE, KP>(const GatedDeltaArgs&, bool);
+#define CUBF_GD_TYPE_UNITS(TYPE) \
+    CUBF_GD_UNIT(TYPE, 64)       \
+    CUBF_GD_UNIT(TYPE, 128)      \
+    template <>                  \
+    cudaError_t launch_gated_delta_step_unit<TYPE>(const GatedDeltaStepArgs&, cudaStream_t);
+CUBF_GD_TYPE_UNITS(0)
+CUBF_GD_TYPE_UNITS(1)
+CUBF_GD_TYPE_UNITS(2)
+#undef CUBF_GD_TYPE_UNITS
+#undef CUBF_GD_UNIT
+
+size_t gated_delta_workspace(BlockType type, const GatedDeltaArgs& a, bool backward) {
+    const bool small = a.k_dim <= 64;
+    switch (type) {
+        case BlockType::kF16:
+            return small ? gated_delta_workspace_unit<0, 64>(a, backward) : gated_delta_workspace_unit<0, 128>(a, backward);
+        case BlockType::kBF16:
+            return small ? gated_delta_workspace_unit<1, 64>(a, backward) : gated_delta_workspace_unit<1, 128>(a, backward);
+        default:
+            return small ? gated_delta_workspace_unit<2, 64>(a, backward) : gated_delta_workspace_unit<2, 128>(a, backward);
+    }
+}
+
+cudaError_t launch_gated_delta(BlockType type, const GatedDeltaArgs& a, bool backward, cudaStream_t stream) {
+    const bool small = a.k_dim <= 64;
+    switch (type) {
+        case BlockType::kF16:
+            return small ? launch_gated_delta_unit<0, 64>(a, backward, stream)
+                         : launch_gated_delta_unit<0, 128>(a, backward, stream);
+        case BlockType::kBF16:
+            return small ? launch_gated_delta_unit<1, 64>(a, backward, stream)
+                         : launch_gated_delta_unit<1, 128>(a, backward, stream);
+        default:
+            return small ? launch_gated_delta_unit<2, 64>(a, backward, stream)
+                         : launch_gated_delta_unit<2, 128>(a, backward, stream);
+    }
+}
+
+cudaError_t launch_gated_delta_step(BlockType type, const GatedDeltaStepArgs& a, cudaStream_t stream) {
+    switch (type) {
+        case BlockType::kF16: return launch_gated_delta_step_unit<0>(a, stream);
+        case BlockType::kBF16: return launch_gated_delta_step_unit<1>(a, stream);
+        default: return launch_gated_delta_step_unit<2>(a, stream);
     }
 }
 

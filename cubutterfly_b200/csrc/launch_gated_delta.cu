@@ -1,0 +1,167 @@
+// launch_gated_delta.cu -- launches of the gated delta rule; compiled once per
+// CUBF_GD_TYPE (0 fp16, 1 bf16, 2 fp32) and CUBF_GD_K (64 or 128: the padded
+// key size).
+#include <algorithm>
+
+#include "gated_delta.cuh"
+#include "launch_util.cuh"
+
+#ifndef CUBF_GD_TYPE
+#define CUBF_GD_TYPE 1
+#endif
+#ifndef CUBF_GD_K
+#define CUBF_GD_K 128
+#endif
+
+namespace cubf {
+
+template <int TYPE, int KP>
+cudaError_t launch_gated_delta_unit(const GatedDeltaArgs& a, bool backward, cudaStream_t stream);
+template <int TYPE, int KP>
+size_t gated_delta_workspace_unit(const GatedDeltaArgs& a, bool backward);
+template <int TYPE>
+cudaError_t launch_gated_delta_step_unit(const GatedDeltaStepArgs& a, cudaStream_t stream);
+
+namespace {
+
+using namespace delta;
+using T = std::conditional_t<CUBF_GD_TYPE == 0, __half, std::conditional_t<CUBF_GD_TYPE == 1, __nv_bfloat16, float>>;
+constexpr int KP = CUBF_GD_K;
+// Two chunks' tiles in shared memory where they fit beside one another, else one.
+constexpr int kStages = CUBF_GD_TYPE == 1 || (CUBF_GD_TYPE == 0 && KP == 64) ? 2 : 1;
+
+int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+bool rows_aligned(const HeadTensor& t, int width) {
+    const size_t bits = (t.batch | t.token | t.head | static_cast<size_t>(width)) * sizeof(T);
+    return ((reinterpret_cast<uintptr_t>(t.p) | bits) & 15u) == 0;
+}
+
+int sequences_of(const GatedDeltaArgs& a) { return a.offsets ? a.sequences : a.batch; }
+
+Places places_of(const GatedDeltaArgs& a, bool backward) {
+    Places w{};
+    w.slots = a.offsets ? a.length / C + a.sequences : a.batch * ceil_div(a.length, C);
+    w.v_pitch = ceil_div(a.v_dim, 16) * 16;
+    w.pack = !std::is_same_v<T, __nv_bfloat16> || !rows_aligned(a.q, a.k_dim) || !rows_aligned(a.k, a.k_dim);
+    const size_t chunks = static_cast<size_t>(w.slots) * a.heads;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    w.factors = take(chunks * kFactors * 4);
+    w.solve = take(chunks * kPieces * kSquare * 2);
+    w.attention = take(chunks * (backward ? kPieces : kOut<T>) * kSquare * 2);
+    w.packed = take(w.pack ? static_cast<size_t>(w.slots) * a.k_heads * 2 * kInput<T> * C * KP * 2 : 0);
+    if (backward) {
+        w.states = take(chunks * w.v_pitch * KP * 4);
+        w.d_states = take(chunks * w.v_pitch * KP * 4);
+        w.errors = take(chunks * C * w.v_pitch * 4);
+        w.d_writes = take(chunks * C * w.v_pitch * 4);
+        if (a.heads != a.k_heads) {
+            const size_t values = static_cast<size_t>(a.batch) * a.length * a.heads * a.k_dim;
+            w.d_q = take(values * 4);
+            w.d_k = take(values * 4);
+        }
+    }
+    w.total = at;
+    return w;
+}
+
+template <typename Kernel, typename... Args>
+cudaError_t launch(KernelSetup& setup, Kernel kernel, size_t grid, int threads, int smem, cudaStream_t stream,
+                   const Args&... args) {
+    if (grid > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
+    int cap = 0;
+    const cudaError_t e = setup_kernel(setup, kernel, threads, smem, &cap, true);
+    if (e != cudaSuccess) return e;
+    return launch_dependent(kernel, static_cast<unsigned>(grid), static_cast<unsigned>(threads), smem, stream, args...);
+}
+
+cudaError_t launch_chains(const GatedDeltaArgs& a, const Places& w, bool backward, cudaStream_t stream) {
+    const int tiles = ceil_div(a.v_dim, 16), chains = sequences_of(a) * a.heads;
+    ChainShape shape{};
+    // a warp runs by itself: as many a CTA as fill the SMs, up to 8, which share the tiles of a chunk
+    shape.warps = 8;
+    while (shape.warps > 2 && (shape.warps / 2 >= tiles || static_cast<long long>(chains) * ceil_div(tiles, shape.warps) < 148))
+        shape.warps /= 2;
+    shape.warps = std::min(shape.warps, tiles);
+    shape.slices = ceil_div(tiles, shape.warps);
+    shape.wide_v = rows_aligned(a.v, a.v_dim);
+    shape.wide_d = rows_aligned(a.d_o, a.v_dim);
+    const HeadTensor out{backward ? a.d_v : a.o, 0, 0, static_cast<size_t>(a.v_dim)};
+    shape.wide_o = rows_aligned(out, a.v_dim);
+    const size_t grid = static_cast<size_t>(chains) * shape.slices;
+    if (backward) {
+        // set up for the largest CTA, launched with what this one's warps need
+        static KernelSetup setup;
+        constexpr int most = kStages * ChainTiles<T, KP, kPieces>::bytes(8);
+        int cap = 0;
+        const auto kernel = &gated_delta_chains_kernel<T, KP, kStages>;
+        const cudaError_t e = setup_kernel(setup, kernel, 256, most, &cap, true);
+        if (e != cudaSuccess) return e;
+        if (2 * grid > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
+        return launch_dependent(kernel, static_cast<unsigned>(2 * grid), 32u * shape.warps,
+                                kStages * ChainTiles<T, KP, kPieces>::bytes(shape.warps), stream, a, w, shape);
+    }
+    static KernelSetup setup;
+    constexpr int most = kStages * ChainTiles<T, KP, kOut<T>>::bytes(8);
+    int cap = 0;
+    const auto kernel = &gated_delta_forward_kernel<T, KP, kStages>;
+    const cudaError_t e = setup_kernel(setup, kernel, 256, most, &cap, true);
+    if (e != cudaSuccess) return e;
+    if (grid > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
+    return launch_dependent(kernel, static_cast<unsigned>(grid), 32u * shape.warps,
+                            kStages * ChainTiles<T, KP, kOut<T>>::bytes(shape.warps), stream, a, w, shape);
+}
+
+}  // namespace
+
+template <>
+size_t gated_delta_workspace_unit<CUBF_GD_TYPE, CUBF_GD_K>(const GatedDeltaArgs& a, bool backward) {
+    return places_of(a, backward).total;
+}
+
+template <>
+cudaError_t launch_gated_delta_unit<CUBF_GD_TYPE, CUBF_GD_K>(const GatedDeltaArgs& a, bool backward, cudaStream_t stream) {
+    const Places w = places_of(a, backward);
+    const size_t chunks = static_cast<size_t>(w.slots) * a.heads;
+    {
+        static KernelSetup setup;
+        const cudaError_t e = launch(setup, &gated_delta_prepare_kernel<T, KP>, chunks, 128, sizeof(PrepareShared<T, KP>),
+                                     stream, a, w, backward ? kPieces : kOut<T>);
+        if (e != cudaSuccess) return e;
+    }
+    if (cudaError_t e = launch_chains(a, w, backward, stream); e != cudaSuccess || !backward) return e;
+    constexpr int smem = sizeof(GradientShared<T, KP>);
+    if (a.heads == a.k_heads) {
+        static KernelSetup setup;
+        return launch(setup, &gated_delta_gradients_kernel<T, KP, false>, chunks, 512, smem, stream, a, w);
+    }
+    {
+        static KernelSetup setup;
+        const cudaError_t e = launch(setup, &gated_delta_gradients_kernel<T, KP, true>, chunks, 512, smem, stream, a, w);
+        if (e != cudaSuccess) return e;
+    }
+    static KernelSetup setup;
+    const size_t values = static_cast<size_t>(a.batch) * a.length * a.k_heads * a.k_dim;
+    return launch(setup, &gated_delta_share_kernel<T>, std::min<size_t>((values + 255) / 256, 148 * 8), 256, 0, stream, a,
+                  w, values);
+}
+
+#if CUBF_GD_K == 128
+template <>
+cudaError_t launch_gated_delta_step_unit<CUBF_GD_TYPE>(const GatedDeltaStepArgs& a, cudaStream_t stream) {
+    const bool wide = a.v_dim % 4 == 0 &&
+                      ((reinterpret_cast<uintptr_t>(a.state) | reinterpret_cast<uintptr_t>(a.new_state)) & 15u) == 0;
+    const int slices = ceil_div(a.v_dim, wide ? 32 : 8);
+    const size_t grid = a.batch * a.heads * slices;
+    if (grid > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
+    const auto kernel = wide ? &gated_delta_step_kernel<T, 4> : &gated_delta_step_kernel<T, 1>;
+    return launch_dependent(kernel, static_cast<unsigned>(grid), 128u, 0, stream, a, slices);
+}
+#endif
+
+}  // namespace cubf

@@ -295,6 +295,72 @@ typedef struct cubutterflyB200GatedScanStep_s {
 CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200GatedScanStep(const cubutterflyB200GatedScanStep_t* args,
                                                                cudaStream_t stream);
 
+/* A (batch, token, head, channel) tensor: strides in elements, adjacent channels. */
+typedef struct cubutterflyB200HeadTensor_s {
+    const void* data;
+    size_t batch, token, head;
+} cubutterflyB200HeadTensor_t;
+
+/* The gated delta rule, per head along `length` tokens, from initial_state
+ * (fp32, (states, heads, k_dim, v_dim); null: zero) to final_state (the same,
+ * required):
+ *   u_t = beta_t (v_t - e^{log_decay_t} S_{t-1}^T k_t)
+ *   S_t = e^{log_decay_t} S_{t-1} + k_t u_t^T,   o_t = scale S_t^T q_t
+ * q and k have k_heads heads, v, the gates and o `heads`, a multiple of
+ * k_heads: head h reads key head h / (heads / k_heads).  log_decay and beta
+ * have data_type or FP32 (their channel is the head); log_decay is at most 0
+ * (-inf: the state is dropped).  Dense and packed batches as in GatedScan.
+ * k_dim and v_dim are at most 128, length at most 2^30.  Tokens of other
+ * sequences, NaN and infinities included, do not reach a sequence; in its own
+ * a value that is not finite reaches all later tokens and up to 63 earlier
+ * ones.  o is contiguous (batch, length, heads, v_dim).
+ * The gradients are contiguous, in the types of their tensors; d_initial_state
+ * null: not computed.  Both directions need a workspace (256-byte aligned). */
+typedef struct cubutterflyB200GatedDelta_s {
+    size_t struct_size;
+    size_t batch, length, k_heads, heads, k_dim, v_dim, sequences;
+    int data_type, log_decay_type, beta_type, reserved;
+    double scale;
+    cubutterflyB200HeadTensor_t q, k, v, log_decay, beta;
+    const float* initial_state;
+    const int* offsets;
+    void* o;
+    float* final_state;
+    /* backward only */
+    cubutterflyB200HeadTensor_t d_o;
+    const float* d_final_state;              /* null: zero */
+    void *d_q, *d_k, *d_v, *d_log_decay, *d_beta;
+    float* d_initial_state;
+    void* workspace;
+    size_t workspace_bytes;
+} cubutterflyB200GatedDelta_t;
+
+CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200GatedDeltaForward(const cubutterflyB200GatedDelta_t* args,
+                                                                   cudaStream_t stream);
+/* Reads the sizes, the types, offsets, q and k. */
+CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200GatedDeltaGetWorkspaceSize(const cubutterflyB200GatedDelta_t* args,
+                                                                            int backward, size_t* bytes);
+CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200GatedDeltaBackward(const cubutterflyB200GatedDelta_t* args,
+                                                                    cudaStream_t stream);
+
+/* One token of the gated delta rule for `batch` requests, whose states
+ * (heads, k_dim, v_dim) lie in pools of slots as in GatedScanStep.  The
+ * tensors' token strides are not read. */
+typedef struct cubutterflyB200GatedDeltaStep_s {
+    size_t struct_size;
+    size_t batch, k_heads, heads, k_dim, v_dim, pool;
+    int data_type, log_decay_type, beta_type, reserved;
+    double scale;
+    cubutterflyB200HeadTensor_t q, k, v, log_decay, beta;
+    const float* state;
+    float* new_state;
+    const int* slots;
+    void* o;
+} cubutterflyB200GatedDeltaStep_t;
+
+CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200GatedDeltaStep(const cubutterflyB200GatedDeltaStep_t* args,
+                                                                cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
