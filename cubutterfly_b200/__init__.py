@@ -274,6 +274,9 @@ B200GatedDeltaForward      p p
 B200GatedDeltaGetWorkspaceSize p i Z
 B200GatedDeltaBackward     p p
 B200GatedDeltaStep         p p
+B200QkNormForward          p p
+B200QkNormGetWorkspaceSize p Z
+B200QkNormBackward         p p
 """
 
 

@@ -52,7 +52,7 @@ def _units():
     for name in ("c_api.cpp", "descriptor.cpp", "planner.cpp", "rns_api.cpp", "launch_bitwise_dispatch.cpp",
                  "launch_ntt_dispatch.cpp", "launch_fft.cu", "noalloc.cu", "fourstep.cu", "bitrev.cu", "fwht_tc.cu",
                  "real_adapter.cu", "real_fft.cu", "calibrate.cu", "fourstep_peer.cu", "unaligned.cu", "structured.cu", "fwht_native.cu", "fft64.cu", "fft_chain.cu",
-                 "heongpu_adapter.cpp", "bluestein.cu", "block_ops_api.cpp", "launch_block_dispatch.cpp"):
+                 "heongpu_adapter.cpp", "bluestein.cu", "block_ops_api.cpp", "launch_block_dispatch.cpp", "launch_qk_norm.cu"):
         src = CSRC / name
         obj = OBJ / (src.stem + ".o")
         units.append((common + ["-c", str(src), "-o", str(obj)], src, obj))

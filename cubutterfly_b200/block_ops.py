@@ -5,11 +5,12 @@
 ``gated_scan``       the gated linear recurrence along sequences, dense or packed;
 ``gated_scan_step``  one token of it for a batch of requests with states in a pool;
 ``gated_delta``      the gated delta rule, a recurrence of matrix states, along sequences;
-``gated_delta_step`` one token of it.
+``gated_delta_step`` one token of it;
+``qk_norm``          norms of queries and keys head by head with the rotation by their positions, in one pass.
 
 The calls run on the caller's current CUDA stream, allocate only through torch, never synchronise and can be captured
-in CUDA graphs.  ``block_norm``, ``gated_scan`` and ``gated_delta`` are
-differentiable (once); arithmetic is fp32 whatever the tensors'
+in CUDA graphs.  ``block_norm``, ``gated_scan``, ``gated_delta``
+and ``qk_norm`` are differentiable (once); arithmetic is fp32 whatever the tensors'
 type, with one rounding per output.  They take plain tensors: one with a forward-mode tangent, without storage of its
 own (DTensor, FakeTensor, under ``torch.func`` transforms) or under a trace (``torch.jit.trace``, ``make_fx``) is
 refused.  ``cubutterfly_b200.torch_ops`` exports the operators beside the transforms.
@@ -31,11 +32,11 @@ except ImportError as e:
     raise ImportError(f"the torch extension of the block operators is not built or does not load ({e}); build it with "
                       "`python -m cubutterfly_b200._build`") from e
 
-__all__ = ["block_norm", "gated_scan", "gated_scan_step", "gated_delta", "gated_delta_step"]
+__all__ = ["block_norm", "gated_scan", "gated_scan_step", "gated_delta", "gated_delta_step", "qk_norm"]
 
 _ENTRIES = ("BlockNormForward", "BlockNormBackward", "BlockNormGetWorkspaceSize", "GatedScanForward",
             "GatedScanBackward", "GatedScanGetWorkspaceSize", "GatedScanStep", "GatedDeltaForward", "GatedDeltaBackward",
-            "GatedDeltaGetWorkspaceSize", "GatedDeltaStep")
+            "GatedDeltaGetWorkspaceSize", "GatedDeltaStep", "QkNormForward", "QkNormBackward", "QkNormGetWorkspaceSize")
 
 
 def _bind():
@@ -133,3 +134,24 @@ def gated_delta_step(state, q, k, v, log_decay, beta, *, scale=None, slots=None,
     and padding are as in ``gated_scan_step``.  Inference only: under grad mode no argument may require grad.
     """
     return _block_ops.gated_delta_step(state, q, k, v, log_decay, beta, scale, slots, new_state)
+
+
+def qk_norm(q, k, *, q_weight=None, k_weight=None, norm="rms", eps=1e-6, positions=None, frequencies=None, axes=None,
+            interleaved=False):
+    """Norms queries and keys head by head and rotates them by their positions: returns (q, k).
+
+    Per head x of D values, at most 256::
+
+        y = x / sqrt(mean(x^2) + eps) weight          (norm="rms")
+        y = x / sqrt(sum(x^2) + eps) weight           (norm="l2": heads of length one, as the delta rule takes them)
+        (a, b) -> (a cos - b sin, b cos + a sin)      for pair j of y, of angle position frequencies[j]
+
+    ``q`` is (..., Hq, D), ``k`` (..., Hk, D) with the same leading dimensions and type (bf16, fp16 or fp32); both may
+    be strided (slices of one projection).  The weights (D,) are fp32 or of q's type.  ``positions`` (int32 or int64,
+    on the device) has the shape of the leading dimensions, or of the last of them; ``frequencies`` is fp32 (R / 2,):
+    the first R values of a head are rotated, as pairs (j, j + R / 2), or (2 j, 2 j + 1) with ``interleaved``.  For
+    positions on several axes (time, height, width) they are (A, ...), and ``axes`` (int32, (R / 2,), values from 0 to
+    A - 1) says which one turns a pair.  Angles are taken modulo a turn in 64 bits: exact to 2e-7 for positions up to
+    2^31.  Differentiable in q, k and the weights.
+    """
+    return _block_ops.qk_norm(q, k, q_weight, k_weight, norm, eps, positions, frequencies, axes, interleaved)

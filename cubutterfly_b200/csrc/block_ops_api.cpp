@@ -1,5 +1,6 @@
 // block_ops_api.cpp -- C entry points of the block norm, the gated linear
-// recurrence and the gated delta rule: argument checks, then launches.  Nothing here allocates device
+// recurrence, the gated delta rule and the norm of queries and keys: argument
+// checks, then launches.  Nothing here allocates device
 // memory, copies or synchronises.
 #include <cmath>
 #include <stdexcept>
@@ -9,6 +10,7 @@
 
 #include "block_ops.hpp"
 #include "gated_delta.hpp"
+#include "qk_norm.hpp"
 
 namespace cubf {
 void set_last_error(const std::string& message);
@@ -381,6 +383,59 @@ void delta_workspace(const cubutterflyB200GatedDelta_t* a, BlockType block, bool
     s.workspace = a->workspace;
 }
 
+// ---- norm of queries and keys -------------------------------------------------------------------
+cubf::QkNormArgs qk_args(const cubutterflyB200QkNorm_t* a, BlockType* block) {
+    require(a != nullptr, "qk norm: null arguments");
+    require(a->struct_size == sizeof(*a), "qk norm: struct_size does not match this library's");
+    require(a->q_heads >= 1 && a->k_heads >= 1 && a->dim >= 1, "qk norm: heads and their size must be at least 1");
+    supported(a->dim <= cubf::kQkNormMaxDim, "qk norm: dim is limited to 256");
+    supported(a->q_heads <= 65536 && a->k_heads <= 65536, "qk norm: at most 65536 heads");
+    supported(a->batch == 0 || a->tokens <= (size_t{1} << 40) / a->batch, "qk norm: too many tokens");
+    require(std::isfinite(a->epsilon) && a->epsilon >= 0, "qk norm: epsilon must be finite and not negative");
+    require((a->flags & ~7) == 0, "qk norm: unknown flags");
+    require(a->rotary % 2 == 0 && a->rotary <= a->dim, "qk norm: rotary must be even and at most dim");
+    require((a->rotary > 0) == (a->positions != nullptr) && (a->rotary > 0) == (a->frequencies != nullptr),
+            "qk norm: rotary, positions and frequencies go together");
+    require(a->rotary == 0 || (a->positions_period >= 1 && a->axis_count >= 1 && a->axis_count <= 0x7fffffffULL),
+            "qk norm: positions need a period and an axis");
+    require(a->axes || a->axis_count <= 1, "qk norm: several axes of positions need axes");
+    *block = type_of(a->data_type, "qk norm data_type");
+    cubf::QkNormArgs n{};
+    n.batch = a->batch;
+    n.tokens = a->tokens;
+    n.q_heads = static_cast<int>(a->q_heads);
+    n.k_heads = static_cast<int>(a->k_heads);
+    n.dim = static_cast<int>(a->dim);
+    n.rotary = static_cast<int>(a->rotary);
+    n.axis_count = static_cast<int>(a->axis_count);
+    n.positions_axis = a->positions_axis;
+    n.positions_period = a->positions_period;
+    n.eps = static_cast<float>(a->epsilon);
+    n.length = a->flags & CUBUTTERFLY_B200_QK_LENGTH;
+    n.interleaved = a->flags & CUBUTTERFLY_B200_QK_INTERLEAVED;
+    n.positions64 = a->flags & CUBUTTERFLY_B200_QK_POSITIONS64;
+    require(element_aligned(a->positions, n.positions64 ? 8 : 4) && element_aligned(a->frequencies, 4) &&
+                element_aligned(a->axes, 4),
+            "qk norm: misaligned positions, frequencies or axes");
+    n.positions = a->positions;
+    n.frequencies = a->frequencies;
+    n.axes = a->axes;
+    n.q_weight = a->q_weight;
+    n.k_weight = a->k_weight;
+    n.q_weight32 = vector_is_32(a->q_weight, a->q_weight_type, *block, "qk norm q_weight_type");
+    n.k_weight32 = vector_is_32(a->k_weight, a->k_weight_type, *block, "qk norm k_weight_type");
+    n.parts = cubf::qk_norm_parts(n);
+    if (a->batch == 0 || a->tokens == 0) return n;
+    n.q = head_tensor(a->q, element(*block), "qk norm: null or misaligned q");
+    n.k = head_tensor(a->k, element(*block), "qk norm: null or misaligned k");
+    return n;
+}
+
+size_t qk_workspace(const cubf::QkNormArgs& a) {
+    if (!a.q_weight && !a.k_weight) return 0;
+    return (static_cast<size_t>(a.parts) * 2 * a.dim * sizeof(float) + 15) / 16 * 16;
+}
+
 }  // namespace
 
 extern "C" cubutterflyStatus_t cubutterflyB200BlockNormForward(const cubutterflyB200BlockNorm_t* args,
@@ -581,5 +636,58 @@ extern "C" cubutterflyStatus_t cubutterflyB200GatedDeltaStep(const cubutterflyB2
         s.batch = a->batch;
         s.pool = a->pool;
         check(cubf::launch_gated_delta_step(block, s, stream), "gated delta step launch");
+    });
+}
+
+extern "C" cubutterflyStatus_t cubutterflyB200QkNormForward(const cubutterflyB200QkNorm_t* args, cudaStream_t stream) {
+    return guarded([&] {
+        BlockType block;
+        cubf::QkNormArgs a = qk_args(args, &block);
+        if (a.batch == 0 || a.tokens == 0) return;
+        const size_t es = element(block);
+        require(args->q_out && args->k_out && element_aligned(args->q_out, es) && element_aligned(args->k_out, es),
+                "qk norm: null or misaligned output");
+        require(args->q_out != args->q.data && args->q_out != args->k.data && args->k_out != args->q.data &&
+                    args->k_out != args->k.data && args->q_out != args->k_out,
+                "qk norm: an output must not alias another tensor");
+        a.q_out = args->q_out;
+        a.k_out = args->k_out;
+        check(cubf::launch_qk_norm(block, a, false, stream), "qk norm launch");
+    });
+}
+
+extern "C" cubutterflyStatus_t cubutterflyB200QkNormGetWorkspaceSize(const cubutterflyB200QkNorm_t* args, size_t* bytes) {
+    return guarded([&] {
+        BlockType block;
+        const cubf::QkNormArgs a = qk_args(args, &block);
+        require(bytes != nullptr, "qk norm: null size");
+        *bytes = qk_workspace(a);
+    });
+}
+
+extern "C" cubutterflyStatus_t cubutterflyB200QkNormBackward(const cubutterflyB200QkNorm_t* args, cudaStream_t stream) {
+    return guarded([&] {
+        BlockType block;
+        cubf::QkNormArgs a = qk_args(args, &block);
+        supported(a.batch > 0 && a.tokens > 0, "qk norm: the backward of zero tokens is the caller's zeros");
+        const size_t es = element(block);
+        a.d_q_out = head_tensor(args->d_q_out, es, "qk norm: null or misaligned d_q_out");
+        a.d_k_out = head_tensor(args->d_k_out, es, "qk norm: null or misaligned d_k_out");
+        require(args->d_q && args->d_k && element_aligned(args->d_q, es) && element_aligned(args->d_k, es),
+                "qk norm: null or misaligned gradient");
+        require((args->d_q_weight != nullptr) == (args->q_weight != nullptr) &&
+                    (args->d_k_weight != nullptr) == (args->k_weight != nullptr),
+                "qk norm: every weight needs its gradient");
+        require(element_aligned(args->d_q_weight, a.q_weight32 ? 4 : es) && element_aligned(args->d_k_weight, a.k_weight32 ? 4 : es),
+                "qk norm: misaligned gradient of a weight");
+        require(qk_workspace(a) == 0 || (args->workspace && args->workspace_bytes >= qk_workspace(a) &&
+                                         element_aligned(args->workspace, 16)),
+                "qk norm: the backward needs a 16-byte aligned workspace of the queried size");
+        a.d_q = args->d_q;
+        a.d_k = args->d_k;
+        a.d_q_weight = args->d_q_weight;
+        a.d_k_weight = args->d_k_weight;
+        a.partials = static_cast<float*>(args->workspace);
+        check(cubf::launch_qk_norm(block, a, true, stream), "qk norm backward launch");
     });
 }

@@ -50,6 +50,9 @@ struct Abi {
     decltype(&cubutterflyB200GatedDeltaBackward) delta_backward = nullptr;
     decltype(&cubutterflyB200GatedDeltaGetWorkspaceSize) delta_workspace = nullptr;
     decltype(&cubutterflyB200GatedDeltaStep) delta_step = nullptr;
+    decltype(&cubutterflyB200QkNormForward) qk_forward = nullptr;
+    decltype(&cubutterflyB200QkNormBackward) qk_backward = nullptr;
+    decltype(&cubutterflyB200QkNormGetWorkspaceSize) qk_workspace = nullptr;
     PyObject* fail = nullptr;  // called with a status: raises the frontend's error
 } abi;
 
@@ -67,6 +70,9 @@ void bind(const std::vector<uintptr_t>& entries, py::object fail) {
     take(abi.delta_backward);
     take(abi.delta_workspace);
     take(abi.delta_step);
+    take(abi.qk_forward);
+    take(abi.qk_backward);
+    take(abi.qk_workspace);
     Py_XDECREF(abi.fail);
     abi.fail = fail.release().ptr();
 }
@@ -1003,6 +1009,236 @@ Tensor gated_delta_step(py::handle hstate, py::handle hq, py::handle hk, py::han
     return o;
 }
 
+// ---- norm of queries and keys -------------------------------------------------------------------
+struct QkCall {
+    int64_t batch = 1, tokens = 1, q_heads = 0, k_heads = 0, dim = 0, rotary = 0, axis_count = 0, period = 0;
+    at::ScalarType type = at::kFloat;
+    int flags = 0;
+    double eps = 0.0;
+
+    // (..., heads, dim) as (batch, tokens, heads, dim): `tokens` is the last leading dimension, the others merge into
+    // one, or the tensor is copied.
+    Heads place(const Tensor& t) const {
+        Heads r{t, {}};
+        const int64_t n = t.dim() - 2;           // leading dimensions
+        bool fits = t.size(-1) == 1 || t.stride(-1) == 1, seen = false;
+        int64_t stride = 0, expected = 0;
+        for (int64_t d = n - 2; d >= 0 && fits; --d) {
+            if (t.size(d) == 1) continue;
+            if (seen)
+                fits = t.stride(d) == expected;
+            else
+                stride = t.stride(d);
+            seen = true;
+            expected = t.stride(d) * t.size(d);
+        }
+        if (!fits) {
+            r.t = t.contiguous();
+            stride = n >= 2 ? r.t.stride(n - 2) : 0;
+        }
+        r.h.batch = stride;
+        r.h.token = n >= 1 ? r.t.stride(n - 1) : 0;
+        r.h.head = r.t.stride(n);
+        r.h.data = r.t.data_ptr();
+        return r;
+    }
+    // The inputs q, k, their weights; positions, frequencies and axes; copies are kept in `alive`.
+    cubutterflyB200QkNorm_t pack(const variable_list& in, const variable_list& turn, std::vector<Tensor>& alive) const {
+        cubutterflyB200QkNorm_t a{};
+        a.struct_size = sizeof(a);
+        a.batch = batch;
+        a.tokens = tokens;
+        a.q_heads = q_heads;
+        a.k_heads = k_heads;
+        a.dim = dim;
+        a.rotary = rotary;
+        a.axis_count = axis_count;
+        a.positions_axis = a.positions_period = period;
+        a.data_type = data_type(type);
+        auto weight = [&](const Tensor& t) { return t.defined() ? data_type(t.scalar_type()) : a.data_type; };
+        a.q_weight_type = weight(in[2]);
+        a.k_weight_type = weight(in[3]);
+        a.flags = flags;
+        a.epsilon = eps;
+        Heads q = place(in[0]), k = place(in[1]);
+        a.q = q.h;
+        a.k = k.h;
+        alive.push_back(std::move(q.t));
+        alive.push_back(std::move(k.t));
+        a.q_weight = pointer(in[2]);
+        a.k_weight = pointer(in[3]);
+        a.positions = pointer(turn[0]);
+        a.frequencies = floats(turn[1]);
+        a.axes = turn[2].defined() ? turn[2].data_ptr<int>() : nullptr;
+        return a;
+    }
+    bool empty() const { return batch == 0 || tokens == 0; }
+    void forward(const variable_list& in, const variable_list& turn, Tensor* q, Tensor* k) const {
+        *q = at::empty(in[0].sizes(), in[0].options().requires_grad(false));
+        *k = at::empty(in[1].sizes(), in[1].options().requires_grad(false));
+        if (empty()) return;
+        const c10::cuda::CUDAGuard guard(in[0].device());
+        std::vector<Tensor> alive;
+        cubutterflyB200QkNorm_t a = pack(in, turn, alive);
+        a.q_out = q->data_ptr();
+        a.k_out = k->data_ptr();
+        check(abi.qk_forward(&a, c10::cuda::getCurrentCUDAStream()));
+    }
+    variable_list backward(const variable_list& in, const variable_list& turn, Tensor d_q, Tensor d_k) const {
+        variable_list grads(4);
+        for (int i = 0; i < 4; ++i)
+            if (in[i].defined())
+                grads[i] = empty() ? at::zeros(in[i].sizes(), in[i].options().requires_grad(false))
+                                   : at::empty(in[i].sizes(), in[i].options().requires_grad(false));
+        if (empty()) return grads;
+        const c10::cuda::CUDAGuard guard(in[0].device());
+        if (!d_q.defined()) d_q = at::zeros(in[0].sizes(), in[0].options().requires_grad(false));
+        if (!d_k.defined()) d_k = at::zeros(in[1].sizes(), in[1].options().requires_grad(false));
+        std::vector<Tensor> alive;
+        cubutterflyB200QkNorm_t a = pack(in, turn, alive);
+        const Heads hq = place(d_q), hk = place(d_k);
+        a.d_q_out = hq.h;
+        a.d_k_out = hk.h;
+        a.d_q = pointer(grads[0]);
+        a.d_k = pointer(grads[1]);
+        a.d_q_weight = pointer(grads[2]);
+        a.d_k_weight = pointer(grads[3]);
+        size_t bytes = 0;
+        check(abi.qk_workspace(&a, &bytes));
+        Tensor space;
+        if (bytes) {
+            space = at::empty({static_cast<int64_t>(bytes)}, in[0].options().dtype(at::kByte).requires_grad(false));
+            a.workspace = space.data_ptr();
+            a.workspace_bytes = bytes;
+        }
+        check(abi.qk_backward(&a, c10::cuda::getCurrentCUDAStream()));
+        return grads;
+    }
+};
+
+struct QkNormBackward : Node {
+    QkCall call;
+    std::vector<SavedVariable> inputs, turn;
+
+    variable_list apply(variable_list&& grads) override {
+        variable_list out(4);
+        if (grads[0].defined() || grads[1].defined()) {
+            variable_list in, rotation;
+            {
+                const std::lock_guard<std::mutex> lock(mutex_);
+                for (const auto& v : inputs) in.push_back(v.unpack());
+                for (const auto& v : turn) rotation.push_back(v.unpack());
+            }
+            at::NoGradGuard no_grad;
+            out = call.backward(in, rotation, grads[0], grads[1]);
+            for (size_t i = 0; i < out.size(); ++i)
+                if (!task_should_compute_output(i)) out[i] = Tensor();
+        }
+        return once(std::move(out), "qk_norm");
+    }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        for (auto& v : inputs) v.reset_data();
+        for (auto& v : turn) v.reset_data();
+    }
+    std::string name() const override { return "QkNormBackward"; }
+};
+
+py::object qk_norm(py::handle hq, py::handle hk, py::handle hqw, py::handle hkw, const std::string& norm, double eps,
+                   py::handle hpositions, py::handle hfrequencies, py::handle haxes, bool interleaved) {
+    const Tensor q = tensor_of(hq, "qk_norm: q"), k = tensor_of(hk, "qk_norm: k");
+    check_type(q, "qk_norm: q");
+    REQUIRE(q.dim() >= 3, "qk_norm: q must be (..., heads, D) with at least one dimension of tokens");
+    REQUIRE(k.dim() == q.dim(), "qk_norm: k must have as many dimensions as q");
+    const int64_t lead = q.dim() - 2;
+    QkCall call;
+    call.q_heads = q.size(-2);
+    call.k_heads = k.size(-2);
+    call.dim = q.size(-1);
+    REQUIRE(call.q_heads >= 1 && call.k_heads >= 1 && call.dim >= 1, "qk_norm requires non-empty heads");
+    REQUIRE(call.dim <= 256, "qk_norm: heads are limited to 256 channels, got ", std::to_string(call.dim));
+    std::vector<int64_t> shape(q.sizes().begin(), q.sizes().end());
+    shape[lead] = call.k_heads;
+    check_like(k, "qk_norm: k", q, shape);
+    REQUIRE(k.scalar_type() == q.scalar_type(), "qk_norm: k must have q's dtype ", c10::toString(q.scalar_type()));
+    call.type = q.scalar_type();
+    call.tokens = q.size(lead - 1);
+    for (int64_t d = 0; d + 1 < lead; ++d) call.batch *= q.size(d);
+    REQUIRE(norm == "rms" || norm == "l2", "qk_norm: norm must be one of rms, l2");
+    REQUIRE(std::isfinite(eps) && eps >= 0, "qk_norm: eps must be finite and not negative");
+    call.eps = eps;
+    call.flags = (norm == "l2" ? CUBUTTERFLY_B200_QK_LENGTH : 0) | (interleaved ? CUBUTTERFLY_B200_QK_INTERLEAVED : 0);
+    Tensor qw = tensor_of(hqw, "qk_norm: q_weight", true), kw = tensor_of(hkw, "qk_norm: k_weight", true);
+    auto weight = [&](Tensor& w, const char* what) {
+        if (!w.defined()) return;
+        check_like(w, what, q, {call.dim});
+        REQUIRE(w.scalar_type() == call.type || w.scalar_type() == at::kFloat, what, " does not support dtype ",
+                c10::toString(w.scalar_type()));
+        w = w.contiguous();
+    };
+    weight(qw, "qk_norm: q_weight");
+    weight(kw, "qk_norm: k_weight");
+    Tensor positions = tensor_of(hpositions, "qk_norm: positions", true),
+           frequencies = tensor_of(hfrequencies, "qk_norm: frequencies", true), axes = tensor_of(haxes, "qk_norm: axes", true);
+    REQUIRE(positions.defined() == frequencies.defined(), "qk_norm: positions and frequencies go together");
+    REQUIRE(positions.defined() || !axes.defined(), "qk_norm: axes need positions");
+    if (positions.defined()) {
+        for (const Tensor* t : {&positions, &frequencies, &axes})
+            REQUIRE(!t->defined() || t->device() == q.device(),
+                    "qk_norm: positions, frequencies and axes must be on q's device ", q.device().str());
+        REQUIRE(frequencies.dim() == 1 && frequencies.numel() >= 1 && 2 * frequencies.numel() <= call.dim,
+                "qk_norm: frequencies must hold one value for each rotated pair of a head's ", std::to_string(call.dim),
+                " channels, got ", text(frequencies.sizes()));
+        REQUIRE(frequencies.scalar_type() == at::kFloat, "qk_norm: frequencies does not support dtype ",
+                c10::toString(frequencies.scalar_type()));
+        REQUIRE(!any_requires_grad({&frequencies}), "qk_norm has no gradient in its frequencies");
+        const bool wide = positions.scalar_type() == at::kLong;
+        REQUIRE(wide || positions.scalar_type() == at::kInt, "qk_norm: positions does not support dtype ",
+                c10::toString(positions.scalar_type()));
+        if (wide) call.flags |= CUBUTTERFLY_B200_QK_POSITIONS64;
+        auto at = positions.sizes();
+        call.axis_count = 1;
+        if (axes.defined()) {
+            REQUIRE(axes.scalar_type() == at::kInt, "qk_norm: axes does not support dtype ", c10::toString(axes.scalar_type()));
+            REQUIRE(axes.sizes() == frequencies.sizes(), "qk_norm: axes must have shape ", text(frequencies.sizes()), ", got ",
+                    text(axes.sizes()));
+            REQUIRE(positions.dim() >= 2 && positions.size(0) >= 1, "qk_norm: with axes, positions must be (axes, tokens ...)");
+            call.axis_count = positions.size(0);
+            at = at.slice(1);
+            axes = axes.contiguous();
+        }
+        const auto all = q.sizes().slice(0, lead);
+        REQUIRE(!at.empty() && at.size() <= all.size() && at == all.slice(all.size() - at.size()),
+                "qk_norm: positions of shape ", text(positions.sizes()), " must match the leading dimensions ", text(all),
+                " of q, or the last of them");
+        call.rotary = 2 * frequencies.numel();
+        call.period = 1;
+        for (const int64_t n : at) call.period *= n;
+        positions = positions.contiguous();
+        frequencies = frequencies.contiguous();
+    }
+    const bool differentiable = any_requires_grad({&q, &k, &qw, &kw});
+    variable_list in{q, k, qw, kw}, turn{positions, frequencies, axes};
+    std::shared_ptr<QkNormBackward> node;
+    if (differentiable) {
+        node = std::shared_ptr<QkNormBackward>(new QkNormBackward(), torch::autograd::deleteNode);
+        node->call = call;
+        node->set_next_edges(torch::autograd::collect_next_edges(q, k, qw, kw));
+        for (const auto& t : in) node->inputs.push_back(saved(t));
+        for (const auto& t : turn) node->turn.push_back(saved(t));
+    }
+    Tensor oq, ok;
+    {
+        at::NoGradGuard no_grad;
+        call.forward(in, turn, &oq, &ok);
+    }
+    if (differentiable) {
+        torch::autograd::set_history(oq, node);
+        torch::autograd::set_history(ok, node);
+    }
+    return py::make_tuple(oq, ok);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_block_ops, m) {
@@ -1010,6 +1246,7 @@ PYBIND11_MODULE(_block_ops, m) {
     m.def("block_norm", &block_norm);
     m.def("gated_scan", &gated_scan);
     m.def("gated_scan_step", &gated_scan_step);
+    m.def("qk_norm", &qk_norm);
     m.def("gated_delta", &gated_delta);
     m.def("gated_delta_step", &gated_delta_step);
     // parts of the checks, for tests without a GPU

@@ -24,8 +24,7 @@
 // shared memory but the tiles that all warps read.  The backward runs the
 // forward chain again (keeping S and R of every chunk) beside the reversed
 // chain, in one launch, then `gradients` (a CTA per chunk and head).
-// All products are split ones (mma_split.cuh): level 3, fp32, wherever a state
-// or an fp32 output depends on them, level 2 where only 16-bit outputs do.
+// All products are split ones (mma_split.cuh), accumulated in fp32.
 #pragma once
 
 #include <algorithm>
@@ -38,7 +37,6 @@ namespace cubf::delta {
 using namespace split;
 
 constexpr int C = kDeltaChunk;
-constexpr int kPieces = 3;               // of L and of the states' operands
 constexpr int kSquare = C * C;           // values of L or P
 constexpr int kPitchC = C + 8;           // of 64-wide tiles
 // Per chunk and head: e^G, e^{G_64 - G}, beta, and G as a sum of two floats
@@ -47,8 +45,14 @@ constexpr float kLeast = -128.f;         // e^-128 is zero in fp32: a log decay 
 
 template <typename T>
 constexpr int kInput = std::is_same_v<T, float> ? 3 : std::is_same_v<T, __half> ? 2 : 1;  // exact pieces of an input
+// Level of the products and pieces of their fp32 operands.  With 16-bit tensors 16 bits of an operand, each product's
+// error 2^-16 at most and 3e-6 in the mean, stay far below one rounding of an output and below 1e-5 of the fp32 states,
+// which are themselves held and added up in fp32; level 3 costs half as much again.
 template <typename T>
-constexpr int kOut = std::is_same_v<T, float> ? 3 : 2;  // level of products that only outputs of type T depend on
+constexpr int kLevel = std::is_same_v<T, float> ? 3 : 2;
+// ... with q, k or dO as the other operand: fp16 ones bring both pieces to both of the state's.
+template <typename T>
+constexpr int kInputLevel = std::is_same_v<T, __nv_bfloat16> ? 2 : 3;
 
 template <typename T>
 CUBF_DEV float widen(T x) {
@@ -207,7 +211,7 @@ CUBF_DEV void pack_rows(const GatedDeltaArgs& a, const HeadTensor& t, const Span
 }
 
 template <typename T, int KP>
-__global__ void __launch_bounds__(128) gated_delta_prepare_kernel(GatedDeltaArgs a, Places w, int attention_pieces) {
+__global__ void __launch_bounds__(128) gated_delta_prepare_kernel(GatedDeltaArgs a, Places w) {
     constexpr int NI = kInput<T>;
     using Shared = PrepareShared<T, KP>;
     extern __shared__ __align__(16) unsigned char raw[];
@@ -287,7 +291,8 @@ __global__ void __launch_bounds__(128) gated_delta_prepare_kernel(GatedDeltaArgs
             }
         }
     }
-    __nv_bfloat16* attention = reinterpret_cast<__nv_bfloat16*>(work + w.attention) + place * attention_pieces * kSquare;
+    constexpr int LEVEL = kLevel<T>;
+    __nv_bfloat16* attention = reinterpret_cast<__nv_bfloat16*>(work + w.attention) + place * LEVEL * kSquare;
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
 #pragma unroll
@@ -302,18 +307,17 @@ __global__ void __launch_bounds__(128) gated_delta_prepare_kernel(GatedDeltaArgs
                 sm.unit[i][j + e] = m[e];
                 sm.m[i][j + e] = m[e] * sm.beta[j + e];
             }
-            uint32_t f[3];
-            pieces<3>(p[0], p[1], f);
+            uint32_t f[LEVEL];
+            pieces<LEVEL>(p[0], p[1], f);
 #pragma unroll
-            for (int n = 0; n < 3; ++n)
-                if (n < attention_pieces) *reinterpret_cast<uint32_t*>(attention + n * kSquare + i * C + j) = f[n];
+            for (int n = 0; n < LEVEL; ++n) *reinterpret_cast<uint32_t*>(attention + n * kSquare + i * C + j) = f[n];
         }
     }
     __syncthreads();
     // column `tid` of L by forward substitution: l_i = M_i - sum over j < i of (M beta)_ij l_j
     if (tid >= C) return;
     float l[C];
-    __nv_bfloat16* solve = reinterpret_cast<__nv_bfloat16*>(work + w.solve) + place * kPieces * kSquare + tid;
+    __nv_bfloat16* solve = reinterpret_cast<__nv_bfloat16*>(work + w.solve) + place * LEVEL * kSquare + tid;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
         float acc[4] = {sm.unit[i][tid], 0.f, 0.f, 0.f};
@@ -328,7 +332,7 @@ __global__ void __launch_bounds__(128) gated_delta_prepare_kernel(GatedDeltaArgs
         l[i] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
         float rest = l[i];
 #pragma unroll
-        for (int n = 0; n < kPieces; ++n) {
+        for (int n = 0; n < LEVEL; ++n) {
             const __nv_bfloat16 piece = __float2bfloat16_rn(rest);
             rest -= __bfloat162float(piece);
             solve[n * kSquare + i * C] = piece;
@@ -338,33 +342,33 @@ __global__ void __launch_bounds__(128) gated_delta_prepare_kernel(GatedDeltaArgs
 
 // ---- chain --------------------------------------------------------------------------------------
 // Shared memory of one chunk's tiles, for W warps (16 columns of v each).
-template <typename T, int KP, int AP>
+template <typename T, int KP>
 struct ChainTiles {
     static constexpr int NI = kInput<T>;
     static constexpr int kQ = 0;
     static constexpr int kK = kQ + NI * C * (KP + 8) * 2;
     static constexpr int kSolve = kK + NI * C * (KP + 8) * 2;
-    static constexpr int kAttention = kSolve + kPieces * C * kPitchC * 2;
-    static constexpr int kFactor = kAttention + AP * C * kPitchC * 2;
+    static constexpr int kAttention = kSolve + kLevel<T> * C * kPitchC * 2;
+    static constexpr int kFactor = kAttention + kLevel<T> * C * kPitchC * 2;
     static constexpr int kRows = kFactor + kFactors * 4;
     static constexpr int bytes(int warps) {
         return kRows + C * (16 * warps + kSpare<T>) * static_cast<int>(sizeof(T));
     }
 };
 
-template <typename T, int KP, int AP>
+template <typename T, int KP>
 CUBF_DEV void load_chunk(const GatedDeltaArgs& a, const Places& w, const HeadTensor& rows, bool wide_rows, const Span& s,
                          int slot, int head, int from, int width, unsigned char* stage, int tid, int threads) {
-    using Tiles = ChainTiles<T, KP, AP>;
+    using Tiles = ChainTiles<T, KP>;
     const int k_head = head / (a.heads / a.k_heads);
     const size_t place = static_cast<size_t>(slot) * a.heads + head;
     char* const work = static_cast<char*>(a.workspace);
     const uint32_t base = smem_addr(stage);
     load_source<kInput<T>, KP>(source_of<T, KP>(a, w, a.q, 0, slot, k_head, s), base + Tiles::kQ, tid, threads);
     load_source<kInput<T>, KP>(source_of<T, KP>(a, w, a.k, 1, slot, k_head, s), base + Tiles::kK, tid, threads);
-    load_squares(reinterpret_cast<const __nv_bfloat16*>(work + w.solve) + place * kPieces * kSquare, kPieces,
+    load_squares(reinterpret_cast<const __nv_bfloat16*>(work + w.solve) + place * kLevel<T> * kSquare, kLevel<T>,
                  base + Tiles::kSolve, tid, threads);
-    load_squares(reinterpret_cast<const __nv_bfloat16*>(work + w.attention) + place * AP * kSquare, AP,
+    load_squares(reinterpret_cast<const __nv_bfloat16*>(work + w.attention) + place * kLevel<T> * kSquare, kLevel<T>,
                  base + Tiles::kAttention, tid, threads);
     const float* f = reinterpret_cast<const float*>(work + w.factors) + place * kFactors;
     for (int e = tid; e < kFactors / 4; e += threads) copy16(base + Tiles::kFactor + e * 16, f + e * 4, true);
@@ -477,11 +481,11 @@ struct ChainShape {
 
 // One sequence of one head, 16 columns of v a warp.  KEEP: the backward's run, which keeps S before each chunk and R
 // instead of writing o.
-template <typename T, int KP, int AP, int STAGES, bool KEEP>
+template <typename T, int KP, int STAGES, bool KEEP>
 CUBF_DEV void forward_chain(const GatedDeltaArgs& a, const Places& w, const ChainShape& shape, int slice, int head,
                             int sequence, unsigned char* raw) {
-    using Tiles = ChainTiles<T, KP, AP>;
-    constexpr int NI = Tiles::NI, LO = kOut<T>;
+    using Tiles = ChainTiles<T, KP>;
+    constexpr int NI = Tiles::NI, LEVEL = kLevel<T>;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = 32 * shape.warps;
     const int width = 16 * shape.warps, from = slice * width, v = from + 16 * warp;
     const int start = a.offsets ? offset_at(a, sequence) : 0;
@@ -491,7 +495,7 @@ CUBF_DEV void forward_chain(const GatedDeltaArgs& a, const Places& w, const Chai
     const int stage_bytes = Tiles::bytes(shape.warps);
     auto span = [&](int c) { return Span{sequence, c, start + c * C, min(C, length - c * C), row}; };
     auto load = [&](int c) {
-        load_chunk<T, KP, AP>(a, w, a.v, shape.wide_v, span(c), base + c, head, from, width,
+        load_chunk<T, KP>(a, w, a.v, shape.wide_v, span(c), base + c, head, from, width,
                               raw + (STAGES == 2 ? (c & 1) * stage_bytes : 0), tid, threads);
     };
     const size_t state = (static_cast<size_t>(sequence) * a.heads + head) * a.k_dim * a.v_dim;
@@ -517,8 +521,8 @@ CUBF_DEV void forward_chain(const GatedDeltaArgs& a, const Places& w, const Chai
             float x[8][4] = {}, o[8][4] = {};
 #pragma unroll
             for (int ks = 0; ks < KP / 16; ++ks) {
-                uint32_t f3[kPieces][4];
-                operand<kPieces>(s[2 * ks], s[2 * ks + 1], f3);
+                uint32_t f3[LEVEL][4];
+                operand<LEVEL>(s[2 * ks], s[2 * ks + 1], f3);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     uint32_t b[NI][2][4];
@@ -527,14 +531,14 @@ CUBF_DEV void forward_chain(const GatedDeltaArgs& a, const Places& w, const Chai
                         k.b_rows(i, 32 * t, 16 * ks, lane, b[i][0]);
                         k.b_rows(i, 32 * t + 16, 16 * ks, lane, b[i][1]);
                     }
-                    products<kPieces, kPieces, NI, 4>(x + 4 * t, f3, b);
+                    products<kInputLevel<T>, LEVEL, NI, 4>(x + 4 * t, f3, b);
                     if (!KEEP) {
 #pragma unroll
                         for (int i = 0; i < NI; ++i) {
                             q.b_rows(i, 32 * t, 16 * ks, lane, b[i][0]);
                             q.b_rows(i, 32 * t + 16, 16 * ks, lane, b[i][1]);
                         }
-                        products<LO, kPieces, NI, 4>(o + 4 * t, f3, b);
+                        products<kInputLevel<T>, LEVEL, NI, 4>(o + 4 * t, f3, b);
                     }
                 }
             }
@@ -553,14 +557,14 @@ CUBF_DEV void forward_chain(const GatedDeltaArgs& a, const Places& w, const Chai
             // R = Y - L (beta Y), the later tokens' columns first: those are added to before they are read
 #pragma unroll
             for (int ks = 3; ks >= 0; --ks) {
-                uint32_t f3[kPieces][4];
-                operand<kPieces>(x[2 * ks], x[2 * ks + 1], f + 2 * C + 16 * ks, -1.f, lane, f3);
+                uint32_t f3[LEVEL][4];
+                operand<LEVEL>(x[2 * ks], x[2 * ks + 1], f + 2 * C + 16 * ks, -1.f, lane, f3);
 #pragma unroll
                 for (int t = ks; t < 4; ++t) {
-                    uint32_t b[kPieces][1][4];
+                    uint32_t b[LEVEL][1][4];
 #pragma unroll
-                    for (int i = 0; i < kPieces; ++i) solve.b_rows(i, 16 * t, 16 * ks, lane, b[i][0]);
-                    products<kPieces, kPieces, kPieces, 2>(x + 2 * t, f3, b);
+                    for (int i = 0; i < LEVEL; ++i) solve.b_rows(i, 16 * t, 16 * ks, lane, b[i][0]);
+                    products<LEVEL, LEVEL, LEVEL, 2>(x + 2 * t, f3, b);
                 }
             }
             if (KEEP)
@@ -578,19 +582,19 @@ CUBF_DEV void forward_chain(const GatedDeltaArgs& a, const Places& w, const Chai
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
                 if (!KEEP) {
-                    uint32_t f2[LO][4];
-                    operand<LO>(x[2 * ks], x[2 * ks + 1], f2);
+                    uint32_t f2[LEVEL][4];
+                    operand<LEVEL>(x[2 * ks], x[2 * ks + 1], f2);
 #pragma unroll
                     for (int t = ks; t < 4; ++t) {
-                        uint32_t b[LO][1][4];
+                        uint32_t b[LEVEL][1][4];
 #pragma unroll
-                        for (int i = 0; i < LO; ++i) attention.b_rows(i, 16 * t, 16 * ks, lane, b[i][0]);
-                        products<LO, LO, LO, 2>(o + 2 * t, f2, b);
+                        for (int i = 0; i < LEVEL; ++i) attention.b_rows(i, 16 * t, 16 * ks, lane, b[i][0]);
+                        products<LEVEL, LEVEL, LEVEL, 2>(o + 2 * t, f2, b);
                     }
                 }
-                uint32_t f3[kPieces][4];
-                operand<kPieces>(x[2 * ks], x[2 * ks + 1], f + C + 16 * ks, 1.f, lane, f3);
-                onto_state<kPieces, kPieces, NI, KP>(s, f3, k, ks, lane);
+                uint32_t f3[LEVEL][4];
+                operand<LEVEL>(x[2 * ks], x[2 * ks + 1], f + C + 16 * ks, 1.f, lane, f3);
+                onto_state<kInputLevel<T>, LEVEL, NI, KP>(s, f3, k, ks, lane);
             }
             if (!KEEP) {
                 const size_t token = static_cast<size_t>(row) * a.length + start + c * C;
@@ -611,8 +615,8 @@ CUBF_DEV void forward_chain(const GatedDeltaArgs& a, const Places& w, const Chai
 template <typename T, int KP, int STAGES>
 CUBF_DEV void backward_chain(const GatedDeltaArgs& a, const Places& w, const ChainShape& shape, int slice, int head,
                              int sequence, unsigned char* raw) {
-    using Tiles = ChainTiles<T, KP, kPieces>;
-    constexpr int NI = Tiles::NI;
+    using Tiles = ChainTiles<T, KP>;
+    constexpr int NI = Tiles::NI, LEVEL = kLevel<T>;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = 32 * shape.warps;
     const int width = 16 * shape.warps, from = slice * width, v = from + 16 * warp;
     const int start = a.offsets ? offset_at(a, sequence) : 0;
@@ -621,7 +625,7 @@ CUBF_DEV void backward_chain(const GatedDeltaArgs& a, const Places& w, const Cha
     const int base = slot_base(a, sequence, start), chunks = (length + C - 1) / C;
     const int stage_bytes = Tiles::bytes(shape.warps);
     auto load = [&](int c) {
-        load_chunk<T, KP, kPieces>(a, w, a.d_o, shape.wide_d, Span{sequence, c, start + c * C, min(C, length - c * C), row},
+        load_chunk<T, KP>(a, w, a.d_o, shape.wide_d, Span{sequence, c, start + c * C, min(C, length - c * C), row},
                                    base + c, head, from, width, raw + (STAGES == 2 ? (c & 1) * stage_bytes : 0), tid, threads);
     };
     const size_t state = (static_cast<size_t>(sequence) * a.heads + head) * a.k_dim * a.v_dim;
@@ -646,8 +650,8 @@ CUBF_DEV void backward_chain(const GatedDeltaArgs& a, const Places& w, const Cha
             float x[8][4] = {};
 #pragma unroll
             for (int ks = 0; ks < KP / 16; ++ks) {
-                uint32_t f3[kPieces][4];
-                operand<kPieces>(s[2 * ks], s[2 * ks + 1], f3);
+                uint32_t f3[LEVEL][4];
+                operand<LEVEL>(s[2 * ks], s[2 * ks + 1], f3);
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     uint32_t b[NI][2][4];
@@ -656,7 +660,7 @@ CUBF_DEV void backward_chain(const GatedDeltaArgs& a, const Places& w, const Cha
                         k.b_rows(i, 32 * t, 16 * ks, lane, b[i][0]);
                         k.b_rows(i, 32 * t + 16, 16 * ks, lane, b[i][1]);
                     }
-                    products<kPieces, kPieces, NI, 4>(x + 4 * t, f3, b);
+                    products<kInputLevel<T>, LEVEL, NI, 4>(x + 4 * t, f3, b);
                 }
             }
 #pragma unroll
@@ -682,26 +686,26 @@ CUBF_DEV void backward_chain(const GatedDeltaArgs& a, const Places& w, const Cha
                 operand<NI>(d[0], d[1], exact);
 #pragma unroll
                 for (int t = 0; t <= ks; ++t) {
-                    uint32_t b[kPieces][1][4];
+                    uint32_t b[LEVEL][1][4];
 #pragma unroll
-                    for (int i = 0; i < kPieces; ++i) attention.b_cols(i, 16 * ks, 16 * t, lane, b[i][0]);
-                    products<kPieces, NI, kPieces, 2>(x + 2 * t, exact, b);
+                    for (int i = 0; i < LEVEL; ++i) attention.b_cols(i, 16 * ks, 16 * t, lane, b[i][0]);
+                    products<kInputLevel<T>, NI, LEVEL, 2>(x + 2 * t, exact, b);
                 }
-                uint32_t f3[kPieces][4];
-                operand<kPieces>(d[0], d[1], f + 16 * ks, a.scale, lane, f3);
-                onto_state<kPieces, kPieces, NI, KP>(s, f3, q, ks, lane);
+                uint32_t f3[LEVEL][4];
+                operand<LEVEL>(d[0], d[1], f + 16 * ks, a.scale, lane, f3);
+                onto_state<kInputLevel<T>, LEVEL, NI, KP>(s, f3, q, ks, lane);
             }
             // W = E - L^T (beta E), the earlier tokens' columns first
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
-                uint32_t f3[kPieces][4];
-                operand<kPieces>(x[2 * ks], x[2 * ks + 1], f + 2 * C + 16 * ks, -1.f, lane, f3);
+                uint32_t f3[LEVEL][4];
+                operand<LEVEL>(x[2 * ks], x[2 * ks + 1], f + 2 * C + 16 * ks, -1.f, lane, f3);
 #pragma unroll
                 for (int t = 0; t <= ks; ++t) {
-                    uint32_t b[kPieces][1][4];
+                    uint32_t b[LEVEL][1][4];
 #pragma unroll
-                    for (int i = 0; i < kPieces; ++i) solve.b_cols(i, 16 * ks, 16 * t, lane, b[i][0]);
-                    products<kPieces, kPieces, kPieces, 2>(x + 2 * t, f3, b);
+                    for (int i = 0; i < LEVEL; ++i) solve.b_cols(i, 16 * ks, 16 * t, lane, b[i][0]);
+                    products<LEVEL, LEVEL, LEVEL, 2>(x + 2 * t, f3, b);
                 }
             }
             rows_keep(reinterpret_cast<float*>(work + w.d_writes) + place * C * w.v_pitch, w.v_pitch, v, lane, x);
@@ -712,9 +716,9 @@ CUBF_DEV void backward_chain(const GatedDeltaArgs& a, const Places& w, const Cha
             }
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
-                uint32_t f3[kPieces][4];
-                operand<kPieces>(x[2 * ks], x[2 * ks + 1], f + 16 * ks, -1.f, lane, f3);
-                onto_state<kPieces, kPieces, NI, KP>(s, f3, k, ks, lane);
+                uint32_t f3[LEVEL][4];
+                operand<LEVEL>(x[2 * ks], x[2 * ks + 1], f + 16 * ks, -1.f, lane, f3);
+                onto_state<kInputLevel<T>, LEVEL, NI, KP>(s, f3, k, ks, lane);
             }
             const size_t token = static_cast<size_t>(row) * a.length + start + c * C;
             rows_store<T>(static_cast<T*>(a.d_v) + (token * a.heads + head) * a.v_dim + v,
@@ -734,7 +738,7 @@ __global__ void __launch_bounds__(256) gated_delta_forward_kernel(GatedDeltaArgs
     extern __shared__ __align__(16) unsigned char raw[];
     pdl_begin();
     const int slice = blockIdx.x % shape.slices, rest = blockIdx.x / shape.slices;
-    forward_chain<T, KP, kOut<T>, STAGES, false>(a, w, shape, slice, rest % a.heads, rest / a.heads, raw);
+    forward_chain<T, KP, STAGES, false>(a, w, shape, slice, rest % a.heads, rest / a.heads, raw);
 }
 
 // Both chains of the backward side by side: neither needs the other's results.
@@ -746,14 +750,14 @@ __global__ void __launch_bounds__(256) gated_delta_chains_kernel(GatedDeltaArgs 
     if (blockIdx.x % 2 == 0)
         backward_chain<T, KP, STAGES>(a, w, shape, slice, rest % a.heads, rest / a.heads, raw);
     else
-        forward_chain<T, KP, kPieces, STAGES, true>(a, w, shape, slice, rest % a.heads, rest / a.heads, raw);
+        forward_chain<T, KP, STAGES, true>(a, w, shape, slice, rest % a.heads, rest / a.heads, raw);
 }
 
 // ---- gradients ----------------------------------------------------------------------------------
 // A CTA per chunk and head: 16 warps, warp (r, c) holds rows 16 r .. of the tokens and a quarter of the channels.
 template <typename T, int KP>
 struct GradientShared {
-    static constexpr int NI = kInput<T>, LB = kOut<T>, ND = NI < LB ? NI : LB;
+    static constexpr int NI = kInput<T>, LB = kLevel<T>, ND = NI < LB ? NI : LB;
     static constexpr int VS = 32;                    // columns of v a turn
     static constexpr int kPitchV = VS + 8;
     alignas(16) __nv_bfloat16 q[NI * C * (KP + 8)];

@@ -52,8 +52,8 @@ Places places_of(const GatedDeltaArgs& a, bool backward) {
         return here;
     };
     w.factors = take(chunks * kFactors * 4);
-    w.solve = take(chunks * kPieces * kSquare * 2);
-    w.attention = take(chunks * (backward ? kPieces : kOut<T>) * kSquare * 2);
+    w.solve = take(chunks * kLevel<T> * kSquare * 2);
+    w.attention = take(chunks * kLevel<T> * kSquare * 2);
     w.packed = take(w.pack ? static_cast<size_t>(w.slots) * a.k_heads * 2 * kInput<T> * C * KP * 2 : 0);
     if (backward) {
         w.states = take(chunks * w.v_pitch * KP * 4);
@@ -97,24 +97,24 @@ cudaError_t launch_chains(const GatedDeltaArgs& a, const Places& w, bool backwar
     if (backward) {
         // set up for the largest CTA, launched with what this one's warps need
         static KernelSetup setup;
-        constexpr int most = kStages * ChainTiles<T, KP, kPieces>::bytes(8);
+        constexpr int most = kStages * ChainTiles<T, KP>::bytes(8);
         int cap = 0;
         const auto kernel = &gated_delta_chains_kernel<T, KP, kStages>;
         const cudaError_t e = setup_kernel(setup, kernel, 256, most, &cap, true);
         if (e != cudaSuccess) return e;
         if (2 * grid > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
         return launch_dependent(kernel, static_cast<unsigned>(2 * grid), 32u * shape.warps,
-                                kStages * ChainTiles<T, KP, kPieces>::bytes(shape.warps), stream, a, w, shape);
+                                kStages * ChainTiles<T, KP>::bytes(shape.warps), stream, a, w, shape);
     }
     static KernelSetup setup;
-    constexpr int most = kStages * ChainTiles<T, KP, kOut<T>>::bytes(8);
+    constexpr int most = kStages * ChainTiles<T, KP>::bytes(8);
     int cap = 0;
     const auto kernel = &gated_delta_forward_kernel<T, KP, kStages>;
     const cudaError_t e = setup_kernel(setup, kernel, 256, most, &cap, true);
     if (e != cudaSuccess) return e;
     if (grid > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
     return launch_dependent(kernel, static_cast<unsigned>(grid), 32u * shape.warps,
-                            kStages * ChainTiles<T, KP, kOut<T>>::bytes(shape.warps), stream, a, w, shape);
+                            kStages * ChainTiles<T, KP>::bytes(shape.warps), stream, a, w, shape);
 }
 
 }  // namespace
@@ -131,7 +131,7 @@ cudaError_t launch_gated_delta_unit<CUBF_GD_TYPE, CUBF_GD_K>(const GatedDeltaArg
     {
         static KernelSetup setup;
         const cudaError_t e = launch(setup, &gated_delta_prepare_kernel<T, KP>, chunks, 128, sizeof(PrepareShared<T, KP>),
-                                     stream, a, w, backward ? kPieces : kOut<T>);
+                                     stream, a, w);
         if (e != cudaSuccess) return e;
     }
     if (cudaError_t e = launch_chains(a, w, backward, stream); e != cudaSuccess || !backward) return e;

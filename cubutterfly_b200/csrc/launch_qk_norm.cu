@@ -1,0 +1,78 @@
+// launch_qk_norm.cu -- launches of the norm of queries and keys.
+#include <algorithm>
+
+#include "launch_util.cuh"
+#include "qk_norm.cuh"
+
+namespace cubf {
+namespace {
+
+using namespace qk;
+
+// Whole 16-byte vectors of every head: both halves of the pairs in the vector's steps, and aligned.
+template <typename T>
+bool vectors(const QkNormArgs& a, bool backward) {
+    constexpr size_t n = 16 / sizeof(T);
+    const size_t half = a.rotary / 2, rest = a.dim - a.rotary;
+    if (a.interleaved ? a.dim % (2 * n) != 0 : (half % n != 0 || rest % (2 * n) != 0)) return false;
+    size_t bits = static_cast<size_t>(a.dim) * sizeof(T);
+    auto take = [&](const HeadTensor& t) {
+        bits |= reinterpret_cast<uintptr_t>(t.p) | (t.batch | t.token | t.head) * sizeof(T);
+    };
+    take(a.q);
+    take(a.k);
+    if (backward) {
+        take(a.d_q_out);
+        take(a.d_k_out);
+    }
+    for (const void* p : {a.q_out, a.k_out, a.d_q, a.d_k}) bits |= reinterpret_cast<uintptr_t>(p);
+    return bits % 16 == 0;
+}
+
+template <typename T, int NP, bool VEC>
+cudaError_t launch_forward(const QkNormArgs& a, cudaStream_t stream) {
+    // all heads of a token a warp, fewer while that leaves SMs without one of their 32 warps
+    const size_t tokens = a.batch * a.tokens;
+    const int heads = a.q_heads + a.k_heads;
+    int lanes = 1;
+    const int pairs = a.rotary / 2 + (a.dim - a.rotary + 1) / 2;
+    while (lanes * NP < pairs) lanes *= 2;
+    const int turn = 32 / lanes;                 // heads that a warp takes side by side
+    int unit = (heads + turn - 1) / turn * turn;
+    while (unit > turn && tokens * ((heads + unit - 1) / unit) < 148 * 32) unit = (unit / turn + 1) / 2 * turn;
+    const int per_token = (heads + unit - 1) / unit;
+    const size_t units = tokens * per_token;
+    const size_t grid = std::min<size_t>((units + kWarps - 1) / kWarps, 0x7fffffffULL);
+    return launch_dependent(&qk_norm_kernel<T, NP, VEC>, static_cast<unsigned>(grid), 32u * kWarps, 0, stream, a, unit,
+                            per_token);
+}
+
+template <typename T>
+cudaError_t launch(QkNormArgs a, bool backward, cudaStream_t stream) {
+    constexpr int N = 16 / sizeof(T);
+    if (a.rotary == 0) a.interleaved = true;     // any pairs do: adjacent ones are read in the widest pieces
+    const bool wide = vectors<T>(a, backward);
+    if (!backward) return wide ? launch_forward<T, N, true>(a, stream) : launch_forward<T, 4, false>(a, stream);
+    const auto kernel = wide ? &qk_norm_backward_kernel<T, N, true> : &qk_norm_backward_kernel<T, 4, false>;
+    const cudaError_t e = launch_dependent(kernel, static_cast<unsigned>(a.parts), 32u * kWarps, 0, stream, a);
+    if (e != cudaSuccess || (!a.q_weight && !a.k_weight)) return e;
+    return launch_dependent(&qk_norm_weights_kernel<T>, static_cast<unsigned>((2 * a.dim + 31) / 32), 32u * kWarps, 0,
+                            stream, a);
+}
+
+}  // namespace
+
+int qk_norm_parts(const QkNormArgs& a) {
+    // a token a warp, four CTAs of 8 warps per SM at most
+    return static_cast<int>(std::min<size_t>((a.batch * a.tokens + kWarps - 1) / kWarps, 148 * 4));
+}
+
+cudaError_t launch_qk_norm(BlockType type, const QkNormArgs& a, bool backward, cudaStream_t stream) {
+    switch (type) {
+        case BlockType::kF16: return launch<__half>(a, backward, stream);
+        case BlockType::kBF16: return launch<__nv_bfloat16>(a, backward, stream);
+        default: return launch<float>(a, backward, stream);
+    }
+}
+
+}  // namespace cubf

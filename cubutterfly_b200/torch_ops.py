@@ -21,7 +21,8 @@ import threading
 import cubutterfly_b200 as cb
 
 __all__ = ["fwht", "hadamard_rotate", "fft", "zeta", "ntt", "plan_cache_size", "clear_plan_cache",
-           "InferenceGraph", "block_norm", "gated_scan", "gated_scan_step", "gated_delta", "gated_delta_step"]
+           "InferenceGraph", "block_norm", "gated_scan", "gated_scan_step", "gated_delta", "gated_delta_step",
+           "qk_norm"]
 
 _LOCK = threading.Lock()
 _PLANS: dict = {}
@@ -29,7 +30,7 @@ _PLANS: dict = {}
 
 def __getattr__(name):
     # the block operators import torch at module level, so they are loaded at first use
-    if name in ("block_norm", "gated_scan", "gated_scan_step", "gated_delta", "gated_delta_step"):
+    if name in ("block_norm", "gated_scan", "gated_scan_step", "gated_delta", "gated_delta_step", "qk_norm"):
         from cubutterfly_b200 import block_ops
 
         return getattr(block_ops, name)

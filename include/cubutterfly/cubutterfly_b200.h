@@ -361,6 +361,48 @@ typedef struct cubutterflyB200GatedDeltaStep_s {
 CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200GatedDeltaStep(const cubutterflyB200GatedDeltaStep_t* args,
                                                                 cudaStream_t stream);
 
+enum {
+    CUBUTTERFLY_B200_QK_LENGTH = 1,       /* heads of length one; else root mean square one */
+    CUBUTTERFLY_B200_QK_INTERLEAVED = 2,  /* pairs (2 j, 2 j + 1); else (j, j + rotary / 2) */
+    CUBUTTERFLY_B200_QK_POSITIONS64 = 4   /* positions are 64-bit integers; else 32-bit */
+};
+
+/* Norms of queries and keys head by head, rotated by their positions:
+ *   y = x / sqrt(mean(x^2) + epsilon) weight     (sum in place of mean with QK_LENGTH)
+ *   pair j of the first `rotary` values of y, angle = positions[axes[j]][token] frequencies[j]:
+ *   (a, b) -> (a cos angle - b sin angle, b cos angle + a sin angle)
+ * dim is at most 256; rotary is even, at most dim, and 0 without positions.
+ * q_weight and k_weight (dim) have data_type or FP32, or are null.  The
+ * position of token t of batch row b on axis x is
+ * positions[x positions_axis + (b tokens + t) mod positions_period]; axes
+ * (rotary / 2 values from 0 to axis_count - 1) is null with one axis.
+ * Angles are exact to 2e-7 up to positions of 2^31 (frequencies up to 1).
+ * Outputs and gradients are contiguous (batch, tokens, heads, dim). */
+typedef struct cubutterflyB200QkNorm_s {
+    size_t struct_size;
+    size_t batch, tokens, q_heads, k_heads, dim, rotary, axis_count, positions_axis, positions_period;
+    int data_type, q_weight_type, k_weight_type, flags;
+    double epsilon;
+    cubutterflyB200HeadTensor_t q, k;
+    const void *q_weight, *k_weight, *positions;
+    const float* frequencies;
+    const int* axes;
+    void *q_out, *k_out;
+    /* backward only */
+    cubutterflyB200HeadTensor_t d_q_out, d_k_out;
+    void *d_q, *d_k, *d_q_weight, *d_k_weight;  /* the last two required with their weights, in their types */
+    void* workspace;                            /* needed with weights */
+    size_t workspace_bytes;
+} cubutterflyB200QkNorm_t;
+
+CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200QkNormForward(const cubutterflyB200QkNorm_t* args,
+                                                               cudaStream_t stream);
+/* Reads batch, tokens, dim and the weights. */
+CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200QkNormGetWorkspaceSize(const cubutterflyB200QkNorm_t* args,
+                                                                        size_t* bytes);
+CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200QkNormBackward(const cubutterflyB200QkNorm_t* args,
+                                                                cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
