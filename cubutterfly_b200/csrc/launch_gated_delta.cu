@@ -4,6 +4,7 @@
 #include <algorithm>
 
 #include "gated_delta.cuh"
+#include "gated_delta_tc.cuh"
 #include "launch_util.cuh"
 
 #ifndef CUBF_GD_TYPE
@@ -43,7 +44,10 @@ Places places_of(const GatedDeltaArgs& a, bool backward) {
     Places w{};
     w.slots = a.offsets ? a.length / C + a.sequences : a.batch * ceil_div(a.length, C);
     w.v_pitch = ceil_div(a.v_dim, 16) * 16;
-    w.pack = !std::is_same_v<T, __nv_bfloat16> || !rows_aligned(a.q, a.k_dim) || !rows_aligned(a.k, a.k_dim);
+    w.v_rows = ceil_div(a.v_dim, 64) * 64;
+    w.state_piece = static_cast<size_t>(KP / 64) * w.v_rows * 128;
+    w.swizzled = sizeof(T) == 2 && !backward;
+    w.pack = w.swizzled || !std::is_same_v<T, __nv_bfloat16> || !rows_aligned(a.q, a.k_dim) || !rows_aligned(a.k, a.k_dim);
     const size_t chunks = static_cast<size_t>(w.slots) * a.heads;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -133,6 +137,14 @@ cudaError_t launch_gated_delta_unit<CUBF_GD_TYPE, CUBF_GD_K>(const GatedDeltaArg
         const cudaError_t e = launch(setup, &gated_delta_prepare_kernel<T, KP>, chunks, 128, sizeof(PrepareShared<T, KP>),
                                      stream, a, w);
         if (e != cudaSuccess) return e;
+    }
+    if constexpr (sizeof(T) == 2) {
+        if (!backward) {
+            static KernelSetup setup;
+            return launch(setup, &gated_delta_tc_forward_kernel<T, KP>, static_cast<size_t>(sequences_of(a)) * a.heads, kTcThreads,
+                          sizeof(TcShared<T, KP>), stream, a, w, rows_aligned(a.v, a.v_dim),
+                          rows_aligned(HeadTensor{a.o, 0, 0, static_cast<size_t>(a.v_dim)}, a.v_dim));
+        }
     }
     if (cudaError_t e = launch_chains(a, w, backward, stream); e != cudaSuccess || !backward) return e;
     constexpr int smem = sizeof(GradientShared<T, KP>);
