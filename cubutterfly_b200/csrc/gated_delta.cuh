@@ -31,7 +31,6 @@
 
 #include "gated_delta.hpp"
 #include "mma_split.cuh"
-#include "tcgen05.cuh"
 
 namespace cubf::delta {
 
@@ -69,11 +68,10 @@ constexpr int kTypeId = std::is_same_v<T, __half> ? 0 : 1;
 
 // ---- where things are ---------------------------------------------------------------------------
 struct Places {                          // of the workspace, in bytes from its start
-    size_t factors, solve, attention, packed, states, d_states, errors, d_writes, d_q, d_k, total;
+    size_t factors, solve, attention, packed, rows, states, d_states, errors, d_writes, d_q, d_k, total;
     size_t state_piece;                  // bytes of a piece of a kept state (gated_delta_tc.cuh)
     int slots, v_pitch, v_rows;          // v_dim rounded up to 16, to 64
     bool pack;                           // q and k are copied as bf16 pieces
-    bool swizzled;                       // ... and with L and P as swizzled tiles
 };
 
 struct Span {                            // a chunk
@@ -191,7 +189,7 @@ struct PrepareShared {
 
 template <typename T, int KP>
 CUBF_DEV void pack_rows(const GatedDeltaArgs& a, const HeadTensor& t, const Span& s, int head, __nv_bfloat16* tile,
-                        __nv_bfloat16* copy, bool swizzled, int tid) {
+                        __nv_bfloat16* copy, int tid) {
     constexpr int NI = kInput<T>;
     const T* p = static_cast<const T*>(t.p) + s.row * t.batch + static_cast<size_t>(s.first) * t.token +
                  static_cast<size_t>(head) * t.head;
@@ -208,8 +206,7 @@ CUBF_DEV void pack_rows(const GatedDeltaArgs& a, const HeadTensor& t, const Span
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             *reinterpret_cast<uint32_t*>(tile + (i * C + row) * (KP + 8) + col) = f[i];
-            if (copy)
-                *reinterpret_cast<uint32_t*>(copy + i * C * KP + (swizzled ? tc::swizzled(row, col) / 2 : row * KP + col)) = f[i];
+            if (copy) *reinterpret_cast<uint32_t*>(copy + (i * C + row) * KP + col) = f[i];
         }
     }
 }
@@ -234,8 +231,8 @@ __global__ void __launch_bounds__(128) gated_delta_prepare_kernel(GatedDeltaArgs
         if (head % group == 0)
             copy = reinterpret_cast<__nv_bfloat16*>(work + w.packed) +
                    (static_cast<size_t>(slot) * a.k_heads + k_head) * 2 * NI * C * KP;
-        pack_rows<T, KP>(a, a.q, s, k_head, sm.q, copy, w.swizzled, tid);
-        pack_rows<T, KP>(a, a.k, s, k_head, sm.k, copy ? copy + NI * C * KP : nullptr, w.swizzled, tid);
+        pack_rows<T, KP>(a, a.q, s, k_head, sm.q, copy, tid);
+        pack_rows<T, KP>(a, a.k, s, k_head, sm.k, copy ? copy + NI * C * KP : nullptr, tid);
     } else {
         load_source<1, KP>(source_of<T, KP>(a, w, a.q, 0, slot, k_head, s), smem_addr(sm.q), tid, 128);
         load_source<1, KP>(source_of<T, KP>(a, w, a.k, 1, slot, k_head, s), smem_addr(sm.k), tid, 128);
@@ -315,7 +312,7 @@ __global__ void __launch_bounds__(128) gated_delta_prepare_kernel(GatedDeltaArgs
             pieces<LEVEL>(p[0], p[1], f);
 #pragma unroll
             for (int n = 0; n < LEVEL; ++n)
-                *reinterpret_cast<uint32_t*>(attention + n * kSquare + (w.swizzled ? tc::swizzled(i, j) / 2 : i * C + j)) = f[n];
+                *reinterpret_cast<uint32_t*>(attention + n * kSquare + i * C + j) = f[n];
         }
     }
     __syncthreads();
@@ -340,7 +337,7 @@ __global__ void __launch_bounds__(128) gated_delta_prepare_kernel(GatedDeltaArgs
         for (int n = 0; n < LEVEL; ++n) {
             const __nv_bfloat16 piece = __float2bfloat16_rn(rest);
             rest -= __bfloat162float(piece);
-            solve[n * kSquare + (w.swizzled ? tc::swizzled(i, tid) / 2 : i * C + tid)] = piece;
+            solve[n * kSquare + i * C + tid] = piece;
         }
     }
 }

@@ -46,8 +46,8 @@ Places places_of(const GatedDeltaArgs& a, bool backward) {
     w.v_pitch = ceil_div(a.v_dim, 16) * 16;
     w.v_rows = ceil_div(a.v_dim, 64) * 64;
     w.state_piece = static_cast<size_t>(KP / 64) * w.v_rows * 128;
-    w.swizzled = sizeof(T) == 2 && !backward;
-    w.pack = w.swizzled || !std::is_same_v<T, __nv_bfloat16> || !rows_aligned(a.q, a.k_dim) || !rows_aligned(a.k, a.k_dim);
+    const bool tensor = sizeof(T) == 2 && !backward;
+    w.pack = tensor || !std::is_same_v<T, __nv_bfloat16> || !rows_aligned(a.q, a.k_dim) || !rows_aligned(a.k, a.k_dim);
     const size_t chunks = static_cast<size_t>(w.slots) * a.heads;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -55,9 +55,9 @@ Places places_of(const GatedDeltaArgs& a, bool backward) {
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    w.factors = take(chunks * kFactors * 4);
-    w.solve = take(chunks * kLevel<T> * kSquare * 2);
-    w.attention = take(chunks * kLevel<T> * kSquare * 2);
+    w.factors = take(chunks * (tensor ? kTcFactors * C : kFactors) * 4);
+    w.solve = take(chunks * (tensor ? 4 : kLevel<T>) * kSquare * 2);
+    w.attention = take(tensor ? 0 : chunks * kLevel<T> * kSquare * 2);
     w.packed = take(w.pack ? static_cast<size_t>(w.slots) * a.k_heads * 2 * kInput<T> * C * KP * 2 : 0);
     if (backward) {
         w.states = take(chunks * w.v_pitch * KP * 4);
@@ -132,19 +132,23 @@ template <>
 cudaError_t launch_gated_delta_unit<CUBF_GD_TYPE, CUBF_GD_K>(const GatedDeltaArgs& a, bool backward, cudaStream_t stream) {
     const Places w = places_of(a, backward);
     const size_t chunks = static_cast<size_t>(w.slots) * a.heads;
+    if constexpr (sizeof(T) == 2) {
+        if (!backward) {
+            static KernelSetup prepare, chain;
+            const cudaError_t e = launch(prepare, &gated_delta_tc_prepare_kernel<T, KP, false>,
+                                         static_cast<size_t>(w.slots) * a.k_heads, 128, sizeof(TcPrepareShared<T, KP, false>),
+                                         stream, a, w, rows_aligned(a.q, a.k_dim) && rows_aligned(a.k, a.k_dim), false);
+            if (e != cudaSuccess) return e;
+            return launch(chain, &gated_delta_tc_forward_kernel<T, KP>, static_cast<size_t>(sequences_of(a)) * a.heads,
+                          kTcThreads, sizeof(TcShared<T, KP>), stream, a, w, rows_aligned(a.v, a.v_dim),
+                          rows_aligned(HeadTensor{a.o, 0, 0, static_cast<size_t>(a.v_dim)}, a.v_dim));
+        }
+    }
     {
         static KernelSetup setup;
         const cudaError_t e = launch(setup, &gated_delta_prepare_kernel<T, KP>, chunks, 128, sizeof(PrepareShared<T, KP>),
                                      stream, a, w);
         if (e != cudaSuccess) return e;
-    }
-    if constexpr (sizeof(T) == 2) {
-        if (!backward) {
-            static KernelSetup setup;
-            return launch(setup, &gated_delta_tc_forward_kernel<T, KP>, static_cast<size_t>(sequences_of(a)) * a.heads, kTcThreads,
-                          sizeof(TcShared<T, KP>), stream, a, w, rows_aligned(a.v, a.v_dim),
-                          rows_aligned(HeadTensor{a.o, 0, 0, static_cast<size_t>(a.v_dim)}, a.v_dim));
-        }
     }
     if (cudaError_t e = launch_chains(a, w, backward, stream); e != cudaSuccess || !backward) return e;
     constexpr int smem = sizeof(GradientShared<T, KP>);
