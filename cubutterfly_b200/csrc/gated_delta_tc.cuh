@@ -60,7 +60,7 @@ struct TcShared {
     alignas(16) T rows[C * 128];                             // v of a chunk
     alignas(16) T out[C * 128];                              // o of a chunk
     alignas(16) float factors[2][3 * C];                     // kTailBeta, kDecay, kScaled
-    alignas(8) unsigned long long full[2], ready[4], done[4], rows_full, out_ready, out_free;
+    alignas(8) unsigned long long full[2], empty[2], ready[5], done[4], rows_full, rows_empty, out_ready, out_free;
     uint32_t base;
 };
 
@@ -343,7 +343,9 @@ struct TcChain {
             for (auto& b : sm.full) tc::barrier_init(smem_addr(&b), 1);
             for (auto& b : sm.done) tc::barrier_init(smem_addr(&b), 1);
             for (auto& b : sm.ready) tc::barrier_init(smem_addr(&b), kTcCompute / 32);
+            for (auto& b : sm.empty) tc::barrier_init(smem_addr(&b), kTcCompute / 32 + 1);  // factors read, products done
             tc::barrier_init(smem_addr(&sm.rows_full), kTcMovers);
+            tc::barrier_init(smem_addr(&sm.rows_empty), kTcCompute / 32);
             tc::barrier_init(smem_addr(&sm.out_ready), kTcCompute / 32);
             tc::barrier_init(smem_addr(&sm.out_free), kTcMovers / 32);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -384,6 +386,11 @@ struct TcChain {
     CUBF_DEV void arrive(unsigned long long& barrier) const {
         tc::wait_store();
         tc::fence_before();
+        __syncwarp();
+        if (lane == 0) tc::barrier_arrive(smem_addr(&barrier));
+    }
+
+    CUBF_DEV void report(unsigned long long& barrier) const {
         __syncwarp();
         if (lane == 0) tc::barrier_arrive(smem_addr(&barrier));
     }
@@ -446,62 +453,86 @@ struct TcChain {
                             i + j + s > 0);
     }
 
+    // What the computing warps report: the state, Y, U and the output's first part are where a product takes them from or
+    // may put its result.
+    enum Ready { kStateReady, kYReady, kUReady, kOutTaken, kOutAdded };
+    // What the products report: S k, L Y, k U, P U.
+    enum Done { kSk, kLy, kKu, kPu };
+
     template <bool KEEP>
     CUBF_DEV void issue_forward() {
         const int chunks = chain.chunks;
         if (chunks > 0) load(0, 0);
+        if (chunks > 1) load(1, 1);
         uint32_t phase = 0;
         for (int c = 0; c < chunks && !failed; ++c, phase ^= 1) {
             const int st = c & 1;
-            wait(sm.ready[0], phase);
             wait(sm.full[st], (c >> 1) & 1);
+            wait(sm.ready[kStateReady], phase);
             if (failed) break;
             if (tc::elect()) {
                 state_times(Tiles::kX, k(st));
-                tc::commit(smem_addr(&sm.done[0]));
-                if (!KEEP) state_times(Tiles::kO, q(st));
+                tc::commit(smem_addr(&sm.done[kSk]));
             }
             __syncwarp();
-            // the other stage is free: its chunk's last products are done, its factors read
-            if (c > 0) wait(sm.done[KEEP ? 2 : 3], phase ^ 1);
-            if (failed) break;
-            if (c + 1 < chunks) load(c + 1, st ^ 1);
-            wait(sm.ready[1], phase);
+            if (!KEEP) {
+                if (c > 0) wait(sm.ready[kOutAdded], phase ^ 1);
+                if (failed) break;
+                if (tc::elect()) state_times(Tiles::kO, q(st));
+                __syncwarp();
+            }
+            wait(sm.ready[kYReady], phase);
             if (failed) break;
             if (tc::elect()) {
                 times_square(Tiles::kX, Tiles::kY, solve(st));
-                tc::commit(smem_addr(&sm.done[1]));
+                tc::commit(smem_addr(&sm.done[kLy]));
             }
             __syncwarp();
-            wait(sm.ready[2], phase);
+            if (c > 0 && c + 1 < chunks) {       // the stage that the chunk before has left
+                wait(sm.empty[st ^ 1], ((c - 1) >> 1) & 1);
+                if (failed) break;
+                load(c + 1, st ^ 1);
+            }
+            wait(sm.ready[kUReady], phase);
             if (failed) break;
             if (tc::elect()) {
                 onto_state(Tiles::kD, Tiles::kU, k(st), false);
-                tc::commit(smem_addr(&sm.done[2]));
+                tc::commit(smem_addr(&sm.done[kKu]));
+                if (KEEP) tc::commit(smem_addr(&sm.empty[st]));
             }
             __syncwarp();
-            if (KEEP) continue;
-            wait(sm.ready[3], phase);
-            if (failed) break;
-            if (tc::elect()) {
-                times_square(Tiles::kX, Tiles::kY, attention(st));
-                tc::commit(smem_addr(&sm.done[3]));
+            if (!KEEP) {
+                wait(sm.ready[kOutTaken], phase);
+                if (failed) break;
+                if (tc::elect()) {
+                    times_square(Tiles::kO, Tiles::kY, attention(st));
+                    tc::commit(smem_addr(&sm.done[kPu]));
+                    tc::commit(smem_addr(&sm.empty[st]));
+                }
+                __syncwarp();
             }
-            __syncwarp();
         }
     }
 
     // ---- the moving warps ----
+    // 16 threads a row of 128 columns, six rows at a time; addresses advance by constants, since these warps share the
+    // schedulers and instruction caches with the computing ones.
+    static constexpr int kSide = kTcMovers / 16, kTurns = (C + kSide - 1) / kSide;
     CUBF_DEV void load_tile(const HeadTensor& t, int c, bool wide) const {
+        const int n = tokens(c), first = tid - kTcCompute - 32;
         const T* p = static_cast<const T*>(t.p) + chain.row * t.batch + (static_cast<size_t>(chain.start) + c * C) * t.token +
                      static_cast<size_t>(chain.head) * t.head;
-        const int n = tokens(c), first = tid - kTcCompute - 32;
-        constexpr int N = 16 / sizeof(T);
         if (wide) {
-            for (int e = first; e < C * 128 / N; e += kTcMovers) {
-                const int r = e / (128 / N), col = e % (128 / N) * N;
-                const bool ok = r < n && col < a.v_dim;
-                copy16(smem_addr(sm.rows + r * 128 + col), p + (ok ? r * t.token + col : 0), ok);
+            const int row = first / 16, col = first % 16 * 8;
+            const T* q = p + (col < a.v_dim ? row * t.token + col : 0);
+            const size_t step = col < a.v_dim ? kSide * t.token : 0;
+            const uint32_t to = smem_addr(sm.rows + row * 128 + col);
+            const int valid = col < a.v_dim ? n - row : 0;
+#pragma unroll
+            for (int i = 0; i < kTurns; ++i) {
+                const bool ok = kSide * i < valid;
+                if (kSide * i + row < C) copy16(to + i * kSide * 256, ok ? q : p, ok);
+                q += step;
             }
         } else {
             for (int e = first; e < C * 128; e += kTcMovers) {
@@ -517,12 +548,14 @@ struct TcChain {
         T* p = out + out_row(c) * a.v_dim;
         const size_t step = static_cast<size_t>(a.heads) * a.v_dim;
         const int n = tokens(c), first = tid - kTcCompute - 32;
-        constexpr int N = 16 / sizeof(T);
         if (wide) {
-            for (int e = first; e < n * (128 / N); e += kTcMovers) {
-                const int r = e / (128 / N), col = e % (128 / N) * N;
-                if (col < a.v_dim)
-                    *reinterpret_cast<uint4*>(p + r * step + col) = *reinterpret_cast<const uint4*>(sm.out + r * 128 + col);
+            const int row = first / 16, col = first % 16 * 8, valid = col < a.v_dim ? n - row : 0;
+            const T* from = sm.out + row * 128 + col;
+            T* to = p + row * step + col;
+#pragma unroll
+            for (int i = 0; i < kTurns; ++i) {
+                if (kSide * i < valid) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from + i * kSide * 128);
+                to += kSide * step;
             }
         } else {
             for (int e = first; e < n * 128; e += kTcMovers) {
@@ -533,21 +566,24 @@ struct TcChain {
         __syncwarp();
         if (lane == 0) tc::barrier_arrive(smem_addr(&sm.out_free));
     }
-    // Rows of chunk c come in once those before were read, the output before leaves.
+    // Rows come in once those before were read, the output leaves.  Every barrier here is one of a ring: none can complete
+    // a second time before its waiter has gone on.
     template <bool KEEP>
     CUBF_DEV void move_forward(bool wide_v, bool wide_o) {
-        for (int c = 0; c < chain.chunks && !failed; ++c) {
-            if (c > 0) wait(sm.ready[1], (c - 1) & 1);
+        const int chunks = chain.chunks;
+        for (int c = 0; c < chunks && !failed; ++c) {
+            if (c > 0) wait(sm.rows_empty, (c - 1) & 1);
             if (!failed) load_tile(a.v, c, wide_v);
-            if (!KEEP && c > 0) {
-                wait(sm.out_ready, (c - 1) & 1);
-                if (!failed) store_tile(static_cast<T*>(a.o), c - 1, wide_o);
+            if (!KEEP && c > 1) {
+                wait(sm.out_ready, c & 1);
+                if (!failed) store_tile(static_cast<T*>(a.o), c - 2, wide_o);
             }
         }
-        if (!KEEP && chain.chunks > 0) {
-            wait(sm.out_ready, (chain.chunks - 1) & 1);
-            if (!failed) store_tile(static_cast<T*>(a.o), chain.chunks - 1, wide_o);
-        }
+        if (!KEEP)
+            for (int c = max(0, chunks - 2); c < chunks && !failed; ++c) {
+                wait(sm.out_ready, c & 1);
+                if (!failed) store_tile(static_cast<T*>(a.o), c, wide_o);
+            }
         copies_wait<0>();
     }
 
@@ -680,30 +716,36 @@ struct TcChain {
     // KEEP: the backward's run, which keeps the state before each chunk and R in place of writing o.
     template <bool KEEP>
     CUBF_DEV void compute_forward() {
-        P s[H / 2], o[16];
+        P s[H / 2], y[16], x[16], o[16];
         state_in(a.initial ? a.initial + state_offset() : nullptr, s);
         const int chunks = chain.chunks;
+        auto add_out = [&](int c) {          // the last part of a chunk's o
+            wait(sm.done[kPu], c & 1);
+            get_tokens(Tiles::kO, x);
+            if (c + 1 < chunks) arrive(sm.ready[kOutAdded]);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = f32x2::add2(o[i], x[i]);
+        };
+        auto move_out = [&](int c) {
+            if (c > 0) wait(sm.out_free, (c - 1) & 1);
+            put_out(o);
+        };
         if (chunks > 0) {
             put_state(s, KEEP ? work(w.states) + place(0) * 2 * w.state_piece : nullptr);
-            arrive(sm.ready[0]);
+            arrive(sm.ready[kStateReady]);
         }
         uint32_t phase = 0;
         for (int c = 0; c < chunks && !failed; ++c, phase ^= 1) {
-            const int st = c & 1;
-            const float* f = sm.factors[st];
-            // while the state meets k and q: the last chunk's o leaves, this one's v is read
-            if (!KEEP && c > 0) {
-                if (c > 1) wait(sm.out_free, phase);
-                put_out(o);
-            }
+            const float* f = sm.factors[c & 1];
+            // while the state meets k
+            if (!KEEP && c > 0) add_out(c - 1);
+            wait(sm.full[c & 1], (c >> 1) & 1);
             wait(sm.rows_full, phase);
-            P y[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 y[i] = f32x2::pk(widen(sm.rows[(32 * half + 2 * i) * 128 + v]), widen(sm.rows[(32 * half + 2 * i + 1) * 128 + v]));
-            wait(sm.full[st], (c >> 1) & 1);
-            wait(sm.done[0], phase);
-            P x[16];
+            report(sm.rows_empty);
+            wait(sm.done[kSk], phase);
             get_tokens(Tiles::kX, x);
 #pragma unroll
             for (int g = 0; g < 8; ++g) {    // Y = v - e^G (S k)
@@ -713,19 +755,21 @@ struct TcChain {
                 y[2 * g + 1] = f32x2::sub2(y[2 * g + 1], f32x2::mul2(b, x[2 * g + 1]));
             }
             put_tokens(Tiles::kY, y);
-            arrive(sm.ready[1]);
-            wait(sm.done[1], phase);
+            arrive(sm.ready[kYReady]);
+            if (!KEEP && c > 0) move_out(c - 1);  // while Y meets L
+            wait(sm.done[kLy], phase);
             get_tokens(Tiles::kX, x);
 #pragma unroll
             for (int i = 0; i < 16; ++i) y[i] = f32x2::sub2(y[i], x[i]);  // R = Y - (L beta) Y
             put_tokens(Tiles::kU, y, f + kTailBeta * C);
-            arrive(sm.ready[2]);
+            arrive(sm.ready[kUReady]);
+            // while U meets k
             if (KEEP) {
                 rows_keep(w.errors, c, y);
             } else {
                 put_tokens(Tiles::kY, y);
-                arrive(sm.ready[3]);
-                get_tokens(Tiles::kO, x);    // q's part of o is there since the products with L
+                get_tokens(Tiles::kO, x);
+                arrive(sm.ready[kOutTaken]);
 #pragma unroll
                 for (int g = 0; g < 8; ++g) {
                     P a, b;
@@ -735,20 +779,17 @@ struct TcChain {
                 }
             }
             const float whole = f[kDecay * C + C - 1];
-            wait(sm.done[2], phase);
+            report(sm.empty[c & 1]);
+            wait(sm.done[kKu], phase);
             state_add(whole, s);
             put_state(s, KEEP && c + 1 < chunks ? work(w.states) + place(c + 1) * 2 * w.state_piece : nullptr);
-            if (!KEEP) {
-                wait(sm.done[3], phase);
-                get_tokens(Tiles::kX, x);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[i] = f32x2::add2(o[i], x[i]);
-            }
-            if (c + 1 < chunks) arrive(sm.ready[0]);
+            if (c + 1 < chunks) arrive(sm.ready[kStateReady]);
         }
         if (!KEEP) {
-            if (chunks > 1) wait(sm.out_free, chunks & 1);
-            if (chunks > 0) put_out(o);
+            if (chunks > 0 && !failed) {
+                add_out(chunks - 1);
+                move_out(chunks - 1);
+            }
             state_out(a.last + state_offset(), s);
         }
     }

@@ -17,7 +17,7 @@ namespace cubf::tc {
 using split::smem_addr;
 
 constexpr int kPanel = 8192;             // bytes of 64 x 64 values
-constexpr uint32_t kSpinLimit = 1u << 20;
+constexpr uint32_t kSpinLimit = 1u << 17;  // tries, of 8 us each where nothing comes: a second
 
 // Byte offset of (row, col) in a tile of panels side by side.
 CUBF_DEV uint32_t swizzled(int row, int col) {
