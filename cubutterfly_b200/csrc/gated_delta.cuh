@@ -68,10 +68,9 @@ constexpr int kTypeId = std::is_same_v<T, __half> ? 0 : 1;
 
 // ---- where things are ---------------------------------------------------------------------------
 struct Places {                          // of the workspace, in bytes from its start
-    size_t factors, solve, attention, packed, rows, states, d_states, errors, d_writes, d_q, d_k, total;
-    size_t state_piece;                  // bytes of a piece of a kept state (gated_delta_tc.cuh)
+    size_t factors, solve, attention, packed, values, rows, states, d_states, errors, d_writes, d_q, d_k, total;
+    size_t state_piece, squares;         // bytes of a piece of a kept state, of a chunk's matrices (gated_delta_tc.cuh)
     int slots, v_pitch, v_rows;          // v_dim rounded up to 16, to 64
-    bool pack;                           // q and k are copied as bf16 pieces
 };
 
 struct Span {                            // a chunk
@@ -113,33 +112,16 @@ CUBF_DEV Span span_of(const GatedDeltaArgs& a, int slot) {
 }
 
 // ---- q and k of a chunk as bf16 pieces ----------------------------------------------------------
-// Straight from the tensors (bf16, 16-byte pieces) or from the copies that `prepare` made.
-struct Source {
-    const __nv_bfloat16* p;
-    size_t row, piece;                   // strides
-    int rows, cols;                      // valid ones
-};
 template <typename T, int KP>
-CUBF_DEV Source source_of(const GatedDeltaArgs& a, const Places& w, const HeadTensor& t, int which, int slot, int head,
-                          const Span& s) {
-    constexpr int NI = kInput<T>;
-    if (w.pack) {
-        const size_t tile = (static_cast<size_t>(slot) * a.k_heads + head) * 2 + which;
-        return {reinterpret_cast<const __nv_bfloat16*>(static_cast<const char*>(a.workspace) + w.packed) + tile * NI * C * KP,
-                KP, static_cast<size_t>(C) * KP, C, KP};
-    }
-    return {static_cast<const __nv_bfloat16*>(t.p) + s.row * t.batch + static_cast<size_t>(s.first) * t.token +
-                static_cast<size_t>(head) * t.head,
-            t.token, 0, s.tokens, a.k_dim};
+CUBF_DEV const __nv_bfloat16* packed_at(const GatedDeltaArgs& a, const Places& w, int which, int slot, int head) {
+    const size_t tile = (static_cast<size_t>(slot) * a.k_heads + head) * 2 + which;
+    return reinterpret_cast<const __nv_bfloat16*>(static_cast<const char*>(a.workspace) + w.packed) + tile * kInput<T> * C * KP;
 }
-template <int NI, int KP, int THREADS = 0>
-CUBF_DEV void load_source(const Source& s, uint32_t tile, int tid, int threads) {
-    constexpr int PIECES = KP / 8;
-    for (int e = tid; e < NI * C * PIECES; e += threads) {
-        const int piece = e / (C * PIECES), row = e / PIECES % C, col = e % PIECES * 8;
-        const bool ok = row < s.rows && col < s.cols;
-        const __nv_bfloat16* p = s.p + (ok ? piece * s.piece + row * s.row + col : 0);
-        copy16(tile + static_cast<uint32_t>((piece * C + row) * (KP + 8) + col) * 2u, p, ok);
+template <int NI, int KP>
+CUBF_DEV void load_packed(const __nv_bfloat16* p, uint32_t tile, int tid, int threads) {
+    for (int e = tid; e < NI * C * (KP / 8); e += threads) {
+        const int row = e / (KP / 8), col = e % (KP / 8) * 8;  // rows of all pieces
+        copy16(tile + static_cast<uint32_t>(row * (KP + 8) + col) * 2u, p + static_cast<size_t>(e) * 8, true);
     }
 }
 // N pieces of 64 x 64
@@ -226,18 +208,12 @@ __global__ void __launch_bounds__(128) gated_delta_prepare_kernel(GatedDeltaArgs
     const size_t place = static_cast<size_t>(slot) * a.heads + head;
     char* const work = static_cast<char*>(a.workspace);
 
-    if (w.pack) {
-        __nv_bfloat16* copy = nullptr;
-        if (head % group == 0)
-            copy = reinterpret_cast<__nv_bfloat16*>(work + w.packed) +
-                   (static_cast<size_t>(slot) * a.k_heads + k_head) * 2 * NI * C * KP;
-        pack_rows<T, KP>(a, a.q, s, k_head, sm.q, copy, tid);
-        pack_rows<T, KP>(a, a.k, s, k_head, sm.k, copy ? copy + NI * C * KP : nullptr, tid);
-    } else {
-        load_source<1, KP>(source_of<T, KP>(a, w, a.q, 0, slot, k_head, s), smem_addr(sm.q), tid, 128);
-        load_source<1, KP>(source_of<T, KP>(a, w, a.k, 1, slot, k_head, s), smem_addr(sm.k), tid, 128);
-        copies_commit();
-    }
+    __nv_bfloat16* copy = nullptr;
+    if (head % group == 0)
+        copy = reinterpret_cast<__nv_bfloat16*>(work + w.packed) +
+               (static_cast<size_t>(slot) * a.k_heads + k_head) * 2 * NI * C * KP;
+    pack_rows<T, KP>(a, a.q, s, k_head, sm.q, copy, tid);
+    pack_rows<T, KP>(a, a.k, s, k_head, sm.k, copy ? copy + NI * C * KP : nullptr, tid);
     if (warp < 2) {  // running sums of the log decays, in 64 bits
         double sum = 0;
         float b = 0.f;
@@ -258,7 +234,6 @@ __global__ void __launch_bounds__(128) gated_delta_prepare_kernel(GatedDeltaArgs
     }
     __syncthreads();
     if (warp == 1) sm.sum[tid] += sm.sum[31];
-    if (!w.pack) copies_wait<0>();
     __syncthreads();
     if (tid < C) {
         float* f = reinterpret_cast<float*>(work + w.factors) + place * kFactors;
@@ -366,8 +341,8 @@ CUBF_DEV void load_chunk(const GatedDeltaArgs& a, const Places& w, const HeadTen
     const size_t place = static_cast<size_t>(slot) * a.heads + head;
     char* const work = static_cast<char*>(a.workspace);
     const uint32_t base = smem_addr(stage);
-    load_source<kInput<T>, KP>(source_of<T, KP>(a, w, a.q, 0, slot, k_head, s), base + Tiles::kQ, tid, threads);
-    load_source<kInput<T>, KP>(source_of<T, KP>(a, w, a.k, 1, slot, k_head, s), base + Tiles::kK, tid, threads);
+    load_packed<kInput<T>, KP>(packed_at<T, KP>(a, w, 0, slot, k_head), base + Tiles::kQ, tid, threads);
+    load_packed<kInput<T>, KP>(packed_at<T, KP>(a, w, 1, slot, k_head), base + Tiles::kK, tid, threads);
     load_squares(reinterpret_cast<const __nv_bfloat16*>(work + w.solve) + place * kLevel<T> * kSquare, kLevel<T>,
                  base + Tiles::kSolve, tid, threads);
     load_squares(reinterpret_cast<const __nv_bfloat16*>(work + w.attention) + place * kLevel<T> * kSquare, kLevel<T>,
@@ -483,7 +458,7 @@ struct ChainShape {
 
 // One sequence of one head, 16 columns of v a warp.  KEEP: the backward's run, which keeps S before each chunk and R
 // instead of writing o.
-template <typename T, int KP, int STAGES, bool KEEP>
+template <typename T, int KP, bool KEEP>
 CUBF_DEV void forward_chain(const GatedDeltaArgs& a, const Places& w, const ChainShape& shape, int slice, int head,
                             int sequence, unsigned char* raw) {
     using Tiles = ChainTiles<T, KP>;
@@ -494,11 +469,10 @@ CUBF_DEV void forward_chain(const GatedDeltaArgs& a, const Places& w, const Chai
     const int length = a.offsets ? max(0, offset_at(a, sequence + 1) - start) : a.length;
     const int row = a.offsets ? 0 : sequence;
     const int base = slot_base(a, sequence, start), chunks = (length + C - 1) / C;
-    const int stage_bytes = Tiles::bytes(shape.warps);
     auto span = [&](int c) { return Span{sequence, c, start + c * C, min(C, length - c * C), row}; };
     auto load = [&](int c) {
         load_chunk<T, KP>(a, w, a.v, shape.wide_v, span(c), base + c, head, from, width,
-                              raw + (STAGES == 2 ? (c & 1) * stage_bytes : 0), tid, threads);
+                              raw, tid, threads);
     };
     const size_t state = (static_cast<size_t>(sequence) * a.heads + head) * a.k_dim * a.v_dim;
     float s[KP / 8][4];
@@ -507,8 +481,7 @@ CUBF_DEV void forward_chain(const GatedDeltaArgs& a, const Places& w, const Chai
     for (int c = 0; c < chunks; ++c) {
         copies_wait<0>();
         __syncthreads();
-        if (STAGES == 2 && c + 1 < chunks) load(c + 1);
-        unsigned char* stage = raw + (STAGES == 2 ? (c & 1) * stage_bytes : 0);
+        unsigned char* const stage = raw;
         const uint32_t at = smem_addr(stage);
         const Tile<KP + 8, C*(KP + 8)> q{at + Tiles::kQ}, k{at + Tiles::kK};
         const Tile<kPitchC, C * kPitchC> solve{at + Tiles::kSolve}, attention{at + Tiles::kAttention};
@@ -605,16 +578,14 @@ CUBF_DEV void forward_chain(const GatedDeltaArgs& a, const Places& w, const Chai
                               tile, pitch, lane, o);
             }
         }
-        if (STAGES == 1) {
-            __syncthreads();
-            if (c + 1 < chunks) load(c + 1);
-        }
+        __syncthreads();
+        if (c + 1 < chunks) load(c + 1);
     }
     if (!KEEP && v < a.v_dim) state_store<KP>(a.last + state, a.k_dim, a.v_dim, v, lane, s);
 }
 
 // The same sequence from its end: dS, W and dv of every chunk.
-template <typename T, int KP, int STAGES>
+template <typename T, int KP>
 CUBF_DEV void backward_chain(const GatedDeltaArgs& a, const Places& w, const ChainShape& shape, int slice, int head,
                              int sequence, unsigned char* raw) {
     using Tiles = ChainTiles<T, KP>;
@@ -625,10 +596,9 @@ CUBF_DEV void backward_chain(const GatedDeltaArgs& a, const Places& w, const Cha
     const int length = a.offsets ? max(0, offset_at(a, sequence + 1) - start) : a.length;
     const int row = a.offsets ? 0 : sequence;
     const int base = slot_base(a, sequence, start), chunks = (length + C - 1) / C;
-    const int stage_bytes = Tiles::bytes(shape.warps);
     auto load = [&](int c) {
         load_chunk<T, KP>(a, w, a.d_o, shape.wide_d, Span{sequence, c, start + c * C, min(C, length - c * C), row},
-                                   base + c, head, from, width, raw + (STAGES == 2 ? (c & 1) * stage_bytes : 0), tid, threads);
+                                   base + c, head, from, width, raw, tid, threads);
     };
     const size_t state = (static_cast<size_t>(sequence) * a.heads + head) * a.k_dim * a.v_dim;
     float s[KP / 8][4];  // dS, transposed
@@ -637,8 +607,7 @@ CUBF_DEV void backward_chain(const GatedDeltaArgs& a, const Places& w, const Cha
     for (int c = chunks - 1; c >= 0; --c) {
         copies_wait<0>();
         __syncthreads();
-        if (STAGES == 2 && c > 0) load(c - 1);
-        unsigned char* stage = raw + (STAGES == 2 ? (c & 1) * stage_bytes : 0);
+        unsigned char* const stage = raw;
         const uint32_t at = smem_addr(stage);
         const Tile<KP + 8, C*(KP + 8)> q{at + Tiles::kQ}, k{at + Tiles::kK};
         const Tile<kPitchC, C * kPitchC> solve{at + Tiles::kSolve}, attention{at + Tiles::kAttention};
@@ -727,38 +696,36 @@ CUBF_DEV void backward_chain(const GatedDeltaArgs& a, const Places& w, const Cha
                           static_cast<size_t>(a.heads) * a.v_dim, min(C, length - c * C), a.v_dim - v, shape.wide_o, tile,
                           pitch, lane, x);
         }
-        if (STAGES == 1) {
-            __syncthreads();
-            if (c > 0) load(c - 1);
-        }
+        __syncthreads();
+        if (c > 0) load(c - 1);
     }
     if (a.d_initial && v < a.v_dim) state_store<KP>(a.d_initial + state, a.k_dim, a.v_dim, v, lane, s);
 }
 
-template <typename T, int KP, int STAGES>
+template <typename T, int KP>
 __global__ void __launch_bounds__(256) gated_delta_forward_kernel(GatedDeltaArgs a, Places w, ChainShape shape) {
     extern __shared__ __align__(16) unsigned char raw[];
     pdl_begin();
     const int slice = blockIdx.x % shape.slices, rest = blockIdx.x / shape.slices;
-    forward_chain<T, KP, STAGES, false>(a, w, shape, slice, rest % a.heads, rest / a.heads, raw);
+    forward_chain<T, KP, false>(a, w, shape, slice, rest % a.heads, rest / a.heads, raw);
 }
 
 // Both chains of the backward side by side: neither needs the other's results.
-template <typename T, int KP, int STAGES>
+template <typename T, int KP>
 __global__ void __launch_bounds__(256) gated_delta_chains_kernel(GatedDeltaArgs a, Places w, ChainShape shape) {
     extern __shared__ __align__(16) unsigned char raw[];
     pdl_begin();
     const int slice = blockIdx.x / 2 % shape.slices, rest = blockIdx.x / 2 / shape.slices;
     if (blockIdx.x % 2 == 0)
-        backward_chain<T, KP, STAGES>(a, w, shape, slice, rest % a.heads, rest / a.heads, raw);
+        backward_chain<T, KP>(a, w, shape, slice, rest % a.heads, rest / a.heads, raw);
     else
-        forward_chain<T, KP, STAGES, true>(a, w, shape, slice, rest % a.heads, rest / a.heads, raw);
+        forward_chain<T, KP, true>(a, w, shape, slice, rest % a.heads, rest / a.heads, raw);
 }
 
 // ---- gradients ----------------------------------------------------------------------------------
 // A CTA per chunk and head: 16 warps, warp (r, c) holds rows 16 r .. of the tokens and a quarter of the channels.
 template <typename T, int KP>
-struct GradientShared {
+struct GradientShared32 {
     static constexpr int NI = kInput<T>, LB = kLevel<T>, ND = NI < LB ? NI : LB;
     static constexpr int VS = 32;                    // columns of v a turn
     static constexpr int kPitchV = VS + 8;
@@ -785,7 +752,7 @@ struct GradientShared {
 
 template <typename T, int KP, bool SHARED>
 __global__ void __launch_bounds__(512) gated_delta_gradients_kernel(GatedDeltaArgs a, Places w) {
-    using Shared = GradientShared<T, KP>;
+    using Shared = GradientShared32<T, KP>;
     constexpr int NI = Shared::NI, LB = Shared::LB, ND = Shared::ND, VS = Shared::VS, PV = Shared::kPitchV;
     constexpr int NT = KP / 32;  // tiles of 8 channels a warp
     extern __shared__ __align__(16) unsigned char raw[];
@@ -799,8 +766,8 @@ __global__ void __launch_bounds__(512) gated_delta_gradients_kernel(GatedDeltaAr
     if (s.tokens == 0) return;
     const size_t place = static_cast<size_t>(slot) * a.heads + head;
     const char* const work = static_cast<const char*>(a.workspace);
-    load_source<NI, KP>(source_of<T, KP>(a, w, a.q, 0, slot, k_head, s), smem_addr(sm.q), tid, 512);
-    load_source<NI, KP>(source_of<T, KP>(a, w, a.k, 1, slot, k_head, s), smem_addr(sm.k), tid, 512);
+    load_packed<NI, KP>(packed_at<T, KP>(a, w, 0, slot, k_head), smem_addr(sm.q), tid, 512);
+    load_packed<NI, KP>(packed_at<T, KP>(a, w, 1, slot, k_head), smem_addr(sm.k), tid, 512);
     copies_commit();
     const float* factors = reinterpret_cast<const float*>(work + w.factors) + place * kFactors;
     if (tid < kFactors) sm.factors[tid] = factors[tid];

@@ -30,6 +30,7 @@ constexpr int kTcCompute = 256;          // threads of the computing warps
 constexpr int kTcMovers = 96;            // ... and of those that move rows; between them, a warp that issues
 constexpr int kTcThreads = kTcCompute + 32 + kTcMovers;
 constexpr uint32_t kTcColumns = 512;     // all of tensor memory
+constexpr int kQkPanel = 2 * tc::kPanel; // a panel of q's rows, then of k's
 // Per chunk and head, 64 values each; the chains load the ones that they need, which lie side by side.
 enum TcFactor : int {
     kTailBeta,                           // e^{G_64 - G} beta
@@ -46,7 +47,7 @@ template <typename T, int KP>
 struct TcTiles {
     static constexpr int NI = kInput<T>;
     static constexpr int kOperand = NI * KP * 128;           // bytes of q or k
-    static constexpr int kSquares = 2 * tc::kPanel;          // of L beta or P beta, two pieces
+    static constexpr int kSquares = 2 * tc::kPanel;          // of a 64 x 64 matrix, two pieces
     static constexpr int kStage = 2 * kOperand + 2 * kSquares;
     // columns of tensor memory
     static constexpr uint32_t kX = 0, kO = 64, kD = 128, kS = 128 + KP, kY = 128 + 2 * KP, kU = 192 + 2 * KP;
@@ -57,10 +58,9 @@ template <typename T, int KP>
 struct TcShared {
     using Tiles = TcTiles<T, KP>;
     alignas(1024) unsigned char stage[2][Tiles::kStage];
-    alignas(16) T rows[C * 128];                             // v of a chunk
-    alignas(16) T out[C * 128];                              // o of a chunk
-    alignas(16) float factors[2][3 * C];                     // kTailBeta, kDecay, kScaled
-    alignas(8) unsigned long long full[2], empty[2], ready[5], done[4], rows_full, rows_empty, out_ready, out_free;
+    alignas(16) T out[C * 128];                              // rows of o or dv on their way out
+    alignas(16) float factors[2][5 * C];
+    alignas(8) unsigned long long full[2], empty[2], ready[5], done[4], out_ready, out_free;
     uint32_t base;
 };
 
@@ -71,69 +71,88 @@ struct TcShared {
 
 template <typename T, int KP, bool BACKWARD>
 struct TcPrepareShared {
-    static constexpr int kOperand = TcTiles<T, KP>::kOperand;
     static constexpr int kSquareTiles = BACKWARD ? 6 : 4;
-    static constexpr int kRows = kInput<T> * 2 * tc::kPanel;     // dO: up to 128 columns
-    union {
+    static constexpr int kRowTile = 2 * tc::kPanel;              // 64 tokens by up to 128 columns of v
+    static constexpr int kRowTiles = 1 + (BACKWARD ? kInput<T> : 0);
+    static_assert(kRowTiles * kRowTile <= kSquareTiles * tc::kPanel, "transposed rows fit where L and P go");
+    union {                                                      // one after another
+        alignas(1024) unsigned char qk[2 * TcTiles<T, KP>::kOperand];
+        alignas(1024) unsigned char rows[kRowTiles][kRowTile];   // v, and dO's pieces
         struct {
-            alignas(1024) unsigned char q[kOperand];
-            alignas(1024) unsigned char k[kOperand];
-        } in;
-        struct {
-            alignas(1024) float m[C][C];     // M beta
-            alignas(1024) float unit[C][C];  // M
+            alignas(1024) float m[C][C];                         // M beta
+            alignas(1024) float unit[C][C];                      // M
         } pairs;
     };
-    alignas(1024) unsigned char squares[kSquareTiles][tc::kPanel];
-    alignas(1024) unsigned char rows[BACKWARD ? kRows : 16];
+    union {
+        alignas(1024) unsigned char columns[kRowTiles][kRowTile];
+        alignas(1024) unsigned char squares[kSquareTiles][tc::kPanel];
+    };
     double sum[C];
     alignas(16) float factors[kTcFactors][C];
 };
 
-// Rows of a tensor as swizzled pieces, `width` (64 or 128) columns, zeros behind the last row and column.
-template <typename T>
-CUBF_DEV void load_swizzled(const T* p, size_t row, int rows, int cols, int width, bool wide, unsigned char* tile, int tid,
-                            int threads) {
-    constexpr int NI = kInput<T>;
-    const uint32_t base = smem_addr(tile), piece = static_cast<uint32_t>(width / 64 * tc::kPanel);
+// Rows of a tensor as NI swizzled pieces (one: the 16-bit values themselves), `width` (64 or 128) columns, zeros behind
+// the last row and column.
+template <typename T, int NI>
+CUBF_DEV void load_swizzled(const T* p, size_t row, int rows, int cols, int width, bool wide, unsigned char* tile, int panel,
+                            int tid, int threads) {
+    const uint32_t base = smem_addr(tile), piece = static_cast<uint32_t>(width / 64 * panel);
     const int per = width / 8;
 #pragma unroll 4
     for (int e = tid; e < C * per; e += threads) {
         const int r = e / per, c = e % per * 8;
         const bool ok = r < rows && c < cols;
         if (NI == 1 && wide) {
-            copy16(base + tc::swizzled(r, c), p + (ok ? r * row + c : 0), ok);
+            copy16(base + tc::swizzled(r, c, panel), p + (ok ? r * row + c : 0), ok);
             continue;
         }
-        float x[8];
+        Vec16<T> x;
         if (wide) {
-            Vec16<T> v{};
-            if (ok) v = *reinterpret_cast<const Vec16<T>*>(p + r * row + c);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = widen(v.v[i]);
+            x = ok ? *reinterpret_cast<const Vec16<T>*>(p + r * row + c) : Vec16<T>{};
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = ok && c + i < cols ? widen(p[r * row + c + i]) : 0.f;
+            for (int i = 0; i < 8; ++i) x.v[i] = ok && c + i < cols ? p[r * row + c + i] : Convert<T, float>::store(0.f);
         }
-        uint32_t f[4][NI];
+        if constexpr (NI == 1) {
+            *reinterpret_cast<Vec16<T>*>(tile + tc::swizzled(r, c, panel)) = x;
+        } else {
+            uint32_t f[4][NI];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pieces<NI>(x[2 * i], x[2 * i + 1], f[i]);
+            for (int i = 0; i < 4; ++i) pieces<NI>(widen(x.v[2 * i]), widen(x.v[2 * i + 1]), f[i]);
 #pragma unroll
-        for (int n = 0; n < NI; ++n)
-            *reinterpret_cast<uint4*>(tile + n * piece + tc::swizzled(r, c)) = make_uint4(f[0][n], f[1][n], f[2][n], f[3][n]);
+            for (int n = 0; n < NI; ++n)
+                *reinterpret_cast<uint4*>(tile + n * piece + tc::swizzled(r, c, panel)) =
+                    make_uint4(f[0][n], f[1][n], f[2][n], f[3][n]);
+        }
+    }
+}
+
+// 64 rows of `width` 16-bit values, panels of 64 columns, to `width` rows of 64 (128 bytes), both swizzled.
+CUBF_DEV void transpose_swizzled(const unsigned char* from, unsigned char* to, int width, int warp, int lane) {
+    for (int b = warp; b < width / 8; b += 4) {          // eight columns: two times 32 rows
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            uint32_t r[4];
+            ldsm_t(smem_addr(from) + tc::swizzled(32 * h + lane, 8 * b), r);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {                // rows 32 h + 8 i + 2 (lane % 4), + 1 of column 8 b + lane / 4
+                const int col = 8 * b + lane / 4;
+                *reinterpret_cast<uint32_t*>(to + col * 128 + (((4 * h + i) ^ (col & 7)) << 4) + lane % 4 * 4) = r[i];
+            }
+        }
     }
 }
 
 // ldmatrix of a swizzled tile: the fragments of split::Tile's a_rows and b_rows.
-CUBF_DEV void swizzled_a(uint32_t tile, int m, int k, int lane, uint32_t (&r)[4]) {
-    ldsm(tile + tc::swizzled(m + ((lane >> 3) & 1) * 8 + (lane & 7), k + ((lane >> 4) << 3)), r);
+CUBF_DEV void swizzled_a(uint32_t tile, int m, int k, int panel, int lane, uint32_t (&r)[4]) {
+    ldsm(tile + tc::swizzled(m + ((lane >> 3) & 1) * 8 + (lane & 7), k + ((lane >> 4) << 3), panel), r);
 }
-CUBF_DEV void swizzled_b(uint32_t tile, int n, int k, int lane, uint32_t (&r)[4]) {
-    ldsm(tile + tc::swizzled(n + ((lane >> 4) << 3) + (lane & 7), k + ((lane >> 3) & 1) * 8), r);
+CUBF_DEV void swizzled_b(uint32_t tile, int n, int k, int panel, int lane, uint32_t (&r)[4]) {
+    ldsm(tile + tc::swizzled(n + ((lane >> 4) << 3) + (lane & 7), k + ((lane >> 3) & 1) * 8, panel), r);
 }
 
 template <typename T, int KP, bool BACKWARD>
-__global__ void __launch_bounds__(128) gated_delta_tc_prepare_kernel(GatedDeltaArgs a, Places w, bool wide_q, bool wide_d) {
+__global__ void __launch_bounds__(128) gated_delta_tc_prepare_kernel(GatedDeltaArgs a, Places w, bool wide_q, bool wide_v, bool wide_d) {
     constexpr int NI = kInput<T>, kOperand = TcTiles<T, KP>::kOperand;
     using Shared = TcPrepareShared<T, KP, BACKWARD>;
     extern __shared__ __align__(1024) unsigned char aligned_raw[];
@@ -149,34 +168,33 @@ __global__ void __launch_bounds__(128) gated_delta_tc_prepare_kernel(GatedDeltaA
         return static_cast<const T*>(t.p) + s.row * t.batch + static_cast<size_t>(s.first) * t.token +
                static_cast<size_t>(head) * t.head;
     };
-    load_swizzled<T>(row_of(a.q, k_head), a.q.token, s.tokens, a.k_dim, KP, wide_q, sm.in.q, tid, 128);
-    load_swizzled<T>(row_of(a.k, k_head), a.k.token, s.tokens, a.k_dim, KP, wide_q, sm.in.k, tid, 128);
+    load_swizzled<T, NI>(row_of(a.q, k_head), a.q.token, s.tokens, a.k_dim, KP, wide_q, sm.qk, kQkPanel, tid, 128);
+    load_swizzled<T, NI>(row_of(a.k, k_head), a.k.token, s.tokens, a.k_dim, KP, wide_q, sm.qk + tc::kPanel, kQkPanel, tid, 128);
     copies_commit();
     copies_wait<0>();
     tc::fence_async();
     __syncthreads();
     if (tid == 0) {
-        char* to = work + w.packed + (static_cast<size_t>(slot) * a.k_heads + k_head) * 2 * kOperand;
-        tc::bulk_store(to, smem_addr(sm.in.q), kOperand);
-        tc::bulk_store(to + kOperand, smem_addr(sm.in.k), kOperand);
+        tc::bulk_store(work + w.packed + (static_cast<size_t>(slot) * a.k_heads + k_head) * 2 * kOperand, smem_addr(sm.qk),
+                       2 * kOperand);
         tc::bulk_commit();
     }
     // rows 16 warp .. + 15 of k k^T and q k^T, up to the diagonal
     float kk[8][4] = {}, qk[8][4] = {};
-    const uint32_t tq = smem_addr(sm.in.q), tk = smem_addr(sm.in.k);
+    const uint32_t tq = smem_addr(sm.qk), tk = tq + tc::kPanel;
     for (int ks = 0; ks < KP / 16; ++ks) {
         uint32_t ak[NI][4], aq[NI][4];
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            swizzled_a(tk + i * KP * 128, 16 * warp, 16 * ks, lane, ak[i]);
-            swizzled_a(tq + i * KP * 128, 16 * warp, 16 * ks, lane, aq[i]);
+            swizzled_a(tk + i * KP * 256, 16 * warp, 16 * ks, kQkPanel, lane, ak[i]);
+            swizzled_a(tq + i * KP * 256, 16 * warp, 16 * ks, kQkPanel, lane, aq[i]);
         }
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
             if (t <= warp) {
                 uint32_t b[NI][1][4];
 #pragma unroll
-                for (int i = 0; i < NI; ++i) swizzled_b(tk + i * KP * 128, 16 * t, 16 * ks, lane, b[i][0]);
+                for (int i = 0; i < NI; ++i) swizzled_b(tk + i * KP * 256, 16 * t, 16 * ks, kQkPanel, lane, b[i][0]);
                 products<3, NI, NI, 2>(kk + 2 * t, ak, b);
                 products<3, NI, NI, 2>(qk + 2 * t, aq, b);
             }
@@ -187,11 +205,28 @@ __global__ void __launch_bounds__(128) gated_delta_tc_prepare_kernel(GatedDeltaA
     for (int g = 0; g < group; ++g) {
         const int head = k_head * group + g;
         const size_t place = static_cast<size_t>(slot) * a.heads + head;
-        if (BACKWARD) {
-            const int width = w.v_rows;
-            load_swizzled<T>(row_of(a.d_o, head), a.d_o.token, s.tokens, a.v_dim, width, wide_d, sm.rows, tid, 128);
-            copies_commit();
+        // v, and dO, to a row for each column
+        load_swizzled<T, 1>(row_of(a.v, head), a.v.token, s.tokens, a.v_dim, w.v_rows, wide_v, sm.rows[0], tc::kPanel, tid, 128);
+        if constexpr (BACKWARD)
+            load_swizzled<T, NI>(row_of(a.d_o, head), a.d_o.token, s.tokens, a.v_dim, w.v_rows, wide_d, sm.rows[1], tc::kPanel, tid,
+                                 128);
+        copies_commit();
+        copies_wait<0>();
+        __syncthreads();
+        const uint32_t tile = static_cast<uint32_t>(w.v_rows * 128);
+        transpose_swizzled(sm.rows[0], sm.columns[0], w.v_rows, warp, lane);
+        if (BACKWARD)
+            for (int n = 0; n < NI; ++n)
+                transpose_swizzled(sm.rows[1] + n * tile, sm.columns[1] + n * tile, w.v_rows, warp, lane);
+        tc::fence_async();
+        __syncthreads();
+        if (tid == 0) {
+            tc::bulk_store(work + w.values + place * tile, smem_addr(sm.columns[0]), tile);
+            if (BACKWARD) tc::bulk_store(work + w.rows + place * NI * tile, smem_addr(sm.columns[1]), NI * tile);
+            tc::bulk_commit();
+            tc::bulk_read();
         }
+        __syncthreads();
         double sum = 0;
         float beta = 0.f;
         if (tid < C) {                   // running sums of the log decays, in 64 bits
@@ -285,16 +320,11 @@ __global__ void __launch_bounds__(128) gated_delta_tc_prepare_kernel(GatedDeltaA
                 }
             }
         }
-        if (BACKWARD) copies_wait<0>();
         tc::fence_async();
         __syncthreads();
         if (tid == 0) {
             tc::bulk_store(work + w.solve + place * sizeof(sm.squares), smem_addr(sm.squares), sizeof(sm.squares));
             tc::bulk_store(work + w.factors + place * sizeof(sm.factors), smem_addr(sm.factors), sizeof(sm.factors));
-            if (BACKWARD) {
-                const uint32_t bytes = static_cast<uint32_t>(NI * w.v_rows * 128);
-                tc::bulk_store(work + w.rows + place * bytes, smem_addr(sm.rows), bytes);
-            }
             tc::bulk_commit();
             if (g + 1 < group)
                 tc::bulk_read();
@@ -344,8 +374,6 @@ struct TcChain {
             for (auto& b : sm.done) tc::barrier_init(smem_addr(&b), 1);
             for (auto& b : sm.ready) tc::barrier_init(smem_addr(&b), kTcCompute / 32);
             for (auto& b : sm.empty) tc::barrier_init(smem_addr(&b), kTcCompute / 32 + 1);  // factors read, products done
-            tc::barrier_init(smem_addr(&sm.rows_full), kTcMovers);
-            tc::barrier_init(smem_addr(&sm.rows_empty), kTcCompute / 32);
             tc::barrier_init(smem_addr(&sm.out_ready), kTcCompute / 32);
             tc::barrier_init(smem_addr(&sm.out_free), kTcMovers / 32);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -396,22 +424,24 @@ struct TcChain {
     }
 
     // ---- the issuing warp ----
-    CUBF_DEV void load(int c, int s) const {
+    // A chunk's q and k, `squares` matrices from the `from`-th on, and `factors` rows of factors from `first` on.
+    CUBF_DEV void load(int c, int s, int from, int squares, int first, int factors) const {
         const uint32_t bar = smem_addr(&sm.full[s]), dst = smem_addr(sm.stage[s]);
         const int k_head = chain.head / (a.heads / a.k_heads);
         const size_t tile = static_cast<size_t>(chain.base + c) * a.k_heads + k_head;
         if (tc::elect()) {
-            tc::barrier_expect(bar, Tiles::kStage + sizeof(sm.factors[s]));
+            tc::barrier_expect(bar, 2 * Tiles::kOperand + squares * Tiles::kSquares + factors * C * 4);
             tc::bulk_copy(dst, work(w.packed) + tile * 2 * Tiles::kOperand, 2 * Tiles::kOperand, bar);
-            tc::bulk_copy(dst + 2 * Tiles::kOperand, work(w.solve) + place(c) * 2 * Tiles::kSquares, 2 * Tiles::kSquares, bar);
-            tc::bulk_copy(smem_addr(sm.factors[s]), work(w.factors) + place(c) * kTcFactors * C * 4, sizeof(sm.factors[s]), bar);
+            tc::bulk_copy(dst + 2 * Tiles::kOperand, work(w.solve) + place(c) * w.squares + from * Tiles::kSquares,
+                          squares * Tiles::kSquares, bar);
+            tc::bulk_copy(smem_addr(sm.factors[s]), work(w.factors) + (place(c) * kTcFactors + first) * C * 4, factors * C * 4,
+                          bar);
         }
         __syncwarp();
     }
     CUBF_DEV uint32_t q(int s) const { return smem_addr(sm.stage[s]); }
-    CUBF_DEV uint32_t k(int s) const { return q(s) + Tiles::kOperand; }
-    CUBF_DEV uint32_t solve(int s) const { return q(s) + 2 * Tiles::kOperand; }
-    CUBF_DEV uint32_t attention(int s) const { return solve(s) + Tiles::kSquares; }
+    CUBF_DEV uint32_t k(int s) const { return q(s) + tc::kPanel; }
+    CUBF_DEV uint32_t square(int s, int which) const { return q(s) + 2 * Tiles::kOperand + which * Tiles::kSquares; }
 
     // d (64 columns) = state (pieces in kS) times a tile of q or k, rows along N.
     CUBF_DEV void state_times(uint32_t d, uint32_t tile) const {
@@ -423,7 +453,7 @@ struct TcChain {
 #pragma unroll
                 for (int s = 0; s < KP / 16; ++s)
                     tc::mma(tmem + d, tmem + Tiles::kS + i * (KP / 2) + 8 * s,
-                            tc::rows_along_n(tile + j * KP * 128 + (s / 4) * tc::kPanel + (s % 4) * 32), idesc, i + j + s > 0);
+                            tc::rows_along_n(tile + j * KP * 256 + (s / 4) * kQkPanel + (s % 4) * 32), idesc, i + j + s > 0);
     }
     // d (KP columns) (+)= the pieces at `x` (64 tokens) times a tile of q or k, rows along K.
     CUBF_DEV void onto_state(uint32_t d, uint32_t x, uint32_t tile, bool add) const {
@@ -434,7 +464,7 @@ struct TcChain {
             for (int j = 0; j < NI; ++j)
 #pragma unroll
                 for (int s = 0; s < 4; ++s)
-                    tc::mma(tmem + d, token_column(x, i, s), tc::rows_along_k(tile + j * KP * 128 + s * 2048), idesc,
+                    tc::mma(tmem + d, token_column(x, i, s), tc::rows_along_k(tile + j * KP * 256 + s * 2048, kQkPanel), idesc,
                             add || i + j + s > 0);
     }
     // Where tokens 16 s .. of piece i lie: a thread's half of the tokens stays in columns of its own.
@@ -459,11 +489,28 @@ struct TcChain {
     // What the products report: S k, L Y, k U, P U.
     enum Done { kSk, kLy, kKu, kPu };
 
+    // The other way: sum over j >= i of x_j M_ji, rows along K; `pieces` of x, all with both of M (2) or at level 2 (1).
+    template <int PIECES, bool EXACT>
+    CUBF_DEV void times_transposed(uint32_t d, uint32_t x, uint32_t square) const {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+            for (int j = 0; j < (EXACT ? 2 : 2 - i); ++j)
+#pragma unroll
+                for (int s = 3; s >= 0; --s)
+                    tc::mma(tmem + d, token_column(x, i, s), tc::rows_along_k(square + j * tc::kPanel + s * 2048),
+                            tc::instruction(16 * (s + 1), true), i + j + (3 - s) > 0);
+    }
+
+    template <bool KEEP>
+    CUBF_DEV void load_forward(int c) const {
+        load(c, c & 1, 0, KEEP ? 1 : 2, kTailBeta, KEEP ? 2 : 3);
+    }
     template <bool KEEP>
     CUBF_DEV void issue_forward() {
         const int chunks = chain.chunks;
-        if (chunks > 0) load(0, 0);
-        if (chunks > 1) load(1, 1);
+        if (chunks > 0) load_forward<KEEP>(0);
+        if (chunks > 1) load_forward<KEEP>(1);
         uint32_t phase = 0;
         for (int c = 0; c < chunks && !failed; ++c, phase ^= 1) {
             const int st = c & 1;
@@ -484,14 +531,14 @@ struct TcChain {
             wait(sm.ready[kYReady], phase);
             if (failed) break;
             if (tc::elect()) {
-                times_square(Tiles::kX, Tiles::kY, solve(st));
+                times_square(Tiles::kX, Tiles::kY, square(st, 0));
                 tc::commit(smem_addr(&sm.done[kLy]));
             }
             __syncwarp();
             if (c > 0 && c + 1 < chunks) {       // the stage that the chunk before has left
                 wait(sm.empty[st ^ 1], ((c - 1) >> 1) & 1);
                 if (failed) break;
-                load(c + 1, st ^ 1);
+                load_forward<KEEP>(c + 1);
             }
             wait(sm.ready[kUReady], phase);
             if (failed) break;
@@ -505,7 +552,7 @@ struct TcChain {
                 wait(sm.ready[kOutTaken], phase);
                 if (failed) break;
                 if (tc::elect()) {
-                    times_square(Tiles::kO, Tiles::kY, attention(st));
+                    times_square(Tiles::kO, Tiles::kY, square(st, 1));
                     tc::commit(smem_addr(&sm.done[kPu]));
                     tc::commit(smem_addr(&sm.empty[st]));
                 }
@@ -514,37 +561,54 @@ struct TcChain {
         }
     }
 
+    // The backward's stage: q, k, beta L, P and the factors from kDecay on.
+    CUBF_DEV void issue_backward() {
+        const int chunks = chain.chunks;
+        auto bring = [&](int n) { load(chunks - 1 - n, n & 1, 1, 2, kDecay, 5); };
+        if (chunks > 0) bring(0);
+        if (chunks > 1) bring(1);
+        uint32_t phase = 0;
+        for (int n = 0; n < chunks && !failed; ++n, phase ^= 1) {
+            const int st = n & 1;
+            wait(sm.full[st], (n >> 1) & 1);
+            wait(sm.ready[kStateReady], phase);
+            if (failed) break;
+            if (tc::elect()) {
+                state_times(Tiles::kX, k(st));
+                times_transposed<NI, true>(Tiles::kO, Tiles::kY, square(st, 1));
+                tc::commit(smem_addr(&sm.done[kSk]));
+                onto_state(Tiles::kD, Tiles::kU, q(st), false);
+            }
+            __syncwarp();
+            wait(sm.ready[kYReady], phase);
+            if (failed) break;
+            if (tc::elect()) {
+                times_transposed<2, false>(Tiles::kX, Tiles::kO, square(st, 0));
+                tc::commit(smem_addr(&sm.done[kLy]));
+            }
+            __syncwarp();
+            if (n > 0 && n + 1 < chunks) {
+                wait(sm.empty[st ^ 1], ((n - 1) >> 1) & 1);
+                if (failed) break;
+                bring(n + 1);
+            }
+            wait(sm.ready[kUReady], phase);
+            if (failed) break;
+            if (tc::elect()) {
+                onto_state(Tiles::kD, Tiles::kO, k(st), true);
+                tc::commit(smem_addr(&sm.done[kKu]));
+                tc::commit(smem_addr(&sm.empty[st]));
+            }
+            __syncwarp();
+        }
+    }
+
     // ---- the moving warps ----
     // 16 threads a row of 128 columns, six rows at a time; addresses advance by constants, since these warps share the
-    // schedulers and instruction caches with the computing ones.
-    static constexpr int kSide = kTcMovers / 16, kTurns = (C + kSide - 1) / kSide;
-    CUBF_DEV void load_tile(const HeadTensor& t, int c, bool wide) const {
-        const int n = tokens(c), first = tid - kTcCompute - 32;
-        const T* p = static_cast<const T*>(t.p) + chain.row * t.batch + (static_cast<size_t>(chain.start) + c * C) * t.token +
-                     static_cast<size_t>(chain.head) * t.head;
-        if (wide) {
-            const int row = first / 16, col = first % 16 * 8;
-            const T* q = p + (col < a.v_dim ? row * t.token + col : 0);
-            const size_t step = col < a.v_dim ? kSide * t.token : 0;
-            const uint32_t to = smem_addr(sm.rows + row * 128 + col);
-            const int valid = col < a.v_dim ? n - row : 0;
-#pragma unroll
-            for (int i = 0; i < kTurns; ++i) {
-                const bool ok = kSide * i < valid;
-                if (kSide * i + row < C) copy16(to + i * kSide * 256, ok ? q : p, ok);
-                q += step;
-            }
-        } else {
-            for (int e = first; e < C * 128; e += kTcMovers) {
-                const int r = e / 128, col = e % 128;
-                sm.rows[e] = r < n && col < a.v_dim ? p[r * t.token + col] : Convert<T, float>::store(0.f);
-            }
-        }
-        // arrives when the thread's copies have; its plain stores before are released with it
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&sm.rows_full)) : "memory");
-        __syncwarp();
-    }
+    // schedulers and instruction caches with the computing ones.  Every barrier is one of a ring: none can complete a
+    // second time before its waiter has gone on.
     CUBF_DEV void store_tile(T* out, int c, bool wide) const {
+        constexpr int SIDE = kTcMovers / 16, TURNS = (C + SIDE - 1) / SIDE;
         T* p = out + out_row(c) * a.v_dim;
         const size_t step = static_cast<size_t>(a.heads) * a.v_dim;
         const int n = tokens(c), first = tid - kTcCompute - 32;
@@ -553,9 +617,9 @@ struct TcChain {
             const T* from = sm.out + row * 128 + col;
             T* to = p + row * step + col;
 #pragma unroll
-            for (int i = 0; i < kTurns; ++i) {
-                if (kSide * i < valid) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from + i * kSide * 128);
-                to += kSide * step;
+            for (int i = 0; i < TURNS; ++i) {
+                if (SIDE * i < valid) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from + i * SIDE * 128);
+                to += SIDE * step;
             }
         } else {
             for (int e = first; e < n * 128; e += kTcMovers) {
@@ -563,33 +627,24 @@ struct TcChain {
                 if (col < a.v_dim) p[r * step + col] = sm.out[e];
             }
         }
-        __syncwarp();
-        if (lane == 0) tc::barrier_arrive(smem_addr(&sm.out_free));
+        report(sm.out_free);
     }
-    // Rows come in once those before were read, the output leaves.  Every barrier here is one of a ring: none can complete
-    // a second time before its waiter has gone on.
-    template <bool KEEP>
-    CUBF_DEV void move_forward(bool wide_v, bool wide_o) {
-        const int chunks = chain.chunks;
-        for (int c = 0; c < chunks && !failed; ++c) {
-            if (c > 0) wait(sm.rows_empty, (c - 1) & 1);
-            if (!failed) load_tile(a.v, c, wide_v);
-            if (!KEEP && c > 1) {
-                wait(sm.out_ready, c & 1);
-                if (!failed) store_tile(static_cast<T*>(a.o), c - 2, wide_o);
-            }
+    CUBF_DEV void move_out(T* out, bool reversed, bool wide) {
+        for (int n = 0; n < chain.chunks && !failed; ++n) {
+            wait(sm.out_ready, n & 1);
+            if (!failed) store_tile(out, reversed ? chain.chunks - 1 - n : n, wide);
         }
-        if (!KEEP)
-            for (int c = max(0, chunks - 2); c < chunks && !failed; ++c) {
-                wait(sm.out_ready, c & 1);
-                if (!failed) store_tile(static_cast<T*>(a.o), c, wide_o);
-            }
-        copies_wait<0>();
     }
 
     // ---- the computing warps ----
     // Values go in pairs: y, o and the state are packed fp32 pairs of neighbouring tokens or channels.
     using P = f32x2::P;
+    static CUBF_DEV float2 widen2(uint32_t x) {
+        if constexpr (std::is_same_v<T, __half>)
+            return __half22float2(*reinterpret_cast<const __half2*>(&x));
+        else
+            return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+    }
     static CUBF_DEV void pieces_of(P x, uint32_t& hi, uint32_t& lo) {
         float a, b;
         f32x2::up(x, a, b);
@@ -601,6 +656,36 @@ struct TcChain {
     CUBF_DEV void factors_of(const float* f, int g, P& a, P& b) const {
         const float4 x = *reinterpret_cast<const float4*>(f + 32 * half + 4 * g);
         a = f32x2::pk(x.x, x.y), b = f32x2::pk(x.z, x.w);
+    }
+    // Where the thread's 32 tokens of a transposed tile (v or dO, R or W) lie, 16-byte chunk g of four.
+    CUBF_DEV uint32_t token_chunk(int g) const {
+        return static_cast<uint32_t>(v * 128 + (((4 * half + g) ^ (v & 7)) << 4));
+    }
+    template <int N>
+    CUBF_DEV void fetch(size_t region, int c, uint4 (&r)[N][4]) const {
+        const char* p = work(region) + place(c) * N * w.v_rows * 128;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                r[n][g] = v < w.v_rows ? *reinterpret_cast<const uint4*>(p + n * w.v_rows * 128 + token_chunk(g))
+                                       : make_uint4(0, 0, 0, 0);
+    }
+    static CUBF_DEV uint32_t word(const uint4& x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
+    // Two pieces of 32 tokens kept for the gradients.
+    CUBF_DEV void keep_tokens(size_t region, int c, const P (&y)[16]) const {
+        if (v < w.v_rows) {
+            char* p = work(region) + place(c) * 2 * w.v_rows * 128;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pieces_of(y[4 * g + i], hi[i], lo[i]);
+                *reinterpret_cast<uint4*>(p + token_chunk(g)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(p + w.v_rows * 128 + token_chunk(g)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+        }
+        __syncwarp();
     }
     // 32 columns of tensor memory from `x` on, the thread's half.
     CUBF_DEV void get_tokens(uint32_t x, P (&y)[16]) const {
@@ -640,7 +725,7 @@ struct TcChain {
             const uint32_t column = half * (H / 2) + 16 * n;
             tc::store<16>(at + Tiles::kS + column, hi);
             tc::store<16>(at + Tiles::kS + KP / 2 + column, lo);
-            if (keep && v < w.v_pitch) {
+            if (keep && v < w.v_rows) {
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const uint32_t to = kept(v, half * H + 32 * n + 8 * g);
@@ -704,15 +789,6 @@ struct TcChain {
         __syncwarp();
         if (lane == 0) tc::barrier_arrive(smem_addr(&sm.out_ready));
     }
-    CUBF_DEV void rows_keep(size_t region, int c, const P (&x)[16]) const {
-        if (v < w.v_pitch) {
-            float* p = reinterpret_cast<float*>(work(region)) + (place(c) * C + 32 * half) * w.v_pitch + v;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) f32x2::up(x[i], p[2 * i * w.v_pitch], p[(2 * i + 1) * w.v_pitch]);
-        }
-        __syncwarp();
-    }
-
     // KEEP: the backward's run, which keeps the state before each chunk and R in place of writing o.
     template <bool KEEP>
     CUBF_DEV void compute_forward() {
@@ -730,7 +806,9 @@ struct TcChain {
             if (c > 0) wait(sm.out_free, (c - 1) & 1);
             put_out(o);
         };
+        uint4 rows[1][4];
         if (chunks > 0) {
+            fetch<1>(w.values, 0, rows);
             put_state(s, KEEP ? work(w.states) + place(0) * 2 * w.state_piece : nullptr);
             arrive(sm.ready[kStateReady]);
         }
@@ -740,17 +818,18 @@ struct TcChain {
             // while the state meets k
             if (!KEEP && c > 0) add_out(c - 1);
             wait(sm.full[c & 1], (c >> 1) & 1);
-            wait(sm.rows_full, phase);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                y[i] = f32x2::pk(widen(sm.rows[(32 * half + 2 * i) * 128 + v]), widen(sm.rows[(32 * half + 2 * i + 1) * 128 + v]));
-            report(sm.rows_empty);
+            for (int i = 0; i < 16; ++i) {
+                const float2 two = widen2(word(rows[0][i / 4], i % 4));
+                y[i] = f32x2::pk(two.x, two.y);
+            }
+            if (c + 1 < chunks) fetch<1>(w.values, c + 1, rows);
             wait(sm.done[kSk], phase);
             get_tokens(Tiles::kX, x);
 #pragma unroll
             for (int g = 0; g < 8; ++g) {    // Y = v - e^G (S k)
                 P a, b;
-                factors_of(f + kDecay * C, g, a, b);
+                factors_of(f + (kDecay - kTailBeta) * C, g, a, b);
                 y[2 * g] = f32x2::sub2(y[2 * g], f32x2::mul2(a, x[2 * g]));
                 y[2 * g + 1] = f32x2::sub2(y[2 * g + 1], f32x2::mul2(b, x[2 * g + 1]));
             }
@@ -761,11 +840,11 @@ struct TcChain {
             get_tokens(Tiles::kX, x);
 #pragma unroll
             for (int i = 0; i < 16; ++i) y[i] = f32x2::sub2(y[i], x[i]);  // R = Y - (L beta) Y
-            put_tokens(Tiles::kU, y, f + kTailBeta * C);
+            put_tokens(Tiles::kU, y, f);
             arrive(sm.ready[kUReady]);
             // while U meets k
             if (KEEP) {
-                rows_keep(w.errors, c, y);
+                keep_tokens(w.errors, c, y);
             } else {
                 put_tokens(Tiles::kY, y);
                 get_tokens(Tiles::kO, x);
@@ -773,12 +852,12 @@ struct TcChain {
 #pragma unroll
                 for (int g = 0; g < 8; ++g) {
                     P a, b;
-                    factors_of(f + kScaled * C, g, a, b);
+                    factors_of(f + (kScaled - kTailBeta) * C, g, a, b);
                     o[2 * g] = f32x2::mul2(a, x[2 * g]);
                     o[2 * g + 1] = f32x2::mul2(b, x[2 * g + 1]);
                 }
             }
-            const float whole = f[kDecay * C + C - 1];
+            const float whole = f[(kDecay - kTailBeta) * C + C - 1];
             report(sm.empty[c & 1]);
             wait(sm.done[kKu], phase);
             state_add(whole, s);
@@ -793,6 +872,97 @@ struct TcChain {
             state_out(a.last + state_offset(), s);
         }
     }
+
+    // The sequence from its end: dS, W and dv of every chunk.
+    CUBF_DEV void compute_backward() {
+        P s[H / 2], y[16], x[16], o[16];
+        state_in(a.d_last ? a.d_last + state_offset() : nullptr, s);
+        const int chunks = chain.chunks;
+        uint4 rows[NI][4];
+        auto put_rows = [&] {                // dO, exactly
+#pragma unroll
+            for (int n = 0; n < NI; ++n) {
+                uint32_t r[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) r[i] = word(rows[n][i / 4], i % 4);
+                tc::store<16>(at + Tiles::kY + 32 * half + 16 * n, r);
+            }
+        };
+        auto put_scaled = [&](const float* f) {  // scale e^G dO
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float2 two = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int n = 0; n < NI; ++n) {
+                    const uint32_t r = word(rows[n][i / 4], i % 4);
+                    two.x += __uint_as_float(r << 16);
+                    two.y += __uint_as_float(r & 0xffff0000u);
+                }
+                x[i] = f32x2::pk(two.x, two.y);
+            }
+            put_tokens(Tiles::kU, x, f + (kScaled - kDecay) * C);
+        };
+        auto kept_at = [&](int n) { return work(w.d_states) + place(chunks - 1 - n) * 2 * w.state_piece; };
+        if (chunks > 0) {
+            fetch<NI>(w.rows, chunks - 1, rows);
+            put_state(s, kept_at(0));
+            put_rows();
+            wait(sm.full[0], 0);
+            put_scaled(sm.factors[0]);
+            arrive(sm.ready[kStateReady]);
+        }
+        uint32_t phase = 0;
+        for (int n = 0; n < chunks && !failed; ++n, phase ^= 1) {
+            const int c = chunks - 1 - n;
+            const float* f = sm.factors[n & 1];
+            if (c > 0) fetch<NI>(w.rows, c - 1, rows);
+            wait(sm.full[n & 1], (n >> 1) & 1);
+            wait(sm.done[kSk], phase);
+            get_tokens(Tiles::kX, x);
+            get_tokens(Tiles::kO, y);
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {    // E = e^{G_64 - G} (dS k) + P^T dO
+                P a, b;
+                factors_of(f + (kTail - kDecay) * C, g, a, b);
+                y[2 * g] = f32x2::fma2(a, x[2 * g], y[2 * g]);
+                y[2 * g + 1] = f32x2::fma2(b, x[2 * g + 1], y[2 * g + 1]);
+            }
+            put_tokens(Tiles::kO, y);
+            arrive(sm.ready[kYReady]);
+            wait(sm.done[kLy], phase);
+            get_tokens(Tiles::kX, x);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {   // W = E - (beta L)^T E
+                y[i] = f32x2::sub2(y[i], x[i]);
+                x[i] = f32x2::mul2(y[i], f32x2::pk(-1.f, -1.f));
+            }
+            put_tokens(Tiles::kO, x, f + (kDecayBeta - kDecay) * C);
+            arrive(sm.ready[kUReady]);
+            // while Z meets k
+            keep_tokens(w.d_writes, c, y);
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {    // dv = beta W
+                P a, b;
+                factors_of(f + (kBeta - kDecay) * C, g, a, b);
+                o[2 * g] = f32x2::mul2(a, y[2 * g]);
+                o[2 * g + 1] = f32x2::mul2(b, y[2 * g + 1]);
+            }
+            if (n > 0) wait(sm.out_free, (n - 1) & 1);
+            put_out(o);
+            const float whole = f[C - 1];
+            report(sm.empty[n & 1]);
+            if (c > 0) put_rows();
+            wait(sm.done[kKu], phase);
+            state_add(whole, s);
+            if (c > 0) {
+                put_state(s, kept_at(n + 1));
+                wait(sm.full[(n + 1) & 1], ((n + 1) >> 1) & 1);
+                put_scaled(sm.factors[(n + 1) & 1]);
+                arrive(sm.ready[kStateReady]);
+            }
+        }
+        if (a.d_initial) state_out(a.d_initial + state_offset(), s);
+    }
 };
 
 // 224 registers for a computing thread, 56 for the others: 256 x 224 + 128 x 56 = 384 x 168, what the CTA starts with.
@@ -806,7 +976,7 @@ CUBF_DEV void fewer_registers() {
 }
 
 template <typename T, int KP>
-__global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_forward_kernel(GatedDeltaArgs a, Places w, bool wide_v, bool wide_o) {
+__global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_forward_kernel(GatedDeltaArgs a, Places w, bool wide) {
     extern __shared__ __align__(1024) unsigned char aligned_raw[];
     pdl_begin();
     TcChain<T, KP> run(a, w, *reinterpret_cast<TcShared<T, KP>*>(aligned_raw), chain_of(a, blockIdx.x));
@@ -815,12 +985,503 @@ __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_forward_kernel(G
         if (run.warp == kTcCompute / 32)
             run.template issue_forward<false>();
         else
-            run.template move_forward<false>(wide_v, wide_o);
+            run.move_out(static_cast<T*>(a.o), false, wide);
     } else {
         more_registers<224>();
         run.template compute_forward<false>();
     }
     run.finish();
+}
+
+// Both chains of the backward side by side: neither needs the other's results.
+template <typename T, int KP>
+__global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_chains_kernel(GatedDeltaArgs a, Places w, bool wide) {
+    extern __shared__ __align__(1024) unsigned char aligned_raw[];
+    pdl_begin();
+    TcChain<T, KP> run(a, w, *reinterpret_cast<TcShared<T, KP>*>(aligned_raw), chain_of(a, blockIdx.x / 2));
+    const bool reversed = blockIdx.x % 2 == 0;
+    if (run.warp >= kTcCompute / 32) {
+        fewer_registers<56>();
+        if (run.warp == kTcCompute / 32) {
+            if (reversed)
+                run.issue_backward();
+            else
+                run.template issue_forward<true>();
+        } else if (reversed) {
+            run.move_out(static_cast<T*>(a.d_v), true, wide);
+        }
+    } else {
+        more_registers<224>();
+        if (reversed)
+            run.compute_backward();
+        else
+            run.template compute_forward<true>();
+    }
+    run.finish();
+}
+
+// ---- gradients ----------------------------------------------------------------------------------
+// A CTA per chunk and key head, the heads of its group one after another.  Products have M = 128: two operands of 64
+// tokens on top of one another, q's side (lanes 0 to 63) and k's (64 to 127), so that a thread's lane is a token and
+// the sums along channels and along the pairs' rows are its own:
+//   [q; k] k^T      [dO; W] R^T      [dO; W] S^T      [.; R] dS^T
+// then, with the pairs' coefficients Cq = D o dP and Cm = D o dM written as one tile of 128 rows,
+//   [Cq; Cm] k      and, the tile turned,  [.; Cq^T q + Cm^T k].
+// Bounded by memory: the kept S and dS, 64 KB each, R and W, 32 KB each, and the tiles of q, k and dO per chunk and head.
+constexpr int kGradientThreads = kTcCompute + 32;
+
+template <typename T, int KP>
+struct GradientShared {
+    static constexpr int NI = kInput<T>;
+    static constexpr int kPiece = KP / 64 * 128 * 128;           // of a state
+    static constexpr int kBuffers = NI == 1 ? 2 : 1;             // pieces of states in shared memory
+    static constexpr int kTile = 128 * 128;                      // a piece of dO, R or W (128 columns of v by 64 tokens)
+    alignas(1024) unsigned char qk[2 * TcTiles<T, KP>::kOperand];
+    alignas(1024) unsigned char d_o[NI][kTile];
+    alignas(1024) unsigned char d_write[2][kTile];               // W
+    alignas(1024) unsigned char error[2][kTile];                 // R
+    alignas(1024) unsigned char state[kBuffers][kPiece];
+    alignas(1024) unsigned char pairs[NI == 1 ? 2 : 1][kTile];   // Cq and Cm; with fp16 in place of dO's pieces
+    alignas(16) float factors[kTcFactors][C];
+    float row[2][2][C], kept[2][C], column[4][C], dot[8], beta[C];
+    double d_sum[C], all[2];
+    alignas(8) unsigned long long full, state_full[kBuffers], state_empty[kBuffers], done[4], ready, free;
+    uint32_t base;
+    CUBF_DEV unsigned char* pair_tile(int n) { return NI == 1 ? pairs[n] : d_o[n]; }
+};
+
+// Sums over the warp's lanes of 32 values a thread; lane l keeps that of value l.
+CUBF_DEV float lane_sums(float (&x)[32], int lane) {
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2)
+#pragma unroll
+        for (int i = 0; i < d; ++i) {
+            const bool upper = lane & d;
+            const float send = upper ? x[i] : x[i + d], keep = upper ? x[i + d] : x[i];
+            x[i] = keep + __shfl_xor_sync(0xffffffffu, send, d);
+        }
+    return x[0];
+}
+
+template <typename T, int KP>
+struct Gradients {
+    using Shared = GradientShared<T, KP>;
+    static constexpr int NI = Shared::NI, H = KP / 2, kOperand = TcTiles<T, KP>::kOperand;
+    static constexpr uint32_t kQS = 0, kKU = KP, kPM = 2 * KP, kQK = 2 * KP + 64, kPairs = 2 * KP + 128, kTurned = kPM;
+    enum Done { kPairsDone, kQsDone, kStatesDone, kAllDone };
+
+    const GatedDeltaArgs& a;
+    const Places& w;
+    Shared& sm;
+    const Span s;
+    const int slot, k_head, group;
+    const int tid, lane, warp;
+    uint32_t tmem;
+    bool failed = false;
+
+    template <typename Barrier>
+    CUBF_DEV void wait(Barrier& barrier, uint32_t phase) {
+        failed = failed || !tc::barrier_wait(smem_addr(&barrier), phase);
+        __syncwarp();
+        tc::fence_after();
+    }
+    CUBF_DEV void report(unsigned long long& barrier) const {
+        __syncwarp();
+        if (lane == 0) tc::barrier_arrive(smem_addr(&barrier));
+    }
+    CUBF_DEV char* work(size_t offset) const { return static_cast<char*>(a.workspace) + offset; }
+    CUBF_DEV size_t place(int g) const { return static_cast<size_t>(slot) * a.heads + k_head * group + g; }
+
+    // ---- the issuing warp ----
+    CUBF_DEV void load_state(int g, int n) const {               // n: S, then dS, two pieces each
+        const int b = n % Shared::kBuffers;
+        const uint32_t bytes = static_cast<uint32_t>(w.state_piece);
+        const char* from = work(n < 2 ? w.states : w.d_states) + (place(g) * 2 + n % 2) * w.state_piece;
+        if (tc::elect()) {
+            tc::barrier_expect(smem_addr(&sm.state_full[b]), bytes);
+            tc::bulk_copy(smem_addr(sm.state[b]), from, bytes, smem_addr(&sm.state_full[b]));
+        }
+        __syncwarp();
+    }
+    CUBF_DEV void load_head(int g) const {
+        const uint32_t bar = smem_addr(&sm.full), tile = static_cast<uint32_t>(w.v_rows * 128);
+        if (tc::elect()) {
+            tc::barrier_expect(bar, (g == 0 ? 2 * kOperand : 0) + (NI + 4) * tile + sizeof(sm.factors));
+            if (g == 0)
+                tc::bulk_copy(smem_addr(sm.qk), work(w.packed) + (static_cast<size_t>(slot) * a.k_heads + k_head) * 2 * kOperand,
+                              2 * kOperand, bar);
+#pragma unroll
+            for (int n = 0; n < NI; ++n)
+                tc::bulk_copy(smem_addr(sm.d_o[n]), work(w.rows) + (place(g) * NI + n) * tile, tile, bar);
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                tc::bulk_copy(smem_addr(sm.d_write[n]), work(w.d_writes) + (place(g) * 2 + n) * tile, tile, bar);
+                tc::bulk_copy(smem_addr(sm.error[n]), work(w.errors) + (place(g) * 2 + n) * tile, tile, bar);
+            }
+            tc::bulk_copy(smem_addr(sm.factors), work(w.factors) + place(g) * sizeof(sm.factors), sizeof(sm.factors), bar);
+        }
+        __syncwarp();
+    }
+    // d (N columns) (+)= [upper tile; lower tile] B over v, both tiles and B with columns of v along K.
+    CUBF_DEV void over_v(uint32_t d, uint32_t upper, uint32_t lower, uint32_t b, uint32_t panel, int n, bool add,
+                         bool only_lower) const {
+        const uint32_t idesc = tc::instruction(n, true, true);
+        for (int s = 0; s < w.v_rows / 16; ++s)
+            tc::mma_shared(tmem + d, tc::rows_along_k(upper + s * 2048, lower - upper), tc::rows_along_k(b + s * 2048, panel),
+                           idesc, add || s > 0, only_lower);
+    }
+    // [dO; W] B for a piece of B: with W's other piece (and fp16 dO's) where `both`
+    CUBF_DEV void stacked(uint32_t d, uint32_t b, uint32_t panel, int n, bool add, bool both) const {
+        over_v(d, smem_addr(sm.d_o[0]), smem_addr(sm.d_write[0]), b, panel, n, add, false);
+        if (NI == 2)
+            over_v(d, smem_addr(sm.d_o[1]), smem_addr(sm.d_write[1]), b, panel, n, true, false);
+        else if (both)
+            over_v(d, smem_addr(sm.d_o[0]), smem_addr(sm.d_write[1]), b, panel, n, true, true);
+    }
+    CUBF_DEV void issue() {
+        const uint32_t qk = smem_addr(sm.qk);
+        const uint32_t panel = static_cast<uint32_t>(w.v_rows * 128);
+        for (int g = 0; g < group && !failed; ++g) {
+            const uint32_t phase = g & 1;
+            if (g > 0) wait(sm.free, phase ^ 1);                 // the head before is done with shared memory
+            if (failed) break;
+            load_head(g);
+            auto use = [&](int n) { return static_cast<uint32_t>(g * (4 / Shared::kBuffers) + n / Shared::kBuffers); };
+            auto bring = [&](int n) {
+                if (use(n) > 0) wait(sm.state_empty[n % Shared::kBuffers], (use(n) - 1) & 1);
+                if (!failed) load_state(g, n);
+            };
+            for (int n = 0; n < Shared::kBuffers; ++n) bring(n);
+            wait(sm.full, phase);
+            if (failed) break;
+            if (tc::elect()) {
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NI; ++j)
+#pragma unroll
+                        for (int s = 0; s < KP / 16; ++s) {
+                            const uint32_t step = (s / 4) * kQkPanel + (s % 4) * 32;
+                            tc::mma_shared(tmem + kQK, tc::rows_along_n(qk + i * KP * 256 + step),
+                                           tc::rows_along_n(qk + tc::kPanel + j * KP * 256 + step), tc::instruction(64, false),
+                                           i + j + s > 0);
+                        }
+                stacked(kPM, smem_addr(sm.error[0]), panel, 64, false, true);
+                over_v(kPM, smem_addr(sm.d_o[0]), smem_addr(sm.d_write[0]), smem_addr(sm.error[1]), panel, 64, true, false);
+                tc::commit(smem_addr(&sm.done[kPairsDone]));
+            }
+            __syncwarp();
+            for (int n = 0; n < 4; ++n) {
+                const int b = n % Shared::kBuffers;
+                wait(sm.state_full[b], use(n) & 1);
+                if (failed) break;
+                if (tc::elect()) {
+                    const uint32_t tile = smem_addr(sm.state[b]);
+                    if (n == 0) stacked(kQS, tile, panel, KP, false, true);
+                    if (n == 1) {
+                        if (NI == 2)
+                            stacked(kQS, tile, panel, KP, true, true);
+                        else
+                            over_v(kQS, smem_addr(sm.d_o[0]), smem_addr(sm.d_write[0]), tile, panel, KP, true, false);
+                        tc::commit(smem_addr(&sm.done[kQsDone]));
+                    }
+                    if (n == 2) {
+                        over_v(kKU, smem_addr(sm.d_write[0]), smem_addr(sm.error[0]), tile, panel, KP, false, false);
+                        over_v(kKU, smem_addr(sm.d_write[1]), smem_addr(sm.error[1]), tile, panel, KP, true, false);
+                    }
+                    if (n == 3) {
+                        over_v(kKU, smem_addr(sm.d_write[0]), smem_addr(sm.error[0]), tile, panel, KP, true, false);
+                        tc::commit(smem_addr(&sm.done[kStatesDone]));
+                    }
+                    tc::commit(smem_addr(&sm.state_empty[b]));
+                }
+                __syncwarp();
+                if (n + Shared::kBuffers < 4) bring(n + Shared::kBuffers);
+            }
+            wait(sm.ready, phase);                               // Cq and Cm are written, dP and q k^T read
+            if (failed) break;
+            if (tc::elect()) {
+                constexpr uint32_t idesc = tc::instruction(KP, true), turned = tc::instruction(KP, true, true);
+                const uint32_t c0 = smem_addr(sm.pair_tile(0)), other = qk;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < NI; ++j) {
+                        const uint32_t c = c0 + i * Shared::kTile;
+#pragma unroll
+                        for (int s = 0; s < 4; ++s)
+                            tc::mma_shared(tmem + kPairs, tc::rows_along_n(c + s * 32),
+                                           tc::rows_along_k(qk + tc::kPanel + j * KP * 256 + s * 2048, kQkPanel), idesc,
+                                           i + j + s > 0);
+#pragma unroll
+                        for (int s = 0; s < 8; ++s)              // lanes below 64 hold nothing of use
+                            tc::mma_shared(tmem + kTurned, tc::rows_along_k(other, c + s * 2048 - other),
+                                           tc::rows_along_k(qk + j * KP * 256 + s * 2048, kQkPanel), turned, i + j + s > 0);
+                    }
+                tc::commit(smem_addr(&sm.done[kAllDone]));
+            }
+            __syncwarp();
+        }
+    }
+
+    // ---- the computing warps ----
+    CUBF_DEV void compute() {
+        const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane, i = row & 63;
+        const bool key = quarter >= 2;
+        const uint32_t at = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+        float total[H];
+#pragma unroll
+        for (int n = 0; n < H; ++n) total[n] = 0.f;
+        const size_t gate_row = static_cast<size_t>(s.row) * a.length + s.first;
+        for (int g = 0; g < group; ++g) {
+            const uint32_t phase = g & 1;
+            const int head = k_head * group + g;
+            wait(sm.full, phase);
+            // the pairs' place is dO's with fp16, whose pieces of states come one at a time: those go first
+            if (NI == 2) inner(g);
+            wait(sm.done[kPairsDone], phase);
+            {
+                uint32_t x[32], kk[32];
+                tc::load<32>(at + kPM + 32 * half, x);
+                tc::load<32>(at + kQK + 32 * half, kk);
+                tc::wait_load();
+                const float high = sm.factors[kSumHigh][i], low = sm.factors[kSumLow][i];
+                const float scale = key ? -sm.factors[kBeta][i] : a.scale;
+                if (key && i / 32 == half) {
+                    float d = 0.f;                               // dbeta = W . R of the token itself
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) d = j == i % 32 ? __uint_as_float(x[j]) : d;
+                    sm.beta[i] = d;
+                }
+                float pair[32], c[32], sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    const int at_j = 32 * half + j;
+                    const bool in = key ? at_j < i : at_j <= i;
+                    const float d = (high - sm.factors[kSumHigh][at_j]) + (low - sm.factors[kSumLow][at_j]);
+                    c[j] = in ? expf(d) * scale * sm.factors[kBeta][at_j] * __uint_as_float(x[j]) : 0.f;
+                    pair[j] = in ? c[j] * __uint_as_float(kk[j]) : 0.f;
+                    sum += pair[j];
+                }
+                sm.row[half][key][i] = sum;
+                if (NI == 2) wait(sm.done[kQsDone], phase);      // dO's place is free
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t f[4][2];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) pieces<2>(c[8 * q + 2 * e], c[8 * q + 2 * e + 1], f[e]);
+                    const uint32_t to = row * 128 + (((4 * half + q) ^ (row & 7)) << 4);
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+                        *reinterpret_cast<uint4*>(sm.pair_tile(n) + to) = make_uint4(f[0][n], f[1][n], f[2][n], f[3][n]);
+                }
+                tc::fence_async();
+                tc::fence_before();
+                report(sm.ready);
+                sm.column[quarter][32 * half + lane] = lane_sums(pair, lane);
+            }
+            if (NI == 1) inner(g);               // while the products with the states run
+            // the states' terms, scaled, and their products with q and k
+            wait(sm.done[kStatesDone], phase);
+            float sum = 0.f, kept = 0.f;
+            const float scale = key ? -sm.factors[kDecayBeta][i] : sm.factors[kScaled][i];
+            const float tail = sm.factors[kTailBeta][i];
+#pragma unroll
+            for (int n = 0; n < H / 32; ++n) {
+                const int channel = half * H + 32 * n;
+                uint32_t x[32];
+                float qk[32];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) qk[8 * q + e] = 0.f;
+#pragma unroll
+                    for (int p = 0; p < NI; ++p) {
+                        const uint4 y = *reinterpret_cast<const uint4*>(sm.qk + p * KP * 256 + tc::swizzled(row, channel + 8 * q, kQkPanel));
+                        const uint32_t z[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            qk[8 * q + 2 * e] += __uint_as_float(z[e] << 16);
+                            qk[8 * q + 2 * e + 1] += __uint_as_float(z[e] & 0xffff0000u);
+                        }
+                    }
+                }
+                tc::load<32>(at + kQS + channel, x);
+                tc::wait_load();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    const float y = scale * __uint_as_float(x[e]);
+                    sum = fmaf(y, qk[e], sum);
+                    total[32 * n + e] += y;
+                }
+                if (key) {
+                    tc::load<32>(at + kKU + channel, x);
+                    tc::wait_load();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const float y = tail * __uint_as_float(x[e]);
+                        kept = fmaf(y, qk[e], kept);
+                        total[32 * n + e] += y;
+                    }
+                }
+                __syncwarp();
+            }
+            sm.row[half][key][i] += sum;
+            if (key) sm.kept[half][i] = kept;
+            __syncwarp();
+            wait(sm.done[kAllDone], phase);
+#pragma unroll
+            for (int n = 0; n < H / 32; ++n) {
+                uint32_t x[32];
+                tc::load<32>(at + kPairs + half * H + 32 * n, x);
+                tc::wait_load();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) total[32 * n + e] += __uint_as_float(x[e]);
+                if (key) {
+                    tc::load<32>(at + kTurned + half * H + 32 * n, x);
+                    tc::wait_load();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) total[32 * n + e] += __uint_as_float(x[e]);
+                }
+                __syncwarp();
+            }
+            tc::fence_before();
+            meet();
+            gates(head, gate_row);
+            meet();
+            report(sm.free);
+        }
+        if (i < s.tokens) {
+            T* out = static_cast<T*>(key ? a.d_k : a.d_q) + ((gate_row + i) * a.k_heads + k_head) * a.k_dim;
+            const int first = half * H;
+            const bool wide = a.k_dim % 8 == 0 && (reinterpret_cast<uintptr_t>(key ? a.d_k : a.d_q) & 15u) == 0;
+#pragma unroll
+            for (int n = 0; n < H; n += 8) {
+                Vec16<T> x;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x.v[e] = Convert<T, float>::store(failed ? __int_as_float(0x7fffffff) : total[n + e]);
+                if (wide) {
+                    if (first + n < a.k_dim) *reinterpret_cast<Vec16<T>*>(out + first + n) = x;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (first + n + e < a.k_dim) out[first + n + e] = x.v[e];
+                }
+            }
+        }
+    }
+    // <S, dS> of the warp's share, as the pieces come by.
+    CUBF_DEV void inner(int g) {
+                    float dot = 0.f;
+                    {
+                        constexpr int PER = Shared::kPiece / 16 / kTcCompute;  // 16-byte chunks a thread
+                        const int chunks = static_cast<int>(w.state_piece / 16);
+                        uint4 x[2][PER];
+                        for (int n = 0; n < 4; ++n) {
+                            const int b = n % Shared::kBuffers;
+                            const uint32_t use = g * (4 / Shared::kBuffers) + n / Shared::kBuffers;
+                            wait(sm.state_full[b], use & 1);
+        #pragma unroll
+                            for (int p = 0; p < PER; ++p) {
+                                const int e = tid + p * kTcCompute;
+                                const uint4 y = e < chunks ? *reinterpret_cast<const uint4*>(sm.state[b] + e * 16) : make_uint4(0, 0, 0, 0);
+                                if (n < 2) {
+                                    if (n == 0)
+                                        x[0][p] = y;
+                                    else
+                                        x[1][p] = y;
+                                } else {
+                                    dot += product(x[0][p].x, x[1][p].x, y.x) + product(x[0][p].y, x[1][p].y, y.y) +
+                                           product(x[0][p].z, x[1][p].z, y.z) + product(x[0][p].w, x[1][p].w, y.w);
+                                }
+                            }
+                            report(sm.state_empty[b]);
+                        }
+                    }
+        #pragma unroll
+                    for (int d = 1; d < 32; d *= 2) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+                    if (lane == 0) sm.dot[warp] = dot;
+    }
+    // (x0 + x1) y over a pair of values
+    static CUBF_DEV float product(uint32_t x0, uint32_t x1, uint32_t y) {
+        const float a = __uint_as_float(x0 << 16) + __uint_as_float(x1 << 16);
+        const float b = __uint_as_float(x0 & 0xffff0000u) + __uint_as_float(x1 & 0xffff0000u);
+        return fmaf(a, __uint_as_float(y << 16), b * __uint_as_float(y & 0xffff0000u));
+    }
+    // The computing warps meet; for that they all run through every head, whatever became of a wait.
+    CUBF_DEV void meet() const { asm volatile("bar.sync 1, %0;" ::"n"(kTcCompute) : "memory"); }
+    // dG and its sums from each token on, in 64 bits: the terms of a sequence's first token cancel exactly.
+    CUBF_DEV void gates(int head, size_t gate_row) {
+        if (warp < 2) {
+            const double kept = static_cast<double>(sm.kept[0][tid]) + sm.kept[1][tid];
+            double d = static_cast<double>(sm.row[0][0][tid]) + sm.row[1][0][tid] + sm.row[0][1][tid] + sm.row[1][1][tid] -
+                       kept - (static_cast<double>(sm.column[0][tid]) + sm.column[1][tid] + sm.column[2][tid] + sm.column[3][tid]);
+            double all = kept;
+#pragma unroll
+            for (int n = 1; n < 32; n *= 2) {
+                const double other = __shfl_down_sync(0xffffffffu, d, n);
+                if (lane + n < 32) d += other;
+                all += __shfl_xor_sync(0xffffffffu, all, n);
+            }
+            sm.d_sum[tid] = d;
+            if (lane == 0) sm.all[warp] = all;
+        }
+        meet();
+        if (tid < s.tokens) {
+            double d = sm.d_sum[tid] + (tid < 32 ? sm.d_sum[32] : 0.0);
+            float inner = 0.f;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) inner += sm.dot[n];
+            d += sm.all[0] + sm.all[1] + static_cast<double>(sm.factors[kDecay][C - 1]) * inner;
+            const float d_log = failed ? __int_as_float(0x7fffffff) : static_cast<float>(d);
+            const size_t at = (gate_row + tid) * a.heads + head;
+            if (a.log_decay32)
+                static_cast<float*>(a.d_log_decay)[at] = d_log;
+            else
+                static_cast<T*>(a.d_log_decay)[at] = Convert<T, float>::store(d_log);
+            if (a.beta32)
+                static_cast<float*>(a.d_beta)[at] = sm.beta[tid];
+            else
+                static_cast<T*>(a.d_beta)[at] = Convert<T, float>::store(sm.beta[tid]);
+        }
+    }
+};
+
+template <typename T, int KP>
+__global__ void __launch_bounds__(kGradientThreads, 1) gated_delta_tc_gradients_kernel(GatedDeltaArgs a, Places w) {
+    using Shared = GradientShared<T, KP>;
+    extern __shared__ __align__(1024) unsigned char aligned_raw[];
+    Shared& sm = *reinterpret_cast<Shared*>(aligned_raw);
+    pdl_begin();
+    const int slot = blockIdx.x / a.k_heads, k_head = blockIdx.x % a.k_heads;
+    const Span s = span_of(a, slot);
+    if (s.tokens == 0) return;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    if (tid == 0) {
+        tc::barrier_init(smem_addr(&sm.full), 1);
+        for (auto& b : sm.state_full) tc::barrier_init(smem_addr(&b), 1);
+        for (auto& b : sm.state_empty) tc::barrier_init(smem_addr(&b), kTcCompute / 32 + 1);
+        for (auto& b : sm.done) tc::barrier_init(smem_addr(&b), 1);
+        tc::barrier_init(smem_addr(&sm.ready), kTcCompute / 32);
+        tc::barrier_init(smem_addr(&sm.free), kTcCompute / 32);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kTcCompute / 32) tc::allocate(&sm.base, kTcColumns);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    Gradients<T, KP> run{a, w, sm, s, slot, k_head, a.heads / a.k_heads, tid, tid & 31, warp, __shfl_sync(0xffffffffu, sm.base, 0),
+                         (smem_addr(&sm) & 1023u) != 0};
+    if (warp == kTcCompute / 32)
+        run.issue();
+    else
+        run.compute();
+    tc::fence_before();
+    __syncthreads();
+    if (warp == kTcCompute / 32) {
+        tc::fence_after();
+        tc::release(run.tmem, kTcColumns);
+    }
 }
 
 }  // namespace cubf::delta

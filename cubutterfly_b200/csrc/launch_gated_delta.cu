@@ -28,8 +28,9 @@ namespace {
 using namespace delta;
 using T = std::conditional_t<CUBF_GD_TYPE == 0, __half, std::conditional_t<CUBF_GD_TYPE == 1, __nv_bfloat16, float>>;
 constexpr int KP = CUBF_GD_K;
-// Two chunks' tiles in shared memory where they fit beside one another, else one.
-constexpr int kStages = CUBF_GD_TYPE == 1 || (CUBF_GD_TYPE == 0 && KP == 64) ? 2 : 1;
+
+// 16-bit tensors go through the 5th-generation tensor cores; three pieces of fp32 ones would not fit tensor memory.
+#define CUBF_GD_TENSOR (CUBF_GD_TYPE != 2)
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
@@ -46,19 +47,31 @@ Places places_of(const GatedDeltaArgs& a, bool backward) {
     w.v_pitch = ceil_div(a.v_dim, 16) * 16;
     w.v_rows = ceil_div(a.v_dim, 64) * 64;
     w.state_piece = static_cast<size_t>(KP / 64) * w.v_rows * 128;
-    const bool tensor = sizeof(T) == 2 && !backward;
-    w.pack = tensor || !std::is_same_v<T, __nv_bfloat16> || !rows_aligned(a.q, a.k_dim) || !rows_aligned(a.k, a.k_dim);
-    const size_t chunks = static_cast<size_t>(w.slots) * a.heads;
+    const size_t chunks = static_cast<size_t>(w.slots) * a.heads, key_chunks = static_cast<size_t>(w.slots) * a.k_heads;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    w.factors = take(chunks * (tensor ? kTcFactors * C : kFactors) * 4);
-    w.solve = take(chunks * (tensor ? 4 : kLevel<T>) * kSquare * 2);
-    w.attention = take(tensor ? 0 : chunks * kLevel<T> * kSquare * 2);
-    w.packed = take(w.pack ? static_cast<size_t>(w.slots) * a.k_heads * 2 * kInput<T> * C * KP * 2 : 0);
+#if CUBF_GD_TENSOR
+    w.squares = (backward ? 6 : 4) * tc::kPanel;
+    w.factors = take(chunks * kTcFactors * C * 4);
+    w.solve = take(chunks * w.squares);
+    w.packed = take(key_chunks * 2 * kInput<T> * KP * 128);
+    w.values = take(chunks * w.v_rows * 128);
+    if (backward) {
+        w.rows = take(chunks * kInput<T> * w.v_rows * 128);
+        w.states = take(chunks * 2 * w.state_piece);
+        w.d_states = take(chunks * 2 * w.state_piece);
+        w.errors = take(chunks * 2 * w.v_rows * 128);
+        w.d_writes = take(chunks * 2 * w.v_rows * 128);
+    }
+#else
+    w.factors = take(chunks * kFactors * 4);
+    w.solve = take(chunks * kLevel<T> * kSquare * 2);
+    w.attention = take(chunks * kLevel<T> * kSquare * 2);
+    w.packed = take(key_chunks * 2 * kInput<T> * C * KP * 2);
     if (backward) {
         w.states = take(chunks * w.v_pitch * KP * 4);
         w.d_states = take(chunks * w.v_pitch * KP * 4);
@@ -70,6 +83,7 @@ Places places_of(const GatedDeltaArgs& a, bool backward) {
             w.d_k = take(values * 4);
         }
     }
+#endif
     w.total = at;
     return w;
 }
@@ -84,6 +98,7 @@ cudaError_t launch(KernelSetup& setup, Kernel kernel, size_t grid, int threads, 
     return launch_dependent(kernel, static_cast<unsigned>(grid), static_cast<unsigned>(threads), smem, stream, args...);
 }
 
+#if !CUBF_GD_TENSOR
 cudaError_t launch_chains(const GatedDeltaArgs& a, const Places& w, bool backward, cudaStream_t stream) {
     const int tiles = ceil_div(a.v_dim, 16), chains = sequences_of(a) * a.heads;
     ChainShape shape{};
@@ -101,25 +116,26 @@ cudaError_t launch_chains(const GatedDeltaArgs& a, const Places& w, bool backwar
     if (backward) {
         // set up for the largest CTA, launched with what this one's warps need
         static KernelSetup setup;
-        constexpr int most = kStages * ChainTiles<T, KP>::bytes(8);
+        constexpr int most = ChainTiles<T, KP>::bytes(8);
         int cap = 0;
-        const auto kernel = &gated_delta_chains_kernel<T, KP, kStages>;
+        const auto kernel = &gated_delta_chains_kernel<T, KP>;
         const cudaError_t e = setup_kernel(setup, kernel, 256, most, &cap, true);
         if (e != cudaSuccess) return e;
         if (2 * grid > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
         return launch_dependent(kernel, static_cast<unsigned>(2 * grid), 32u * shape.warps,
-                                kStages * ChainTiles<T, KP>::bytes(shape.warps), stream, a, w, shape);
+                                ChainTiles<T, KP>::bytes(shape.warps), stream, a, w, shape);
     }
     static KernelSetup setup;
-    constexpr int most = kStages * ChainTiles<T, KP>::bytes(8);
+    constexpr int most = ChainTiles<T, KP>::bytes(8);
     int cap = 0;
-    const auto kernel = &gated_delta_forward_kernel<T, KP, kStages>;
+    const auto kernel = &gated_delta_forward_kernel<T, KP>;
     const cudaError_t e = setup_kernel(setup, kernel, 256, most, &cap, true);
     if (e != cudaSuccess) return e;
     if (grid > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
     return launch_dependent(kernel, static_cast<unsigned>(grid), 32u * shape.warps,
-                            kStages * ChainTiles<T, KP>::bytes(shape.warps), stream, a, w, shape);
+                             ChainTiles<T, KP>::bytes(shape.warps), stream, a, w, shape);
 }
+#endif
 
 }  // namespace
 
@@ -132,39 +148,45 @@ template <>
 cudaError_t launch_gated_delta_unit<CUBF_GD_TYPE, CUBF_GD_K>(const GatedDeltaArgs& a, bool backward, cudaStream_t stream) {
     const Places w = places_of(a, backward);
     const size_t chunks = static_cast<size_t>(w.slots) * a.heads;
-    if constexpr (sizeof(T) == 2) {
-        if (!backward) {
-            static KernelSetup prepare, chain;
-            const cudaError_t e = launch(prepare, &gated_delta_tc_prepare_kernel<T, KP, false>,
-                                         static_cast<size_t>(w.slots) * a.k_heads, 128, sizeof(TcPrepareShared<T, KP, false>),
-                                         stream, a, w, rows_aligned(a.q, a.k_dim) && rows_aligned(a.k, a.k_dim), false);
-            if (e != cudaSuccess) return e;
-            return launch(chain, &gated_delta_tc_forward_kernel<T, KP>, static_cast<size_t>(sequences_of(a)) * a.heads,
-                          kTcThreads, sizeof(TcShared<T, KP>), stream, a, w, rows_aligned(a.v, a.v_dim),
-                          rows_aligned(HeadTensor{a.o, 0, 0, static_cast<size_t>(a.v_dim)}, a.v_dim));
-        }
-    }
-    {
-        static KernelSetup setup;
-        const cudaError_t e = launch(setup, &gated_delta_prepare_kernel<T, KP>, chunks, 128, sizeof(PrepareShared<T, KP>),
-                                     stream, a, w);
+#if CUBF_GD_TENSOR
+    const size_t key_chunks = static_cast<size_t>(w.slots) * a.k_heads;
+    const size_t chains = static_cast<size_t>(sequences_of(a)) * a.heads;
+    const bool wide_q = rows_aligned(a.q, a.k_dim) && rows_aligned(a.k, a.k_dim);
+    const HeadTensor out{backward ? a.d_v : a.o, 0, 0, static_cast<size_t>(a.v_dim)};
+    const bool wide_out = rows_aligned(out, a.v_dim);
+    if (!backward) {
+        static KernelSetup prepare, chain;
+        const cudaError_t e = launch(prepare, &gated_delta_tc_prepare_kernel<T, KP, false>, key_chunks, 128,
+                                     sizeof(TcPrepareShared<T, KP, false>), stream, a, w, wide_q, rows_aligned(a.v, a.v_dim), false);
         if (e != cudaSuccess) return e;
+        return launch(chain, &gated_delta_tc_forward_kernel<T, KP>, chains, kTcThreads, sizeof(TcShared<T, KP>), stream, a, w,
+                      wide_out);
     }
-    if (cudaError_t e = launch_chains(a, w, backward, stream); e != cudaSuccess || !backward) return e;
-    constexpr int smem = sizeof(GradientShared<T, KP>);
-    if (a.heads == a.k_heads) {
-        static KernelSetup setup;
-        return launch(setup, &gated_delta_gradients_kernel<T, KP, false>, chunks, 512, smem, stream, a, w);
-    }
-    {
-        static KernelSetup setup;
-        const cudaError_t e = launch(setup, &gated_delta_gradients_kernel<T, KP, true>, chunks, 512, smem, stream, a, w);
-        if (e != cudaSuccess) return e;
-    }
-    static KernelSetup setup;
+    static KernelSetup prepare, chain, gradients;
+    cudaError_t e = launch(prepare, &gated_delta_tc_prepare_kernel<T, KP, true>, key_chunks, 128,
+                           sizeof(TcPrepareShared<T, KP, true>), stream, a, w, wide_q, rows_aligned(a.v, a.v_dim),
+                           rows_aligned(a.d_o, a.v_dim));
+    if (e != cudaSuccess) return e;
+    e = launch(chain, &gated_delta_tc_chains_kernel<T, KP>, 2 * chains, kTcThreads, sizeof(TcShared<T, KP>), stream, a, w,
+               wide_out);
+    if (e != cudaSuccess) return e;
+    return launch(gradients, &gated_delta_tc_gradients_kernel<T, KP>, key_chunks, kGradientThreads,
+                  sizeof(GradientShared<T, KP>), stream, a, w);
+#else
+    static KernelSetup prepare, gradients, shared, share;
+    cudaError_t e = launch(prepare, &gated_delta_prepare_kernel<T, KP>, chunks, 128, sizeof(PrepareShared<T, KP>), stream, a, w);
+    if (e != cudaSuccess) return e;
+    e = launch_chains(a, w, backward, stream);
+    if (e != cudaSuccess || !backward) return e;
+    constexpr int smem = sizeof(GradientShared32<T, KP>);
+    if (a.heads == a.k_heads)
+        return launch(gradients, &gated_delta_gradients_kernel<T, KP, false>, chunks, 512, smem, stream, a, w);
+    e = launch(shared, &gated_delta_gradients_kernel<T, KP, true>, chunks, 512, smem, stream, a, w);
+    if (e != cudaSuccess) return e;
     const size_t values = static_cast<size_t>(a.batch) * a.length * a.k_heads * a.k_dim;
-    return launch(setup, &gated_delta_share_kernel<T>, std::min<size_t>((values + 255) / 256, 148 * 8), 256, 0, stream, a,
-                  w, values);
+    return launch(share, &gated_delta_share_kernel<T>, std::min<size_t>((values + 255) / 256, 148 * 8), 256, 0, stream, a, w,
+                  values);
+#endif
 }
 
 #if CUBF_GD_K == 128

@@ -19,9 +19,9 @@ using split::smem_addr;
 constexpr int kPanel = 8192;             // bytes of 64 x 64 values
 constexpr uint32_t kSpinLimit = 1u << 17;  // tries, of 8 us each where nothing comes: a second
 
-// Byte offset of (row, col) in a tile of panels side by side.
-CUBF_DEV uint32_t swizzled(int row, int col) {
-    return static_cast<uint32_t>((col >> 6) * kPanel + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 7) * 2);
+// Byte offset of (row, col) in a tile of panels `panel` bytes apart.
+CUBF_DEV uint32_t swizzled(int row, int col, int panel = kPanel) {
+    return static_cast<uint32_t>((col >> 6) * panel + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4) + (col & 7) * 2);
 }
 
 // Start, leading and stride byte offsets in 16-byte units, version 1, 128-byte swizzle.
@@ -46,12 +46,13 @@ CUBF_DEV void mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) 
         "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
         : "memory");
 }
-// The same with A in shared memory.
-CUBF_DEV void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// The same with A in shared memory; rows 0 to 63 of D stay as they are with `upper`.
+CUBF_DEV void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add, bool upper = false) {
+    const uint32_t off = upper ? 0xffffffffu : 0u;
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %6, %6}, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add)), "r"(off), "r"(0u)
         : "memory");
 }
 CUBF_DEV void commit(uint32_t barrier) {
