@@ -79,8 +79,9 @@ struct TcPrepareShared {
         alignas(1024) unsigned char qk[2 * TcTiles<T, KP>::kOperand];
         alignas(1024) unsigned char rows[kRowTiles][kRowTile];   // v, and dO's pieces
         struct {
-            alignas(1024) float m[C][C];                         // M beta
-            alignas(1024) float unit[C][C];                      // M
+            alignas(16) float m[C][C + 4];                       // M
+            alignas(16) __nv_bfloat16 scaled[3 * C * kPitchC];   // M beta, three pieces
+            alignas(16) __nv_bfloat16 inverse[3 * C * 24];       // of the 16 x 16 blocks of I + M beta on its diagonal
         } pairs;
     };
     union {
@@ -168,6 +169,11 @@ __global__ void __launch_bounds__(128) gated_delta_tc_prepare_kernel(GatedDeltaA
         return static_cast<const T*>(t.p) + s.row * t.batch + static_cast<size_t>(s.first) * t.token +
                static_cast<size_t>(head) * t.head;
     };
+    if ((wide_v && tid < s.tokens) || (BACKWARD && wide_d && tid >= C && tid - C < s.tokens)) {
+        const HeadTensor& t = tid < C ? a.v : a.d_o;
+        for (int g = 0; g < group; ++g)
+            prefetch_l2(row_of(t, k_head * group + g) + static_cast<size_t>(tid % C) * t.token, static_cast<uint32_t>(a.v_dim * sizeof(T)));
+    }
     load_swizzled<T, NI>(row_of(a.q, k_head), a.q.token, s.tokens, a.k_dim, KP, wide_q, sm.qk, kQkPanel, tid, 128);
     load_swizzled<T, NI>(row_of(a.k, k_head), a.k.token, s.tokens, a.k_dim, KP, wide_q, sm.qk + tc::kPanel, kQkPanel, tid, 128);
     copies_commit();
@@ -261,63 +267,110 @@ __global__ void __launch_bounds__(128) gated_delta_tc_prepare_kernel(GatedDeltaA
         }
         __syncthreads();
         const float *bf = sm.factors[kBeta], *gh = sm.factors[kSumHigh], *gl = sm.factors[kSumLow];
+        // P and M; the blocks above the diagonal are never read
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
+            if (t > 2 * warp + 1) continue;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int i = 16 * warp + lane / 4 + 8 * h, j = 8 * t + lane % 4 * 2;
                 float p[2], m[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float d = j + e <= i ? expf((gh[i] - gh[j + e]) + (gl[i] - gl[j + e])) : 0.f;
+                    const float d = expf((gh[i] - gh[j + e]) + (gl[i] - gl[j + e]));
                     p[e] = j + e <= i ? d * qk[t][2 * h + e] * a.scale : 0.f;
                     m[e] = j + e < i ? d * kk[t][2 * h + e] : 0.f;
                     if (!BACKWARD) p[e] *= bf[j + e];
                 }
-                *reinterpret_cast<float2*>(&sm.pairs.unit[i][j]) = make_float2(m[0], m[1]);
-                *reinterpret_cast<float2*>(&sm.pairs.m[i][j]) = make_float2(m[0] * bf[j], m[1] * bf[j + 1]);
-                uint32_t f[2];
-                pieces<2>(p[0], p[1], f);
+                *reinterpret_cast<float2*>(&sm.pairs.m[i][j]) = make_float2(m[0], m[1]);
+                uint32_t f[3];
+                pieces<3>(m[0] * bf[j], m[1] * bf[j + 1], f);
+#pragma unroll
+                for (int n = 0; n < 3; ++n)
+                    *reinterpret_cast<uint32_t*>(sm.pairs.scaled + (n * C + i) * kPitchC + j) = f[n];
+                uint32_t x[2];
+                pieces<2>(p[0], p[1], x);
                 constexpr int at = BACKWARD ? 4 : 2;
-                *reinterpret_cast<uint32_t*>(sm.squares[at] + tc::swizzled(i, j)) = f[0];
-                *reinterpret_cast<uint32_t*>(sm.squares[at + 1] + tc::swizzled(i, j)) = f[1];
+                *reinterpret_cast<uint32_t*>(sm.squares[at] + tc::swizzled(i, j)) = x[0];
+                *reinterpret_cast<uint32_t*>(sm.squares[at + 1] + tc::swizzled(i, j)) = x[1];
+            }
+        }
+        __syncwarp();
+        {   // the inverse of the warp's block on the diagonal, a lane a column, row by row
+            const int col = lane & 15, base = 16 * warp;
+            float t[16];                 // times beta
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                float acc[4] = {r == col ? 1.f : 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < r; j += 4) {
+                    const float4 m = *reinterpret_cast<const float4*>(&sm.pairs.m[base + r][base + j]);
+                    acc[0] = fmaf(-m.x, t[j], acc[0]);
+                    if (j + 1 < r) acc[1] = fmaf(-m.y, t[j + 1], acc[1]);
+                    if (j + 2 < r) acc[2] = fmaf(-m.z, t[j + 2], acc[2]);
+                    if (j + 3 < r) acc[3] = fmaf(-m.w, t[j + 3], acc[3]);
+                }
+                const float x = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+                t[r] = x * bf[base + r];
+                float rest = x;
+                if (lane < 16)
+#pragma unroll
+                    for (int n = 0; n < 3; ++n) {
+                        const __nv_bfloat16 piece = __float2bfloat16_rn(rest);
+                        rest -= __bfloat162float(piece);
+                        sm.pairs.inverse[(n * C + base + r) * 24 + col] = piece;
+                    }
             }
         }
         __syncthreads();
-        // column tid / 2 of L by forward substitution: l_i = M_i - sum over j < i of (M beta)_ij l_j, every other four
-        // values of j a thread
-        {
-            const int col = tid / 2, part = tid % 2;
-            const float beta_col = bf[col];
-            float l[C / 2] = {};         // the thread's own l_j; what is not known yet meets zeros of M
+        {   // 16 columns of L a warp, transposed, block by block of 16 rows: L_i = (I + M beta)_ii^-1 (M_i - sum over j < i
+            // of (M beta)_ij L_j), products of three pieces
+            const Tile<kPitchC, C * kPitchC> scaled{smem_addr(sm.pairs.scaled)};
+            const Tile<24, C * 24> inverse{smem_addr(sm.pairs.inverse)};
+            uint32_t done[3][3][4];      // rows of L before, negated, as operands
+            const int c0 = 16 * warp + lane / 4;
 #pragma unroll
-            for (int i = 0; i < C; ++i) {
-                float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int step = 0; step < 4; ++step) {
+                const int block = warp + step;
+                if (block > 3) break;
+                float x[2][4];
 #pragma unroll
-                for (int j = 0; j < i; j += 8) {
-                    const float4 m = *reinterpret_cast<const float4*>(&sm.pairs.m[i][j + 4 * part]);
-                    acc[0] = fmaf(-m.x, l[j / 2], acc[0]);
-                    acc[1] = fmaf(-m.y, l[j / 2 + 1], acc[1]);
-                    acc[2] = fmaf(-m.z, l[j / 2 + 2], acc[2]);
-                    acc[3] = fmaf(-m.w, l[j / 2 + 3], acc[3]);
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        x[t][e] = sm.pairs.m[16 * block + 8 * t + lane % 4 * 2 + e % 2][c0 + e / 2 * 8];
+#pragma unroll
+                for (int j = 0; j < step; ++j) {
+                    uint32_t b[3][1][4];
+#pragma unroll
+                    for (int n = 0; n < 3; ++n) scaled.b_rows(n, 16 * block, 16 * (warp + j), lane, b[n][0]);
+                    products<3, 3, 3, 2>(x, done[j], b);
                 }
-                float x = (acc[0] + acc[1]) + (acc[2] + acc[3]);
-                x += __shfl_xor_sync(0xffffffffu, x, 1);
-                x += sm.pairs.unit[i][col];
-                if (i / 4 % 2 == part) l[i / 8 * 4 + i % 4] = x;
-                if (i % 2 == part) {
-                    const float c = x * beta_col;
-                    __nv_bfloat16 hi = __float2bfloat16_rn(c);
-                    const uint32_t to = tc::swizzled(i, col);
-                    *reinterpret_cast<__nv_bfloat16*>(sm.squares[0] + to) = hi;
-                    *reinterpret_cast<__nv_bfloat16*>(sm.squares[1] + to) = __float2bfloat16_rn(c - __bfloat162float(hi));
-                    if (BACKWARD) {
-                        const float r = x * bf[i];
-                        hi = __float2bfloat16_rn(r);
-                        *reinterpret_cast<__nv_bfloat16*>(sm.squares[2] + to) = hi;
-                        *reinterpret_cast<__nv_bfloat16*>(sm.squares[3] + to) = __float2bfloat16_rn(r - __bfloat162float(hi));
+                uint32_t f[3][4], b[3][1][4];
+                operand<3>(x[0], x[1], f);
+#pragma unroll
+                for (int n = 0; n < 3; ++n) inverse.b_rows(n, 16 * block, 0, lane, b[n][0]);
+                float l[2][4] = {};
+                products<3, 3, 3, 2>(l, f, b);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = 16 * block + 8 * t + lane % 4 * 2 + e % 2, col = c0 + e / 2 * 8;
+                        const uint32_t to = tc::swizzled(i, col);
+                        const float c = l[t][e] * bf[col];
+                        __nv_bfloat16 hi = __float2bfloat16_rn(c);
+                        *reinterpret_cast<__nv_bfloat16*>(sm.squares[0] + to) = hi;
+                        *reinterpret_cast<__nv_bfloat16*>(sm.squares[1] + to) = __float2bfloat16_rn(c - __bfloat162float(hi));
+                        if (BACKWARD) {
+                            const float r = l[t][e] * bf[i];
+                            hi = __float2bfloat16_rn(r);
+                            *reinterpret_cast<__nv_bfloat16*>(sm.squares[2] + to) = hi;
+                            *reinterpret_cast<__nv_bfloat16*>(sm.squares[3] + to) = __float2bfloat16_rn(r - __bfloat162float(hi));
+                        }
+                        l[t][e] = -l[t][e];
                     }
-                }
+                if (step < 3) operand<3>(l[0], l[1], done[step]);
             }
         }
         tc::fence_async();
