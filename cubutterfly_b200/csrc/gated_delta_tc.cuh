@@ -80,8 +80,8 @@ struct TcPrepareShared {
         alignas(1024) unsigned char rows[kRowTiles][kRowTile];   // v, and dO's pieces
         struct {
             alignas(16) float m[C][C + 4];                       // M
-            alignas(16) __nv_bfloat16 scaled[3 * C * kPitchC];   // M beta, three pieces
-            alignas(16) __nv_bfloat16 inverse[3 * C * 24];       // of the 16 x 16 blocks of I + M beta on its diagonal
+            alignas(16) __nv_bfloat16 scaled[2 * C * kPitchC];   // M beta, two pieces
+            alignas(16) __nv_bfloat16 inverse[2 * C * 24];       // of the 16 x 16 blocks of I + M beta on its diagonal
         } pairs;
     };
     union {
@@ -98,10 +98,10 @@ template <typename T, int NI>
 CUBF_DEV void load_swizzled(const T* p, size_t row, int rows, int cols, int width, bool wide, unsigned char* tile, int panel,
                             int tid, int threads) {
     const uint32_t base = smem_addr(tile), piece = static_cast<uint32_t>(width / 64 * panel);
-    const int per = width / 8;
+    const int shift = width == 128 ? 4 : 3;          // vectors of eight a row
 #pragma unroll 4
-    for (int e = tid; e < C * per; e += threads) {
-        const int r = e / per, c = e % per * 8;
+    for (int e = tid; e < C << shift; e += threads) {
+        const int r = e >> shift, c = (e & ((1 << shift) - 1)) * 8;
         const bool ok = r < rows && c < cols;
         if (NI == 1 && wide) {
             copy16(base + tc::swizzled(r, c, panel), p + (ok ? r * row + c : 0), ok);
@@ -153,7 +153,7 @@ CUBF_DEV void swizzled_b(uint32_t tile, int n, int k, int panel, int lane, uint3
 }
 
 template <typename T, int KP, bool BACKWARD>
-__global__ void __launch_bounds__(128) gated_delta_tc_prepare_kernel(GatedDeltaArgs a, Places w, bool wide_q, bool wide_v, bool wide_d) {
+__global__ void __launch_bounds__(128, BACKWARD ? 2 : 3) gated_delta_tc_prepare_kernel(GatedDeltaArgs a, Places w, bool wide_q, bool wide_v, bool wide_d) {
     constexpr int NI = kInput<T>, kOperand = TcTiles<T, KP>::kOperand;
     using Shared = TcPrepareShared<T, KP, BACKWARD>;
     extern __shared__ __align__(1024) unsigned char aligned_raw[];
@@ -174,6 +174,17 @@ __global__ void __launch_bounds__(128) gated_delta_tc_prepare_kernel(GatedDeltaA
         for (int g = 0; g < group; ++g)
             prefetch_l2(row_of(t, k_head * group + g) + static_cast<size_t>(tid % C) * t.token, static_cast<uint32_t>(a.v_dim * sizeof(T)));
     }
+    auto gates = [&](int head, float& log_decay, float& beta) {  // of token `tid`
+        log_decay = beta = 0.f;
+        if (tid < s.tokens) {
+            const size_t token = static_cast<size_t>(s.first) + tid;
+            log_decay = gate_at(a.log_decay, a.log_decay32,
+                                s.row * a.log_decay.batch + token * a.log_decay.token + head * a.log_decay.head, kTypeId<T>);
+            beta = gate_at(a.beta, a.beta32, s.row * a.beta.batch + token * a.beta.token + head * a.beta.head, kTypeId<T>);
+        }
+    };
+    float log_decay, beta;
+    gates(k_head * group, log_decay, beta);
     load_swizzled<T, NI>(row_of(a.q, k_head), a.q.token, s.tokens, a.k_dim, KP, wide_q, sm.qk, kQkPanel, tid, 128);
     load_swizzled<T, NI>(row_of(a.k, k_head), a.k.token, s.tokens, a.k_dim, KP, wide_q, sm.qk + tc::kPanel, kQkPanel, tid, 128);
     copies_commit();
@@ -234,16 +245,8 @@ __global__ void __launch_bounds__(128) gated_delta_tc_prepare_kernel(GatedDeltaA
         }
         __syncthreads();
         double sum = 0;
-        float beta = 0.f;
         if (tid < C) {                   // running sums of the log decays, in 64 bits
-            if (tid < s.tokens) {
-                const size_t token = static_cast<size_t>(s.first) + tid;
-                const float d = gate_at(a.log_decay, a.log_decay32,
-                                        s.row * a.log_decay.batch + token * a.log_decay.token + head * a.log_decay.head,
-                                        kTypeId<T>);
-                sum = d < kLeast ? kLeast : d;  // NaN stays
-                beta = gate_at(a.beta, a.beta32, s.row * a.beta.batch + token * a.beta.token + head * a.beta.head, kTypeId<T>);
-            }
+            sum = log_decay < kLeast ? kLeast : log_decay;  // NaN stays
 #pragma unroll
             for (int d = 1; d < 32; d *= 2) {
                 const double other = __shfl_up_sync(0xffffffffu, sum, d);
@@ -264,6 +267,7 @@ __global__ void __launch_bounds__(128) gated_delta_tc_prepare_kernel(GatedDeltaA
             sm.factors[kDecayBeta][tid] = from_start * beta;
             sm.factors[kSumHigh][tid] = high;
             sm.factors[kSumLow][tid] = static_cast<float>(sum - high);
+            if (g + 1 < group) gates(head + 1, log_decay, beta);
         }
         __syncthreads();
         const float *bf = sm.factors[kBeta], *gh = sm.factors[kSumHigh], *gl = sm.factors[kSumLow];
@@ -283,10 +287,10 @@ __global__ void __launch_bounds__(128) gated_delta_tc_prepare_kernel(GatedDeltaA
                     if (!BACKWARD) p[e] *= bf[j + e];
                 }
                 *reinterpret_cast<float2*>(&sm.pairs.m[i][j]) = make_float2(m[0], m[1]);
-                uint32_t f[3];
-                pieces<3>(m[0] * bf[j], m[1] * bf[j + 1], f);
+                uint32_t f[2];
+                pieces<2>(m[0] * bf[j], m[1] * bf[j + 1], f);
 #pragma unroll
-                for (int n = 0; n < 3; ++n)
+                for (int n = 0; n < 2; ++n)
                     *reinterpret_cast<uint32_t*>(sm.pairs.scaled + (n * C + i) * kPitchC + j) = f[n];
                 uint32_t x[2];
                 pieces<2>(p[0], p[1], x);
@@ -315,7 +319,7 @@ __global__ void __launch_bounds__(128) gated_delta_tc_prepare_kernel(GatedDeltaA
                 float rest = x;
                 if (lane < 16)
 #pragma unroll
-                    for (int n = 0; n < 3; ++n) {
+                    for (int n = 0; n < 2; ++n) {
                         const __nv_bfloat16 piece = __float2bfloat16_rn(rest);
                         rest -= __bfloat162float(piece);
                         sm.pairs.inverse[(n * C + base + r) * 24 + col] = piece;
@@ -324,10 +328,10 @@ __global__ void __launch_bounds__(128) gated_delta_tc_prepare_kernel(GatedDeltaA
         }
         __syncthreads();
         {   // 16 columns of L a warp, transposed, block by block of 16 rows: L_i = (I + M beta)_ii^-1 (M_i - sum over j < i
-            // of (M beta)_ij L_j), products of three pieces
+            // of (M beta)_ij L_j), products at level 2
             const Tile<kPitchC, C * kPitchC> scaled{smem_addr(sm.pairs.scaled)};
             const Tile<24, C * 24> inverse{smem_addr(sm.pairs.inverse)};
-            uint32_t done[3][3][4];      // rows of L before, negated, as operands
+            uint32_t done[3][2][4];      // rows of L before, negated, as operands
             const int c0 = 16 * warp + lane / 4;
 #pragma unroll
             for (int step = 0; step < 4; ++step) {
@@ -341,17 +345,17 @@ __global__ void __launch_bounds__(128) gated_delta_tc_prepare_kernel(GatedDeltaA
                         x[t][e] = sm.pairs.m[16 * block + 8 * t + lane % 4 * 2 + e % 2][c0 + e / 2 * 8];
 #pragma unroll
                 for (int j = 0; j < step; ++j) {
-                    uint32_t b[3][1][4];
+                    uint32_t b[2][1][4];
 #pragma unroll
-                    for (int n = 0; n < 3; ++n) scaled.b_rows(n, 16 * block, 16 * (warp + j), lane, b[n][0]);
-                    products<3, 3, 3, 2>(x, done[j], b);
+                    for (int n = 0; n < 2; ++n) scaled.b_rows(n, 16 * block, 16 * (warp + j), lane, b[n][0]);
+                    products<2, 2, 2, 2>(x, done[j], b);
                 }
-                uint32_t f[3][4], b[3][1][4];
-                operand<3>(x[0], x[1], f);
+                uint32_t f[2][4], b[2][1][4];
+                operand<2>(x[0], x[1], f);
 #pragma unroll
-                for (int n = 0; n < 3; ++n) inverse.b_rows(n, 16 * block, 0, lane, b[n][0]);
+                for (int n = 0; n < 2; ++n) inverse.b_rows(n, 16 * block, 0, lane, b[n][0]);
                 float l[2][4] = {};
-                products<3, 3, 3, 2>(l, f, b);
+                products<2, 2, 2, 2>(l, f, b);
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -370,7 +374,7 @@ __global__ void __launch_bounds__(128) gated_delta_tc_prepare_kernel(GatedDeltaA
                         }
                         l[t][e] = -l[t][e];
                     }
-                if (step < 3) operand<3>(l[0], l[1], done[step]);
+                if (step < 3) operand<2>(l[0], l[1], done[step]);
             }
         }
         tc::fence_async();
