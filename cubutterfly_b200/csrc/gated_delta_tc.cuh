@@ -88,7 +88,6 @@ struct TcPrepareShared {
         alignas(1024) unsigned char columns[kRowTiles][kRowTile];
         alignas(1024) unsigned char squares[kSquareTiles][tc::kPanel];
     };
-    double sum[C];
     alignas(16) float factors[kTcFactors][C];
 };
 
@@ -244,6 +243,7 @@ __global__ void __launch_bounds__(128, BACKWARD ? 2 : 3) gated_delta_tc_prepare_
             tc::bulk_read();
         }
         __syncthreads();
+        double* const ends = reinterpret_cast<double*>(sm.pairs.inverse);  // of the two warps' sums
         double sum = 0;
         if (tid < C) {                   // running sums of the log decays, in 64 bits
             sum = log_decay < kLeast ? kLeast : log_decay;  // NaN stays
@@ -252,12 +252,12 @@ __global__ void __launch_bounds__(128, BACKWARD ? 2 : 3) gated_delta_tc_prepare_
                 const double other = __shfl_up_sync(0xffffffffu, sum, d);
                 if (lane >= d) sum += other;
             }
-            sm.sum[tid] = sum;
+            if (lane == 31) ends[warp] = sum;
         }
         __syncthreads();
         if (tid < C) {
-            if (warp == 1) sum += sm.sum[31];
-            const double all = sm.sum[31] + sm.sum[63];
+            if (warp == 1) sum += ends[0];
+            const double all = ends[0] + ends[1];
             const float high = static_cast<float>(sum), from_start = expf(high), to_end = expf(static_cast<float>(all - sum));
             sm.factors[kTailBeta][tid] = to_end * beta;
             sm.factors[kDecay][tid] = from_start;

@@ -29,9 +29,12 @@ bool vectors(const QkNormArgs& a, bool backward) {
     return bits % 16 == 0;
 }
 
-template <typename T, int NP, bool VEC>
-cudaError_t launch_forward(const QkNormArgs& a, cudaStream_t stream) {
-    // all heads of a token a warp, fewer while that leaves SMs without one of their 32 warps
+template <typename T, int NP, bool VEC, bool WEIGHTED, bool TURNED>
+cudaError_t launch_kernel(const QkNormArgs& a, bool backward, cudaStream_t stream) {
+    if (backward)
+        return launch_dependent(&qk_norm_backward_kernel<T, NP, VEC, WEIGHTED, TURNED>, static_cast<unsigned>(a.parts),
+                                32u * kWarps, 0, stream, a);
+    // all heads of a token a warp, fewer while that leaves an SM less than two turns of its 32 warps
     const size_t tokens = a.batch * a.tokens;
     const int heads = a.q_heads + a.k_heads;
     int lanes = 1;
@@ -39,23 +42,29 @@ cudaError_t launch_forward(const QkNormArgs& a, cudaStream_t stream) {
     while (lanes * NP < pairs) lanes *= 2;
     const int turn = 32 / lanes;                 // heads that a warp takes side by side
     int unit = (heads + turn - 1) / turn * turn;
-    while (unit > turn && tokens * ((heads + unit - 1) / unit) < 148 * 32) unit = (unit / turn + 1) / 2 * turn;
+    while (unit > turn && tokens * ((heads + unit - 1) / unit) < 148 * 64) unit = (unit / turn + 1) / 2 * turn;
     const int per_token = (heads + unit - 1) / unit;
-    const size_t units = tokens * per_token;
-    const size_t grid = std::min<size_t>((units + kWarps - 1) / kWarps, 0x7fffffffULL);
-    return launch_dependent(&qk_norm_kernel<T, NP, VEC>, static_cast<unsigned>(grid), 32u * kWarps, 0, stream, a, unit,
-                            per_token);
+    // CTAs that stay, since each lays out weights and frequencies first
+    const size_t grid = std::min<size_t>((tokens * per_token + kWarps - 1) / kWarps, 148 * 8);
+    return launch_dependent(&qk_norm_kernel<T, NP, VEC, WEIGHTED, TURNED>, static_cast<unsigned>(grid), 32u * kWarps, 0, stream,
+                            a, unit, per_token);
+}
+
+template <typename T, int NP, bool VEC>
+cudaError_t launch_options(const QkNormArgs& a, bool backward, cudaStream_t stream) {
+    if (a.q_weight || a.k_weight)
+        return a.positions ? launch_kernel<T, NP, VEC, true, true>(a, backward, stream)
+                           : launch_kernel<T, NP, VEC, true, false>(a, backward, stream);
+    return a.positions ? launch_kernel<T, NP, VEC, false, true>(a, backward, stream)
+                       : launch_kernel<T, NP, VEC, false, false>(a, backward, stream);
 }
 
 template <typename T>
 cudaError_t launch(QkNormArgs a, bool backward, cudaStream_t stream) {
-    constexpr int N = 16 / sizeof(T);
     if (a.rotary == 0) a.interleaved = true;     // any pairs do: adjacent ones are read in the widest pieces
-    const bool wide = vectors<T>(a, backward);
-    if (!backward) return wide ? launch_forward<T, N, true>(a, stream) : launch_forward<T, 4, false>(a, stream);
-    const auto kernel = wide ? &qk_norm_backward_kernel<T, N, true> : &qk_norm_backward_kernel<T, 4, false>;
-    const cudaError_t e = launch_dependent(kernel, static_cast<unsigned>(a.parts), 32u * kWarps, 0, stream, a);
-    if (e != cudaSuccess || (!a.q_weight && !a.k_weight)) return e;
+    const cudaError_t e = vectors<T>(a, backward) ? launch_options<T, 16 / sizeof(T), true>(a, backward, stream)
+                                                  : launch_options<T, 4, false>(a, backward, stream);
+    if (e != cudaSuccess || !backward || (!a.q_weight && !a.k_weight)) return e;
     return launch_dependent(&qk_norm_weights_kernel<T>, static_cast<unsigned>((2 * a.dim + 31) / 32), 32u * kWarps, 0,
                             stream, a);
 }
