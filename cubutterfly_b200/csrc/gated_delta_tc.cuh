@@ -39,7 +39,7 @@ enum TcFactor : int {
     kTail,                               // e^{G_64 - G}
     kBeta,
     kDecayBeta,                          // e^G beta
-    kSumHigh, kSumLow,                   // G as a sum of two floats
+    kSumHigh, kSumLow,                   // G / log 2 as a sum of two floats
     kTcFactors
 };
 
@@ -127,7 +127,8 @@ CUBF_DEV void load_swizzled(const T* p, size_t row, int rows, int cols, int widt
     }
 }
 
-// 64 rows of `width` 16-bit values, panels of 64 columns, to `width` rows of 64 (128 bytes), both swizzled.
+// 64 swizzled rows of `width` 16-bit values, panels of 64 columns, to chunks of eight rows with a place of 16 bytes for each
+// column (tcgen05.cuh).
 CUBF_DEV void transpose_swizzled(const unsigned char* from, unsigned char* to, int width, int warp, int lane) {
     for (int b = warp; b < width / 8; b += 4) {          // eight columns: two times 32 rows
 #pragma unroll
@@ -137,7 +138,7 @@ CUBF_DEV void transpose_swizzled(const unsigned char* from, unsigned char* to, i
 #pragma unroll
             for (int i = 0; i < 4; ++i) {                // rows 32 h + 8 i + 2 (lane % 4), + 1 of column 8 b + lane / 4
                 const int col = 8 * b + lane / 4;
-                *reinterpret_cast<uint32_t*>(to + col * 128 + (((4 * h + i) ^ (col & 7)) << 4) + lane % 4 * 4) = r[i];
+                *reinterpret_cast<uint32_t*>(to + ((4 * h + i) * width + col) * 16 + lane % 4 * 4) = r[i];
             }
         }
     }
@@ -258,7 +259,9 @@ __global__ void __launch_bounds__(128, BACKWARD ? 2 : 3) gated_delta_tc_prepare_
         if (tid < C) {
             if (warp == 1) sum += ends[0];
             const double all = ends[0] + ends[1];
-            const float high = static_cast<float>(sum), from_start = expf(high), to_end = expf(static_cast<float>(all - sum));
+            const double log2 = sum * 1.4426950408889634074;
+            const float high = static_cast<float>(log2);
+            const float from_start = expf(static_cast<float>(sum)), to_end = expf(static_cast<float>(all - sum));
             sm.factors[kTailBeta][tid] = to_end * beta;
             sm.factors[kDecay][tid] = from_start;
             sm.factors[kScaled][tid] = from_start * a.scale;
@@ -266,7 +269,7 @@ __global__ void __launch_bounds__(128, BACKWARD ? 2 : 3) gated_delta_tc_prepare_
             sm.factors[kBeta][tid] = beta;
             sm.factors[kDecayBeta][tid] = from_start * beta;
             sm.factors[kSumHigh][tid] = high;
-            sm.factors[kSumLow][tid] = static_cast<float>(sum - high);
+            sm.factors[kSumLow][tid] = static_cast<float>(log2 - high);
             if (g + 1 < group) gates(head + 1, log_decay, beta);
         }
         __syncthreads();
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(128, BACKWARD ? 2 : 3) gated_delta_tc_prepare_
                 float p[2], m[2];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const float d = expf((gh[i] - gh[j + e]) + (gl[i] - gl[j + e]));
+                    const float d = exp2f((gh[i] - gh[j + e]) + (gl[i] - gl[j + e]));
                     p[e] = j + e <= i ? d * qk[t][2 * h + e] * a.scale : 0.f;
                     m[e] = j + e < i ? d * kk[t][2 * h + e] : 0.f;
                     if (!BACKWARD) p[e] *= bf[j + e];
@@ -716,7 +719,7 @@ struct TcChain {
     }
     // Where the thread's 32 tokens of a transposed tile (v or dO, R or W) lie, 16-byte chunk g of four.
     CUBF_DEV uint32_t token_chunk(int g) const {
-        return static_cast<uint32_t>(v * 128 + (((4 * half + g) ^ (v & 7)) << 4));
+        return static_cast<uint32_t>(((4 * half + g) * w.v_rows + v) * 16);
     }
     template <int N>
     CUBF_DEV void fetch(size_t region, int c, uint4 (&r)[N][4]) const {
@@ -794,10 +797,8 @@ struct TcChain {
             __syncwarp();
         }
     }
-    // Byte of (column of v, channel) in a kept state's piece: panels of 64 channels, a row for each column of v.
-    CUBF_DEV uint32_t kept(int row, int col) const {
-        return static_cast<uint32_t>((col >> 6) * (w.v_rows * 128) + row * 128 + ((((col & 63) >> 3) ^ (row & 7)) << 4));
-    }
+    // Byte of (column of v, channel) in a kept state's piece: chunks of eight channels.
+    CUBF_DEV uint32_t kept(int row, int col) const { return static_cast<uint32_t>(((col >> 3) * w.v_rows + row) * 16); }
     CUBF_DEV void state_in(const float* p, P (&s)[H / 2]) const {
 #pragma unroll
         for (int i = 0; i < H / 2; ++i) {
@@ -1050,7 +1051,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_forward_kernel(G
     run.finish();
 }
 
-// Both chains of the backward side by side: neither needs the other's results.
+// Both chains of the backward side by side: neither needs the other's results.  (One kind after the other is no faster for
+// training's 128 + 128 chains on 148 SMs, 420 us against 433, and slower for packed sequences, 587 against 350.)
 template <typename T, int KP>
 __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_chains_kernel(GatedDeltaArgs a, Places w, bool wide) {
     extern __shared__ __align__(1024) unsigned char aligned_raw[];
@@ -1094,17 +1096,17 @@ struct GradientShared {
     static constexpr int kBuffers = NI == 1 ? 2 : 1;             // pieces of states in shared memory
     static constexpr int kTile = 128 * 128;                      // a piece of dO, R or W (128 columns of v by 64 tokens)
     alignas(1024) unsigned char qk[2 * TcTiles<T, KP>::kOperand];
-    alignas(1024) unsigned char d_o[NI][kTile];
-    alignas(1024) unsigned char d_write[2][kTile];               // W
-    alignas(1024) unsigned char error[2][kTile];                 // R
+    // dO, W, R and then the second pieces of (fp16) dO, W, R, one after another: two neighbours are one operand
+    alignas(1024) unsigned char tiles[4 + NI][kTile];
     alignas(1024) unsigned char state[kBuffers][kPiece];
-    alignas(1024) unsigned char pairs[NI == 1 ? 2 : 1][kTile];   // Cq and Cm; with fp16 in place of dO's pieces
+    alignas(1024) unsigned char pairs[NI == 1 ? 2 : 1][NI == 1 ? kTile : 16];  // pieces of Cq and Cm
     alignas(16) float factors[kTcFactors][C];
     float row[2][2][C], kept[2][C], column[4][C], dot[8], beta[C];
     double d_sum[C], all[2];
     alignas(8) unsigned long long full, state_full[kBuffers], state_empty[kBuffers], done[4], ready, free;
     uint32_t base;
-    CUBF_DEV unsigned char* pair_tile(int n) { return NI == 1 ? pairs[n] : d_o[n]; }
+    // With fp16 the pairs take dO's place, or with few columns of v the end of the tiles, which those do not reach.
+    CUBF_DEV unsigned char* pair_tile(int n, int v_rows) { return NI == 1 ? pairs[n] : v_rows == 128 ? tiles[3 * n] : tiles[4 + n]; }
 };
 
 // Sums over the warp's lanes of 32 values a thread; lane l keeps that of value l.
@@ -1168,36 +1170,34 @@ struct Gradients {
                 tc::bulk_copy(smem_addr(sm.qk), work(w.packed) + (static_cast<size_t>(slot) * a.k_heads + k_head) * 2 * kOperand,
                               2 * kOperand, bar);
 #pragma unroll
-            for (int n = 0; n < NI; ++n)
-                tc::bulk_copy(smem_addr(sm.d_o[n]), work(w.rows) + (place(g) * NI + n) * tile, tile, bar);
-#pragma unroll
             for (int n = 0; n < 2; ++n) {
-                tc::bulk_copy(smem_addr(sm.d_write[n]), work(w.d_writes) + (place(g) * 2 + n) * tile, tile, bar);
-                tc::bulk_copy(smem_addr(sm.error[n]), work(w.errors) + (place(g) * 2 + n) * tile, tile, bar);
+                if (n < NI) tc::bulk_copy(stack(n), work(w.rows) + (place(g) * NI + n) * tile, tile, bar);
+                tc::bulk_copy(stack(n) + tile, work(w.d_writes) + (place(g) * 2 + n) * tile, tile, bar);
+                tc::bulk_copy(stack(n) + 2 * tile, work(w.errors) + (place(g) * 2 + n) * tile, tile, bar);
             }
             tc::bulk_copy(smem_addr(sm.factors), work(w.factors) + place(g) * sizeof(sm.factors), sizeof(sm.factors), bar);
         }
         __syncwarp();
     }
-    // d (N columns) (+)= [upper tile; lower tile] B over v, both tiles and B with columns of v along K.
-    CUBF_DEV void over_v(uint32_t d, uint32_t upper, uint32_t lower, uint32_t b, uint32_t panel, int n, bool add,
-                         bool only_lower) const {
-        const uint32_t idesc = tc::instruction(n, true, true);
-        for (int s = 0; s < w.v_rows / 16; ++s)
-            tc::mma_shared(tmem + d, tc::rows_along_k(upper + s * 2048, lower - upper), tc::rows_along_k(b + s * 2048, panel),
-                           idesc, add || s > 0, only_lower);
+    // Where piece n of [dO; W; R] begins; with bf16 dO has one piece, and what lies before W's second is not of use.
+    CUBF_DEV uint32_t stack(int n) const {
+        return smem_addr(sm.tiles) + static_cast<uint32_t>(n * (NI + 1) * w.v_rows * 128);
     }
-    // [dO; W] B for a piece of B: with W's other piece (and fp16 dO's) where `both`
-    CUBF_DEV void stacked(uint32_t d, uint32_t b, uint32_t panel, int n, bool add, bool both) const {
-        over_v(d, smem_addr(sm.d_o[0]), smem_addr(sm.d_write[0]), b, panel, n, add, false);
-        if (NI == 2)
-            over_v(d, smem_addr(sm.d_o[1]), smem_addr(sm.d_write[1]), b, panel, n, true, false);
-        else if (both)
-            over_v(d, smem_addr(sm.d_o[0]), smem_addr(sm.d_write[1]), b, panel, n, true, true);
+    // d (n columns) (+)= two neighbouring tiles from `a` on times b over v.
+    CUBF_DEV void over_v(uint32_t d, uint32_t a, uint32_t b, int n, bool add, bool only_lower) const {
+        const uint32_t idesc = tc::instruction(n, true, true), chunk = static_cast<uint32_t>(w.v_rows * 16);
+        for (int s = 0; s < w.v_rows / 16; ++s)
+            tc::mma_shared(tmem + d, tc::chunks_along_k(a + s * 256, chunk), tc::chunks_along_k(b + s * 256, chunk), idesc,
+                           add || s > 0, only_lower);
+    }
+    // [dO; W] b, with both pieces of the first.
+    CUBF_DEV void stacked(uint32_t d, uint32_t b, int n, bool add) const {
+        over_v(d, stack(0), b, n, add, false);
+        over_v(d, stack(1), b, n, true, NI == 1);
     }
     CUBF_DEV void issue() {
         const uint32_t qk = smem_addr(sm.qk);
-        const uint32_t panel = static_cast<uint32_t>(w.v_rows * 128);
+        const uint32_t tile = static_cast<uint32_t>(w.v_rows * 128);
         for (int g = 0; g < group && !failed; ++g) {
             const uint32_t phase = g & 1;
             if (g > 0) wait(sm.free, phase ^ 1);                 // the head before is done with shared memory
@@ -1223,8 +1223,8 @@ struct Gradients {
                                            tc::rows_along_n(qk + tc::kPanel + j * KP * 256 + step), tc::instruction(64, false),
                                            i + j + s > 0);
                         }
-                stacked(kPM, smem_addr(sm.error[0]), panel, 64, false, true);
-                over_v(kPM, smem_addr(sm.d_o[0]), smem_addr(sm.d_write[0]), smem_addr(sm.error[1]), panel, 64, true, false);
+                stacked(kPM, stack(0) + 2 * tile, 64, false);
+                over_v(kPM, stack(0), stack(1) + 2 * tile, 64, true, false);
                 tc::commit(smem_addr(&sm.done[kPairsDone]));
             }
             __syncwarp();
@@ -1233,21 +1233,21 @@ struct Gradients {
                 wait(sm.state_full[b], use(n) & 1);
                 if (failed) break;
                 if (tc::elect()) {
-                    const uint32_t tile = smem_addr(sm.state[b]);
-                    if (n == 0) stacked(kQS, tile, panel, KP, false, true);
+                    const uint32_t state = smem_addr(sm.state[b]);
+                    if (n == 0) stacked(kQS, state, KP, false);
                     if (n == 1) {
                         if (NI == 2)
-                            stacked(kQS, tile, panel, KP, true, true);
+                            stacked(kQS, state, KP, true);
                         else
-                            over_v(kQS, smem_addr(sm.d_o[0]), smem_addr(sm.d_write[0]), tile, panel, KP, true, false);
+                            over_v(kQS, stack(0), state, KP, true, false);
                         tc::commit(smem_addr(&sm.done[kQsDone]));
                     }
                     if (n == 2) {
-                        over_v(kKU, smem_addr(sm.d_write[0]), smem_addr(sm.error[0]), tile, panel, KP, false, false);
-                        over_v(kKU, smem_addr(sm.d_write[1]), smem_addr(sm.error[1]), tile, panel, KP, true, false);
+                        over_v(kKU, stack(0) + tile, state, KP, false, false);
+                        over_v(kKU, stack(1) + tile, state, KP, true, false);
                     }
                     if (n == 3) {
-                        over_v(kKU, smem_addr(sm.d_write[0]), smem_addr(sm.error[0]), tile, panel, KP, true, false);
+                        over_v(kKU, stack(0) + tile, state, KP, true, false);
                         tc::commit(smem_addr(&sm.done[kStatesDone]));
                     }
                     tc::commit(smem_addr(&sm.state_empty[b]));
@@ -1259,12 +1259,11 @@ struct Gradients {
             if (failed) break;
             if (tc::elect()) {
                 constexpr uint32_t idesc = tc::instruction(KP, true), turned = tc::instruction(KP, true, true);
-                const uint32_t c0 = smem_addr(sm.pair_tile(0)), other = qk;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int j = 0; j < NI; ++j) {
-                        const uint32_t c = c0 + i * Shared::kTile;
+                        const uint32_t c = smem_addr(sm.pair_tile(i, w.v_rows));
 #pragma unroll
                         for (int s = 0; s < 4; ++s)
                             tc::mma_shared(tmem + kPairs, tc::rows_along_n(c + s * 32),
@@ -1272,7 +1271,7 @@ struct Gradients {
                                            i + j + s > 0);
 #pragma unroll
                         for (int s = 0; s < 8; ++s)              // lanes below 64 hold nothing of use
-                            tc::mma_shared(tmem + kTurned, tc::rows_along_k(other, c + s * 2048 - other),
+                            tc::mma_shared(tmem + kTurned, tc::rows_along_k(qk, c + s * 2048 - qk),
                                            tc::rows_along_k(qk + j * KP * 256 + s * 2048, kQkPanel), turned, i + j + s > 0);
                     }
                 tc::commit(smem_addr(&sm.done[kAllDone]));
@@ -1294,8 +1293,10 @@ struct Gradients {
             const uint32_t phase = g & 1;
             const int head = k_head * group + g;
             wait(sm.full, phase);
-            // the pairs' place is dO's with fp16, whose pieces of states come one at a time: those go first
-            if (NI == 2) inner(g);
+            // the pairs' place is dO's with fp16, whose pieces of states come one at a time: all of those go first
+            uint4 states[2][kShare];
+            take_states(g, states);
+            if (NI == 2) inner(g, states);
             wait(sm.done[kPairsDone], phase);
             {
                 uint32_t x[32], kk[32];
@@ -1311,14 +1312,26 @@ struct Gradients {
                     sm.beta[i] = d;
                 }
                 float pair[32], c[32], sum = 0.f;
+                if ((quarter & 1) == 0 && half == 1) {           // all behind their row
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const int at_j = 32 * half + j;
-                    const bool in = key ? at_j < i : at_j <= i;
-                    const float d = (high - sm.factors[kSumHigh][at_j]) + (low - sm.factors[kSumLow][at_j]);
-                    c[j] = in ? expf(d) * scale * sm.factors[kBeta][at_j] * __uint_as_float(x[j]) : 0.f;
-                    pair[j] = in ? c[j] * __uint_as_float(kk[j]) : 0.f;
-                    sum += pair[j];
+                    for (int j = 0; j < 32; ++j) pair[j] = c[j] = 0.f;
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) {
+                        const float4 h = *reinterpret_cast<const float4*>(&sm.factors[kSumHigh][32 * half + 4 * q]);
+                        const float4 l = *reinterpret_cast<const float4*>(&sm.factors[kSumLow][32 * half + 4 * q]);
+                        const float4 b = *reinterpret_cast<const float4*>(&sm.factors[kBeta][32 * half + 4 * q]);
+                        const float hs[4] = {h.x, h.y, h.z, h.w}, ls[4] = {l.x, l.y, l.z, l.w}, bs[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int j = 4 * q + e, at_j = 32 * half + j;
+                            const bool in = key ? at_j < i : at_j <= i;
+                            const float d = exp2f((high - hs[e]) + (low - ls[e])) * scale * bs[e] * __uint_as_float(x[j]);
+                            c[j] = in ? d : 0.f;
+                            pair[j] = in ? d * __uint_as_float(kk[j]) : 0.f;
+                            sum += pair[j];
+                        }
+                    }
                 }
                 sm.row[half][key][i] = sum;
                 if (NI == 2) wait(sm.done[kQsDone], phase);      // dO's place is free
@@ -1330,14 +1343,14 @@ struct Gradients {
                     const uint32_t to = row * 128 + (((4 * half + q) ^ (row & 7)) << 4);
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
-                        *reinterpret_cast<uint4*>(sm.pair_tile(n) + to) = make_uint4(f[0][n], f[1][n], f[2][n], f[3][n]);
+                        *reinterpret_cast<uint4*>(sm.pair_tile(n, w.v_rows) + to) = make_uint4(f[0][n], f[1][n], f[2][n], f[3][n]);
                 }
                 tc::fence_async();
                 tc::fence_before();
                 report(sm.ready);
                 sm.column[quarter][32 * half + lane] = lane_sums(pair, lane);
             }
-            if (NI == 1) inner(g);               // while the products with the states run
+            if (NI == 1) inner(g, states);       // while the products with the states run
             // the states' terms, scaled, and their products with q and k
             wait(sm.done[kStatesDone], phase);
             float sum = 0.f, kept = 0.f;
@@ -1427,37 +1440,40 @@ struct Gradients {
             }
         }
     }
-    // <S, dS> of the warp's share, as the pieces come by.
-    CUBF_DEV void inner(int g) {
-                    float dot = 0.f;
-                    {
-                        constexpr int PER = Shared::kPiece / 16 / kTcCompute;  // 16-byte chunks a thread
-                        const int chunks = static_cast<int>(w.state_piece / 16);
-                        uint4 x[2][PER];
-                        for (int n = 0; n < 4; ++n) {
-                            const int b = n % Shared::kBuffers;
-                            const uint32_t use = g * (4 / Shared::kBuffers) + n / Shared::kBuffers;
-                            wait(sm.state_full[b], use & 1);
-        #pragma unroll
-                            for (int p = 0; p < PER; ++p) {
-                                const int e = tid + p * kTcCompute;
-                                const uint4 y = e < chunks ? *reinterpret_cast<const uint4*>(sm.state[b] + e * 16) : make_uint4(0, 0, 0, 0);
-                                if (n < 2) {
-                                    if (n == 0)
-                                        x[0][p] = y;
-                                    else
-                                        x[1][p] = y;
-                                } else {
-                                    dot += product(x[0][p].x, x[1][p].x, y.x) + product(x[0][p].y, x[1][p].y, y.y) +
-                                           product(x[0][p].z, x[1][p].z, y.z) + product(x[0][p].w, x[1][p].w, y.w);
-                                }
-                            }
-                            report(sm.state_empty[b]);
-                        }
-                    }
-        #pragma unroll
-                    for (int d = 1; d < 32; d *= 2) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-                    if (lane == 0) sm.dot[warp] = dot;
+    // <S, dS> of the thread's share, as the pieces come by: S's are kept until dS's are there.
+    static constexpr int kShare = Shared::kPiece / 16 / kTcCompute;  // 16-byte chunks
+    CUBF_DEV uint4 share(int g, int n, int p) const {
+        const int e = tid + p * kTcCompute;
+        return e * 16 < static_cast<int>(w.state_piece)
+                   ? *reinterpret_cast<const uint4*>(sm.state[n % Shared::kBuffers] + e * 16)
+                   : make_uint4(0, 0, 0, 0);
+    }
+    CUBF_DEV uint32_t use_of(int g, int n) const { return static_cast<uint32_t>(g * (4 / Shared::kBuffers) + n / Shared::kBuffers); }
+    CUBF_DEV void take_states(int g, uint4 (&x)[2][kShare]) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            wait(sm.state_full[n % Shared::kBuffers], use_of(g, n) & 1);
+#pragma unroll
+            for (int p = 0; p < kShare; ++p) x[n][p] = share(g, n, p);
+            report(sm.state_empty[n % Shared::kBuffers]);
+        }
+    }
+    CUBF_DEV void inner(int g, const uint4 (&x)[2][kShare]) {
+        float dot = 0.f;
+#pragma unroll
+        for (int n = 2; n < 4; ++n) {
+            wait(sm.state_full[n % Shared::kBuffers], use_of(g, n) & 1);
+#pragma unroll
+            for (int p = 0; p < kShare; ++p) {
+                const uint4 y = share(g, n, p);
+                dot += product(x[0][p].x, x[1][p].x, y.x) + product(x[0][p].y, x[1][p].y, y.y) +
+                       product(x[0][p].z, x[1][p].z, y.z) + product(x[0][p].w, x[1][p].w, y.w);
+            }
+            report(sm.state_empty[n % Shared::kBuffers]);
+        }
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+        if (lane == 0) sm.dot[warp] = dot;
     }
     // (x0 + x1) y over a pair of values
     static CUBF_DEV float product(uint32_t x0, uint32_t x1, uint32_t y) {

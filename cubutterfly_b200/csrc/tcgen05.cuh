@@ -32,6 +32,14 @@ CUBF_DEV uint64_t descriptor(uint32_t addr, uint32_t leading) {
 CUBF_DEV uint64_t rows_along_n(uint32_t addr) { return descriptor(addr, 16); }
 CUBF_DEV uint64_t rows_along_k(uint32_t addr, uint32_t panel = kPanel) { return descriptor(addr, panel); }
 
+// The other form of a tile, written and read by threads that hold a row of it each: chunks of eight values along N (or M),
+// `chunk` bytes apart, each with the rows along K 16 bytes apart and not swizzled, so that a warp's 16-byte accesses to one
+// chunk are side by side.  K steps of 16 are 256 bytes apart.
+CUBF_DEV uint64_t chunks_along_k(uint32_t addr, uint32_t chunk) {
+    return static_cast<uint64_t>((addr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(128 >> 4) << 16) |
+           (static_cast<uint64_t>((chunk >> 4) & 0x3FFFu) << 32) | (1ull << 46);
+}
+
 // fp32 accumulators, bf16 operands, M = 128; A K-major (tensor memory) unless `a_mn`, B K-major unless `b_mn`.
 constexpr uint32_t instruction(int n, bool b_mn, bool a_mn = false, int m = 128) {
     return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(a_mn) << 15) | (static_cast<uint32_t>(b_mn) << 16) |
