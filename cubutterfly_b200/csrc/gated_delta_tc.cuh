@@ -71,7 +71,8 @@ struct TcShared {
 
 template <typename T, int KP, bool BACKWARD>
 struct TcPrepareShared {
-    static constexpr int kSquareTiles = BACKWARD ? 6 : 4;
+    // P leaves before L is there; fp16's rows, transposed, need more
+    static constexpr int kSquareTiles = BACKWARD && kInput<T> == 2 ? 6 : 4;
     static constexpr int kRowTile = 2 * tc::kPanel;              // 64 tokens by up to 128 columns of v
     static constexpr int kRowTiles = 1 + (BACKWARD ? kInput<T> : 0);
     static_assert(kRowTiles * kRowTile <= kSquareTiles * tc::kPanel, "transposed rows fit where L and P go");
@@ -153,7 +154,7 @@ CUBF_DEV void swizzled_b(uint32_t tile, int n, int k, int panel, int lane, uint3
 }
 
 template <typename T, int KP, bool BACKWARD>
-__global__ void __launch_bounds__(128, BACKWARD ? 2 : 3) gated_delta_tc_prepare_kernel(GatedDeltaArgs a, Places w, bool wide_q, bool wide_v, bool wide_d) {
+__global__ void __launch_bounds__(128, 3) gated_delta_tc_prepare_kernel(GatedDeltaArgs a, Places w, bool wide_q, bool wide_v, bool wide_d) {
     constexpr int NI = kInput<T>, kOperand = TcTiles<T, KP>::kOperand;
     using Shared = TcPrepareShared<T, KP, BACKWARD>;
     extern __shared__ __align__(1024) unsigned char aligned_raw[];
@@ -297,12 +298,18 @@ __global__ void __launch_bounds__(128, BACKWARD ? 2 : 3) gated_delta_tc_prepare_
                     *reinterpret_cast<uint32_t*>(sm.pairs.scaled + (n * C + i) * kPitchC + j) = f[n];
                 uint32_t x[2];
                 pieces<2>(p[0], p[1], x);
-                constexpr int at = BACKWARD ? 4 : 2;
-                *reinterpret_cast<uint32_t*>(sm.squares[at] + tc::swizzled(i, j)) = x[0];
-                *reinterpret_cast<uint32_t*>(sm.squares[at + 1] + tc::swizzled(i, j)) = x[1];
+                *reinterpret_cast<uint32_t*>(sm.squares[0] + tc::swizzled(i, j)) = x[0];
+                *reinterpret_cast<uint32_t*>(sm.squares[1] + tc::swizzled(i, j)) = x[1];
             }
         }
-        __syncwarp();
+        tc::fence_async();
+        __syncthreads();
+        constexpr int L_TILES = BACKWARD ? 4 : 2;
+        char* const matrices = work + w.solve + place * w.squares;
+        if (tid == 0) {
+            tc::bulk_store(matrices + L_TILES * tc::kPanel, smem_addr(sm.squares), 2 * tc::kPanel);
+            tc::bulk_commit();
+        }
         {   // the inverse of the warp's block on the diagonal, a lane a column, row by row
             const int col = lane & 15, base = 16 * warp;
             float t[16];                 // times beta
@@ -329,6 +336,7 @@ __global__ void __launch_bounds__(128, BACKWARD ? 2 : 3) gated_delta_tc_prepare_
                     }
             }
         }
+        if (tid == 0) tc::bulk_read();
         __syncthreads();
         {   // 16 columns of L a warp, transposed, block by block of 16 rows: L_i = (I + M beta)_ii^-1 (M_i - sum over j < i
             // of (M beta)_ij L_j), products at level 2
@@ -383,7 +391,7 @@ __global__ void __launch_bounds__(128, BACKWARD ? 2 : 3) gated_delta_tc_prepare_
         tc::fence_async();
         __syncthreads();
         if (tid == 0) {
-            tc::bulk_store(work + w.solve + place * sizeof(sm.squares), smem_addr(sm.squares), sizeof(sm.squares));
+            tc::bulk_store(matrices, smem_addr(sm.squares), L_TILES * tc::kPanel);
             tc::bulk_store(work + w.factors + place * sizeof(sm.factors), smem_addr(sm.factors), sizeof(sm.factors));
             tc::bulk_commit();
             if (g + 1 < group)
@@ -1398,7 +1406,8 @@ struct Gradients {
             }
             sm.row[half][key][i] += sum;
             if (key) sm.kept[half][i] = kept;
-            __syncwarp();
+            meet();
+            if (warp < 2) gates(head, gate_row);                 // while the last products run
             wait(sm.done[kAllDone], phase);
 #pragma unroll
             for (int n = 0; n < H / 32; ++n) {
@@ -1416,9 +1425,7 @@ struct Gradients {
                 __syncwarp();
             }
             tc::fence_before();
-            meet();
-            gates(head, gate_row);
-            meet();
+            if (g + 1 < group) meet();                           // the sums are read
             report(sm.free);
         }
         if (i < s.tokens) {
@@ -1484,22 +1491,20 @@ struct Gradients {
     // The computing warps meet; for that they all run through every head, whatever became of a wait.
     CUBF_DEV void meet() const { asm volatile("bar.sync 1, %0;" ::"n"(kTcCompute) : "memory"); }
     // dG and its sums from each token on, in 64 bits: the terms of a sequence's first token cancel exactly.
-    CUBF_DEV void gates(int head, size_t gate_row) {
-        if (warp < 2) {
-            const double kept = static_cast<double>(sm.kept[0][tid]) + sm.kept[1][tid];
-            double d = static_cast<double>(sm.row[0][0][tid]) + sm.row[1][0][tid] + sm.row[0][1][tid] + sm.row[1][1][tid] -
-                       kept - (static_cast<double>(sm.column[0][tid]) + sm.column[1][tid] + sm.column[2][tid] + sm.column[3][tid]);
-            double all = kept;
+    CUBF_DEV void gates(int head, size_t gate_row) {             // two warps
+        const double kept = static_cast<double>(sm.kept[0][tid]) + sm.kept[1][tid];
+        double d = static_cast<double>(sm.row[0][0][tid]) + sm.row[1][0][tid] + sm.row[0][1][tid] + sm.row[1][1][tid] - kept -
+                   (static_cast<double>(sm.column[0][tid]) + sm.column[1][tid] + sm.column[2][tid] + sm.column[3][tid]);
+        double all = kept;
 #pragma unroll
-            for (int n = 1; n < 32; n *= 2) {
-                const double other = __shfl_down_sync(0xffffffffu, d, n);
-                if (lane + n < 32) d += other;
-                all += __shfl_xor_sync(0xffffffffu, all, n);
-            }
-            sm.d_sum[tid] = d;
-            if (lane == 0) sm.all[warp] = all;
+        for (int n = 1; n < 32; n *= 2) {
+            const double other = __shfl_down_sync(0xffffffffu, d, n);
+            if (lane + n < 32) d += other;
+            all += __shfl_xor_sync(0xffffffffu, all, n);
         }
-        meet();
+        sm.d_sum[tid] = d;
+        if (lane == 0) sm.all[warp] = all;
+        asm volatile("bar.sync 2, 64;" ::: "memory");
         if (tid < s.tokens) {
             double d = sm.d_sum[tid] + (tid < 32 ? sm.d_sum[32] : 0.0);
             float inner = 0.f;
@@ -1517,6 +1522,7 @@ struct Gradients {
             else
                 static_cast<T*>(a.d_beta)[at] = Convert<T, float>::store(sm.beta[tid]);
         }
+        __syncwarp();
     }
 };
 
