@@ -67,10 +67,17 @@ template <typename T>
 constexpr int kTypeId = std::is_same_v<T, __half> ? 0 : 1;
 
 // ---- where things are ---------------------------------------------------------------------------
+// Long sequences of few chains in segments (gated_delta_tc.cuh): of `length` chunks, 0 for none.
+struct Segments {
+    int length, total;
+    size_t ends, d_ends, maps;           // in the workspace: states where segments end, gradients where they begin, A
+};
+
 struct Places {                          // of the workspace, in bytes from its start
     size_t factors, solve, attention, packed, values, rows, states, d_states, errors, d_writes, d_q, d_k, total;
     size_t state_piece, squares;         // bytes of a piece of a kept state, of a chunk's matrices (gated_delta_tc.cuh)
     int slots, v_pitch, v_rows;          // v_dim rounded up to 16, to 64
+    Segments segments;
 };
 
 struct Span {                            // a chunk

@@ -403,18 +403,50 @@ __global__ void __launch_bounds__(128, 3) gated_delta_tc_prepare_kernel(GatedDel
     }
 }
 
-// One chain's place in the grid.
+// One chain's place in the grid: a sequence of a head, or a segment of one.
 struct Chain {
     int head, sequence, start, length, row, base, chunks;
+    int index, segment, segments;        // place among all segments, number in the sequence, and how many that has
 };
-CUBF_DEV Chain chain_of(const GatedDeltaArgs& a, int index) {
-    Chain c;
+// Segments have places as chunks have: base(j) / length + j + s for segment s of sequence j.
+CUBF_DEV int segments_of(int chunks, int length) { return max(1, (chunks + length - 1) / length); }
+CUBF_DEV void locate(const GatedDeltaArgs& a, int sequence, Chain& c) {
+    c.sequence = sequence;
+    c.start = a.offsets ? offset_at(a, sequence) : 0;
+    c.length = a.offsets ? max(0, offset_at(a, sequence + 1) - c.start) : a.length;
+    c.row = a.offsets ? 0 : sequence;
+    c.base = slot_base(a, sequence, c.start);
+    c.chunks = (c.length + C - 1) / C;
+}
+CUBF_DEV int segment_base(const GatedDeltaArgs& a, const Segments& s, int sequence) {
+    const int base = slot_base(a, sequence, a.offsets ? offset_at(a, sequence) : 0);
+    return a.offsets ? base / s.length + sequence : sequence * segments_of((a.length + C - 1) / C, s.length);
+}
+// segment >= segments: a place that no segment has
+CUBF_DEV Chain chain_of(const GatedDeltaArgs& a, const Segments& s, int index) {
+    Chain c{};
     c.head = index % a.heads;
-    c.sequence = index / a.heads;
-    c.start = a.offsets ? offset_at(a, c.sequence) : 0;
-    c.length = a.offsets ? max(0, offset_at(a, c.sequence + 1) - c.start) : a.length;
-    c.row = a.offsets ? 0 : c.sequence;
-    c.base = slot_base(a, c.sequence, c.start);
+    c.index = index / a.heads;
+    c.segments = 1;
+    if (s.length == 0) {
+        locate(a, c.index, c);
+        return c;
+    }
+    int low = 0, high = a.offsets ? a.sequences : a.batch;
+    while (high - low > 1) {
+        const int mid = (low + high) / 2;
+        if (segment_base(a, s, mid) <= c.index)
+            low = mid;
+        else
+            high = mid;
+    }
+    locate(a, low, c);
+    c.segments = segments_of(c.chunks, s.length);
+    c.segment = c.index - segment_base(a, s, low);
+    const int first = c.segment * s.length;
+    c.start += first * C;
+    c.base += first;
+    c.length = min(max(0, c.length - first * C), s.length * C);
     c.chunks = (c.length + C - 1) / C;
     return c;
 }
@@ -807,6 +839,7 @@ struct TcChain {
     }
     // Byte of (column of v, channel) in a kept state's piece: chunks of eight channels.
     CUBF_DEV uint32_t kept(int row, int col) const { return static_cast<uint32_t>(((col >> 3) * w.v_rows + row) * 16); }
+    // A state of `columns` columns (null: zero), and where to: NaN where a wait ran out.
     CUBF_DEV void state_in(const float* p, P (&s)[H / 2]) const {
 #pragma unroll
         for (int i = 0; i < H / 2; ++i) {
@@ -819,8 +852,7 @@ struct TcChain {
             s[i] = f32x2::pk(x[0], x[1]);
         }
     }
-    // NaN where a wait ran out.
-    CUBF_DEV void state_out(float* p, const P (&s)[H / 2]) const {
+    CUBF_DEV void state_out(float* p, int columns, const P (&s)[H / 2]) const {
 #pragma unroll
         for (int i = 0; i < H / 2; ++i) {
             float x[2];
@@ -828,10 +860,17 @@ struct TcChain {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int k = half * H + 2 * i + e;
-                if (k < a.k_dim && v < a.v_dim)
-                    p[static_cast<size_t>(k) * a.v_dim + v] = failed ? __int_as_float(0x7fffffff) : x[e];
+                if (k < a.k_dim && v < columns)
+                    p[static_cast<size_t>(k) * columns + v] = failed ? __int_as_float(0x7fffffff) : x[e];
             }
         }
+    }
+    CUBF_DEV float* end_of(size_t region, int index) const {
+        return reinterpret_cast<float*>(work(region)) + (static_cast<size_t>(index) * a.heads + chain.head) * a.k_dim * a.v_dim;
+    }
+    CUBF_DEV float* map_of(int index) const {
+        return reinterpret_cast<float*>(work(w.segments.maps)) +
+               (static_cast<size_t>(index) * a.heads + chain.head) * a.k_dim * a.k_dim;
     }
     // S = whole S + what the products left in kD
     CUBF_DEV void state_add(float whole, P (&s)[H / 2]) const {
@@ -855,11 +894,23 @@ struct TcChain {
         __syncwarp();
         if (lane == 0) tc::barrier_arrive(smem_addr(&sm.out_ready));
     }
-    // KEEP: the backward's run, which keeps the state before each chunk and R in place of writing o.
-    template <bool KEEP>
+    // Results of a forward run: o and the final state, or, the backward's, the state before each chunk and R, or the state
+    // at the end of a segment alone, from the one before it (kEnd) or as the map of a segment (kMap: from the identity,
+    // with v = 0).
+    enum Mode { kOut, kKeep, kEnd, kMap };
+    template <int MODE>
     CUBF_DEV void compute_forward() {
+        constexpr bool OUT = MODE == kOut, KEEP = MODE == kKeep;
         P s[H / 2], y[16], x[16], o[16];
-        state_in(a.initial ? a.initial + state_offset() : nullptr, s);
+        if (MODE == kMap) {
+#pragma unroll
+            for (int i = 0; i < H / 2; ++i)
+                s[i] = f32x2::pk(half * H + 2 * i == v && v < a.k_dim ? 1.f : 0.f, half * H + 2 * i + 1 == v && v < a.k_dim ? 1.f : 0.f);
+        } else if (chain.segment == 0) {
+            state_in(a.initial ? a.initial + state_offset() : nullptr, s);
+        } else {
+            state_in(MODE == kEnd ? nullptr : end_of(w.segments.ends, chain.index - 1), s);
+        }
         const int chunks = chain.chunks;
         auto add_out = [&](int c) {          // the last part of a chunk's o
             wait(sm.done[kPu], c & 1);
@@ -874,7 +925,7 @@ struct TcChain {
         };
         uint4 rows[1][4];
         if (chunks > 0) {
-            fetch<1>(w.values, 0, rows);
+            if (MODE != kMap) fetch<1>(w.values, 0, rows);
             put_state(s, KEEP ? work(w.states) + place(0) * 2 * w.state_piece : nullptr);
             arrive(sm.ready[kStateReady]);
         }
@@ -882,14 +933,14 @@ struct TcChain {
         for (int c = 0; c < chunks && !failed; ++c, phase ^= 1) {
             const float* f = sm.factors[c & 1];
             // while the state meets k
-            if (!KEEP && c > 0) add_out(c - 1);
+            if (OUT && c > 0) add_out(c - 1);
             wait(sm.full[c & 1], (c >> 1) & 1);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float2 two = widen2(word(rows[0][i / 4], i % 4));
+                const float2 two = MODE == kMap ? make_float2(0.f, 0.f) : widen2(word(rows[0][i / 4], i % 4));
                 y[i] = f32x2::pk(two.x, two.y);
             }
-            if (c + 1 < chunks) fetch<1>(w.values, c + 1, rows);
+            if (MODE != kMap && c + 1 < chunks) fetch<1>(w.values, c + 1, rows);
             wait(sm.done[kSk], phase);
             get_tokens(Tiles::kX, x);
 #pragma unroll
@@ -901,7 +952,7 @@ struct TcChain {
             }
             put_tokens(Tiles::kY, y);
             arrive(sm.ready[kYReady]);
-            if (!KEEP && c > 0) move_out(c - 1);  // while Y meets L
+            if (OUT && c > 0) move_out(c - 1);  // while Y meets L
             wait(sm.done[kLy], phase);
             get_tokens(Tiles::kX, x);
 #pragma unroll
@@ -911,7 +962,7 @@ struct TcChain {
             // while U meets k
             if (KEEP) {
                 keep_tokens(w.errors, c, y);
-            } else {
+            } else if (OUT) {
                 put_tokens(Tiles::kY, y);
                 get_tokens(Tiles::kO, x);
                 arrive(sm.ready[kOutTaken]);
@@ -930,19 +981,25 @@ struct TcChain {
             put_state(s, KEEP && c + 1 < chunks ? work(w.states) + place(c + 1) * 2 * w.state_piece : nullptr);
             if (c + 1 < chunks) arrive(sm.ready[kStateReady]);
         }
-        if (!KEEP) {
+        if (OUT) {
             if (chunks > 0 && !failed) {
                 add_out(chunks - 1);
                 move_out(chunks - 1);
             }
-            state_out(a.last + state_offset(), s);
+            if (chain.segment + 1 == chain.segments) state_out(a.last + state_offset(), a.v_dim, s);
         }
+        if (MODE == kEnd) state_out(end_of(w.segments.ends, chain.index), a.v_dim, s);
+        if (MODE == kMap) state_out(map_of(chain.index), a.k_dim, s);
     }
 
-    // The sequence from its end: dS, W and dv of every chunk.
+    // The sequence from its end: dS, W and dv of every chunk, or (END) dS where a segment begins alone.
+    template <bool END>
     CUBF_DEV void compute_backward() {
         P s[H / 2], y[16], x[16], o[16];
-        state_in(a.d_last ? a.d_last + state_offset() : nullptr, s);
+        if (chain.segment + 1 == chain.segments)
+            state_in(a.d_last ? a.d_last + state_offset() : nullptr, s);
+        else
+            state_in(END ? nullptr : end_of(w.segments.d_ends, chain.index + 1), s);
         const int chunks = chain.chunks;
         uint4 rows[NI][4];
         auto put_rows = [&] {                // dO, exactly
@@ -968,7 +1025,7 @@ struct TcChain {
             }
             put_tokens(Tiles::kU, x, f + (kScaled - kDecay) * C);
         };
-        auto kept_at = [&](int n) { return work(w.d_states) + place(chunks - 1 - n) * 2 * w.state_piece; };
+        auto kept_at = [&](int n) -> char* { return END ? nullptr : work(w.d_states) + place(chunks - 1 - n) * 2 * w.state_piece; };
         if (chunks > 0) {
             fetch<NI>(w.rows, chunks - 1, rows);
             put_state(s, kept_at(0));
@@ -1005,16 +1062,18 @@ struct TcChain {
             put_tokens(Tiles::kO, x, f + (kDecayBeta - kDecay) * C);
             arrive(sm.ready[kUReady]);
             // while Z meets k
-            keep_tokens(w.d_writes, c, y);
+            if (!END) {
+                keep_tokens(w.d_writes, c, y);
 #pragma unroll
-            for (int g = 0; g < 8; ++g) {    // dv = beta W
-                P a, b;
-                factors_of(f + (kBeta - kDecay) * C, g, a, b);
-                o[2 * g] = f32x2::mul2(a, y[2 * g]);
-                o[2 * g + 1] = f32x2::mul2(b, y[2 * g + 1]);
+                for (int g = 0; g < 8; ++g) {    // dv = beta W
+                    P a, b;
+                    factors_of(f + (kBeta - kDecay) * C, g, a, b);
+                    o[2 * g] = f32x2::mul2(a, y[2 * g]);
+                    o[2 * g + 1] = f32x2::mul2(b, y[2 * g + 1]);
+                }
+                if (n > 0) wait(sm.out_free, (n - 1) & 1);
+                put_out(o);
             }
-            if (n > 0) wait(sm.out_free, (n - 1) & 1);
-            put_out(o);
             const float whole = f[C - 1];
             report(sm.empty[n & 1]);
             if (c > 0) put_rows();
@@ -1027,7 +1086,10 @@ struct TcChain {
                 arrive(sm.ready[kStateReady]);
             }
         }
-        if (a.d_initial) state_out(a.d_initial + state_offset(), s);
+        if (END)
+            state_out(end_of(w.segments.d_ends, chain.index), a.v_dim, s);
+        else if (chain.segment == 0 && a.d_initial)
+            state_out(a.d_initial + state_offset(), a.v_dim, s);
     }
 };
 
@@ -1045,7 +1107,10 @@ template <typename T, int KP>
 __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_forward_kernel(GatedDeltaArgs a, Places w, bool wide) {
     extern __shared__ __align__(1024) unsigned char aligned_raw[];
     pdl_begin();
-    TcChain<T, KP> run(a, w, *reinterpret_cast<TcShared<T, KP>*>(aligned_raw), chain_of(a, blockIdx.x));
+    using Run = TcChain<T, KP>;
+    const Chain chain = chain_of(a, w.segments, blockIdx.x);
+    if (chain.segment >= chain.segments) return;
+    Run run(a, w, *reinterpret_cast<TcShared<T, KP>*>(aligned_raw), chain);
     if (run.warp >= kTcCompute / 32) {
         fewer_registers<56>();
         if (run.warp == kTcCompute / 32)
@@ -1054,7 +1119,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_forward_kernel(G
             run.move_out(static_cast<T*>(a.o), false, wide);
     } else {
         more_registers<224>();
-        run.template compute_forward<false>();
+        run.template compute_forward<Run::kOut>();
     }
     run.finish();
 }
@@ -1065,7 +1130,10 @@ template <typename T, int KP>
 __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_chains_kernel(GatedDeltaArgs a, Places w, bool wide) {
     extern __shared__ __align__(1024) unsigned char aligned_raw[];
     pdl_begin();
-    TcChain<T, KP> run(a, w, *reinterpret_cast<TcShared<T, KP>*>(aligned_raw), chain_of(a, blockIdx.x / 2));
+    using Run = TcChain<T, KP>;
+    const Chain chain = chain_of(a, w.segments, blockIdx.x / 2);
+    if (chain.segment >= chain.segments) return;
+    Run run(a, w, *reinterpret_cast<TcShared<T, KP>*>(aligned_raw), chain);
     const bool reversed = blockIdx.x % 2 == 0;
     if (run.warp >= kTcCompute / 32) {
         fewer_registers<56>();
@@ -1080,11 +1148,105 @@ __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_chains_kernel(Ga
     } else {
         more_registers<224>();
         if (reversed)
-            run.compute_backward();
+            run.template compute_backward<false>();
         else
-            run.template compute_forward<true>();
+            run.template compute_forward<Run::kKeep>();
     }
     run.finish();
+}
+
+// ---- segments -----------------------------------------------------------------------------------
+// A chunk takes a chain from one state to the next by a map that is the same for all columns of v: S' = A S + D.  Where
+// chains are few and long they are cut into segments that run side by side, twice: first each for its D (from a state of
+// zero) and its A (from the identity, v = 0); then, from the states that those give, for its results.  Backward the map
+// is A transposed.  The first segment starts from the true state and needs no A, the last needs nothing of the first run.
+// That doubles the work and more, and is worth it where SMs would idle.
+template <typename T, int KP>
+__global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_ends_kernel(GatedDeltaArgs a, Places w, int kinds) {
+    extern __shared__ __align__(1024) unsigned char aligned_raw[];
+    pdl_begin();
+    using Run = TcChain<T, KP>;
+    const int kind = blockIdx.x % kinds;                        // D, A and, backward, the reversed chain's D
+    const Chain chain = chain_of(a, w.segments, blockIdx.x / kinds);
+    const bool first = chain.segment == 0, last = chain.segment + 1 == chain.segments;
+    if (chain.segment >= chain.segments || (kind == 2 ? first : last) || (kind == 1 && first)) return;
+    Run run(a, w, *reinterpret_cast<TcShared<T, KP>*>(aligned_raw), chain);
+    if (run.warp >= kTcCompute / 32) {
+        fewer_registers<56>();
+        if (run.warp == kTcCompute / 32) {
+            if (kind == 2)
+                run.issue_backward();
+            else
+                run.template issue_forward<true>();
+        }
+    } else {
+        more_registers<224>();
+        if (kind == 0)
+            run.template compute_forward<Run::kEnd>();
+        else if (kind == 1)
+            run.template compute_forward<Run::kMap>();
+        else
+            run.template compute_backward<true>();
+    }
+    run.finish();
+}
+
+// The states where segments end, one after another, in place of the D's: a CTA takes 16 columns of a chain's state, a thread
+// a row of it; fp32 throughout.  Odd CTAs go backward through the gradients.
+constexpr int kJoinColumns = 16;
+struct JoinShared {
+    float map[kDeltaMaxDim][kDeltaMaxDim + 1];
+    alignas(16) float state[2][kDeltaMaxDim][kJoinColumns];
+};
+static __global__ void __launch_bounds__(kDeltaMaxDim) gated_delta_join_kernel(GatedDeltaArgs a, Places w, int slices, bool backward) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    JoinShared& sm = *reinterpret_cast<JoinShared*>(raw);
+    pdl_begin();
+    const int tid = threadIdx.x;
+    int index = blockIdx.x;
+    const bool reversed = backward && index % 2;
+    if (backward) index /= 2;
+    const int from = index % slices * kJoinColumns, head = index / slices % a.heads, sequence = index / slices / a.heads;
+    Chain c{};
+    locate(a, sequence, c);
+    const int segments = segments_of(c.chunks, w.segments.length), base = segment_base(a, w.segments, sequence);
+    const size_t state = static_cast<size_t>(a.k_dim) * a.v_dim, map = static_cast<size_t>(a.k_dim) * a.k_dim;
+    float* const ends = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + (reversed ? w.segments.d_ends : w.segments.ends));
+    const float* const maps = reinterpret_cast<const float*>(static_cast<const char*>(a.workspace) + w.segments.maps);
+    auto row_at = [&](int s) {
+        return ends + (static_cast<size_t>(base + s) * a.heads + head) * state + static_cast<size_t>(tid) * a.v_dim + from;
+    };
+    const int columns = min(kJoinColumns, a.v_dim - from);
+    const bool row = tid < a.k_dim;
+#pragma unroll
+    for (int e = 0; e < kJoinColumns; ++e)
+        sm.state[0][tid][e] = row && segments > 2 && e < columns ? row_at(reversed ? segments - 1 : 0)[e] : 0.f;
+    int now = 0;
+    for (int n = 1; n + 1 < segments; ++n) {
+        const int s = reversed ? segments - 1 - n : n;
+        const float* m = maps + (static_cast<size_t>(base + s) * a.heads + head) * map;
+        __syncthreads();
+        for (int e = tid; e < a.k_dim * a.k_dim; e += kDeltaMaxDim) sm.map[e / a.k_dim][e % a.k_dim] = m[e];
+        float x[kJoinColumns];
+#pragma unroll
+        for (int e = 0; e < kJoinColumns; ++e) x[e] = row && e < columns ? row_at(s)[e] : 0.f;
+        __syncthreads();
+        for (int k = 0; k < a.k_dim; ++k) {
+            const float f = reversed ? sm.map[k][tid] : sm.map[tid][k];
+#pragma unroll
+            for (int e = 0; e < kJoinColumns; e += 4) {
+                const float4 y = *reinterpret_cast<const float4*>(&sm.state[now][k][e]);
+                x[e] = fmaf(f, y.x, x[e]), x[e + 1] = fmaf(f, y.y, x[e + 1]);
+                x[e + 2] = fmaf(f, y.z, x[e + 2]), x[e + 3] = fmaf(f, y.w, x[e + 3]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < kJoinColumns; ++e) {
+            sm.state[now ^ 1][tid][e] = row ? x[e] : 0.f;
+            if (row && e < columns) row_at(s)[e] = x[e];
+        }
+        now ^= 1;
+    }
 }
 
 // ---- gradients ----------------------------------------------------------------------------------

@@ -2,6 +2,7 @@
 // CUBF_GD_TYPE (0 fp16, 1 bf16, 2 fp32) and CUBF_GD_K (64 or 128: the padded
 // key size).
 #include <algorithm>
+#include <cmath>
 
 #include "gated_delta.cuh"
 #include "gated_delta_tc.cuh"
@@ -41,6 +42,36 @@ bool rows_aligned(const HeadTensor& t, int width) {
 
 int sequences_of(const GatedDeltaArgs& a) { return a.offsets ? a.sequences : a.batch; }
 
+#if CUBF_GD_TENSOR
+// Chunks a segment, 0 for none: the shortest time by what a chunk of a chain takes on one SM (2.4 us with its results
+// forward, 2.9 backward, 1.9 without them), a state's join (3 us) and the CTAs that run at once, one per SM.  Of a packed
+// batch the host knows the tokens and the sequences alone; n random cuts leave a longest piece of (1 + 1/2 + .. + 1/n) / n.
+// One sequence of 16384 tokens and 32 heads: %s us in three segments, 622 in one; of 4 heads %s in %s against 617.
+int segment_length(const GatedDeltaArgs& a, bool backward) {
+    double longest = ceil_div(a.length, C), all = longest * a.batch;
+    const double sequences = sequences_of(a);
+    if (a.offsets) {
+        double share = 0;
+        for (int n = 1; n <= a.sequences && n <= 1000; ++n) share += 1.0 / n;
+        longest *= std::min(1.0, share / sequences);
+    }
+    if (longest < 16) return 0;
+    const double full = backward ? 2.9 : 2.4;
+    auto waves = [](double ctas) { return std::max(1.0, std::ceil(ctas / 148)); };
+    double best = std::max(waves((backward ? 2 : 1) * sequences * a.heads) * all / sequences, longest) * full;
+    int length = 0;
+    for (int n = 2; n <= 64 && longest / n >= 4; ++n) {
+        const int chunks = static_cast<int>(std::ceil(longest / n));
+        const double segments = all / chunks + (a.offsets ? sequences : 0);  // of all sequences
+        const double first = segments * a.heads * (backward ? 3 : 2) - (backward ? 5 : 3) * sequences * a.heads;
+        const double time = waves(first) * chunks * 1.9 + (n - 2) * 3 + 10 +
+                            waves((backward ? 2 : 1) * segments * a.heads) * chunks * full;
+        if (time < 0.95 * best) best = time, length = chunks;
+    }
+    return length;
+}
+#endif
+
 Places places_of(const GatedDeltaArgs& a, bool backward) {
     Places w{};
     w.slots = a.offsets ? a.length / C + a.sequences : a.batch * ceil_div(a.length, C);
@@ -60,6 +91,14 @@ Places places_of(const GatedDeltaArgs& a, bool backward) {
     w.solve = take(chunks * w.squares);
     w.packed = take(key_chunks * 2 * kInput<T> * KP * 128);
     w.values = take(chunks * w.v_rows * 128);
+    w.segments.length = segment_length(a, backward);
+    if (const int n = w.segments.length; n > 0) {
+        w.segments.total = a.offsets ? (a.length / C + a.sequences) / n + a.sequences : a.batch * ceil_div(ceil_div(a.length, C), n);
+        const size_t ends = static_cast<size_t>(w.segments.total) * a.heads;
+        w.segments.ends = take(ends * a.k_dim * a.v_dim * 4);
+        w.segments.maps = take(ends * a.k_dim * a.k_dim * 4);
+        if (backward) w.segments.d_ends = take(ends * a.k_dim * a.v_dim * 4);
+    }
     if (backward) {
         w.rows = take(chunks * kInput<T> * w.v_rows * 128);
         w.states = take(chunks * 2 * w.state_piece);
@@ -150,25 +189,30 @@ cudaError_t launch_gated_delta_unit<CUBF_GD_TYPE, CUBF_GD_K>(const GatedDeltaArg
     const size_t chunks = static_cast<size_t>(w.slots) * a.heads;
 #if CUBF_GD_TENSOR
     const size_t key_chunks = static_cast<size_t>(w.slots) * a.k_heads;
-    const size_t chains = static_cast<size_t>(sequences_of(a)) * a.heads;
+    const int sequences = sequences_of(a);
+    const size_t chains = static_cast<size_t>(w.segments.length ? w.segments.total : sequences) * a.heads;
     const bool wide_q = rows_aligned(a.q, a.k_dim) && rows_aligned(a.k, a.k_dim);
     const HeadTensor out{backward ? a.d_v : a.o, 0, 0, static_cast<size_t>(a.v_dim)};
     const bool wide_out = rows_aligned(out, a.v_dim);
-    if (!backward) {
-        static KernelSetup prepare, chain;
-        const cudaError_t e = launch(prepare, &gated_delta_tc_prepare_kernel<T, KP, false>, key_chunks, 128,
-                                     sizeof(TcPrepareShared<T, KP, false>), stream, a, w, wide_q, rows_aligned(a.v, a.v_dim), false);
-        if (e != cudaSuccess) return e;
-        return launch(chain, &gated_delta_tc_forward_kernel<T, KP>, chains, kTcThreads, sizeof(TcShared<T, KP>), stream, a, w,
-                      wide_out);
-    }
-    static KernelSetup prepare, chain, gradients;
-    cudaError_t e = launch(prepare, &gated_delta_tc_prepare_kernel<T, KP, true>, key_chunks, 128,
-                           sizeof(TcPrepareShared<T, KP, true>), stream, a, w, wide_q, rows_aligned(a.v, a.v_dim),
-                           rows_aligned(a.d_o, a.v_dim));
+    static KernelSetup prepare, prepare_backward, ends, join, forward, both, gradients;
+    cudaError_t e = backward ? launch(prepare_backward, &gated_delta_tc_prepare_kernel<T, KP, true>, key_chunks, 128,
+                                      sizeof(TcPrepareShared<T, KP, true>), stream, a, w, wide_q, rows_aligned(a.v, a.v_dim),
+                                      rows_aligned(a.d_o, a.v_dim))
+                             : launch(prepare, &gated_delta_tc_prepare_kernel<T, KP, false>, key_chunks, 128,
+                                      sizeof(TcPrepareShared<T, KP, false>), stream, a, w, wide_q, rows_aligned(a.v, a.v_dim), false);
     if (e != cudaSuccess) return e;
-    e = launch(chain, &gated_delta_tc_chains_kernel<T, KP>, 2 * chains, kTcThreads, sizeof(TcShared<T, KP>), stream, a, w,
-               wide_out);
+    if (w.segments.length) {
+        const int kinds = backward ? 3 : 2, slices = ceil_div(a.v_dim, kJoinColumns);
+        e = launch(ends, &gated_delta_tc_ends_kernel<T, KP>, chains * kinds, kTcThreads, sizeof(TcShared<T, KP>), stream, a, w, kinds);
+        if (e != cudaSuccess) return e;
+        e = launch(join, &gated_delta_join_kernel, static_cast<size_t>(sequences) * a.heads * slices * (backward ? 2 : 1),
+                   kDeltaMaxDim, sizeof(JoinShared), stream, a, w, slices, backward);
+        if (e != cudaSuccess) return e;
+    }
+    if (!backward)
+        return launch(forward, &gated_delta_tc_forward_kernel<T, KP>, chains, kTcThreads, sizeof(TcShared<T, KP>), stream, a, w,
+                      wide_out);
+    e = launch(both, &gated_delta_tc_chains_kernel<T, KP>, 2 * chains, kTcThreads, sizeof(TcShared<T, KP>), stream, a, w, wide_out);
     if (e != cudaSuccess) return e;
     return launch(gradients, &gated_delta_tc_gradients_kernel<T, KP>, key_chunks, kGradientThreads,
                   sizeof(GradientShared<T, KP>), stream, a, w);
