@@ -869,8 +869,7 @@ struct TcChain {
         return reinterpret_cast<float*>(work(region)) + (static_cast<size_t>(index) * a.heads + chain.head) * a.k_dim * a.v_dim;
     }
     CUBF_DEV float* map_of(int index) const {
-        return reinterpret_cast<float*>(work(w.segments.maps)) +
-               (static_cast<size_t>(index) * a.heads + chain.head) * a.k_dim * a.k_dim;
+        return reinterpret_cast<float*>(work(w.segments.maps)) + (static_cast<size_t>(index) * a.heads + chain.head) * KP * KP;
     }
     // S = whole S + what the products left in kD
     CUBF_DEV void state_add(float whole, P (&s)[H / 2]) const {
@@ -989,7 +988,7 @@ struct TcChain {
             if (chain.segment + 1 == chain.segments) state_out(a.last + state_offset(), a.v_dim, s);
         }
         if (MODE == kEnd) state_out(end_of(w.segments.ends, chain.index), a.v_dim, s);
-        if (MODE == kMap) state_out(map_of(chain.index), a.k_dim, s);
+        if (MODE == kMap) state_out(map_of(chain.index), KP, s);
     }
 
     // The sequence from its end: dS, W and dv of every chunk, or (END) dS where a segment begins alone.
@@ -1191,18 +1190,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_ends_kernel(Gate
     run.finish();
 }
 
-// The states where segments end, one after another, in place of the D's: a CTA takes 16 columns of a chain's state, a thread
-// a row of it; fp32 throughout.  Odd CTAs go backward through the gradients.
-constexpr int kJoinColumns = 16;
+// The states where segments end, one after another, in place of the D's: a CTA takes 8 columns of a chain's state, a thread
+// four columns of a row; fp32 throughout.  The next map and D are on their way in registers while one map is used.  Odd CTAs of the
+// backward go through the gradients from the end.
+constexpr int kJoinColumns = 8;
+template <int KP>
 struct JoinShared {
-    float map[kDeltaMaxDim][kDeltaMaxDim + 1];
-    alignas(16) float state[2][kDeltaMaxDim][kJoinColumns];
+    alignas(16) float map[2][KP][KP + 4];
+    alignas(16) float state[2][KP][kJoinColumns];
 };
-static __global__ void __launch_bounds__(kDeltaMaxDim) gated_delta_join_kernel(GatedDeltaArgs a, Places w, int slices, bool backward) {
+template <int KP>
+__global__ void __launch_bounds__(2 * KP) gated_delta_join_kernel(GatedDeltaArgs a, Places w, int slices, bool backward) {
     extern __shared__ __align__(16) unsigned char raw[];
-    JoinShared& sm = *reinterpret_cast<JoinShared*>(raw);
+    JoinShared<KP>& sm = *reinterpret_cast<JoinShared<KP>*>(raw);
     pdl_begin();
-    const int tid = threadIdx.x;
+    const int row = threadIdx.x % KP, part = threadIdx.x / KP * 4;
     int index = blockIdx.x;
     const bool reversed = backward && index % 2;
     if (backward) index /= 2;
@@ -1210,42 +1212,64 @@ static __global__ void __launch_bounds__(kDeltaMaxDim) gated_delta_join_kernel(G
     Chain c{};
     locate(a, sequence, c);
     const int segments = segments_of(c.chunks, w.segments.length), base = segment_base(a, w.segments, sequence);
-    const size_t state = static_cast<size_t>(a.k_dim) * a.v_dim, map = static_cast<size_t>(a.k_dim) * a.k_dim;
-    float* const ends = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + (reversed ? w.segments.d_ends : w.segments.ends));
-    const float* const maps = reinterpret_cast<const float*>(static_cast<const char*>(a.workspace) + w.segments.maps);
-    auto row_at = [&](int s) {
-        return ends + (static_cast<size_t>(base + s) * a.heads + head) * state + static_cast<size_t>(tid) * a.v_dim + from;
+    if (segments < 3) return;
+    char* const work = static_cast<char*>(a.workspace);
+    float* const ends = reinterpret_cast<float*>(work + (reversed ? w.segments.d_ends : w.segments.ends));
+    auto place = [&](int s) { return static_cast<size_t>(base + s) * a.heads + head; };
+    auto row_at = [&](int s) { return ends + (place(s) * a.k_dim + row) * a.v_dim + from + part; };
+    auto segment = [&](int n) { return reversed ? segments - 1 - n : n; };
+    constexpr int VECTORS = KP / 8;              // of a map, a thread
+    float4 next[VECTORS];
+    float x[4];
+    const bool own = row < a.k_dim;
+    auto fetch = [&](int s) {
+        const float4* m = reinterpret_cast<const float4*>(work + w.segments.maps) + place(s) * (KP * KP / 4);
+#pragma unroll
+        for (int e = 0; e < VECTORS; ++e) {
+            const int at = threadIdx.x + e * 2 * KP;
+            next[e] = at < a.k_dim * (KP / 4) ? m[at] : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
     };
-    const int columns = min(kJoinColumns, a.v_dim - from);
-    const bool row = tid < a.k_dim;
+    auto read = [&](int s) {
 #pragma unroll
-    for (int e = 0; e < kJoinColumns; ++e)
-        sm.state[0][tid][e] = row && segments > 2 && e < columns ? row_at(reversed ? segments - 1 : 0)[e] : 0.f;
-    int now = 0;
+        for (int e = 0; e < 4; ++e) x[e] = own && from + part + e < a.v_dim ? row_at(s)[e] : 0.f;
+    };
+    read(segment(0));
+    *reinterpret_cast<float4*>(&sm.state[0][row][part]) = make_float4(x[0], x[1], x[2], x[3]);
+    fetch(segment(1));
+    read(segment(1));
     for (int n = 1; n + 1 < segments; ++n) {
-        const int s = reversed ? segments - 1 - n : n;
-        const float* m = maps + (static_cast<size_t>(base + s) * a.heads + head) * map;
-        __syncthreads();
-        for (int e = tid; e < a.k_dim * a.k_dim; e += kDeltaMaxDim) sm.map[e / a.k_dim][e % a.k_dim] = m[e];
-        float x[kJoinColumns];
+        const int now = (n - 1) & 1;
+        float (*const map)[KP + 4] = sm.map[now];
 #pragma unroll
-        for (int e = 0; e < kJoinColumns; ++e) x[e] = row && e < columns ? row_at(s)[e] : 0.f;
-        __syncthreads();
-        for (int k = 0; k < a.k_dim; ++k) {
-            const float f = reversed ? sm.map[k][tid] : sm.map[tid][k];
+        for (int e = 0; e < VECTORS; ++e) {
+            const int at = threadIdx.x + e * 2 * KP;
+            *reinterpret_cast<float4*>(&map[at / (KP / 4)][at % (KP / 4) * 4]) = next[e];
+        }
+        float sum[4] = {x[0], x[1], x[2], x[3]};
+        if (n + 2 < segments) fetch(segment(n + 1)), read(segment(n + 1));
+        __syncthreads();  // all have this map and state, and are past the ones that the next step writes over
+#pragma unroll 4
+        for (int k = 0; k < KP; k += 4) {
+            float f[4];
+            if (reversed) {
 #pragma unroll
-            for (int e = 0; e < kJoinColumns; e += 4) {
-                const float4 y = *reinterpret_cast<const float4*>(&sm.state[now][k][e]);
-                x[e] = fmaf(f, y.x, x[e]), x[e + 1] = fmaf(f, y.y, x[e + 1]);
-                x[e + 2] = fmaf(f, y.z, x[e + 2]), x[e + 3] = fmaf(f, y.w, x[e + 3]);
+                for (int e = 0; e < 4; ++e) f[e] = map[k + e][row];
+            } else {
+                const float4 y = *reinterpret_cast<const float4*>(&map[row][k]);
+                f[0] = y.x, f[1] = y.y, f[2] = y.z, f[3] = y.w;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float4 y = *reinterpret_cast<const float4*>(&sm.state[now][k + e][part]);
+                sum[0] = fmaf(f[e], y.x, sum[0]), sum[1] = fmaf(f[e], y.y, sum[1]);
+                sum[2] = fmaf(f[e], y.z, sum[2]), sum[3] = fmaf(f[e], y.w, sum[3]);
             }
         }
+        *reinterpret_cast<float4*>(&sm.state[now ^ 1][row][part]) = make_float4(sum[0], sum[1], sum[2], sum[3]);
 #pragma unroll
-        for (int e = 0; e < kJoinColumns; ++e) {
-            sm.state[now ^ 1][tid][e] = row ? x[e] : 0.f;
-            if (row && e < columns) row_at(s)[e] = x[e];
-        }
-        now ^= 1;
+        for (int e = 0; e < 4; ++e)
+            if (own && from + part + e < a.v_dim) row_at(segment(n))[e] = sum[e];
     }
 }
 

@@ -44,9 +44,10 @@ int sequences_of(const GatedDeltaArgs& a) { return a.offsets ? a.sequences : a.b
 
 #if CUBF_GD_TENSOR
 // Chunks a segment, 0 for none: the shortest time by what a chunk of a chain takes on one SM (2.4 us with its results
-// forward, 2.9 backward, 1.9 without them), a state's join (3 us) and the CTAs that run at once, one per SM.  Of a packed
+// forward, 2.9 backward, 1.9 without them), a state's join (4 us) and the CTAs that run at once, one per SM.  Of a packed
 // batch the host knows the tokens and the sequences alone; n random cuts leave a longest piece of (1 + 1/2 + .. + 1/n) / n.
-// One sequence of 16384 tokens and 32 heads: %s us in three segments, 622 in one; of 4 heads %s in %s against 617.
+// Whole calls forward, one sequence of 16384 tokens: 32 heads 680 us in three segments against 870 in one, 12 heads 369 in
+// seven against 735, 4 heads 213 in 16 against 670; forward and backward of 4 heads 655 in 14 against 1960.
 int segment_length(const GatedDeltaArgs& a, bool backward) {
     double longest = ceil_div(a.length, C), all = longest * a.batch;
     const double sequences = sequences_of(a);
@@ -64,7 +65,7 @@ int segment_length(const GatedDeltaArgs& a, bool backward) {
         const int chunks = static_cast<int>(std::ceil(longest / n));
         const double segments = all / chunks + (a.offsets ? sequences : 0);  // of all sequences
         const double first = segments * a.heads * (backward ? 3 : 2) - (backward ? 5 : 3) * sequences * a.heads;
-        const double time = waves(first) * chunks * 1.9 + (n - 2) * 3 + 10 +
+        const double time = waves(first) * chunks * 1.9 + (n - 2) * 4 + 10 +
                             waves((backward ? 2 : 1) * segments * a.heads) * chunks * full;
         if (time < 0.95 * best) best = time, length = chunks;
     }
@@ -96,7 +97,7 @@ Places places_of(const GatedDeltaArgs& a, bool backward) {
         w.segments.total = a.offsets ? (a.length / C + a.sequences) / n + a.sequences : a.batch * ceil_div(ceil_div(a.length, C), n);
         const size_t ends = static_cast<size_t>(w.segments.total) * a.heads;
         w.segments.ends = take(ends * a.k_dim * a.v_dim * 4);
-        w.segments.maps = take(ends * a.k_dim * a.k_dim * 4);
+        w.segments.maps = take(ends * KP * KP * 4);
         if (backward) w.segments.d_ends = take(ends * a.k_dim * a.v_dim * 4);
     }
     if (backward) {
@@ -205,8 +206,8 @@ cudaError_t launch_gated_delta_unit<CUBF_GD_TYPE, CUBF_GD_K>(const GatedDeltaArg
         const int kinds = backward ? 3 : 2, slices = ceil_div(a.v_dim, kJoinColumns);
         e = launch(ends, &gated_delta_tc_ends_kernel<T, KP>, chains * kinds, kTcThreads, sizeof(TcShared<T, KP>), stream, a, w, kinds);
         if (e != cudaSuccess) return e;
-        e = launch(join, &gated_delta_join_kernel, static_cast<size_t>(sequences) * a.heads * slices * (backward ? 2 : 1),
-                   kDeltaMaxDim, sizeof(JoinShared), stream, a, w, slices, backward);
+        e = launch(join, &gated_delta_join_kernel<KP>, static_cast<size_t>(sequences) * a.heads * slices * (backward ? 2 : 1),
+                   2 * KP, sizeof(JoinShared<KP>), stream, a, w, slices, backward);
         if (e != cudaSuccess) return e;
     }
     if (!backward)

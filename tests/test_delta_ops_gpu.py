@@ -121,6 +121,32 @@ def test_gated_delta_packed_with_batch_dimension(cuda):
     assert torch.equal(o4[0], o) and torch.equal(final4, final)
 
 
+# Few long chains are cut into segments whose ends are found side by side and joined.
+LONG = [(1, 1024, 1, 1, 16, 16, None), (1, 1025, 1, 2, 128, 128, None), (2, 1663, 1, 1, 100, 120, None), (1, 2111, 1, 3, 37, 65, None),
+        (1, 2300, 1, 2, 64, 64, [0, 2300]), (1, 2500, 2, 2, 128, 48, [0, 0, 1151, 1152, 1152, 2399, 2500]),
+        (1, 2400, 1, 1, 70, 128, [0, 64, 128, 1600, 2400, 2400])]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("state", [False, True])
+@pytest.mark.parametrize("batch,length,k_heads,heads,k_dim,v_dim,cuts", LONG, ids=str)
+def test_gated_delta_few_long_chains(cuda, batch, length, k_heads, heads, k_dim, v_dim, cuts, state, dtype):
+    t = delta_case(batch, length, k_heads, heads, k_dim, v_dim, dtype, cuts=cuts, state=state, seed=40)
+    t["g"] = t["g"] * 0.02  # states reach from segment to segment
+    check_delta(t, cuts)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_gated_delta_long_chain_is_causal(cuda, dtype):
+    t = {n: None if v is None else v.cuda() for n, v in delta_case(1, 2300, 1, 1, 64, 64, dtype, state=True, seed=44).items()}
+    o, final = run_delta(t)
+    t["v"] = t["v"].clone()
+    t["v"][0, 1500] = float("nan")
+    bad, _ = run_delta(t)
+    assert torch.equal(bad[:, :1472], o[:, :1472])  # the chunk of token 1500 begins there
+    assert bad[:, 1500:].isnan().any(-1).all()
+
+
 @pytest.mark.parametrize("grads", [("o",), ("final",)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_gated_delta_gradient_of_one_output(cuda, grads, dtype):
