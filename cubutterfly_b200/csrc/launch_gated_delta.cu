@@ -4,16 +4,21 @@
 #include <algorithm>
 #include <cmath>
 
-#include "gated_delta.cuh"
-#include "gated_delta_tc.cuh"
-#include "launch_util.cuh"
-
 #ifndef CUBF_GD_TYPE
 #define CUBF_GD_TYPE 1
 #endif
 #ifndef CUBF_GD_K
 #define CUBF_GD_K 128
 #endif
+
+// 16-bit tensors go through the 5th-generation tensor cores; three pieces of fp32 ones would not fit tensor memory.
+#define CUBF_GD_TENSOR (CUBF_GD_TYPE != 2)
+#if CUBF_GD_TENSOR
+#include "gated_delta_tc.cuh"
+#else
+#include "gated_delta_fp32.cuh"
+#endif
+#include "launch_util.cuh"
 
 namespace cubf {
 
@@ -29,9 +34,6 @@ namespace {
 using namespace delta;
 using T = std::conditional_t<CUBF_GD_TYPE == 0, __half, std::conditional_t<CUBF_GD_TYPE == 1, __nv_bfloat16, float>>;
 constexpr int KP = CUBF_GD_K;
-
-// 16-bit tensors go through the 5th-generation tensor cores; three pieces of fp32 ones would not fit tensor memory.
-#define CUBF_GD_TENSOR (CUBF_GD_TYPE != 2)
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
@@ -109,9 +111,9 @@ Places places_of(const GatedDeltaArgs& a, bool backward) {
     }
 #else
     w.factors = take(chunks * kFactors * 4);
-    w.solve = take(chunks * kLevel<T> * kSquare * 2);
-    w.attention = take(chunks * kLevel<T> * kSquare * 2);
-    w.packed = take(key_chunks * 2 * kInput<T> * C * KP * 2);
+    w.solve = take(chunks * kPieces * kSquare * 2);
+    w.attention = take(chunks * kPieces * kSquare * 2);
+    w.packed = take(key_chunks * 2 * kPieces * C * KP * 2);
     if (backward) {
         w.states = take(chunks * w.v_pitch * KP * 4);
         w.d_states = take(chunks * w.v_pitch * KP * 4);
@@ -156,24 +158,24 @@ cudaError_t launch_chains(const GatedDeltaArgs& a, const Places& w, bool backwar
     if (backward) {
         // set up for the largest CTA, launched with what this one's warps need
         static KernelSetup setup;
-        constexpr int most = ChainTiles<T, KP>::bytes(8);
+        constexpr int most = ChainTiles<KP>::bytes(8);
         int cap = 0;
-        const auto kernel = &gated_delta_chains_kernel<T, KP>;
+        const auto kernel = &gated_delta_chains_kernel<KP>;
         const cudaError_t e = setup_kernel(setup, kernel, 256, most, &cap, true);
         if (e != cudaSuccess) return e;
         if (2 * grid > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
         return launch_dependent(kernel, static_cast<unsigned>(2 * grid), 32u * shape.warps,
-                                ChainTiles<T, KP>::bytes(shape.warps), stream, a, w, shape);
+                                ChainTiles<KP>::bytes(shape.warps), stream, a, w, shape);
     }
     static KernelSetup setup;
-    constexpr int most = ChainTiles<T, KP>::bytes(8);
+    constexpr int most = ChainTiles<KP>::bytes(8);
     int cap = 0;
-    const auto kernel = &gated_delta_forward_kernel<T, KP>;
+    const auto kernel = &gated_delta_forward_kernel<KP>;
     const cudaError_t e = setup_kernel(setup, kernel, 256, most, &cap, true);
     if (e != cudaSuccess) return e;
     if (grid > 0x7fffffffULL) return cudaErrorInvalidConfiguration;
     return launch_dependent(kernel, static_cast<unsigned>(grid), 32u * shape.warps,
-                             ChainTiles<T, KP>::bytes(shape.warps), stream, a, w, shape);
+                             ChainTiles<KP>::bytes(shape.warps), stream, a, w, shape);
 }
 #endif
 
@@ -218,18 +220,16 @@ cudaError_t launch_gated_delta_unit<CUBF_GD_TYPE, CUBF_GD_K>(const GatedDeltaArg
     return launch(gradients, &gated_delta_tc_gradients_kernel<T, KP>, key_chunks, kGradientThreads,
                   sizeof(GradientShared<T, KP>), stream, a, w);
 #else
-    static KernelSetup prepare, gradients, shared, share;
-    cudaError_t e = launch(prepare, &gated_delta_prepare_kernel<T, KP>, chunks, 128, sizeof(PrepareShared<T, KP>), stream, a, w);
+    static KernelSetup prepare, gradients, share;
+    cudaError_t e = launch(prepare, &gated_delta_prepare_kernel<KP>, chunks, 128, sizeof(PrepareShared<KP>), stream, a, w);
     if (e != cudaSuccess) return e;
     e = launch_chains(a, w, backward, stream);
     if (e != cudaSuccess || !backward) return e;
-    constexpr int smem = sizeof(GradientShared32<T, KP>);
-    if (a.heads == a.k_heads)
-        return launch(gradients, &gated_delta_gradients_kernel<T, KP, false>, chunks, 512, smem, stream, a, w);
-    e = launch(shared, &gated_delta_gradients_kernel<T, KP, true>, chunks, 512, smem, stream, a, w);
-    if (e != cudaSuccess) return e;
+    constexpr int smem = sizeof(GradientsShared<KP>);
+    e = launch(gradients, &gated_delta_gradients_kernel<KP>, chunks, 512, smem, stream, a, w);
+    if (e != cudaSuccess || a.heads == a.k_heads) return e;
     const size_t values = static_cast<size_t>(a.batch) * a.length * a.k_heads * a.k_dim;
-    return launch(share, &gated_delta_share_kernel<T>, std::min<size_t>((values + 255) / 256, 148 * 8), 256, 0, stream, a, w,
+    return launch(share, &gated_delta_share_kernel, std::min<size_t>((values + 255) / 256, 148 * 8), 256, 0, stream, a, w,
                   values);
 #endif
 }
