@@ -5,7 +5,10 @@ the block's output, gates it, adds it to the residual stream and makes the next 
 ``rotate=True`` that input is Hadamard-rotated in the same pass, as the input of a quantised projection is; the
 projections' weights are rotated once to match, so the model's function stays the same.
 
-    python examples/recurrent_lm.py [--steps N] [--dim D] [--layers L]
+With ``--mixer delta`` a block's recurrence is the gated delta rule instead: queries and keys of length one (``qk_norm``,
+which also turns them by their positions) read and write a state of keys by values per head (``gated_delta``).
+
+    python examples/recurrent_lm.py [--steps N] [--dim D] [--layers L] [--mixer scan|delta]
 
 needs a CUDA device and the built library.
 """
@@ -42,17 +45,49 @@ class RecurrentBlock(torch.nn.Module):
         h, state = torch_ops.gated_scan(x, r, i, self.decay, initial_state=state, offsets=offsets)
         return self.outward(h), state
 
-    def step(self, u, pool, slots):
+    def step(self, u, pool, slots, positions):
         x, r, i = self.inward(u).split(self.dim, dim=-1)
         return self.outward(torch_ops.gated_scan_step(pool, x, r, i, self.decay, slots=slots))
 
 
+class DeltaBlock(torch.nn.Module):
+    """u -> y: one projection to queries, keys, values and both gates, the delta rule, one projection back."""
+
+    def __init__(self, dim, dtype, head=32):
+        super().__init__()
+        self.heads, self.k_heads, self.head = dim // head, max(1, dim // head // 2), head
+        self.widths = [self.k_heads * head, self.k_heads * head, dim, self.heads, self.heads]
+        self.inward = torch.nn.Linear(dim, sum(self.widths), bias=False, dtype=dtype)
+        self.outward = torch.nn.Linear(dim, dim, bias=False, dtype=dtype)
+        self.decay = torch.nn.Parameter(torch.linspace(-6.0, -3.0, self.heads))
+        self.post_weight = torch.nn.Parameter(torch.ones(dim))
+        self.gate = torch.nn.Parameter(torch.full((dim,), 0.5, dtype=dtype))
+        self.register_buffer("frequencies", 100.0 ** -torch.linspace(0, 1, head // 4))
+
+    def _project(self, u, positions):
+        q, k, v, decay, beta = self.inward(u).split(self.widths, dim=-1)
+        q, k, v = (t.unflatten(-1, (-1, self.head)) for t in (q, k, v))
+        q, k = torch_ops.qk_norm(q, k, norm="l2", positions=positions, frequencies=self.frequencies)
+        log_decay = -torch.nn.functional.softplus(decay.float() + self.decay)
+        return q, k, v, log_decay, torch.sigmoid(beta.float())
+
+    def forward(self, u, state=None, offsets=None):
+        positions = torch.arange(u.shape[-2], dtype=torch.int32, device=u.device)
+        if offsets is not None:  # counted from each sequence's start
+            positions -= torch.repeat_interleave(offsets[:-1], offsets.diff(), output_size=u.shape[-2])
+        o, state = torch_ops.gated_delta(*self._project(u, positions), initial_state=state, offsets=offsets)
+        return self.outward(o.flatten(-2)), state
+
+    def step(self, u, pool, slots, positions):
+        return self.outward(torch_ops.gated_delta_step(pool, *self._project(u, positions), slots=slots).flatten(-2))
+
+
 class RecurrentLM(torch.nn.Module):
-    def __init__(self, vocabulary, dim, layers, dtype=torch.bfloat16):
+    def __init__(self, vocabulary, dim, layers, dtype=torch.bfloat16, block=RecurrentBlock):
         super().__init__()
         self.dtype, self.rotate = dtype, False
         self.embedding = torch.nn.Embedding(vocabulary, dim)
-        self.blocks = torch.nn.ModuleList(RecurrentBlock(dim, dtype) for _ in range(layers))
+        self.blocks = torch.nn.ModuleList(block(dim, dtype) for _ in range(layers))
         # the norm before block k, and the last one before the head
         self.norms = torch.nn.ParameterList(torch.nn.Parameter(torch.ones(dim)) for _ in range(layers + 1))
         self.head = torch.nn.Linear(dim, vocabulary, bias=False, dtype=dtype)
@@ -77,9 +112,10 @@ class RecurrentLM(torch.nn.Module):
         return self._run(tokens, mixer), states
 
     @torch.no_grad()
-    def step(self, tokens, pools, slots=None):
-        """Logits of one token per request; the states in `pools` (one per layer) move on."""
-        return self._run(tokens, lambda k, block, u: block.step(u, pools[k], slots))
+    def step(self, tokens, pools, slots=None, positions=None):
+        """Logits of one token per request; the states in `pools` (one per layer) move on.  `positions`: of the tokens in
+        their sequences, for blocks that use them."""
+        return self._run(tokens, lambda k, block, u: block.step(u, pools[k], slots, positions))
 
     @torch.no_grad()
     def rotate_inputs(self):
@@ -94,10 +130,12 @@ def main(argv=None):
     p.add_argument("--steps", type=int, default=60)
     p.add_argument("--dim", type=int, default=256)
     p.add_argument("--layers", type=int, default=2)
+    p.add_argument("--mixer", choices=("scan", "delta"), default="scan")
     args = p.parse_args(argv)
     device, vocabulary = torch.device("cuda"), 64
     torch.manual_seed(0)
-    model = RecurrentLM(vocabulary, args.dim, args.layers).to(device)
+    block = DeltaBlock if args.mixer == "delta" else RecurrentBlock
+    model = RecurrentLM(vocabulary, args.dim, args.layers, block=block).to(device)
     optimizer = torch.optim.AdamW(model.parameters(), lr=3e-3)
 
     # counting with a stride that each sequence keeps: the next token needs the two before it
@@ -125,13 +163,13 @@ def main(argv=None):
         offsets = torch.tensor([0, *torch.tensor(lengths).cumsum(0).tolist()], dtype=torch.int32, device=device)
         logits, states = model(packed, offsets)
         slots = torch.tensor([4, 1, 2], dtype=torch.int32, device=device)
-        pools = [torch.zeros(6, args.dim, device=device) for _ in states]
+        pools = [torch.zeros(6, *state.shape[1:], device=device) for state in states]
         for pool, state in zip(pools, states):
             pool[slots.long()] = state
         worst = 0.0
         for t in range(8):
             given = torch.stack([tokens[k, n + t] for k, n in enumerate(lengths)])
-            step = model.step(given, pools, slots)
+            step = model.step(given, pools, slots, torch.tensor(lengths, dtype=torch.int32, device=device) + t)
             for k, n in enumerate(lengths):
                 whole, _ = model(tokens[k:k + 1, :n + t + 1])
                 worst = max(worst, float((whole[0, -1].float() - step[k].float()).abs().max()))
