@@ -73,12 +73,14 @@ struct TcShared {
 // ---- prepare ------------------------------------------------------------------------------------
 // The tiles of a chunk, a CTA for each key head: q and k (and, backward, dO of its heads) swizzled, and for each head of
 // its group L beta, (backward: beta L,) and P as two pieces each, beta folded into P's columns forward.  q k^T and k k^T
-// stay in registers for the group.  L is solved column by column, two threads a column.
+// stay in registers for the group.  L comes block by block of 16 rows, from the inverses of the blocks on the diagonal.
+// What leaves by bulk copies is read while the next step computes, and v of the next head comes in meanwhile.
 
 template <typename T, int KP, bool BACKWARD>
 struct TcPrepareShared {
     // P leaves before L is there; fp16's rows, transposed, need more
-    static constexpr int kSquareTiles = BACKWARD && kInput<T> == 2 ? 6 : 4;
+    static constexpr int kSquareTiles = !BACKWARD ? 2 : kInput<T> == 2 ? 6 : 4;
+    static constexpr int kBelow = C - 16, kPitchBelow = kBelow + 8;
     static constexpr int kRowTile = 2 * tc::kPanel;              // 64 tokens by up to 128 columns of v
     static constexpr int kRowTiles = 1 + (BACKWARD ? kInput<T> : 0);
     static_assert(kRowTiles * kRowTile <= kSquareTiles * tc::kPanel, "transposed rows fit where L and P go");
@@ -87,7 +89,7 @@ struct TcPrepareShared {
         alignas(1024) unsigned char rows[kRowTiles][kRowTile];   // v, and dO's pieces
         struct {
             alignas(16) float m[C][C + 4];                       // M
-            alignas(16) __nv_bfloat16 scaled[2 * C * kPitchC];   // M beta, two pieces
+            alignas(16) __nv_bfloat16 scaled[2 * kBelow * kPitchBelow];  // M beta's blocks below the diagonal, two pieces
             alignas(16) __nv_bfloat16 inverse[2 * C * 24];       // of the 16 x 16 blocks of I + M beta on its diagonal
         } pairs;
     };
@@ -96,7 +98,11 @@ struct TcPrepareShared {
         alignas(1024) unsigned char squares[kSquareTiles][tc::kPanel];
     };
     alignas(16) float factors[kTcFactors][C];
+    double ends[2];                                              // of two warps' sums of log decays
 };
+// As many CTAs an SM as shared memory allows, up to four: what registers leave to each.
+template <typename T, int KP, bool BACKWARD>
+constexpr int kPrepareCtas = sizeof(TcPrepareShared<T, KP, BACKWARD>) <= 55 * 1024 ? 4 : 3;
 
 // Rows of a tensor as NI swizzled pieces (one: the 16-bit values themselves), `width` (64 or 128) columns, zeros behind
 // the last row and column.
@@ -160,13 +166,16 @@ CUBF_DEV void swizzled_b(uint32_t tile, int n, int k, int panel, int lane, uint3
 }
 
 template <typename T, int KP, bool BACKWARD>
-__global__ void __launch_bounds__(128, 3) gated_delta_tc_prepare_kernel(GatedDeltaArgs a, Places w, bool wide_q, bool wide_v, bool wide_d) {
+__global__ void __launch_bounds__(128, kPrepareCtas<T, KP, BACKWARD>)
+    gated_delta_tc_prepare_kernel(GatedDeltaArgs a, Places w, bool wide_q, bool wide_v, bool wide_d) {
     constexpr int NI = kInput<T>, kOperand = TcTiles<T, KP>::kOperand;
     using Shared = TcPrepareShared<T, KP, BACKWARD>;
     extern __shared__ __align__(1024) unsigned char aligned_raw[];
     Shared& sm = *reinterpret_cast<Shared*>(aligned_raw);
     pdl_begin();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // the blocks of a triangle that a warp takes, other ones in the CTAs beside it
+    const int part = (warp + blockIdx.x + blockIdx.x / 148) & 3;
     const int slot = blockIdx.x / a.k_heads, k_head = blockIdx.x % a.k_heads;
     const int group = a.heads / a.k_heads;
     const Span s = span_of(a, slot);
@@ -176,10 +185,14 @@ __global__ void __launch_bounds__(128, 3) gated_delta_tc_prepare_kernel(GatedDel
         return static_cast<const T*>(t.p) + s.row * t.batch + static_cast<size_t>(s.first) * t.token +
                static_cast<size_t>(head) * t.head;
     };
-    if ((wide_v && tid < s.tokens) || (BACKWARD && wide_d && tid >= C && tid - C < s.tokens)) {
-        const HeadTensor& t = tid < C ? a.v : a.d_o;
-        for (int g = 0; g < group; ++g)
-            prefetch_l2(row_of(t, k_head * group + g) + static_cast<size_t>(tid % C) * t.token, static_cast<uint32_t>(a.v_dim * sizeof(T)));
+    if (tid % C < s.tokens) {            // by lines: prefetches of whole rows queue up before the copies of q and k
+        auto prefetch = [&](const T* p) {
+            for (int at = tid / C * 64; at < a.v_dim; at += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + at));
+        };
+        for (int g = 0; g < group; ++g) {
+            prefetch(row_of(a.v, k_head * group + g) + static_cast<size_t>(tid % C) * a.v.token);
+            if (BACKWARD) prefetch(row_of(a.d_o, k_head * group + g) + static_cast<size_t>(tid % C) * a.d_o.token);
+        }
     }
     auto gates = [&](int head, float& log_decay, float& beta) {  // of token `tid`
         log_decay = beta = 0.f;
@@ -203,55 +216,47 @@ __global__ void __launch_bounds__(128, 3) gated_delta_tc_prepare_kernel(GatedDel
                        2 * kOperand);
         tc::bulk_commit();
     }
-    // rows 16 warp .. + 15 of k k^T and q k^T, up to the diagonal
-    float kk[8][4] = {}, qk[8][4] = {};
+    // The ten 16 x 16 blocks of k k^T and q k^T up to the diagonal, two or three a warp: the rows 1 to 3 of blocks to the warps
+    // of their numbers, but for the first of row 3, which is with row 0.
+    auto row_block = [&](int n) { return part == 0 ? 3 * n : part; };
+    auto col_block = [&](int n) { return part == 0 ? 0 : part == 3 ? n + 1 : n; };
+    const int blocks = part < 2 ? 2 : 3;
+    float kk[6][4] = {}, qk[6][4] = {};
     const uint32_t tq = smem_addr(sm.qk), tk = tq + tc::kPanel;
+#pragma unroll 2
     for (int ks = 0; ks < KP / 16; ++ks) {
         uint32_t ak[NI][4], aq[NI][4];
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            swizzled_a(tk + i * KP * 256, 16 * warp, 16 * ks, kQkPanel, lane, ak[i]);
-            swizzled_a(tq + i * KP * 256, 16 * warp, 16 * ks, kQkPanel, lane, aq[i]);
-        }
+        for (int n = 0; n < 3; ++n) {
+            if (n >= blocks) break;
+            if (n == 0 || part == 0) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            if (t <= warp) {
-                uint32_t b[NI][1][4];
-#pragma unroll
-                for (int i = 0; i < NI; ++i) swizzled_b(tk + i * KP * 256, 16 * t, 16 * ks, kQkPanel, lane, b[i][0]);
-                products<3, NI, NI, 2>(kk + 2 * t, ak, b);
-                products<3, NI, NI, 2>(qk + 2 * t, aq, b);
+                for (int i = 0; i < NI; ++i) {
+                    swizzled_a(tk + i * KP * 256, 16 * row_block(n), 16 * ks, kQkPanel, lane, ak[i]);
+                    swizzled_a(tq + i * KP * 256, 16 * row_block(n), 16 * ks, kQkPanel, lane, aq[i]);
+                }
             }
+            uint32_t b[NI][1][4];
+#pragma unroll
+            for (int i = 0; i < NI; ++i) swizzled_b(tk + i * KP * 256, 16 * col_block(n), 16 * ks, kQkPanel, lane, b[i][0]);
+            products<3, NI, NI, 2>(kk + 2 * n, ak, b);
+            products<3, NI, NI, 2>(qk + 2 * n, aq, b);
         }
     }
     if (tid == 0) tc::bulk_read();
     __syncthreads();                     // q and k have left: their place is M's now
-    for (int g = 0; g < group; ++g) {
-        const int head = k_head * group + g;
-        const size_t place = static_cast<size_t>(slot) * a.heads + head;
-        // v, and dO, to a row for each column
+    // v, and dO, of a head
+    auto fetch = [&](int head) {
         load_swizzled<T, 1>(row_of(a.v, head), a.v.token, s.tokens, a.v_dim, w.v_rows, wide_v, sm.rows[0], tc::kPanel, tid, 128);
         if constexpr (BACKWARD)
             load_swizzled<T, NI>(row_of(a.d_o, head), a.d_o.token, s.tokens, a.v_dim, w.v_rows, wide_d, sm.rows[1], tc::kPanel, tid,
                                  128);
         copies_commit();
-        copies_wait<0>();
-        __syncthreads();
-        const uint32_t tile = static_cast<uint32_t>(w.v_rows * 128);
-        transpose_swizzled(sm.rows[0], sm.columns[0], w.v_rows, warp, lane);
-        if (BACKWARD)
-            for (int n = 0; n < NI; ++n)
-                transpose_swizzled(sm.rows[1] + n * tile, sm.columns[1] + n * tile, w.v_rows, warp, lane);
-        tc::fence_async();
-        __syncthreads();
-        if (tid == 0) {
-            tc::bulk_store(work + w.values + place * tile, smem_addr(sm.columns[0]), tile);
-            if (BACKWARD) tc::bulk_store(work + w.rows + place * NI * tile, smem_addr(sm.columns[1]), NI * tile);
-            tc::bulk_commit();
-            tc::bulk_read();
-        }
-        __syncthreads();
-        double* const ends = reinterpret_cast<double*>(sm.pairs.inverse);  // of the two warps' sums
+    };
+    fetch(k_head * group);
+    for (int g = 0; g < group; ++g) {
+        const int head = k_head * group + g;
+        const size_t place = static_cast<size_t>(slot) * a.heads + head;
         double sum = 0;
         if (tid < C) {                   // running sums of the log decays, in 64 bits
             sum = log_decay < kLeast ? kLeast : log_decay;  // NaN stays
@@ -260,12 +265,14 @@ __global__ void __launch_bounds__(128, 3) gated_delta_tc_prepare_kernel(GatedDel
                 const double other = __shfl_up_sync(0xffffffffu, sum, d);
                 if (lane >= d) sum += other;
             }
-            if (lane == 31) ends[warp] = sum;
+            if (lane == 31) sm.ends[warp] = sum;
         }
+        if (tid == 0) tc::bulk_read();   // the head before has left
+        copies_wait<0>();
         __syncthreads();
         if (tid < C) {
-            if (warp == 1) sum += ends[0];
-            const double all = ends[0] + ends[1];
+            if (warp == 1) sum += sm.ends[0];
+            const double all = sm.ends[0] + sm.ends[1];
             const double log2 = sum * 1.4426950408889634074;
             const float high = static_cast<float>(log2);
             const float from_start = expf(static_cast<float>(sum)), to_end = expf(static_cast<float>(all - sum));
@@ -279,34 +286,63 @@ __global__ void __launch_bounds__(128, 3) gated_delta_tc_prepare_kernel(GatedDel
             sm.factors[kSumLow][tid] = static_cast<float>(log2 - high);
             if (g + 1 < group) gates(head + 1, log_decay, beta);
         }
+        // to a row for each column
+        const uint32_t tile = static_cast<uint32_t>(w.v_rows * 128);
+        transpose_swizzled(sm.rows[0], sm.columns[0], w.v_rows, warp, lane);
+        if (BACKWARD)
+            for (int n = 0; n < NI; ++n)
+                transpose_swizzled(sm.rows[1] + n * tile, sm.columns[1] + n * tile, w.v_rows, warp, lane);
+        tc::fence_async();
         __syncthreads();
+        if (tid == 0) {
+            tc::bulk_store(work + w.values + place * tile, smem_addr(sm.columns[0]), tile);
+            if (BACKWARD) tc::bulk_store(work + w.rows + place * NI * tile, smem_addr(sm.columns[1]), NI * tile);
+            tc::bulk_commit();
+        }
         const float *bf = sm.factors[kBeta], *gh = sm.factors[kSumHigh], *gl = sm.factors[kSumLow];
-        // P and M; the blocks above the diagonal are never read
+        // M and P; the blocks above the diagonal are never read
+        uint32_t p[3][2][2][2];
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            if (t > 2 * warp + 1) continue;
+        for (int n = 0; n < 3; ++n) {
+            if (n >= blocks) break;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int i = 16 * warp + lane / 4 + 8 * h, j = 8 * t + lane % 4 * 2;
-                float p[2], m[2];
+            for (int t = 0; t < 2; ++t) {
+                const int j = 16 * col_block(n) + 8 * t + lane % 4 * 2;
+                const float2 high = *reinterpret_cast<const float2*>(gh + j), low = *reinterpret_cast<const float2*>(gl + j);
+                const float2 b = *reinterpret_cast<const float2*>(bf + j);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float d = exp2f((gh[i] - gh[j + e]) + (gl[i] - gl[j + e]));
-                    p[e] = j + e <= i ? d * qk[t][2 * h + e] * a.scale : 0.f;
-                    m[e] = j + e < i ? d * kk[t][2 * h + e] : 0.f;
-                    if (!BACKWARD) p[e] *= bf[j + e];
+                for (int h = 0; h < 2; ++h) {
+                    const int i = 16 * row_block(n) + lane / 4 + 8 * h;
+                    const float dx = j <= i ? exp2f((gh[i] - high.x) + (gl[i] - low.x)) : 0.f;
+                    const float dy = j + 1 <= i ? exp2f((gh[i] - high.y) + (gl[i] - low.y)) : 0.f;
+                    const float mx = j < i ? dx * kk[2 * n + t][2 * h] : 0.f, my = j + 1 < i ? dy * kk[2 * n + t][2 * h + 1] : 0.f;
+                    *reinterpret_cast<float2*>(&sm.pairs.m[i][j]) = make_float2(mx, my);
+                    float px = j <= i ? dx * qk[2 * n + t][2 * h] * a.scale : 0.f;
+                    float py = j + 1 <= i ? dy * qk[2 * n + t][2 * h + 1] * a.scale : 0.f;
+                    if (!BACKWARD) px *= b.x, py *= b.y;
+                    pieces<2>(px, py, p[n][t][h]);
+                    if (row_block(n) == col_block(n)) continue;
+                    uint32_t f[2];
+                    pieces<2>(mx * b.x, my * b.y, f);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        *reinterpret_cast<uint32_t*>(sm.pairs.scaled + (e * Shared::kBelow + i - 16) * Shared::kPitchBelow + j) = f[e];
                 }
-                *reinterpret_cast<float2*>(&sm.pairs.m[i][j]) = make_float2(m[0], m[1]);
-                uint32_t f[2];
-                pieces<2>(m[0] * bf[j], m[1] * bf[j + 1], f);
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-                    *reinterpret_cast<uint32_t*>(sm.pairs.scaled + (n * C + i) * kPitchC + j) = f[n];
-                uint32_t x[2];
-                pieces<2>(p[0], p[1], x);
-                *reinterpret_cast<uint32_t*>(sm.squares[0] + tc::swizzled(i, j)) = x[0];
-                *reinterpret_cast<uint32_t*>(sm.squares[1] + tc::swizzled(i, j)) = x[1];
             }
+        }
+        if (tid == 0) tc::bulk_read();
+        __syncthreads();                 // v's columns have left
+#pragma unroll
+        for (int n = 0; n < 3; ++n) {
+            if (n >= blocks) break;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t to = tc::swizzled(16 * row_block(n) + lane / 4 + 8 * h, 16 * col_block(n) + 8 * t + lane % 4 * 2);
+                    *reinterpret_cast<uint32_t*>(sm.squares[0] + to) = p[n][t][h][0];
+                    *reinterpret_cast<uint32_t*>(sm.squares[1] + to) = p[n][t][h][1];
+                }
         }
         tc::fence_async();
         __syncthreads();
@@ -317,7 +353,7 @@ __global__ void __launch_bounds__(128, 3) gated_delta_tc_prepare_kernel(GatedDel
             tc::bulk_commit();
         }
         {   // the inverse of the warp's block on the diagonal, a lane a column, row by row
-            const int col = lane & 15, base = 16 * warp;
+            const int col = lane & 15, base = 16 * part;
             float t[16];                 // times beta
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
@@ -346,13 +382,13 @@ __global__ void __launch_bounds__(128, 3) gated_delta_tc_prepare_kernel(GatedDel
         __syncthreads();
         {   // 16 columns of L a warp, transposed, block by block of 16 rows: L_i = (I + M beta)_ii^-1 (M_i - sum over j < i
             // of (M beta)_ij L_j), products at level 2
-            const Tile<kPitchC, C * kPitchC> scaled{smem_addr(sm.pairs.scaled)};
+            const Tile<Shared::kPitchBelow, Shared::kBelow * Shared::kPitchBelow> scaled{smem_addr(sm.pairs.scaled)};
             const Tile<24, C * 24> inverse{smem_addr(sm.pairs.inverse)};
             uint32_t done[3][2][4];      // rows of L before, negated, as operands
-            const int c0 = 16 * warp + lane / 4;
+            const int c0 = 16 * part + lane / 4;
 #pragma unroll
             for (int step = 0; step < 4; ++step) {
-                const int block = warp + step;
+                const int block = part + step;
                 if (block > 3) break;
                 float x[2][4];
 #pragma unroll
@@ -364,7 +400,7 @@ __global__ void __launch_bounds__(128, 3) gated_delta_tc_prepare_kernel(GatedDel
                 for (int j = 0; j < step; ++j) {
                     uint32_t b[2][1][4];
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) scaled.b_rows(n, 16 * block, 16 * (warp + j), lane, b[n][0]);
+                    for (int n = 0; n < 2; ++n) scaled.b_rows(n, 16 * (block - 1), 16 * (part + j), lane, b[n][0]);
                     products<2, 2, 2, 2>(x, done[j], b);
                 }
                 uint32_t f[2][4], b[2][1][4];
@@ -400,13 +436,10 @@ __global__ void __launch_bounds__(128, 3) gated_delta_tc_prepare_kernel(GatedDel
             tc::bulk_store(matrices, smem_addr(sm.squares), L_TILES * tc::kPanel);
             tc::bulk_store(work + w.factors + place * sizeof(sm.factors), smem_addr(sm.factors), sizeof(sm.factors));
             tc::bulk_commit();
-            if (g + 1 < group)
-                tc::bulk_read();
-            else
-                tc::bulk_done();
         }
-        __syncthreads();
+        if (g + 1 < group) fetch(head + 1);
     }
+    if (tid == 0) tc::bulk_done();
 }
 
 // One chain's place in the grid: a sequence of a head, or a segment of one.
