@@ -1320,7 +1320,7 @@ __global__ void __launch_bounds__(2 * KP) gated_delta_join_kernel(GatedDeltaArgs
 // then, with the pairs' coefficients Cq = D o dP and Cm = D o dM written as one tile of 128 rows,
 //   [Cq; Cm] k      and, the tile turned,  [.; Cq^T q + Cm^T k].
 // Bounded by memory: the kept S and dS, 64 KB each, R and W, 32 KB each, and the tiles of q, k and dO per chunk and head.
-constexpr int kGradientThreads = kTcCompute + 32;
+constexpr int kGradientThreads = kTcThreads;  // three warps only leave their registers to the computing ones
 
 template <typename T, int KP>
 struct GradientShared {
@@ -1532,52 +1532,57 @@ struct Gradients {
             if (NI == 2) inner(g, states);
             wait(sm.done[kPairsDone], phase);
             {
-                uint32_t x[32], kk[32];
-                tc::load<32>(at + kPM + 32 * half, x);
-                tc::load<32>(at + kQK + 32 * half, kk);
-                tc::wait_load();
                 const float high = sm.factors[kSumHigh][i], low = sm.factors[kSumLow][i];
                 const float scale = key ? -sm.factors[kBeta][i] : a.scale;
-                if (key && i / 32 == half) {
-                    float d = 0.f;                               // dbeta = W . R of the token itself
+                if (NI == 2) wait(sm.done[kQsDone], phase);      // dO's place is free
+                float pair[32], sum = 0.f;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) d = j == i % 32 ? __uint_as_float(x[j]) : d;
-                    sm.beta[i] = d;
-                }
-                float pair[32], c[32], sum = 0.f;
-                if ((quarter & 1) == 0 && half == 1) {           // all behind their row
+                for (int part = 0; part < 2; ++part) {           // 16 columns at a time: all 32 would not stay in registers
+                    const int from = 32 * half + 16 * part;
+                    uint32_t x[16], kk[16];
+                    tc::load<16>(at + kPM + from, x);
+                    tc::load<16>(at + kQK + from, kk);
+                    tc::wait_load();
+                    if (key && i / 16 == 2 * half + part) {
+                        float d = 0.f;                           // dbeta = W . R of the token itself
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) pair[j] = c[j] = 0.f;
-                } else {
+                        for (int j = 0; j < 16; ++j) d = j == i % 16 ? __uint_as_float(x[j]) : d;
+                        sm.beta[i] = d;
+                    }
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        const float4 h = *reinterpret_cast<const float4*>(&sm.factors[kSumHigh][32 * half + 4 * q]);
-                        const float4 l = *reinterpret_cast<const float4*>(&sm.factors[kSumLow][32 * half + 4 * q]);
-                        const float4 b = *reinterpret_cast<const float4*>(&sm.factors[kBeta][32 * half + 4 * q]);
-                        const float hs[4] = {h.x, h.y, h.z, h.w}, ls[4] = {l.x, l.y, l.z, l.w}, bs[4] = {b.x, b.y, b.z, b.w};
+                    for (int q = 0; q < 2; ++q) {
+                        float c[8];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int j = 4 * q + e, at_j = 32 * half + j;
-                            const bool in = key ? at_j < i : at_j <= i;
-                            const float d = exp2f((high - hs[e]) + (low - ls[e])) * scale * bs[e] * __uint_as_float(x[j]);
-                            c[j] = in ? d : 0.f;
-                            pair[j] = in ? d * __uint_as_float(kk[j]) : 0.f;
-                            sum += pair[j];
+                        for (int e = 0; e < 8; ++e) c[e] = pair[16 * part + 8 * q + e] = 0.f;
+                        if ((quarter & 1) == 1 || half == 0) {   // the others are all behind their row
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                const int first = from + 8 * q + 4 * r;
+                                const float4 h = *reinterpret_cast<const float4*>(&sm.factors[kSumHigh][first]);
+                                const float4 l = *reinterpret_cast<const float4*>(&sm.factors[kSumLow][first]);
+                                const float4 b = *reinterpret_cast<const float4*>(&sm.factors[kBeta][first]);
+                                const float hs[4] = {h.x, h.y, h.z, h.w}, ls[4] = {l.x, l.y, l.z, l.w}, bs[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const int j = 8 * q + 4 * r + e, at_j = from + j;
+                                    const bool in = key ? at_j < i : at_j <= i;
+                                    const float d = exp2f((high - hs[e]) + (low - ls[e])) * scale * bs[e] * __uint_as_float(x[j]);
+                                    c[4 * r + e] = in ? d : 0.f;
+                                    pair[16 * part + j] = in ? d * __uint_as_float(kk[j]) : 0.f;
+                                    sum += pair[16 * part + j];
+                                }
+                            }
                         }
+                        uint32_t f[4][2];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) pieces<2>(c[2 * e], c[2 * e + 1], f[e]);
+                        const uint32_t to = row * 128 + (((4 * half + 2 * part + q) ^ (row & 7)) << 4);
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+                            *reinterpret_cast<uint4*>(sm.pair_tile(n, w.v_rows) + to) = make_uint4(f[0][n], f[1][n], f[2][n], f[3][n]);
                     }
                 }
                 sm.row[half][key][i] = sum;
-                if (NI == 2) wait(sm.done[kQsDone], phase);      // dO's place is free
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t f[4][2];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) pieces<2>(c[8 * q + 2 * e], c[8 * q + 2 * e + 1], f[e]);
-                    const uint32_t to = row * 128 + (((4 * half + q) ^ (row & 7)) << 4);
-#pragma unroll
-                    for (int n = 0; n < 2; ++n)
-                        *reinterpret_cast<uint4*>(sm.pair_tile(n, w.v_rows) + to) = make_uint4(f[0][n], f[1][n], f[2][n], f[3][n]);
-                }
                 tc::fence_async();
                 tc::fence_before();
                 report(sm.ready);
@@ -1776,10 +1781,13 @@ __global__ void __launch_bounds__(kGradientThreads, 1) gated_delta_tc_gradients_
     tc::fence_after();
     Gradients<T, KP> run{a, w, sm, s, slot, k_head, a.heads / a.k_heads, tid, tid & 31, warp, __shfl_sync(0xffffffffu, sm.base, 0),
                          (smem_addr(&sm) & 1023u) != 0};
-    if (warp == kTcCompute / 32)
-        run.issue();
-    else
+    if (warp >= kTcCompute / 32) {
+        fewer_registers<56>();
+        if (warp == kTcCompute / 32) run.issue();
+    } else {
+        more_registers<224>();
         run.compute();
+    }
     tc::fence_before();
     __syncthreads();
     if (warp == kTcCompute / 32) {
