@@ -1412,6 +1412,22 @@ struct Gradients {
         }
         __syncwarp();
     }
+    // What the next head reads, or the first one of the CTA a resident wave later, to L2 while this head computes.
+    CUBF_DEV void prefetch_next(int g) const {
+        const unsigned next = blockIdx.x + 148;
+        const uint32_t tile = static_cast<uint32_t>(w.v_rows * 128), states = 2 * static_cast<uint32_t>(w.state_piece);
+        if (g + 1 == group && next >= gridDim.x) return;
+        const size_t at = g + 1 < group ? place(g + 1) : static_cast<size_t>(next) * group;
+        if (tc::elect()) {
+            if (g + 1 == group) prefetch_l2(work(w.packed) + static_cast<size_t>(next) * 2 * kOperand, 2 * kOperand);
+            prefetch_l2(work(w.rows) + at * NI * tile, NI * tile);
+            prefetch_l2(work(w.d_writes) + at * 2 * tile, 2 * tile);
+            prefetch_l2(work(w.errors) + at * 2 * tile, 2 * tile);
+            prefetch_l2(work(w.states) + at * states, states);
+            prefetch_l2(work(w.d_states) + at * states, states);
+        }
+        __syncwarp();
+    }
     // Where piece n of [dO; W; R] begins; with bf16 dO has one piece, and what lies before W's second is not of use.
     CUBF_DEV uint32_t stack(int n) const {
         return smem_addr(sm.tiles) + static_cast<uint32_t>(n * (NI + 1) * w.v_rows * 128);
@@ -1444,6 +1460,7 @@ struct Gradients {
             for (int n = 0; n < Shared::kBuffers; ++n) bring(n);
             wait(sm.full, phase);
             if (failed) break;
+            prefetch_next(g);
             if (tc::elect()) {
 #pragma unroll
                 for (int i = 0; i < NI; ++i)
