@@ -104,6 +104,13 @@ struct TcPrepareShared {
 template <typename T, int KP, bool BACKWARD>
 constexpr int kPrepareCtas = sizeof(TcPrepareShared<T, KP, BACKWARD>) <= 55 * 1024 ? 4 : 3;
 
+// 2^x with exp2f's error, but zero below 2^-126, as no decay of that size is told from none.
+CUBF_DEV float exp2_flushed(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Rows of a tensor as NI swizzled pieces (one: the 16-bit values themselves), `width` (64 or 128) columns, zeros behind
 // the last row and column.
 template <typename T, int NI>
@@ -313,8 +320,8 @@ __global__ void __launch_bounds__(128, kPrepareCtas<T, KP, BACKWARD>)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int i = 16 * row_block(n) + lane / 4 + 8 * h;
-                    const float dx = j <= i ? exp2f((gh[i] - high.x) + (gl[i] - low.x)) : 0.f;
-                    const float dy = j + 1 <= i ? exp2f((gh[i] - high.y) + (gl[i] - low.y)) : 0.f;
+                    const float dx = j <= i ? exp2_flushed((gh[i] - high.x) + (gl[i] - low.x)) : 0.f;
+                    const float dy = j + 1 <= i ? exp2_flushed((gh[i] - high.y) + (gl[i] - low.y)) : 0.f;
                     const float mx = j < i ? dx * kk[2 * n + t][2 * h] : 0.f, my = j + 1 < i ? dy * kk[2 * n + t][2 * h + 1] : 0.f;
                     *reinterpret_cast<float2*>(&sm.pairs.m[i][j]) = make_float2(mx, my);
                     float px = j <= i ? dx * qk[2 * n + t][2 * h] * a.scale : 0.f;
@@ -1583,7 +1590,7 @@ struct Gradients {
                                 for (int e = 0; e < 4; ++e) {
                                     const int j = 8 * q + 4 * r + e, at_j = from + j;
                                     const bool in = key ? at_j < i : at_j <= i;
-                                    const float d = exp2f((high - hs[e]) + (low - ls[e])) * scale * bs[e] * __uint_as_float(x[j]);
+                                    const float d = exp2_flushed((high - hs[e]) + (low - ls[e])) * scale * bs[e] * __uint_as_float(x[j]);
                                     c[4 * r + e] = in ? d : 0.f;
                                     pair[16 * part + j] = in ? d * __uint_as_float(kk[j]) : 0.f;
                                     sum += pair[16 * part + j];
