@@ -11,11 +11,13 @@
 // chain, in one launch, then `gradients` (a CTA per chunk and head); where
 // heads share keys, `share` adds their gradients up.
 //
-// Every operand is three bf16 pieces and every product six (mma_split.cuh):
-// an fp32 product but for the tensor pipe's sums, which cut what they add to
-// the largest term's last bits: 1e-6 to 5e-6 of a result, measured against 64
-// bits.  Three pieces of these tiles would not fit beside an accumulator in
-// tensor memory, so this path stays on the register-fed tensor instructions.
+// Every operand is three bf16 pieces and every product six (mma_split.cuh),
+// added up in fp32 (products_rounded): 1.2e-7 to 2.3e-7 of a result against 64
+// bits, and 1e-6 to 5e-6 with one accumulator through all sums, which took 57
+// us for 65 (257 tokens, both chains).  Three pieces of these tiles would not
+// fit beside an accumulator in tensor memory, so this path stays on the
+// register-fed tensor instructions, and bounded by the latency of a chunk's
+// three products in one warp: 9 us a chunk of K = 64 forward, 13 of K = 128.
 #pragma once
 
 #include <algorithm>
@@ -175,8 +177,8 @@ __global__ void __launch_bounds__(128) gated_delta_prepare_kernel(GatedDeltaArgs
                 uint32_t b[kPieces][1][4];
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) tk.b_rows(i, 16 * t, 16 * ks, lane, b[i][0]);
-                products<3, kPieces, kPieces, 2>(kk + 2 * t, ak, b);
-                products<3, kPieces, kPieces, 2>(qk + 2 * t, aq, b);
+                products_rounded<3, kPieces, kPieces, 2>(kk + 2 * t, ak, b);
+                products_rounded<3, kPieces, kPieces, 2>(qk + 2 * t, aq, b);
             }
         }
     }
@@ -288,7 +290,7 @@ CUBF_DEV void onto_state(float (*d)[4], const uint32_t (&a)[kPieces][4], const O
             b.b_cols(i, 16 * ks, 32 * t, lane, f[i][0]);
             b.b_cols(i, 16 * ks, 32 * t + 16, lane, f[i][1]);
         }
-        products<kPieces, kPieces, kPieces, 4>(d + 4 * t, a, f);
+        products_rounded<kPieces, kPieces, kPieces, 4>(d + 4 * t, a, f);
     }
 }
 
@@ -411,14 +413,14 @@ CUBF_DEV void forward_chain(const GatedDeltaArgs& a, const Places& w, const Chai
                         k.b_rows(i, 32 * t, 16 * ks, lane, b[i][0]);
                         k.b_rows(i, 32 * t + 16, 16 * ks, lane, b[i][1]);
                     }
-                    products<kPieces, kPieces, kPieces, 4>(x + 4 * t, f3, b);
+                    products_rounded<kPieces, kPieces, kPieces, 4>(x + 4 * t, f3, b);
                     if (!KEEP) {
 #pragma unroll
                         for (int i = 0; i < kPieces; ++i) {
                             q.b_rows(i, 32 * t, 16 * ks, lane, b[i][0]);
                             q.b_rows(i, 32 * t + 16, 16 * ks, lane, b[i][1]);
                         }
-                        products<kPieces, kPieces, kPieces, 4>(o + 4 * t, f3, b);
+                        products_rounded<kPieces, kPieces, kPieces, 4>(o + 4 * t, f3, b);
                     }
                 }
             }
@@ -444,7 +446,7 @@ CUBF_DEV void forward_chain(const GatedDeltaArgs& a, const Places& w, const Chai
                     uint32_t b[kPieces][1][4];
 #pragma unroll
                     for (int i = 0; i < kPieces; ++i) solve.b_rows(i, 16 * t, 16 * ks, lane, b[i][0]);
-                    products<kPieces, kPieces, kPieces, 2>(x + 2 * t, f3, b);
+                    products_rounded<kPieces, kPieces, kPieces, 2>(x + 2 * t, f3, b);
                 }
             }
             if (KEEP)
@@ -469,7 +471,7 @@ CUBF_DEV void forward_chain(const GatedDeltaArgs& a, const Places& w, const Chai
                         uint32_t b[kPieces][1][4];
 #pragma unroll
                         for (int i = 0; i < kPieces; ++i) attention.b_rows(i, 16 * t, 16 * ks, lane, b[i][0]);
-                        products<kPieces, kPieces, kPieces, 2>(o + 2 * t, f2, b);
+                        products_rounded<kPieces, kPieces, kPieces, 2>(o + 2 * t, f2, b);
                     }
                 }
                 uint32_t f3[kPieces][4];
@@ -535,7 +537,7 @@ CUBF_DEV void backward_chain(const GatedDeltaArgs& a, const Places& w, const Cha
                         k.b_rows(i, 32 * t, 16 * ks, lane, b[i][0]);
                         k.b_rows(i, 32 * t + 16, 16 * ks, lane, b[i][1]);
                     }
-                    products<kPieces, kPieces, kPieces, 4>(x + 4 * t, f3, b);
+                    products_rounded<kPieces, kPieces, kPieces, 4>(x + 4 * t, f3, b);
                 }
             }
 #pragma unroll
@@ -564,7 +566,7 @@ CUBF_DEV void backward_chain(const GatedDeltaArgs& a, const Places& w, const Cha
                     uint32_t b[kPieces][1][4];
 #pragma unroll
                     for (int i = 0; i < kPieces; ++i) attention.b_cols(i, 16 * ks, 16 * t, lane, b[i][0]);
-                    products<kPieces, kPieces, kPieces, 2>(x + 2 * t, exact, b);
+                    products_rounded<kPieces, kPieces, kPieces, 2>(x + 2 * t, exact, b);
                 }
                 uint32_t f3[kPieces][4];
                 operand<kPieces>(d[0], d[1], f + 16 * ks, a.scale, lane, f3);
@@ -580,7 +582,7 @@ CUBF_DEV void backward_chain(const GatedDeltaArgs& a, const Places& w, const Cha
                     uint32_t b[kPieces][1][4];
 #pragma unroll
                     for (int i = 0; i < kPieces; ++i) solve.b_cols(i, 16 * ks, 16 * t, lane, b[i][0]);
-                    products<kPieces, kPieces, kPieces, 2>(x + 2 * t, f3, b);
+                    products_rounded<kPieces, kPieces, kPieces, 2>(x + 2 * t, f3, b);
                 }
             }
             rows_keep(reinterpret_cast<float*>(work + w.d_writes) + place * C * w.v_pitch, w.v_pitch, v, lane, x);
@@ -759,8 +761,8 @@ __global__ void __launch_bounds__(512) gated_delta_gradients_kernel(GatedDeltaAr
                 uint32_t b[kPieces][1][4];
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) tu.b_rows(i, 16 * cg, 16 * step, lane, b[i][0]);
-                products<kPieces, kPieces, kPieces, 2>(dp, ao, b);
-                products<kPieces, kPieces, kPieces, 2>(dm, az, b);
+                products_rounded<kPieces, kPieces, kPieces, 2>(dp, ao, b);
+                products_rounded<kPieces, kPieces, kPieces, 2>(dm, az, b);
             }
 #pragma unroll
             for (int t = 0; t < NT / 2; ++t) {
@@ -768,11 +770,11 @@ __global__ void __launch_bounds__(512) gated_delta_gradients_kernel(GatedDeltaAr
                 const int col = cg * (KP / 4) + 16 * t;
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) ts.b_cols(i, 16 * step, col, lane, b[i][0]);
-                products<kPieces, kPieces, kPieces, 2>(qs + 2 * t, ao, b);
-                products<kPieces, kPieces, kPieces, 2>(ks + 2 * t, az, b);
+                products_rounded<kPieces, kPieces, kPieces, 2>(qs + 2 * t, ao, b);
+                products_rounded<kPieces, kPieces, kPieces, 2>(ks + 2 * t, az, b);
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) td.b_cols(i, 16 * step, col, lane, b[i][0]);
-                products<kPieces, kPieces, kPieces, 2>(ku + 2 * t, au, b);
+                products_rounded<kPieces, kPieces, kPieces, 2>(ku + 2 * t, au, b);
             }
         }
         __syncthreads();
@@ -840,8 +842,8 @@ __global__ void __launch_bounds__(512) gated_delta_gradients_kernel(GatedDeltaAr
                 tk.a_rows(i, 16 * rb, 16 * step, lane, ak[i]);
                 tk.b_rows(i, 16 * cg, 16 * step, lane, b[i][0]);
             }
-            products<kPieces, kPieces, kPieces, 2>(qk, aq, b);
-            products<kPieces, kPieces, kPieces, 2>(kk, ak, b);
+            products_rounded<kPieces, kPieces, kPieces, 2>(qk, aq, b);
+            products_rounded<kPieces, kPieces, kPieces, 2>(kk, ak, b);
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -905,8 +907,8 @@ __global__ void __launch_bounds__(512) gated_delta_gradients_kernel(GatedDeltaAr
                 uint32_t b[kPieces][1][4];
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) tk.b_cols(i, 16 * step, cg * (KP / 4) + 16 * t, lane, b[i][0]);
-                products<kPieces, kPieces, kPieces, 2>(qs + 2 * t, f, b);
-                products<kPieces, kPieces, kPieces, 2>(ks + 2 * t, g, b);
+                products_rounded<kPieces, kPieces, kPieces, 2>(qs + 2 * t, f, b);
+                products_rounded<kPieces, kPieces, kPieces, 2>(ks + 2 * t, g, b);
             }
         }
         if (step >= rb) {  // columns rb: tokens from their own on
@@ -921,10 +923,10 @@ __global__ void __launch_bounds__(512) gated_delta_gradients_kernel(GatedDeltaAr
                 uint32_t b[kPieces][1][4];
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) tq.b_cols(i, 16 * step, cg * (KP / 4) + 16 * t, lane, b[i][0]);
-                products<kPieces, kPieces, kPieces, 2>(ks + 2 * t, f, b);
+                products_rounded<kPieces, kPieces, kPieces, 2>(ks + 2 * t, f, b);
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) tk.b_cols(i, 16 * step, cg * (KP / 4) + 16 * t, lane, b[i][0]);
-                products<kPieces, kPieces, kPieces, 2>(ks + 2 * t, g, b);
+                products_rounded<kPieces, kPieces, kPieces, 2>(ks + 2 * t, g, b);
             }
         }
     }

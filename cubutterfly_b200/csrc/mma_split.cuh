@@ -116,6 +116,27 @@ CUBF_DEV void products(float (*d)[4], const uint32_t (&a)[NA][4], const uint32_t
             }
 }
 
+// The same in full fp32: the tensor pipe cuts a sum's last bits at every step, always towards zero, so that an accumulator
+// that runs through all piece products of a long sum loses 2^-24 of itself at each.  Here the products of 16 terms are added
+// up by themselves, the smallest first, and go to the accumulator by an addition that rounds to nearest.
+template <int LEVEL, int NA, int NB, int NT>
+CUBF_DEV void products_rounded(float (*d)[4], const uint32_t (&a)[NA][4], const uint32_t (&b)[NB][NT / 2][4]) {
+    float sum[NT][4] = {};
+#pragma unroll
+    for (int size = LEVEL - 1; size >= 0; --size)
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+            const int j = size - i;
+            if (j < 0 || j >= NB) continue;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) mma(sum[t], a[i], b[j][t / 2][(t & 1) * 2], b[j][t / 2][(t & 1) * 2 + 1]);
+        }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[t][e] += sum[t][e];
+}
+
 CUBF_DEV void copy16(uint32_t dst, const void* src, bool ok) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
