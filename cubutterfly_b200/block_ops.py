@@ -118,10 +118,11 @@ def gated_delta(q, k, v, log_decay, beta, *, scale=None, initial_state=None, off
     be strided (slices of one projection).  The states are fp32 (B, H, K, V), ``initial_state`` zero unless given.  With
     ``offsets`` (int32 on the device, n + 1 ascending values from 0 to T) the batch is packed: q is (T, Hk, K) or
     (1, T, Hk, K) and so on, sequence j the tokens offsets[j] .. offsets[j + 1] - 1 (there may be none: its final state
-    is its initial one), the states are (n, H, K, V), and nothing of one sequence, NaN included, reaches another.  In
-    its own sequence a value that is not finite reaches later tokens and up to 63 before it.  Keys are meant to be of
-    length about one (``qk_norm``): with beta (k . k) above 2 the rule itself diverges.  Differentiable in q, k, v, both
-    gates and initial_state; the backward computes the states again, so that nothing but the inputs is kept.
+    is its initial one), the states are (n, H, K, V), and nothing of one sequence, NaN included, reaches another;
+    tokens before the first offset or behind the last one (padding) have outputs and gradients of zero.  In its own
+    sequence a value that is not finite reaches later tokens and up to 63 before it.  Keys are meant to be of length
+    about one (``qk_norm``): with beta (k . k) above 2 the rule itself diverges.  Differentiable in q, k, v, both gates
+    and initial_state; the backward computes the states again, so that nothing but the inputs is kept.
     """
     return _block_ops.gated_delta(q, k, v, log_decay, beta, scale, initial_state, offsets)
 

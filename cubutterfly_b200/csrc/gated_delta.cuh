@@ -102,6 +102,29 @@ CUBF_DEV void operand(const float (&a)[4], const float (&b)[4], uint32_t (&f)[N]
     fragment<N>(a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3], f);
 }
 
+// ---- tokens of no sequence ----------------------------------------------------------------------
+// Before the first offset of a packed batch and behind the last one: their outputs or gradients are zero, as a padded
+// batch's other rows are.  (Left as they were allocated they could be NaN, which a zero gradient does not mask.)
+template <typename T>
+__global__ void __launch_bounds__(256) gated_delta_rest_kernel(GatedDeltaArgs a, bool backward) {
+    pdl_begin();
+    const size_t first = static_cast<size_t>(offset_at(a, 0)), last = static_cast<size_t>(offset_at(a, a.sequences));
+    auto zero = [&](void* p, size_t width) {             // 16-bit units a token
+        auto* const x = static_cast<uint16_t*>(p);
+        const size_t step = static_cast<size_t>(gridDim.x) * 256, from = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+        for (size_t e = from; e < first * width; e += step) x[e] = 0;
+        for (size_t e = last * width + from; e < a.length * width; e += step) x[e] = 0;
+    };
+    constexpr size_t units = sizeof(T) / 2;
+    const size_t values = a.heads * a.v_dim * units, keys = a.k_heads * a.k_dim * units;
+    if (!backward) return zero(a.o, values);
+    zero(a.d_q, keys);
+    zero(a.d_k, keys);
+    zero(a.d_v, values);
+    zero(a.d_log_decay, a.heads * (a.log_decay32 ? 2 : 1));
+    zero(a.d_beta, a.heads * (a.beta32 ? 2 : 1));
+}
+
 // ---- one token ----------------------------------------------------------------------------------
 // A CTA takes VW columns of a head's state: each thread one vector of VEC columns of K / 16 rows, all loaded before the
 // first use.  o = scale (e^g q^T S + (q . k) u), so that both products with the old state share one reduction.

@@ -17,7 +17,7 @@
 // us for 65 (257 tokens, both chains).  Three pieces of these tiles would not
 // fit beside an accumulator in tensor memory, so this path stays on the
 // register-fed tensor instructions, and bounded by the latency of a chunk's
-// three products in one warp: 9 us a chunk of K = 64 forward, 13 of K = 128.
+// three products in one warp, 11 us a chunk of K = 64 forward.
 #pragma once
 
 #include <algorithm>

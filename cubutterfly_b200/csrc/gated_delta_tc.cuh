@@ -75,6 +75,10 @@ struct TcShared {
 // its group L beta, (backward: beta L,) and P as two pieces each, beta folded into P's columns forward.  q k^T and k k^T
 // stay in registers for the group.  L comes block by block of 16 rows, from the inverses of the blocks on the diagonal.
 // What leaves by bulk copies is read while the next step computes, and v of the next head comes in meanwhile.
+// Bounded by latency: 16384 tokens of 16 key and 32 value heads (bf16, K = V = 128) take 178 us forward, of which its own
+// 0.82 GB would take 125.  A CTA waits 10000 of its 50000 cycles for q and k; prefetches of them a wave ahead gave nothing
+// (190 us), four CTAs an SM instead of three 5 %, the triangles' blocks spread over the warps and lines instead of rows
+// prefetched 15 %, fewer instructions to a decay 6 %.
 
 template <typename T, int KP, bool BACKWARD>
 struct TcPrepareShared {
@@ -468,7 +472,6 @@ CUBF_DEV int segment_base(const GatedDeltaArgs& a, const Segments& s, int sequen
     const int base = slot_base(a, sequence, a.offsets ? offset_at(a, sequence) : 0);
     return a.offsets ? base / s.length + sequence : sequence * segments_of((a.length + C - 1) / C, s.length);
 }
-// segment >= segments: a place that no segment has
 CUBF_DEV Chain chain_of(const GatedDeltaArgs& a, const Segments& s, int index) {
     Chain c{};
     c.head = index % a.heads;
@@ -496,6 +499,8 @@ CUBF_DEV Chain chain_of(const GatedDeltaArgs& a, const Segments& s, int index) {
     c.chunks = (c.length + C - 1) / C;
     return c;
 }
+// Places behind a sequence's last segment, and before the first sequence where that begins behind the first token.
+CUBF_DEV bool no_segment(const Chain& c) { return c.segment < 0 || c.segment >= c.segments; }
 
 template <typename T, int KP>
 struct TcChain {
@@ -1148,13 +1153,15 @@ CUBF_DEV void fewer_registers() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+// A chunk takes 2.4 us of its chain (K = V = 128, bf16), tensor pipe 41 % busy: 32 heads of 16384 tokens 622 us in one piece,
+// 236 in three segments whose ends took 189 (1.9 to 2.2 us a chunk without outputs) and their joins 10 to 27.
 template <typename T, int KP>
 __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_forward_kernel(GatedDeltaArgs a, Places w, bool wide) {
     extern __shared__ __align__(1024) unsigned char aligned_raw[];
     pdl_begin();
     using Run = TcChain<T, KP>;
     const Chain chain = chain_of(a, w.segments, blockIdx.x);
-    if (chain.segment >= chain.segments) return;
+    if (no_segment(chain)) return;
     Run run(a, w, *reinterpret_cast<TcShared<T, KP>*>(aligned_raw), chain);
     if (run.warp >= kTcCompute / 32) {
         fewer_registers<56>();
@@ -1170,14 +1177,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_forward_kernel(G
 }
 
 // Both chains of the backward side by side: neither needs the other's results.  (One kind after the other is no faster for
-// training's 128 + 128 chains on 148 SMs, 420 us against 433, and slower for packed sequences, 587 against 350.)
+// training's 128 + 128 chains on 148 SMs, 420 us against 433, and slower for packed sequences, 587 against 350, both measured
+// before the chains' later steps; the 256 chains of 32 chunks take 290 now, two rounds of 4.5 us a chunk, 2.5 TB/s of writes.)
 template <typename T, int KP>
 __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_chains_kernel(GatedDeltaArgs a, Places w, bool wide) {
     extern __shared__ __align__(1024) unsigned char aligned_raw[];
     pdl_begin();
     using Run = TcChain<T, KP>;
     const Chain chain = chain_of(a, w.segments, blockIdx.x / 2);
-    if (chain.segment >= chain.segments) return;
+    if (no_segment(chain)) return;
     Run run(a, w, *reinterpret_cast<TcShared<T, KP>*>(aligned_raw), chain);
     const bool reversed = blockIdx.x % 2 == 0;
     if (run.warp >= kTcCompute / 32) {
@@ -1214,7 +1222,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_ends_kernel(Gate
     const int kind = blockIdx.x % kinds;                        // D, A and, backward, the reversed chain's D
     const Chain chain = chain_of(a, w.segments, blockIdx.x / kinds);
     const bool first = chain.segment == 0, last = chain.segment + 1 == chain.segments;
-    if (chain.segment >= chain.segments || (kind == 2 ? first : last) || (kind == 1 && first)) return;
+    if (no_segment(chain) || (kind == 2 ? first : last) || (kind == 1 && first)) return;
     Run run(a, w, *reinterpret_cast<TcShared<T, KP>*>(aligned_raw), chain);
     if (run.warp >= kTcCompute / 32) {
         fewer_registers<56>();
@@ -1326,7 +1334,10 @@ __global__ void __launch_bounds__(2 * KP) gated_delta_join_kernel(GatedDeltaArgs
 //   [q; k] k^T      [dO; W] R^T      [dO; W] S^T      [.; R] dS^T
 // then, with the pairs' coefficients Cq = D o dP and Cm = D o dM written as one tile of 128 rows,
 //   [Cq; Cm] k      and, the tile turned,  [.; Cq^T q + Cm^T k].
-// Bounded by memory: the kept S and dS, 64 KB each, R and W, 32 KB each, and the tiles of q, k and dO per chunk and head.
+// What has to come is the kept S and dS, 64 KB each, R and W, 32 KB each, and the tiles of q, k and dO per chunk and head;
+// they fill shared memory, so a head's steps are one after another and their latency bounds it.  8 sequences of 2048 tokens,
+// 16 heads (bf16, K = V = 128): 330 us, where the bytes alone take 145; 353 without the next head's prefetch to L2, and 490
+// with 168 registers a thread (1 KB spilled) instead of 224 and all 32 columns of the pairs at once.
 constexpr int kGradientThreads = kTcThreads;  // three warps only leave their registers to the computing ones
 
 template <typename T, int KP>

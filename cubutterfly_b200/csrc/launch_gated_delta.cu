@@ -48,8 +48,8 @@ int sequences_of(const GatedDeltaArgs& a) { return a.offsets ? a.sequences : a.b
 // Chunks a segment, 0 for none: the shortest time by what a chunk of a chain takes on one SM (2.4 us with its results
 // forward, 2.9 backward, 1.9 without them), a state's join (4 us) and the CTAs that run at once, one per SM.  Of a packed
 // batch the host knows the tokens and the sequences alone; n random cuts leave a longest piece of (1 + 1/2 + .. + 1/n) / n.
-// Whole calls forward, one sequence of 16384 tokens: 32 heads 680 us in three segments against 870 in one, 12 heads 369 in
-// seven against 735, 4 heads 213 in 16 against 670; forward and backward of 4 heads 655 in 14 against 1960.
+// Whole calls forward, one sequence of 16384 tokens: 32 heads 624 us in three segments against 840 in one, 12 heads 335 in
+// seven against 725, 4 heads 205 in 16 against 666; forward and backward of 4 heads 600 in 14 against 1910.
 int segment_length(const GatedDeltaArgs& a, bool backward) {
     double longest = ceil_div(a.length, C), all = longest * a.batch;
     const double sequences = sequences_of(a);
@@ -186,8 +186,8 @@ size_t gated_delta_workspace_unit<CUBF_GD_TYPE, CUBF_GD_K>(const GatedDeltaArgs&
     return places_of(a, backward).total;
 }
 
-template <>
-cudaError_t launch_gated_delta_unit<CUBF_GD_TYPE, CUBF_GD_K>(const GatedDeltaArgs& a, bool backward, cudaStream_t stream) {
+namespace {
+cudaError_t launch_kernels(const GatedDeltaArgs& a, bool backward, cudaStream_t stream) {
     const Places w = places_of(a, backward);
     const size_t chunks = static_cast<size_t>(w.slots) * a.heads;
 #if CUBF_GD_TENSOR
@@ -232,6 +232,15 @@ cudaError_t launch_gated_delta_unit<CUBF_GD_TYPE, CUBF_GD_K>(const GatedDeltaArg
     return launch(share, &gated_delta_share_kernel, std::min<size_t>((values + 255) / 256, 148 * 8), 256, 0, stream, a, w,
                   values);
 #endif
+}
+}  // namespace
+
+template <>
+cudaError_t launch_gated_delta_unit<CUBF_GD_TYPE, CUBF_GD_K>(const GatedDeltaArgs& a, bool backward, cudaStream_t stream) {
+    const cudaError_t e = launch_kernels(a, backward, stream);
+    if (e != cudaSuccess || !a.offsets) return e;
+    static KernelSetup rest;
+    return launch(rest, &gated_delta_rest_kernel<T>, 148, 256, 0, stream, a, backward);
 }
 
 #if CUBF_GD_K == 128

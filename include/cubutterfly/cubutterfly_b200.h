@@ -313,7 +313,8 @@ typedef struct cubutterflyB200HeadTensor_s {
  * k_dim and v_dim are at most 128, length at most 2^30.  Tokens of other
  * sequences, NaN and infinities included, do not reach a sequence; in its own
  * a value that is not finite reaches all later tokens and up to 63 earlier
- * ones.  o is contiguous (batch, length, heads, v_dim).
+ * ones.  o is contiguous (batch, length, heads, v_dim).  Tokens before the first
+ * offset or behind the last one have outputs and gradients of zero.
  * The gradients are contiguous, in the types of their tensors; d_initial_state
  * null: not computed.  Both directions need a workspace (256-byte aligned). */
 typedef struct cubutterflyB200GatedDelta_s {

@@ -136,6 +136,36 @@ def test_gated_delta_few_long_chains(cuda, batch, length, k_heads, heads, k_dim,
     check_delta(t, cuts)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("first,last", [(1, 200), (70, 190), (700, 2500), (1300, 2431)])
+def test_gated_delta_offsets_that_leave_tokens_out(cuda, first, last, dtype):
+    """Tokens before the first offset and behind the last one belong to no sequence: what they hold, NaN here, goes nowhere, and
+    their outputs and gradients are zero."""
+    t = {n: v for n, v in delta_case(1, 2500 if last > 200 else 200, 1, 2, 64, 48, dtype, cuts=[0, 1], seed=48).items()
+         if v is not None}
+    exact = {n: v[first:last].double().requires_grad_() for n, v in t.items()}
+    outside = torch.ones(t["q"].shape[0], dtype=torch.bool)
+    outside[first:last] = False
+    dev = {}
+    for n, v in t.items():
+        v[outside] = float("nan")
+        dev[n] = v.cuda().requires_grad_()
+    names = list(t)
+    o, final = run_delta({**dev, "state": None}, [first, last])
+    eo, efinal = ref.gated_delta(*(exact[n] for n in names), cuts=[0, last - first])
+    loss = ref.DELTA_LOSS[dtype]
+    ref.assert_close(o[first:last], eo.detach(), loss, "o")
+    ref.assert_close(final, efinal.detach(), loss, "final")
+    d_o, d_final = normal(93, *o.shape, dtype=dtype), normal(94, *final.shape, scale=0.3)
+    d_o[outside] = float("nan")
+    got = torch.autograd.grad([o, final], [dev[n] for n in names], [d_o.cuda(), d_final.cuda()])
+    want = torch.autograd.grad([eo, efinal], [exact[n] for n in names], [d_o[first:last].double(), d_final.double()])
+    assert not o[outside.cuda()].any()
+    for n, x, y in zip(names, got, want):
+        ref.assert_close(x[first:last], y, 4 * loss, "d_" + n)
+        assert not x[outside.cuda()].any(), n
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 def test_gated_delta_long_chain_is_causal(cuda, dtype):
     t = {n: None if v is None else v.cuda() for n, v in delta_case(1, 2300, 1, 1, 64, 64, dtype, state=True, seed=44).items()}
