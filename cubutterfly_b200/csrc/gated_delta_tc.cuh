@@ -472,13 +472,31 @@ CUBF_DEV int segment_base(const GatedDeltaArgs& a, const Segments& s, int sequen
     const int base = slot_base(a, sequence, a.offsets ? offset_at(a, sequence) : 0);
     return a.offsets ? base / s.length + sequence : sequence * segments_of((a.length + C - 1) / C, s.length);
 }
+// The sequence of `rank` among those of a packed batch by length, the longest first, so that no long chain starts last.  Each
+// lane ranks two sequences; beyond 64 their order stays.  16384 tokens in 13 sequences, 32 heads forward: 417 us for 480; in 6,
+// 643 for 675; 8 heads' training in 24 sequences 698 for 729; forward in 40, whose chains are many and short, 446 for 432.
+CUBF_DEV int by_length(const GatedDeltaArgs& a, int rank) {
+    if (a.sequences > 64) return rank;
+    const int lane = threadIdx.x & 31;
+    auto length = [&](int j) { return j < a.sequences ? max(0, offset_at(a, j + 1) - offset_at(a, j)) : -1; };
+    const int mine[2] = {length(lane), length(lane + 32)};
+    int before[2] = {0, 0};
+    for (int j = 0; j < a.sequences; ++j) {
+        const int other = length(j);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) before[n] += other > mine[n] || (other == mine[n] && j < lane + 32 * n);
+    }
+    const unsigned low = __ballot_sync(0xffffffffu, lane < a.sequences && before[0] == rank);
+    const unsigned high = __ballot_sync(0xffffffffu, lane + 32 < a.sequences && before[1] == rank);
+    return low ? __ffs(low) - 1 : high ? 31 + __ffs(high) : rank;
+}
 CUBF_DEV Chain chain_of(const GatedDeltaArgs& a, const Segments& s, int index) {
     Chain c{};
     c.head = index % a.heads;
     c.index = index / a.heads;
     c.segments = 1;
     if (s.length == 0) {
-        locate(a, c.index, c);
+        locate(a, a.offsets ? by_length(a, c.index) : c.index, c);
         return c;
     }
     int low = 0, high = a.offsets ? a.sequences : a.batch;
