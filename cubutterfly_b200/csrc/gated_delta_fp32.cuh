@@ -12,7 +12,7 @@
 // heads share keys, `share` adds their gradients up.
 //
 // Every operand is three bf16 pieces and every product six (mma_split.cuh),
-// added up in fp32 (products_rounded): 1.2e-7 to 2.3e-7 of a result against 64
+// added up in fp32 (products_rounded): 1.2e-7 to 2.7e-7 of a result against 64
 // bits, and 1e-6 to 5e-6 with one accumulator through all sums, which took 57
 // us for 65 (257 tokens, both chains).  Three pieces of these tiles would not
 // fit beside an accumulator in tensor memory, so this path stays on the
