@@ -2,6 +2,7 @@
 // recurrence, the gated delta rule and the norm of queries and keys: argument
 // checks, then launches.  Nothing here allocates device
 // memory, copies or synchronises.
+#include <algorithm>
 #include <cmath>
 #include <stdexcept>
 #include <string>
@@ -362,6 +363,8 @@ cubf::GatedDeltaArgs delta_args(const cubutterflyB200GatedDelta_t* a, BlockType*
     s.sequences = static_cast<int>(a->sequences);
     s.initial = a->initial_state;
     s.offsets = a->offsets;
+    constexpr int most = cubf::kDeltaWaitLimit;
+    s.wait_limit = a->wait_limit == 0 ? most : std::clamp(a->wait_limit, 0, most);
     if (a->batch > 0 && a->length > 0) delta_gates(a, *block, s);
     // a CTA for each chunk of 64 tokens of each head
     const size_t chunks = a->offsets ? a->length / cubf::kDeltaChunk + a->sequences

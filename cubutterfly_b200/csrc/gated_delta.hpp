@@ -13,6 +13,7 @@ namespace cubf {
 constexpr int kDeltaChunk = 64;          // tokens a chunk
 constexpr int kDeltaMaxDim = 128;        // of keys and of values
 constexpr int kDeltaMaxLength = 1 << 30;
+constexpr int kDeltaWaitLimit = 1 << 17;  // tries, of 8 us each where nothing comes: a second
 
 // A (batch, token, head, channel) tensor: strides in elements, the channels adjacent.
 struct HeadTensor {
@@ -37,6 +38,7 @@ struct GatedDeltaArgs {
     int batch, length, k_heads, heads, k_dim, v_dim, sequences;
     float scale;
     bool log_decay32, beta32;    // fp32 gates beside 16-bit tensors
+    uint32_t wait_limit;         // tries of a wait on a barrier
     void* workspace;
 };
 

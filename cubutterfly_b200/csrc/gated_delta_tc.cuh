@@ -66,8 +66,9 @@ struct TcShared {
     alignas(1024) unsigned char stage[2][Tiles::kStage];
     alignas(16) T out[C * 128];                              // rows of o or dv on their way out
     alignas(16) float factors[2][5 * C];
-    alignas(8) unsigned long long full[2], empty[2], ready[5], done[4], out_ready, out_free;
+    alignas(8) unsigned long long full[2], empty[2], ready[5], done[4], out_ready, out_free, drained;
     uint32_t base;
+    int lost;                                                // a wait ran out
 };
 
 // ---- prepare ------------------------------------------------------------------------------------
@@ -520,6 +521,20 @@ CUBF_DEV Chain chain_of(const GatedDeltaArgs& a, const Segments& s, int index) {
 // Places behind a sequence's last segment, and before the first sequence where that begins behind the first token.
 CUBF_DEV bool no_segment(const Chain& c) { return c.segment < 0 || c.segment >= c.segments; }
 
+constexpr uint32_t kLost = 0x7fff7fff;   // NaN as one fp32 value and as two fp16 or bf16 ones
+
+// All roles of a CTA, from wherever they end.
+CUBF_DEV void meet_all() { asm volatile("bar.sync 3, %0;" ::"n"(kTcThreads) : "memory"); }
+// What the warp has in flight has ended, or another limit has passed: a copy into shared memory, all its products.
+CUBF_DEV void drain_copy(unsigned long long& barrier, uint32_t phase) {
+    for (int n = 0; n < kDeltaWaitLimit && !__all_sync(0xffffffffu, tc::barrier_try(smem_addr(&barrier), phase)); ++n) {}
+}
+CUBF_DEV void drain_products(unsigned long long& barrier) {
+    if (tc::elect()) tc::commit(smem_addr(&barrier));
+    __syncwarp();
+    drain_copy(barrier, 0);
+}
+
 template <typename T, int KP>
 struct TcChain {
     using Tiles = TcTiles<T, KP>;
@@ -532,12 +547,14 @@ struct TcChain {
     const Chain chain;
     const int tid, lane, warp, half, v;  // v: the thread's column
     uint32_t tmem, at;                   // tensor memory; with the warp's lanes
-    bool failed;
+    int loads = 0;                       // of chunks, by the issuing warp
+    bool failed;                         // a wait of this warp ran out
 
     CUBF_DEV TcChain(const GatedDeltaArgs& a, const Places& w, Shared& sm, const Chain& chain)
         : a(a), w(w), sm(sm), chain(chain), tid(threadIdx.x), lane(tid & 31), warp(__shfl_sync(0xffffffffu, tid >> 5, 0)),
           half(warp >> 2), v((warp & 3) * 32 + lane),
-          failed((smem_addr(&sm) & 1023u) != 0) {  // the swizzle acts on address bits
+          // the swizzle acts on address bits; a chain without tokens waits for nothing
+          failed(chain.chunks > 0 && ((smem_addr(&sm) & 1023u) != 0 || a.wait_limit == 0)) {
         if (tid == 0) {
             for (auto& b : sm.full) tc::barrier_init(smem_addr(&b), 1);
             for (auto& b : sm.done) tc::barrier_init(smem_addr(&b), 1);
@@ -545,6 +562,8 @@ struct TcChain {
             for (auto& b : sm.empty) tc::barrier_init(smem_addr(&b), kTcCompute / 32 + 1);  // factors read, products done
             tc::barrier_init(smem_addr(&sm.out_ready), kTcCompute / 32);
             tc::barrier_init(smem_addr(&sm.out_free), kTcMovers / 32);
+            tc::barrier_init(smem_addr(&sm.drained), 1);
+            sm.lost = 0;
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
         if (warp == kTcCompute / 32) tc::allocate(&sm.base, kTcColumns);
@@ -554,14 +573,23 @@ struct TcChain {
         tmem = __shfl_sync(0xffffffffu, sm.base, 0);
         at = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     }
-    // Also where a wait ran out: what was in flight had another such limit's time to end.
-    CUBF_DEV void finish() {
+    // True where a wait of the CTA ran out.  Shared and tensor memory are then given back when the copies and products in
+    // flight have ended (within another limit).
+    CUBF_DEV bool finish() {
+        tc::wait_load();
+        tc::wait_store();
+        if (failed && lane == 0) sm.lost = 1;
         tc::fence_before();
-        __syncthreads();
+        meet_all();
         if (warp == kTcCompute / 32) {
             tc::fence_after();
+            if (sm.lost) {
+                for (int n = max(0, loads - 2); n < loads; ++n) drain_copy(sm.full[n & 1], (n >> 1) & 1);
+                drain_products(sm.drained);
+            }
             tc::release(tmem, kTcColumns);
         }
+        return sm.lost;
     }
     CUBF_DEV char* work(size_t offset) const { return static_cast<char*>(a.workspace) + offset; }
     CUBF_DEV size_t place(int c) const { return static_cast<size_t>(chain.base + c) * a.heads + chain.head; }
@@ -573,10 +601,11 @@ struct TcChain {
         return (static_cast<size_t>(chain.row) * a.length + chain.start + c * C) * a.heads + chain.head;
     }
 
+    // The lanes of a warp go on alike, or give up alike.
     template <typename Barrier>
     CUBF_DEV void wait(Barrier& barrier, uint32_t phase) {
-        failed = failed || !tc::barrier_wait(smem_addr(&barrier), phase);
-        __syncwarp();
+        uint32_t tries = 0;
+        while (!failed && !__all_sync(0xffffffffu, tc::barrier_try(smem_addr(&barrier), phase))) failed = ++tries >= a.wait_limit;
         tc::fence_after();
     }
     // A computing warp's stores to tensor memory are seen by the products that the barrier lets be issued.
@@ -594,7 +623,8 @@ struct TcChain {
 
     // ---- the issuing warp ----
     // A chunk's q and k, `squares` matrices from the `from`-th on, and `factors` rows of factors from `first` on.
-    CUBF_DEV void load(int c, int s, int from, int squares, int first, int factors) const {
+    CUBF_DEV void load(int c, int s, int from, int squares, int first, int factors) {
+        ++loads;
         const uint32_t bar = smem_addr(&sm.full[s]), dst = smem_addr(sm.stage[s]);
         const int k_head = chain.head / (a.heads / a.k_heads);
         const size_t tile = static_cast<size_t>(chain.base + c) * a.k_heads + k_head;
@@ -672,12 +702,13 @@ struct TcChain {
     }
 
     template <bool KEEP>
-    CUBF_DEV void load_forward(int c) const {
+    CUBF_DEV void load_forward(int c) {
         load(c, c & 1, 0, KEEP ? 1 : 2, kTailBeta, KEEP ? 2 : 3);
     }
     template <bool KEEP>
     CUBF_DEV void issue_forward() {
         const int chunks = chain.chunks;
+        if (failed) return;
         if (chunks > 0) load_forward<KEEP>(0);
         if (chunks > 1) load_forward<KEEP>(1);
         uint32_t phase = 0;
@@ -734,6 +765,7 @@ struct TcChain {
     CUBF_DEV void issue_backward() {
         const int chunks = chain.chunks;
         auto bring = [&](int n) { load(chunks - 1 - n, n & 1, 1, 2, kDecay, 5); };
+        if (failed) return;
         if (chunks > 0) bring(0);
         if (chunks > 1) bring(1);
         uint32_t phase = 0;
@@ -908,7 +940,7 @@ struct TcChain {
     }
     // Byte of (column of v, channel) in a kept state's piece: chunks of eight channels.
     CUBF_DEV uint32_t kept(int row, int col) const { return static_cast<uint32_t>(((col >> 3) * w.v_rows + row) * 16); }
-    // A state of `columns` columns (null: zero), and where to: NaN where a wait ran out.
+    // A state (null: zero), and where to, a row of `columns` values a channel.
     CUBF_DEV void state_in(const float* p, P (&s)[H / 2]) const {
 #pragma unroll
         for (int i = 0; i < H / 2; ++i) {
@@ -930,7 +962,7 @@ struct TcChain {
             for (int e = 0; e < 2; ++e) {
                 const int k = half * H + 2 * i + e;
                 if (k < a.k_dim && v < columns)
-                    p[static_cast<size_t>(k) * columns + v] = failed ? __int_as_float(0x7fffffff) : x[e];
+                    p[static_cast<size_t>(k) * columns + v] = x[e];
             }
         }
     }
@@ -1159,6 +1191,41 @@ struct TcChain {
         else if (chain.segment == 0 && a.d_initial)
             state_out(a.d_initial + state_offset(), a.v_dim, s);
     }
+
+    // ---- where a wait ran out ----
+    // NaN in all that the chain leaves, by the computing warps when every role has ended: its rows of o or dv, its states,
+    // and what other kernels go by, so that nothing that comes of it passes for a result: the ends and maps of segments,
+    // R (of which dq, dk and the gates' gradients come) and W (dk and the gates').
+    CUBF_DEV void lose(void* p, size_t words) const {
+        for (size_t e = tid; e < words; e += kTcCompute) static_cast<uint32_t*>(p)[e] = kLost;
+    }
+    CUBF_DEV void lose_rows(T* out) const {
+        const size_t step = static_cast<size_t>(a.heads) * a.v_dim, values = static_cast<size_t>(chain.length) * a.v_dim;
+        uint16_t* const p = reinterpret_cast<uint16_t*>(out + out_row(0) * a.v_dim);
+        for (size_t e = tid; e < values; e += kTcCompute) p[e / a.v_dim * step + e % a.v_dim] = kLost & 0xffff;
+    }
+    CUBF_DEV void lose_kept(size_t region) const {
+        for (int c = 0; c < chain.chunks; ++c) lose(work(region) + place(c) * 2 * w.v_rows * 128, 2 * w.v_rows * 32);
+    }
+    template <int MODE>
+    CUBF_DEV void lose_forward() const {
+        const size_t state = static_cast<size_t>(a.k_dim) * a.v_dim;
+        if (MODE == kOut) {
+            lose_rows(static_cast<T*>(a.o));
+            if (chain.segment + 1 == chain.segments) lose(a.last + state_offset(), state);
+        }
+        if (MODE == kKeep) lose_kept(w.errors);
+        if (MODE == kEnd) lose(end_of(w.segments.ends, chain.index), state);
+        if (MODE == kMap) lose(map_of(chain.index), KP * KP);
+    }
+    template <bool END>
+    CUBF_DEV void lose_backward() const {
+        const size_t state = static_cast<size_t>(a.k_dim) * a.v_dim;
+        if (END) return lose(end_of(w.segments.d_ends, chain.index), state);
+        lose_rows(static_cast<T*>(a.d_v));
+        lose_kept(w.d_writes);
+        if (chain.segment == 0 && a.d_initial) lose(a.d_initial + state_offset(), state);
+    }
 };
 
 // 224 registers for a computing thread, 56 for the others: 256 x 224 + 128 x 56 = 384 x 168, what the CTA starts with.
@@ -1187,11 +1254,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_forward_kernel(G
             run.template issue_forward<false>();
         else
             run.move_out(static_cast<T*>(a.o), false, wide);
+        run.finish();
     } else {
         more_registers<224>();
         run.template compute_forward<Run::kOut>();
+        if (run.finish()) run.template lose_forward<Run::kOut>();
     }
-    run.finish();
 }
 
 // Both chains of the backward side by side: neither needs the other's results.  (One kind after the other is no faster for
@@ -1216,14 +1284,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_chains_kernel(Ga
         } else if (reversed) {
             run.move_out(static_cast<T*>(a.d_v), true, wide);
         }
+        run.finish();
     } else {
         more_registers<224>();
         if (reversed)
             run.template compute_backward<false>();
         else
             run.template compute_forward<Run::kKeep>();
+        if (!run.finish()) return;
+        if (reversed)
+            run.template lose_backward<false>();
+        else
+            run.template lose_forward<Run::kKeep>();
     }
-    run.finish();
 }
 
 // ---- segments -----------------------------------------------------------------------------------
@@ -1250,6 +1323,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_ends_kernel(Gate
             else
                 run.template issue_forward<true>();
         }
+        run.finish();
     } else {
         more_registers<224>();
         if (kind == 0)
@@ -1258,8 +1332,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_ends_kernel(Gate
             run.template compute_forward<Run::kMap>();
         else
             run.template compute_backward<true>();
+        if (!run.finish()) return;
+        if (kind == 0)
+            run.template lose_forward<Run::kEnd>();
+        else if (kind == 1)
+            run.template lose_forward<Run::kMap>();
+        else
+            run.template lose_backward<true>();
     }
-    run.finish();
 }
 
 // The states where segments end, one after another, in place of the D's: a CTA takes 8 columns of a chain's state, a thread
@@ -1372,8 +1452,9 @@ struct GradientShared {
     alignas(16) float factors[kTcFactors][C];
     float row[2][2][C], kept[2][C], column[4][C], dot[8], beta[C];
     double d_sum[C], all[2];
-    alignas(8) unsigned long long full, state_full[kBuffers], state_empty[kBuffers], done[4], ready, free;
+    alignas(8) unsigned long long full, state_full[kBuffers], state_empty[kBuffers], done[4], ready, free, drained;
     uint32_t base;
+    int lost;                                                    // a wait ran out
     // With fp16 the pairs take dO's place, or with few columns of v the end of the tiles, which those do not reach.
     CUBF_DEV unsigned char* pair_tile(int n, int v_rows) { return NI == 1 ? pairs[n] : v_rows == 128 ? tiles[3 * n] : tiles[4 + n]; }
 };
@@ -1406,12 +1487,49 @@ struct Gradients {
     const int tid, lane, warp;
     uint32_t tmem;
     bool failed = false;
+    int head_loads = 0, state_loads = 0; // by the issuing warp
 
     template <typename Barrier>
     CUBF_DEV void wait(Barrier& barrier, uint32_t phase) {
-        failed = failed || !tc::barrier_wait(smem_addr(&barrier), phase);
-        __syncwarp();
+        uint32_t tries = 0;
+        while (!failed && !__all_sync(0xffffffffu, tc::barrier_try(smem_addr(&barrier), phase))) failed = ++tries >= a.wait_limit;
         tc::fence_after();
+    }
+    // As a chain's.
+    CUBF_DEV bool finish() {
+        tc::wait_load();
+        if (failed && lane == 0) sm.lost = 1;
+        tc::fence_before();
+        meet_all();
+        if (warp == kTcCompute / 32) {
+            tc::fence_after();
+            if (sm.lost) {
+                if (head_loads > 0) drain_copy(sm.full, (head_loads - 1) & 1);
+                for (int n = max(0, state_loads - Shared::kBuffers); n < state_loads; ++n)
+                    drain_copy(sm.state_full[n % Shared::kBuffers], n / Shared::kBuffers & 1);
+                drain_products(sm.drained);
+            }
+            tc::release(tmem, kTcColumns);
+        }
+        return sm.lost;
+    }
+    CUBF_DEV void lose() const {
+        const size_t first = static_cast<size_t>(s.row) * a.length + s.first;
+        for (int e = tid; e < s.tokens * a.k_dim; e += kTcCompute) {
+            const size_t at = ((first + e / a.k_dim) * a.k_heads + k_head) * a.k_dim + e % a.k_dim;
+            static_cast<uint16_t*>(a.d_q)[at] = static_cast<uint16_t*>(a.d_k)[at] = kLost & 0xffff;
+        }
+        for (int e = tid; e < s.tokens * group; e += kTcCompute) {
+            const size_t at = (first + e / group) * a.heads + k_head * group + e % group;
+            auto lose = [&](void* p, bool wide) {
+                if (wide)
+                    static_cast<uint32_t*>(p)[at] = kLost;
+                else
+                    static_cast<uint16_t*>(p)[at] = kLost & 0xffff;
+            };
+            lose(a.d_log_decay, a.log_decay32);
+            lose(a.d_beta, a.beta32);
+        }
     }
     CUBF_DEV void report(unsigned long long& barrier) const {
         __syncwarp();
@@ -1421,7 +1539,8 @@ struct Gradients {
     CUBF_DEV size_t place(int g) const { return static_cast<size_t>(slot) * a.heads + k_head * group + g; }
 
     // ---- the issuing warp ----
-    CUBF_DEV void load_state(int g, int n) const {               // n: S, then dS, two pieces each
+    CUBF_DEV void load_state(int g, int n) {                     // n: S, then dS, two pieces each
+        ++state_loads;
         const int b = n % Shared::kBuffers;
         const uint32_t bytes = static_cast<uint32_t>(w.state_piece);
         const char* from = work(n < 2 ? w.states : w.d_states) + (place(g) * 2 + n % 2) * w.state_piece;
@@ -1431,7 +1550,8 @@ struct Gradients {
         }
         __syncwarp();
     }
-    CUBF_DEV void load_head(int g) const {
+    CUBF_DEV void load_head(int g) {
+        ++head_loads;
         const uint32_t bar = smem_addr(&sm.full), tile = static_cast<uint32_t>(w.v_rows * 128);
         if (tc::elect()) {
             tc::barrier_expect(bar, (g == 0 ? 2 * kOperand : 0) + (NI + 4) * tile + sizeof(sm.factors));
@@ -1719,7 +1839,7 @@ struct Gradients {
             for (int n = 0; n < H; n += 8) {
                 Vec16<T> x;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x.v[e] = Convert<T, float>::store(failed ? __int_as_float(0x7fffffff) : total[n + e]);
+                for (int e = 0; e < 8; ++e) x.v[e] = Convert<T, float>::store(total[n + e]);
                 if (wide) {
                     if (first + n < a.k_dim) *reinterpret_cast<Vec16<T>*>(out + first + n) = x;
                 } else {
@@ -1794,7 +1914,7 @@ struct Gradients {
 #pragma unroll
             for (int n = 0; n < 8; ++n) inner += sm.dot[n];
             d += sm.all[0] + sm.all[1] + static_cast<double>(sm.factors[kDecay][C - 1]) * inner;
-            const float d_log = failed ? __int_as_float(0x7fffffff) : static_cast<float>(d);
+            const float d_log = static_cast<float>(d);
             const size_t at = (gate_row + tid) * a.heads + head;
             if (a.log_decay32)
                 static_cast<float*>(a.d_log_decay)[at] = d_log;
@@ -1826,6 +1946,8 @@ __global__ void __launch_bounds__(kGradientThreads, 1) gated_delta_tc_gradients_
         for (auto& b : sm.done) tc::barrier_init(smem_addr(&b), 1);
         tc::barrier_init(smem_addr(&sm.ready), kTcCompute / 32);
         tc::barrier_init(smem_addr(&sm.free), kTcCompute / 32);
+        tc::barrier_init(smem_addr(&sm.drained), 1);
+        sm.lost = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kTcCompute / 32) tc::allocate(&sm.base, kTcColumns);
@@ -1833,19 +1955,15 @@ __global__ void __launch_bounds__(kGradientThreads, 1) gated_delta_tc_gradients_
     __syncthreads();
     tc::fence_after();
     Gradients<T, KP> run{a, w, sm, s, slot, k_head, a.heads / a.k_heads, tid, tid & 31, warp, __shfl_sync(0xffffffffu, sm.base, 0),
-                         (smem_addr(&sm) & 1023u) != 0};
+                         (smem_addr(&sm) & 1023u) != 0 || a.wait_limit == 0};
     if (warp >= kTcCompute / 32) {
         fewer_registers<56>();
         if (warp == kTcCompute / 32) run.issue();
+        run.finish();
     } else {
         more_registers<224>();
         run.compute();
-    }
-    tc::fence_before();
-    __syncthreads();
-    if (warp == kTcCompute / 32) {
-        tc::fence_after();
-        tc::release(run.tmem, kTcColumns);
+        if (run.finish()) run.lose();
     }
 }
 

@@ -17,7 +17,6 @@ namespace cubf::tc {
 using split::smem_addr;
 
 constexpr int kPanel = 8192;             // bytes of 64 x 64 values
-constexpr uint32_t kSpinLimit = 1u << 17;  // tries, of 8 us each where nothing comes: a second
 
 // Byte offset of (row, col) in a tile of panels `panel` bytes apart.
 CUBF_DEV uint32_t swizzled(int row, int col, int panel = kPanel) {
@@ -120,19 +119,16 @@ CUBF_DEV bool elect() {
 CUBF_DEV void barrier_expect(uint32_t barrier, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(barrier), "r"(bytes) : "memory");
 }
-// Bounded wait for a phase; false when the limit expired.
-CUBF_DEV bool barrier_wait(uint32_t barrier, uint32_t phase) {
-    for (uint32_t i = 0; i < kSpinLimit; ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred P1;\n\tmbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2;\n\t"
-            "selp.b32 %0, 1, 0, P1;\n\t}"
-            : "=r"(done)
-            : "r"(barrier), "r"(phase)
-            : "memory");
-        if (done) return true;
-    }
-    return false;
+// A phase has ended: within some 8 us, or at once.
+CUBF_DEV bool barrier_try(uint32_t barrier, uint32_t phase) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred P1;\n\tmbarrier.try_wait.parity.shared::cta.b64 P1, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, P1;\n\t}"
+        : "=r"(done)
+        : "r"(barrier), "r"(phase)
+        : "memory");
+    return done != 0;
 }
 // `bytes` (a multiple of 16, both addresses 16-byte aligned) to shared memory, counted by a barrier.
 CUBF_DEV void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t barrier) {

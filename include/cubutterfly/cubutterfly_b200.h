@@ -316,11 +316,16 @@ typedef struct cubutterflyB200HeadTensor_s {
  * ones.  o is contiguous (batch, length, heads, v_dim).  Tokens before the first
  * offset or behind the last one have outputs and gradients of zero.
  * The gradients are contiguous, in the types of their tensors; d_initial_state
- * null: not computed.  Both directions need a workspace (256-byte aligned). */
+ * null: not computed.  Both directions need a workspace (256-byte aligned).
+ * The kernels of 16-bit tensors wait for copies and products of their own.  A
+ * wait that runs out ends what depends on it, with NaN in the rows, states and
+ * gradients concerned.  wait_limit: tries of a wait (8 us where nothing
+ * comes); 0: 2^17, about a second, and at most that; negative: none, so that
+ * all is NaN. */
 typedef struct cubutterflyB200GatedDelta_s {
     size_t struct_size;
     size_t batch, length, k_heads, heads, k_dim, v_dim, sequences;
-    int data_type, log_decay_type, beta_type, reserved;
+    int data_type, log_decay_type, beta_type, wait_limit;
     double scale;
     cubutterflyB200HeadTensor_t q, k, v, log_decay, beta;
     const float* initial_state;
