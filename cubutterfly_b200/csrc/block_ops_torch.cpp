@@ -116,10 +116,18 @@ void check_plain(const Tensor& t, const char* what) {
                          c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value();
     REQUIRE(!proxies && !torch::jit::tracer::isTracing(), what,
             " is being traced: the block operators cannot be recorded, only run or captured in a CUDA graph");
-    REQUIRE(t.has_storage() && !t.unsafeGetTensorImpl()->is_python_dispatch(), what,
+    REQUIRE(t.has_storage() && !t._is_zerotensor() && !t.unsafeGetTensorImpl()->is_python_dispatch(), what,
             " must be a CUDA tensor with storage of its own, not a wrapper of others");
     REQUIRE(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), what,
             " carries a forward-mode tangent: the block operators have reverse-mode gradients only");
+}
+
+// A view that is negated lazily (the imaginary part of a conjugate, say) is taken as a copy, whose memory holds its values.
+// Gradients that come to a node:
+variable_list plain_gradients(variable_list&& grads) {
+    for (auto& g : grads)
+        if (g.defined() && g.is_neg()) g = g.resolve_neg();
+    return std::move(grads);
 }
 
 // A CUDA tensor out of an argument; None where `optional`.
@@ -129,7 +137,13 @@ Tensor tensor_of(py::handle h, const char* what, bool optional = false) {
     const Tensor& t = THPVariable_Unpack(h.ptr());
     check_plain(t, what);
     REQUIRE(t.is_cuda(), what, " must be a CUDA tensor");
-    return t;
+    return t.is_neg() ? t.resolve_neg() : t;
+}
+// A pool of states, which is written where it lies.
+Tensor pool_of(py::handle h, const char* what) {
+    REQUIRE(!THPVariable_Check(h.ptr()) || !THPVariable_Unpack(h.ptr()).is_neg(), what,
+            " must not be a lazily negated view: its memory does not hold its values");
+    return tensor_of(h, what);
 }
 void check_type(const Tensor& t, const char* what) {
     REQUIRE(data_type(t.scalar_type()) >= 0, what, " does not support dtype ", c10::toString(t.scalar_type()));
@@ -302,7 +316,8 @@ struct BlockNormBackward : Node {
     std::vector<SavedVariable> inputs;
     SavedVariable rms;
 
-    variable_list apply(variable_list&& grads) override {
+    variable_list apply(variable_list&& incoming) override {
+        const variable_list grads = plain_gradients(std::move(incoming));
         variable_list in;
         Tensor r;
         {
@@ -544,7 +559,8 @@ struct GatedScanBackward : Node {
     std::vector<SavedVariable> inputs;
     SavedVariable offsets, chunk_states;
 
-    variable_list apply(variable_list&& grads) override {
+    variable_list apply(variable_list&& incoming) override {
+        const variable_list grads = plain_gradients(std::move(incoming));
         variable_list out(5);
         if (grads[0].defined() || grads[1].defined()) {
             variable_list in;
@@ -653,8 +669,8 @@ Tensor gated_scan_step(py::handle hstate, py::handle hx, py::handle hr, py::hand
     Tensor decay = tensor_of(hdecay, "gated_scan_step: decay");
     check_type(decay, "gated_scan_step: decay");
     check_like(decay, "gated_scan_step: decay", x, {dim});
-    const Tensor state = tensor_of(hstate, "gated_scan_step: state");
-    const Tensor next = hnew.is_none() ? state : tensor_of(hnew, "gated_scan_step: new_state");
+    const Tensor state = pool_of(hstate, "gated_scan_step: state");
+    const Tensor next = hnew.is_none() ? state : pool_of(hnew, "gated_scan_step: new_state");
     for (const Tensor* t : {&state, &next}) {
         REQUIRE(t->scalar_type() == at::kFloat, "gated_scan_step: a state pool does not support dtype ",
                 c10::toString(t->scalar_type()));
@@ -859,7 +875,8 @@ struct GatedDeltaBackward : Node {
     std::vector<SavedVariable> inputs;
     SavedVariable offsets;
 
-    variable_list apply(variable_list&& grads) override {
+    variable_list apply(variable_list&& incoming) override {
+        const variable_list grads = plain_gradients(std::move(incoming));
         variable_list out(6);
         if (grads[0].defined() || grads[1].defined()) {
             variable_list in;
@@ -951,8 +968,8 @@ Tensor gated_delta_step(py::handle hstate, py::handle hq, py::handle hk, py::han
     REQUIRE(q.dim() == 3 && v.dim() == 3, "gated_delta_step: q must be (B, heads, K) and v (B, heads, V)");
     const DeltaSizes sizes = check_delta("gated_delta_step", q, k, v, decay, beta);
     const int64_t batch = q.size(0);
-    const Tensor state = tensor_of(hstate, "gated_delta_step: state");
-    const Tensor next = hnew.is_none() ? state : tensor_of(hnew, "gated_delta_step: new_state");
+    const Tensor state = pool_of(hstate, "gated_delta_step: state");
+    const Tensor next = hnew.is_none() ? state : pool_of(hnew, "gated_delta_step: new_state");
     for (const Tensor* t : {&state, &next}) {
         REQUIRE(t->scalar_type() == at::kFloat, "gated_delta_step: a state pool does not support dtype ",
                 c10::toString(t->scalar_type()));
@@ -1120,7 +1137,8 @@ struct QkNormBackward : Node {
     QkCall call;
     std::vector<SavedVariable> inputs, turn;
 
-    variable_list apply(variable_list&& grads) override {
+    variable_list apply(variable_list&& incoming) override {
+        const variable_list grads = plain_gradients(std::move(incoming));
         variable_list out(4);
         if (grads[0].defined() || grads[1].defined()) {
             variable_list in, rotation;
