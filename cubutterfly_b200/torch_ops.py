@@ -94,11 +94,12 @@ def _run(key, transform, x, out):
 
     stream = torch.cuda.current_stream(x.device)
     plan = _plan(key + (x.device.index, int(stream.cuda_stream)), transform, x.device, stream.cuda_stream)
-    src = x.contiguous()
+    src = x.resolve_conj().resolve_neg().contiguous()  # memory alone does not say what a lazy view holds
     if out is None:
         out = torch.empty_like(src)
-    elif out.shape != src.shape or out.dtype != src.dtype or out.device != src.device or not out.is_contiguous():
-        raise ValueError("out must be a contiguous tensor of the input's shape, dtype and device")
+    elif (out.shape != src.shape or out.dtype != src.dtype or out.device != src.device or not out.is_contiguous()
+          or out.is_conj() or out.is_neg()):
+        raise ValueError("out must be a contiguous tensor of the input's shape, dtype and device, not a lazy view")
     if out.data_ptr() == src.data_ptr():
         raise ValueError("these operators are out of place: out must not alias the input")
     plan.execute(src.data_ptr(), out.data_ptr())

@@ -1,4 +1,4 @@
-"""Views that carry their sign or their zeros beside their memory: the block operators read memory."""
+"""Views that carry their sign or their zeros beside their memory: the operators read memory."""
 import pytest
 import torch
 
@@ -115,3 +115,16 @@ def test_negated_steps_and_pools(cuda):
             torch_ops.gated_delta_step(lazy["state"], q, q, v, g, beta, new_state=lazy.get("new_state"))
     with pytest.raises(ValueError, match="lazily negated"):
         torch_ops.gated_scan_step(torch._neg_view(rows), x, r, r, decay)
+
+
+@pytest.mark.gpu
+def test_transforms_of_lazy_views(cuda):
+    x = normal(1, 3, 64)
+    assert torch.equal(torch_ops.fwht(torch._neg_view(x)), torch_ops.fwht(-x))
+    z = torch.complex(x, normal(2, 3, 64))
+    want = torch_ops.fft(z.conj().resolve_conj())
+    assert torch.equal(torch_ops.fft(z.conj()), want)
+    assert torch.allclose(want, torch.fft.fft(z.conj()), atol=1e-4)
+    for out in (torch.empty_like(z).conj(), torch._neg_view(torch.empty_like(z))):
+        with pytest.raises(ValueError, match="lazy view"):
+            torch_ops.fft(z, out=out)
