@@ -330,6 +330,35 @@ cubf::HeadTensor head_tensor(const cubutterflyB200HeadTensor_t& t, size_t size, 
     return {t.data, t.batch, t.token, t.head};
 }
 
+// ---- tensors apart from one another -----------------------------------------
+struct Bytes {                   // an output, or another contiguous tensor
+    uintptr_t from = 0, to = 0;
+    Bytes(const void* p, size_t size) : from(reinterpret_cast<uintptr_t>(p)), to(p ? from + size : from) {}
+};
+bool meet(const Bytes& a, const Bytes& b) { return a.from < b.to && b.from < a.to; }
+
+struct HeadSizes {
+    size_t batch, tokens, heads, channels, size;
+    size_t bytes() const { return batch * tokens * heads * channels * size; }
+};
+// `out` meets a batch row of `t`, from the row's first value to its last.
+bool meet(const Bytes& out, const cubf::HeadTensor& t, const HeadSizes& n) {
+    if (!t.p || n.bytes() == 0 || out.from == out.to) return false;
+    const uintptr_t base = reinterpret_cast<uintptr_t>(t.p);
+    const size_t row = ((n.tokens - 1) * t.token + (n.heads - 1) * t.head + n.channels) * n.size, step = t.batch * n.size;
+    size_t b = 0;                // the first row that ends behind out's beginning
+    if (base + row <= out.from) {
+        if (step == 0) return false;
+        b = (out.from - base - row) / step + 1;
+    }
+    return b < n.batch && base + b * step < out.to;
+}
+// `p`, contiguous, is `t` itself: read and written at the same places.
+bool in_place(const void* p, const cubf::HeadTensor& t, const HeadSizes& n) {
+    return p == t.p && (n.heads == 1 || t.head == n.channels) && (n.tokens == 1 || t.token == n.heads * n.channels) &&
+           (n.batch == 1 || t.batch == n.tokens * n.heads * n.channels);
+}
+
 template <typename Args, typename Call>
 void delta_gates(const Args* a, BlockType block, Call& s) {
     s.log_decay32 = vector_is_32(a->log_decay.data, a->log_decay_type, block, "gated delta log_decay_type");
@@ -384,6 +413,26 @@ void delta_workspace(const cubutterflyB200GatedDelta_t* a, BlockType block, bool
                 element_aligned(a->workspace, 256),
             "gated delta: a 256-byte aligned workspace of the queried size is needed");
     s.workspace = a->workspace;
+}
+
+struct DeltaSizes {
+    HeadSizes keys, values, decay, beta;
+    size_t state, offsets;       // bytes
+};
+DeltaSizes delta_sizes(const cubf::GatedDeltaArgs& a, BlockType block) {
+    const size_t batch = a.batch, length = a.length, heads = a.heads, states = a.offsets ? a.sequences : a.batch;
+    const size_t k_heads = a.k_heads, k = a.k_dim, v = a.v_dim, es = element(block);
+    return {{batch, length, k_heads, k, es},
+            {batch, length, heads, v, es},
+            {batch, length, heads, 1, a.log_decay32 ? 4 : es},
+            {batch, length, heads, 1, a.beta32 ? 4 : es},
+            states * heads * k * v * sizeof(float),
+            a.offsets ? (a.sequences + size_t{1}) * sizeof(int) : 0};
+}
+// An output meets what both directions read.
+bool delta_meets(const Bytes& out, const cubf::GatedDeltaArgs& a, const DeltaSizes& n) {
+    return meet(out, a.q, n.keys) || meet(out, a.k, n.keys) || meet(out, a.v, n.values) || meet(out, a.log_decay, n.decay) ||
+           meet(out, a.beta, n.beta) || meet(out, {a.initial, n.state}) || meet(out, {a.offsets, n.offsets});
 }
 
 // ---- norm of queries and keys -------------------------------------------------------------------
@@ -574,12 +623,13 @@ extern "C" cubutterflyStatus_t cubutterflyB200GatedDeltaForward(const cubutterfl
         if (a.batch == 0) return;
         require(args->o && element_aligned(args->o, element(block)), "gated delta: null or misaligned o");
         require(args->final_state != nullptr, "gated delta: null final_state");
-        require(args->o != args->q.data && args->o != args->k.data && args->o != args->v.data,
-                "gated delta: o must not alias an input");
-        require(args->final_state != args->initial_state, "gated delta: final_state must not alias initial_state");
         a.o = args->o;
         a.last = args->final_state;
         delta_workspace(args, block, false, a);
+        const DeltaSizes n = delta_sizes(a, block);
+        const Bytes o(a.o, n.values.bytes()), last(a.last, n.state);
+        require(!delta_meets(o, a, n) && !delta_meets(last, a, n) && !meet(o, last),
+                "gated delta: o and final_state must not alias an input or one another");
         check(cubf::launch_gated_delta(block, a, false, stream), "gated delta launch");
     });
 }
@@ -606,6 +656,15 @@ extern "C" cubutterflyStatus_t cubutterflyB200GatedDeltaBackward(const cubutterf
         a.d_beta = args->d_beta;
         a.d_initial = args->d_initial_state;
         delta_workspace(args, block, true, a);
+        const DeltaSizes n = delta_sizes(a, block);
+        const Bytes outs[] = {{a.d_q, n.keys.bytes()},          {a.d_k, n.keys.bytes()}, {a.d_v, n.values.bytes()},
+                              {a.d_log_decay, n.decay.bytes()}, {a.d_beta, n.beta.bytes()}, {a.d_initial, n.state}};
+        for (const Bytes& out : outs) {
+            require(!delta_meets(out, a, n) && !meet(out, a.d_o, n.values) && !meet(out, {a.d_last, n.state}),
+                    "gated delta: a gradient must not alias a tensor that is read");
+            for (const Bytes& other : outs)
+                require(&out == &other || !meet(out, other), "gated delta: gradients must not alias one another");
+        }
         check(cubf::launch_gated_delta(block, a, true, stream), "gated delta backward launch");
     });
 }
@@ -638,6 +697,14 @@ extern "C" cubutterflyStatus_t cubutterflyB200GatedDeltaStep(const cubutterflyB2
         s.o = a->o;
         s.batch = a->batch;
         s.pool = a->pool;
+        const size_t es = element(block), heads = a->heads;
+        const HeadSizes keys{a->batch, 1, a->k_heads, a->k_dim, es}, values{a->batch, 1, heads, a->v_dim, es};
+        const Bytes o(s.o, values.bytes());
+        require(!meet(o, s.q, keys) && !meet(o, s.k, keys) && (in_place(s.o, s.v, values) || !meet(o, s.v, values)) &&
+                    !meet(o, s.log_decay, {a->batch, 1, heads, 1, s.log_decay32 ? 4 : es}) &&
+                    !meet(o, s.beta, {a->batch, 1, heads, 1, s.beta32 ? 4 : es}) && !meet(o, {s.state, bytes}) &&
+                    !meet(o, {s.new_state, bytes}),
+                "gated delta step: o must not alias another tensor (v itself excepted)");
         check(cubf::launch_gated_delta_step(block, s, stream), "gated delta step launch");
     });
 }
@@ -650,11 +717,12 @@ extern "C" cubutterflyStatus_t cubutterflyB200QkNormForward(const cubutterflyB20
         const size_t es = element(block);
         require(args->q_out && args->k_out && element_aligned(args->q_out, es) && element_aligned(args->k_out, es),
                 "qk norm: null or misaligned output");
-        require(args->q_out != args->q.data && args->q_out != args->k.data && args->k_out != args->q.data &&
-                    args->k_out != args->k.data && args->q_out != args->k_out,
-                "qk norm: an output must not alias another tensor");
         a.q_out = args->q_out;
         a.k_out = args->k_out;
+        const HeadSizes q{a.batch, a.tokens, args->q_heads, args->dim, es}, k{a.batch, a.tokens, args->k_heads, args->dim, es};
+        const Bytes qs(a.q_out, q.bytes()), ks(a.k_out, k.bytes());
+        require(!meet(qs, a.q, q) && !meet(qs, a.k, k) && !meet(ks, a.q, q) && !meet(ks, a.k, k) && !meet(qs, ks),
+                "qk norm: an output must not alias another tensor");
         check(cubf::launch_qk_norm(block, a, false, stream), "qk norm launch");
     });
 }
@@ -691,6 +759,16 @@ extern "C" cubutterflyStatus_t cubutterflyB200QkNormBackward(const cubutterflyB2
         a.d_q_weight = args->d_q_weight;
         a.d_k_weight = args->d_k_weight;
         a.partials = static_cast<float*>(args->workspace);
+        // a head's gradient may take its own place, or that of the gradient it comes from
+        const HeadSizes q{a.batch, a.tokens, args->q_heads, args->dim, es}, k{a.batch, a.tokens, args->k_heads, args->dim, es};
+        const Bytes qs(a.d_q, q.bytes()), ks(a.d_k, k.bytes());
+        auto apart = [](const void* p, const Bytes& out, const cubf::HeadTensor& t, const HeadSizes& n) {
+            return in_place(p, t, n) || !meet(out, t, n);
+        };
+        require(apart(a.d_q, qs, a.q, q) && apart(a.d_q, qs, a.d_q_out, q) && apart(a.d_k, ks, a.k, k) &&
+                    apart(a.d_k, ks, a.d_k_out, k) && !meet(qs, a.k, k) && !meet(qs, a.d_k_out, k) && !meet(ks, a.q, q) &&
+                    !meet(ks, a.d_q_out, q) && !meet(qs, ks),
+                "qk norm: a gradient must not alias another tensor (that of its own head excepted)");
         check(cubf::launch_qk_norm(block, a, true, stream), "qk norm backward launch");
     });
 }

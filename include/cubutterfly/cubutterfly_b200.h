@@ -317,6 +317,8 @@ typedef struct cubutterflyB200HeadTensor_s {
  * offset or behind the last one have outputs and gradients of zero.
  * The gradients are contiguous, in the types of their tensors; d_initial_state
  * null: not computed.  Both directions need a workspace (256-byte aligned).
+ * No output or gradient may share memory with what the call reads, or with
+ * another one.
  * The kernels of 16-bit tensors wait for copies and products of their own.  A
  * wait that runs out ends what depends on it, with NaN in the rows, states and
  * gradients concerned.  wait_limit: tries of a wait (8 us where nothing
@@ -351,7 +353,8 @@ CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200GatedDeltaBackward(const cubut
 
 /* One token of the gated delta rule for `batch` requests, whose states
  * (heads, k_dim, v_dim) lie in pools of slots as in GatedScanStep.  The
- * tensors' token strides are not read. */
+ * tensors' token strides are not read.  o may be v, in the same layout, and
+ * no other tensor; new_state is state or does not overlap it. */
 typedef struct cubutterflyB200GatedDeltaStep_s {
     size_t struct_size;
     size_t batch, k_heads, heads, k_dim, v_dim, pool;
@@ -383,7 +386,9 @@ enum {
  * positions[x positions_axis + (b tokens + t) mod positions_period]; axes
  * (rotary / 2 values from 0 to axis_count - 1) is null with one axis.
  * Angles are exact to 2e-7 up to positions of 2^31 (frequencies up to 1).
- * Outputs and gradients are contiguous (batch, tokens, heads, dim). */
+ * Outputs and gradients are contiguous (batch, tokens, heads, dim) and share
+ * no memory with other tensors, but that d_q may be q or d_q_out (d_k likewise)
+ * in the same layout. */
 typedef struct cubutterflyB200QkNorm_s {
     size_t struct_size;
     size_t batch, tokens, q_heads, k_heads, dim, rotary, axis_count, positions_axis, positions_period;
