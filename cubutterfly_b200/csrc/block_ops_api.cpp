@@ -330,6 +330,16 @@ cubf::HeadTensor head_tensor(const cubutterflyB200HeadTensor_t& t, size_t size, 
     return {t.data, t.batch, t.token, t.head};
 }
 
+template <typename Args, typename Call>
+void delta_heads(const Args* a, Call& s) {
+    check_delta_heads(a);
+    s.k_heads = static_cast<int>(a->k_heads);
+    s.heads = static_cast<int>(a->heads);
+    s.k_dim = static_cast<int>(a->k_dim);
+    s.v_dim = static_cast<int>(a->v_dim);
+    s.scale = static_cast<float>(a->scale);
+}
+
 // ---- tensors apart from one another -----------------------------------------
 struct Bytes {                   // an output, or another contiguous tensor
     uintptr_t from = 0, to = 0;
@@ -369,24 +379,20 @@ void delta_gates(const Args* a, BlockType block, Call& s) {
     s.v = head_tensor(a->v, es, "gated delta: null or misaligned v");
     s.log_decay = head_tensor(a->log_decay, 2, "gated delta: null or misaligned log_decay");
     s.beta = head_tensor(a->beta, 2, "gated delta: null or misaligned beta");
-    s.k_heads = static_cast<int>(a->k_heads);
-    s.heads = static_cast<int>(a->heads);
-    s.k_dim = static_cast<int>(a->k_dim);
-    s.v_dim = static_cast<int>(a->v_dim);
-    s.scale = static_cast<float>(a->scale);
 }
 
-cubf::GatedDeltaArgs delta_args(const cubutterflyB200GatedDelta_t* a, BlockType* block) {
+// Without `tensors`: of what the workspace's size depends on.
+cubf::GatedDeltaArgs delta_args(const cubutterflyB200GatedDelta_t* a, BlockType* block, bool tensors = true) {
     require(a != nullptr, "gated delta: null arguments");
     require(a->struct_size == sizeof(*a), "gated delta: struct_size does not match this library's");
-    check_delta_heads(a);
+    cubf::GatedDeltaArgs s{};
+    delta_heads(a, s);
     supported(a->length <= cubf::kDeltaMaxLength, "gated delta: length is limited to 2^30 tokens");
     supported(a->batch <= (1u << 24) && a->sequences <= (1u << 30), "gated delta: too many sequences");
     require(!a->offsets || (a->batch == 1 && a->sequences >= 1),
             "gated delta: a packed batch has batch = 1 and at least one sequence");
     require(a->offsets || a->sequences == 0, "gated delta: sequences without offsets");
     *block = type_of(a->data_type, "gated delta data_type");
-    cubf::GatedDeltaArgs s{};
     s.batch = static_cast<int>(a->batch);
     s.length = static_cast<int>(a->length);
     s.sequences = static_cast<int>(a->sequences);
@@ -394,7 +400,7 @@ cubf::GatedDeltaArgs delta_args(const cubutterflyB200GatedDelta_t* a, BlockType*
     s.offsets = a->offsets;
     constexpr int most = cubf::kDeltaWaitLimit;
     s.wait_limit = a->wait_limit == 0 ? most : std::clamp(a->wait_limit, 0, most);
-    if (a->batch > 0 && a->length > 0) delta_gates(a, *block, s);
+    if (tensors && a->batch > 0 && a->length > 0) delta_gates(a, *block, s);
     // a CTA for each chunk of 64 tokens of each head
     const size_t chunks = a->offsets ? a->length / cubf::kDeltaChunk + a->sequences
                                      : a->batch * ((a->length + cubf::kDeltaChunk - 1) / cubf::kDeltaChunk);
@@ -436,13 +442,26 @@ bool delta_meets(const Bytes& out, const cubf::GatedDeltaArgs& a, const DeltaSiz
 }
 
 // ---- norm of queries and keys -------------------------------------------------------------------
-cubf::QkNormArgs qk_args(const cubutterflyB200QkNorm_t* a, BlockType* block) {
+// What the workspace's size depends on.
+cubf::QkNormArgs qk_sizes(const cubutterflyB200QkNorm_t* a) {
     require(a != nullptr, "qk norm: null arguments");
     require(a->struct_size == sizeof(*a), "qk norm: struct_size does not match this library's");
-    require(a->q_heads >= 1 && a->k_heads >= 1 && a->dim >= 1, "qk norm: heads and their size must be at least 1");
+    require(a->dim >= 1, "qk norm: heads and their size must be at least 1");
     supported(a->dim <= cubf::kQkNormMaxDim, "qk norm: dim is limited to 256");
-    supported(a->q_heads <= 65536 && a->k_heads <= 65536, "qk norm: at most 65536 heads");
     supported(a->batch == 0 || a->tokens <= (size_t{1} << 40) / a->batch, "qk norm: too many tokens");
+    cubf::QkNormArgs n{};
+    n.batch = a->batch;
+    n.tokens = a->tokens;
+    n.dim = static_cast<int>(a->dim);
+    n.q_weight = a->q_weight;
+    n.k_weight = a->k_weight;
+    n.parts = cubf::qk_norm_parts(n);
+    return n;
+}
+cubf::QkNormArgs qk_args(const cubutterflyB200QkNorm_t* a, BlockType* block) {
+    cubf::QkNormArgs n = qk_sizes(a);
+    require(a->q_heads >= 1 && a->k_heads >= 1, "qk norm: heads and their size must be at least 1");
+    supported(a->q_heads <= 65536 && a->k_heads <= 65536, "qk norm: at most 65536 heads");
     require(std::isfinite(a->epsilon) && a->epsilon >= 0, "qk norm: epsilon must be finite and not negative");
     require((a->flags & ~7) == 0, "qk norm: unknown flags");
     require(a->rotary % 2 == 0 && a->rotary <= a->dim, "qk norm: rotary must be even and at most dim");
@@ -452,12 +471,8 @@ cubf::QkNormArgs qk_args(const cubutterflyB200QkNorm_t* a, BlockType* block) {
             "qk norm: positions need a period and an axis");
     require(a->axes || a->axis_count <= 1, "qk norm: several axes of positions need axes");
     *block = type_of(a->data_type, "qk norm data_type");
-    cubf::QkNormArgs n{};
-    n.batch = a->batch;
-    n.tokens = a->tokens;
     n.q_heads = static_cast<int>(a->q_heads);
     n.k_heads = static_cast<int>(a->k_heads);
-    n.dim = static_cast<int>(a->dim);
     n.rotary = static_cast<int>(a->rotary);
     n.axis_count = static_cast<int>(a->axis_count);
     n.positions_axis = a->positions_axis;
@@ -472,11 +487,8 @@ cubf::QkNormArgs qk_args(const cubutterflyB200QkNorm_t* a, BlockType* block) {
     n.positions = a->positions;
     n.frequencies = a->frequencies;
     n.axes = a->axes;
-    n.q_weight = a->q_weight;
-    n.k_weight = a->k_weight;
     n.q_weight32 = vector_is_32(a->q_weight, a->q_weight_type, *block, "qk norm q_weight_type");
     n.k_weight32 = vector_is_32(a->k_weight, a->k_weight_type, *block, "qk norm k_weight_type");
-    n.parts = cubf::qk_norm_parts(n);
     if (a->batch == 0 || a->tokens == 0) return n;
     n.q = head_tensor(a->q, element(*block), "qk norm: null or misaligned q");
     n.k = head_tensor(a->k, element(*block), "qk norm: null or misaligned k");
@@ -608,7 +620,7 @@ extern "C" cubutterflyStatus_t cubutterflyB200GatedDeltaGetWorkspaceSize(const c
                                                                         int backward, size_t* bytes) {
     return guarded([&] {
         BlockType block;
-        const cubf::GatedDeltaArgs a = delta_args(args, &block);
+        const cubf::GatedDeltaArgs a = delta_args(args, &block, false);
         require(bytes != nullptr, "gated delta: null size");
         *bytes = a.batch == 0 || a.length == 0 ? 0 : cubf::gated_delta_workspace(block, a, backward != 0);
     });
@@ -674,11 +686,11 @@ extern "C" cubutterflyStatus_t cubutterflyB200GatedDeltaStep(const cubutterflyB2
     return guarded([&] {
         require(a != nullptr, "gated delta step: null arguments");
         require(a->struct_size == sizeof(*a), "gated delta step: struct_size does not match this library's");
-        check_delta_heads(a);
+        cubf::GatedDeltaStepArgs s{};
+        delta_heads(a, s);
         supported(a->batch <= 0x7fffffffULL && a->pool <= 0x7fffffffULL, "gated delta step: too many requests or slots");
         const BlockType block = type_of(a->data_type, "gated delta step data_type");
         if (a->batch == 0) return;
-        cubf::GatedDeltaStepArgs s{};
         delta_gates(a, block, s);
         require(a->o && element_aligned(a->o, element(block)), "gated delta step: null or misaligned o");
         require((a->state && a->new_state) || a->pool == 0, "gated delta step: null state");
@@ -729,8 +741,7 @@ extern "C" cubutterflyStatus_t cubutterflyB200QkNormForward(const cubutterflyB20
 
 extern "C" cubutterflyStatus_t cubutterflyB200QkNormGetWorkspaceSize(const cubutterflyB200QkNorm_t* args, size_t* bytes) {
     return guarded([&] {
-        BlockType block;
-        const cubf::QkNormArgs a = qk_args(args, &block);
+        const cubf::QkNormArgs a = qk_sizes(args);
         require(bytes != nullptr, "qk norm: null size");
         *bytes = qk_workspace(a);
     });

@@ -345,7 +345,7 @@ typedef struct cubutterflyB200GatedDelta_s {
 
 CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200GatedDeltaForward(const cubutterflyB200GatedDelta_t* args,
                                                                    cudaStream_t stream);
-/* Reads the sizes, the types, offsets, q and k. */
+/* Reads the sizes, data_type and whether there are offsets. */
 CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200GatedDeltaGetWorkspaceSize(const cubutterflyB200GatedDelta_t* args,
                                                                             int backward, size_t* bytes);
 CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200GatedDeltaBackward(const cubutterflyB200GatedDelta_t* args,
@@ -408,7 +408,7 @@ typedef struct cubutterflyB200QkNorm_s {
 
 CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200QkNormForward(const cubutterflyB200QkNorm_t* args,
                                                                cudaStream_t stream);
-/* Reads batch, tokens, dim and the weights. */
+/* Reads batch, tokens, dim and whether there are weights. */
 CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200QkNormGetWorkspaceSize(const cubutterflyB200QkNorm_t* args,
                                                                         size_t* bytes);
 CUBUTTERFLYAPI cubutterflyStatus_t cubutterflyB200QkNormBackward(const cubutterflyB200QkNorm_t* args,
