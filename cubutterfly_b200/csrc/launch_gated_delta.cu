@@ -65,8 +65,9 @@ int segment_length(const GatedDeltaArgs& a, bool backward) {
     int length = 0;
     for (int n = 2; n <= 64 && longest / n >= 4; ++n) {
         const int chunks = static_cast<int>(std::ceil(longest / n));
-        const double segments = all / chunks + (a.offsets ? sequences : 0);  // of all sequences
-        const double first = segments * a.heads * (backward ? 3 : 2) - (backward ? 5 : 3) * sequences * a.heads;
+        const double segments = a.offsets ? all / chunks + sequences : sequences * std::ceil(longest / chunks);  // of all
+        // of s segments, s - 1 ends, s - 2 maps and, backward, s - 1 ends of the reversed chain
+        const double first = segments * a.heads * (backward ? 3 : 2) - (backward ? 4 : 3) * sequences * a.heads;
         const double time = waves(first) * chunks * 1.9 + (n - 2) * 4 + 10 +
                             waves((backward ? 2 : 1) * segments * a.heads) * chunks * full;
         if (time < 0.95 * best) best = time, length = chunks;
