@@ -474,18 +474,21 @@ CUBF_DEV int segment_base(const GatedDeltaArgs& a, const Segments& s, int sequen
     return a.offsets ? base / s.length + sequence : sequence * segments_of((a.length + C - 1) / C, s.length);
 }
 // The sequence of `rank` among those of a packed batch by length, the longest first, so that no long chain starts last.  Each
-// lane ranks two sequences; beyond 64 their order stays.  16384 tokens in 13 sequences, 32 heads forward: 417 us for 480; in 6,
-// 643 for 675; 8 heads' training in 24 sequences 698 for 729; forward in 40, whose chains are many and short, 446 for 432.
+// lane ranks two sequences, whose lengths go round by shuffles (read again by every lane they cost 2 us a CTA with 64
+// sequences); beyond 64 their order stays.  16384 tokens with and without the order, random cuts: forward of 16 heads in 33
+// sequences 223 us for 225 to 274, of 32 heads in 64 sequences 452 for 439 to 466; training of 8 heads in 33 sequences 656
+// and 697 for 670 and 742, in 64 672 for 694 to 766.
 CUBF_DEV int by_length(const GatedDeltaArgs& a, int rank) {
     if (a.sequences > 64) return rank;
     const int lane = threadIdx.x & 31;
     auto length = [&](int j) { return j < a.sequences ? max(0, offset_at(a, j + 1) - offset_at(a, j)) : -1; };
     const int mine[2] = {length(lane), length(lane + 32)};
-    int before[2] = {0, 0};
-    for (int j = 0; j < a.sequences; ++j) {
-        const int other = length(j);
-#pragma unroll
-        for (int n = 0; n < 2; ++n) before[n] += other > mine[n] || (other == mine[n] && j < lane + 32 * n);
+    int before[2] = {0, 0};              // longer ones, and those as long that come first
+#pragma unroll 8
+    for (int j = 0; j < 32; ++j) {
+        const int one = __shfl_sync(0xffffffffu, mine[0], j), two = __shfl_sync(0xffffffffu, mine[1], j);
+        before[0] += (one > mine[0] || (one == mine[0] && j < lane)) + (two > mine[0]);
+        before[1] += (one >= mine[1]) + (two > mine[1] || (two == mine[1] && j < lane));
     }
     const unsigned low = __ballot_sync(0xffffffffu, lane < a.sequences && before[0] == rank);
     const unsigned high = __ballot_sync(0xffffffffu, lane + 32 < a.sequences && before[1] == rank);
