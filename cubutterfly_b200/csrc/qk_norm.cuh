@@ -17,9 +17,10 @@
 // exchange.
 //
 // Angles: a position times a frequency is taken modulo one turn in 64-bit
-// integers (the frequency in turns times 2^64, from a product in fp64), so
-// that far positions keep every bit: the angle's error is 2e-7 at position
-// 2^31 and frequency 1, where fp32 products would be off by whole turns.
+// integers (the frequency in turns times 2^64, from a product of two fp64
+// parts), so that far positions keep every bit: the angle's error is 1e-7, the
+// half turn's rounding to fp32, up to position 2^31 and frequency 1, where fp32
+// products would be off by whole turns.
 #pragma once
 
 #include "common.cuh"
@@ -194,9 +195,13 @@ CUBF_DEV void prepare(const QkNormArgs& a, const Layout& l, Shared& sm) {
         }
         if (TURNED) {
             const bool turned = p < l.half;
-            double x = turned ? static_cast<double>(a.frequencies[p]) * 0.15915494309189533577 : 0.0;
-            x -= floor(x);                          // whole turns a position drop out
-            sm.turns[p] = static_cast<unsigned long long>(x * 18446744073709551616.0);
+            // 1 / 2 pi in two parts: rounded to one, times 2^31 positions, it alone would turn by 2e-7, the product as much
+            constexpr double part = 0.15915494309189535, rest = -9.839338337591243e-18, turn = 18446744073709551616.0;
+            const double frequency = turned ? static_cast<double>(a.frequencies[p]) : 0.0;
+            double x = frequency * part;
+            const double low = fma(frequency, part, -x) + frequency * rest;
+            x -= rint(x);                           // whole turns a position drop out; exact, as less floor(x) is not below zero
+            sm.turns[p] = static_cast<unsigned long long>(llrint(x * turn)) + static_cast<unsigned long long>(llrint(low * turn));
             sm.axis[p] = turned && a.axes ? min(max(a.axes[p], 0), a.axis_count - 1) : 0;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {      // what stays as it is beyond the rotated pairs
