@@ -20,10 +20,15 @@
 // other chains fill the other SMs.
 //
 // bf16 inputs are one exact bf16 piece, fp16 ones two.  fp32 operands (states,
-// L, P, beta Y, U) are taken as two pieces, 16 bits: a product's error is 2^-16
-// at most, 3e-6 in the mean, far below one rounding of a 16-bit output and
-// below 1e-5 of the fp32 states, which are themselves held and added up in
-// fp32; a third piece would cost half as much again.
+// L, P, beta Y, U) are taken as two pieces, within 2^-16 of themselves, and of
+// two such operands the product of the second pieces is left out: a product is
+// off by 2^-16 at most with one of them and by 3 x 2^-16 with two.  In the mean
+// that is 2.5e-6 to 4e-6 of a final state or an initial one's gradient, which
+// are themselves held and added up in fp32, and far below one rounding of a
+// 16-bit output.  Third pieces of S, Y, U and L (in the columns that D, X and U
+// leave free meanwhile) gave final states to 2e-7 to 8e-7, at 929 us for 609 of
+// the prefill and 1189 for 1034 of training: not worth it beside 16-bit tensors;
+// fp32 ones have them.
 #pragma once
 
 #include "f32x2.cuh"
@@ -1242,7 +1247,7 @@ CUBF_DEV void fewer_registers() {
 }
 
 // A chunk takes 2.4 us of its chain (K = V = 128, bf16), tensor pipe 41 % busy: 32 heads of 16384 tokens 622 us in one piece,
-// 236 in three segments whose ends took 189 (1.9 to 2.2 us a chunk without outputs) and their joins 10 to 27.
+// 229 in three segments whose ends took 193 (1.9 to 2.2 us a chunk without outputs) and their joins 10 to 27.
 template <typename T, int KP>
 __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_forward_kernel(GatedDeltaArgs a, Places w, bool wide) {
     extern __shared__ __align__(1024) unsigned char aligned_raw[];
@@ -1267,7 +1272,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_forward_kernel(G
 
 // Both chains of the backward side by side: neither needs the other's results.  (One kind after the other is no faster for
 // training's 128 + 128 chains on 148 SMs, 420 us against 433, and slower for packed sequences, 587 against 350, both measured
-// before the chains' later steps; the 256 chains of 32 chunks take 290 now, two rounds of 4.5 us a chunk, 2.5 TB/s of writes.)
+// before the chains' later steps; the 256 chains of 32 chunks take 296 now, two rounds of 4.5 us a chunk, 2.5 TB/s of writes.)
 template <typename T, int KP>
 __global__ void __launch_bounds__(kTcThreads, 1) gated_delta_tc_chains_kernel(GatedDeltaArgs a, Places w, bool wide) {
     extern __shared__ __align__(1024) unsigned char aligned_raw[];
@@ -1437,7 +1442,7 @@ __global__ void __launch_bounds__(2 * KP) gated_delta_join_kernel(GatedDeltaArgs
 //   [Cq; Cm] k      and, the tile turned,  [.; Cq^T q + Cm^T k].
 // What has to come is the kept S and dS, 64 KB each, R and W, 32 KB each, and the tiles of q, k and dO per chunk and head;
 // they fill shared memory, so a head's steps are one after another and their latency bounds it.  8 sequences of 2048 tokens,
-// 16 heads (bf16, K = V = 128): 330 us, where the bytes alone take 145; 353 without the next head's prefetch to L2, and 490
+// 16 heads (bf16, K = V = 128): 330 to 336 us, where the bytes alone take 145; 353 without the next head's prefetch to L2, and 490
 // with 168 registers a thread (1 KB spilled) instead of 224 and all 32 columns of the pairs at once.
 constexpr int kGradientThreads = kTcThreads;  // three warps only leave their registers to the computing ones
 

@@ -48,8 +48,10 @@ int sequences_of(const GatedDeltaArgs& a) { return a.offsets ? a.sequences : a.b
 // Chunks a segment, 0 for none: the shortest time by what a chunk of a chain takes on one SM (2.4 us with its results
 // forward, 2.9 backward, 1.9 without them), a state's join (4 us) and the CTAs that run at once, one per SM.  Of a packed
 // batch the host knows the tokens and the sequences alone; n random cuts leave a longest piece of (1 + 1/2 + .. + 1/n) / n.
-// Whole calls forward, one sequence of 16384 tokens: 32 heads 624 us in three segments against 840 in one, 12 heads 335 in
-// seven against 725, 4 heads 205 in 16 against 666; forward and backward of 4 heads 600 in 14 against 1910.
+// Whole calls forward, one sequence of 16384 tokens: 32 heads 606 us in three segments against 804 in one, 12 heads 319 in
+// seven against 705, 4 heads 192 in 16 against 649; forward and backward of 4 heads 582 in 12 against 1890.  Backward a
+// chunk takes 4.5 us while every SM writes; but with 4.5 here the choices were the same or worse (training 4 x 4096 tokens of
+// 20 heads 1615 us for 1490, 10007 tokens of 4 heads in 13 sequences 430 for 395).
 int segment_length(const GatedDeltaArgs& a, bool backward) {
     double longest = ceil_div(a.length, C), all = longest * a.batch;
     const double sequences = sequences_of(a);

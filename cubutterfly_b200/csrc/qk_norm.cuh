@@ -10,7 +10,7 @@
 // (sum in place of mean for heads of length one).
 //
 // Bounded by memory: every head is read once and written once.  A warp takes
-// one token and runs through its heads, 32 / G at a time, a group of G lanes
+// one token (of few tokens, a part of its heads) and runs through its heads, 32 / G at a time, a group of G lanes
 // each; its sines and cosines are computed once, a pair a lane, into a table
 // that all heads read.  A lane holds pairs: of rotated halves the same 16 bytes
 // of either half, of adjacent pairs 32 bytes side by side, so neither needs an
